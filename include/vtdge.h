@@ -590,6 +590,71 @@ int vtdge_chain_layout(const vtdge_chain *chain, int64_t *layout_host);
 int vtdge_chain_forward(const vtdge_chain *chain, const void *const *params_host, const void *front_rows, void *x,
                         void *ints, void *big, void *scratch, void *out, void *stream, void *side_stream);
 
+/* Balance of router gates over `tokens` rows of logits, [tokens, E] with `pitch` elements between rows:
+ *   loss = E sum_e f_e P_e,  f_e = counts[e] / (K T),  P_e = mean softmax probability of e, over the T tokens that count
+ *   indices  nullable int64 [tokens, K]: the choices, made elsewhere; those outside 0 .. E - 1 are not counted.  NULL: the K
+ *            largest logits of each token, among equals the lowest expert, NaN above all
+ *   mask     nullable, one byte a token: 0 leaves it out, whatever its logits are.  A token whose logits are all -inf is
+ *            left out too.  T = 0: loss and gradients are 0
+ *   loss     fp32 [1]   counts int64 [E]   share fp32 [E + 1], for the gradient
+ *   workspace  vtdge_gate_balance_workspace bytes (0 for few tokens), contents do not matter, nothing else using it
+ * _backward: grad [tokens, E] dense = grad_loss[0] * d loss / d gate; zeros for tokens left out. */
+#define VTDGE_MAX_EXPERTS 512
+int64_t vtdge_gate_balance_workspace(int64_t tokens, int E);
+int vtdge_gate_balance(const void *gate, int64_t pitch, const int64_t *indices, const uint8_t *mask, int64_t tokens, int E,
+                       int K, void *workspace, int64_t workspace_bytes, float *loss, int64_t *counts, float *share, int dtype,
+                       void *stream);
+int vtdge_gate_balance_backward(const void *gate, int64_t pitch, const uint8_t *mask, const float *share,
+                                const float *grad_loss, void *grad, int64_t tokens, int E, int dtype, void *stream);
+
+/* Softmax cross entropy of a Linear's outputs, z = x weight^T + bias over `classes`, without z in memory:
+ *   loss_rows[r] = logsumexp_v z[r, v] - (1 - smoothing) z[r, target[r]] - smoothing mean_v z[r, v]
+ *   x [rows, width], ldx elements between rows; weight [classes, width], ldw; bias nullable [classes]; target int64 [rows]
+ *   Rows whose target is ignore_index, or no class, are left out: their loss is 0, and so is what they add to any gradient,
+ *   whatever they hold.
+ *   row_max, row_inv  fp32 [rows], for the gradients: the largest z (times log2 e), and 1 / sum exp(z - largest)
+ *   loss, inv_count   fp32 [1] each, nullable: the mean of the losses of the rows that count and 1 / their number (0 and 0
+ *                     without any); without inv_count the loss is their sum
+ * _backward, of grad * loss_rows summed over the rows:
+ *   grad      fp32, one value for each row (grad_stride 1) or one for all (0), times inv_count[0] where that is given
+ *   dx [rows, width], dweight [classes, width], dbias [classes]: dense, of `dtype`, each nullable
+ * fp32 operands are multiplied as exactly as fp32 products are, on the bf16 matrix instructions.
+ *   workspace  vtdge_cross_entropy_workspace(..., backward) bytes, 256-byte aligned, contents do not matter */
+int64_t vtdge_cross_entropy_workspace(int64_t rows, int64_t classes, int width, int dtype, int backward);
+int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, const int64_t *target,
+                        int64_t rows, int64_t classes, int width, int64_t ignore_index, float smoothing, void *workspace,
+                        int64_t workspace_bytes, float *loss_rows, float *row_max, float *row_inv, float *loss,
+                        float *inv_count, int dtype, void *stream);
+int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias,
+                                 const int64_t *target, const float *row_max, const float *row_inv, const float *grad,
+                                 int grad_stride, const float *inv_count, int64_t rows, int64_t classes, int width,
+                                 int64_t ignore_index, float smoothing, void *workspace, int64_t workspace_bytes, void *dx,
+                                 void *dweight, void *dbias, int dtype, void *stream);
+
+/* One AdamW step over `count` tensors, in one launch for each 92 of them (64 with 8-bit moments):
+ *   p *= 1 - lr weight_decay;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
+ *   p -= lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ *   tensors_host  HOST table; param and grad of `dtype`, n elements each, any alignment of their type
+ *   state_bits    32: exp_avg, exp_avg_sq fp32.  8: exp_avg e4m3, exp_avg_sq e5m2 (OCP), one byte an element, with an fp32
+ *                 scale for each 256 consecutive elements (ceil(n / 256) of them): largest magnitude / 448 and / 57344.
+ *                 Values are rounded down or up by a hash of the element's index and `step`; the same on every run
+ *   step          counted from 1
+ *   scalars       nullable: VTDGE_ADAMW_SCALARS bytes on the device from vtdge_adamw_scalars, in place of lr .. step
+ * vtdge_adamw_scalars works the factors of step *step + 1 - skipped (device) out on the device, and with `advance` then adds
+ * 1 to *step, so that both calls may be captured into a graph and replayed; lr_dev (nullable, device) stands in for lr. */
+typedef struct {
+    void *param;
+    const void *grad;
+    void *exp_avg, *exp_avg_sq;
+    float *exp_avg_scale, *exp_avg_sq_scale; /* 8-bit moments only */
+    int64_t n;
+} vtdge_adamw_tensor;
+#define VTDGE_ADAMW_SCALARS 64
+int vtdge_adamw(const vtdge_adamw_tensor *tensors_host, int count, double lr, double beta1, double beta2, double eps,
+                double weight_decay, int64_t step, const void *scalars, int dtype, int state_bits, void *stream);
+int vtdge_adamw_scalars(int64_t *step, int64_t skipped, int advance, const float *lr_dev, double lr, double beta1,
+                        double beta2, double eps, double weight_decay, void *scalars, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,282 @@
+"""The classifier's cross entropy and its gradients against the formula in float64: tiles and slabs around their edges, rows that
+are left out, infinite biases, pieces of the classes, strides, graphs, streams.
+
+Bounds.  fp32: every sum is six times its length of products in fp32, sixteen a step of the matrix instruction, and its error
+grows as a walk of that many half steps: 2^-24 (8 + 2 sqrt(6 n / 16)) of the 2-norm, n the longest sum.  bf16: the
+gradients of the logits are rounded once (neighbours between 1 and 2 are 2^-7 apart: half a step is 2^-8 of a term at most) and so is
+the result: element by element 2^-8 |d| |w| + 2^-8 |result|, and what the fp32 sums add."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+HALF = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16]
+
+
+def _operands(dev, rows, classes, width, dtype, seed=0, bias=True, left_out=0.0):
+    g = torch.Generator().manual_seed(seed * 7919 + rows * 31 + classes * 7 + width)
+    x = torch.randn(rows, width, generator=g)
+    w = torch.randn(classes, width, generator=g) * (1.5 / math.sqrt(width))
+    b = torch.randn(classes, generator=g) * 0.5 if bias else None
+    t = torch.randint(0, classes, (rows,), generator=g)
+    if left_out:
+        t[torch.rand(rows, generator=g) < left_out] = -100
+    return [None if v is None else v.to(dev, v.dtype if v.dtype == torch.int64 else dtype) for v in (x, w, b, t)]
+
+
+def _reference(x, w, b, t, smoothing=0.0, ignore=-100, weights=None):
+    """-> losses of the rows, d of the logits with the weights of the rows in it, (dx, dw, db), all float64."""
+    x, w = x.double(), w.double()
+    classes = w.shape[0]
+    z = x @ w.t().contiguous() + (0 if b is None else b.double())
+    live = (t != ignore) & (t >= 0) & (t < classes)
+    rows = torch.arange(x.shape[0], device=x.device)[live]
+    lse = torch.logsumexp(z, 1)
+    loss = torch.zeros_like(lse)
+    loss[live] = lse[live] - (1 - smoothing) * z[rows, t[live]]
+    if smoothing:
+        loss[live] -= smoothing * z[live].mean(1)
+    weights = live.double() / max(1, int(live.sum())) if weights is None else live * weights.double()
+    d = torch.exp(z - lse[:, None]) - smoothing / classes
+    d[rows, t[live]] -= 1 - smoothing
+    d = torch.where(live[:, None], d * weights[:, None], torch.zeros_like(d))
+    x = torch.where(live[:, None], x, torch.zeros_like(x))
+    return loss, weights, d, (d @ w, d.t().contiguous() @ x, d.sum(0))
+
+
+def _tolerance(x, w):
+    return HALF * (8 + 2 * math.sqrt(6 * max(*x.shape, *w.shape) / 16))
+
+
+def _near(got, want, tol, floor=0.0):
+    assert torch.isfinite(got).all()
+    assert float((got.double() - want).norm()) <= tol * float(want.norm()) + floor
+
+
+def _check(x, w, b, t, smoothing=0.0, reduction="mean", ignore=-100, grad=None):
+    from vtpack_amd.layers import linear_cross_entropy
+    leaves = [None if v is None else v.detach().requires_grad_() for v in (x, w, b)]
+    loss = linear_cross_entropy(*leaves, t, ignore_index=ignore, label_smoothing=smoothing, reduction=reduction)
+    scale = grad if grad is not None else torch.ones((), device=x.device) if reduction == "sum" else None
+    want, weights, d, grads = _reference(x, w, b, t, smoothing, ignore, scale)
+    tol = _tolerance(x, w)
+    # of a loss: of the logits it is the difference of
+    size = 1 + float((x.double().nan_to_num(0, 0, 0) @ w.double().t()).abs().max()) if x.shape[0] * w.shape[0] < 1 << 22 else 16.0
+    if reduction == "none":
+        assert (loss.double() - want).abs().max() <= tol * size
+    else:
+        total = want.sum() if reduction == "sum" else (want * weights).sum()
+        assert abs(float(loss.detach()) - float(total)) <= tol * size * (x.shape[0] if reduction == "sum" else 1)
+    got = torch.autograd.grad(loss, [v for v in leaves if v is not None], grad)
+    for name, g, r in zip("xwb", got, grads):
+        assert g.dtype == x.dtype and g.shape == r.shape
+        if x.dtype == torch.float32:
+            _near(g, r, tol, 1e-30)
+        else:
+            e = 2.0 ** -8 * r.abs() + tol * float(r.abs().max())
+            if name == "x":
+                e = e + 2.0 ** -8 * (d.abs() @ w.double().abs()) * 1.01
+            elif name == "w":
+                e = e + 2.0 ** -8 * (d.abs().t().contiguous() @ x.nan_to_num(0, 0, 0).double().abs()) * 1.01
+            over = float(((g.double() - r).abs() / (e + 1e-30)).max())
+            assert over <= 1, name
+    return loss, got
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,classes,width", [(1, 1, 1), (1, 2, 8), (2, 10, 64), (3, 1000, 192), (127, 129, 65), (128, 128, 128),
+                                                (129, 127, 63), (64, 1000, 384), (255, 257, 200), (300, 130, 72), (1021, 1000, 384),
+                                                (65, 2049, 320), (17, 3, 1027)])
+def test_sizes(dev, dtype, rows, classes, width):
+    _check(*_operands(dev, rows, classes, width, dtype))
+    _check(*_operands(dev, rows, classes, width, dtype, seed=1, bias=False), smoothing=0.1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_rows_left_out(dev, dtype, reduction):
+    """Padding, targets that are no class, features of such rows that are not finite; a weight for every row."""
+    x, w, b, t = _operands(dev, 200, 300, 96, dtype, left_out=0.3)
+    t[3], t[4], t[150] = 300, -7, 1 << 40
+    x[t < 0] = float("nan")
+    x[3], x[150] = float("inf"), float("-inf")
+    grad = None
+    if reduction == "none":
+        grad = torch.rand(200, generator=torch.Generator().manual_seed(5)).to(dev) + 0.5
+    loss, got = _check(x, w, b, t, smoothing=0.1, reduction=reduction, grad=grad)
+    out = (t < 0) | (t >= 300)
+    assert not got[0][out].any()
+    if reduction == "none":
+        assert not loss[out].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_no_row_counts(dev, dtype):
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 20, 30, 64, dtype)
+    x[:] = float("nan")
+    t[:] = -100
+    leaves = [v.requires_grad_() for v in (x, w, b)]
+    loss = linear_cross_entropy(*leaves, t)
+    assert float(loss.detach()) == 0.0
+    for g in torch.autograd.grad(loss, leaves):
+        assert not g.any()
+    empty = [x.detach()[:0].requires_grad_(), w, b]
+    loss = linear_cross_entropy(*empty, t[:0])
+    assert float(loss) == 0.0
+    for g, v in zip(torch.autograd.grad(loss, empty), empty):
+        assert g.shape == v.shape and not g.any()
+    assert linear_cross_entropy(*empty, t[:0], reduction="none").shape == (0,)
+
+
+def test_ignore_index_that_is_a_class(dev):
+    x, w, b, t = _operands(dev, 100, 10, 64, torch.float32)
+    _check(x, w, b, t, ignore=3)
+
+
+def test_classes_shut_out_by_the_bias(dev):
+    """A bias of -inf takes a class out of the sum; a row whose own class it is loses all, and its gradients stay finite."""
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 90, 400, 64, torch.float32)
+    b[::3] = float("-inf")
+    t = t // 3 * 3 + 1
+    t[t >= 400] = 1
+    loss, got = _check(x, w, b, t)
+    assert not got[1][::3].any()
+    b[:] = float("-inf")
+    b[7] = 0.0
+    assert torch.equal(linear_cross_entropy(x, w, b, torch.full_like(t, 7), reduction="none"), torch.zeros(90, device=dev))
+    assert linear_cross_entropy(x, w, b, torch.full_like(t, 8), reduction="none").isposinf().all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_not_a_number(dev, dtype):
+    """A NaN or an infinity in a row that counts shows in its loss and leaves the other rows' alone."""
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 140, 150, 64, dtype)
+    want = linear_cross_entropy(x, w, b, t, reduction="none")
+    x[7, 3], x[131, 0] = float("nan"), float("inf")
+    got = linear_cross_entropy(x, w, b, t, reduction="none")
+    rest = torch.ones(140, dtype=torch.bool, device=dev)
+    rest[7] = rest[131] = False
+    assert torch.equal(got[rest], want[rest]) and not torch.isfinite(got[~rest]).any()
+
+
+def test_large_logits(dev):
+    """Logits of hundreds: the loss is a difference of neighbours, not of sums."""
+    x, w, b, t = _operands(dev, 64, 128, 64, torch.float32)
+    _check(x * 30, w * 10, b, t)
+
+
+@pytest.mark.parametrize("dtype,rows,classes,width", [(torch.bfloat16, 8192, 21841, 128), (torch.float32, 4096, 12000, 64), (torch.bfloat16, 1, 70001, 256),
+                                                      (torch.float32, 3, 40000, 100), (torch.bfloat16, 9000, 3, 64)])
+def test_pieces_and_long_sums(dev, dtype, rows, classes, width):
+    """More classes than a piece holds; one row against many classes and the other way around, where sums are cut."""
+    _check(*_operands(dev, rows, classes, width, dtype, left_out=0.1 if rows > 10 else 0.0))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_strides_and_places(dev, dtype):
+    """Rows apart, columns of a wider matrix, storage off the 16-byte boundary, leading dimensions, expanded gradients."""
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 60, 70, 64, dtype)
+    want = [linear_cross_entropy(x, w, b, t), *_check(x, w, b, t)[1]]
+    wide = torch.zeros(60, 200, dtype=dtype, device=dev)
+    wide[:, 3:67] = x
+    off = torch.zeros(70 * 64 + 1, dtype=dtype, device=dev)
+    off[1:] = w.reshape(-1)
+    for xs, ws in ((wide[:, 3:67], off[1:].view(70, 64)), (x.t().contiguous().t(), w.t().contiguous().t())):
+        xs, ws = xs.detach().requires_grad_(), ws.detach().requires_grad_()
+        bs = b.detach().requires_grad_()
+        loss = linear_cross_entropy(xs, ws, bs, t)
+        got = [loss, *torch.autograd.grad(loss, [xs, ws, bs])]
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    cube = x.view(3, 4, 5, 64).detach().requires_grad_()
+    rows = linear_cross_entropy(cube, w, b, t.view(3, 4, 5), reduction="none")
+    assert rows.shape == (3, 4, 5)
+    rows.sum().backward()
+    assert torch.equal(cube.grad.view(60, 64), _check(x, w, b, t, reduction="sum")[1][0])
+
+
+def test_only_what_is_needed(dev):
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 50, 60, 64, torch.float32)
+    full = _check(x, w, b, t)[1]
+    for i in range(3):
+        leaves = [v.detach().requires_grad_(k == i) for k, v in enumerate((x, w, b))]
+        linear_cross_entropy(*leaves, t).backward()
+        assert torch.equal(leaves[i].grad, full[i])
+
+
+def test_result_may_be_changed_in_place(dev):
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 50, 60, 64, torch.float32)
+    want = _check(x, w, b, t)[1][0]
+    x = x.detach().requires_grad_()
+    loss = linear_cross_entropy(x, w, b, t)
+    loss /= 2
+    loss.backward()
+    assert torch.equal(x.grad, want / 2)
+
+
+def test_against_differences(dev):
+    """The gradient of the loss against its differences along random directions: fp32 losses of about 5, steps of 1e-2."""
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 40, 50, 64, torch.float32, left_out=0.2)
+    got = _check(x, w, b, t, smoothing=0.2)[1]
+    g = torch.Generator().manual_seed(1)
+    for i in range(3):
+        v = torch.randn((x, w, b)[i].shape, generator=g).to(dev)
+        v /= v.norm()
+        at = [[p + s * 1e-2 * v if k == i else p for k, p in enumerate((x, w, b))] for s in (1, -1)]
+        up, down = (float(_reference(*a, t, 0.2)[0].sum() / int((t >= 0).sum())) for a in at)
+        # a difference of step h is off by h^2 / 6 of the third derivative, which is below 1 here
+        assert abs((up - down) / 2e-2 - float((got[i] * v).sum())) <= 1e-4 / 6 + 1e-5
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_same_bits_on_another_stream_and_in_a_graph(dev, dtype):
+    from vtpack_amd import ops
+    x, w, b, t = _operands(dev, 700, 1500, 192, dtype, left_out=0.1)
+    g = torch.ones((), device=dev)
+
+    def run():
+        rows, loss, saved = ops.cross_entropy(x, w, b, t, -100, 0.1, "mean")
+        return [rows, loss, *ops.cross_entropy_backward(x, w, b, t, saved, g, -100, 0.1)]
+
+    want = [v.clone() for v in run()]
+    assert all(torch.equal(p, q) for p, q in zip(run(), want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = run()
+    side.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for k in range(3):
+        x.copy_(x.roll(1, 0))
+        t.copy_(t.roll(1, 0))
+        graph.replay()
+        torch.cuda.synchronize()
+        again = run()
+        assert all(torch.equal(p, q) for p, q in zip(out, again)), k
+
+
+def test_refusals(dev):
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 8, 9, 16, torch.float32)
+    for args, kw, error in [((x, w.bfloat16(), b, t), {}, TypeError), ((x.half(), w.half(), b.half(), t), {}, TypeError),
+                            ((x, w, b, t.int()), {}, TypeError), ((x, w, b, t.cpu()), {}, RuntimeError), ((x, w[:, :8], b, t), {}, ValueError),
+                            ((x, w, b[:3], t), {}, ValueError), ((x, w, b, t[:3]), {}, ValueError), ((x, w, b, t), {"reduction": "max"}, ValueError),
+                            ((x, w, b, t), {"label_smoothing": 1.5}, ValueError), ((x, w[:0], b[:0], t), {}, ValueError)]:
+        with pytest.raises(error):
+            linear_cross_entropy(*args, **kw)
+    with pytest.raises(RuntimeError):                    # gradients of the gradients are not to be had
+        x = x.requires_grad_()
+        dx, = torch.autograd.grad(linear_cross_entropy(x, w, b, t), x, create_graph=True)
+        dx.sum().backward()

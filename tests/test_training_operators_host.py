@@ -1,0 +1,102 @@
+"""The operators of a training step without a GPU: what they refuse, and the checks of the library's arguments."""
+import ctypes
+
+import pytest
+import torch
+
+from vtpack_amd import _lib
+from vtpack_amd.layers import gate_balance, linear_cross_entropy
+from vtpack_amd.optim import AdamW
+
+
+def test_tensors_on_the_cpu_are_refused():
+    x, w, t = torch.randn(4, 8), torch.randn(3, 8), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        linear_cross_entropy(x, w, None, t)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        gate_balance(x)
+    p = torch.nn.Parameter(x)
+    p.grad = x.clone()
+    with pytest.raises(RuntimeError, match="GPU only"):
+        AdamW([p]).step()
+
+
+@pytest.mark.parametrize("kw", [{"lr": -1.0}, {"betas": (1.0, 0.9)}, {"betas": (0.9, -0.1)}, {"eps": -1e-8}, {"weight_decay": -1.0},
+                                {"state_bits": 16}, {"lr": torch.tensor(1e-3)}, {"lr": torch.tensor(1e-3), "capturable": True},
+                                {"lr": float("nan")}])
+def test_settings_of_the_optimizer(kw):
+    with pytest.raises(ValueError):
+        AdamW([torch.nn.Parameter(torch.zeros(3))], **kw)
+
+
+def test_a_step_without_gradients_does_nothing():
+    opt = AdamW([torch.nn.Parameter(torch.zeros(3))])
+    assert opt.step(lambda: 5.0) == 5.0 and opt.param_groups[0]["step"] == 0
+
+
+def test_state_dict_round_trip_without_steps():
+    p = torch.nn.Parameter(torch.zeros(3))
+    opt = AdamW([p], lr=0.5, state_bits=8)
+    other = AdamW([p])
+    other.load_state_dict(opt.state_dict())
+    assert other.param_groups[0]["state_bits"] == 8 and other.param_groups[0]["lr"] == 0.5
+
+
+class _Tensor(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")] + [("n", ctypes.c_int64)]
+
+
+def test_arguments_of_the_library():
+    """Before anything is launched."""
+    lib = _lib.load()
+    p = 4096                                              # never read: the sizes are refused first
+    ce = [p, 8, p, 8, p, p, 4, 3, 8, -100, 0.0, p, 1 << 40, p, p, p, p, p, 0, None]
+
+    def call(**put):
+        args = list(ce)
+        for i, v in put.items():
+            args[int(i[1:])] = v
+        return lib.vtdge_cross_entropy(*args)
+
+    assert call(_0=None) == _lib.ERR_ARG and b"NULL" in lib.vtdge_last_error()
+    assert call(_18=7) == _lib.ERR_ARG                    # type
+    assert call(_1=7) == _lib.ERR_ARG                     # rows that overlap
+    assert call(_6=0) == _lib.ERR_ARG and call(_7=0) == _lib.ERR_ARG and call(_8=0) == _lib.ERR_ARG
+    assert call(_6=1 << 24) == _lib.ERR_UNSUPPORTED and call(_8=(1 << 16) + 1) == _lib.ERR_UNSUPPORTED
+    assert call(_10=1.5) == _lib.ERR_ARG and call(_10=float("nan")) == _lib.ERR_ARG
+    assert call(_12=0) == _lib.ERR_ARG and b"workspace" in lib.vtdge_last_error()
+    assert call(_11=p + 16) == _lib.ERR_ARG               # a workspace off its boundary
+    assert call(_16=None) == _lib.ERR_ARG                 # a count of rows without their mean
+    assert lib.vtdge_cross_entropy_workspace(4, 3, 0, 0, 0) == -1
+    back = [p, 8, p, 8, p, p, p, p, p, 1, p, 4, 3, 8, -100, 0.0, p, 1 << 40, p, p, p, 0, None]
+    assert lib.vtdge_cross_entropy_backward(*back) == _lib.ERR_ARG and b"grad_stride" in lib.vtdge_last_error()
+    gb = [p, 3, None, None, 100, 3, 1, None, 0, p, p, p, 0, None]
+    for i, v, want in ((4, 0, -1), (5, 0, -1), (5, 513, -1), (6, 4, -1), (6, 0, -1), (1, 2, -1), (12, 5, -1), (4, 1 << 31, -2), (4, 100000, -1)):
+        args = list(gb)
+        args[i] = v
+        assert lib.vtdge_gate_balance(*args) == want, (i, v)
+    args = list(gb)
+    args[1] = args[5] = 513
+    assert lib.vtdge_gate_balance(*args) == _lib.ERR_UNSUPPORTED
+    table = (_Tensor * 1)(_Tensor(p, p, p, p, None, None, 10))
+    at = ctypes.addressof(table)
+    adamw = [at, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, None, 0, 32, None]
+    for i, v, want in ((1, -1, -1), (2, -1.0, -1), (3, 1.0, -1), (4, 1.5, -1), (5, -1.0, -1), (6, -1.0, -1), (7, 0, -1), (9, 3, -1), (10, 16, -2),
+                       (10, 8, -1)):                     # (8-bit moments without scales)
+        args = list(adamw)
+        args[i] = v
+        assert lib.vtdge_adamw(*args) == want, (i, v)
+    assert lib.vtdge_adamw(None, 0, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, None, 0, 32, None) == 0
+    table[0].n = 0
+    table[0].param = None
+    assert lib.vtdge_adamw(*adamw) == 0                   # nothing to do, nothing touched
+    assert lib.vtdge_adamw_scalars(None, 0, 1, None, 1e-3, 0.9, 0.999, 1e-8, 0.0, p, None) == _lib.ERR_ARG
+
+
+def test_workspaces_follow_the_sizes():
+    lib = _lib.load()
+    size = lib.vtdge_cross_entropy_workspace
+    assert size(256, 1000, 384, 1, 0) % 256 == 0 and size(256, 1000, 384, 1, 0) < size(256, 1000, 384, 0, 0)
+    # d of a piece: no more than 128 MB, or eight tiles of classes, however many classes there are
+    assert size(8192, 65536, 1024, 1, 1) < (128 << 20) + 2 * 65536 * 1024 * 2 + 3 * 8192 * 1024 * 4 + (8 << 20) * 4 * 2
+    assert lib.vtdge_gate_balance_workspace(100, 8) == 0 and lib.vtdge_gate_balance_workspace(1 << 20, 8) == 512 * 17 * 4

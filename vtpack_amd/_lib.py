@@ -22,6 +22,7 @@ _p = ctypes.c_void_p
 _i = ctypes.c_int
 _l = ctypes.c_int64
 _f = ctypes.c_float
+_d = ctypes.c_double
 
 # name -> argtypes, in the order of include/vtdge.h
 SIGNATURES = {
@@ -88,9 +89,17 @@ SIGNATURES = {
     "vtdge_block_tail_fits": [_l, _i, _i, _i],
     "vtdge_block_tail_wanted": [_l, _i, _i, _i],
     "vtdge_block_tail": [_p, _p, _p, _p, _p, _p, _f, _p, _p, _p, _p, _p, _p, _l, _i, _i, _i, _p],
+    "vtdge_gate_balance": [_p, _l, _p, _p, _l, _i, _i, _p, _l, _p, _p, _p, _i, _p],
+    "vtdge_gate_balance_backward": [_p, _l, _p, _p, _p, _p, _l, _i, _i, _p],
+    "vtdge_cross_entropy": [_p, _l, _p, _l, _p, _p, _l, _l, _i, _l, _f, _p, _l, _p, _p, _p, _p, _p, _i, _p],
+    "vtdge_cross_entropy_backward": [_p, _l, _p, _l, _p, _p, _p, _p, _p, _i, _p, _l, _l, _i, _l, _f, _p, _l, _p, _p, _p, _i,
+                                     _p],
+    "vtdge_adamw": [_p, _i, _d, _d, _d, _d, _d, _l, _p, _i, _i, _p],
+    "vtdge_adamw_scalars": [_p, _l, _i, _p, _d, _d, _d, _d, _d, _p, _p],
     "vtdge_chain_layout": [_p, _p],
     "vtdge_chain_forward": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p],
 }
+ADAMW_SCALARS = 64                                     # include/vtdge.h
 CHAIN_PARAMS, CHAIN_LAYOUT_HEAD, CHAIN_LAYOUT_BLOCK = 35, 8, 8      # include/vtdge.h
 
 
@@ -143,6 +152,10 @@ def load():
     lib.vtdge_decompress_router_compress_workspace.argtypes = [_i, _i, _i, _i]
     lib.vtdge_region_step_workspace.restype = _l
     lib.vtdge_region_step_workspace.argtypes = [_i, _i, _i]
+    lib.vtdge_gate_balance_workspace.restype = _l
+    lib.vtdge_gate_balance_workspace.argtypes = [_l, _i]
+    lib.vtdge_cross_entropy_workspace.restype = _l
+    lib.vtdge_cross_entropy_workspace.argtypes = [_l, _l, _i, _i, _i]
     for name, args in SIGNATURES.items():
         fn = getattr(lib, name)
         fn.restype = _i

@@ -1,0 +1,358 @@
+// One AdamW step over many tensors (gfx950):  p *= 1 - lr wd;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
+// p -= lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps), moments in fp32 or in 8 bits.
+//
+// Bound by memory: 28 bytes an element in fp32, 22 with bf16 weights, 16 and 10 with 8-bit moments.  The tensors of a launch are a
+// table in its arguments (no copy to the device, nothing to keep between calls), a workgroup takes a chunk of one of them and finds
+// it by halving.  A wave takes 256 consecutive elements at a time, four a lane: weights, gradients and moments all come in one load
+// a lane, and the 256 are the block that shares a scale, so that its largest magnitude is one reduction over the wave.
+//
+// Moments in 8 bits: the first as e4m3 over max|m| / 448, the second as e5m2 over max v / 57344.  Adam's slow decay (b2 = 0.999)
+// is far below half a step of either (1/16 and 1/8), and would be lost under rounding to the nearest; a value is therefore rounded
+// down or up at random, by 16 random bits added below the last bit that stays, a hash of the element's place in its tensor and of t:
+// the same on every run, unbiased to 2^-17 of a step.  A second moment above zero does not become zero, where it would let a
+// weight jump by m / eps.  What the codes are made from (m, v, their quotients by the scale) is rounded to fp32 at each
+// operation as written, products and sums apart.  A block whose largest magnitude is below 2^-100 is stored as zeros.  Magnitudes
+// compare as integers, where NaN is above infinity: a block with either gets a scale that shows it.
+#include "common.h"
+
+#include <math.h>
+
+namespace vtdge {
+
+constexpr int OPT_BLOCK = 256;                  // elements of a scale, and of a wave
+constexpr int OPT_CHUNK = 4096;                 // elements of a workgroup
+constexpr int OPT_WAVES = 4;
+constexpr int64_t OPT_MOST_CHUNKS = (1 << 24) - 1;      // of a launch: fewer than 2^32 threads
+
+struct OptScalars {                             // of one step, in fp32; also what vtdge_adamw_scalars leaves on the device
+    float decay, beta1, rest1, beta2, rest2, size, root, eps;
+    uint32_t step;
+};
+
+template <int BITS> struct OptTable {
+    // 4 KB of kernel arguments hold this many tensors
+    static constexpr int MOST = BITS == 8 ? 64 : 92;
+    void *p[MOST];
+    const void *g[MOST];
+    void *m[MOST];
+    void *v[MOST];
+    float *ms[BITS == 8 ? MOST : 1];
+    float *vs[BITS == 8 ? MOST : 1];
+    uint32_t first[MOST];                       // chunk it starts with
+    uint32_t last[MOST];                        // elements of its last chunk, 1 .. OPT_CHUNK
+    uint32_t count, chunks;
+};
+static_assert(sizeof(OptTable<8>) + sizeof(OptScalars) + 8 <= 4096 && sizeof(OptTable<32>) + sizeof(OptScalars) + 8 <= 4096, "arguments");
+
+// ---- four elements of a lane: a vector where the tensor's buffers allow it, else one by one
+template <typename T> struct Four;
+template <> struct Four<float> {
+    static __device__ __forceinline__ void load(const float *p, float (&f)[4])
+    {
+        const f32x4 r = *reinterpret_cast<const f32x4 *>(p);
+        f[0] = r.x, f[1] = r.y, f[2] = r.z, f[3] = r.w;
+    }
+    static __device__ __forceinline__ void store(float *p, const float (&f)[4]) { *reinterpret_cast<f32x4 *>(p) = f32x4{f[0], f[1], f[2], f[3]}; }
+};
+template <> struct Four<bf16_t> {
+    static __device__ __forceinline__ void load(const bf16_t *p, float (&f)[4])
+    {
+        const u32x2 r = *reinterpret_cast<const u32x2 *>(p);
+        f[0] = bf16lo(r.x), f[1] = bf16hi(r.x), f[2] = bf16lo(r.y), f[3] = bf16hi(r.y);
+    }
+    static __device__ __forceinline__ void store(bf16_t *p, const float (&f)[4])
+    {
+        *reinterpret_cast<u32x2 *>(p) = u32x2{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
+    }
+};
+template <typename T> __device__ __forceinline__ void load4(const T *p, int live, bool whole, float (&f)[4])
+{
+    if (whole) {
+        Four<T>::load(p, f);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) f[e] = e < live ? Elem<T>::load(p + e) : 0.f;
+    }
+}
+template <typename T> __device__ __forceinline__ void store4(T *p, int live, bool whole, const float (&f)[4])
+{
+    if (whole) {
+        Four<T>::store(p, f);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (e < live) Elem<T>::store(p + e, f[e]);
+    }
+}
+__device__ __forceinline__ uint32_t load_codes(const uint8_t *p, int live, bool whole)
+{
+    if (whole) return *reinterpret_cast<const uint32_t *>(p);
+    uint32_t c = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (e < live) c |= (uint32_t)p[e] << (8 * e);
+    return c;
+}
+__device__ __forceinline__ void store_codes(uint8_t *p, int live, bool whole, uint32_t c)
+{
+    if (whole) {
+        *reinterpret_cast<uint32_t *>(p) = c;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (e < live) p[e] = (uint8_t)(c >> (8 * e));
+    }
+}
+
+// ---- 8-bit codes.  M bits of mantissa, SMALL the smallest normal number: FIRST is e4m3, else e5m2.
+template <bool FIRST> __device__ __forceinline__ void decode4(uint32_t codes, float scale, float (&f)[4])
+{
+    f32x2 lo, hi;
+    if constexpr (FIRST) {
+        lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
+        hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
+    } else {
+        lo = __builtin_amdgcn_cvt_pk_f32_bf8((int)codes, false);
+        hi = __builtin_amdgcn_cvt_pk_f32_bf8((int)codes, true);
+    }
+    f[0] = lo.x * scale, f[1] = lo.y * scale, f[2] = hi.x * scale, f[3] = hi.y * scale;
+}
+// largest of the wave as an integer
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v)
+{
+#define VT_UMAX(ctrl, mask)                                                                                          \
+    {                                                                                                                \
+        const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, mask, 0xf, true);                  \
+        v = v > o ? v : o;                                                                                           \
+    }
+    VT_UMAX(0x111, 0xf)
+    VT_UMAX(0x112, 0xf)
+    VT_UMAX(0x114, 0xf)
+    VT_UMAX(0x118, 0xf)
+    VT_UMAX(0x142, 0xa)
+    VT_UMAX(0x143, 0xc)
+#undef VT_UMAX
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+// the wave's 256 values as codes, and their scale
+template <bool FIRST> __device__ __forceinline__ uint32_t encode4(const float (&f)[4], const uint32_t (&noise)[4], float &scale)
+{
+#pragma clang fp contract(off)
+    constexpr float TOP = FIRST ? 448.f : 57344.f, SMALL = FIRST ? 0x1p-6f : 0x1p-14f;
+    constexpr int DROP = FIRST ? 20 : 21;
+    uint32_t most = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const uint32_t a = __float_as_uint(f[e]) & 0x7fffffffu;
+        most = most > a ? most : a;
+    }
+    most = wave_umax(most);
+    const bool zero = most < 0x0d800000u;       // 2^-100
+    scale = zero ? 0.f : __uint_as_float(most) * (1.0f / TOP);
+    const float inverse = zero ? 0.f : TOP / __uint_as_float(most);
+    float q[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float x = fminf(fabsf(f[e]) * inverse, TOP);
+        const float lift = x < SMALL ? SMALL : 0.f;            // in the octave above SMALL the last bit kept is that of the numbers below
+        const uint32_t n = (FIRST ? noise[e] & 0xffffu : noise[e] >> 16) << (DROP - 16);
+        const uint32_t kept = (__float_as_uint(x + lift) + n) & ~((1u << DROP) - 1);
+        float r = __uint_as_float(kept) - lift;
+        if (!FIRST && x > 0.f) r = fmaxf(r, 0x1p-16f);
+        q[e] = __builtin_copysignf(r, f[e]);
+    }
+    uint32_t c = 0;
+    if constexpr (FIRST) {
+        c = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+        c = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], (int)c, true);
+    } else {
+        c = (uint32_t)__builtin_amdgcn_cvt_pk_bf8_f32(q[0], q[1], 0, false);
+        c = (uint32_t)__builtin_amdgcn_cvt_pk_bf8_f32(q[2], q[3], (int)c, true);
+    }
+    return c;
+}
+// 32 random bits of an element: odd multipliers, the first 32 bits behind the point of the roots of 2, 3, 5 and 7, last bit set
+__device__ __forceinline__ uint32_t dither(uint32_t place, uint32_t step)
+{
+    uint32_t h = place * 0x6a09e667u + step * 0xbb67ae85u;
+    h = (h ^ (h >> 16)) * 0x3c6ef373u;
+    h = (h ^ (h >> 15)) * 0xa54ff53bu;
+    return h ^ (h >> 16);
+}
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(64 * OPT_WAVES) void adamw_kernel(OptTable<BITS> t, OptScalars host, const OptScalars *__restrict__ device)
+{
+#pragma clang fp contract(off)
+    const OptScalars s = device != nullptr ? *device : host;
+    // the tensor of this chunk: the last one that starts at or before it
+    uint32_t at = 0, end = t.count;
+    while (end - at > 1) {
+        const uint32_t mid = (at + end) >> 1;
+        if (t.first[mid] <= blockIdx.x) at = mid;
+        else end = mid;
+    }
+    const uint32_t chunk = blockIdx.x - t.first[at];
+    const bool is_last = blockIdx.x + 1 == (at + 1 < t.count ? t.first[at + 1] : t.chunks);
+    const int live = is_last ? (int)t.last[at] : OPT_CHUNK;
+    const int64_t base = (int64_t)chunk * OPT_CHUNK;
+    T *const p = static_cast<T *>(t.p[at]) + base;
+    const T *const g = static_cast<const T *>(t.g[at]) + base;
+    const uint64_t places = (uint64_t)(uintptr_t)p | (uint64_t)(uintptr_t)g;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if constexpr (BITS == 32) {
+        float *const m = static_cast<float *>(t.m[at]) + base, *const v = static_cast<float *>(t.v[at]) + base;
+        const bool vec = (places % (4 * sizeof(T))) == 0 && (((uintptr_t)m | (uintptr_t)v) & 15) == 0;
+        for (int i = wave * OPT_BLOCK + lane * 4; i < live; i += OPT_WAVES * OPT_BLOCK) {
+            const bool whole = vec && i + 4 <= live;
+            float fp[4], fg[4], fm[4], fv[4];
+            load4(p + i, live - i, whole, fp);
+            load4(g + i, live - i, whole, fg);
+            load4(m + i, live - i, whole, fm);
+            load4(v + i, live - i, whole, fv);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                fm[e] = fm[e] * s.beta1 + fg[e] * s.rest1;
+                fv[e] = fv[e] * s.beta2 + fg[e] * s.rest2 * fg[e];
+                fp[e] = fp[e] * s.decay - s.size * (fm[e] / (sqrtf(fv[e]) * s.root + s.eps));
+            }
+            store4(p + i, live - i, whole, fp);
+            store4(m + i, live - i, whole, fm);
+            store4(v + i, live - i, whole, fv);
+        }
+    } else {
+        uint8_t *const m = static_cast<uint8_t *>(t.m[at]) + base, *const v = static_cast<uint8_t *>(t.v[at]) + base;
+        float *const ms = t.ms[at] + (int64_t)chunk * (OPT_CHUNK / OPT_BLOCK), *const vs = t.vs[at] + (int64_t)chunk * (OPT_CHUNK / OPT_BLOCK);
+        const bool vec = (places % (4 * sizeof(T))) == 0 && (((uintptr_t)m | (uintptr_t)v) & 3) == 0;
+        for (int b = wave; b * OPT_BLOCK < live; b += OPT_WAVES) {
+            const int i = b * OPT_BLOCK + lane * 4;           // lanes behind the tensor's end hold zeros
+            const bool whole = vec && i + 4 <= live;
+            float fp[4], fg[4], fm[4], fv[4];
+            load4(p + i, live - i, whole, fp);
+            load4(g + i, live - i, whole, fg);
+            const uint32_t cm = load_codes(m + i, live - i, whole), cv = load_codes(v + i, live - i, whole);
+            decode4<true>(cm, ms[b], fm);
+            decode4<false>(cv, vs[b], fv);
+            uint32_t noise[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                fm[e] = fm[e] * s.beta1 + fg[e] * s.rest1;
+                fv[e] = fv[e] * s.beta2 + fg[e] * s.rest2 * fg[e];
+                if (i + e >= live) fm[e] = fv[e] = 0.f;        // (0 times a scale that is not finite)
+                fp[e] = fp[e] * s.decay - s.size * (fm[e] / (sqrtf(fv[e]) * s.root + s.eps));
+                noise[e] = dither((uint32_t)(base + i + e), s.step);
+            }
+            float sm, sv;
+            const uint32_t em = encode4<true>(fm, noise, sm), ev = encode4<false>(fv, noise, sv);
+            store4(p + i, live - i, whole, fp);
+            store_codes(m + i, live - i, whole, em);
+            store_codes(v + i, live - i, whole, ev);
+            if (lane == 0) ms[b] = sm, vs[b] = sv;
+        }
+    }
+}
+
+static OptScalars scalars_of(double lr, double beta1, double beta2, double eps, double decay, int64_t step)
+{
+    OptScalars s;
+    s.decay = (float)(1.0 - lr * decay);
+    s.beta1 = (float)beta1, s.rest1 = (float)(1.0 - beta1);
+    s.beta2 = (float)beta2, s.rest2 = (float)(1.0 - beta2);
+    s.size = (float)(lr / (1.0 - pow(beta1, (double)step)));
+    s.root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+    s.eps = (float)eps;
+    s.step = (uint32_t)step;
+    return s;
+}
+
+__global__ void adamw_scalars_kernel(int64_t *step, int64_t skipped, int advance, const float *lr_dev, double lr, double beta1, double beta2, double eps, double decay,
+                                     OptScalars *out)
+{
+    const int64_t t = *step + 1 - skipped;
+    if (advance) *step += 1;
+    if (lr_dev != nullptr) lr = (double)*lr_dev;
+    OptScalars s;
+    s.decay = (float)(1.0 - lr * decay);
+    s.beta1 = (float)beta1, s.rest1 = (float)(1.0 - beta1);
+    s.beta2 = (float)beta2, s.rest2 = (float)(1.0 - beta2);
+    s.size = (float)(lr / (1.0 - pow(beta1, (double)t)));
+    s.root = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)t)));
+    s.eps = (float)eps;
+    s.step = (uint32_t)t;
+    *out = s;
+}
+
+template <typename T, int BITS>
+static int go_adamw(const vtdge_adamw_tensor *tensors, int count, const OptScalars &s, const OptScalars *device, hipStream_t st)
+{
+    OptTable<BITS> t;
+    int i = 0;
+    while (i < count) {
+        uint32_t k = 0;
+        int64_t chunks = 0;
+        for (; i < count && k < (uint32_t)OptTable<BITS>::MOST; i++) {
+            const vtdge_adamw_tensor &x = tensors[i];
+            if (x.n == 0) continue;
+            const int64_t c = ceil_div(x.n, OPT_CHUNK);
+            if (chunks + c > OPT_MOST_CHUNKS) break;
+            t.p[k] = x.param, t.g[k] = x.grad, t.m[k] = x.exp_avg, t.v[k] = x.exp_avg_sq;
+            if constexpr (BITS == 8) t.ms[k] = x.exp_avg_scale, t.vs[k] = x.exp_avg_sq_scale;
+            t.first[k] = (uint32_t)chunks;
+            t.last[k] = (uint32_t)(x.n - (c - 1) * OPT_CHUNK);
+            chunks += c;
+            k++;
+        }
+        if (k == 0) break;
+        t.count = k;
+        t.chunks = (uint32_t)chunks;
+        auto kern = adamw_kernel<T, BITS>;
+        note_kernel(reinterpret_cast<const void *>(kern));
+        kern<<<dim3((unsigned)chunks), dim3(64 * OPT_WAVES), 0, st>>>(t, s, device);
+        const int rc = check_launch("adamw");
+        if (rc != VTDGE_OK) return rc;
+    }
+    return VTDGE_OK;
+}
+
+static bool bad_rates(double lr, double beta1, double beta2, double eps, double decay)
+{
+    return !(lr >= 0) || !(beta1 >= 0 && beta1 < 1) || !(beta2 >= 0 && beta2 < 1) || !(eps >= 0) || !(decay >= 0);
+}
+
+}  // namespace vtdge
+
+using namespace vtdge;
+
+extern "C" int vtdge_adamw_scalars(int64_t *step, int64_t skipped, int advance, const float *lr_dev, double lr, double beta1,
+                                   double beta2, double eps, double weight_decay, void *scalars, void *stream)
+{
+    VT_REQUIRE(step && scalars, VTDGE_ERR_ARG, "adamw_scalars: NULL operand");
+    VT_REQUIRE(skipped >= 0, VTDGE_ERR_ARG, "adamw_scalars: skipped is %lld", (long long)skipped);
+    VT_REQUIRE(!bad_rates(lr, beta1, beta2, eps, weight_decay), VTDGE_ERR_ARG, "adamw_scalars: lr, betas, eps or weight_decay out of range");
+    note_kernel(reinterpret_cast<const void *>(adamw_scalars_kernel));
+    adamw_scalars_kernel<<<1, 1, 0, (hipStream_t)stream>>>(step, skipped, advance, lr_dev, lr, beta1, beta2, eps, weight_decay, (OptScalars *)scalars);
+    return check_launch("adamw_scalars");
+}
+
+extern "C" int vtdge_adamw(const vtdge_adamw_tensor *tensors_host, int count, double lr, double beta1, double beta2, double eps,
+                           double weight_decay, int64_t step, const void *scalars, int dtype, int state_bits, void *stream)
+{
+    VT_REQUIRE(count >= 0 && (tensors_host || count == 0), VTDGE_ERR_ARG, "adamw: bad table of %d tensors", count);
+    VT_REQUIRE(dtype == VTDGE_F32 || dtype == VTDGE_BF16, VTDGE_ERR_ARG, "adamw: dtype %d", dtype);
+    VT_REQUIRE(state_bits == 32 || state_bits == 8, VTDGE_ERR_UNSUPPORTED, "adamw: moments of %d bits", state_bits);
+    VT_REQUIRE(scalars != nullptr || (step >= 1 && !bad_rates(lr, beta1, beta2, eps, weight_decay)), VTDGE_ERR_ARG,
+               "adamw: step, lr, betas, eps or weight_decay out of range");
+    const int64_t most = OPT_MOST_CHUNKS * OPT_CHUNK;
+    for (int i = 0; i < count; i++) {
+        const vtdge_adamw_tensor &x = tensors_host[i];
+        VT_REQUIRE(x.n >= 0 && x.n <= most, VTDGE_ERR_ARG, "adamw: tensor %d has %lld elements", i, (long long)x.n);
+        VT_REQUIRE(x.n == 0 || (x.param && x.grad && x.exp_avg && x.exp_avg_sq && (state_bits == 32 || (x.exp_avg_scale && x.exp_avg_sq_scale))),
+                   VTDGE_ERR_ARG, "adamw: NULL operand in tensor %d", i);
+    }
+    const OptScalars s = scalars != nullptr ? OptScalars{} : scalars_of(lr, beta1, beta2, eps, weight_decay, step);
+    const OptScalars *device = (const OptScalars *)scalars;
+    const hipStream_t st = (hipStream_t)stream;
+    if (dtype == VTDGE_F32)
+        return state_bits == 32 ? go_adamw<float, 32>(tensors_host, count, s, device, st) : go_adamw<float, 8>(tensors_host, count, s, device, st);
+    return state_bits == 32 ? go_adamw<bf16_t, 32>(tensors_host, count, s, device, st) : go_adamw<bf16_t, 8>(tensors_host, count, s, device, st);
+}

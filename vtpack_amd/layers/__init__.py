@@ -11,3 +11,7 @@ from .sparse_ops import (
     batched_sparse_gemm,
     batched_sparse_attention,
 )
+from .losses import (
+    gate_balance,
+    linear_cross_entropy,
+)

@@ -1,0 +1,114 @@
+"""The losses of a training step behind the encoder: the classifier's cross entropy (the reference trains with timm's, main.py:346-352,
+on the logits of `model.head`) and the balance of the routers' gates, which stands beside the budget loss of the harness."""
+import torch
+from torch.autograd import Function
+from torch.autograd.function import once_differentiable
+
+from .. import ops
+
+
+class _LinearCrossEntropy(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, ignore_index, label_smoothing, reduction):
+        loss_rows, loss, saved = ops.cross_entropy(x, weight, bias, target, ignore_index, label_smoothing, reduction)
+        ctx.how = (ignore_index, label_smoothing)
+        ctx.save_for_backward(x, weight, bias, target, *saved)
+        return loss_rows if loss is None else loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, bias, target, *saved = ctx.saved_tensors
+        # (a saved-tensor hook may lay them out anew)
+        x, weight, target = ops._rows_of(x), ops._rows_of(weight), target.contiguous()
+        if grad.dim() == 1 and grad.numel() > 1 and grad.stride(0) == 0:
+            grad = grad[0]                       # the same for every row, as a sum over the losses leaves it
+        dx, dw, db = ops.cross_entropy_backward(x, weight, bias, target, saved, grad.contiguous(), *ctx.how,
+                                                needs=ctx.needs_input_grad[:3])
+        return dx, dw, db, None, None, None, None
+
+
+def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+    """`F.cross_entropy(F.linear(x, weight, bias), target, ...)` with its gradients, without the logits in memory.
+
+    x [..., width], weight [classes, width], bias [classes] or None, all float32 or all bfloat16; target int64 of x's leading
+    shape.  -> float32: the mean over the rows that count ("mean"), their sum ("sum"), or every row's own ("none", of target's
+    shape).  A row whose target is `ignore_index` is left out, whatever its features hold; so is one whose target is no class
+    (F.cross_entropy stops the program there).  Without a row that counts the loss is 0, and so are the gradients.
+
+    The logits are fp32 sums and are not rounded; in bfloat16 the gradients of the logits are, once, before the products that
+    take them to x and weight.  Those work in pieces of the classes, with at most 128 MB of scratch for a piece and 8 rows by the
+    width for each of its tiles; float32 operands are laid out anew in three parts of two bytes for the time of a call."""
+    ops._need_gpu(x, weight, bias, target)
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError(f"reduction is {reduction!r}, expected 'mean', 'sum' or 'none'")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"label_smoothing is {label_smoothing}, expected 0 .. 1")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"features {tuple(x.shape)} do not match a weight of {tuple(weight.shape)}")
+    if x.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"vtdge kernels are built for float32 and bfloat16, got {x.dtype}")
+    ops._check_like(x, weight=weight, bias=bias)
+    ops._check_vector("bias", bias, weight.shape[0])
+    if target.dtype != torch.int64 or target.device != x.device:
+        raise TypeError(f"target is {target.dtype} on {target.device}, expected int64 on {x.device}")
+    if target.shape != x.shape[:-1]:
+        raise ValueError(f"target has shape {tuple(target.shape)}, expected {tuple(x.shape[:-1])}")
+    if x.numel() == 0:                           # no row: a loss of 0 that still belongs to its operands
+        zero = (x.sum() + weight.sum() * 0 + (0 if bias is None else bias.sum() * 0)).float()
+        return zero if reduction != "none" else zero.expand(target.shape)
+    loss = _LinearCrossEntropy.apply(ops._rows_of(x), ops._rows_of(weight), None if bias is None else bias.contiguous(),
+                                     target.reshape(-1).contiguous(), int(ignore_index), float(label_smoothing), reduction)
+    return loss.view(target.shape) if reduction == "none" else loss
+
+
+class _GateBalance(Function):
+    @staticmethod
+    def forward(ctx, gate, indices, mask, top_k):
+        loss, counts, share = ops.gate_balance(gate, indices, mask, top_k)
+        ctx.save_for_backward(gate, mask, share)
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _):
+        gate, mask, share = ctx.saved_tensors
+        mask = None if mask is None else mask.contiguous()
+        return ops.gate_balance_backward(ops._rows_of(gate), mask, share.contiguous(), grad.contiguous()), None, None, None
+
+
+def gate_balance(gate, indices=None, top_k=1, mask=None):
+    """How evenly a router's choices fall on its experts (here: granularities): -> (loss, counts).
+
+    gate [..., E] (2 .. 512 logits a token, float32 or bfloat16); loss = E sum_e f_e P_e in float32, f_e the fraction of the choices that
+    fell on e and P_e the mean softmax probability of e, with the gradient through P; counts int64 [E] are the choices.  1 is
+    even, E is all on one.  The choices are the `top_k` largest logits of a token (among equals the lowest index), or `indices`
+    int64 [..., k] (or of gate's leading shape, k = 1) if they were made elsewhere, as by a Gumbel sample.  `mask` (bool, gate's leading shape): False leaves a token
+    out, whatever its logits are; a token whose logits are all -inf is left out too.  Without a token the loss is 0."""
+    ops._need_gpu(gate, indices, mask)
+    if gate.dim() < 1 or not 1 <= gate.shape[-1] <= 512:
+        raise ValueError(f"gate has shape {tuple(gate.shape)}, expected 1 .. 512 logits a token")
+    if gate.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"vtdge kernels are built for float32 and bfloat16, got {gate.dtype}")
+    E, lead = gate.shape[-1], gate.shape[:-1]
+    if indices is not None:
+        if indices.dtype != torch.int64 or indices.device != gate.device:
+            raise TypeError(f"indices are {indices.dtype} on {indices.device}, expected int64 on {gate.device}")
+        if indices.shape == lead:
+            indices = indices.unsqueeze(-1)
+        if indices.shape[:-1] != lead or not 1 <= indices.shape[-1] <= 512:
+            raise ValueError(f"indices of shape {tuple(indices.shape)} do not match a gate of {tuple(gate.shape)}")
+        top_k = indices.shape[-1]
+        indices = indices.reshape(-1, top_k).contiguous()
+    elif not 1 <= top_k <= E:
+        raise ValueError(f"top_k is {top_k}, expected 1 .. {E}")
+    if mask is not None:
+        if mask.dtype != torch.bool or mask.device != gate.device:
+            raise TypeError(f"mask is {mask.dtype} on {mask.device}, expected bool on {gate.device}")
+        if mask.shape != lead:
+            raise ValueError(f"mask has shape {tuple(mask.shape)}, expected {tuple(lead)}")
+        mask = mask.reshape(-1).contiguous()
+    if gate.numel() == 0:
+        return gate.sum().float(), torch.zeros((E,), dtype=torch.int64, device=gate.device)
+    return _GateBalance.apply(ops._rows_of(gate), indices, mask, int(top_k))

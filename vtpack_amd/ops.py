@@ -1086,3 +1086,85 @@ def sparse_attention_backward(q, k, v, out, grad, offsets, scale, max_rows_per_s
          gs[0], ptr(offsets), ptr(dq), dqs[1], dqs[0], ptr(dk), ptr(dv), dks[1], dks[2], dks[0], ptr(work), L, B, h, d,
          n, max_rows_per_sample, float(scale), dtype_code(q), stream_ptr(), tag=("attention_backward", B, h, d, n))
     return dq, dk, dv
+
+
+# ------------------------------------------------------------------ a training step's losses
+def _on(t):
+    """The device of t made the current one, where it is not."""
+    return torch.cuda.device(t.device)
+
+
+def _rows_of(t):
+    """t [..., n] as [rows, n] with dense rows, as it lies where that can be."""
+    t = t.reshape(-1, t.shape[-1])
+    return t if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def _pitch(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _workspace(size, t):
+    if size < 0:
+        raise _lib.VtdgeError(_lib.load().vtdge_last_error().decode("utf-8", "replace"))
+    return torch.empty((size,), dtype=torch.uint8, device=t.device)
+
+
+def cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
+    """Softmax cross entropy of x [rows, width] @ weight [classes, width]^T + bias against int64 target [rows]: -> (losses of
+    the rows, their mean or sum or None, what `cross_entropy_backward` wants).  rows > 0, rows of x and weight dense."""
+    rows, width = x.shape
+    classes = weight.shape[0]
+    with _on(x):
+        ws = _workspace(_lib.load().vtdge_cross_entropy_workspace(rows, classes, width, dtype_code(x), 0), x)
+        # (memory of their own: a caller may change the losses in place, the rest is kept for the gradients)
+        loss_rows = torch.empty((rows,), dtype=torch.float32, device=x.device)
+        row_max, row_inv = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind(0)
+        loss = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=x.device)
+        inv_count = torch.empty((), dtype=torch.float32, device=x.device) if reduction == "mean" else None
+        call("vtdge_cross_entropy", x.data_ptr(), _pitch(x), weight.data_ptr(), _pitch(weight), ptr(bias), target.data_ptr(), rows,
+             classes, width, ignore_index, label_smoothing, ws.data_ptr(), ws.numel(), loss_rows.data_ptr(), row_max.data_ptr(),
+             row_inv.data_ptr(), ptr(loss), ptr(inv_count), dtype_code(x), stream_ptr(), tag=("cross_entropy", rows, classes, width))
+    return loss_rows, loss, (row_max, row_inv, inv_count)
+
+
+def cross_entropy_backward(x, weight, bias, target, saved, grad, ignore_index=-100, label_smoothing=0.0, needs=(True, True, True)):
+    """Gradients (dx, dweight, dbias; None where not needed) of `cross_entropy`; grad is fp32, a scalar or one value
+    for each row."""
+    rows, width = x.shape
+    classes = weight.shape[0]
+    row_max, row_inv, inv_count = saved
+    with _on(x):
+        ws = _workspace(_lib.load().vtdge_cross_entropy_workspace(rows, classes, width, dtype_code(x), 1), x)
+        dx = torch.empty((rows, width), dtype=x.dtype, device=x.device) if needs[0] else None
+        dw = torch.empty((classes, width), dtype=x.dtype, device=x.device) if needs[1] else None
+        db = torch.empty((classes,), dtype=x.dtype, device=x.device) if needs[2] and bias is not None else None
+        call("vtdge_cross_entropy_backward", x.data_ptr(), _pitch(x), weight.data_ptr(), _pitch(weight), ptr(bias), target.data_ptr(),
+             row_max.data_ptr(), row_inv.data_ptr(), grad.data_ptr(), grad.dim(),
+             ptr(inv_count), rows, classes, width, ignore_index, label_smoothing, ws.data_ptr(), ws.numel(), ptr(dx), ptr(dw), ptr(db),
+             dtype_code(x), stream_ptr(), tag=("cross_entropy_backward", rows, classes, width))
+    return dx, dw, db
+
+
+def gate_balance(gate, indices, mask, top_k):
+    """gate [tokens, E] with dense rows, tokens > 0; indices int64 [tokens, k] or None; mask [tokens] of bytes or None
+    -> (loss, counts int64 [E], share for `gate_balance_backward`)."""
+    tokens, E = gate.shape
+    with _on(gate):
+        ws = _workspace(_lib.load().vtdge_gate_balance_workspace(tokens, E), gate)
+        loss = torch.empty((), dtype=torch.float32, device=gate.device)
+        share = torch.empty((E + 1,), dtype=torch.float32, device=gate.device)
+        counts = torch.empty((E,), dtype=torch.int64, device=gate.device)
+        call("vtdge_gate_balance", gate.data_ptr(), _pitch(gate), ptr(indices), ptr(mask), tokens, E, top_k, ptr(ws), ws.numel(),
+             loss.data_ptr(), counts.data_ptr(), share.data_ptr(), dtype_code(gate), stream_ptr(), tag=("gate_balance", tokens, E))
+    return loss, counts, share
+
+
+def gate_balance_backward(gate, mask, share, grad):
+    """The gradient of `gate_balance`'s gate, dense, for the fp32 gradient of its loss."""
+    tokens, E = gate.shape
+    with _on(gate):
+        out = torch.empty((tokens, E), dtype=gate.dtype, device=gate.device)
+        call("vtdge_gate_balance_backward", gate.data_ptr(), _pitch(gate), ptr(mask), share.data_ptr(), grad.data_ptr(), out.data_ptr(),
+             tokens, E, dtype_code(gate), stream_ptr(), tag=("gate_balance_backward", tokens, E))
+    return out
