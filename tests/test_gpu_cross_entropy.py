@@ -81,6 +81,8 @@ def _check(x, w, b, t, smoothing=0.0, reduction="mean", ignore=-100, grad=None):
                 e = e + 2.0 ** -8 * (d.abs() @ w.double().abs()) * 1.01
             elif name == "w":
                 e = e + 2.0 ** -8 * (d.abs().t().contiguous() @ x.nan_to_num(0, 0, 0).double().abs()) * 1.01
+            else:                                        # the sum of the rounded d: |rounded d - d| <= 2^-8 |d|, summed over the rows
+                e = e + 2.0 ** -8 * d.abs().sum(0) * 1.01
             over = float(((g.double() - r).abs() / (e + 1e-30)).max())
             assert over <= 1, name
     return loss, got

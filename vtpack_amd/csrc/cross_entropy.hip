@@ -23,86 +23,67 @@
 namespace vtdge {
 
 constexpr float LOG2E = 1.44269504f, LN2 = 0.69314718f;
-constexpr int CE_SLAB = 64;                        // of the summed dimension a stage
-constexpr int CE_TILE = 128;                       // rows and columns of a tile
-
 __device__ __forceinline__ int wave_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// ------------------------------------------------------------------------------------------------ operands
+// ------------------------------------------------------------------------------------------------ the product of a tile
 // A bf16 matrix, or the three parts of an fp32 one `plane` elements apart.
 struct Operand {
     const bf16_t *p;
     int64_t pitch, plane;
 };
-// parts of the two operands that are multiplied, smallest products first
-__device__ __forceinline__ void parts_of(int segs, int seg, int &pa, int &pb)
-{
-    if (segs == 1) {
-        pa = pb = 0;
-    } else {
-        // (2,0) (0,2) (1,1) (1,0) (0,1) (0,0), two bits each
-        pa = (0x0052 >> (2 * seg)) & 3;
-        pb = (0x0118 >> (2 * seg)) & 3;
-    }
-}
 
-// ------------------------------------------------------------------------------------------------ the product of a tile
-// ALONG: the summed dimension lies along the rows of memory: tile rows are rows of memory, `limit` of them.
+// A shape of the product: WM x WN waves, each with IM x JN blocks of 32 x 32; slabs of SLAB of the summed dimension in a ring of
+// SLOTS; PARTS 3 for fp32 operands.
+template <int IM_, int JN_, int WM_, int WN_, int SLAB_, int SLOTS_, int PARTS_> struct Shape {
+    static constexpr int IM = IM_, JN = JN_, WM = WM_, WN = WN_, SLAB = SLAB_, SLOTS = SLOTS_, PARTS = PARTS_;
+    static constexpr int ROWS = 32 * IM * WM, COLS = 32 * JN * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
+    static constexpr int STAGE = PARTS * (ROWS + COLS) * SLAB * 2, RING = SLOTS * STAGE;
+    static constexpr int LDS = RING + COLS * 4;                          // and the bias of the tile's classes
+    static constexpr int PER_SIMD = WAVES / 4 * (2 * LDS <= 160 * 1024 ? 2 : 1);
+    static_assert(LDS <= 160 * 1024 && 6 * ROWS * 4 <= RING, "LDS");
+};
+
+// Direct loads of one operand of a tile.  T = rows of the tile on its side.
+// ALONG: the summed dimension lies along the rows of memory: tile rows are rows of memory, `limit` of them from the first on.
 // Across: the summed dimension counts the rows of memory, `limit` of them, and tile rows are elements of a row, which has a multiple
-// of 8 of them, `span`.  No stage begins behind `limit`: a sum of n rows of memory has ceil(n / 64) stages.
-// R: tile rows / 32 of a wave; a tile has 64 R.
-template <bool ALONG, int R> struct Loader {
-    static constexpr int PIECES = 2 * R;            // direct loads of a wave and stage
-    static constexpr int ROW = ALONG ? 128 : 128 * R, STAGE = 8192 * R;
+// of 8 of them, `span`.  No stage begins behind `limit`: a sum of n rows of memory has ceil(n / SLAB) stages.
+// LDS rows are 2 SLAB bytes (ALONG) or 2 T bytes (across) without gaps; their 16-byte pieces are XOR-ed by the row, so that the
+// sixteen lanes that read together meet every bank once.
+template <bool ALONG, int T, int SLAB, int WAVES> struct Loader {
+    static constexpr int ROW = ALONG ? 2 * SLAB : 2 * T, STAGE = 2 * SLAB * T;
+    static constexpr int LPR = ROW / 16, RPI = 64 / LPR;                  // lanes a row, rows an instruction
+    static constexpr int PIECES = STAGE / 1024 / WAVES;                   // instructions of a wave
+    static_assert(PIECES * WAVES * 1024 == STAGE && LPR <= 64, "whole instructions");
     const unsigned char *base;
-    int64_t plane, pitch;                           // bytes
-    int limit, row0, col;
+    int64_t plane, pitch;                                                 // bytes
+    int limit, row0, last;
 
     __device__ __forceinline__ Loader(const Operand &o, int64_t first, int64_t lim, int64_t span)
-        : base(reinterpret_cast<const unsigned char *>(o.p)), plane(o.plane * 2), pitch(o.pitch * 2)
+        : base(reinterpret_cast<const unsigned char *>(o.p) + (ALONG ? first * o.pitch * 2 : first * 2)), plane(o.plane * 2), pitch(o.pitch * 2)
     {
         const int lane = threadIdx.x & 63, wid = wave_uniform(threadIdx.x >> 6);
-        if constexpr (ALONG) {
-            base += first * pitch;
-            limit = (int)(lim - first < 64 * R ? lim - first : 64 * R);
-            row0 = wid * 8 + (lane >> 3);
-            col = ((lane & 7) ^ ((row0 >> 1) & 7)) * 16;
-        } else {
-            constexpr int LPR = 8 * R, RPI = 64 / LPR;      // lanes a row, rows an instruction
-            base += first * 2;
-            limit = (int)lim;
-            row0 = wid * RPI + lane / LPR;
-            // (the rows of an instruction's successors are 4 RPI apart: the swizzle follows in load())
-            col = (lane % LPR) * 16;
-            row_span = (int)(span - first < 64 * R ? span - first : 64 * R) * 2 - 16;
-        }
+        row0 = wid * RPI + lane / LPR;
+        if constexpr (ALONG) limit = (int)(lim - first < T ? lim - first : T);
+        else limit = (int)lim;
+        last = ALONG ? 0 : (int)(span - first < T ? span - first : T) * 2 - 16;
     }
-    int row_span;
-    static __device__ __forceinline__ int swizzle(int k) { return R == 1 ? ((k >> 1) & 3) << 1 : (k & 7) << 1; }
-
+    static __device__ __forceinline__ int swizzle(int r)
+    {
+        if constexpr (ALONG) return SLAB == 64 ? (r >> 1) & 7 : SLAB == 32 ? (r >> 2) & 3 : (r >> 3) & 1;
+        else return LPR == 8 ? ((r >> 1) & 3) << 1 : (r & 7) << 1;
+    }
     // stage `kt` of part `part` to LDS byte `lds`
     __device__ __forceinline__ void load(int part, int kt, uint32_t lds) const
     {
-        const int wid = wave_uniform(threadIdx.x >> 6);
-        const unsigned char *at = base + part * plane + (ALONG ? (int64_t)kt * 128 : (int64_t)kt * CE_SLAB * pitch);
-        const void *from = uniform_ptr(at);
-        const int p32 = (int)pitch;
+        const int lane = threadIdx.x & 63, wid = wave_uniform(threadIdx.x >> 6);
+        const void *from = uniform_ptr(base + part * plane + (ALONG ? (int64_t)kt * (2 * SLAB) : (int64_t)kt * SLAB * pitch));
 #pragma unroll
         for (int d = 0; d < PIECES; d++) {
-            uint32_t off, to;
-            if constexpr (ALONG) {
-                const int r = min(d * 32 + row0, limit - 1);
-                off = (uint32_t)r * (uint32_t)p32 + col;
-                to = lds + (d * 32 + wid * 8) * 128;
-            } else {
-                constexpr int RPI = 64 / (8 * R);
-                const int k = d * 4 * RPI + row0;
-                const int r = min(k, limit - 1 - kt * CE_SLAB);
-                const int c = min(col ^ (swizzle(k) * 16), row_span);
-                off = (uint32_t)r * (uint32_t)p32 + c;
-                to = lds + (d * 4 * RPI + wid * RPI) * ROW;
-            }
-            dma16(from, off, wave_uniform(to));
+            const int r = d * WAVES * RPI + row0;
+            const int at = ((lane % LPR) ^ swizzle(r)) * 16;
+            const int row = ALONG ? min(r, limit - 1) : min(r, limit - 1 - kt * SLAB);
+            const int col = ALONG ? at : min(at, last);
+            dma16(from, (uint32_t)row * (uint32_t)pitch + col, wave_uniform(lds + (d * WAVES + wid) * 1024));
         }
     }
     // the 8 values of step s (16 of the summed dimension) of tile row `block` * 32 + lane % 32
@@ -110,7 +91,7 @@ template <bool ALONG, int R> struct Loader {
     {
         const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
         if constexpr (ALONG) {
-            return *reinterpret_cast<const u32x4 *>(stage + (block * 32 + lr) * 128 + (((2 * s + lg) ^ ((lr >> 1) & 7)) * 16));
+            return *reinterpret_cast<const u32x4 *>(stage + (block * 32 + lr) * ROW + (((2 * s + lg) ^ swizzle(lr)) * 16));
         } else {
             const int k = 16 * s + 8 * lg + ((lane & 15) >> 2);
             const int at = block * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;       // byte of the row
@@ -121,43 +102,79 @@ template <bool ALONG, int R> struct Loader {
     }
 };
 
-// acc[i][j][v] += A[row i*32 + lane%32 of the wave] . B[row j*32 + 8*(v/4) + 4*(lane/32) + v%4], stages t0 .. t1 - 1 of nk a segment
-template <class LA, class LB, int IM, int JN>
-__device__ __forceinline__ void multiply_tile(const LA &a, const LB &b, int nk, int segs, int t0, int t1, unsigned char *smem, f32x16 (&acc)[IM][JN])
+// acc[i][j][v] += A[row i*32 + lane%32 of the wave] . B[row j*32 + 8*(v/4) + 4*(lane/32) + v%4], stages t0 .. t1 - 1.  SUMS: also the sums of
+// A's rows (of this half of the lanes' values), for what `sums_wanted` says.
+template <class S, bool A_ALONG, bool B_ALONG, bool SUMS>
+__device__ __forceinline__ void multiply_tile(const Loader<A_ALONG, S::ROWS, S::SLAB, S::WAVES> &a, const Loader<B_ALONG, S::COLS, S::SLAB, S::WAVES> &b,
+                                              int t0, int t1, unsigned char *smem, f32x16 (&acc)[S::IM][S::JN], bool sums_wanted, float (&sums)[S::IM])
 {
-    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid >> 1, wn = wid & 1;
-    constexpr int STAGE = LA::STAGE + LB::STAGE;
+    using LA = Loader<A_ALONG, S::ROWS, S::SLAB, S::WAVES>;
+    using LB = Loader<B_ALONG, S::COLS, S::SLAB, S::WAVES>;
+    constexpr int IM = S::IM, JN = S::JN, PARTS = S::PARTS, SLOTS = S::SLOTS, A_BYTES = PARTS * LA::STAGE;
+    constexpr int LOADS = PARTS * (LA::PIECES + LB::PIECES);
+    static_assert(LOADS * (SLOTS - 2) < 64, "the counter of outstanding loads");
+    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
-    int seg = t0 / nk, kt = t0 - seg * nk;
-    auto issue = [&](int slot) {
-        int pa, pb;
-        parts_of(segs, seg, pa, pb);
-        a.load(pa, kt, lds0 + slot * STAGE);
-        b.load(pb, kt, lds0 + slot * STAGE + LA::STAGE);
-        if (++kt == nk) kt = 0, seg++;
+    auto issue = [&](int t, int slot) {
+        const uint32_t at = lds0 + slot * S::STAGE;
+#pragma unroll
+        for (int p = 0; p < PARTS; p++) {
+            a.load(p, t, at + p * LA::STAGE);
+            b.load(p, t, at + A_BYTES + p * LB::STAGE);
+        }
     };
-    issue(0);
+    int in = 0, out = 0;                            // slots
+#pragma unroll
+    for (int d = 0; d < SLOTS - 1; d++)
+        if (t0 + d < t1) {
+            issue(t0 + d, in);
+            in++;
+        }
     for (int t = t0; t < t1; t++) {
-        const int slot = (t - t0) & 1;
-        // this stage's loads have landed, for all waves; the other slot is read no more
-        wait_vmcnt<0>();
-        lds_barrier();
-        if (t + 1 < t1) issue(slot ^ 1);
-        const unsigned char *sa = smem + slot * STAGE, *sb = sa + LA::STAGE;
+        // this wave's loads of the stage have landed when only those of the stages behind it are outstanding
+        const int behind = min(t1 - 1 - t, SLOTS - 2);
+        static_for<SLOTS - 1>([&](auto X) {
+            constexpr int x = decltype(X)::value;
+            if (behind == x) wait_vmcnt<x * LOADS>();
+        });
+        lds_barrier();                              // everybody's have, and the slot before this one is read no more
+        if (t + SLOTS - 1 < t1) {
+            issue(t + SLOTS - 1, in);
+            in = in == SLOTS - 1 ? 0 : in + 1;
+        }
+        const unsigned char *sa = smem + out * S::STAGE, *sb = sa + A_BYTES;
+        out = out == SLOTS - 1 ? 0 : out + 1;
 #pragma unroll
-        for (int s = 0; s < CE_SLAB / 16; s++) {
-            u32x4 fa[IM], fb[JN];
+        for (int s = 0; s < S::SLAB / 16; s++) {
+            u32x4 fa[PARTS][IM], fb[PARTS][JN];
 #pragma unroll
-            for (int i = 0; i < IM; i++) fa[i] = LA::fragment(sa, wm * IM + i, s);
+            for (int p = 0; p < PARTS; p++) {
 #pragma unroll
-            for (int j = 0; j < JN; j++) fb[j] = LB::fragment(sb, wn * JN + j, s);
+                for (int i = 0; i < IM; i++) fa[p][i] = LA::fragment(sa + p * LA::STAGE, wm * IM + i, s);
 #pragma unroll
-            for (int i = 0; i < IM; i++)
+                for (int j = 0; j < JN; j++) fb[p][j] = LB::fragment(sb + p * LB::STAGE, wn * JN + j, s);
+            }
+            // smallest products first: parts whose numbers add up to 2, to 1, to 0
 #pragma unroll
-                for (int j = 0; j < JN; j++) Slab<bf16_t>::mma(fb[j], fa[i], acc[i][j]);
+            for (int order = PARTS - 1; order >= 0; order--)
+#pragma unroll
+                for (int p = 0; p <= order; p++)
+#pragma unroll
+                    for (int i = 0; i < IM; i++)
+#pragma unroll
+                        for (int j = 0; j < JN; j++) Slab<bf16_t>::mma(fb[order - p][j], fa[p][i], acc[i][j]);
+            if constexpr (SUMS) {
+                if (sums_wanted) {
+#pragma unroll
+                    for (int p = PARTS - 1; p >= 0; p--)
+#pragma unroll
+                        for (int i = 0; i < IM; i++)
+                            sums[i] = bf16_pair_sum(fa[p][i].x, bf16_pair_sum(fa[p][i].y, bf16_pair_sum(fa[p][i].z, bf16_pair_sum(fa[p][i].w, sums[i]))));
+                }
+            }
         }
     }
-    lds_barrier();                                  // the slots are free for the epilogue
+    lds_barrier();                                  // the ring is free for the epilogue
 }
 
 // Workgroup id -> tile: an XCD (every eighth id) takes a contiguous run of the list, which goes through eight row tiles for each
@@ -174,90 +191,82 @@ __device__ __forceinline__ void tile_of(int id, int count, int tm, int tn, int &
 
 struct CeArgs {
     Operand x, w;
-    const void *bias; const int64_t *target; int64_t rows, classes; int64_t ignore; float smoothing; int nk, segs;
+    const void *bias; const int64_t *target; int64_t rows, classes; int64_t ignore; float smoothing; int stages;
     int64_t v0, v1;                                 // classes of this piece
+    int bias_f32;
     // forward: [class tiles][rows] each
     float *tile_max, *tile_sum, *tile_total, *target_z;
     // backward
-    const float *row_max, *row_inv, *row_scale; bf16_t *d; int64_t d_pitch, d_plane; float *bias_part; int64_t bias_stride;
-    int bias_f32;
+    const float *row_max, *row_inv, *row_scale; bf16_t *d; int64_t d_pitch, d_plane;
+    bf16_t *x_copy; int width;                      // nullable: x with zeros for the rows that are left out
 };
 
 __device__ __forceinline__ bool counts(int64_t target, int64_t ignore, int64_t classes) { return target != ignore && target >= 0 && target < classes; }
 
-// the sums over lane % 32 of 32 values a lane: lane r ends with the sum of value index_of(r)
-template <int O> __device__ __forceinline__ float from_lane_xor(float v)
+// the bias of the tile's classes times log2 e, -inf behind the last class
+template <class S> __device__ __forceinline__ void read_bias(const CeArgs &p, int64_t c0, float *bias)
 {
-    if constexpr (O == 1) return dpp_move<0xB1>(v);
-    else if constexpr (O == 2) return dpp_move<0x4E>(v);
-    else if constexpr (O == 4) return dpp_move<0x141>(dpp_move<0x1B>(v));
-    else if constexpr (O == 8) return dpp_move<0x128>(v);
-    else return __shfl_xor(v, O, WAVE);
-}
-__device__ __forceinline__ float sum_by_halves(float (&f)[32], int lr)
-{
-    static_for<5>([&](auto S) {
-        constexpr int o = 1 << decltype(S)::value, half = 16 >> decltype(S)::value;
-        const bool up = (lr & o) != 0;
-#pragma unroll
-        for (int i = 0; i < half; i++) {
-            const float keep = up ? f[half + i] : f[i], send = up ? f[i] : f[half + i];
-            f[i] = keep + from_lane_xor<o>(send);
+    for (int c = threadIdx.x; c < S::COLS; c += S::THREADS) {
+        float b = -INFINITY;
+        if (c0 + c < p.v1) {
+            b = 0.f;
+            if (p.bias != nullptr)
+                b = LOG2E * (p.bias_f32 ? static_cast<const float *>(p.bias)[c0 + c] : bf16_to_f32(static_cast<const bf16_t *>(p.bias)[c0 + c]));
         }
-    });
-    return f[0];
+        bias[c] = b;
+    }
 }
-
-// z of a tile, times log2 e, in place of acc; -inf behind the last class
-template <int IM, int JN> __device__ __forceinline__ void logits(const CeArgs &p, int64_t c0, f32x16 (&acc)[IM][JN])
+// z of a tile, times log2 e, in place of acc; `bias` of the wave's first class
+template <class S> __device__ __forceinline__ void logits(const float *bias, f32x16 (&acc)[S::IM][S::JN])
 {
     const int lg = (threadIdx.x & 63) >> 5;
 #pragma unroll
-    for (int j = 0; j < JN; j++)
+    for (int j = 0; j < S::JN; j++)
 #pragma unroll
-        for (int q = 0; q < 4; q++)
+        for (int q = 0; q < 4; q++) {
+            const f32x4 b = *reinterpret_cast<const f32x4 *>(bias + j * 32 + 8 * q + 4 * lg);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int64_t c = c0 + j * 32 + 8 * q + 4 * lg + e;
-                const bool in = c < p.v1;
-                float b = 0.f;
-                if (p.bias != nullptr && in)
-                    b = p.bias_f32 ? static_cast<const float *>(p.bias)[c] : bf16_to_f32(static_cast<const bf16_t *>(p.bias)[c]);
-                b *= LOG2E;
+            for (int e = 0; e < 4; e++)
 #pragma unroll
-                for (int i = 0; i < IM; i++) acc[i][j][4 * q + e] = in ? __builtin_fmaf(acc[i][j][4 * q + e], LOG2E, b) : -INFINITY;
-            }
+                for (int i = 0; i < S::IM; i++) acc[i][j][4 * q + e] = __builtin_fmaf(acc[i][j][4 * q + e], LOG2E, b[e]);
+        }
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-template <bool TOTAL> __global__ __launch_bounds__(256, 2) void cross_entropy_tiles_kernel(CeArgs p, int tm, int tn)
+template <class S, bool TOTAL> __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void cross_entropy_tiles_kernel(CeArgs p, int tm, int tn)
 {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    constexpr int IM = S::IM, JN = S::JN, ROWS = S::ROWS;
     int m, n;
     tile_of(blockIdx.x, gridDim.x, tm, tn, m, n);
-    const int64_t r0 = (int64_t)m * CE_TILE, c0 = (int64_t)n * CE_TILE;
-    f32x16 acc[2][2] = {};
-    const Loader<true, 2> a(p.x, r0, p.rows, 0), b(p.w, c0, p.classes, 0);
-    multiply_tile(a, b, p.nk, p.segs, 0, p.nk * p.segs, smem, acc);
+    const int64_t r0 = (int64_t)m * ROWS, c0 = (int64_t)n * S::COLS;
+    float *const bias = reinterpret_cast<float *>(smem + S::RING);
+    read_bias<S>(p, c0, bias);
+    f32x16 acc[IM][JN] = {};
+    float none[IM];
+    const Loader<true, ROWS, S::SLAB, S::WAVES> a(p.x, r0, p.rows, 0);
+    const Loader<true, S::COLS, S::SLAB, S::WAVES> b(p.w, c0, p.classes, 0);
+    multiply_tile<S, true, true, false>(a, b, 0, p.stages, smem, acc, false, none);
     const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
-    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid >> 1, wn = wid & 1;
-    const int64_t cw = c0 + wn * 64;
-    logits<2, 2>(p, cw, acc);
-    float *const shared = reinterpret_cast<float *>(smem);          // [2 halves of the classes][largest, sum, total][128 rows]
+    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
+    const int64_t cw = c0 + wn * 32 * JN;
+    logits<S>(bias + wn * 32 * JN, acc);
+    float *const shared = reinterpret_cast<float *>(smem);          // [waves along the classes][largest, sum, total][rows]
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int row = wm * 64 + i * 32 + lr;
+    for (int i = 0; i < IM; i++) {
+        const int row = (wm * IM + i) * 32 + lr;
         const int64_t r = r0 + row;
+        const int64_t t = r < p.rows ? p.target[r] : -1;
         float top = -INFINITY, total = 0.f;
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+        for (int j = 0; j < JN; j++)
 #pragma unroll
             for (int v = 0; v < 16; v++) top = fmaxf(top, acc[i][j][v]);
         top = fmaxf(top, __shfl_xor(top, 32, WAVE));
         const float from = top == -INFINITY ? 0.f : top;            // nothing in sight: exp2(-inf) = 0, and NaN stays NaN
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+        for (int j = 0; j < JN; j++)
 #pragma unroll
             for (int v = 0; v < 16; v++) {
                 sum += __builtin_amdgcn_exp2f(acc[i][j][v] - from);
@@ -266,94 +275,49 @@ template <bool TOTAL> __global__ __launch_bounds__(256, 2) void cross_entropy_ti
         sum += __shfl_xor(sum, 32, WAVE);
         if constexpr (TOTAL) total += __shfl_xor(total, 32, WAVE);
         if (lg == 0) {
-            shared[(wn * 3 + 0) * CE_TILE + row] = top;
-            shared[(wn * 3 + 1) * CE_TILE + row] = sum;
-            if constexpr (TOTAL) shared[(wn * 3 + 2) * CE_TILE + row] = total;
+            shared[(wn * 3 + 0) * ROWS + row] = top;
+            shared[(wn * 3 + 1) * ROWS + row] = sum;
+            if constexpr (TOTAL) shared[(wn * 3 + 2) * ROWS + row] = total;
         }
         // the z of the row's own class
-        const int64_t t = r < p.rows ? p.target[r] : -1;
-        const bool mine = counts(t, p.ignore, p.classes) && t >= cw && t < cw + 64 && (((int)(t - cw) >> 2) & 1) == lg;
+        const bool mine = counts(t, p.ignore, p.classes) && t >= cw && t < cw + 32 * JN && (((int)(t - cw) >> 2) & 1) == lg;
         if (__ballot(mine) != 0) {
             const int at = (int)(t - cw), reg = (at >> 5) * 16 + ((at & 31) >> 3) * 4 + (at & 3);
             float z = 0.f;
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < JN; j++)
 #pragma unroll
                 for (int v = 0; v < 16; v++) z = reg == j * 16 + v ? acc[i][j][v] : z;
             if (mine) p.target_z[r] = z;
         }
     }
     __syncthreads();
-    const int row = threadIdx.x;
-    if (row < CE_TILE && r0 + row < p.rows) {
-        const float t0 = shared[row], t1 = shared[3 * CE_TILE + row], top = fmaxf(t0, t1);
+    for (int row = threadIdx.x; row < ROWS && r0 + row < p.rows; row += S::THREADS) {
+        static_assert(S::WN == 2, "two waves along the classes");
+        const float t0 = shared[row], t1 = shared[3 * ROWS + row], top = fmaxf(t0, t1);
         const float from = top == -INFINITY ? 0.f : top;
-        const float sum = shared[CE_TILE + row] * __builtin_amdgcn_exp2f((t0 == -INFINITY ? from : t0) - from) +
-                          shared[4 * CE_TILE + row] * __builtin_amdgcn_exp2f((t1 == -INFINITY ? from : t1) - from);
+        const float sum = shared[ROWS + row] * __builtin_amdgcn_exp2f((t0 == -INFINITY ? from : t0) - from) +
+                          shared[4 * ROWS + row] * __builtin_amdgcn_exp2f((t1 == -INFINITY ? from : t1) - from);
         const int64_t at = (int64_t)n * p.rows + r0 + row;
         p.tile_max[at] = top;
         p.tile_sum[at] = sum;
-        if constexpr (TOTAL) p.tile_total[at] = shared[2 * CE_TILE + row] + shared[5 * CE_TILE + row];
+        if constexpr (TOTAL) p.tile_total[at] = shared[2 * ROWS + row] + shared[5 * ROWS + row];
     }
 }
 
-// joins the class tiles of each row; with `mean` given a single workgroup goes on to the mean of the losses
-__global__ __launch_bounds__(256) void cross_entropy_join_kernel(CeArgs p, int tn, float *loss_rows, float *row_max, float *row_inv)
-{
-    // 64 rows a workgroup, four waves along the tiles
-    __shared__ float tops[4][64], sums[4][64], totals[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t r = (int64_t)blockIdx.x * 64 + lane;
-    const bool in = r < p.rows;
-    float top = -INFINITY, sum = 0.f, total = 0.f;
-    if (in) {
-        for (int n = wave; n < tn; n += 4) {
-            const int64_t at = (int64_t)n * p.rows + r;
-            const float t = p.tile_max[at], s = p.tile_sum[at], next = fmaxf(top, t);
-            const float from = next == -INFINITY ? 0.f : next;
-            sum = sum * __builtin_amdgcn_exp2f((top == -INFINITY ? from : top) - from) + s * __builtin_amdgcn_exp2f((t == -INFINITY ? from : t) - from);
-            top = next;
-            if (p.smoothing != 0.f) total += p.tile_total[at];
-        }
-    }
-    tops[wave][lane] = top;
-    sums[wave][lane] = sum;
-    totals[wave][lane] = total;
-    __syncthreads();
-    if (wave != 0 || !in) return;
-    top = fmaxf(fmaxf(tops[0][lane], tops[1][lane]), fmaxf(tops[2][lane], tops[3][lane]));
-    const float from = top == -INFINITY ? 0.f : top;
-    sum = total = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-        const float t = tops[w][lane];
-        sum += sums[w][lane] * __builtin_amdgcn_exp2f((t == -INFINITY ? from : t) - from);
-        total += totals[w][lane];
-    }
-    const int64_t t = p.target[r];
-    float loss = 0.f;
-    if (counts(t, p.ignore, p.classes)) {
-        // log2 sum + (1 - eps) (largest - z_t) + eps (largest - mean): differences of like size, not of large sums
-        loss = __builtin_amdgcn_logf(sum) + (1.f - p.smoothing) * (top - p.target_z[r]);
-        if (p.smoothing != 0.f) loss += p.smoothing * (top - total / (float)p.classes);
-        loss *= LN2;
-    }
-    loss_rows[r] = loss;
-    row_max[r] = top;
-    row_inv[r] = 1.0f / sum;
-}
+// A row's tiles joined, by the waves of a workgroup side by side (64 rows, one a lane).  `mean`: the only workgroup goes through
+// all rows and on to their mean or sum.
+constexpr int JOIN_WAVES = 16;
+struct JoinArgs {
+    const float *tile_max, *tile_sum, *tile_total, *target_z; const int64_t *target; int64_t rows, classes, ignore; float smoothing; int tn;
+    float *loss_rows, *row_max, *row_inv, *loss, *inv_count;
+};
+__device__ __forceinline__ float scaled(float sum, float top, float to) { return sum * __builtin_amdgcn_exp2f((top == -INFINITY ? to : top) - to); }
 
-__global__ __launch_bounds__(1024) void cross_entropy_mean_kernel(const float *loss_rows, const int64_t *target, int64_t rows, int64_t classes,
-                                                                  int64_t ignore, float *loss, float *inv_count)
+__device__ void mean_of(double sum, int64_t n, const JoinArgs &p)
 {
-    __shared__ double sums[16];
-    __shared__ int64_t ns[16];
-    double sum = 0.0;
-    int64_t n = 0;
-    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
-        sum += loss_rows[r];
-        n += counts(target[r], ignore, classes) ? 1 : 0;
-    }
+    __shared__ double sums[JOIN_WAVES];
+    __shared__ int64_t ns[JOIN_WAVES];
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         sum += __shfl_xor(sum, o, WAVE);
@@ -361,155 +325,298 @@ __global__ __launch_bounds__(1024) void cross_entropy_mean_kernel(const float *l
     }
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum, ns[threadIdx.x >> 6] = n;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        sum = 0.0, n = 0;
-        for (int w = 0; w < 16; w++) sum += sums[w], n += ns[w];
-        if (inv_count == nullptr) {
-            *loss = (float)sum;
-        } else {
-            *loss = n > 0 ? (float)(sum / (double)n) : 0.f;
-            *inv_count = n > 0 ? (float)(1.0 / (double)n) : 0.f;
-        }
+    if (threadIdx.x != 0) return;
+    sum = 0.0, n = 0;
+    for (int w = 0; w < JOIN_WAVES; w++) sum += sums[w], n += ns[w];
+    if (p.inv_count == nullptr) {
+        *p.loss = (float)sum;
+    } else {
+        *p.loss = n > 0 ? (float)(sum / (double)n) : 0.f;
+        *p.inv_count = n > 0 ? (float)(1.0 / (double)n) : 0.f;
     }
+}
+__device__ __forceinline__ float loss_of(const JoinArgs &p, int64_t r, float top, float sum, float total, bool &live)
+{
+    const int64_t t = p.target[r];
+    live = counts(t, p.ignore, p.classes);
+    if (!live) return 0.f;
+    // log2 sum + (1 - eps) (largest - z_t) + eps (largest - mean): differences of like size, not of large sums
+    float loss = __builtin_amdgcn_logf(sum) + (1.f - p.smoothing) * (top - p.target_z[r]);
+    if (p.smoothing != 0.f) loss += p.smoothing * (top - total / (float)p.classes);
+    return loss * LN2;
+}
+__device__ __forceinline__ void join_tiles(const JoinArgs &p, int64_t r, int first, int step, float &top, float &sum, float &total)
+{
+#pragma unroll 8
+    for (int n = first; n < p.tn; n += step) {
+        const int64_t at = (int64_t)n * p.rows + r;
+        const float t = p.tile_max[at], s = p.tile_sum[at], next = fmaxf(top, t), to = next == -INFINITY ? 0.f : next;
+        sum = scaled(sum, top, to) + scaled(s, t, to);
+        top = next;
+        if (p.smoothing != 0.f) total += p.tile_total[at];
+    }
+}
+
+__global__ __launch_bounds__(64 * JOIN_WAVES) void cross_entropy_join_kernel(JoinArgs p)
+{
+    __shared__ float tops[JOIN_WAVES][64], sums[JOIN_WAVES][64], totals[JOIN_WAVES][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t r = (int64_t)blockIdx.x * 64 + lane;
+    const bool in = r < p.rows;
+    float top = -INFINITY, sum = 0.f, total = 0.f;
+    if (in) join_tiles(p, r, wave, JOIN_WAVES, top, sum, total);
+    tops[wave][lane] = top;
+    sums[wave][lane] = sum;
+    totals[wave][lane] = total;
+    __syncthreads();
+    if (wave != 0 || !in) return;
+    top = -INFINITY;
+    for (int w = 0; w < JOIN_WAVES; w++) top = fmaxf(top, tops[w][lane]);
+    const float to = top == -INFINITY ? 0.f : top;
+    sum = total = 0.f;
+    for (int w = 0; w < JOIN_WAVES; w++) {
+        sum += scaled(sums[w][lane], tops[w][lane], to);
+        total += totals[w][lane];
+    }
+    bool live;
+    p.loss_rows[r] = loss_of(p, r, top, sum, total, live);
+    p.row_max[r] = top;
+    p.row_inv[r] = 1.0f / sum;
+}
+// few rows of many tiles: a workgroup takes one row, its threads the tiles
+__global__ __launch_bounds__(64 * JOIN_WAVES) void cross_entropy_join_row_kernel(JoinArgs p)
+{
+    __shared__ float tops[JOIN_WAVES], sums[JOIN_WAVES], totals[JOIN_WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t r = blockIdx.x;
+    float top = -INFINITY, sum = 0.f, total = 0.f;
+    join_tiles(p, r, threadIdx.x, 64 * JOIN_WAVES, top, sum, total);
+    const float all = wave_max(top), to = all == -INFINITY ? 0.f : all;
+    sum = wave_sum(scaled(sum, top, to));
+    total = wave_sum(total);
+    if (lane == 0) tops[wave] = all, sums[wave] = sum, totals[wave] = total;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    top = -INFINITY;
+    for (int w = 0; w < JOIN_WAVES; w++) top = fmaxf(top, tops[w]);
+    const float base = top == -INFINITY ? 0.f : top;
+    sum = total = 0.f;
+    for (int w = 0; w < JOIN_WAVES; w++) {
+        sum += scaled(sums[w], tops[w], base);
+        total += totals[w];
+    }
+    bool live;
+    p.loss_rows[r] = loss_of(p, r, top, sum, total, live);
+    p.row_max[r] = top;
+    p.row_inv[r] = 1.0f / sum;
+}
+// few rows of few tiles: one workgroup does all of it, a row a thread
+__global__ __launch_bounds__(64 * JOIN_WAVES) void cross_entropy_join_mean_kernel(JoinArgs p)
+{
+    double all = 0.0;
+    int64_t n = 0;
+    for (int64_t r = threadIdx.x; r < p.rows; r += 64 * JOIN_WAVES) {
+        float top = -INFINITY, sum = 0.f, total = 0.f;
+        join_tiles(p, r, 0, 1, top, sum, total);
+        bool live;
+        const float loss = loss_of(p, r, top, sum, total, live);
+        p.loss_rows[r] = loss;
+        p.row_max[r] = top;
+        p.row_inv[r] = 1.0f / sum;
+        all += loss;
+        n += live ? 1 : 0;
+    }
+    if (p.loss != nullptr) mean_of(all, n, p);
+}
+__global__ __launch_bounds__(64 * JOIN_WAVES) void cross_entropy_mean_kernel(JoinArgs p)
+{
+    double sum = 0.0;
+    int64_t n = 0;
+    for (int64_t r = threadIdx.x; r < p.rows; r += 64 * JOIN_WAVES) {
+        sum += p.loss_rows[r];
+        n += counts(p.target[r], p.ignore, p.classes) ? 1 : 0;
+    }
+    mean_of(sum, n, p);
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-// d of a piece of the classes; rows and classes behind the last are written as zeros up to whole slabs
-template <bool SPLIT> __global__ __launch_bounds__(256, 2) void cross_entropy_d_kernel(CeArgs p, int tm, int tn)
+// d of a piece of the classes; rows and classes behind the last are written as zeros, so that slabs may run over them
+template <class S> __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void cross_entropy_d_kernel(CeArgs p, int tm, int tn)
 {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    constexpr int IM = S::IM, JN = S::JN;
     int m, n;
     tile_of(blockIdx.x, gridDim.x, tm, tn, m, n);
-    const int64_t r0 = (int64_t)m * CE_TILE, c0 = p.v0 + (int64_t)n * CE_TILE;
-    f32x16 acc[2][2] = {};
-    const Loader<true, 2> a(p.x, r0, p.rows, 0), b(p.w, c0, p.classes, 0);
-    multiply_tile(a, b, p.nk, p.segs, 0, p.nk * p.segs, smem, acc);
+    const int64_t r0 = (int64_t)m * S::ROWS, c0 = p.v0 + (int64_t)n * S::COLS;
+    float *const bias = reinterpret_cast<float *>(smem + S::RING);
+    read_bias<S>(p, c0, bias);
+    if (p.x_copy != nullptr) {
+        // this tile's share of the rows: all class tiles together copy them
+        const int vecs = p.width / 8, share = (S::ROWS + tn - 1) / tn;
+        for (int i = threadIdx.x; i < share * vecs; i += S::THREADS) {
+            const int k = n * share + i / vecs, c = (i % vecs) * 8;
+            const int64_t r = r0 + k;
+            if (k >= S::ROWS || r >= p.rows) break;
+            u32x4 v = *reinterpret_cast<const u32x4 *>(p.x.p + r * p.x.pitch + c);
+            if (!counts(p.target[r], p.ignore, p.classes)) v = u32x4{0u, 0u, 0u, 0u};
+            *reinterpret_cast<u32x4 *>(p.x_copy + r * p.width + c) = v;
+        }
+    }
+    f32x16 acc[IM][JN] = {};
+    float none[IM];
+    const Loader<true, S::ROWS, S::SLAB, S::WAVES> a(p.x, r0, p.rows, 0);
+    const Loader<true, S::COLS, S::SLAB, S::WAVES> b(p.w, c0, p.classes, 0);
+    multiply_tile<S, true, true, false>(a, b, 0, p.stages, smem, acc, false, none);
     const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
-    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid >> 1, wn = wid & 1;
-    const int64_t cw = c0 + wn * 64;
-    logits<2, 2>(p, cw, acc);
+    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
+    const int64_t cw = c0 + wn * 32 * JN;
+    logits<S>(bias + wn * 32 * JN, acc);
     const float even = p.smoothing / (float)p.classes;
+    const bool edge = cw + 32 * JN > p.v1;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int64_t r = r0 + wm * 64 + i * 32 + lr;
+    for (int i = 0; i < IM; i++) {
+        const int64_t r = r0 + (wm * IM + i) * 32 + lr;
         const int64_t t = r < p.rows ? p.target[r] : -1;
         const bool live = r < p.rows && counts(t, p.ignore, p.classes);
-        const float top = live ? p.row_max[r] : 0.f, inv = live ? p.row_inv[r] : 0.f;
         const float g = live ? (p.row_scale != nullptr ? p.row_scale[r] : 1.f) : 0.f;
+        const float top = live ? p.row_max[r] : 0.f, inv = live ? p.row_inv[r] * g : 0.f, minus = -even * g;
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+        for (int j = 0; j < JN; j++)
 #pragma unroll
-            for (int v = 0; v < 16; v++) {
-                const bool in = cw + j * 32 + 8 * (v / 4) + 4 * lg + v % 4 < p.v1;
-                const float d = __builtin_fmaf(__builtin_amdgcn_exp2f(acc[i][j][v] - top), inv, -even);
-                acc[i][j][v] = live && in ? d : 0.f;
-            }
-        const bool mine = live && t >= cw && t < cw + 64 && t < p.v1 && (((int)(t - cw) >> 2) & 1) == lg;
+            for (int v = 0; v < 16; v++) acc[i][j][v] = __builtin_fmaf(__builtin_amdgcn_exp2f(acc[i][j][v] - top), inv, minus);
+        const bool mine = live && t >= cw && t < cw + 32 * JN && t < p.v1 && (((int)(t - cw) >> 2) & 1) == lg;
         if (__ballot(mine) != 0) {
             const int at = (int)(t - cw), reg = mine ? (at >> 5) * 16 + ((at & 31) >> 3) * 4 + (at & 3) : -1;
+            const float one = (1.f - p.smoothing) * g;
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < JN; j++)
 #pragma unroll
-                for (int v = 0; v < 16; v++) acc[i][j][v] -= reg == j * 16 + v ? 1.f - p.smoothing : 0.f;
+                for (int v = 0; v < 16; v++) acc[i][j][v] -= reg == j * 16 + v ? one : 0.f;
         }
-        if (p.row_scale != nullptr) {
+        if (edge || __ballot(!live) != 0) {
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < JN; j++)
 #pragma unroll
-                for (int v = 0; v < 16; v++) acc[i][j][v] = live ? acc[i][j][v] * g : 0.f;
+                for (int v = 0; v < 16; v++) acc[i][j][v] = live && cw + j * 32 + 8 * (v / 4) + 4 * lg + v % 4 < p.v1 ? acc[i][j][v] : 0.f;
         }
-    }
-    if (p.bias_part != nullptr) {
-        float *const shared = reinterpret_cast<float *>(smem);      // [2 halves of the rows][128 classes]
-        float f[32];
+        // to memory: half-wave swaps leave a lane 8 consecutive classes
+        bf16_t *const row = p.d + r * p.d_pitch + (cw - p.v0) + 8 * lg;
 #pragma unroll
-        for (int c = 0; c < 32; c++) f[c] = acc[0][c >> 4][c & 15] + acc[1][c >> 4][c & 15];
-        const float sum = sum_by_halves(f, lr);
-        // lane bit b chose bit 4 - b of the value's number
-        const int c = ((lr & 1) << 4) | ((lr & 2) << 2) | (lr & 4) | ((lr & 8) >> 2) | ((lr & 16) >> 4);
-        shared[wm * CE_TILE + wn * 64 + (c >> 4) * 32 + 8 * ((c & 15) >> 2) + 4 * lg + (c & 3)] = sum;
-        __syncthreads();
-        const int at = threadIdx.x;
-        if (at < CE_TILE && c0 + at < p.v1) p.bias_part[m * p.bias_stride + c0 + at] = shared[at] + shared[CE_TILE + at];
-    }
-    // to memory: 4 consecutive classes a lane
+        for (int j = 0; j < JN; j++)
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int64_t r = r0 + wm * 64 + i * 32 + lr;
-        bf16_t *const row = p.d + r * p.d_pitch + (cw - p.v0) + 4 * lg;
+            for (int q = 0; q < 2; q++) {
+                float f[8];
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+                for (int e = 0; e < 8; e++) f[e] = acc[i][j][8 * q + e];
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                float f[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) f[e] = acc[i][j][4 * q + e];
-#pragma unroll
-                for (int part = 0; part < (SPLIT ? 3 : 1); part++) {
-                    const u32x2 o = {pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
-                    *reinterpret_cast<u32x2 *>(row + part * p.d_plane + j * 32 + 8 * q) = o;
-                    if constexpr (SPLIT) f[0] -= bf16lo(o.x), f[1] -= bf16hi(o.x), f[2] -= bf16lo(o.y), f[3] -= bf16hi(o.y);
+                for (int part = 0; part < S::PARTS; part++) {
+                    const uint32_t o0 = pack_bf16x2(f[0], f[1]), o1 = pack_bf16x2(f[2], f[3]), o2 = pack_bf16x2(f[4], f[5]), o3 = pack_bf16x2(f[6], f[7]);
+                    const auto s0 = __builtin_amdgcn_permlane32_swap(o0, o2, false, false), s1 = __builtin_amdgcn_permlane32_swap(o1, o3, false, false);
+                    *reinterpret_cast<u32x4 *>(row + part * p.d_plane + j * 32 + 16 * q) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+                    if (part + 1 < S::PARTS) {
+                        f[0] -= bf16lo(o0), f[1] -= bf16hi(o0), f[2] -= bf16lo(o1), f[3] -= bf16hi(o1);
+                        f[4] -= bf16lo(o2), f[5] -= bf16hi(o2), f[6] -= bf16lo(o3), f[7] -= bf16hi(o3);
+                    }
                 }
             }
     }
 }
 
-// ---- out = A B over a dimension that may be cut into several parts, which leave sums of their own
+// ---- out = A B, dx = d W or dW = d^T x, over a dimension that may be cut into several parts, which leave sums of their own
 struct GradArgs {
     Operand a, b;
     int64_t rows, cols, span_a, span_b, sum_a, sum_b;      // of the result; elements of a row of memory; rows of memory that may be read
-    int nk, segs, splits;
+    int tm, tn, stages, splits;
     float *part; int64_t part_stride; int accumulate;       // [splits], [rows][cols] fp32 each
-    void *out; int f32; const float *scale, *scale2;       // without `part`: the result, times what they point to
+    void *out;                                              // without `part`: the result, scaled; neither: only the sums
+    float *sums_part; int64_t sums_stride; void *sums;     // nullable: the sums of A's rows, in the same way
+};
+struct GradPair {
+    GradArgs dx, dw;
+    int first_dw;                                           // workgroups before are dx's
+    const float *scale, *scale2; int f32;
 };
 
-template <bool A_ALONG> __global__ __launch_bounds__(256, 2) void cross_entropy_grad_kernel(GradArgs p, int tm, int tn)
+template <class S, bool A_ALONG> __device__ __forceinline__ void gradient_tile(const GradArgs &p, const GradPair &all, int id, unsigned char *smem)
 {
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    const int tiles = tm * tn, z = blockIdx.x / tiles;
+    constexpr int IM = S::IM, JN = S::JN;
+    const int tiles = p.tm * p.tn, z = id / tiles;
     int m, n;
-    tile_of(blockIdx.x - z * tiles, tiles, tm, tn, m, n);
-    const int64_t r0 = (int64_t)m * CE_TILE, c0 = (int64_t)n * CE_TILE;
-    const int stages = p.nk * p.segs;
-    const int t0 = (int)((int64_t)stages * z / p.splits), t1 = (int)((int64_t)stages * (z + 1) / p.splits);
-    f32x16 acc[2][2] = {};
-    const Loader<A_ALONG, 2> a(p.a, r0, A_ALONG ? p.rows : p.sum_a, p.span_a);
-    const Loader<false, 2> b(p.b, c0, p.sum_b, p.span_b);
-    multiply_tile(a, b, p.nk, p.segs, t0, t1, smem, acc);
+    tile_of(id - z * tiles, tiles, p.tm, p.tn, m, n);
+    const int64_t r0 = (int64_t)m * S::ROWS, c0 = (int64_t)n * S::COLS;
+    const int t0 = (int)((int64_t)p.stages * z / p.splits), t1 = (int)((int64_t)p.stages * (z + 1) / p.splits);
+    f32x16 acc[IM][JN] = {};
+    float sums[IM] = {};
+    const Loader<A_ALONG, S::ROWS, S::SLAB, S::WAVES> a(p.a, r0, A_ALONG ? p.rows : p.sum_a, p.span_a);
+    const Loader<false, S::COLS, S::SLAB, S::WAVES> b(p.b, c0, p.sum_b, p.span_b);
     const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
-    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid >> 1, wn = wid & 1;
+    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
+    const bool with_sums = !A_ALONG && n == 0 && wn == 0 && (p.sums_part != nullptr || p.sums != nullptr);
+    multiply_tile<S, A_ALONG, false, !A_ALONG>(a, b, t0, t1, smem, acc, with_sums, sums);
     float scale = 1.f;
-    if (p.part == nullptr) {
-        if (p.scale != nullptr) scale = *p.scale;
-        if (p.scale2 != nullptr) scale *= *p.scale2;
-    }
+    if (all.scale != nullptr) scale = *all.scale;
+    if (all.scale2 != nullptr) scale *= *all.scale2;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int64_t r = r0 + wm * 64 + i * 32 + lr;
+    for (int i = 0; i < IM; i++) {
+        const int64_t r = r0 + (wm * IM + i) * 32 + lr;
+        if constexpr (!A_ALONG) {
+            if (with_sums) {
+                const float sum = sums[i] + __shfl_xor(sums[i], 32, WAVE);
+                if (lg == 0 && r < p.rows) {
+                    if (p.sums_part != nullptr) p.sums_part[z * p.sums_stride + r] = sum;
+                    else if (all.f32) static_cast<float *>(p.sums)[r] = sum * scale;
+                    else static_cast<bf16_t *>(p.sums)[r] = f32_to_bf16(sum * scale);
+                }
+            }
+        }
         if (r >= p.rows) continue;
 #pragma unroll
-        for (int j = 0; j < 2; j++)
+        for (int j = 0; j < JN; j++)
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                const int64_t c = c0 + wn * 64 + j * 32 + 8 * q + 4 * lg;
+                const int64_t c = c0 + (wn * JN + j) * 32 + 8 * q + 4 * lg;
+                const int left = (int)(p.cols - c);
+                f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
                 if (p.part != nullptr) {
                     float *const to = p.part + z * p.part_stride + r * p.cols + c;
+                    if (left >= 4 && p.cols % 4 == 0) {
+                        if (p.accumulate) v += *reinterpret_cast<const f32x4 *>(to);
+                        *reinterpret_cast<f32x4 *>(to) = v;
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (c + e < p.cols) to[e] = acc[i][j][4 * q + e] + (p.accumulate ? to[e] : 0.f);
-                } else if (p.f32) {
-                    float *const to = static_cast<float *>(p.out) + r * p.cols + c;
+                        for (int e = 0; e < 4; e++)
+                            if (e < left) to[e] = v[e] + (p.accumulate ? to[e] : 0.f);
+                    }
+                } else if (p.out != nullptr) {
+                    v *= scale;
+                    if (all.f32) {
+                        float *const to = static_cast<float *>(p.out) + r * p.cols + c;
+                        if (left >= 4 && p.cols % 4 == 0) {
+                            *reinterpret_cast<f32x4 *>(to) = v;
+                        } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (c + e < p.cols) to[e] = acc[i][j][4 * q + e] * scale;
-                } else {
-                    bf16_t *const to = static_cast<bf16_t *>(p.out) + r * p.cols + c;
+                            for (int e = 0; e < 4; e++)
+                                if (e < left) to[e] = v[e];
+                        }
+                    } else {
+                        bf16_t *const to = static_cast<bf16_t *>(p.out) + r * p.cols + c;
+                        if (left >= 4 && p.cols % 4 == 0) {
+                            *reinterpret_cast<u32x2 *>(to) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+                        } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (c + e < p.cols) to[e] = f32_to_bf16(acc[i][j][4 * q + e] * scale);
+                            for (int e = 0; e < 4; e++)
+                                if (e < left) to[e] = f32_to_bf16(v[e]);
+                        }
+                    }
                 }
             }
     }
+}
+template <class S> __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void cross_entropy_grad_kernel(GradPair p)
+{
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    if ((int)blockIdx.x < p.first_dw) gradient_tile<S, true>(p.dx, p, blockIdx.x, smem);
+    else gradient_tile<S, false>(p.dw, p, blockIdx.x - p.first_dw, smem);
 }
 
 // out = scale * (sum over the parts), for up to three results in one launch
@@ -575,17 +682,33 @@ template <typename T> __global__ __launch_bounds__(256) void cross_entropy_pack_
 }
 
 // ------------------------------------------------------------------------------------------------ on the host
+// Shapes.  Large tiles where there are enough of them to fill the chip; tiles of 64 x 64 with a deep ring else, where a call waits for
+// memory and not for products; 64 rows by 128 classes for few rows of many classes, which wait for W.
+using LogitsLarge = Shape<2, 4, 2, 2, 32, 3, 1>;
+using LogitsFlat = Shape<1, 2, 2, 2, 64, 3, 1>;
+using LogitsSmall = Shape<1, 1, 2, 2, 64, 6, 1>;
+using GradLarge = Shape<4, 2, 2, 2, 32, 3, 1>;
+using GradSmall = Shape<1, 1, 2, 2, 64, 6, 1>;
+using SplitLarge = Shape<2, 2, 4, 2, 32, 2, 3>;
+using SplitFlat = Shape<1, 2, 2, 2, 32, 3, 3>;
+using SplitSmall = Shape<1, 1, 2, 2, 32, 4, 3>;
+
+constexpr int CE_PAD = 64;                          // rows of operands are filled up to whole slabs of any shape
+constexpr int64_t CE_PIECE_BYTES = 256ll << 20;     // of d
+enum { CE_LARGE, CE_FLAT, CE_SMALL };
+
 // Everything a call lays out, the same for the size and the call.
 struct CePlan {
-    int64_t rows, classes; int width, padded, parts, segs, nk;
-    bool backward;
+    int64_t rows, classes; int width, padded, parts;
+    bool backward, split;
+    int logits, grads;                              // shapes
+    int lm, ln, gm, gn, slab_l, slab_g;             // their tiles and slabs
     int64_t tm, tn;                                 // row and class tiles of all classes
     int64_t piece, d_rows;                          // classes of a piece, rows of d
     int dx_splits, dw_splits;
     // bytes of the workspace
-    int64_t x_at, w_at, xz_at, max_at, sum_at, total_at, z_at, d_at, dx_at, dw_at, db_at, bytes;
+    int64_t x_at, w_at, max_at, sum_at, total_at, z_at, d_at, dx_at, dw_at, db_at, bytes;
 };
-constexpr int64_t CE_PIECE_BYTES = 128ll << 20;     // of d
 
 static int64_t part_of(int64_t n) { return (n + 63) / 64 * 64; }      // elements from one part of a sum to the next
 static int64_t take(int64_t &at, int64_t bytes)
@@ -594,22 +717,88 @@ static int64_t take(int64_t &at, int64_t bytes)
     at += (bytes + 255) / 256 * 256;
     return here;
 }
-// into how many parts a sum of `stages` is cut so that `tiles` of it fill the chip twice, none shorter than 4 stages
-static int splits_for(int64_t tiles, int64_t stages)
+template <class S> static void use(int &m, int &n, int &slab) { m = S::ROWS, n = S::COLS, slab = S::SLAB; }
+
+// When `slots` workers are done with n1 jobs of l1 and then n2 of l2, each taken by whoever is free first.
+static int64_t makespan(int64_t slots, int64_t n1, int64_t l1, int64_t n2, int64_t l2)
 {
-    const int64_t wanted = 2 * (int64_t)compute_units() / tiles, most = stages / 4;
-    const int64_t s = wanted < most ? wanted : most;
-    return (int)(s < 1 ? 1 : s);
+    int64_t at[8] = {0}, count[8] = {slots};        // workers by the time they are free, soonest first
+    int groups = 1;
+    auto work = [&](int64_t n, int64_t l) {
+        while (n > 0) {
+            const int64_t now = n < count[0] ? n : count[0], t = at[0] + l;
+            n -= now;
+            count[0] -= now;
+            int from = 0;
+            if (count[0] == 0) from = 1;            // the group is gone; else it stays (and n is 0)
+            int to = groups;
+            while (to > from && at[to - 1] > t) at[to] = at[to - 1], count[to] = count[to - 1], to--;
+            at[to] = t, count[to] = now;
+            groups++;
+            if (from == 1) {
+                for (int g = 1; g < groups; g++) at[g - 1] = at[g], count[g - 1] = count[g];
+                groups--;
+            }
+        }
+    };
+    work(n1, l1);                                   // (a group is split only by the last jobs of a kind: four at most)
+    work(n2, l2);
+    return at[groups - 1];
 }
+
+// Shape and cuts of both gradients of a piece.  Large tiles where their work is 16 slabs for each workgroup that runs at a time; then as
+// many parts of each sum as end first: a slab of a large tile takes about a microsecond (two workgroups a compute unit, 1 PFLOP/s;
+// with fp32 operands a workgroup has the unit for itself and six times the products), a tile four for its epilogue, and parts are
+// written and read again at 4 TB/s.
+static void plan_gradients(CePlan &p, int64_t of_piece)
+{
+    const int64_t cu = compute_units();
+    int64_t slots = p.split ? cu : 2 * cu;
+    if (p.split) use<SplitLarge>(p.gm, p.gn, p.slab_g);
+    else use<GradLarge>(p.gm, p.gn, p.slab_g);
+    auto tiles = [&](int64_t rows) { return ceil_div(rows, p.gm) * ceil_div(p.width, p.gn); };
+    if (tiles(p.rows) * ceil_div(of_piece, p.slab_g) + tiles(of_piece) * ceil_div(p.rows, p.slab_g) >= 16 * slots) {
+        p.grads = CE_LARGE;
+    } else {
+        p.grads = CE_SMALL, slots = cu;
+        if (p.split) use<SplitSmall>(p.gm, p.gn, p.slab_g);
+        else use<GradSmall>(p.gm, p.gn, p.slab_g);
+    }
+    const int64_t tx = tiles(p.rows), tw = tiles(of_piece), sx = ceil_div(of_piece, p.slab_g), sw = ceil_div(p.rows, p.slab_g);
+    const double slab = p.grads == CE_LARGE ? (p.split ? 3.0 : 1.05) : (p.split ? 0.6 : 0.35);
+    double best = 1e30;
+    p.dx_splits = p.dw_splits = 1;
+    for (int64_t x = 1; x <= 32 && (x == 1 || sx / x >= 8); x++)
+        for (int64_t w = 1; w <= 32 && (w == 1 || sw / w >= 8); w++) {
+            if (x > 1 && tx * x > 4 * slots) continue;
+            if (w > 1 && tw * w > 4 * slots) continue;
+            const double bytes = ((x > 1 ? 8.0 * x * p.rows : 0.0) + (w > 1 ? 8.0 * w * of_piece : 0.0)) * p.width;
+            const double t = slab * makespan(slots, tx * x, ceil_div(sx, x) + 4, tw * w, ceil_div(sw, w) + 4) + bytes / 4e6 + (x > 1 || w > 1 ? 5.0 : 0.0);
+            if (t < best) best = t, p.dx_splits = (int)x, p.dw_splits = (int)w;
+        }
+}
+
 static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool backward)
 {
     CePlan p{};
     p.rows = rows, p.classes = classes, p.width = width, p.backward = backward;
-    p.padded = (int)ceil_div(width, CE_SLAB) * CE_SLAB;
-    p.parts = dtype == VTDGE_F32 ? 3 : 1;
-    p.segs = dtype == VTDGE_F32 ? 6 : 1;
-    p.nk = p.padded / CE_SLAB;
-    p.tm = ceil_div(rows, CE_TILE), p.tn = ceil_div(classes, CE_TILE);
+    p.padded = (int)ceil_div(width, CE_PAD) * CE_PAD;
+    p.split = dtype == VTDGE_F32;
+    p.parts = p.split ? 3 : 1;
+    const int cu = compute_units();
+    const int64_t large = p.split ? ceil_div(rows, SplitLarge::ROWS) * ceil_div(classes, SplitLarge::COLS)
+                                  : ceil_div(rows, LogitsLarge::ROWS) * ceil_div(classes, LogitsLarge::COLS);
+    p.logits = rows <= 64 && classes >= 64 * cu ? CE_FLAT : large >= cu ? CE_LARGE : CE_SMALL;
+    if (p.split) {
+        if (p.logits == CE_LARGE) use<SplitLarge>(p.lm, p.ln, p.slab_l);
+        else if (p.logits == CE_FLAT) use<SplitFlat>(p.lm, p.ln, p.slab_l);
+        else use<SplitSmall>(p.lm, p.ln, p.slab_l);
+    } else {
+        if (p.logits == CE_LARGE) use<LogitsLarge>(p.lm, p.ln, p.slab_l);
+        else if (p.logits == CE_FLAT) use<LogitsFlat>(p.lm, p.ln, p.slab_l);
+        else use<LogitsSmall>(p.lm, p.ln, p.slab_l);
+    }
+    p.tm = ceil_div(rows, p.lm), p.tn = ceil_div(classes, p.ln);
     int64_t at = 0;
     p.x_at = take(at, rows * p.padded * 2 * p.parts);
     p.w_at = take(at, classes * p.padded * 2 * p.parts);
@@ -619,20 +808,17 @@ static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool 
         p.total_at = take(at, p.tn * rows * 4);
         p.z_at = take(at, rows * 4);
     } else {
-        p.xz_at = take(at, rows * p.padded * 2 * p.parts);
-        p.d_rows = p.tm * CE_TILE;
-        int64_t piece = CE_PIECE_BYTES / (p.d_rows * 2 * p.parts) / CE_TILE * CE_TILE;
-        if (piece < 8 * CE_TILE) piece = 8 * CE_TILE;
-        // pieces of equal size
-        const int64_t pieces = ceil_div(classes, piece);
-        p.piece = ceil_div(ceil_div(classes, pieces), CE_TILE) * CE_TILE;
-        const int64_t cols = ceil_div(width, CE_TILE);
-        p.dx_splits = splits_for(p.tm * cols, ceil_div(p.piece, CE_SLAB) * p.segs);
-        p.dw_splits = splits_for(p.piece / CE_TILE * cols, ceil_div(rows, CE_SLAB) * p.segs);
+        p.d_rows = ceil_div(rows, 256) * 256;
+        int64_t piece = CE_PIECE_BYTES / (p.d_rows * 2 * p.parts) / 256 * 256;
+        if (piece < 1024) piece = 1024;
+        const int64_t pieces = ceil_div(classes, piece);                      // of equal size
+        p.piece = ceil_div(ceil_div(classes, pieces), 256) * 256;
+        const int64_t of_piece = p.piece < classes ? p.piece : classes;
+        plan_gradients(p, p.piece < classes ? p.piece : classes);
         p.d_at = take(at, p.d_rows * p.piece * 2 * p.parts);
         p.dx_at = take(at, part_of(rows * width) * 4 * p.dx_splits);
         p.dw_at = take(at, part_of(p.piece * width) * 4 * p.dw_splits);
-        p.db_at = take(at, p.tm * part_of(classes) * 4);
+        p.db_at = take(at, part_of(p.piece) * 4 * p.dw_splits);
     }
     p.bytes = at;
     return p;
@@ -642,25 +828,35 @@ static int check_sizes(const char *what, int64_t rows, int64_t classes, int widt
 {
     VT_REQUIRE(dtype == VTDGE_F32 || dtype == VTDGE_BF16, VTDGE_ERR_ARG, "%s: dtype %d", what, dtype);
     VT_REQUIRE(rows > 0 && classes > 0 && width > 0, VTDGE_ERR_ARG, "%s: %lld rows, %lld classes of %d", what, (long long)rows, (long long)classes, width);
-    VT_REQUIRE(rows < (1 << 24) && classes < (1 << 24) && width <= (1 << 16), VTDGE_ERR_UNSUPPORTED, "%s: %lld rows, %lld classes of %d", what,
-               (long long)rows, (long long)classes, width);
-    VT_REQUIRE(rows * (int64_t)width < (1ll << 31) && classes * (int64_t)width < (1ll << 31), VTDGE_ERR_UNSUPPORTED,
-               "%s: %lld rows, %lld classes of %d", what, (long long)rows, (long long)classes, width);
+    VT_REQUIRE(rows < (1 << 24) && classes < (1 << 24) && width <= (1 << 16) && rows * (int64_t)width < (1ll << 31) &&
+                   classes * (int64_t)width < (1ll << 31) && ceil_div(rows, 64) * ceil_div(classes, 64) < (1 << 23),
+               VTDGE_ERR_UNSUPPORTED, "%s: %lld rows, %lld classes of %d", what, (long long)rows, (long long)classes, width);
     return VTDGE_OK;
 }
 
-// an operand as it lies, where the product routine can read it so, else packed at `at`
-static int operand_of(Operand &o, const void *src, int64_t ld, int64_t rows, const CePlan &p, int dtype, const int64_t *target, int64_t ignore,
-                      unsigned char *at, hipStream_t st)
+#define VT_STEP(call)                        \
+    do {                                     \
+        const int vt_rc = (call);            \
+        if (vt_rc != VTDGE_OK) return vt_rc; \
+    } while (0)
+
+// whether the product routine can read an operand where it lies
+static bool lies_well(const void *src, int64_t ld, const CePlan &p)
 {
-    if (dtype == VTDGE_BF16 && target == nullptr && p.width == p.padded && ld % 8 == 0 && ld < (1 << 22) && ((uintptr_t)src & 15) == 0) {
+    return !p.split && p.width == p.padded && ld % 8 == 0 && ld < (1 << 22) && ((uintptr_t)src & 15) == 0;
+}
+// an operand as it lies, else packed at `at`; rows that are left out as zeros where `target` is given
+static int operand_of(Operand &o, const void *src, int64_t ld, int64_t rows, const CePlan &p, const int64_t *target, int64_t ignore, unsigned char *at,
+                      hipStream_t st)
+{
+    if (lies_well(src, ld, p)) {
         o = Operand{(const bf16_t *)src, ld, 0};
         return VTDGE_OK;
     }
     o = Operand{(const bf16_t *)at, p.padded, rows * p.padded};
     const int64_t blocks = ceil_div(rows * (p.padded / 8), 256);
     VT_REQUIRE(blocks < (1 << 24), VTDGE_ERR_UNSUPPORTED, "cross_entropy: %lld rows of %d", (long long)rows, p.width);
-    if (dtype == VTDGE_F32) {
+    if (p.split) {
         note_kernel(reinterpret_cast<const void *>(cross_entropy_pack_kernel<float>));
         cross_entropy_pack_kernel<float><<<(unsigned)blocks, 256, 0, st>>>((const float *)src, ld, rows, p.width, p.padded, target, ignore, p.classes,
                                                                            (bf16_t *)at, o.plane);
@@ -672,23 +868,43 @@ static int operand_of(Operand &o, const void *src, int64_t ld, int64_t rows, con
     return check_launch("cross_entropy");
 }
 
-constexpr int CE_LDS = 2 * 2 * 16384;
-
-#define VT_STEP(call)                      \
-    do {                                   \
-        const int vt_rc = (call);          \
-        if (vt_rc != VTDGE_OK) return vt_rc; \
-    } while (0)
-
-template <bool A_ALONG> static int go_grad(const GradArgs &g, hipStream_t st)
+template <class S> static int go_tiles(const CeArgs &a, const CePlan &p, hipStream_t st)
 {
-    const int tm = (int)ceil_div(g.rows, CE_TILE), tn = (int)ceil_div(g.cols, CE_TILE);
-    VT_REQUIRE(g.nk <= ceil_div(g.sum_b, CE_SLAB) && (A_ALONG || g.nk <= ceil_div(g.sum_a, CE_SLAB)) && g.splits >= 1 && g.splits <= g.nk * g.segs,
-               VTDGE_ERR_ARG, "cross_entropy_backward: %d stages over %lld rows", g.nk, (long long)g.sum_b);
-    auto kern = cross_entropy_grad_kernel<A_ALONG>;
-    VT_RESERVE_LDS(kern, CE_LDS, "cross_entropy_backward");
+    auto kern = a.smoothing != 0.f ? cross_entropy_tiles_kernel<S, true> : cross_entropy_tiles_kernel<S, false>;
+    VT_RESERVE_LDS((cross_entropy_tiles_kernel<S, true>), S::LDS, "cross_entropy");
+    VT_RESERVE_LDS((cross_entropy_tiles_kernel<S, false>), S::LDS, "cross_entropy");
     note_kernel(reinterpret_cast<const void *>(kern));
-    kern<<<(unsigned)(tm * tn * g.splits), 256, CE_LDS, st>>>(g, tm, tn);
+    kern<<<(unsigned)(p.tm * p.tn), S::THREADS, S::LDS, st>>>(a, (int)p.tm, (int)p.tn);
+    return check_launch("cross_entropy");
+}
+template <class S> static int go_d(const CeArgs &a, const CePlan &p, hipStream_t st)
+{
+    auto kern = cross_entropy_d_kernel<S>;
+    VT_RESERVE_LDS(kern, S::LDS, "cross_entropy_backward");
+    note_kernel(reinterpret_cast<const void *>(kern));
+    const int tn = (int)ceil_div(a.v1 - a.v0, S::COLS);
+    kern<<<(unsigned)(p.tm * tn), S::THREADS, S::LDS, st>>>(a, (int)p.tm, tn);
+    return check_launch("cross_entropy_backward");
+}
+template <class S> static int go_grad(GradPair &g, hipStream_t st)
+{
+    int64_t blocks = 0;
+    for (GradArgs *a : {&g.dx, &g.dw}) {
+        const bool along = a == &g.dx;
+        if (!along) g.first_dw = (int)blocks;
+        if (a->rows == 0) continue;
+        a->tm = (int)ceil_div(a->rows, S::ROWS), a->tn = (int)ceil_div(a->cols, S::COLS);
+        if (a->out == nullptr && a->part == nullptr) a->tn = 1;                // the sums alone
+        VT_REQUIRE(a->stages <= ceil_div(a->sum_b, S::SLAB) && (along || a->stages <= ceil_div(a->sum_a, S::SLAB)) && a->splits >= 1 && a->splits <= a->stages,
+                   VTDGE_ERR_ARG, "cross_entropy_backward: %d stages over %lld rows in %d parts", a->stages, (long long)a->sum_b, a->splits);
+        blocks += (int64_t)a->tm * a->tn * a->splits;
+    }
+    VT_REQUIRE(blocks < (1 << 23), VTDGE_ERR_UNSUPPORTED, "cross_entropy_backward: %lld tiles", (long long)blocks);
+    if (blocks == 0) return VTDGE_OK;
+    auto kern = cross_entropy_grad_kernel<S>;
+    VT_RESERVE_LDS(kern, S::LDS, "cross_entropy_backward");
+    note_kernel(reinterpret_cast<const void *>(kern));
+    kern<<<(unsigned)blocks, S::THREADS, S::LDS, st>>>(g);
     return check_launch("cross_entropy_backward");
 }
 
@@ -697,7 +913,7 @@ static int sum_up(const SumJob *jobs, int count, const float *scale, const float
     SumArgs a{};
     int n = 0;
     for (int i = 0; i < count; i++) {
-        if (jobs[i].out == nullptr) continue;
+        if (jobs[i].out == nullptr || jobs[i].part == nullptr) continue;
         a.job[n] = jobs[i];
         a.first[n + 1] = a.first[n] + ceil_div(jobs[i].n, 1024);
         n++;
@@ -735,31 +951,33 @@ extern "C" int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weigh
     const CePlan p = plan_of(rows, classes, width, dtype, false);
     VT_REQUIRE(workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG, "cross_entropy: workspace of %lld bytes, %lld needed",
                (long long)workspace_bytes, (long long)p.bytes);
-    VT_REQUIRE(p.tm * p.tn < (1 << 24), VTDGE_ERR_UNSUPPORTED, "cross_entropy: %lld tiles", (long long)(p.tm * p.tn));
     unsigned char *const ws = (unsigned char *)workspace;
     const hipStream_t st = (hipStream_t)stream;
     CeArgs a{};
-    VT_STEP(operand_of(a.x, x, ldx, rows, p, dtype, nullptr, ignore_index, ws + p.x_at, st));
-    VT_STEP(operand_of(a.w, weight, ldw, classes, p, dtype, nullptr, ignore_index, ws + p.w_at, st));
-    a.bias = bias, a.bias_f32 = dtype == VTDGE_F32, a.target = target, a.rows = rows, a.classes = classes, a.ignore = ignore_index;
-    a.smoothing = smoothing, a.nk = p.nk, a.segs = p.segs, a.v0 = 0, a.v1 = classes;
+    VT_STEP(operand_of(a.x, x, ldx, rows, p, nullptr, ignore_index, ws + p.x_at, st));
+    VT_STEP(operand_of(a.w, weight, ldw, classes, p, nullptr, ignore_index, ws + p.w_at, st));
+    a.bias = bias, a.bias_f32 = p.split, a.target = target, a.rows = rows, a.classes = classes, a.ignore = ignore_index;
+    a.smoothing = smoothing, a.stages = (int)ceil_div(p.padded, p.slab_l), a.v0 = 0, a.v1 = classes;
     a.tile_max = (float *)(ws + p.max_at), a.tile_sum = (float *)(ws + p.sum_at), a.tile_total = (float *)(ws + p.total_at);
     a.target_z = (float *)(ws + p.z_at);
-    auto kern = smoothing != 0.f ? cross_entropy_tiles_kernel<true> : cross_entropy_tiles_kernel<false>;
-    VT_RESERVE_LDS(cross_entropy_tiles_kernel<true>, CE_LDS, "cross_entropy");
-    VT_RESERVE_LDS(cross_entropy_tiles_kernel<false>, CE_LDS, "cross_entropy");
-    note_kernel(reinterpret_cast<const void *>(kern));
-    kern<<<(unsigned)(p.tm * p.tn), 256, CE_LDS, st>>>(a, (int)p.tm, (int)p.tn);
-    VT_STEP(check_launch("cross_entropy"));
-    note_kernel(reinterpret_cast<const void *>(cross_entropy_join_kernel));
-    cross_entropy_join_kernel<<<(unsigned)ceil_div(rows, 64), 256, 0, st>>>(a, (int)p.tn, loss_rows, row_max, row_inv);
-    VT_STEP(check_launch("cross_entropy"));
-    if (loss != nullptr) {
-        note_kernel(reinterpret_cast<const void *>(cross_entropy_mean_kernel));
-        cross_entropy_mean_kernel<<<1, 1024, 0, st>>>(loss_rows, target, rows, classes, ignore_index, loss, inv_count);
-        VT_STEP(check_launch("cross_entropy"));
+    if (p.split) VT_STEP(p.logits == CE_LARGE ? go_tiles<SplitLarge>(a, p, st) : p.logits == CE_FLAT ? go_tiles<SplitFlat>(a, p, st) : go_tiles<SplitSmall>(a, p, st));
+    else VT_STEP(p.logits == CE_LARGE ? go_tiles<LogitsLarge>(a, p, st) : p.logits == CE_FLAT ? go_tiles<LogitsFlat>(a, p, st) : go_tiles<LogitsSmall>(a, p, st));
+    const JoinArgs j{a.tile_max, a.tile_sum, a.tile_total, a.target_z, target, rows, classes, ignore_index, smoothing, (int)p.tn,
+                     loss_rows, row_max, row_inv, loss, inv_count};
+    // one workgroup is done with some 20000 values before a second launch would have begun (by sizes alone: the same bits for each reduction)
+    if (rows <= 2048 && rows * p.tn <= 20480 && p.tn <= 32) {
+        note_kernel(reinterpret_cast<const void *>(cross_entropy_join_mean_kernel));
+        cross_entropy_join_mean_kernel<<<1, 64 * JOIN_WAVES, 0, st>>>(j);
+        return check_launch("cross_entropy");
     }
-    return VTDGE_OK;
+    auto join = rows <= 256 && p.tn > 128 ? cross_entropy_join_row_kernel : cross_entropy_join_kernel;
+    note_kernel(reinterpret_cast<const void *>(join));
+    join<<<(unsigned)(join == cross_entropy_join_kernel ? ceil_div(rows, 64) : rows), 64 * JOIN_WAVES, 0, st>>>(j);
+    VT_STEP(check_launch("cross_entropy"));
+    if (loss == nullptr) return VTDGE_OK;
+    note_kernel(reinterpret_cast<const void *>(cross_entropy_mean_kernel));
+    cross_entropy_mean_kernel<<<1, 64 * JOIN_WAVES, 0, st>>>(j);
+    return check_launch("cross_entropy");
 }
 
 extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, const int64_t *target,
@@ -776,63 +994,55 @@ extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const vo
     const CePlan p = plan_of(rows, classes, width, dtype, true);
     VT_REQUIRE(workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG,
                "cross_entropy_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.bytes);
-    const int64_t cols = ceil_div(width, CE_TILE), piece_tiles = p.piece / CE_TILE;
-    VT_REQUIRE(p.tm * piece_tiles < (1 << 24) && p.tm * cols * p.dx_splits < (1 << 24) && piece_tiles * cols * p.dw_splits < (1 << 24), VTDGE_ERR_UNSUPPORTED,
-               "cross_entropy_backward: %lld x %lld tiles", (long long)p.tm, (long long)p.tn);
     if (dx == nullptr && dweight == nullptr && dbias == nullptr) return VTDGE_OK;
     unsigned char *const ws = (unsigned char *)workspace;
     const hipStream_t st = (hipStream_t)stream;
-    const bool f32 = dtype == VTDGE_F32;
     CeArgs a{};
-    Operand xz{};                                   // x with the rows that are left out as zeros
-    VT_STEP(operand_of(a.w, weight, ldw, classes, p, dtype, nullptr, ignore_index, ws + p.w_at, st));
-    VT_STEP(operand_of(xz, x, ldx, rows, p, dtype, target, ignore_index, ws + p.xz_at, st));
-    a.x = xz;
-    a.bias = bias, a.bias_f32 = f32, a.target = target, a.rows = rows, a.classes = classes, a.ignore = ignore_index;
-    a.smoothing = smoothing, a.nk = p.nk, a.segs = p.segs;
+    VT_STEP(operand_of(a.w, weight, ldw, classes, p, nullptr, ignore_index, ws + p.w_at, st));
+    VT_STEP(operand_of(a.x, x, ldx, rows, p, target, ignore_index, ws + p.x_at, st));
+    Operand clean = a.x;                            // x with zeros for the rows that are left out, so that what they hold reaches no gradient
+    const bool copy = lies_well(x, ldx, p) && (dweight != nullptr || dbias != nullptr);
+    if (copy) clean = Operand{(const bf16_t *)(ws + p.x_at), p.padded, 0};
+    a.bias = bias, a.bias_f32 = p.split, a.target = target, a.rows = rows, a.classes = classes, a.ignore = ignore_index;
+    a.smoothing = smoothing, a.stages = (int)ceil_div(p.padded, p.slab_l), a.width = p.padded;
     a.row_max = row_max, a.row_inv = row_inv, a.row_scale = grad_stride == 1 ? grad : nullptr;
     a.d = (bf16_t *)(ws + p.d_at), a.d_pitch = p.piece, a.d_plane = p.d_rows * p.piece;
-    a.bias_part = dbias != nullptr ? (float *)(ws + p.db_at) : nullptr, a.bias_stride = part_of(classes);
     const float *const scale = grad_stride == 1 ? nullptr : grad;
     const bool one_piece = p.piece >= classes;
     float *const dx_part = one_piece && p.dx_splits == 1 ? nullptr : (float *)(ws + p.dx_at);
-    float *const dw_part = p.dw_splits == 1 ? nullptr : (float *)(ws + p.dw_at);
-    auto kern = f32 ? cross_entropy_d_kernel<true> : cross_entropy_d_kernel<false>;
-    VT_RESERVE_LDS(cross_entropy_d_kernel<true>, CE_LDS, "cross_entropy_backward");
-    VT_RESERVE_LDS(cross_entropy_d_kernel<false>, CE_LDS, "cross_entropy_backward");
-    const size_t elem = f32 ? 4 : 2;
+    float *const dw_part = p.dw_splits == 1 ? nullptr : (float *)(ws + p.dw_at), *const db_part = p.dw_splits == 1 ? nullptr : (float *)(ws + p.db_at);
+    const int64_t elem = p.split ? 4 : 2;
     for (int64_t v0 = 0; v0 < classes; v0 += p.piece) {
         a.v0 = v0, a.v1 = v0 + p.piece < classes ? v0 + p.piece : classes;
+        a.x_copy = copy && v0 == 0 ? (bf16_t *)(ws + p.x_at) : nullptr;
         const int64_t live = a.v1 - a.v0;
-        const int tn = (int)ceil_div(live, CE_TILE);
-        note_kernel(reinterpret_cast<const void *>(kern));
-        kern<<<(unsigned)(p.tm * tn), 256, CE_LDS, st>>>(a, (int)p.tm, tn);
-        VT_STEP(check_launch("cross_entropy_backward"));
-        const Operand d{a.d, a.d_pitch, a.d_plane};
+        if (p.split) VT_STEP(p.logits == CE_LARGE ? go_d<SplitLarge>(a, p, st) : p.logits == CE_FLAT ? go_d<SplitFlat>(a, p, st) : go_d<SplitSmall>(a, p, st));
+        else VT_STEP(p.logits == CE_LARGE ? go_d<LogitsLarge>(a, p, st) : p.logits == CE_FLAT ? go_d<LogitsFlat>(a, p, st) : go_d<LogitsSmall>(a, p, st));
+        GradPair g{};
+        g.scale = scale, g.scale2 = inv_count, g.f32 = p.split;
         if (dx != nullptr) {
-            GradArgs g{};
-            g.a = d, g.b = Operand{a.w.p + v0 * a.w.pitch, a.w.pitch, a.w.plane};
-            g.rows = rows, g.cols = width, g.sum_b = live, g.span_b = p.padded;
-            g.nk = (int)ceil_div(live, CE_SLAB), g.segs = p.segs;
-            g.splits = p.dx_splits < g.nk * g.segs ? p.dx_splits : g.nk * g.segs;
-            g.part = dx_part, g.part_stride = part_of(rows * width), g.accumulate = v0 > 0, g.out = dx, g.f32 = f32, g.scale = scale, g.scale2 = inv_count;
-            VT_STEP(go_grad<true>(g, st));
+            g.dx.a = Operand{a.d, a.d_pitch, a.d_plane}, g.dx.b = Operand{a.w.p + v0 * a.w.pitch, a.w.pitch, a.w.plane};
+            g.dx.rows = rows, g.dx.cols = width, g.dx.sum_b = live, g.dx.span_b = p.padded;
+            g.dx.stages = (int)ceil_div(live, p.slab_g), g.dx.splits = p.dx_splits < g.dx.stages ? p.dx_splits : g.dx.stages;
+            g.dx.part = dx_part, g.dx.part_stride = part_of(rows * width), g.dx.accumulate = v0 > 0, g.dx.out = dx;
         }
-        if (dweight != nullptr) {
-            GradArgs g{};
-            g.a = d, g.b = xz;
-            g.rows = live, g.cols = width, g.sum_a = p.d_rows, g.span_a = p.piece, g.sum_b = rows, g.span_b = p.padded;
-            g.nk = (int)ceil_div(rows, CE_SLAB), g.segs = p.segs, g.splits = p.dw_splits;
-            g.part = dw_part, g.part_stride = part_of(p.piece * width), g.out = (unsigned char *)dweight + v0 * width * elem, g.f32 = f32, g.scale = scale, g.scale2 = inv_count;
-            VT_STEP(go_grad<false>(g, st));
-            if (dw_part != nullptr && !one_piece) {
-                const SumJob job{dw_part, g.out, live * width, g.part_stride, p.dw_splits};
-                VT_STEP(sum_up(&job, 1, scale, inv_count, f32, st));
-            }
+        if (dweight != nullptr || dbias != nullptr) {
+            g.dw.a = Operand{a.d, a.d_pitch, a.d_plane}, g.dw.b = clean;
+            g.dw.rows = live, g.dw.cols = width, g.dw.sum_a = p.d_rows, g.dw.span_a = p.piece, g.dw.sum_b = rows, g.dw.span_b = p.padded;
+            g.dw.stages = (int)ceil_div(rows, p.slab_g), g.dw.splits = p.dw_splits;
+            g.dw.part = dweight != nullptr ? dw_part : nullptr, g.dw.part_stride = part_of(p.piece * width);
+            g.dw.out = dweight != nullptr ? (unsigned char *)dweight + v0 * width * elem : nullptr;
+            g.dw.sums_part = dbias != nullptr ? db_part : nullptr, g.dw.sums_stride = part_of(p.piece);
+            g.dw.sums = dbias != nullptr ? (unsigned char *)dbias + v0 * elem : nullptr;
         }
+        if (p.split) VT_STEP(p.grads == CE_LARGE ? go_grad<SplitLarge>(g, st) : go_grad<SplitSmall>(g, st));
+        else VT_STEP(p.grads == CE_LARGE ? go_grad<GradLarge>(g, st) : go_grad<GradSmall>(g, st));
+        // parts of this piece's dW and db, and of dx behind the last piece
+        const bool last = a.v1 == classes;
+        const SumJob jobs[3] = {{dx_part, last ? dx : nullptr, rows * width, part_of(rows * width), p.dx_splits},
+                                {g.dw.part, g.dw.out, live * width, g.dw.part_stride, p.dw_splits},
+                                {g.dw.sums_part, g.dw.sums, live, g.dw.sums_stride, p.dw_splits}};
+        VT_STEP(sum_up(jobs, 3, scale, inv_count, p.split, st));
     }
-    SumJob jobs[3] = {{dx_part, dx_part != nullptr ? dx : nullptr, rows * width, part_of(rows * width), p.dx_splits},
-                      {dw_part, dw_part != nullptr && one_piece ? dweight : nullptr, classes * width, part_of(p.piece * width), p.dw_splits},
-                      {a.bias_part, dbias, classes, part_of(classes), (int)p.tm}};
-    return sum_up(jobs, 3, scale, inv_count, f32, st);
+    return VTDGE_OK;
 }

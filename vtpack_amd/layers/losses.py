@@ -37,8 +37,8 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     (F.cross_entropy stops the program there).  Without a row that counts the loss is 0, and so are the gradients.
 
     The logits are fp32 sums and are not rounded; in bfloat16 the gradients of the logits are, once, before the products that
-    take them to x and weight.  Those work in pieces of the classes, with at most 128 MB of scratch for a piece and 8 rows by the
-    width for each of its tiles; float32 operands are laid out anew in three parts of two bytes for the time of a call."""
+    take them to x, weight and bias.  They work in pieces of the classes with some 256 MB of scratch for a piece; float32
+    operands are laid out anew in three parts of two bytes for the time of a call."""
     ops._need_gpu(x, weight, bias, target)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction is {reduction!r}, expected 'mean', 'sum' or 'none'")
