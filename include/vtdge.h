@@ -597,7 +597,8 @@ int vtdge_chain_forward(const vtdge_chain *chain, const void *const *params_host
  *   mask     nullable, one byte a token: 0 leaves it out, whatever its logits are.  A token whose logits are all -inf is
  *            left out too.  T = 0: loss and gradients are 0
  *   loss     fp32 [1]   counts int64 [E]   share fp32 [E + 1], for the gradient
- *   workspace  vtdge_gate_balance_workspace bytes (0 for few tokens), contents do not matter, nothing else using it
+ *   workspace  vtdge_gate_balance_workspace bytes (0 for few tokens), 16-byte aligned, contents do not matter, nothing else
+ *              using it
  * _backward: grad [tokens, E] dense = grad_loss[0] * d loss / d gate; zeros for tokens left out. */
 #define VTDGE_MAX_EXPERTS 512
 int64_t vtdge_gate_balance_workspace(int64_t tokens, int E);

@@ -99,4 +99,4 @@ def test_workspaces_follow_the_sizes():
     assert size(256, 1000, 384, 1, 0) % 256 == 0 and size(256, 1000, 384, 1, 0) < size(256, 1000, 384, 0, 0)
     # d of a piece: no more than 256 MB, or 1024 classes, however many classes there are
     assert size(8192, 65536, 1024, 1, 1) < (256 << 20) + 2 * 65536 * 1024 * 2 + 3 * 8192 * 1024 * 4 + (8 << 20) * 4 * 2
-    assert lib.vtdge_gate_balance_workspace(100, 8) == 0 and lib.vtdge_gate_balance_workspace(1 << 20, 8) == 512 * 17 * 4
+    assert lib.vtdge_gate_balance_workspace(100, 8) == 0 and lib.vtdge_gate_balance_workspace(1 << 20, 8) == 256 * 17 * 4

@@ -2,29 +2,33 @@
 on the logits of `model.head`) and the balance of the routers' gates, which stands beside the budget loss of the harness."""
 import torch
 from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from .. import ops
+
+
+def _no_second_order(name):
+    """A gradient that is itself being differentiated, as `create_graph=True` asks for."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name}: gradients of the gradients are not supported")
 
 
 class _LinearCrossEntropy(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, ignore_index, label_smoothing, reduction):
-        loss_rows, loss, saved = ops.cross_entropy(x, weight, bias, target, ignore_index, label_smoothing, reduction)
-        ctx.how = (ignore_index, label_smoothing)
-        ctx.save_for_backward(x, weight, bias, target, *saved)
-        return loss_rows if loss is None else loss
+        loss, stats = ops.cross_entropy(x, weight, bias, target, ignore_index, label_smoothing, reduction)
+        ctx.how = (ignore_index, label_smoothing, reduction)
+        ctx.save_for_backward(x, weight, bias, target, stats)
+        return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        x, weight, bias, target, *saved = ctx.saved_tensors
-        # (a saved-tensor hook may lay them out anew)
-        x, weight, target = ops._rows_of(x), ops._rows_of(weight), target.contiguous()
-        if grad.dim() == 1 and grad.numel() > 1 and grad.stride(0) == 0:
-            grad = grad[0]                       # the same for every row, as a sum over the losses leaves it
-        dx, dw, db = ops.cross_entropy_backward(x, weight, bias, target, saved, grad.contiguous(), *ctx.how,
-                                                needs=ctx.needs_input_grad[:3])
+        _no_second_order("linear_cross_entropy")
+        x, weight, bias, target, stats = ctx.saved_tensors
+        if grad.dim() == 1:
+            # the same for every row, as a sum over the losses leaves it: one value
+            grad = grad[0] if grad.stride(0) == 0 else grad.contiguous()
+        dx, dw, db = ops.cross_entropy_backward(ops._rows_of(x), ops._rows_of(weight), bias, target, stats, grad, *ctx.how,
+                                                needs=ctx.needs_input_grad)
         return dx, dw, db, None, None, None, None
 
 
@@ -55,11 +59,11 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     if target.shape != x.shape[:-1]:
         raise ValueError(f"target has shape {tuple(target.shape)}, expected {tuple(x.shape[:-1])}")
     if x.numel() == 0:                           # no row: a loss of 0 that still belongs to its operands
-        zero = (x.sum() + weight.sum() * 0 + (0 if bias is None else bias.sum() * 0)).float()
+        zero = (x.sum() + weight[:0].sum() + (0 if bias is None else bias[:0].sum())).float()
         return zero if reduction != "none" else zero.expand(target.shape)
     loss = _LinearCrossEntropy.apply(ops._rows_of(x), ops._rows_of(weight), None if bias is None else bias.contiguous(),
                                      target.reshape(-1).contiguous(), int(ignore_index), float(label_smoothing), reduction)
-    return loss.view(target.shape) if reduction == "none" else loss
+    return loss.view(target.shape) if reduction == "none" and target.dim() != 1 else loss
 
 
 class _GateBalance(Function):
@@ -68,14 +72,16 @@ class _GateBalance(Function):
         loss, counts, share = ops.gate_balance(gate, indices, mask, top_k)
         ctx.save_for_backward(gate, mask, share)
         ctx.mark_non_differentiable(counts)
+        ctx.set_materialize_grads(False)
         return loss, counts
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad, _):
+        _no_second_order("gate_balance")
+        if grad is None:
+            return None, None, None, None
         gate, mask, share = ctx.saved_tensors
-        mask = None if mask is None else mask.contiguous()
-        return ops.gate_balance_backward(ops._rows_of(gate), mask, share.contiguous(), grad.contiguous()), None, None, None
+        return ops.gate_balance_backward(ops._rows_of(gate), mask, share, grad), None, None, None
 
 
 def gate_balance(gate, indices=None, top_k=1, mask=None):

@@ -6,6 +6,7 @@ packed operands may stay on the device (`rows_dev`), so no call here waits for
 the GPU but `index_to_patch_host`, which gives counts on the host, and the first
 use of a weight whose packed copy is kept (`done_before_shared`).
 """
+import contextlib
 import ctypes
 import functools
 
@@ -1089,74 +1090,88 @@ def sparse_attention_backward(q, k, v, out, grad, offsets, scale, max_rows_per_s
 
 
 # ------------------------------------------------------------------ a training step's losses
+_HERE = contextlib.nullcontext()
+
+
 def _on(t):
     """The device of t made the current one, where it is not."""
-    return torch.cuda.device(t.device)
+    return _HERE if t.device.index == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def _rows_of(t):
     """t [..., n] as [rows, n] with dense rows, as it lies where that can be."""
-    t = t.reshape(-1, t.shape[-1])
-    return t if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1] else t.contiguous()
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    return t if t.is_contiguous() or t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
 
 
 def _pitch(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _workspace(size, t):
+@functools.lru_cache(maxsize=1024)
+def _cross_entropy_workspace(rows, classes, width, dtype, backward):
+    size = _lib.load().vtdge_cross_entropy_workspace(rows, classes, width, dtype, backward)
     if size < 0:
         raise _lib.VtdgeError(_lib.load().vtdge_last_error().decode("utf-8", "replace"))
-    return torch.empty((size,), dtype=torch.uint8, device=t.device)
+    return size
 
 
 def cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
-    """Softmax cross entropy of x [rows, width] @ weight [classes, width]^T + bias against int64 target [rows]: -> (losses of
-    the rows, their mean or sum or None, what `cross_entropy_backward` wants).  rows > 0, rows of x and weight dense."""
-    rows, width = x.shape
-    classes = weight.shape[0]
+    """Softmax cross entropy of x [rows, width] @ weight [classes, width]^T + bias against int64 target [rows] (rows > 0, rows of
+    x and weight dense): -> (fp32 loss, stats for `cross_entropy_backward`).  The loss is the rows' mean or sum, or each
+    row's own ("none")."""
+    (rows, width), classes, dtype, device = x.shape, weight.shape[0], dtype_code(x), x.device
     with _on(x):
-        ws = _workspace(_lib.load().vtdge_cross_entropy_workspace(rows, classes, width, dtype_code(x), 0), x)
-        # (memory of their own: a caller may change the losses in place, the rest is kept for the gradients)
-        loss_rows = torch.empty((rows,), dtype=torch.float32, device=x.device)
-        row_max, row_inv = torch.empty((2, rows), dtype=torch.float32, device=x.device).unbind(0)
-        loss = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=x.device)
-        inv_count = torch.empty((), dtype=torch.float32, device=x.device) if reduction == "mean" else None
+        ws = torch.empty((_cross_entropy_workspace(rows, classes, width, dtype, 0),), dtype=torch.uint8, device=device)
+        # stats: the rows' largest logits, 1 / sums, 1 / the number of rows that count, the rows' losses; the loss is memory of its
+        # own, for a caller to change in place
+        stats = torch.empty((3 * rows + 1,), dtype=torch.float32, device=device)
+        loss = torch.empty((rows,) if reduction == "none" else (), dtype=torch.float32, device=device)
+        at, out = stats.data_ptr(), loss.data_ptr()
         call("vtdge_cross_entropy", x.data_ptr(), _pitch(x), weight.data_ptr(), _pitch(weight), ptr(bias), target.data_ptr(), rows,
-             classes, width, ignore_index, label_smoothing, ws.data_ptr(), ws.numel(), loss_rows.data_ptr(), row_max.data_ptr(),
-             row_inv.data_ptr(), ptr(loss), ptr(inv_count), dtype_code(x), stream_ptr(), tag=("cross_entropy", rows, classes, width))
-    return loss_rows, loss, (row_max, row_inv, inv_count)
+             classes, width, ignore_index, label_smoothing, ws.data_ptr(), ws.numel(),
+             out if reduction == "none" else at + 8 * rows + 4, at, at + 4 * rows, 0 if reduction == "none" else out,
+             at + 8 * rows if reduction == "mean" else 0, dtype, stream_ptr(), tag=("cross_entropy", rows, classes, width))
+    return loss, stats
 
 
-def cross_entropy_backward(x, weight, bias, target, saved, grad, ignore_index=-100, label_smoothing=0.0, needs=(True, True, True)):
-    """Gradients (dx, dweight, dbias; None where not needed) of `cross_entropy`; grad is fp32, a scalar or one value
-    for each row."""
-    rows, width = x.shape
-    classes = weight.shape[0]
-    row_max, row_inv, inv_count = saved
+def cross_entropy_backward(x, weight, bias, target, stats, grad, ignore_index=-100, label_smoothing=0.0, reduction="mean",
+                           needs=(True, True, True)):
+    """Gradients (dx, dweight, dbias; None where not needed) of `cross_entropy` for the fp32 gradient of its loss: a scalar, with
+    "none" also one value for each row."""
+    (rows, width), classes, dtype, device = x.shape, weight.shape[0], dtype_code(x), x.device
     with _on(x):
-        ws = _workspace(_lib.load().vtdge_cross_entropy_workspace(rows, classes, width, dtype_code(x), 1), x)
-        dx = torch.empty((rows, width), dtype=x.dtype, device=x.device) if needs[0] else None
-        dw = torch.empty((classes, width), dtype=x.dtype, device=x.device) if needs[1] else None
-        db = torch.empty((classes,), dtype=x.dtype, device=x.device) if needs[2] and bias is not None else None
+        ws = torch.empty((_cross_entropy_workspace(rows, classes, width, dtype, 1),), dtype=torch.uint8, device=device)
+        dx = torch.empty((rows, width), dtype=x.dtype, device=device) if needs[0] else None
+        dw = torch.empty((classes, width), dtype=x.dtype, device=device) if needs[1] else None
+        db = torch.empty((classes,), dtype=x.dtype, device=device) if needs[2] and bias is not None else None
+        at = stats.data_ptr()
         call("vtdge_cross_entropy_backward", x.data_ptr(), _pitch(x), weight.data_ptr(), _pitch(weight), ptr(bias), target.data_ptr(),
-             row_max.data_ptr(), row_inv.data_ptr(), grad.data_ptr(), grad.dim(),
-             ptr(inv_count), rows, classes, width, ignore_index, label_smoothing, ws.data_ptr(), ws.numel(), ptr(dx), ptr(dw), ptr(db),
-             dtype_code(x), stream_ptr(), tag=("cross_entropy_backward", rows, classes, width))
+             at, at + 4 * rows, grad.data_ptr(), grad.dim(), at + 8 * rows if reduction == "mean" else 0, rows, classes, width,
+             ignore_index, label_smoothing, ws.data_ptr(), ws.numel(), ptr(dx), ptr(dw), ptr(db), dtype, stream_ptr(),
+             tag=("cross_entropy_backward", rows, classes, width))
     return dx, dw, db
+
+
+@functools.lru_cache(maxsize=1024)
+def _gate_balance_workspace(tokens, E):
+    return _lib.load().vtdge_gate_balance_workspace(tokens, E)
 
 
 def gate_balance(gate, indices, mask, top_k):
     """gate [tokens, E] with dense rows, tokens > 0; indices int64 [tokens, k] or None; mask [tokens] of bytes or None
     -> (loss, counts int64 [E], share for `gate_balance_backward`)."""
-    tokens, E = gate.shape
+    (tokens, E), device = gate.shape, gate.device
     with _on(gate):
-        ws = _workspace(_lib.load().vtdge_gate_balance_workspace(tokens, E), gate)
-        loss = torch.empty((), dtype=torch.float32, device=gate.device)
-        share = torch.empty((E + 1,), dtype=torch.float32, device=gate.device)
-        counts = torch.empty((E,), dtype=torch.int64, device=gate.device)
-        call("vtdge_gate_balance", gate.data_ptr(), _pitch(gate), ptr(indices), ptr(mask), tokens, E, top_k, ptr(ws), ws.numel(),
-             loss.data_ptr(), counts.data_ptr(), share.data_ptr(), dtype_code(gate), stream_ptr(), tag=("gate_balance", tokens, E))
+        # share: fp32 [E + 1], behind the sums of the workgroups
+        size = _gate_balance_workspace(tokens, E)
+        share = torch.empty((size // 4 + E + 1,), dtype=torch.float32, device=device)
+        loss = torch.empty((), dtype=torch.float32, device=device)
+        counts = torch.empty((E,), dtype=torch.int64, device=device)
+        at = share.data_ptr()
+        call("vtdge_gate_balance", gate.data_ptr(), _pitch(gate), ptr(indices), ptr(mask), tokens, E, top_k, at, size,
+             loss.data_ptr(), counts.data_ptr(), at + size, dtype_code(gate), stream_ptr(), tag=("gate_balance", tokens, E))
     return loss, counts, share
 
 
@@ -1165,6 +1180,6 @@ def gate_balance_backward(gate, mask, share, grad):
     tokens, E = gate.shape
     with _on(gate):
         out = torch.empty((tokens, E), dtype=gate.dtype, device=gate.device)
-        call("vtdge_gate_balance_backward", gate.data_ptr(), _pitch(gate), ptr(mask), share.data_ptr(), grad.data_ptr(), out.data_ptr(),
-             tokens, E, dtype_code(gate), stream_ptr(), tag=("gate_balance_backward", tokens, E))
+        call("vtdge_gate_balance_backward", gate.data_ptr(), _pitch(gate), ptr(mask),
+             share.data_ptr() + 4 * (share.numel() - E - 1), grad.data_ptr(), out.data_ptr(), tokens, E, dtype_code(gate), stream_ptr(), tag=("gate_balance_backward", tokens, E))
     return out

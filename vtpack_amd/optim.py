@@ -1,6 +1,7 @@
 """The AdamW step of the reference's training runs (main.py:339-343: `create_optimizer`, `adamw` by default) as one kernel over all
 weights, with moments in 32 or in 8 bits.
 """
+import itertools
 import operator
 
 import numpy as np
@@ -31,7 +32,7 @@ class _Batch:
         self.moments = [[s[k] for s in states] for k in self.keys]
         self.kept = [p.detach() for p in params]            # no other storage can come to lie where one of these is
         self.at = [p.data_ptr() for p in params]
-        self.bytes = [p.nbytes for p in params]
+        self.bytes = [p.nbytes for p in params]                # of a gradient
         self.plain = all(p.is_contiguous() for p in params)
         self.table = np.zeros((len(params), 7), dtype=np.uint64)
         self.table[:, 0] = self.at
@@ -40,7 +41,7 @@ class _Batch:
         self.table[:, 6] = [p.numel() for p in params]
 
     def holds(self):
-        return (list(map(_ptr, self.params)) == self.at and list(map(_nbytes, self.params)) == self.bytes
+        return (list(map(_ptr, self.params)) == self.at
                 and all(all(map(operator.is_, map(operator.itemgetter(k), self.states), old))
                         for k, old in zip(self.keys, self.moments)))
 
@@ -182,7 +183,7 @@ class AdamW(torch.optim.Optimizer):
             grads = list(map(_grad, params))
             if capturing and not group["capturable"]:
                 raise RuntimeError("AdamW: a step that is captured needs capturable=True (its count of steps would stand still)")
-            if any(g is None for g in grads):
+            if not all(map(operator.is_not, grads, itertools.repeat(None))):
                 params = [p for p, g in zip(params, grads) if g is not None]
                 if not params:
                     continue
@@ -210,7 +211,7 @@ class AdamW(torch.optim.Optimizer):
         (b1, b2), eps, decay = group["betas"], group["eps"], group["weight_decay"]
         grads = batch.take_gradients(grads)
         first, lr, step, scalars = batch.params[0], group["lr"], 0, None
-        with torch.cuda.device(first.device):
+        with ops._on(first):
             if group["capturable"]:
                 if not torch.is_tensor(group["step"]):
                     group["step"] = torch.tensor([group["step"]], dtype=torch.int64, device=first.device)
