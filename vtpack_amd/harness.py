@@ -1,9 +1,12 @@
-"""Evaluation-side mirror of the reference's harness for DGE models (vtpack/engine/engine.py, main.py:372-392).
+"""Mirror of the reference's harness for DGE models (vtpack/engine/engine.py, main.py:372-392).
 
-Only what touches the query path is here: the complexity ratio, the budget loss built on it, an `evaluate` loop that
-reports the same meters under the same names, and loading a `{"model": state_dict}` checkpoint.  Datasets,
-samplers, optimisers, EMA, distillation and logging back-ends stay with the caller.
+Evaluation: the complexity ratio, the budget loss built on it, an `evaluate` loop that reports the same meters under the same
+names, and loading a `{"model": state_dict}` checkpoint.  Training: `train_step` and `train_one_epoch` on the classifier's cross
+entropy, the budget and the balance of the gates, with `optim.AdamW`.  Datasets, samplers, schedules, EMA, mixed labels, distillation
+and logging back-ends stay with the caller.
 """
+import math
+
 import torch
 
 from .layers import DynamicGrainedEncoder
@@ -34,6 +37,15 @@ def budget_loss(model, samples, dge_budget=1.0, dge_lr_scale=1.0):
     comp = unwrap(model).complexity(samples)
     ratio = comp["dynamic"] / comp["static"].clamp(min=1.0)
     return dge_lr_scale * (ratio - dge_budget) ** 2, ratio, comp
+
+
+def balance_loss(model):
+    """-> (loss, counts int64 [encoders, S]): the mean of `DynamicGrainedEncoder.balance` over the model's encoders, after a forward
+    pass in training mode, and how often each granularity was sampled.  1 is even; the gradient reaches every router."""
+    each = [m.balance() for m in unwrap(model).modules() if isinstance(m, DynamicGrainedEncoder)]
+    if not each:
+        raise ValueError("the model has no DynamicGrainedEncoder")
+    return torch.stack([loss for loss, _ in each]).mean(), torch.stack([counts for _, counts in each])
 
 
 class _Meter:
@@ -89,6 +101,65 @@ def evaluate(data_loader, model, device, dge_enable=False, dge_budget=1.0, dge_l
         update("loss", loss)
         update("acc1", acc1, n=images.shape[0])
         update("acc5", acc5, n=images.shape[0])
+    return {k: m.global_avg for k, m in meters.items()}
+
+
+def weight_decay_groups(model, weight_decay):
+    """Parameter groups for the optimiser: no decay for vectors, biases and what the model's `no_weight_decay()` names (what
+    timm's `create_optimizer` does for main.py:339)."""
+    skip = unwrap(model).no_weight_decay() if hasattr(unwrap(model), "no_weight_decay") else set()
+    decay, rest = [], []
+    for name, p in unwrap(model).named_parameters():
+        if p.requires_grad:
+            (rest if p.dim() == 1 or name.endswith(".bias") or name in skip else decay).append(p)
+    return [g for g in ({"params": decay, "weight_decay": weight_decay}, {"params": rest, "weight_decay": 0.0}) if g["params"]]
+
+
+def train_step(model, images, target, optimizer, label_smoothing=0.0, dge_enable=False, dge_budget=1.0, dge_lr_scale=1.0,
+               balance_scale=0.0, clip_grad=None):
+    """One update of a model in training mode (vtpack/engine/engine.py:48-90 without autocast): the classifier's cross entropy against
+    int64 `target`, with `dge_enable` the budget loss, `balance_scale` times the balance of the gates, gradients, their norm cut
+    to `clip_grad`, the optimiser's step (any; `optim.AdamW` takes one launch for some 90 weights).  -> {name: tensor on the GPU},
+    nothing of which is waited for: loss, loss_cls, and loss_dge, dge_ratio, loss_balance, gate_counts, grad_norm where they are made.
+
+    Weights are float32: the dense training branch multiplies with the library's batched products."""
+    if not unwrap(model).training:
+        raise RuntimeError("train_step: the model is not in training mode")
+    for name, p in unwrap(model).named_parameters():
+        if p.requires_grad and p.dtype != torch.float32:
+            raise TypeError(f"train_step: {name} is {p.dtype}, expected float32 weights")
+    loss_cls = model(images, target, label_smoothing=label_smoothing)
+    loss, out = loss_cls, {"loss_cls": loss_cls.detach()}
+    if dge_enable:
+        loss_dge, ratio, _ = budget_loss(model, images, dge_budget, dge_lr_scale)
+        loss = loss + loss_dge
+        out.update(loss_dge=loss_dge.detach(), dge_ratio=ratio.detach())
+    if balance_scale:
+        balance, counts = balance_loss(model)
+        loss = loss + balance_scale * balance
+        out.update(loss_balance=balance.detach(), gate_counts=counts)
+    optimizer.zero_grad(set_to_none=True)
+    loss.backward()
+    if clip_grad is not None:
+        out["grad_norm"] = torch.nn.utils.clip_grad_norm_(unwrap(model).parameters(), clip_grad)
+    optimizer.step()
+    out["loss"] = loss.detach()
+    return out
+
+
+def train_one_epoch(data_loader, model, optimizer, device, **how):
+    """vtpack/engine/engine.py:35-99: `train_step(**how)` for every (images, target) batch.  -> {meter name: global average} of its scalars and `lr`;
+    a loss that is not finite ends the epoch with an error, as the reference's run does (engine.py:74-76)."""
+    meters = {}
+    model.train()
+    for images, target in data_loader:
+        out = train_step(model, images.to(device, non_blocking=True), target.to(device, non_blocking=True), optimizer, **how)
+        if not math.isfinite(float(out["loss"])):
+            raise FloatingPointError(f"the loss is {float(out['loss'])}")
+        for name, value in out.items():
+            if value.dim() == 0:
+                meters.setdefault(name, _Meter()).update(float(value))
+        meters.setdefault("lr", _Meter()).update(float(optimizer.param_groups[0]["lr"]))
     return {k: m.global_avg for k, m in meters.items()}
 
 

@@ -18,6 +18,7 @@ from torch import nn
 from .. import ops
 from .grained_sample import (grained_sample_compress, grained_sample_compress_dense, grained_sample_decompress,
                              grained_sample_decompress_dense, grained_sample_index_to_patch)
+from .losses import gate_balance
 
 
 class Deferred:
@@ -172,6 +173,13 @@ class DynamicGrainedEncoder(nn.Module):
         return {"static": self.complexity_handler(num_inputs, num_inputs) + router_cost,
                 "dynamic": self.complexity_handler(num_inputs, num_queries) + router_cost}
 
+    def balance(self):
+        """After a forward pass in training mode: (loss, counts) of `gate_balance` over the regions' sampled granularities, 1 where
+        they come up equally often and S where they are all the same."""
+        if not self.training or self.states.get("gate_logits") is None:
+            raise RuntimeError("the balance of the gates is that of a forward pass in training mode")
+        return gate_balance(self.states["gate_logits"], indices=self.states["gate"].detach().argmax(dim=-1))
+
     def compress(self, x, H, W, gate=None):
         """x [B, extra+H*W, C] -> packed queries [L, C].  `gate` overrides the router output (tests)."""
         B, N, C = x.shape
@@ -180,6 +188,7 @@ class DynamicGrainedEncoder(nn.Module):
             # dge.py:64-72: hard Gumbel sample of the gate; every granularity (dense) or the sampled one (sparse)
             if gate is None:
                 gate = self.router(x[:, extra:, :].reshape(B, H, W, C))
+            self.states["gate_logits"] = gate                # what `balance` needs beside the sample
             gate = F.gumbel_softmax(gate, dim=-1, hard=True)
             if not self.sparse_train:
                 comp, batches = grained_sample_compress_dense(x, self.splits, self.region_size, H, W, extra)

@@ -21,7 +21,7 @@ import torch
 from torch import nn
 
 from ... import engine
-from ...layers import DynamicGrainedEncoder
+from ...layers import DynamicGrainedEncoder, linear_cross_entropy
 from ...layers.sparse_ops import batched_sparse_attention, sparse_attention_train
 
 __all__ = ["VisionTransformer", "Block", "Attention", "Mlp", "PatchEmbed", "deit_dge_s124_tiny_patch16_256",
@@ -222,7 +222,25 @@ class VisionTransformer(nn.Module):
             return (a, b) if self.training else (a + b) / 2
         return self.head(feats if self.cls_token is not None else feats.mean(dim=1))
 
-    def forward(self, x):
+    def loss(self, x, target, label_smoothing=0.0, ignore_index=-100, reduction="mean"):
+        """Cross entropy of the (class) head's logits on images x against int64 target [B], without the logits in memory; see
+        `layers.linear_cross_entropy`.  With a distillation token the class token's head alone, as the reference's base
+        criterion takes it (vtpack/engine/losses.py:41-48)."""
+        if self.num_classes <= 0:
+            raise ValueError("a model without a classifier has no loss")
+        if self.training and any(self.drop_rates):
+            raise NotImplementedError("dropout / stochastic depth in training mode are not part of this package")
+        feats = self.forward_features(x)
+        if self.head_dist is not None:
+            feats = feats[0]
+        elif self.cls_token is None:
+            feats = feats.mean(dim=1)
+        return linear_cross_entropy(feats, self.head.weight, self.head.bias, target, ignore_index, label_smoothing, reduction)
+
+    def forward(self, x, target=None, **how):
+        """Logits of images x; with `target` the `loss` (so that a wrapper around the model sees its training pass)."""
+        if target is not None:
+            return self.loss(x, target, **how)
         if self.fused and not self.training:
             return engine.model_forward(self, x)
         if self.training and any(self.drop_rates):

@@ -14,7 +14,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from ... import engine
-from ...layers import DynamicGrainedEncoder
+from ...layers import DynamicGrainedEncoder, linear_cross_entropy
 from ...layers.sparse_ops import batched_sparse_attention, sparse_attention_train
 from .deit_dge import Mlp
 
@@ -206,7 +206,17 @@ class PyramidVisionTransformer(nn.Module):
             return outputs
         return self.norm(x)[:, 0]
 
-    def forward(self, x):
+    def loss(self, x, target, label_smoothing=0.0, ignore_index=-100, reduction="mean"):
+        """Cross entropy of the logits of images x against int64 target [B], without the logits in memory; see
+        `layers.linear_cross_entropy`."""
+        if self.num_classes <= 0:
+            raise ValueError("a model without a classifier has no loss")
+        return linear_cross_entropy(self.forward_features(x), self.head.weight, self.head.bias, target, ignore_index, label_smoothing,
+                                    reduction)
+
+    def forward(self, x, target=None, **how):
+        if target is not None:
+            return self.loss(x, target, **how)
         if self.fused and not self.training:
             return engine.pvt_forward(self, x)
         x = self.forward_features(x)
