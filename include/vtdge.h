@@ -619,8 +619,11 @@ int vtdge_gate_balance_backward(const void *gate, int64_t pitch, const uint8_t *
  * _backward, of grad * loss_rows summed over the rows:
  *   grad      fp32, one value for each row (grad_stride 1) or one for all (0), times inv_count[0] where that is given
  *   dx [rows, width], dweight [classes, width], dbias [classes]: dense, of `dtype`, each nullable
+ *   laid_out  nullable: the workspace of the forward call on the same operands, as that call left it; what it laid out of
+ *             them (its first vtdge_cross_entropy_laid_out bytes) is not laid out again
  * fp32 operands are multiplied as exactly as fp32 products are, on the bf16 matrix instructions.
  *   workspace  vtdge_cross_entropy_workspace(..., backward) bytes, 256-byte aligned, contents do not matter */
+int64_t vtdge_cross_entropy_laid_out(int64_t rows, int64_t classes, int width, int dtype);
 int64_t vtdge_cross_entropy_workspace(int64_t rows, int64_t classes, int width, int dtype, int backward);
 int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, const int64_t *target,
                         int64_t rows, int64_t classes, int width, int64_t ignore_index, float smoothing, void *workspace,
@@ -629,8 +632,8 @@ int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weight, int64_t 
 int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias,
                                  const int64_t *target, const float *row_max, const float *row_inv, const float *grad,
                                  int grad_stride, const float *inv_count, int64_t rows, int64_t classes, int width,
-                                 int64_t ignore_index, float smoothing, void *workspace, int64_t workspace_bytes, void *dx,
-                                 void *dweight, void *dbias, int dtype, void *stream);
+                                 int64_t ignore_index, float smoothing, const void *laid_out, void *workspace,
+                                 int64_t workspace_bytes, void *dx, void *dweight, void *dbias, int dtype, void *stream);
 
 /* One AdamW step over `count` tensors, in one launch for each 92 of them (64 with 8-bit moments):
  *   p *= 1 - lr weight_decay;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;

@@ -246,8 +246,8 @@ def test_same_bits_on_another_stream_and_in_a_graph(dev, dtype):
     g = torch.ones((), device=dev)
 
     def run():
-        loss, stats = ops.cross_entropy(x, w, b, t, -100, 0.1, "mean")
-        return [loss, *ops.cross_entropy_backward(x, w, b, t, stats, g, -100, 0.1)]
+        loss, stats, laid_out = ops.cross_entropy(x, w, b, t, -100, 0.1, "mean")
+        return [loss, *ops.cross_entropy_backward(x, w, b, t, stats, laid_out, g, -100, 0.1)]
 
     want = [v.clone() for v in run()]
     assert all(torch.equal(p, q) for p, q in zip(run(), want))

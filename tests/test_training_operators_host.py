@@ -68,7 +68,7 @@ def test_arguments_of_the_library():
     assert call(_11=p + 16) == _lib.ERR_ARG               # a workspace off its boundary
     assert call(_16=None) == _lib.ERR_ARG                 # a count of rows without their mean
     assert lib.vtdge_cross_entropy_workspace(4, 3, 0, 0, 0) == -1
-    back = [p, 8, p, 8, p, p, p, p, p, 1, p, 4, 3, 8, -100, 0.0, p, 1 << 40, p, p, p, 0, None]
+    back = [p, 8, p, 8, p, p, p, p, p, 1, p, 4, 3, 8, -100, 0.0, None, p, 1 << 40, p, p, p, 0, None]
     assert lib.vtdge_cross_entropy_backward(*back) == _lib.ERR_ARG and b"grad_stride" in lib.vtdge_last_error()
     gb = [p, 3, None, None, 100, 3, 1, None, 0, p, p, p, 0, None]
     for i, v, want in ((4, 0, -1), (5, 0, -1), (5, 513, -1), (6, 4, -1), (6, 0, -1), (1, 2, -1), (12, 5, -1), (4, 1 << 31, -2), (4, 100000, -1)):
@@ -97,6 +97,6 @@ def test_workspaces_follow_the_sizes():
     lib = _lib.load()
     size = lib.vtdge_cross_entropy_workspace
     assert size(256, 1000, 384, 1, 0) % 256 == 0 and size(256, 1000, 384, 1, 0) < size(256, 1000, 384, 0, 0)
-    # d of a piece: no more than 256 MB, or 1024 classes, however many classes there are
-    assert size(8192, 65536, 1024, 1, 1) < (256 << 20) + 2 * 65536 * 1024 * 2 + 3 * 8192 * 1024 * 4 + (8 << 20) * 4 * 2
+    # d of a piece: no more than 320 MB, or 1024 classes, however many classes there are
+    assert size(8192, 65536, 1024, 1, 1) < (320 << 20) + 2 * 65536 * 1024 * 2 + 3 * 8192 * 1024 * 4 + (8 << 20) * 4 * 2
     assert lib.vtdge_gate_balance_workspace(100, 8) == 0 and lib.vtdge_gate_balance_workspace(1 << 20, 8) == 256 * 17 * 4

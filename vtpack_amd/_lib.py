@@ -92,8 +92,8 @@ SIGNATURES = {
     "vtdge_gate_balance": [_p, _l, _p, _p, _l, _i, _i, _p, _l, _p, _p, _p, _i, _p],
     "vtdge_gate_balance_backward": [_p, _l, _p, _p, _p, _p, _l, _i, _i, _p],
     "vtdge_cross_entropy": [_p, _l, _p, _l, _p, _p, _l, _l, _i, _l, _f, _p, _l, _p, _p, _p, _p, _p, _i, _p],
-    "vtdge_cross_entropy_backward": [_p, _l, _p, _l, _p, _p, _p, _p, _p, _i, _p, _l, _l, _i, _l, _f, _p, _l, _p, _p, _p, _i,
-                                     _p],
+    "vtdge_cross_entropy_backward": [_p, _l, _p, _l, _p, _p, _p, _p, _p, _i, _p, _l, _l, _i, _l, _f, _p, _p, _l, _p, _p, _p,
+                                     _i, _p],
     "vtdge_adamw": [_p, _i, _d, _d, _d, _d, _d, _l, _p, _i, _i, _p],
     "vtdge_adamw_scalars": [_p, _l, _i, _p, _d, _d, _d, _d, _d, _p, _p],
     "vtdge_chain_layout": [_p, _p],
@@ -154,6 +154,8 @@ def load():
     lib.vtdge_region_step_workspace.argtypes = [_i, _i, _i]
     lib.vtdge_gate_balance_workspace.restype = _l
     lib.vtdge_gate_balance_workspace.argtypes = [_l, _i]
+    lib.vtdge_cross_entropy_laid_out.restype = _l
+    lib.vtdge_cross_entropy_laid_out.argtypes = [_l, _l, _i, _i]
     lib.vtdge_cross_entropy_workspace.restype = _l
     lib.vtdge_cross_entropy_workspace.argtypes = [_l, _l, _i, _i, _i]
     for name, args in SIGNATURES.items():

@@ -242,21 +242,26 @@ template <class S, bool TOTAL> __global__ __launch_bounds__(S::THREADS, S::PER_S
     const int64_t r0 = (int64_t)m * ROWS, c0 = (int64_t)n * S::COLS;
     float *const bias = reinterpret_cast<float *>(smem + S::RING);
     read_bias<S>(p, c0, bias);
+    const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
+    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
+    const int64_t cw = c0 + wn * 32 * JN;
+    // the rows' own classes, asked for before the product: which of the wave's classes, or less than 0
+    int own[IM];
+#pragma unroll
+    for (int i = 0; i < IM; i++) {
+        const int64_t r = r0 + (wm * IM + i) * 32 + lr, t = r < p.rows ? p.target[r] : -1;
+        own[i] = r < p.rows && counts(t, p.ignore, p.classes) && t >= cw && t < cw + 32 * JN ? (int)(t - cw) : -1;
+    }
     f32x16 acc[IM][JN] = {};
     float none[IM];
     const Loader<true, ROWS, S::SLAB, S::WAVES> a(p.x, r0, p.rows, 0);
     const Loader<true, S::COLS, S::SLAB, S::WAVES> b(p.w, c0, p.classes, 0);
     multiply_tile<S, true, true, false>(a, b, 0, p.stages, smem, acc, false, none);
-    const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
-    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
-    const int64_t cw = c0 + wn * 32 * JN;
     logits<S>(bias + wn * 32 * JN, acc);
     float *const shared = reinterpret_cast<float *>(smem);          // [waves along the classes][largest, sum, total][rows]
 #pragma unroll
     for (int i = 0; i < IM; i++) {
         const int row = (wm * IM + i) * 32 + lr;
-        const int64_t r = r0 + row;
-        const int64_t t = r < p.rows ? p.target[r] : -1;
         float top = -INFINITY, total = 0.f;
 #pragma unroll
         for (int j = 0; j < JN; j++)
@@ -280,15 +285,16 @@ template <class S, bool TOTAL> __global__ __launch_bounds__(S::THREADS, S::PER_S
             if constexpr (TOTAL) shared[(wn * 3 + 2) * ROWS + row] = total;
         }
         // the z of the row's own class
-        const bool mine = counts(t, p.ignore, p.classes) && t >= cw && t < cw + 32 * JN && (((int)(t - cw) >> 2) & 1) == lg;
+        const int at = own[i];
+        const bool mine = at >= 0 && ((at >> 2) & 1) == lg;
         if (__ballot(mine) != 0) {
-            const int at = (int)(t - cw), reg = (at >> 5) * 16 + ((at & 31) >> 3) * 4 + (at & 3);
+            const int reg = (at >> 5) * 16 + ((at & 31) >> 3) * 4 + (at & 3);
             float z = 0.f;
 #pragma unroll
             for (int j = 0; j < JN; j++)
 #pragma unroll
                 for (int v = 0; v < 16; v++) z = reg == j * 16 + v ? acc[i][j][v] : z;
-            if (mine) p.target_z[r] = z;
+            if (mine) p.target_z[r0 + row] = z;
         }
     }
     __syncthreads();
@@ -462,32 +468,68 @@ template <class S> __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void cr
             *reinterpret_cast<u32x4 *>(p.x_copy + r * p.width + c) = v;
         }
     }
+    const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
+    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
+    const int64_t cw = c0 + wn * 32 * JN;
+    const bool edge = cw + 32 * JN > p.v1;
+    // what the rows bring, asked for before the product
+    const float even = p.smoothing / (float)p.classes;
+    int own[IM];
+    bool lives[IM];
+    float tops[IM], invs[IM], scales[IM];
+#pragma unroll
+    for (int i = 0; i < IM; i++) {
+        const int64_t r = r0 + (wm * IM + i) * 32 + lr, at = r < p.rows ? r : p.rows - 1, t = p.target[at];
+        lives[i] = r < p.rows && counts(t, p.ignore, p.classes);
+        own[i] = lives[i] && t >= cw && t < cw + 32 * JN && t < p.v1 ? (int)(t - cw) : -1;
+        const float top = p.row_max[at], inv = p.row_inv[at], g = p.row_scale != nullptr ? p.row_scale[at] : 1.f;
+        tops[i] = lives[i] ? top : 0.f;
+        scales[i] = lives[i] ? g : 0.f;
+        invs[i] = lives[i] ? inv * g : 0.f;
+    }
     f32x16 acc[IM][JN] = {};
     float none[IM];
     const Loader<true, S::ROWS, S::SLAB, S::WAVES> a(p.x, r0, p.rows, 0);
     const Loader<true, S::COLS, S::SLAB, S::WAVES> b(p.w, c0, p.classes, 0);
     multiply_tile<S, true, true, false>(a, b, 0, p.stages, smem, acc, false, none);
-    const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
-    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
-    const int64_t cw = c0 + wn * 32 * JN;
     logits<S>(bias + wn * 32 * JN, acc);
-    const float even = p.smoothing / (float)p.classes;
-    const bool edge = cw + 32 * JN > p.v1;
+    // To memory: half-wave swaps leave a lane 8 consecutive classes.  bf16: as they are, 32 bytes of a row side by side, while the other
+    // workgroup of the compute unit multiplies (8192 x 1024 x 65536: 313 us a piece, by way of LDS 328).  fp32, where a workgroup
+    // is alone: part by part through LDS, rows in whole lines (2048 x 384 x 21841: 290 us without, 251 so).
+    constexpr int PITCH = S::COLS * 2 + 16, VECS = S::COLS / 8;
+    static_assert(S::PARTS == 1 || S::ROWS * PITCH <= S::RING, "LDS");
+    auto put = [&](int i, bool rest) {              // and what is left of the values for the next part
+        bf16_t *const row = p.d + (r0 + (wm * IM + i) * 32 + lr) * p.d_pitch + (cw - p.v0) + 8 * lg;
+        unsigned char *const at = smem + ((wm * IM + i) * 32 + lr) * PITCH + wn * 64 * JN + 16 * lg;
+#pragma unroll
+        for (int j = 0; j < JN; j++)
+#pragma unroll
+            for (int q = 0; q < 2; q++) {
+                uint32_t o[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    o[e] = pack_bf16x2(acc[i][j][8 * q + 2 * e], acc[i][j][8 * q + 2 * e + 1]);
+                    if (rest) acc[i][j][8 * q + 2 * e] -= bf16lo(o[e]), acc[i][j][8 * q + 2 * e + 1] -= bf16hi(o[e]);
+                }
+                const auto s0 = __builtin_amdgcn_permlane32_swap(o[0], o[2], false, false), s1 = __builtin_amdgcn_permlane32_swap(o[1], o[3], false, false);
+                const u32x4 v = {s0[0], s1[0], s0[1], s1[1]};
+                if constexpr (S::PARTS == 1) *reinterpret_cast<u32x4 *>(row + j * 32 + 16 * q) = v;
+                else *reinterpret_cast<u32x4 *>(at + j * 64 + 32 * q) = v;
+            }
+    };
 #pragma unroll
     for (int i = 0; i < IM; i++) {
-        const int64_t r = r0 + (wm * IM + i) * 32 + lr;
-        const int64_t t = r < p.rows ? p.target[r] : -1;
-        const bool live = r < p.rows && counts(t, p.ignore, p.classes);
-        const float g = live ? (p.row_scale != nullptr ? p.row_scale[r] : 1.f) : 0.f;
-        const float top = live ? p.row_max[r] : 0.f, inv = live ? p.row_inv[r] * g : 0.f, minus = -even * g;
+        const bool live = lives[i];
+        const float top = tops[i], inv = invs[i], minus = -even * scales[i];
 #pragma unroll
         for (int j = 0; j < JN; j++)
 #pragma unroll
             for (int v = 0; v < 16; v++) acc[i][j][v] = __builtin_fmaf(__builtin_amdgcn_exp2f(acc[i][j][v] - top), inv, minus);
-        const bool mine = live && t >= cw && t < cw + 32 * JN && t < p.v1 && (((int)(t - cw) >> 2) & 1) == lg;
+        const int at = own[i];
+        const bool mine = at >= 0 && ((at >> 2) & 1) == lg;
         if (__ballot(mine) != 0) {
-            const int at = (int)(t - cw), reg = mine ? (at >> 5) * 16 + ((at & 31) >> 3) * 4 + (at & 3) : -1;
-            const float one = (1.f - p.smoothing) * g;
+            const int reg = mine ? (at >> 5) * 16 + ((at & 31) >> 3) * 4 + (at & 3) : -1;
+            const float one = (1.f - p.smoothing) * scales[i];
 #pragma unroll
             for (int j = 0; j < JN; j++)
 #pragma unroll
@@ -499,26 +541,22 @@ template <class S> __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void cr
 #pragma unroll
                 for (int v = 0; v < 16; v++) acc[i][j][v] = live && cw + j * 32 + 8 * (v / 4) + 4 * lg + v % 4 < p.v1 ? acc[i][j][v] : 0.f;
         }
-        // to memory: half-wave swaps leave a lane 8 consecutive classes
-        bf16_t *const row = p.d + r * p.d_pitch + (cw - p.v0) + 8 * lg;
+        put(i, S::PARTS > 1);
+    }
+    if constexpr (S::PARTS > 1) {
+        for (int part = 0; part < S::PARTS; part++) {
+            if (part > 0) {
+                __syncthreads();
 #pragma unroll
-        for (int j = 0; j < JN; j++)
-#pragma unroll
-            for (int q = 0; q < 2; q++) {
-                float f[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) f[e] = acc[i][j][8 * q + e];
-#pragma unroll
-                for (int part = 0; part < S::PARTS; part++) {
-                    const uint32_t o0 = pack_bf16x2(f[0], f[1]), o1 = pack_bf16x2(f[2], f[3]), o2 = pack_bf16x2(f[4], f[5]), o3 = pack_bf16x2(f[6], f[7]);
-                    const auto s0 = __builtin_amdgcn_permlane32_swap(o0, o2, false, false), s1 = __builtin_amdgcn_permlane32_swap(o1, o3, false, false);
-                    *reinterpret_cast<u32x4 *>(row + part * p.d_plane + j * 32 + 16 * q) = u32x4{s0[0], s1[0], s0[1], s1[1]};
-                    if (part + 1 < S::PARTS) {
-                        f[0] -= bf16lo(o0), f[1] -= bf16hi(o0), f[2] -= bf16lo(o1), f[3] -= bf16hi(o1);
-                        f[4] -= bf16lo(o2), f[5] -= bf16hi(o2), f[6] -= bf16lo(o3), f[7] -= bf16hi(o3);
-                    }
-                }
+                for (int i = 0; i < IM; i++) put(i, part + 1 < S::PARTS);
             }
+            __syncthreads();
+            bf16_t *const to = p.d + part * p.d_plane + r0 * p.d_pitch + (c0 - p.v0);
+#pragma unroll 4
+            for (int k = threadIdx.x; k < S::ROWS * VECS; k += S::THREADS)
+                *reinterpret_cast<u32x4 *>(to + (int64_t)(k / VECS) * p.d_pitch + (k % VECS) * 8) =
+                    *reinterpret_cast<const u32x4 *>(smem + (k / VECS) * PITCH + (k % VECS) * 16);
+        }
     }
 }
 
@@ -552,10 +590,10 @@ template <class S, bool A_ALONG> __device__ __forceinline__ void gradient_tile(c
     const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
     const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
     const bool with_sums = !A_ALONG && n == 0 && wn == 0 && (p.sums_part != nullptr || p.sums != nullptr);
-    multiply_tile<S, A_ALONG, false, !A_ALONG>(a, b, t0, t1, smem, acc, with_sums, sums);
     float scale = 1.f;
     if (all.scale != nullptr) scale = *all.scale;
     if (all.scale2 != nullptr) scale *= *all.scale2;
+    multiply_tile<S, A_ALONG, false, !A_ALONG>(a, b, t0, t1, smem, acc, with_sums, sums);
 #pragma unroll
     for (int i = 0; i < IM; i++) {
         const int64_t r = r0 + (wm * IM + i) * 32 + lr;
@@ -652,20 +690,34 @@ __global__ __launch_bounds__(256) void cross_entropy_sum_kernel(SumArgs p)
 }
 
 // Rows as the product routine reads them: `width` filled up with zeros to whole slabs, fp32 in three parts; rows that are left out
-// (target given) as zeros, so that what they hold reaches no gradient.
-template <typename T> __global__ __launch_bounds__(256) void cross_entropy_pack_kernel(const T *__restrict__ from, int64_t ld, int64_t rows, int width, int padded,
-                                                                                       const int64_t *__restrict__ target, int64_t ignore, int64_t classes,
-                                                                                       bf16_t *__restrict__ to, int64_t plane)
+// (target given) as zeros, so that what they hold reaches no gradient.  Up to two operands in one launch.
+struct PackJob {
+    const void *from; int64_t ld, rows; const int64_t *target; bf16_t *to;
+};
+struct PackArgs {
+    PackJob job[2];
+    int64_t first;                                  // workgroups of the first
+    int width, padded; int64_t ignore, classes;
+};
+template <typename T> __global__ __launch_bounds__(256) void cross_entropy_pack_kernel(PackArgs p)
 {
-    const int per_row = padded / 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, r = i / per_row;
-    if (r >= rows) return;
+    const bool second = (int64_t)blockIdx.x >= p.first;
+    const PackJob &job = p.job[second ? 1 : 0];
+    const int per_row = p.padded / 8;
+    const int64_t i = ((int64_t)blockIdx.x - (second ? p.first : 0)) * 256 + threadIdx.x, r = i / per_row;
+    if (r >= job.rows) return;
     const int c = (int)(i - r * per_row) * 8;
-    const bool live = target == nullptr || counts(target[r], ignore, classes);
+    const bool live = job.target == nullptr || counts(job.target[r], p.ignore, p.classes);
+    const T *const from = static_cast<const T *>(job.from) + r * job.ld + c;
     float f[8];
+    if (live && c + 8 <= p.width && ((uintptr_t)from & 15) == 0) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) f[e] = live && c + e < width ? Elem<T>::load(from + r * ld + c + e) : 0.f;
-    bf16_t *const at = to + r * padded + c;
+        for (int e = 0; e < 8; e += Elem<T>::VEC) Elem<T>::unpack(*reinterpret_cast<const u32x4 *>(from + e), f + e);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[e] = live && c + e < p.width ? Elem<T>::load(from + e) : 0.f;
+    }
+    bf16_t *const at = job.to + r * p.padded + c;
     *reinterpret_cast<u32x4 *>(at) = Elem<bf16_t>::pack(f);
     if constexpr (sizeof(T) == 4) {
         // (infinity and NaN have no rest)
@@ -676,7 +728,7 @@ template <typename T> __global__ __launch_bounds__(256) void cross_entropy_pack_
                 const float rest = f[e] - Elem<bf16_t>::round(f[e]);
                 f[e] = fabsf(rest) < INFINITY ? rest : 0.f;
             }
-            *reinterpret_cast<u32x4 *>(at + part * plane) = Elem<bf16_t>::pack(f);
+            *reinterpret_cast<u32x4 *>(at + part * job.rows * p.padded) = Elem<bf16_t>::pack(f);
         }
     }
 }
@@ -694,7 +746,7 @@ using SplitFlat = Shape<1, 2, 2, 2, 32, 3, 3>;
 using SplitSmall = Shape<1, 1, 2, 2, 32, 4, 3>;
 
 constexpr int CE_PAD = 64;                          // rows of operands are filled up to whole slabs of any shape
-constexpr int64_t CE_PIECE_BYTES = 256ll << 20;     // of d
+constexpr int64_t CE_PIECE_BYTES = 320ll << 20;     // of d
 enum { CE_LARGE, CE_FLAT, CE_SMALL };
 
 // Everything a call lays out, the same for the size and the call.
@@ -845,26 +897,31 @@ static bool lies_well(const void *src, int64_t ld, const CePlan &p)
 {
     return !p.split && p.width == p.padded && ld % 8 == 0 && ld < (1 << 22) && ((uintptr_t)src & 15) == 0;
 }
-// an operand as it lies, else packed at `at`; rows that are left out as zeros where `target` is given
-static int operand_of(Operand &o, const void *src, int64_t ld, int64_t rows, const CePlan &p, const int64_t *target, int64_t ignore, unsigned char *at,
-                      hipStream_t st)
+// x and W as they lie, else packed in the workspace; rows of x that are left out as zeros there
+static int operands_of(CeArgs &a, const void *x, int64_t ldx, const void *w, int64_t ldw, const CePlan &p, unsigned char *ws, hipStream_t st)
 {
-    if (lies_well(src, ld, p)) {
-        o = Operand{(const bf16_t *)src, ld, 0};
-        return VTDGE_OK;
-    }
-    o = Operand{(const bf16_t *)at, p.padded, rows * p.padded};
-    const int64_t blocks = ceil_div(rows * (p.padded / 8), 256);
-    VT_REQUIRE(blocks < (1 << 24), VTDGE_ERR_UNSUPPORTED, "cross_entropy: %lld rows of %d", (long long)rows, p.width);
-    if (p.split) {
-        note_kernel(reinterpret_cast<const void *>(cross_entropy_pack_kernel<float>));
-        cross_entropy_pack_kernel<float><<<(unsigned)blocks, 256, 0, st>>>((const float *)src, ld, rows, p.width, p.padded, target, ignore, p.classes,
-                                                                           (bf16_t *)at, o.plane);
-    } else {
-        note_kernel(reinterpret_cast<const void *>(cross_entropy_pack_kernel<bf16_t>));
-        cross_entropy_pack_kernel<bf16_t><<<(unsigned)blocks, 256, 0, st>>>((const bf16_t *)src, ld, rows, p.width, p.padded, target, ignore, p.classes,
-                                                                            (bf16_t *)at, o.plane);
-    }
+    PackArgs g{};
+    int n = 0;
+    int64_t blocks = 0;
+    auto take = [&](Operand &o, const void *src, int64_t ld, int64_t rows, const int64_t *target, int64_t at) {
+        if (lies_well(src, ld, p)) {
+            o = Operand{(const bf16_t *)src, ld, 0};
+            return;
+        }
+        bf16_t *const to = (bf16_t *)(ws + at);
+        o = Operand{to, p.padded, rows * p.padded};
+        g.job[n++] = PackJob{src, ld, rows, target, to};
+        blocks += ceil_div(rows * (p.padded / 8), 256);
+        if (n == 1) g.first = blocks;
+    };
+    take(a.x, x, ldx, p.rows, a.target, p.x_at);
+    take(a.w, w, ldw, p.classes, nullptr, p.w_at);
+    if (n == 0) return VTDGE_OK;
+    g.width = p.width, g.padded = p.padded, g.ignore = a.ignore, g.classes = p.classes;
+    VT_REQUIRE(blocks < (1 << 24), VTDGE_ERR_UNSUPPORTED, "cross_entropy: %lld blocks to lay out", (long long)blocks);
+    auto kern = p.split ? cross_entropy_pack_kernel<float> : cross_entropy_pack_kernel<bf16_t>;
+    note_kernel(reinterpret_cast<const void *>(kern));
+    kern<<<(unsigned)blocks, 256, 0, st>>>(g);
     return check_launch("cross_entropy");
 }
 
@@ -932,6 +989,12 @@ static int sum_up(const SumJob *jobs, int count, const float *scale, const float
 
 using namespace vtdge;
 
+extern "C" int64_t vtdge_cross_entropy_laid_out(int64_t rows, int64_t classes, int width, int dtype)
+{
+    if (check_sizes("cross_entropy_laid_out", rows, classes, width, dtype) != VTDGE_OK) return -1;
+    return plan_of(rows, classes, width, dtype, false).max_at;
+}
+
 extern "C" int64_t vtdge_cross_entropy_workspace(int64_t rows, int64_t classes, int width, int dtype, int backward)
 {
     if (check_sizes("cross_entropy_workspace", rows, classes, width, dtype) != VTDGE_OK) return -1;
@@ -954,9 +1017,9 @@ extern "C" int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weigh
     unsigned char *const ws = (unsigned char *)workspace;
     const hipStream_t st = (hipStream_t)stream;
     CeArgs a{};
-    VT_STEP(operand_of(a.x, x, ldx, rows, p, nullptr, ignore_index, ws + p.x_at, st));
-    VT_STEP(operand_of(a.w, weight, ldw, classes, p, nullptr, ignore_index, ws + p.w_at, st));
-    a.bias = bias, a.bias_f32 = p.split, a.target = target, a.rows = rows, a.classes = classes, a.ignore = ignore_index;
+    a.target = target, a.ignore = ignore_index;
+    VT_STEP(operands_of(a, x, ldx, weight, ldw, p, ws, st));
+    a.bias = bias, a.bias_f32 = p.split, a.rows = rows, a.classes = classes;
     a.smoothing = smoothing, a.stages = (int)ceil_div(p.padded, p.slab_l), a.v0 = 0, a.v1 = classes;
     a.tile_max = (float *)(ws + p.max_at), a.tile_sum = (float *)(ws + p.sum_at), a.tile_total = (float *)(ws + p.total_at);
     a.target_z = (float *)(ws + p.z_at);
@@ -983,12 +1046,13 @@ extern "C" int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weigh
 extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, const int64_t *target,
                                             const float *row_max, const float *row_inv, const float *grad, int grad_stride,
                                             const float *inv_count, int64_t rows, int64_t classes, int width, int64_t ignore_index,
-                                            float smoothing, void *workspace, int64_t workspace_bytes, void *dx, void *dweight, void *dbias,
-                                            int dtype, void *stream)
+                                            float smoothing, const void *laid_out, void *workspace, int64_t workspace_bytes, void *dx,
+                                            void *dweight, void *dbias, int dtype, void *stream)
 {
     VT_STEP(check_sizes("cross_entropy_backward", rows, classes, width, dtype));
     VT_REQUIRE(x && weight && target && row_max && row_inv && grad && workspace, VTDGE_ERR_ARG, "cross_entropy_backward: NULL operand");
     VT_REQUIRE(ldx >= width && ldw >= width, VTDGE_ERR_ARG, "cross_entropy_backward: rows of %d, %lld and %lld apart", width, (long long)ldx, (long long)ldw);
+    VT_REQUIRE(((uintptr_t)laid_out & 255) == 0, VTDGE_ERR_ARG, "cross_entropy_backward: laid_out off its boundary");
     VT_REQUIRE(grad_stride == 0 || (grad_stride == 1 && inv_count == nullptr), VTDGE_ERR_ARG, "cross_entropy_backward: grad_stride %d", grad_stride);
     VT_REQUIRE(smoothing >= 0.f && smoothing <= 1.f, VTDGE_ERR_ARG, "cross_entropy_backward: smoothing %g", (double)smoothing);
     const CePlan p = plan_of(rows, classes, width, dtype, true);
@@ -998,12 +1062,19 @@ extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const vo
     unsigned char *const ws = (unsigned char *)workspace;
     const hipStream_t st = (hipStream_t)stream;
     CeArgs a{};
-    VT_STEP(operand_of(a.w, weight, ldw, classes, p, nullptr, ignore_index, ws + p.w_at, st));
-    VT_STEP(operand_of(a.x, x, ldx, rows, p, target, ignore_index, ws + p.x_at, st));
+    a.target = target, a.ignore = ignore_index;
+    if (laid_out != nullptr) {
+        // as the forward call left them: both plans begin alike
+        unsigned char *const from = (unsigned char *)const_cast<void *>(laid_out);
+        a.x = lies_well(x, ldx, p) ? Operand{(const bf16_t *)x, ldx, 0} : Operand{(const bf16_t *)(from + p.x_at), p.padded, rows * p.padded};
+        a.w = lies_well(weight, ldw, p) ? Operand{(const bf16_t *)weight, ldw, 0} : Operand{(const bf16_t *)(from + p.w_at), p.padded, classes * p.padded};
+    } else {
+        VT_STEP(operands_of(a, x, ldx, weight, ldw, p, ws, st));
+    }
     Operand clean = a.x;                            // x with zeros for the rows that are left out, so that what they hold reaches no gradient
     const bool copy = lies_well(x, ldx, p) && (dweight != nullptr || dbias != nullptr);
     if (copy) clean = Operand{(const bf16_t *)(ws + p.x_at), p.padded, 0};
-    a.bias = bias, a.bias_f32 = p.split, a.target = target, a.rows = rows, a.classes = classes, a.ignore = ignore_index;
+    a.bias = bias, a.bias_f32 = p.split, a.rows = rows, a.classes = classes;
     a.smoothing = smoothing, a.stages = (int)ceil_div(p.padded, p.slab_l), a.width = p.padded;
     a.row_max = row_max, a.row_inv = row_inv, a.row_scale = grad_stride == 1 ? grad : nullptr;
     a.d = (bf16_t *)(ws + p.d_at), a.d_pitch = p.piece, a.d_plane = p.d_rows * p.piece;

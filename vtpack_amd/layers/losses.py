@@ -15,7 +15,7 @@ def _no_second_order(name):
 class _LinearCrossEntropy(Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, ignore_index, label_smoothing, reduction):
-        loss, stats = ops.cross_entropy(x, weight, bias, target, ignore_index, label_smoothing, reduction)
+        loss, stats, ctx.laid_out = ops.cross_entropy(x, weight, bias, target, ignore_index, label_smoothing, reduction)
         ctx.how = (ignore_index, label_smoothing, reduction)
         ctx.save_for_backward(x, weight, bias, target, stats)
         return loss
@@ -27,7 +27,7 @@ class _LinearCrossEntropy(Function):
         if grad.dim() == 1:
             # the same for every row, as a sum over the losses leaves it: one value
             grad = grad[0] if grad.stride(0) == 0 else grad.contiguous()
-        dx, dw, db = ops.cross_entropy_backward(ops._rows_of(x), ops._rows_of(weight), bias, target, stats, grad, *ctx.how,
+        dx, dw, db = ops.cross_entropy_backward(ops._rows_of(x), ops._rows_of(weight), bias, target, stats, ctx.laid_out, grad, *ctx.how,
                                                 needs=ctx.needs_input_grad)
         return dx, dw, db, None, None, None, None
 
@@ -41,7 +41,7 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     (F.cross_entropy stops the program there).  Without a row that counts the loss is 0, and so are the gradients.
 
     The logits are fp32 sums and are not rounded; in bfloat16 the gradients of the logits are, once, before the products that
-    take them to x, weight and bias.  They work in pieces of the classes with some 256 MB of scratch for a piece; float32
+    take them to x, weight and bias.  They work in pieces of the classes with some 320 MB of scratch for a piece; float32
     operands are laid out anew in three parts of two bytes for the time of a call."""
     ops._need_gpu(x, weight, bias, target)
     if reduction not in ("mean", "sum", "none"):

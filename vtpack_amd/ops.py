@@ -1117,10 +1117,18 @@ def _cross_entropy_workspace(rows, classes, width, dtype, backward):
     return size
 
 
+KEEP_LAID_OUT = 16 << 20           # bytes
+
+
+@functools.lru_cache(maxsize=1024)
+def _cross_entropy_laid_out(rows, classes, width, dtype):
+    return _lib.load().vtdge_cross_entropy_laid_out(rows, classes, width, dtype)
+
+
 def cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
     """Softmax cross entropy of x [rows, width] @ weight [classes, width]^T + bias against int64 target [rows] (rows > 0, rows of
-    x and weight dense): -> (fp32 loss, stats for `cross_entropy_backward`).  The loss is the rows' mean or sum, or each
-    row's own ("none")."""
+    x and weight dense): -> (fp32 loss, stats and laid_out for `cross_entropy_backward`).  The loss is the rows' mean or sum, or
+    each row's own ("none")."""
     (rows, width), classes, dtype, device = x.shape, weight.shape[0], dtype_code(x), x.device
     with _on(x):
         ws = torch.empty((_cross_entropy_workspace(rows, classes, width, dtype, 0),), dtype=torch.uint8, device=device)
@@ -1133,10 +1141,13 @@ def cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoothing=0.
              classes, width, ignore_index, label_smoothing, ws.data_ptr(), ws.numel(),
              out if reduction == "none" else at + 8 * rows + 4, at, at + 4 * rows, 0 if reduction == "none" else out,
              at + 8 * rows if reduction == "mean" else 0, dtype, stream_ptr(), tag=("cross_entropy", rows, classes, width))
-    return loss, stats
+    # Operands that do not lie as the kernels read them were laid out in the workspace.  Where that is little beside what a call
+    # takes anyway (another launch), it is kept for the gradients; larger ones are laid out again there.
+    kept = (dtype != _lib.BF16 or width % 64 != 0) and _cross_entropy_laid_out(rows, classes, width, dtype) <= KEEP_LAID_OUT
+    return loss, stats, ws if kept else None
 
 
-def cross_entropy_backward(x, weight, bias, target, stats, grad, ignore_index=-100, label_smoothing=0.0, reduction="mean",
+def cross_entropy_backward(x, weight, bias, target, stats, laid_out, grad, ignore_index=-100, label_smoothing=0.0, reduction="mean",
                            needs=(True, True, True)):
     """Gradients (dx, dweight, dbias; None where not needed) of `cross_entropy` for the fp32 gradient of its loss: a scalar, with
     "none" also one value for each row."""
@@ -1149,7 +1160,7 @@ def cross_entropy_backward(x, weight, bias, target, stats, grad, ignore_index=-1
         at = stats.data_ptr()
         call("vtdge_cross_entropy_backward", x.data_ptr(), _pitch(x), weight.data_ptr(), _pitch(weight), ptr(bias), target.data_ptr(),
              at, at + 4 * rows, grad.data_ptr(), grad.dim(), at + 8 * rows if reduction == "mean" else 0, rows, classes, width,
-             ignore_index, label_smoothing, ws.data_ptr(), ws.numel(), ptr(dx), ptr(dw), ptr(db), dtype, stream_ptr(),
+             ignore_index, label_smoothing, ptr(laid_out), ws.data_ptr(), ws.numel(), ptr(dx), ptr(dw), ptr(db), dtype, stream_ptr(),
              tag=("cross_entropy_backward", rows, classes, width))
     return dx, dw, db
 
