@@ -177,16 +177,20 @@ __device__ __forceinline__ void multiply_tile(const Loader<A_ALONG, S::ROWS, S::
     lds_barrier();                                  // the ring is free for the epilogue
 }
 
-// Workgroup id -> tile: an XCD (every eighth id) takes a contiguous run of the list, which goes through eight row tiles for each
-// column tile, so that what its L2 holds is used again.
-__device__ __forceinline__ void tile_of(int id, int count, int tm, int tn, int &m, int &n)
+// Workgroup id -> part of the sum and tile: an XCD (every eighth id) takes a contiguous run of the list of all parts' tiles, which
+// goes through eight row tiles for each column tile, so that what its L2 holds is used again.
+__device__ __forceinline__ int tile_of(int id, int parts, int tm, int tn, int &m, int &n)
 {
+    const int tiles = tm * tn, count = tiles * parts;
     const int xcd = id & 7, at = id >> 3, whole = count >> 3, rest = count & 7;
     id = xcd * whole + (xcd < rest ? xcd : rest) + at;
+    const int part = id / tiles;
+    id -= part * tiles;
     const int group = 8 * tn, g = id / group, first = g * 8, size = min(8, tm - first);
     const int in = id - g * group;
     m = first + in % size;
     n = in / size;
+    return part;
 }
 
 struct CeArgs {
@@ -238,7 +242,7 @@ template <class S, bool TOTAL> __global__ __launch_bounds__(S::THREADS, S::PER_S
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr int IM = S::IM, JN = S::JN, ROWS = S::ROWS;
     int m, n;
-    tile_of(blockIdx.x, gridDim.x, tm, tn, m, n);
+    tile_of(blockIdx.x, 1, tm, tn, m, n);
     const int64_t r0 = (int64_t)m * ROWS, c0 = (int64_t)n * S::COLS;
     float *const bias = reinterpret_cast<float *>(smem + S::RING);
     read_bias<S>(p, c0, bias);
@@ -452,7 +456,7 @@ template <class S> __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void cr
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr int IM = S::IM, JN = S::JN;
     int m, n;
-    tile_of(blockIdx.x, gridDim.x, tm, tn, m, n);
+    tile_of(blockIdx.x, 1, tm, tn, m, n);
     const int64_t r0 = (int64_t)m * S::ROWS, c0 = p.v0 + (int64_t)n * S::COLS;
     float *const bias = reinterpret_cast<float *>(smem + S::RING);
     read_bias<S>(p, c0, bias);
@@ -578,9 +582,8 @@ struct GradPair {
 template <class S, bool A_ALONG> __device__ __forceinline__ void gradient_tile(const GradArgs &p, const GradPair &all, int id, unsigned char *smem)
 {
     constexpr int IM = S::IM, JN = S::JN;
-    const int tiles = p.tm * p.tn, z = id / tiles;
     int m, n;
-    tile_of(id - z * tiles, tiles, p.tm, p.tn, m, n);
+    const int z = tile_of(id, p.splits, p.tm, p.tn, m, n);
     const int64_t r0 = (int64_t)m * S::ROWS, c0 = (int64_t)n * S::COLS;
     const int t0 = (int)((int64_t)p.stages * z / p.splits), t1 = (int)((int64_t)p.stages * (z + 1) / p.splits);
     f32x16 acc[IM][JN] = {};
@@ -799,33 +802,33 @@ static int64_t makespan(int64_t slots, int64_t n1, int64_t l1, int64_t n2, int64
 }
 
 // Shape and cuts of both gradients of a piece.  Large tiles where their work is 16 slabs for each workgroup that runs at a time; then as
-// many parts of each sum as end first: a slab of a large tile takes about a microsecond (two workgroups a compute unit, 1 PFLOP/s;
-// with fp32 operands a workgroup has the unit for itself and six times the products), a tile four for its epilogue, and parts are
-// written and read again at 4 TB/s.
+// many parts of each sum as end first, for compute units that take one tile after the other (two workgroups side by side share one):
+// a slab of a large tile takes 0.55 us there, six times the products of fp32 operands 3 us, of a small tile 0.35 and 0.6, a tile four
+// slabs for its epilogue, and parts are written and read again at 4 TB/s.  us of a backward call, uncut / as chosen: bf16 2999 x
+// 768 x 21841 555 / 385, 300 x 768 x 21841 389 / 83, 8192 x 384 x 1000 116 / 82, 5000 x 1024 x 5000 227 / 203; fp32 2048 x 384 x
+// 21841 1715 / 640, 128 x 768 x 21841 1338 / 166.  All but one of 15 sizes are within 4 percent of their best cut.
 static void plan_gradients(CePlan &p, int64_t of_piece)
 {
     const int64_t cu = compute_units();
-    int64_t slots = p.split ? cu : 2 * cu;
     if (p.split) use<SplitLarge>(p.gm, p.gn, p.slab_g);
     else use<GradLarge>(p.gm, p.gn, p.slab_g);
     auto tiles = [&](int64_t rows) { return ceil_div(rows, p.gm) * ceil_div(p.width, p.gn); };
-    if (tiles(p.rows) * ceil_div(of_piece, p.slab_g) + tiles(of_piece) * ceil_div(p.rows, p.slab_g) >= 16 * slots) {
+    if (tiles(p.rows) * ceil_div(of_piece, p.slab_g) + tiles(of_piece) * ceil_div(p.rows, p.slab_g) >= 16 * cu * (p.split ? 1 : 2)) {
         p.grads = CE_LARGE;
     } else {
-        p.grads = CE_SMALL, slots = cu;
+        p.grads = CE_SMALL;
         if (p.split) use<SplitSmall>(p.gm, p.gn, p.slab_g);
         else use<GradSmall>(p.gm, p.gn, p.slab_g);
     }
     const int64_t tx = tiles(p.rows), tw = tiles(of_piece), sx = ceil_div(of_piece, p.slab_g), sw = ceil_div(p.rows, p.slab_g);
-    const double slab = p.grads == CE_LARGE ? (p.split ? 3.0 : 1.05) : (p.split ? 0.6 : 0.35);
+    const double slab = p.grads == CE_LARGE ? (p.split ? 3.0 : 0.55) : (p.split ? 0.6 : 0.35);
     double best = 1e30;
     p.dx_splits = p.dw_splits = 1;
     for (int64_t x = 1; x <= 32 && (x == 1 || sx / x >= 8); x++)
         for (int64_t w = 1; w <= 32 && (w == 1 || sw / w >= 8); w++) {
-            if (x > 1 && tx * x > 4 * slots) continue;
-            if (w > 1 && tw * w > 4 * slots) continue;
+            if ((x > 1 && tx * x > 8 * cu) || (w > 1 && tw * w > 8 * cu)) continue;
             const double bytes = ((x > 1 ? 8.0 * x * p.rows : 0.0) + (w > 1 ? 8.0 * w * of_piece : 0.0)) * p.width;
-            const double t = slab * makespan(slots, tx * x, ceil_div(sx, x) + 4, tw * w, ceil_div(sw, w) + 4) + bytes / 4e6 + (x > 1 || w > 1 ? 5.0 : 0.0);
+            const double t = slab * makespan(cu, tx * x, ceil_div(sx, x) + 4, tw * w, ceil_div(sw, w) + 4) + bytes / 4e6 + (x > 1 || w > 1 ? 5.0 : 0.0);
             if (t < best) best = t, p.dx_splits = (int)x, p.dw_splits = (int)w;
         }
 }
