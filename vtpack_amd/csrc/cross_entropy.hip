@@ -138,22 +138,31 @@ __device__ __forceinline__ void multiply_tile(const Loader<A_ALONG, S::ROWS, S::
             if (behind == x) wait_vmcnt<x * LOADS>();
         });
         lds_barrier();                              // everybody's have, and the slot before this one is read no more
+        const unsigned char *sa = smem + out * S::STAGE, *sb = sa + A_BYTES;
+        out = out == SLOTS - 1 ? 0 : out + 1;
+        // fragments a step ahead of their products, the direct loads behind the first of them
+        constexpr int STEPS = S::SLAB / 16;
+        u32x4 fa[2][PARTS][IM], fb[2][PARTS][JN];
+        auto fetch = [&](int s) {
+#pragma unroll
+            for (int p = 0; p < PARTS; p++) {
+#pragma unroll
+                for (int i = 0; i < IM; i++) fa[s & 1][p][i] = LA::fragment(sa + p * LA::STAGE, wm * IM + i, s);
+#pragma unroll
+                for (int j = 0; j < JN; j++) fb[s & 1][p][j] = LB::fragment(sb + p * LB::STAGE, wn * JN + j, s);
+            }
+        };
+        fetch(0);
+        __builtin_amdgcn_sched_barrier(0);
         if (t + SLOTS - 1 < t1) {
             issue(t + SLOTS - 1, in);
             in = in == SLOTS - 1 ? 0 : in + 1;
         }
-        const unsigned char *sa = smem + out * S::STAGE, *sb = sa + A_BYTES;
-        out = out == SLOTS - 1 ? 0 : out + 1;
 #pragma unroll
-        for (int s = 0; s < S::SLAB / 16; s++) {
-            u32x4 fa[PARTS][IM], fb[PARTS][JN];
-#pragma unroll
-            for (int p = 0; p < PARTS; p++) {
-#pragma unroll
-                for (int i = 0; i < IM; i++) fa[p][i] = LA::fragment(sa + p * LA::STAGE, wm * IM + i, s);
-#pragma unroll
-                for (int j = 0; j < JN; j++) fb[p][j] = LB::fragment(sb + p * LB::STAGE, wn * JN + j, s);
-            }
+        for (int s = 0; s < STEPS; s++) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (s + 1 < STEPS) fetch(s + 1);
+            __builtin_amdgcn_sched_barrier(0);
             // smallest products first: parts whose numbers add up to 2, to 1, to 0
 #pragma unroll
             for (int order = PARTS - 1; order >= 0; order--)
@@ -162,14 +171,16 @@ __device__ __forceinline__ void multiply_tile(const Loader<A_ALONG, S::ROWS, S::
 #pragma unroll
                     for (int i = 0; i < IM; i++)
 #pragma unroll
-                        for (int j = 0; j < JN; j++) Slab<bf16_t>::mma(fb[order - p][j], fa[p][i], acc[i][j]);
+                        for (int j = 0; j < JN; j++) Slab<bf16_t>::mma(fb[s & 1][order - p][j], fa[s & 1][p][i], acc[i][j]);
             if constexpr (SUMS) {
                 if (sums_wanted) {
 #pragma unroll
                     for (int p = PARTS - 1; p >= 0; p--)
 #pragma unroll
-                        for (int i = 0; i < IM; i++)
-                            sums[i] = bf16_pair_sum(fa[p][i].x, bf16_pair_sum(fa[p][i].y, bf16_pair_sum(fa[p][i].z, bf16_pair_sum(fa[p][i].w, sums[i]))));
+                        for (int i = 0; i < IM; i++) {
+                            const u32x4 &f = fa[s & 1][p][i];
+                            sums[i] = bf16_pair_sum(f.x, bf16_pair_sum(f.y, bf16_pair_sum(f.z, bf16_pair_sum(f.w, sums[i]))));
+                        }
                 }
             }
         }
@@ -737,12 +748,18 @@ template <typename T> __global__ __launch_bounds__(256) void cross_entropy_pack_
 }
 
 // ------------------------------------------------------------------------------------------------ on the host
-// Shapes.  Large tiles where there are enough of them to fill the chip; tiles of 64 x 64 with a deep ring else, where a call waits for
-// memory and not for products; 64 rows by 128 classes for few rows of many classes, which wait for W.
-using LogitsLarge = Shape<2, 4, 2, 2, 32, 3, 1>;
+// Shapes.  What bounds the large ones is how fast a compute unit takes its operands in: a slab of a 256 x 256 tile by eight waves is 64 KB
+// for 2048 clocks of products, of 128 x 256 96 KB, and direct loads of whole lines (slabs of 64) pass faster than of half ones.  The
+// matrix units of the first are busy for about 60 percent of a long product at the 1.8 GHz that remain, 1.1 PFLOP/s (8192 x 1024 x
+// 65536, with its epilogue); tiles of 128 x 256, two workgroups a compute unit, 0.97, but one's epilogue runs beside the other's
+// products, which makes up for it in short sums.  Tiles of 64 x 64 with a deep ring where a call waits for memory and not for products,
+// 64 rows by 128 classes for few rows of many classes, which wait for W.
+using LogitsLarge = Shape<2, 4, 4, 2, 64, 2, 1>;
+using LogitsMiddle = Shape<2, 4, 2, 2, 32, 3, 1>;
 using LogitsFlat = Shape<1, 2, 2, 2, 64, 3, 1>;
 using LogitsSmall = Shape<1, 1, 2, 2, 64, 6, 1>;
-using GradLarge = Shape<4, 2, 2, 2, 32, 3, 1>;
+using GradLarge = Shape<2, 4, 4, 2, 64, 2, 1>;
+using GradMiddle = Shape<2, 2, 4, 2, 64, 3, 1>;
 using GradSmall = Shape<1, 1, 2, 2, 64, 6, 1>;
 using SplitLarge = Shape<2, 2, 4, 2, 32, 2, 3>;
 using SplitFlat = Shape<1, 2, 2, 2, 32, 3, 3>;
@@ -750,7 +767,7 @@ using SplitSmall = Shape<1, 1, 2, 2, 32, 4, 3>;
 
 constexpr int CE_PAD = 64;                          // rows of operands are filled up to whole slabs of any shape
 constexpr int64_t CE_PIECE_BYTES = 320ll << 20;     // of d
-enum { CE_LARGE, CE_FLAT, CE_SMALL };
+enum { CE_LARGE, CE_MIDDLE, CE_FLAT, CE_SMALL };
 
 // Everything a call lays out, the same for the size and the call.
 struct CePlan {
@@ -801,36 +818,55 @@ static int64_t makespan(int64_t slots, int64_t n1, int64_t l1, int64_t n2, int64
     return at[groups - 1];
 }
 
-// Shape and cuts of both gradients of a piece.  Large tiles where their work is 16 slabs for each workgroup that runs at a time; then as
-// many parts of each sum as end first, for compute units that take one tile after the other (two workgroups side by side share one):
-// a slab of a large tile takes 0.55 us there, six times the products of fp32 operands 3 us, of a small tile 0.35 and 0.6, a tile four
-// slabs for its epilogue, and parts are written and read again at 4 TB/s.  us of a backward call, uncut / as chosen: bf16 2999 x
-// 768 x 21841 555 / 385, 300 x 768 x 21841 389 / 83, 8192 x 384 x 1000 116 / 82, 5000 x 1024 x 5000 227 / 203; fp32 2048 x 384 x
-// 21841 1715 / 640, 128 x 768 x 21841 1338 / 166.  All but one of 15 sizes are within 4 percent of their best cut.
-static void plan_gradients(CePlan &p, int64_t of_piece)
+// Shape and cuts of both gradients of a piece.  Large tiles where their work is 16 slabs for each compute unit; then the tiles and as
+// many parts of each sum as end first: a compute unit takes one tile after the other, a tile as long as its slabs (measured in long
+// products) and an epilogue, and parts are written and read again at 4 TB/s.  us of a backward call, uncut / as chosen: bf16 2999 x
+// 768 x 21841 555 / 360, 300 x 768 x 21841 389 / 83, 8192 x 384 x 1000 116 / 82; fp32 2048 x 384 x 21841 1715 / 640, 128 x 768 x
+// 21841 1338 / 166.
+struct GradShape {
+    int grads, m, n, slab;
+    double us, tile_us;                             // of a slab, of an epilogue
+};
+static double cuts(CePlan &p, const GradShape &s, int64_t of_piece, bool choose)
 {
-    const int64_t cu = compute_units();
-    if (p.split) use<SplitLarge>(p.gm, p.gn, p.slab_g);
-    else use<GradLarge>(p.gm, p.gn, p.slab_g);
-    auto tiles = [&](int64_t rows) { return ceil_div(rows, p.gm) * ceil_div(p.width, p.gn); };
-    if (tiles(p.rows) * ceil_div(of_piece, p.slab_g) + tiles(of_piece) * ceil_div(p.rows, p.slab_g) >= 16 * cu * (p.split ? 1 : 2)) {
-        p.grads = CE_LARGE;
-    } else {
-        p.grads = CE_SMALL;
-        if (p.split) use<SplitSmall>(p.gm, p.gn, p.slab_g);
-        else use<GradSmall>(p.gm, p.gn, p.slab_g);
-    }
-    const int64_t tx = tiles(p.rows), tw = tiles(of_piece), sx = ceil_div(of_piece, p.slab_g), sw = ceil_div(p.rows, p.slab_g);
-    const double slab = p.grads == CE_LARGE ? (p.split ? 3.0 : 0.55) : (p.split ? 0.6 : 0.35);
+    const int64_t cu = compute_units(), across = ceil_div(p.width, s.n);
+    const int64_t tx = ceil_div(p.rows, s.m) * across, tw = ceil_div(of_piece, s.m) * across, sx = ceil_div(of_piece, s.slab), sw = ceil_div(p.rows, s.slab);
+    const int64_t extra = (int64_t)(s.tile_us / s.us + 0.5);
     double best = 1e30;
-    p.dx_splits = p.dw_splits = 1;
     for (int64_t x = 1; x <= 32 && (x == 1 || sx / x >= 8); x++)
         for (int64_t w = 1; w <= 32 && (w == 1 || sw / w >= 8); w++) {
             if ((x > 1 && tx * x > 8 * cu) || (w > 1 && tw * w > 8 * cu)) continue;
             const double bytes = ((x > 1 ? 8.0 * x * p.rows : 0.0) + (w > 1 ? 8.0 * w * of_piece : 0.0)) * p.width;
-            const double t = slab * makespan(cu, tx * x, ceil_div(sx, x) + 4, tw * w, ceil_div(sw, w) + 4) + bytes / 4e6 + (x > 1 || w > 1 ? 5.0 : 0.0);
-            if (t < best) best = t, p.dx_splits = (int)x, p.dw_splits = (int)w;
+            const double t = s.us * makespan(cu, tx * x, ceil_div(sx, x) + extra, tw * w, ceil_div(sw, w) + extra) + bytes / 4e6 + (x > 1 || w > 1 ? 5.0 : 0.0);
+            if (t >= best) continue;
+            best = t;
+            if (choose) p.dx_splits = (int)x, p.dw_splits = (int)w;
         }
+    if (choose) p.grads = s.grads, p.gm = s.m, p.gn = s.n, p.slab_g = s.slab;
+    return best;
+}
+template <class S> static GradShape grad_shape(int grads, double us, double tile_us) { return GradShape{grads, S::ROWS, S::COLS, S::SLAB, us, tile_us}; }
+
+static void plan_gradients(CePlan &p, int64_t of_piece)
+{
+    const GradShape large = p.split ? grad_shape<SplitLarge>(CE_LARGE, 3.0, 12.0) : grad_shape<GradLarge>(CE_LARGE, 2.0, 6.0);
+    const GradShape middle = grad_shape<GradMiddle>(CE_MIDDLE, 1.3, 4.0);
+    const GradShape small = p.split ? grad_shape<SplitSmall>(CE_SMALL, 0.6, 2.4) : grad_shape<GradSmall>(CE_SMALL, 0.35, 1.4);
+    // slabs of 32 of 256 x 128 tiles
+    const int64_t work = ceil_div(p.width, 128) * (ceil_div(p.rows, 256) * ceil_div(of_piece, 32) + ceil_div(of_piece, 256) * ceil_div(p.rows, 32));
+    if (work < 16 * compute_units() * (p.split ? 1 : 2)) cuts(p, small, of_piece, true);
+    else if (p.split || cuts(p, large, of_piece, false) <= cuts(p, middle, of_piece, false)) cuts(p, large, of_piece, true);
+    else cuts(p, middle, of_piece, true);
+}
+
+// us of the tiles of the logits: rounds of large tiles, or of middle ones two on a compute unit, a last one of which may have it alone
+static bool large_logits(int64_t rows, int64_t classes, int padded)
+{
+    const int64_t cu = compute_units(), slabs = padded / 64;
+    const int64_t large = ceil_div(rows, LogitsLarge::ROWS) * ceil_div(classes, LogitsLarge::COLS);
+    const int64_t middle = ceil_div(rows, LogitsMiddle::ROWS) * ceil_div(classes, LogitsMiddle::COLS), rest = middle % (2 * cu);
+    const double t = (double)(middle / (2 * cu)) + (rest == 0 ? 0.0 : rest <= cu ? 0.6 : 1.0);
+    return ceil_div(large, cu) * (1.57 * slabs + 6.0) <= t * (1.98 * slabs + 3.5);
 }
 
 static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool backward)
@@ -841,18 +877,17 @@ static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool 
     p.split = dtype == VTDGE_F32;
     p.parts = p.split ? 3 : 1;
     const int cu = compute_units();
-    const int64_t large = p.split ? ceil_div(rows, SplitLarge::ROWS) * ceil_div(classes, SplitLarge::COLS)
-                                  : ceil_div(rows, LogitsLarge::ROWS) * ceil_div(classes, LogitsLarge::COLS);
-    p.logits = rows <= 64 && classes >= 64 * cu ? CE_FLAT : large >= cu ? CE_LARGE : CE_SMALL;
-    if (p.split) {
-        if (p.logits == CE_LARGE) use<SplitLarge>(p.lm, p.ln, p.slab_l);
-        else if (p.logits == CE_FLAT) use<SplitFlat>(p.lm, p.ln, p.slab_l);
-        else use<SplitSmall>(p.lm, p.ln, p.slab_l);
-    } else {
-        if (p.logits == CE_LARGE) use<LogitsLarge>(p.lm, p.ln, p.slab_l);
-        else if (p.logits == CE_FLAT) use<LogitsFlat>(p.lm, p.ln, p.slab_l);
-        else use<LogitsSmall>(p.lm, p.ln, p.slab_l);
-    }
+    const int64_t tiles = p.split ? ceil_div(rows, SplitLarge::ROWS) * ceil_div(classes, SplitLarge::COLS)
+                                  : ceil_div(rows, LogitsMiddle::ROWS) * ceil_div(classes, LogitsMiddle::COLS);
+    p.logits = rows <= 64 && classes >= 64 * cu ? CE_FLAT : tiles < cu ? CE_SMALL : p.split || large_logits(rows, classes, p.padded) ? CE_LARGE : CE_MIDDLE;
+    auto shape = [&](auto large, auto middle, auto flat, auto small) {
+        if (p.logits == CE_LARGE) use<decltype(large)>(p.lm, p.ln, p.slab_l);
+        else if (p.logits == CE_MIDDLE) use<decltype(middle)>(p.lm, p.ln, p.slab_l);
+        else if (p.logits == CE_FLAT) use<decltype(flat)>(p.lm, p.ln, p.slab_l);
+        else use<decltype(small)>(p.lm, p.ln, p.slab_l);
+    };
+    if (p.split) shape(SplitLarge{}, SplitLarge{}, SplitFlat{}, SplitSmall{});
+    else shape(LogitsLarge{}, LogitsMiddle{}, LogitsFlat{}, LogitsSmall{});
     p.tm = ceil_div(rows, p.lm), p.tn = ceil_div(classes, p.ln);
     int64_t at = 0;
     p.x_at = take(at, rows * p.padded * 2 * p.parts);
@@ -1027,7 +1062,7 @@ extern "C" int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weigh
     a.tile_max = (float *)(ws + p.max_at), a.tile_sum = (float *)(ws + p.sum_at), a.tile_total = (float *)(ws + p.total_at);
     a.target_z = (float *)(ws + p.z_at);
     if (p.split) VT_STEP(p.logits == CE_LARGE ? go_tiles<SplitLarge>(a, p, st) : p.logits == CE_FLAT ? go_tiles<SplitFlat>(a, p, st) : go_tiles<SplitSmall>(a, p, st));
-    else VT_STEP(p.logits == CE_LARGE ? go_tiles<LogitsLarge>(a, p, st) : p.logits == CE_FLAT ? go_tiles<LogitsFlat>(a, p, st) : go_tiles<LogitsSmall>(a, p, st));
+    else VT_STEP(p.logits == CE_LARGE ? go_tiles<LogitsLarge>(a, p, st) : p.logits == CE_MIDDLE ? go_tiles<LogitsMiddle>(a, p, st) : p.logits == CE_FLAT ? go_tiles<LogitsFlat>(a, p, st) : go_tiles<LogitsSmall>(a, p, st));
     const JoinArgs j{a.tile_max, a.tile_sum, a.tile_total, a.target_z, target, rows, classes, ignore_index, smoothing, (int)p.tn,
                      loss_rows, row_max, row_inv, loss, inv_count};
     // one workgroup is done with some 20000 values before a second launch would have begun (by sizes alone: the same bits for each reduction)
@@ -1091,7 +1126,7 @@ extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const vo
         a.x_copy = copy && v0 == 0 ? (bf16_t *)(ws + p.x_at) : nullptr;
         const int64_t live = a.v1 - a.v0;
         if (p.split) VT_STEP(p.logits == CE_LARGE ? go_d<SplitLarge>(a, p, st) : p.logits == CE_FLAT ? go_d<SplitFlat>(a, p, st) : go_d<SplitSmall>(a, p, st));
-        else VT_STEP(p.logits == CE_LARGE ? go_d<LogitsLarge>(a, p, st) : p.logits == CE_FLAT ? go_d<LogitsFlat>(a, p, st) : go_d<LogitsSmall>(a, p, st));
+        else VT_STEP(p.logits == CE_LARGE ? go_d<LogitsLarge>(a, p, st) : p.logits == CE_MIDDLE ? go_d<LogitsMiddle>(a, p, st) : p.logits == CE_FLAT ? go_d<LogitsFlat>(a, p, st) : go_d<LogitsSmall>(a, p, st));
         GradPair g{};
         g.scale = scale, g.scale2 = inv_count, g.f32 = p.split;
         if (dx != nullptr) {
@@ -1110,7 +1145,7 @@ extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const vo
             g.dw.sums = dbias != nullptr ? (unsigned char *)dbias + v0 * elem : nullptr;
         }
         if (p.split) VT_STEP(p.grads == CE_LARGE ? go_grad<SplitLarge>(g, st) : go_grad<SplitSmall>(g, st));
-        else VT_STEP(p.grads == CE_LARGE ? go_grad<GradLarge>(g, st) : go_grad<GradSmall>(g, st));
+        else VT_STEP(p.grads == CE_LARGE ? go_grad<GradLarge>(g, st) : p.grads == CE_MIDDLE ? go_grad<GradMiddle>(g, st) : go_grad<GradSmall>(g, st));
         // parts of this piece's dW and db, and of dx behind the last piece
         const bool last = a.v1 == classes;
         const SumJob jobs[3] = {{dx_part, last ? dx : nullptr, rows * width, part_of(rows * width), p.dx_splits},
