@@ -635,7 +635,7 @@ int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const void *weight,
                                  int64_t ignore_index, float smoothing, const void *laid_out, void *workspace,
                                  int64_t workspace_bytes, void *dx, void *dweight, void *dbias, int dtype, void *stream);
 
-/* One AdamW step over `count` tensors, in one launch for each 92 of them (64 with 8-bit moments):
+/* One AdamW step over `count` tensors, in one launch for each 134 of them (96 with 8-bit moments):
  *   p *= 1 - lr weight_decay;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
  *   p -= lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
  *   tensors_host  HOST table; param and grad of `dtype`, n elements each, any alignment of their type
