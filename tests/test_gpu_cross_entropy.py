@@ -282,3 +282,123 @@ def test_refusals(dev):
         x = x.requires_grad_()
         dx, = torch.autograd.grad(linear_cross_entropy(x, w, b, t), x, create_graph=True)
         dx.sum().backward()
+
+
+LARGE, MIDDLE, SMALL, SPLIT = "Shape<2, 4, 4, 2, 64, 2, 1>", "Shape<2, 2, 4, 2, 64, 3, 1>", "Shape<1, 1, 2, 2, 64, 6, 1>", "Shape<2, 2, 4, 2, 32, 2, 3>"
+
+
+@pytest.mark.parametrize("dtype,rows,classes,width,logits,grads", [
+    (torch.bfloat16, 4097, 16385, 1032, LARGE, LARGE), (torch.bfloat16, 8193, 4097, 1024, "Shape<2, 4, 2, 2, 32, 3, 1>", LARGE),
+    (torch.bfloat16, 1000, 16640, 260, "Shape<2, 4, 2, 2, 32, 3, 1>", LARGE), (torch.bfloat16, 2049, 16385, 136, "Shape<2, 4, 2, 2, 32, 3, 1>", MIDDLE),
+    (torch.bfloat16, 2000, 2000, 1027, SMALL, MIDDLE), (torch.bfloat16, 1025, 8191, 72, "Shape<2, 4, 2, 2, 32, 3, 1>", SMALL),
+    (torch.bfloat16, 64, 16384, 64, "Shape<1, 2, 2, 2, 64, 3, 1>", SMALL), (torch.float32, 2049, 16385, 136, SPLIT, SPLIT),
+    (torch.float32, 257, 32769, 130, SPLIT, SPLIT), (torch.float32, 64, 16384, 64, "Shape<1, 2, 2, 2, 32, 3, 3>", "Shape<1, 1, 2, 2, 32, 4, 3>")])
+def test_shapes_of_tiles(dev, dtype, rows, classes, width, logits, grads):
+    """Every shape of the product, one row, class or feature around its tiles and slabs, with sums cut and classes in pieces."""
+    from vtpack_amd import _lib, ops
+    x, w, b, t = _operands(dev, rows, classes, width, dtype, left_out=0.1)
+    loss, stats, laid_out = ops.cross_entropy(x, w, b, t)
+    assert any(f"cross_entropy_tiles_kernel<vtdge::{logits}, false>" in _lib.last_kernel(k) for k in range(3))
+    ops.cross_entropy_backward(x, w, b, t, stats, laid_out, torch.ones((), device=dev))
+    used = [_lib.last_kernel(k) for k in range(3)]
+    assert any(f"cross_entropy_grad_kernel<vtdge::{grads} >" in n for n in used) and any(f"cross_entropy_d_kernel<vtdge::{logits} >" in n for n in used)
+    _check(x, w, b, t, smoothing=0.1)
+
+
+@pytest.mark.parametrize("dtype,width", [(torch.float32, 64), (torch.bfloat16, 72), (torch.bfloat16, 128)])
+def test_operands_kept_or_laid_out_again(dev, dtype, width):
+    """What the forward call leaves for the gradients is what they would lay out themselves; and they leave it as it is."""
+    from vtpack_amd import ops
+    x, w, b, t = _operands(dev, 300, 500, width, dtype, left_out=0.2)
+    x[t < 0] = float("nan")
+    one = torch.ones((), device=dev)
+    loss, stats, laid_out = ops.cross_entropy(x, w, b, t)
+    assert (laid_out is not None) == (dtype == torch.float32 or width % 64 != 0)
+    want = ops.cross_entropy_backward(x, w, b, t, stats, None, one)
+    for _ in range(2):
+        got = ops.cross_entropy_backward(x, w, b, t, stats, laid_out, one)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_backward_twice_and_a_weight_used_twice(dev, dtype):
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 130, 200, 96, dtype)
+    x2, _, _, t2 = _operands(dev, 77, 200, 96, dtype, seed=3)
+    one, two = _check(x, w, b, t)[1][1], _check(x2, w, b, t2)[1][1]
+    leaf = w.detach().requires_grad_()
+    loss = linear_cross_entropy(x, leaf, b, t)
+    again = [torch.autograd.grad(loss, leaf, retain_graph=True)[0] for _ in range(2)]
+    assert torch.equal(again[0], one) and torch.equal(again[1], one)
+    (loss + linear_cross_entropy(x2, leaf, b, t2)).backward()
+    assert torch.equal(leaf.grad, one + two)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_captured_training_pass(dev, dtype):
+    """Forward and backward through autograd in one graph, on leaves of its own, replayed over new data beside eager calls."""
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 520, 900, 136, dtype, left_out=0.1)
+    leaves = [v.clone().requires_grad_() for v in (x, w, b)]
+    targets = t.clone()
+
+    def run(leaves, t):
+        loss = linear_cross_entropy(*leaves, t, label_smoothing=0.1)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(leaves, targets)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(leaves, targets)
+    for k in range(4):
+        x, t = x.roll(1, 0), t.roll(1, 0)
+        with torch.no_grad():
+            leaves[0].copy_(x)
+            leaves[1].mul_(0.9)
+        targets.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run([v.detach().clone().requires_grad_() for v in leaves], t)
+        assert all(torch.equal(p, q) for p, q in zip(out, want)), k
+
+
+def test_two_calls_at_once(dev):
+    """Two threads, each on a stream of its own, over calls of several sizes."""
+    import threading
+    from vtpack_amd.layers import linear_cross_entropy
+    sizes = [(300, 500, 96), (1021, 1000, 192), (64, 17000, 64)]
+    data = [[_operands(dev, *s, dtype) for s in sizes] for dtype in DTYPES]
+
+    def run(sets):
+        out = []
+        for x, w, b, t in sets:
+            leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+            loss = linear_cross_entropy(*leaves, t)
+            out += [loss.detach(), *torch.autograd.grad(loss, leaves)]
+        return out
+
+    want = [run(sets) for sets in data]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i] = run(data[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors
+    for p, q in zip(got, want):
+        assert all(torch.equal(a, b) for a, b in zip(p, q))
