@@ -368,3 +368,42 @@ def test_refusals(dev):
     opt.param_groups[0]["lr"] = torch.tensor(1e-3)
     with pytest.raises(ValueError):
         opt.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_that_find_everything_in_place(dev, bits, monkeypatch):
+    """Two groups over several steps: those after the first are one native call each; what has moved in between is found."""
+    from vtpack_amd import optim
+    looked = []
+    take = optim._Batch.take_gradients
+    monkeypatch.setattr(optim._Batch, "take_gradients", lambda self, grads: looked.append(1) or take(self, grads))
+    shapes = [(700,), (3, 50), (1025,), (8,)]
+    params = [torch.nn.Parameter(t) for t in _tensors(dev, shapes, torch.float32, 21)]
+    refs = [_Reference(p, bits) for p in params]
+    opt = _optimizer([{"params": params[:2]}, {"params": params[2:]}], bits)
+    expect = {0: 2, 3: 1, 4: 2, 6: 1, 7: 1}                # groups that are looked over in Python at a step
+    for k in range(9):
+        for p, g in zip(params, _tensors(dev, shapes, torch.float32, 80 + k, 1e-3)):
+            p.grad = g
+        if k == 3:                                         # a moment whose storage is another
+            m = opt.state[params[0]]["exp_avg"]
+            m.data = m.data.clone()
+        if k == 4:                                         # all states replaced by copies
+            opt.load_state_dict(opt.state_dict())
+        if k == 6:                                         # a weight with storage of its own, at another place
+            params[3].data = params[3].data.clone()
+        if k == 7:                                         # a gradient of other strides
+            params[1].grad = params[1].grad.t().contiguous().t()
+        for g in opt.param_groups:
+            g["lr"] = LR * (1 + k % 2)
+        before, versions = len(looked), [p._version for p in params]
+        opt.step()
+        assert len(looked) - before == expect.get(k, 0), k
+        assert all(p._version > v for p, v in zip(params, versions))
+        for p, r in zip(params, refs):
+            r.step(p.grad, LR * (1 + k % 2))
+            r.check(p, opt.state[p])
+    assert all(g["step"] == 9 for g in opt.param_groups)
+    params[0].grad.data = params[0].grad.data[:10]         # a gradient that no longer fits
+    with pytest.raises(ValueError):
+        opt.step()

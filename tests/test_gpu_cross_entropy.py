@@ -402,3 +402,32 @@ def test_two_calls_at_once(dev):
     assert not errors
     for p, q in zip(got, want):
         assert all(torch.equal(a, b) for a, b in zip(p, q))
+
+
+def test_saved_operands(dev):
+    """Operands changed in place before the backward pass are noticed; a checkpointed loss is worked out again."""
+    from torch.utils.checkpoint import checkpoint
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 50, 60, 64, torch.float32)
+    want = _check(x, w, b, t)[1]
+    for change in range(3):
+        operands = [v.clone() for v in (x, w, t)]
+        leaf = b.detach().requires_grad_()
+        loss = linear_cross_entropy(operands[0], operands[1], leaf, operands[2])
+        operands[change].zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+    checkpoint(linear_cross_entropy, *leaves, t, use_reentrant=False).backward()
+    assert all(torch.equal(v.grad, g) for v, g in zip(leaves, want))
+
+
+def test_no_graph_without_gradients(dev):
+    from vtpack_amd.layers import gate_balance, linear_cross_entropy
+    x, w, b, t = _operands(dev, 50, 60, 64, torch.float32)
+    assert not linear_cross_entropy(x, w, b, t).requires_grad
+    with torch.no_grad():
+        assert not linear_cross_entropy(x.requires_grad_(), w, b, t).requires_grad
+        assert not gate_balance(x)[0].requires_grad
+    loss, counts = gate_balance(x)
+    assert loss.requires_grad and not counts.requires_grad

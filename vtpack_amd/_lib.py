@@ -110,6 +110,14 @@ class Chain(ctypes.Structure):
                [(n, ctypes.c_float) for n in ("eps1", "eps2", "sr_eps", "scale")]
 
 
+# bytes of a workspace
+_WORKSPACES = {
+    "vtdge_decompress_router_compress_workspace": [_i, _i, _i, _i],
+    "vtdge_region_step_workspace": [_i, _i, _i],
+    "vtdge_gate_balance_workspace": [_l, _i],
+    "vtdge_cross_entropy_laid_out": [_l, _l, _i, _i],
+    "vtdge_cross_entropy_workspace": [_l, _l, _i, _i, _i],
+}
 EXPORTS = ["vtdge_version", "vtdge_last_error", "vtdge_last_kernel", "vtdge_recent_kernel"] + list(SIGNATURES)
 
 _lib = None
@@ -148,22 +156,35 @@ def load():
     lib.vtdge_last_kernel.argtypes = []
     lib.vtdge_recent_kernel.restype = ctypes.c_char_p
     lib.vtdge_recent_kernel.argtypes = [_i]
-    lib.vtdge_decompress_router_compress_workspace.restype = _l
-    lib.vtdge_decompress_router_compress_workspace.argtypes = [_i, _i, _i, _i]
-    lib.vtdge_region_step_workspace.restype = _l
-    lib.vtdge_region_step_workspace.argtypes = [_i, _i, _i]
-    lib.vtdge_gate_balance_workspace.restype = _l
-    lib.vtdge_gate_balance_workspace.argtypes = [_l, _i]
-    lib.vtdge_cross_entropy_laid_out.restype = _l
-    lib.vtdge_cross_entropy_laid_out.argtypes = [_l, _l, _i, _i]
-    lib.vtdge_cross_entropy_workspace.restype = _l
-    lib.vtdge_cross_entropy_workspace.argtypes = [_l, _l, _i, _i, _i]
+    for name, args in _WORKSPACES.items():
+        fn = getattr(lib, name)
+        fn.restype = _l
+        fn.argtypes = args
     for name, args in SIGNATURES.items():
         fn = getattr(lib, name)
         fn.restype = _i
         fn.argtypes = args
     _lib = lib
     return lib
+
+
+_training = None
+
+
+def training():
+    """The native module of the training operators (csrc/training.cpp), with the addresses of the library's entry points."""
+    global _training
+    if _training is None:
+        lib = load()
+        try:
+            from . import _training as module
+        except ImportError as e:
+            raise ImportError(f"vtpack_amd/_training.so is missing or does not load: {e}. Run `make -C {CSRC}` "
+                              "(or __graft_entry__.build()); this package has no fallback path.") from e
+        names = [n for n in (*SIGNATURES, "vtdge_last_error", *_WORKSPACES)]
+        module.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names}, VtdgeError)
+        _training = module
+    return _training
 
 
 # Optional per-launch timer (benchmarks only): an object with begin(name, tag) / end(); None = off.

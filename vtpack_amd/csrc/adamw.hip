@@ -1,7 +1,7 @@
 // One AdamW step over many tensors (gfx950):  p *= 1 - lr wd;  m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;
 // p -= lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps), moments in fp32 or in 8 bits.
 //
-// Bound by memory: 28 bytes an element in fp32, 22 with bf16 weights, 14 and 8 with 8-bit moments.  The tensors of a launch are a
+// Bound by memory: 28 bytes an element in fp32, 22 with bf16 weights, 16 and 10 with 8-bit moments.  The tensors of a launch are a
 // table in its arguments (no copy to the device, nothing to keep between calls), a workgroup takes a chunk of one of them and finds
 // it by halving.  A wave takes 256 consecutive elements at a time, four a lane: weights, gradients and moments all come in one load
 // a lane, and the 256 are the block that shares a scale, so that its largest magnitude is one reduction over the wave.

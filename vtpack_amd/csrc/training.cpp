@@ -1,0 +1,477 @@
+// The operators of a training step as torch calls them: cross entropy and balance of gates as autograd nodes, the checks of an
+// AdamW step.  Host code only; the kernels are behind the C entry points of vtdge.h, whose addresses `bind` takes.
+//
+// Why this is native: small calls of these operators are bound by the host.  A backward pass runs in the engine's own thread, whose
+// core comes out of its sleep for it, and what Python does there (the interpreter lock, four allocations, 24 arguments) took 32 of
+// the 122 us of a DeiT-S classifier's loss with its gradients; a step over 200 weights looked at some 1000 objects, 77 us beside the
+// 31 us of its kernels.
+#include <Python.h>
+
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <map>
+#include <mutex>
+#include <optional>
+#include <stdexcept>
+#include <string>
+#include <tuple>
+#include <vector>
+
+#include "../../include/vtdge.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+#define VT_FUNCTIONS(X)                                                                                                \
+    X(last_error) X(cross_entropy) X(cross_entropy_backward) X(cross_entropy_workspace) X(cross_entropy_laid_out)      \
+    X(gate_balance) X(gate_balance_backward) X(gate_balance_workspace) X(adamw)
+struct Library {
+#define VT_MEMBER(name) decltype(&vtdge_##name) name = nullptr;
+    VT_FUNCTIONS(VT_MEMBER)
+#undef VT_MEMBER
+};
+Library lib;
+PyObject *error_type = nullptr;                 // vtpack_amd._lib.VtdgeError
+
+struct Failure : std::runtime_error {
+    using std::runtime_error::runtime_error;
+};
+void must(int rc, const char *what)
+{
+    if (rc != VTDGE_OK) throw Failure(std::string(what) + " failed (" + std::to_string(rc) + "): " + lib.last_error());
+}
+
+int code_of(const Tensor &t) { return t.scalar_type() == at::kFloat ? VTDGE_F32 : VTDGE_BF16; }
+// from one row to the next; one row alone has no distance
+int64_t pitch_of(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+void *at_of(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+void *stream_of(const Tensor &t) { return (void *)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+Tensor fresh(const Tensor &like, at::IntArrayRef sizes, at::ScalarType type) { return at::empty(sizes, like.options().dtype(type).requires_grad(false)); }
+
+// A workspace's bytes by the sizes it is for (working them out looks through many cuts of a sum).
+template <size_t N, class F> int64_t bytes_of(const std::array<int64_t, N> &key, F ask)
+{
+    static std::mutex lock;
+    static std::map<std::array<int64_t, N>, int64_t> known;
+    std::lock_guard<std::mutex> hold(lock);
+    const auto it = known.find(key);
+    if (it != known.end()) return it->second;
+    const int64_t bytes = ask();
+    if (bytes < 0) throw Failure(lib.last_error());
+    if (known.size() >= 1024) known.clear();
+    return known[key] = bytes;
+}
+
+// ------------------------------------------------------------------------------------------------ cross entropy
+enum Reduction { NONE, MEAN, SUM };
+constexpr int64_t KEEP_LAID_OUT = 16 << 20;     // bytes
+
+struct Rows {
+    int64_t rows, classes; int width, dtype;
+    Rows(const Tensor &x, const Tensor &w) : rows(x.size(0)), classes(w.size(0)), width((int)x.size(1)), dtype(code_of(x)) {}
+    int64_t workspace(bool backward) const
+    {
+        return bytes_of<5>({rows, classes, width, dtype, backward}, [&] { return lib.cross_entropy_workspace(rows, classes, width, dtype, backward); });
+    }
+    // Operands that do not lie as the kernels read them were laid out in the workspace.  Where that is little beside what a call
+    // takes anyway (another launch), it is kept for the gradients; larger ones are laid out again there.
+    bool keeps() const { return (dtype != VTDGE_BF16 || width % 64 != 0) && lib.cross_entropy_laid_out(rows, classes, width, dtype) <= KEEP_LAID_OUT; }
+};
+
+struct Forward {
+    Tensor loss, stats, laid_out;
+};
+Forward cross_entropy(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &target, int64_t ignore, double smoothing, int reduction)
+{
+    const c10::DeviceGuard guard(x.device());
+    const Rows s(x, w);
+    Tensor ws = fresh(x, {s.workspace(false)}, at::kByte);
+    // the rows' largest logits, 1 / sums, 1 / the number of rows that count, the rows' losses; the loss is memory of its own, for a
+    // caller to change in place
+    const Tensor stats = fresh(x, {3 * s.rows + 1}, at::kFloat);
+    const Tensor loss = reduction == NONE ? fresh(x, {s.rows}, at::kFloat) : fresh(x, {}, at::kFloat);
+    float *const at = stats.data_ptr<float>(), *const out = loss.data_ptr<float>();
+    must(lib.cross_entropy(x.data_ptr(), pitch_of(x), w.data_ptr(), pitch_of(w), at_of(bias), target.data_ptr<int64_t>(), s.rows, s.classes, s.width,
+                           ignore, (float)smoothing, ws.data_ptr(), ws.numel(), reduction == NONE ? out : at + 2 * s.rows + 1, at, at + s.rows,
+                           reduction == NONE ? nullptr : out, reduction == MEAN ? at + 2 * s.rows : nullptr, s.dtype, stream_of(x)),
+         "vtdge_cross_entropy");
+    return {loss, stats, s.keeps() ? ws : Tensor()};
+}
+
+std::array<Tensor, 3> cross_entropy_backward(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &target, const Tensor &stats,
+                                             const Tensor &laid_out, const Tensor &grad, int64_t ignore, double smoothing, int reduction,
+                                             std::array<bool, 3> needs)
+{
+    const c10::DeviceGuard guard(x.device());
+    const Rows s(x, w);
+    const Tensor ws = fresh(x, {s.workspace(true)}, at::kByte);
+    std::array<Tensor, 3> out;
+    if (needs[0]) out[0] = fresh(x, {s.rows, s.width}, x.scalar_type());
+    if (needs[1]) out[1] = fresh(x, {s.classes, s.width}, x.scalar_type());
+    if (needs[2] && bias.defined()) out[2] = fresh(x, {s.classes}, x.scalar_type());
+    const float *const at = stats.data_ptr<float>();
+    must(lib.cross_entropy_backward(x.data_ptr(), pitch_of(x), w.data_ptr(), pitch_of(w), at_of(bias), target.data_ptr<int64_t>(), at, at + s.rows,
+                                    grad.data_ptr<float>(), (int)grad.dim(), reduction == MEAN ? at + 2 * s.rows : nullptr, s.rows, s.classes,
+                                    s.width, ignore, (float)smoothing, at_of(laid_out), ws.data_ptr(), ws.numel(), at_of(out[0]), at_of(out[1]),
+                                    at_of(out[2]), s.dtype, stream_of(x)),
+         "vtdge_cross_entropy_backward");
+    return out;
+}
+
+void no_second_order(const char *name)
+{
+    if (at::GradMode::is_enabled()) throw std::runtime_error(std::string(name) + ": gradients of the gradients are not supported");
+}
+
+struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const std::optional<Tensor> &b, const Tensor &target,
+                          int64_t ignore, double smoothing, int64_t reduction)
+    {
+        const Tensor bias = b.value_or(Tensor());
+        const Forward f = cross_entropy(x, w, bias, target, ignore, smoothing, (int)reduction);
+        ctx->save_for_backward({x, w, bias, target, f.stats, f.laid_out});
+        ctx->saved_data["ignore"] = ignore;
+        ctx->saved_data["smoothing"] = smoothing;
+        ctx->saved_data["reduction"] = reduction;
+        return f.loss;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        no_second_order("linear_cross_entropy");
+        const variable_list t = ctx->get_saved_variables();
+        Tensor grad = grads[0];
+        // the same for every row, as a sum over the losses leaves it: one value
+        if (grad.dim() == 1) grad = grad.stride(0) == 0 ? grad.select(0, 0) : grad.contiguous();
+        const auto out = cross_entropy_backward(t[0], t[1], t[2], t[3], t[4], t[5], grad, ctx->saved_data["ignore"].toInt(),
+                                                ctx->saved_data["smoothing"].toDouble(), (int)ctx->saved_data["reduction"].toInt(),
+                                                {ctx->needs_input_grad(0), ctx->needs_input_grad(1), t[2].defined() && ctx->needs_input_grad(2)});
+        return {out[0], out[1], out[2], Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ balance of gates
+std::array<Tensor, 3> gate_balance(const Tensor &gate, const Tensor &indices, const Tensor &mask, int top_k)
+{
+    const c10::DeviceGuard guard(gate.device());
+    const int64_t tokens = gate.size(0);
+    const int experts = (int)gate.size(1);
+    // share: fp32 [experts + 1], behind the sums of the workgroups
+    const int64_t size = bytes_of<2>({tokens, experts}, [&] { return lib.gate_balance_workspace(tokens, experts); });
+    const Tensor share = fresh(gate, {size / 4 + experts + 1}, at::kFloat), loss = fresh(gate, {}, at::kFloat), counts = fresh(gate, {experts}, at::kLong);
+    float *const at = share.data_ptr<float>();
+    must(lib.gate_balance(gate.data_ptr(), pitch_of(gate), (const int64_t *)at_of(indices), (const unsigned char *)at_of(mask), tokens, experts,
+                          top_k, at, size, loss.data_ptr<float>(), counts.data_ptr<int64_t>(), at + size / 4, code_of(gate), stream_of(gate)),
+         "vtdge_gate_balance");
+    return {loss, counts, share};
+}
+Tensor gate_balance_backward(const Tensor &gate, const Tensor &mask, const Tensor &share, const Tensor &grad)
+{
+    const c10::DeviceGuard guard(gate.device());
+    const int experts = (int)gate.size(1);
+    const Tensor out = fresh(gate, {gate.size(0), experts}, gate.scalar_type());
+    must(lib.gate_balance_backward(gate.data_ptr(), pitch_of(gate), (const unsigned char *)at_of(mask),
+                                   share.data_ptr<float>() + share.numel() - experts - 1, grad.data_ptr<float>(), out.data_ptr(), gate.size(0),
+                                   experts, code_of(gate), stream_of(gate)),
+         "vtdge_gate_balance_backward");
+    return out;
+}
+
+struct GateBalance : torch::autograd::Function<GateBalance> {
+    static variable_list forward(AutogradContext *ctx, const Tensor &gate, const std::optional<Tensor> &indices, const std::optional<Tensor> &mask,
+                                 int64_t top_k)
+    {
+        const auto out = gate_balance(gate, indices.value_or(Tensor()), mask.value_or(Tensor()), (int)top_k);
+        ctx->save_for_backward({gate, mask.value_or(Tensor()), out[2]});
+        ctx->mark_non_differentiable({out[1]});
+        ctx->set_materialize_grads(false);
+        return {out[0], out[1]};
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads)
+    {
+        no_second_order("gate_balance");
+        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+        const variable_list t = ctx->get_saved_variables();
+        return {gate_balance_backward(t[0], t[1], t[2], grads[0]), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ AdamW
+// Weights of one type, device and count of steps, with the table the library reads.  Every step looks again at all that a program can
+// put in another's place: the weights and their storage, their states and the tensors in them, the gradients.
+struct Batch {
+    std::vector<PyObject *> params, states, moments, keys;      // moments: keys.size() of them for each state; all held
+    std::vector<Tensor> kept;                   // no other storage can come to lie where a weight or a moment is
+    std::vector<vtdge_adamw_tensor> table;
+    at::ScalarType type;
+    ~Batch()
+    {
+        for (auto *list : {&params, &states, &moments, &keys})
+            for (PyObject *o : *list) Py_DECREF(o);
+    }
+};
+const char *const BATCH = "vtpack_amd.adamw_batch";
+
+std::vector<PyObject *> held(PyObject *list)
+{
+    std::vector<PyObject *> out;
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); i++) {
+        out.push_back(PyList_GET_ITEM(list, i));
+        Py_INCREF(out.back());
+    }
+    return out;
+}
+bool same(const std::vector<PyObject *> &kept, PyObject *list)
+{
+    if (!PyList_Check(list) || PyList_GET_SIZE(list) != (Py_ssize_t)kept.size()) return false;
+    for (size_t i = 0; i < kept.size(); i++)
+        if (PyList_GET_ITEM(list, i) != kept[i]) return false;
+    return true;
+}
+// Everything as it was, and a gradient for every weight that can be read as it lies; its address into the table then.
+bool ready(Batch &b, PyObject *params, PyObject *state)
+{
+    if (!same(b.params, params)) return false;
+    // states lie in the order of their weights, other groups' between them
+    Py_ssize_t at = 0;
+    PyObject *key, *value;
+    size_t met = 0;
+    while (met < b.params.size() && PyDict_Next(state, &at, &key, &value))
+        if (key == b.params[met] && value != b.states[met++]) return false;
+    if (met < b.params.size()) return false;
+    const size_t of = b.keys.size();
+    for (size_t i = 0; i < b.params.size(); i++) {
+        vtdge_adamw_tensor &row = b.table[i];
+        const void *const lies[4] = {row.exp_avg, row.exp_avg_sq, row.exp_avg_scale, row.exp_avg_sq_scale};
+        for (size_t k = 0; k < of; k++) {
+            PyObject *const m = b.moments[i * of + k];
+            if (PyDict_GetItem(b.states[i], b.keys[k]) != m || THPVariable_Unpack(m).data_ptr() != lies[k]) return false;
+        }
+        const Tensor &p = THPVariable_Unpack(b.params[i]), &g = p.grad();
+        if (p.data_ptr() != row.param || p.numel() != row.n || p.scalar_type() != b.type || !p.is_contiguous() || !g.defined() ||
+            g.layout() != at::kStrided || g.scalar_type() != b.type || g.device() != p.device() || g.sizes() != p.sizes() || !g.is_contiguous())
+            return false;
+        row.grad = g.data_ptr();
+    }
+    return true;
+}
+
+// ------------------------------------------------------------------------------------------------ for Python
+struct NoGil {
+    PyThreadState *state = PyEval_SaveThread();
+    ~NoGil() { PyEval_RestoreThread(state); }
+};
+std::optional<Tensor> given(const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+Tensor tensor(PyObject *o)
+{
+    if (o == Py_None) return Tensor();
+    if (!THPVariable_Check(o)) throw std::runtime_error("expected a tensor or None");
+    return THPVariable_Unpack(o);
+}
+int64_t whole(PyObject *o)
+{
+    const long long v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw python_error();
+    return v;
+}
+double real(PyObject *o)
+{
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1 && PyErr_Occurred()) throw python_error();
+    return v;
+}
+PyObject *wrap(const Tensor &t)
+{
+    if (!t.defined()) Py_RETURN_NONE;
+    return THPVariable_Wrap(t);
+}
+PyObject *tuple(std::initializer_list<Tensor> ts)
+{
+    PyObject *out = PyTuple_New((Py_ssize_t)ts.size());
+    Py_ssize_t i = 0;
+    for (const Tensor &t : ts) PyTuple_SET_ITEM(out, i++, wrap(t));
+    return out;
+}
+
+// f(arguments) with `count` of them, what it throws as a Python exception
+template <class F> PyObject *call(PyObject *const *args, Py_ssize_t given, Py_ssize_t count, F f)
+{
+    HANDLE_TH_ERRORS
+    try {
+        if (given != count) throw std::runtime_error("expected " + std::to_string(count) + " arguments, got " + std::to_string(given));
+        return f();
+    } catch (const Failure &e) {
+        PyErr_SetString(error_type, e.what());
+        return nullptr;
+    }
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t n)
+{
+    return call(args, n, 2, [&]() -> PyObject * {
+#define VT_BIND(name)                                                                    \
+    {                                                                                    \
+        PyObject *const o = PyDict_GetItemString(args[0], "vtdge_" #name);               \
+        if (o == nullptr) throw std::runtime_error("bind: no address of vtdge_" #name);  \
+        lib.name = reinterpret_cast<decltype(lib.name)>((uintptr_t)whole(o));            \
+    }
+        VT_FUNCTIONS(VT_BIND)
+#undef VT_BIND
+        Py_INCREF(args[1]);
+        error_type = args[1];
+        Py_RETURN_NONE;
+    });
+}
+
+PyObject *py_linear_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return call(a, n, 7, [&] {
+        const Tensor x = tensor(a[0]), w = tensor(a[1]), b = tensor(a[2]), t = tensor(a[3]);
+        const int64_t ignore = whole(a[4]), reduction = whole(a[6]);
+        const double smoothing = real(a[5]);
+        Tensor loss;
+        {
+            const NoGil no;
+            loss = LinearCrossEntropy::apply(x, w, given(b), t, ignore, smoothing, reduction);
+        }
+        return wrap(loss);
+    });
+}
+PyObject *py_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return call(a, n, 7, [&] {
+        const Tensor x = tensor(a[0]), w = tensor(a[1]), b = tensor(a[2]), t = tensor(a[3]);
+        const int64_t ignore = whole(a[4]), reduction = whole(a[6]);
+        const double smoothing = real(a[5]);
+        Forward f;
+        {
+            const NoGil no;
+            f = cross_entropy(x, w, b, t, ignore, smoothing, (int)reduction);
+        }
+        return tuple({f.loss, f.stats, f.laid_out});
+    });
+}
+PyObject *py_cross_entropy_backward(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return call(a, n, 13, [&] {
+        Tensor t[7];
+        for (int i = 0; i < 7; i++) t[i] = tensor(a[i]);
+        const int64_t ignore = whole(a[7]), reduction = whole(a[9]);
+        const double smoothing = real(a[8]);
+        const std::array<bool, 3> needs = {whole(a[10]) != 0, whole(a[11]) != 0, whole(a[12]) != 0};
+        std::array<Tensor, 3> out;
+        {
+            const NoGil no;
+            out = cross_entropy_backward(t[0], t[1], t[2], t[3], t[4], t[5], t[6], ignore, smoothing, (int)reduction, needs);
+        }
+        return tuple({out[0], out[1], out[2]});
+    });
+}
+PyObject *py_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return call(a, n, 4, [&] {
+        const Tensor gate = tensor(a[0]), indices = tensor(a[1]), mask = tensor(a[2]);
+        const int64_t top_k = whole(a[3]);
+        variable_list out;
+        {
+            const NoGil no;
+            out = GateBalance::apply(gate, given(indices), given(mask), top_k);
+        }
+        return tuple({out[0], out[1]});
+    });
+}
+PyObject *py_gate_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return call(a, n, 4, [&] {
+        const Tensor gate = tensor(a[0]), indices = tensor(a[1]), mask = tensor(a[2]);
+        const int64_t top_k = whole(a[3]);
+        std::array<Tensor, 3> out;
+        {
+            const NoGil no;
+            out = gate_balance(gate, indices, mask, (int)top_k);
+        }
+        return tuple({out[0], out[1], out[2]});
+    });
+}
+PyObject *py_gate_balance_backward(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return call(a, n, 4, [&] {
+        const Tensor gate = tensor(a[0]), mask = tensor(a[1]), share = tensor(a[2]), grad = tensor(a[3]);
+        Tensor out;
+        {
+            const NoGil no;
+            out = gate_balance_backward(gate, mask, share, grad);
+        }
+        return wrap(out);
+    });
+}
+
+// (params, states, keys): lists of weights, of their states and of the names of the moments in them, scales behind
+PyObject *py_adamw_batch(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return call(a, n, 3, [&] {
+        auto b = std::make_unique<Batch>();
+        b->params = held(a[0]), b->states = held(a[1]), b->keys = held(a[2]);
+        if (b->params.empty() || b->states.size() != b->params.size() || b->keys.size() > 4) throw std::runtime_error("adamw_batch: lists that do not match");
+        for (size_t i = 0; i < b->params.size(); i++) {
+            const Tensor p = tensor(b->params[i]);
+            vtdge_adamw_tensor x{};
+            void *at[4] = {};
+            for (size_t k = 0; k < b->keys.size(); k++) {
+                PyObject *const m = PyDict_GetItem(b->states[i], b->keys[k]);
+                if (m == nullptr || !THPVariable_Check(m)) throw std::runtime_error("adamw_batch: a state without its moments");
+                Py_INCREF(m);
+                b->moments.push_back(m);
+                b->kept.push_back(tensor(m).detach());
+                at[k] = b->kept.back().data_ptr();
+            }
+            b->kept.push_back(p.detach());
+            b->type = p.scalar_type();
+            x.param = p.data_ptr(), x.n = p.numel();
+            x.exp_avg = at[0], x.exp_avg_sq = at[1], x.exp_avg_scale = (float *)at[2], x.exp_avg_sq_scale = (float *)at[3];
+            b->table.push_back(x);
+        }
+        return PyCapsule_New(b.release(), BATCH, [](PyObject *o) { delete static_cast<Batch *>(PyCapsule_GetPointer(o, BATCH)); });
+    });
+}
+// (batch, the group's weights, the optimizer's states, lr, beta1, beta2, eps, decay, step, bits): whether the step was made; if
+// not, something is not as it was and nothing was done
+PyObject *py_adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return call(a, n, 10, [&]() -> PyObject * {
+        Batch *const b = static_cast<Batch *>(PyCapsule_GetPointer(a[0], BATCH));
+        if (b == nullptr) throw python_error();
+        double rate[5];
+        for (int i = 0; i < 5; i++) rate[i] = real(a[3 + i]);
+        const int64_t step = whole(a[8]), bits = whole(a[9]);
+        if (!PyDict_Check(a[2]) || !ready(*b, a[1], a[2])) Py_RETURN_FALSE;
+        const Tensor &first = THPVariable_Unpack(b->params[0]);
+        const c10::DeviceGuard guard(first.device());
+        {
+            const NoGil no;
+            must(lib.adamw(b->table.data(), (int)b->table.size(), rate[0], rate[1], rate[2], rate[3], rate[4], step, nullptr, code_of(first),
+                           (int)bits, stream_of(first)),
+                 "vtdge_adamw");
+        }
+        for (PyObject *p : b->params) THPVariable_Unpack(p).unsafeGetTensorImpl()->bump_version();
+        Py_RETURN_TRUE;
+    });
+}
+
+#define VT_METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {VT_METHOD(bind), VT_METHOD(linear_cross_entropy), VT_METHOD(cross_entropy), VT_METHOD(cross_entropy_backward),
+                         VT_METHOD(balance), VT_METHOD(gate_balance), VT_METHOD(gate_balance_backward), VT_METHOD(adamw_batch),
+                         VT_METHOD(adamw_step), {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_training", "The operators of a training step as torch calls them.", -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__training() { return PyModule_Create(&module); }

@@ -1,35 +1,8 @@
 """The losses of a training step behind the encoder: the classifier's cross entropy (the reference trains with timm's, main.py:346-352,
 on the logits of `model.head`) and the balance of the routers' gates, which stands beside the budget loss of the harness."""
 import torch
-from torch.autograd import Function
 
-from .. import ops
-
-
-def _no_second_order(name):
-    """A gradient that is itself being differentiated, as `create_graph=True` asks for."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{name}: gradients of the gradients are not supported")
-
-
-class _LinearCrossEntropy(Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, target, ignore_index, label_smoothing, reduction):
-        loss, stats, ctx.laid_out = ops.cross_entropy(x, weight, bias, target, ignore_index, label_smoothing, reduction)
-        ctx.how = (ignore_index, label_smoothing, reduction)
-        ctx.save_for_backward(x, weight, bias, target, stats)
-        return loss
-
-    @staticmethod
-    def backward(ctx, grad):
-        _no_second_order("linear_cross_entropy")
-        x, weight, bias, target, stats = ctx.saved_tensors
-        if grad.dim() == 1:
-            # the same for every row, as a sum over the losses leaves it: one value
-            grad = grad[0] if grad.stride(0) == 0 else grad.contiguous()
-        dx, dw, db = ops.cross_entropy_backward(ops._rows_of(x), ops._rows_of(weight), bias, target, stats, ctx.laid_out, grad, *ctx.how,
-                                                needs=ctx.needs_input_grad)
-        return dx, dw, db, None, None, None, None
+from .. import _lib, ops
 
 
 def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
@@ -61,27 +34,9 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     if x.numel() == 0:                           # no row: a loss of 0 that still belongs to its operands
         zero = (x.sum() + weight[:0].sum() + (0 if bias is None else bias[:0].sum())).float()
         return zero if reduction != "none" else zero.expand(target.shape)
-    loss = _LinearCrossEntropy.apply(ops._rows_of(x), ops._rows_of(weight), None if bias is None else bias.contiguous(),
-                                     target.reshape(-1).contiguous(), int(ignore_index), float(label_smoothing), reduction)
+    loss = _lib.training().linear_cross_entropy(ops._rows_of(x), ops._rows_of(weight), None if bias is None else bias.contiguous(),
+                                                target.reshape(-1).contiguous(), ignore_index, label_smoothing, ops.REDUCTIONS[reduction])
     return loss.view(target.shape) if reduction == "none" and target.dim() != 1 else loss
-
-
-class _GateBalance(Function):
-    @staticmethod
-    def forward(ctx, gate, indices, mask, top_k):
-        loss, counts, share = ops.gate_balance(gate, indices, mask, top_k)
-        ctx.save_for_backward(gate, mask, share)
-        ctx.mark_non_differentiable(counts)
-        ctx.set_materialize_grads(False)
-        return loss, counts
-
-    @staticmethod
-    def backward(ctx, grad, _):
-        _no_second_order("gate_balance")
-        if grad is None:
-            return None, None, None, None
-        gate, mask, share = ctx.saved_tensors
-        return ops.gate_balance_backward(ops._rows_of(gate), mask, share, grad), None, None, None
 
 
 def gate_balance(gate, indices=None, top_k=1, mask=None):
@@ -117,4 +72,4 @@ def gate_balance(gate, indices=None, top_k=1, mask=None):
         mask = mask.reshape(-1).contiguous()
     if gate.numel() == 0:
         return gate.sum().float(), torch.zeros((E,), dtype=torch.int64, device=gate.device)
-    return _GateBalance.apply(ops._rows_of(gate), indices, mask, int(top_k))
+    return _lib.training().balance(ops._rows_of(gate), indices, mask, top_k)

@@ -1105,92 +1105,30 @@ def _rows_of(t):
     return t if t.is_contiguous() or t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
 
 
-def _pitch(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-@functools.lru_cache(maxsize=1024)
-def _cross_entropy_workspace(rows, classes, width, dtype, backward):
-    size = _lib.load().vtdge_cross_entropy_workspace(rows, classes, width, dtype, backward)
-    if size < 0:
-        raise _lib.VtdgeError(_lib.load().vtdge_last_error().decode("utf-8", "replace"))
-    return size
-
-
-KEEP_LAID_OUT = 16 << 20           # bytes
-
-
-@functools.lru_cache(maxsize=1024)
-def _cross_entropy_laid_out(rows, classes, width, dtype):
-    return _lib.load().vtdge_cross_entropy_laid_out(rows, classes, width, dtype)
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
 def cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
     """Softmax cross entropy of x [rows, width] @ weight [classes, width]^T + bias against int64 target [rows] (rows > 0, rows of
     x and weight dense): -> (fp32 loss, stats and laid_out for `cross_entropy_backward`).  The loss is the rows' mean or sum, or
     each row's own ("none")."""
-    (rows, width), classes, dtype, device = x.shape, weight.shape[0], dtype_code(x), x.device
-    with _on(x):
-        ws = torch.empty((_cross_entropy_workspace(rows, classes, width, dtype, 0),), dtype=torch.uint8, device=device)
-        # stats: the rows' largest logits, 1 / sums, 1 / the number of rows that count, the rows' losses; the loss is memory of its
-        # own, for a caller to change in place
-        stats = torch.empty((3 * rows + 1,), dtype=torch.float32, device=device)
-        loss = torch.empty((rows,) if reduction == "none" else (), dtype=torch.float32, device=device)
-        at, out = stats.data_ptr(), loss.data_ptr()
-        call("vtdge_cross_entropy", x.data_ptr(), _pitch(x), weight.data_ptr(), _pitch(weight), ptr(bias), target.data_ptr(), rows,
-             classes, width, ignore_index, label_smoothing, ws.data_ptr(), ws.numel(),
-             out if reduction == "none" else at + 8 * rows + 4, at, at + 4 * rows, 0 if reduction == "none" else out,
-             at + 8 * rows if reduction == "mean" else 0, dtype, stream_ptr(), tag=("cross_entropy", rows, classes, width))
-    # Operands that do not lie as the kernels read them were laid out in the workspace.  Where that is little beside what a call
-    # takes anyway (another launch), it is kept for the gradients; larger ones are laid out again there.
-    kept = (dtype != _lib.BF16 or width % 64 != 0) and _cross_entropy_laid_out(rows, classes, width, dtype) <= KEEP_LAID_OUT
-    return loss, stats, ws if kept else None
+    return _lib.training().cross_entropy(x, weight, bias, target, ignore_index, label_smoothing, REDUCTIONS[reduction])
 
 
 def cross_entropy_backward(x, weight, bias, target, stats, laid_out, grad, ignore_index=-100, label_smoothing=0.0, reduction="mean",
                            needs=(True, True, True)):
     """Gradients (dx, dweight, dbias; None where not needed) of `cross_entropy` for the fp32 gradient of its loss: a scalar, with
     "none" also one value for each row."""
-    (rows, width), classes, dtype, device = x.shape, weight.shape[0], dtype_code(x), x.device
-    with _on(x):
-        ws = torch.empty((_cross_entropy_workspace(rows, classes, width, dtype, 1),), dtype=torch.uint8, device=device)
-        dx = torch.empty((rows, width), dtype=x.dtype, device=device) if needs[0] else None
-        dw = torch.empty((classes, width), dtype=x.dtype, device=device) if needs[1] else None
-        db = torch.empty((classes,), dtype=x.dtype, device=device) if needs[2] and bias is not None else None
-        at = stats.data_ptr()
-        call("vtdge_cross_entropy_backward", x.data_ptr(), _pitch(x), weight.data_ptr(), _pitch(weight), ptr(bias), target.data_ptr(),
-             at, at + 4 * rows, grad.data_ptr(), grad.dim(), at + 8 * rows if reduction == "mean" else 0, rows, classes, width,
-             ignore_index, label_smoothing, ptr(laid_out), ws.data_ptr(), ws.numel(), ptr(dx), ptr(dw), ptr(db), dtype, stream_ptr(),
-             tag=("cross_entropy_backward", rows, classes, width))
-    return dx, dw, db
-
-
-@functools.lru_cache(maxsize=1024)
-def _gate_balance_workspace(tokens, E):
-    return _lib.load().vtdge_gate_balance_workspace(tokens, E)
+    return _lib.training().cross_entropy_backward(x, weight, bias, target, stats, laid_out, grad, ignore_index, label_smoothing,
+                                                  REDUCTIONS[reduction], *needs[:3])
 
 
 def gate_balance(gate, indices, mask, top_k):
     """gate [tokens, E] with dense rows, tokens > 0; indices int64 [tokens, k] or None; mask [tokens] of bytes or None
     -> (loss, counts int64 [E], share for `gate_balance_backward`)."""
-    (tokens, E), device = gate.shape, gate.device
-    with _on(gate):
-        # share: fp32 [E + 1], behind the sums of the workgroups
-        size = _gate_balance_workspace(tokens, E)
-        share = torch.empty((size // 4 + E + 1,), dtype=torch.float32, device=device)
-        loss = torch.empty((), dtype=torch.float32, device=device)
-        counts = torch.empty((E,), dtype=torch.int64, device=device)
-        at = share.data_ptr()
-        call("vtdge_gate_balance", gate.data_ptr(), _pitch(gate), ptr(indices), ptr(mask), tokens, E, top_k, at, size,
-             loss.data_ptr(), counts.data_ptr(), at + size, dtype_code(gate), stream_ptr(), tag=("gate_balance", tokens, E))
-    return loss, counts, share
+    return _lib.training().gate_balance(gate, indices, mask, top_k)
 
 
 def gate_balance_backward(gate, mask, share, grad):
     """The gradient of `gate_balance`'s gate, dense, for the fp32 gradient of its loss."""
-    tokens, E = gate.shape
-    with _on(gate):
-        out = torch.empty((tokens, E), dtype=gate.dtype, device=gate.device)
-        call("vtdge_gate_balance_backward", gate.data_ptr(), _pitch(gate), ptr(mask),
-             share.data_ptr() + 4 * (share.numel() - E - 1), grad.data_ptr(), out.data_ptr(), tokens, E, dtype_code(gate), stream_ptr(), tag=("gate_balance_backward", tokens, E))
-    return out
+    return _lib.training().gate_balance_backward(gate, mask, share, grad)

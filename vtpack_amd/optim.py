@@ -30,20 +30,20 @@ class _Batch:
     def __init__(self, params, states, bits, skipped):
         self.params, self.states, self.skipped, self.keys = params, states, skipped, _KEYS[bits]
         self.moments = [[s[k] for s in states] for k in self.keys]
-        self.kept = [p.detach() for p in params]            # no other storage can come to lie where one of these is
-        self.at = [p.data_ptr() for p in params]
+        self.kept = [t.detach() for t in itertools.chain(params, *self.moments)]      # no other storage can come to lie where one of these is
+        self.at = [t.data_ptr() for t in self.kept]
         self.bytes = [p.nbytes for p in params]                # of a gradient
         self.plain = all(p.is_contiguous() for p in params)
         self.table = np.zeros((len(params), 7), dtype=np.uint64)
-        self.table[:, 0] = self.at
+        self.table[:, 0] = self.at[:len(params)]
         for column, moment in enumerate(self.moments):
             self.table[:, 2 + column] = [t.data_ptr() for t in moment]
         self.table[:, 6] = [p.numel() for p in params]
+        self.native = _lib.training().adamw_batch(params, states, list(self.keys)) if self.plain else None
 
     def holds(self):
-        return (list(map(_ptr, self.params)) == self.at
-                and all(all(map(operator.is_, map(operator.itemgetter(k), self.states), old))
-                        for k, old in zip(self.keys, self.moments)))
+        return (all(all(map(operator.is_, map(operator.itemgetter(k), self.states), old)) for k, old in zip(self.keys, self.moments))
+                and list(map(_ptr, itertools.chain(self.params, *self.moments))) == self.at)
 
     def take_gradients(self, grads):
         if not self.plain or not all(map(_dense, grads)) or list(map(_nbytes, grads)) != self.bytes:
@@ -179,6 +179,8 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         for index, group in enumerate(self.param_groups):
+            if not capturing and self._same_again(index, group):
+                continue
             params = group["params"]
             grads = list(map(_grad, params))
             if capturing and not group["capturable"]:
@@ -197,6 +199,20 @@ class AdamW(torch.optim.Optimizer):
                 group["step"] += 1
             increment_version(params)
         return loss
+
+    def _same_again(self, index, group):
+        """The step of a group of which nothing has moved since its last one, in one call that looks it all over and launches."""
+        kept = self._batches.get(index)
+        if kept is None or len(kept[2]) != 1 or group["capturable"] or _lib.timer is not None:
+            return False
+        b, (beta1, beta2) = kept[2][0], group["betas"]
+        if b.native is None or b.keys != _KEYS[group["state_bits"]]:
+            return False
+        if not _lib.training().adamw_step(b.native, group["params"], self.state, group["lr"], beta1, beta2, group["eps"], group["weight_decay"],
+                                          int(group["step"]) + 1 - b.skipped, group["state_bits"]):
+            return False
+        group["step"] += 1
+        return True
 
     def _skip(self, index, params, capturing):
         """Weights without a gradient miss this step."""
