@@ -331,12 +331,33 @@ PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t n)
     });
 }
 
+// Operands as the kernels take them.  The entry points below answer None to any other, for their callers to bring them into this
+// form or to say what is wrong with them.
+bool number(PyObject *o) { return PyLong_Check(o) || PyFloat_Check(o); }
+bool plain_rows(const Tensor &t)
+{
+    return t.defined() && t.is_cuda() && t.dim() == 2 && t.numel() > 0 && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) &&
+           t.layout() == at::kStrided && (t.is_contiguous() || (t.stride(1) == 1 && t.stride(0) >= t.size(1)));
+}
+bool plain_beside(const Tensor &t, const Tensor &x, at::ScalarType type)
+{
+    return t.defined() && t.device() == x.device() && t.scalar_type() == type && t.layout() == at::kStrided && t.is_contiguous();
+}
+
+// (x, weight, bias or None, target, ignore_index, label_smoothing, reduction's code)
 PyObject *py_linear_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
-    return call(a, n, 7, [&] {
+    return call(a, n, 7, [&]() -> PyObject * {
+        for (int i = 0; i < 4; i++)
+            if (!THPVariable_Check(a[i]) && !(i == 2 && a[i] == Py_None)) Py_RETURN_NONE;
+        if (!PyLong_Check(a[4]) || !number(a[5]) || !PyLong_Check(a[6])) Py_RETURN_NONE;
         const Tensor x = tensor(a[0]), w = tensor(a[1]), b = tensor(a[2]), t = tensor(a[3]);
         const int64_t ignore = whole(a[4]), reduction = whole(a[6]);
         const double smoothing = real(a[5]);
+        if (!plain_rows(x) || !plain_rows(w) || w.device() != x.device() || w.scalar_type() != x.scalar_type() || w.size(1) != x.size(1) ||
+            !plain_beside(t, x, at::kLong) || t.dim() != 1 || t.size(0) != x.size(0) ||
+            (b.defined() && (!plain_beside(b, x, x.scalar_type()) || b.dim() != 1 || b.size(0) != w.size(0))) || !(smoothing >= 0 && smoothing <= 1))
+            Py_RETURN_NONE;
         Tensor loss;
         {
             const NoGil no;
@@ -375,11 +396,19 @@ PyObject *py_cross_entropy_backward(PyObject *, PyObject *const *a, Py_ssize_t n
         return tuple({out[0], out[1], out[2]});
     });
 }
+// (gate, indices [tokens, k] or None, mask or None, top_k)
 PyObject *py_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
-    return call(a, n, 4, [&] {
+    return call(a, n, 4, [&]() -> PyObject * {
+        for (int i = 0; i < 3; i++)
+            if (!THPVariable_Check(a[i]) && !(i > 0 && a[i] == Py_None)) Py_RETURN_NONE;
+        if (!PyLong_Check(a[3])) Py_RETURN_NONE;
         const Tensor gate = tensor(a[0]), indices = tensor(a[1]), mask = tensor(a[2]);
         const int64_t top_k = whole(a[3]);
+        if (!plain_rows(gate) || gate.size(1) > 512 || top_k < 1 || top_k > 512 || (!indices.defined() && top_k > gate.size(1)) ||
+            (indices.defined() && (!plain_beside(indices, gate, at::kLong) || indices.dim() != 2 || indices.size(0) != gate.size(0) || indices.size(1) != top_k)) ||
+            (mask.defined() && (!plain_beside(mask, gate, at::kBool) || mask.dim() != 1 || mask.size(0) != gate.size(0))))
+            Py_RETURN_NONE;
         variable_list out;
         {
             const NoGil no;

@@ -16,6 +16,11 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     The logits are fp32 sums and are not rounded; in bfloat16 the gradients of the logits are, once, before the products that
     take them to x, weight and bias.  They work in pieces of the classes with some 320 MB of scratch for a piece; float32
     operands are laid out anew in three parts of two bytes for the time of a call."""
+    how = (ignore_index, label_smoothing, ops.REDUCTIONS.get(reduction))
+    loss = _lib.training().linear_cross_entropy(x, weight, bias, target, *how)
+    if loss is not None:
+        return loss
+    # operands that are not the kernels' rows and vectors yet, or none that they can become
     ops._need_gpu(x, weight, bias, target)
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction is {reduction!r}, expected 'mean', 'sum' or 'none'")
@@ -35,7 +40,7 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
         zero = (x.sum() + weight[:0].sum() + (0 if bias is None else bias[:0].sum())).float()
         return zero if reduction != "none" else zero.expand(target.shape)
     loss = _lib.training().linear_cross_entropy(ops._rows_of(x), ops._rows_of(weight), None if bias is None else bias.contiguous(),
-                                                target.reshape(-1).contiguous(), ignore_index, label_smoothing, ops.REDUCTIONS[reduction])
+                                                target.reshape(-1).contiguous(), int(ignore_index), float(label_smoothing), how[2])
     return loss.view(target.shape) if reduction == "none" and target.dim() != 1 else loss
 
 
@@ -47,6 +52,9 @@ def gate_balance(gate, indices=None, top_k=1, mask=None):
     even, E is all on one.  The choices are the `top_k` largest logits of a token (among equals the lowest index), or `indices`
     int64 [..., k] (or of gate's leading shape, k = 1) if they were made elsewhere, as by a Gumbel sample.  `mask` (bool, gate's leading shape): False leaves a token
     out, whatever its logits are; a token whose logits are all -inf is left out too.  Without a token the loss is 0."""
+    out = _lib.training().balance(gate, indices, mask, top_k) if indices is None else None
+    if out is not None:
+        return out
     ops._need_gpu(gate, indices, mask)
     if gate.dim() < 1 or not 1 <= gate.shape[-1] <= 512:
         raise ValueError(f"gate has shape {tuple(gate.shape)}, expected 1 .. 512 logits a token")
@@ -72,4 +80,4 @@ def gate_balance(gate, indices=None, top_k=1, mask=None):
         mask = mask.reshape(-1).contiguous()
     if gate.numel() == 0:
         return gate.sum().float(), torch.zeros((E,), dtype=torch.int64, device=gate.device)
-    return _lib.training().balance(ops._rows_of(gate), indices, mask, top_k)
+    return _lib.training().balance(ops._rows_of(gate), indices, mask, int(top_k))
