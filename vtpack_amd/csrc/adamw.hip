@@ -4,10 +4,10 @@
 // Bound by memory: 28 bytes an element in fp32, 22 with bf16 weights, 16 and 10 with 8-bit moments.  The tensors of a launch are a
 // table in its arguments (no copy to the device, nothing to keep between calls), a workgroup takes a chunk of one of them and finds
 // it by halving.  A wave takes 256 consecutive elements at a time, four a lane: weights, gradients and moments all come in one load
-// a lane, and the 256 are the block that shares a scale, so that its largest magnitude is one reduction over the wave.
-// Measured: 106 M bf16 weights with 32-bit moments 444 us, 5.3 TB/s; the 5.7 M and 22 M fp32 weights of a vision transformer in 200
-// tensors 31 us with 32-bit moments (5.2 TB/s) and 76 us with 8-bit ones (4.1 TB/s; 87 us with IEEE roots and quotients: there the
-// arithmetic of the codes shows).
+// a lane, and the 256 are the block that shares a scale, so that its largest magnitude is one reduction over the wave.  Waves take one
+// block each: while some wait others compute, with no loop to keep in order (four blocks a wave 10 to 20 percent slower).
+// Measured, on weights that are in no cache: 103 M bf16 weights with 32-bit moments 403 us, 5.6 TB/s; the 5.7 M and 22 M fp32 weights of
+// a vision transformer in 200 tensors 32 us with 32-bit moments (5.0 TB/s) and 75 us with 8-bit ones (4.7 TB/s).
 //
 // Moments in 8 bits: the first as e4m3 over max|m| / 448, the second as e5m2 over max v / 57344.  Adam's slow decay (b2 = 0.999)
 // is far below half a step of either (1/16 and 1/8), and would be lost under rounding to the nearest; a value is therefore rounded
@@ -23,8 +23,8 @@
 namespace vtdge {
 
 constexpr int OPT_BLOCK = 256;                  // elements of a scale, and of a wave
-constexpr int OPT_CHUNK = 4096;                 // elements of a workgroup
 constexpr int OPT_WAVES = 4;
+constexpr int OPT_CHUNK = OPT_WAVES * OPT_BLOCK;        // elements of a workgroup: a block for each wave
 constexpr int64_t OPT_MOST_CHUNKS = (1 << 24) - 1;      // of a launch: fewer than 2^32 threads
 
 struct OptScalars {                             // of one step, in fp32; also what vtdge_adamw_scalars leaves on the device
@@ -203,75 +203,90 @@ __device__ __forceinline__ float change(float m, float v, float root, float eps)
     return m * __builtin_amdgcn_rcpf((small ? r * 0x1p-16f : r) * root + eps);
 }
 
+// A lane's four elements of a block of 256 with 8-bit moments; `live` of them are the tensor's.
+template <typename T> struct Lane {
+    float p[4], g[4], sm, sv;
+    uint32_t cm, cv;
+
+    __device__ __forceinline__ Lane(const T *from, const T *grad, const uint8_t *m, const uint8_t *v, float m_scale, float v_scale, int live, bool whole)
+        : sm(m_scale), sv(v_scale)
+    {
+        load4(from, live, whole, p);
+        load4(grad, live, whole, g);
+        cm = load_codes(m, live, whole), cv = load_codes(v, live, whole);
+    }
+    __device__ __forceinline__ void step(const OptScalars &s, T *to, uint8_t *m, uint8_t *v, float *ms, float *vs, int64_t place, int live, bool whole)
+    {
+#pragma clang fp contract(off)
+        float fm[4], fv[4];
+        decode4<true>(cm, sm, fm);
+        decode4<false>(cv, sv, fv);
+        uint32_t noise[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            fm[e] = fm[e] * s.beta1 + g[e] * s.rest1;
+            fv[e] = fv[e] * s.beta2 + g[e] * s.rest2 * g[e];
+            if (e >= live) fm[e] = fv[e] = 0.f;                // (0 times a scale that is not finite)
+            p[e] = p[e] * s.decay - s.size * change(fm[e], fv[e], s.root, s.eps);
+            noise[e] = dither((uint32_t)(place + e), s.step);
+        }
+        const uint32_t em = encode4<true>(fm, noise, sm), ev = encode4<false>(fv, noise, sv);
+        store4(to, live, whole, p);
+        store_codes(m, live, whole, em);
+        store_codes(v, live, whole, ev);
+        if ((threadIdx.x & 63) == 0) *ms = sm, *vs = sv;
+    }
+};
+
 template <typename T, int BITS>
 __global__ __launch_bounds__(64 * OPT_WAVES) void adamw_kernel(OptTable<BITS> t, OptScalars host, const OptScalars *__restrict__ device)
 {
 #pragma clang fp contract(off)
     const OptScalars s = device != nullptr ? *device : host;
     // the tensor of this chunk: the last one that starts at or before it
-    uint32_t at = 0, end = t.count;
-    while (end - at > 1) {
-        const uint32_t mid = (at + end) >> 1;
-        if (t.first[mid] <= blockIdx.x) at = mid;
+    uint32_t n = 0, end = t.count;
+    while (end - n > 1) {
+        const uint32_t mid = (n + end) >> 1;
+        if (t.first[mid] <= blockIdx.x) n = mid;
         else end = mid;
     }
-    const uint32_t chunk = blockIdx.x - t.first[at];
-    const bool is_last = blockIdx.x + 1 == (at + 1 < t.count ? t.first[at + 1] : t.chunks);
-    const int live = is_last ? (int)(t.last[at >> 1] >> (at & 1) * 16 & 0xffffu) : OPT_CHUNK;
+    const uint32_t chunk = blockIdx.x - t.first[n];
+    const bool is_last = blockIdx.x + 1 == (n + 1 < t.count ? t.first[n + 1] : t.chunks);
+    const int live = is_last ? (int)(t.last[n >> 1] >> (n & 1) * 16 & 0xffffu) : OPT_CHUNK;
     const int64_t base = (int64_t)chunk * OPT_CHUNK;
-    T *const p = t.template get<T>(0, at) + base;
-    const T *const g = t.template get<const T>(1, at) + base;
+    T *const p = t.template get<T>(0, n);
+    const T *const g = t.template get<const T>(1, n);
     const uint64_t places = (uint64_t)(uintptr_t)p | (uint64_t)(uintptr_t)g;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int block = __builtin_amdgcn_readfirstlane(wave), left = live - block * OPT_BLOCK, at = lane * 4;
+    if (left <= 0) return;
+    const int64_t i = base + block * OPT_BLOCK + at;
     if constexpr (BITS == 32) {
-        float *const m = t.template get<float>(2, at) + base, *const v = t.template get<float>(3, at) + base;
-        const bool vec = (places % (4 * sizeof(T))) == 0 && (((uintptr_t)m | (uintptr_t)v) & 15) == 0;
-        for (int i = wave * OPT_BLOCK + lane * 4; i < live; i += OPT_WAVES * OPT_BLOCK) {
-            const bool whole = vec && i + 4 <= live;
-            float fp[4], fg[4], fm[4], fv[4];
-            load4(p + i, live - i, whole, fp);
-            load4(g + i, live - i, whole, fg);
-            load4(m + i, live - i, whole, fm);
-            load4(v + i, live - i, whole, fv);
+        float *const m = t.template get<float>(2, n) + i, *const v = t.template get<float>(3, n) + i;
+        const bool whole = (places % (4 * sizeof(T))) == 0 && (((uintptr_t)m | (uintptr_t)v) & 15) == 0 && at + 4 <= left;
+        float fp[4], fg[4], fm[4], fv[4];
+        load4(p + i, left - at, whole, fp);
+        load4(g + i, left - at, whole, fg);
+        load4(m, left - at, whole, fm);
+        load4(v, left - at, whole, fv);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                fm[e] = fm[e] * s.beta1 + fg[e] * s.rest1;
-                fv[e] = fv[e] * s.beta2 + fg[e] * s.rest2 * fg[e];
-                fp[e] = fp[e] * s.decay - s.size * change(fm[e], fv[e], s.root, s.eps);
-            }
-            store4(p + i, live - i, whole, fp);
-            store4(m + i, live - i, whole, fm);
-            store4(v + i, live - i, whole, fv);
+        for (int e = 0; e < 4; e++) {
+            fm[e] = fm[e] * s.beta1 + fg[e] * s.rest1;
+            fv[e] = fv[e] * s.beta2 + fg[e] * s.rest2 * fg[e];
+            fp[e] = fp[e] * s.decay - s.size * change(fm[e], fv[e], s.root, s.eps);
         }
+        store4(p + i, left - at, whole, fp);
+        store4(m, left - at, whole, fm);
+        store4(v, left - at, whole, fv);
     } else {
-        uint8_t *const m = t.template get<uint8_t>(2, at) + base, *const v = t.template get<uint8_t>(3, at) + base;
-        const int64_t blocks = (int64_t)chunk * (OPT_CHUNK / OPT_BLOCK);
-        float *const ms = t.template get<float>(4, at) + blocks, *const vs = t.template get<float>(5, at) + blocks;
+        uint8_t *const m = t.template get<uint8_t>(2, n), *const v = t.template get<uint8_t>(3, n);
+        const int64_t k = (int64_t)chunk * OPT_WAVES + block;
+        float *const ms = t.template get<float>(4, n) + k, *const vs = t.template get<float>(5, n) + k;
         const bool vec = (places % (4 * sizeof(T))) == 0 && (((uintptr_t)m | (uintptr_t)v) & 3) == 0;
-        for (int b = wave; b * OPT_BLOCK < live; b += OPT_WAVES) {
-            const int i = b * OPT_BLOCK + lane * 4;           // lanes behind the tensor's end hold zeros
-            const bool whole = vec && i + 4 <= live;
-            float fp[4], fg[4], fm[4], fv[4];
-            load4(p + i, live - i, whole, fp);
-            load4(g + i, live - i, whole, fg);
-            const uint32_t cm = load_codes(m + i, live - i, whole), cv = load_codes(v + i, live - i, whole);
-            decode4<true>(cm, ms[b], fm);
-            decode4<false>(cv, vs[b], fv);
-            uint32_t noise[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                fm[e] = fm[e] * s.beta1 + fg[e] * s.rest1;
-                fv[e] = fv[e] * s.beta2 + fg[e] * s.rest2 * fg[e];
-                if (i + e >= live) fm[e] = fv[e] = 0.f;        // (0 times a scale that is not finite)
-                fp[e] = fp[e] * s.decay - s.size * change(fm[e], fv[e], s.root, s.eps);
-                noise[e] = dither((uint32_t)(base + i + e), s.step);
-            }
-            float sm, sv;
-            const uint32_t em = encode4<true>(fm, noise, sm), ev = encode4<false>(fv, noise, sv);
-            store4(p + i, live - i, whole, fp);
-            store_codes(m + i, live - i, whole, em);
-            store_codes(v + i, live - i, whole, ev);
-            if (lane == 0) ms[b] = sm, vs[b] = sv;
+        if (vec && left >= OPT_BLOCK) Lane<T>(p + i, g + i, m + i, v + i, *ms, *vs, 4, true).step(s, p + i, m + i, v + i, ms, vs, i, 4, true);
+        else {                                                // lanes behind the tensor's end hold zeros
+            const bool whole = vec && at + 4 <= left;
+            Lane<T>(p + i, g + i, m + i, v + i, *ms, *vs, left - at, whole).step(s, p + i, m + i, v + i, ms, vs, i, left - at, whole);
         }
     }
 }
