@@ -135,10 +135,34 @@ def test_many_tensors(dev, bits):
     for p, g in zip(params, _tensors(dev, shapes, torch.float32, 4, 1e-3) + _tensors(dev, shapes, torch.bfloat16, 5, 1e-3)):
         p.grad = g
     opt.step()
-    assert f"adamw_kernel<unsigned short, {bits}>" in _lib.last_kernel()
+    assert f"adamw_kernel<unsigned short, {bits}, false>" in _lib.last_kernel()
     for p, r in zip(params, refs):
         r.step(p.grad)
         r.check(p, opt.state[p])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_more_than_the_caches_hold(dev, dtype, bits):
+    """The steps of weights that go past the caches: a large one, and small ones of the same call, against a call of their own."""
+    from vtpack_amd import _lib
+    sizes = [(1 << 25) + 1029, 100003, 77]
+    values, grads = _tensors(dev, [(n,) for n in sizes], dtype, 31), _tensors(dev, [(n,) for n in sizes], dtype, 32, 1e-3)
+    ends = [torch.nn.Parameter(t[:5000].clone()) for t in values[:1]] + [torch.nn.Parameter(t.clone()) for t in values[1:]]
+    large = [torch.nn.Parameter(t) for t in values]
+    opts = [_optimizer(ps, bits) for ps in (large, ends)]
+    for k in range(2):
+        for ps in (large, ends):
+            for p, g in zip(ps, grads):
+                p.grad = g[:p.numel()] * (1 + k)
+        for opt, name in zip(opts, ("true", "false")):
+            opt.step()
+            assert _lib.last_kernel().endswith(f", {bits}, {name}>")
+        for p, q in zip(large, ends):
+            # the same elements in the same places: whole blocks are the same, and so are whole tensors
+            n = q.numel() if q.numel() == p.numel() else q.numel() // 256 * 256
+            assert torch.equal(p[:n], q[:n])
+            assert all(torch.equal(opts[0].state[p][key][:n].view(torch.uint8), opts[1].state[q][key][:n].view(torch.uint8)) for key in ("exp_avg", "exp_avg_sq"))
 
 
 @pytest.mark.parametrize("bits", [32, 8])

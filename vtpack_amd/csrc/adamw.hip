@@ -6,8 +6,8 @@
 // it by halving.  A wave takes 256 consecutive elements at a time, four a lane: weights, gradients and moments all come in one load
 // a lane, and the 256 are the block that shares a scale, so that its largest magnitude is one reduction over the wave.  Waves take one
 // block each: while some wait others compute, with no loop to keep in order (four blocks a wave 10 to 20 percent slower).
-// Measured, on weights that are in no cache: 103 M bf16 weights with 32-bit moments 403 us, 5.6 TB/s; the 5.7 M and 22 M fp32 weights of
-// a vision transformer in 200 tensors 32 us with 32-bit moments (5.0 TB/s) and 75 us with 8-bit ones (4.7 TB/s).
+// Measured: 103 M bf16 weights with 32-bit moments 367 us, 6.2 TB/s; the 5.7 M and 22 M fp32 weights of a vision transformer in 200
+// tensors 32 us with 32-bit moments (5.1 TB/s) and 67 us with 8-bit ones (5.3 TB/s); a large copy reaches 4.9.
 //
 // Moments in 8 bits: the first as e4m3 over max|m| / 448, the second as e5m2 over max v / 57344.  Adam's slow decay (b2 = 0.999)
 // is far below half a step of either (1/16 and 1/8), and would be lost under rounding to the nearest; a value is therefore rounded
@@ -58,44 +58,41 @@ template <int BITS> struct OptTable {
 };
 static_assert(sizeof(OptTable<8>) + sizeof(OptScalars) + 8 <= 4096 && sizeof(OptTable<32>) + sizeof(OptScalars) + 8 <= 4096, "arguments");
 
-// ---- four elements of a lane: a vector where the tensor's buffers allow it, else one by one
-template <typename T> struct Four;
-template <> struct Four<float> {
-    static __device__ __forceinline__ void load(const float *p, float (&f)[4])
-    {
-        const f32x4 r = *reinterpret_cast<const f32x4 *>(p);
-        f[0] = r.x, f[1] = r.y, f[2] = r.z, f[3] = r.w;
-    }
-    static __device__ __forceinline__ void store(float *p, const float (&f)[4]) { *reinterpret_cast<f32x4 *>(p) = f32x4{f[0], f[1], f[2], f[3]}; }
-};
-template <> struct Four<bf16_t> {
-    static __device__ __forceinline__ void load(const bf16_t *p, float (&f)[4])
-    {
-        const u32x2 r = *reinterpret_cast<const u32x2 *>(p);
-        f[0] = bf16lo(r.x), f[1] = bf16hi(r.x), f[2] = bf16lo(r.y), f[3] = bf16hi(r.y);
-    }
-    static __device__ __forceinline__ void store(bf16_t *p, const float (&f)[4])
-    {
-        *reinterpret_cast<u32x2 *>(p) = u32x2{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
-    }
-};
-template <typename T> __device__ __forceinline__ void load4(const T *p, int live, bool whole, float (&f)[4])
+// ---- four elements of a lane: a vector where the tensor's buffers allow it, else one by one.  STREAM: past the caches, for weights,
+// gradients and moments of more than the last one holds.
+template <bool STREAM, typename V> __device__ __forceinline__ V get(const V *p)
 {
-    if (whole) {
-        Four<T>::load(p, f);
-    } else {
+    if constexpr (STREAM) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <bool STREAM, typename V> __device__ __forceinline__ void set(V *p, V v)
+{
+    if constexpr (STREAM) __builtin_nontemporal_store(v, p);
+    else *p = v;
+}
+template <bool STREAM, typename T> __device__ __forceinline__ void load4(const T *p, int live, bool whole, float (&f)[4])
+{
+    if (!whole) {
 #pragma unroll
         for (int e = 0; e < 4; e++) f[e] = e < live ? Elem<T>::load(p + e) : 0.f;
+    } else if constexpr (sizeof(T) == 4) {
+        const f32x4 r = get<STREAM>(reinterpret_cast<const f32x4 *>(p));
+        f[0] = r.x, f[1] = r.y, f[2] = r.z, f[3] = r.w;
+    } else {
+        const u32x2 r = get<STREAM>(reinterpret_cast<const u32x2 *>(p));
+        f[0] = bf16lo(r.x), f[1] = bf16hi(r.x), f[2] = bf16lo(r.y), f[3] = bf16hi(r.y);
     }
 }
-template <typename T> __device__ __forceinline__ void store4(T *p, int live, bool whole, const float (&f)[4])
+template <bool STREAM, typename T> __device__ __forceinline__ void store4(T *p, int live, bool whole, const float (&f)[4])
 {
-    if (whole) {
-        Four<T>::store(p, f);
-    } else {
+    if (!whole) {
 #pragma unroll
         for (int e = 0; e < 4; e++)
             if (e < live) Elem<T>::store(p + e, f[e]);
+    } else if constexpr (sizeof(T) == 4) {
+        set<STREAM>(reinterpret_cast<f32x4 *>(p), f32x4{f[0], f[1], f[2], f[3]});
+    } else {
+        set<STREAM>(reinterpret_cast<u32x2 *>(p), u32x2{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])});
     }
 }
 __device__ __forceinline__ uint32_t load_codes(const uint8_t *p, int live, bool whole)
@@ -204,15 +201,15 @@ __device__ __forceinline__ float change(float m, float v, float root, float eps)
 }
 
 // A lane's four elements of a block of 256 with 8-bit moments; `live` of them are the tensor's.
-template <typename T> struct Lane {
+template <typename T, bool STREAM> struct Lane {
     float p[4], g[4], sm, sv;
     uint32_t cm, cv;
 
     __device__ __forceinline__ Lane(const T *from, const T *grad, const uint8_t *m, const uint8_t *v, float m_scale, float v_scale, int live, bool whole)
         : sm(m_scale), sv(v_scale)
     {
-        load4(from, live, whole, p);
-        load4(grad, live, whole, g);
+        load4<STREAM>(from, live, whole, p);
+        load4<STREAM>(grad, live, whole, g);
         cm = load_codes(m, live, whole), cv = load_codes(v, live, whole);
     }
     __device__ __forceinline__ void step(const OptScalars &s, T *to, uint8_t *m, uint8_t *v, float *ms, float *vs, int64_t place, int live, bool whole)
@@ -231,14 +228,14 @@ template <typename T> struct Lane {
             noise[e] = dither((uint32_t)(place + e), s.step);
         }
         const uint32_t em = encode4<true>(fm, noise, sm), ev = encode4<false>(fv, noise, sv);
-        store4(to, live, whole, p);
+        store4<STREAM>(to, live, whole, p);
         store_codes(m, live, whole, em);
         store_codes(v, live, whole, ev);
         if ((threadIdx.x & 63) == 0) *ms = sm, *vs = sv;
     }
 };
 
-template <typename T, int BITS>
+template <typename T, int BITS, bool STREAM>
 __global__ __launch_bounds__(64 * OPT_WAVES) void adamw_kernel(OptTable<BITS> t, OptScalars host, const OptScalars *__restrict__ device)
 {
 #pragma clang fp contract(off)
@@ -265,28 +262,28 @@ __global__ __launch_bounds__(64 * OPT_WAVES) void adamw_kernel(OptTable<BITS> t,
         float *const m = t.template get<float>(2, n) + i, *const v = t.template get<float>(3, n) + i;
         const bool whole = (places % (4 * sizeof(T))) == 0 && (((uintptr_t)m | (uintptr_t)v) & 15) == 0 && at + 4 <= left;
         float fp[4], fg[4], fm[4], fv[4];
-        load4(p + i, left - at, whole, fp);
-        load4(g + i, left - at, whole, fg);
-        load4(m, left - at, whole, fm);
-        load4(v, left - at, whole, fv);
+        load4<STREAM>(p + i, left - at, whole, fp);
+        load4<STREAM>(g + i, left - at, whole, fg);
+        load4<STREAM>(m, left - at, whole, fm);
+        load4<STREAM>(v, left - at, whole, fv);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             fm[e] = fm[e] * s.beta1 + fg[e] * s.rest1;
             fv[e] = fv[e] * s.beta2 + fg[e] * s.rest2 * fg[e];
             fp[e] = fp[e] * s.decay - s.size * change(fm[e], fv[e], s.root, s.eps);
         }
-        store4(p + i, left - at, whole, fp);
-        store4(m, left - at, whole, fm);
-        store4(v, left - at, whole, fv);
+        store4<STREAM>(p + i, left - at, whole, fp);
+        store4<STREAM>(m, left - at, whole, fm);
+        store4<STREAM>(v, left - at, whole, fv);
     } else {
         uint8_t *const m = t.template get<uint8_t>(2, n), *const v = t.template get<uint8_t>(3, n);
         const int64_t k = (int64_t)chunk * OPT_WAVES + block;
         float *const ms = t.template get<float>(4, n) + k, *const vs = t.template get<float>(5, n) + k;
         const bool vec = (places % (4 * sizeof(T))) == 0 && (((uintptr_t)m | (uintptr_t)v) & 3) == 0;
-        if (vec && left >= OPT_BLOCK) Lane<T>(p + i, g + i, m + i, v + i, *ms, *vs, 4, true).step(s, p + i, m + i, v + i, ms, vs, i, 4, true);
+        if (vec && left >= OPT_BLOCK) Lane<T, STREAM>(p + i, g + i, m + i, v + i, *ms, *vs, 4, true).step(s, p + i, m + i, v + i, ms, vs, i, 4, true);
         else {                                                // lanes behind the tensor's end hold zeros
             const bool whole = vec && at + 4 <= left;
-            Lane<T>(p + i, g + i, m + i, v + i, *ms, *vs, left - at, whole).step(s, p + i, m + i, v + i, ms, vs, i, left - at, whole);
+            Lane<T, STREAM>(p + i, g + i, m + i, v + i, *ms, *vs, left - at, whole).step(s, p + i, m + i, v + i, ms, vs, i, left - at, whole);
         }
     }
 }
@@ -324,6 +321,11 @@ __global__ void adamw_scalars_kernel(int64_t *step, int64_t skipped, int advance
 template <typename T, int BITS>
 static int go_adamw(const vtdge_adamw_tensor *tensors, int count, const OptScalars &s, const OptScalars *device, hipStream_t st)
 {
+    // bytes of the call against the last cache's 256 MB: 22 M fp32 weights with 8-bit moments (355 MB) 75 us through the caches, 67 past
+    // them, 103 M bf16 weights (2.3 GB) 401 and 365; 5.7 M fp32 weights (160 MB) 31.8 and 32.9
+    double bytes = 0;
+    for (int k = 0; k < count; k++) bytes += (3.0 * sizeof(T) + (BITS == 8 ? 4 : 16)) * tensors[k].n;
+    auto kern = bytes > (256 << 20) ? adamw_kernel<T, BITS, true> : adamw_kernel<T, BITS, false>;
     OptTable<BITS> t{};
     int i = 0;
     while (i < count) {
@@ -344,7 +346,6 @@ static int go_adamw(const vtdge_adamw_tensor *tensors, int count, const OptScala
         if (k == 0) break;
         t.count = k;
         t.chunks = (uint32_t)chunks;
-        auto kern = adamw_kernel<T, BITS>;
         note_kernel(reinterpret_cast<const void *>(kern));
         kern<<<dim3((unsigned)chunks), dim3(64 * OPT_WAVES), 0, st>>>(t, s, device);
         const int rc = check_launch("adamw");
