@@ -9,13 +9,19 @@
 // operand; the sums over it are fp32) and kept for this piece only, and two products take it to dx and dW.  Four products of
 // rows x classes x width in place of three, and no more than rows x piece values of scratch.
 //
-// One product routine does all of it: tiles through LDS by direct loads in slabs of 64 of the summed dimension, two in turn.  An
-// operand either lies with the summed dimension along its rows (x and W for z, d for dx) or across them (W for dx, d and x for
+// One product routine does all of it: tiles through LDS by direct loads, in slabs of 32 or 64 of the summed dimension and a ring of two
+// to six of them.  An operand either lies with the summed dimension along its rows (x and W for z, d for dx) or across them (W for dx, d and x for
 // dW); the second kind goes into LDS as it lies and is transposed by the LDS reads.  16-byte pieces are XOR-ed by their row against
 // bank conflicts, on the side of the global address.
 // fp32 operands are split into three bf16 parts each (24 bits), and the six products of parts down to 2^-24 are a six times longer
 // sum, smallest first, in the same fp32 sums: the same kernels at a sixth of their rate, which is above that of the fp32 matrix
-// instructions.
+// instructions.  (Two fp16 parts and three products would be 22 bits of a row's largest value and fewer of its small ones.)
+//
+// Bound by the matrix units in long products: 8192 rows x 65536 classes x 1024 in bf16, tiles 0.98 ms (1.12 PFLOP/s), d 4 x 0.29 (0.94,
+// with the writing of d), gradients 4 x 0.51 (1.07); in fp32 2048 x 21841 x 384, tiles 0.21 ms (166 TFLOP/s of fp32, 1.0 PFLOP/s issued), d
+// 0.26, gradients 0.39.  Their units are busy for 57 percent at the 1.7 - 1.9 GHz that the clock falls to, waves wait for them half of the
+// time.  By the reading of W where rows are few (1 row x 65536 x 1024 in 21.6 us, 6.2 TB/s), by launches where all is small (256 x 1000 x
+// 384: five kernels of 6 - 10 us).
 #include "common.h"
 
 #include <math.h>

