@@ -638,7 +638,8 @@ int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const void *weight,
 /* One AdamW step over `count` tensors, in one launch for each 134 of them (96 with 8-bit moments):
  *   p *= 1 - lr weight_decay;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
  *   p -= lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
- *   tensors_host  HOST table; param and grad of `dtype`, n elements each, any alignment of their type
+ *   tensors_host  HOST table; param and grad of `dtype`, n elements each, any alignment of their type, no two params or moments
+ *                 over the same memory, all below address 2^48
  *   state_bits    32: exp_avg, exp_avg_sq fp32.  8: exp_avg e4m3, exp_avg_sq e5m2 (OCP), one byte an element, with an fp32
  *                 scale for each 256 consecutive elements (ceil(n / 256) of them): largest magnitude / 448 and / 57344.
  *                 Values are rounded down or up by a hash of the element's index and `step`; the same on every run

@@ -431,3 +431,44 @@ def test_steps_that_find_everything_in_place(dev, bits, monkeypatch):
     params[0].grad.data = params[0].grad.data[:10]         # a gradient that no longer fits
     with pytest.raises(ValueError):
         opt.step()
+
+
+def test_weights_over_each_other_are_refused(dev):
+    from vtpack_amd.optim import AdamW
+    flat = torch.randn(1000, device=dev)
+    for a, b in ((flat, flat), (flat[:600], flat[599:])):
+        params = [torch.nn.Parameter(a), torch.nn.Parameter(b)]
+        for p in params:
+            p.grad = torch.ones_like(p)
+        with pytest.raises(ValueError, match="over each other"):
+            AdamW(params).step()
+    p = torch.nn.Parameter(flat)
+    p.grad = torch.ones_like(p)
+    with pytest.warns(UserWarning, match="duplicate"):
+        opt = AdamW([p, p])
+    with pytest.raises(ValueError, match="over each other"):
+        opt.step()
+    halves = [torch.nn.Parameter(flat[:500]), torch.nn.Parameter(flat[500:])]       # side by side
+    for p in halves:
+        p.grad = torch.ones_like(p)
+    AdamW(halves).step()
+
+
+def test_steps_leave_no_memory_behind(dev):
+    import gc
+    from vtpack_amd.layers import gate_balance, linear_cross_entropy
+    x, w = (torch.randn(n, 64, device=dev, requires_grad=True) for n in (100, 50))
+    t = torch.randint(0, 50, (100,), device=dev)
+    opt = _optimizer([x, w], 8)
+    used = []
+    for k in range(6):
+        for _ in range(50):
+            opt.zero_grad()
+            (linear_cross_entropy(x, w, None, t) + gate_balance(x, mask=t > 3)[0]).backward()
+            opt.step()
+        if k == 3:
+            opt.load_state_dict(opt.state_dict())          # tables are made anew
+        opt.zero_grad()
+        gc.collect()
+        used.append(torch.cuda.memory_allocated())
+    assert used[-1] <= used[0]

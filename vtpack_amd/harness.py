@@ -119,7 +119,7 @@ def train_step(model, images, target, optimizer, label_smoothing=0.0, dge_enable
                balance_scale=0.0, clip_grad=None):
     """One update of a model in training mode (vtpack/engine/engine.py:48-90 without autocast): the classifier's cross entropy against
     int64 `target`, with `dge_enable` the budget loss, `balance_scale` times the balance of the gates, gradients, their norm cut
-    to `clip_grad`, the optimiser's step (any; `optim.AdamW` takes one launch for some 90 weights).  -> {name: tensor on the GPU},
+    to `clip_grad`, the optimiser's step (any; `optim.AdamW` takes one launch for 134 weights).  -> {name: tensor on the GPU},
     nothing of which is waited for: loss, loss_cls, and loss_dge, dge_ratio, loss_balance, gate_counts, grad_norm where they are made.
 
     Weights are float32: the dense training branch multiplies with the library's batched products."""

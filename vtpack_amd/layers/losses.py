@@ -41,6 +41,8 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
         return zero if reduction != "none" else zero.expand(target.shape)
     loss = _lib.training().linear_cross_entropy(ops._rows_of(x), ops._rows_of(weight), None if bias is None else bias.contiguous(),
                                                 target.reshape(-1).contiguous(), int(ignore_index), float(label_smoothing), how[2])
+    if loss is None:
+        raise ValueError("linear_cross_entropy takes strided tensors")
     return loss.view(target.shape) if reduction == "none" and target.dim() != 1 else loss
 
 
@@ -80,4 +82,7 @@ def gate_balance(gate, indices=None, top_k=1, mask=None):
         mask = mask.reshape(-1).contiguous()
     if gate.numel() == 0:
         return gate.sum().float(), torch.zeros((E,), dtype=torch.int64, device=gate.device)
-    return _lib.training().balance(ops._rows_of(gate), indices, mask, int(top_k))
+    out = _lib.training().balance(ops._rows_of(gate), indices, mask, int(top_k))
+    if out is None:
+        raise ValueError("gate_balance takes strided tensors")
+    return out

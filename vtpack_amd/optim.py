@@ -74,7 +74,8 @@ class AdamW(torch.optim.Optimizer):
     without torch's knowledge, so that what is derived from them is made anew only after `ops.invalidate_packed`.
 
     Gradients are read where they lie and have their weight's type; one of other strides than its weight is copied first.
-    Refused: types the kernels do not have, sparse gradients, weights with gaps between their elements."""
+    Refused: types the kernels do not have, sparse gradients, weights with gaps between their elements, weights of a group that lie over
+    each other."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, capturable=False):
         if torch.is_tensor(lr):
@@ -152,6 +153,9 @@ class AdamW(torch.optim.Optimizer):
                 state.update(self._lay_out(p, bits, int(group["step"])))
             self._check(p, g, state, bits)
             sets.setdefault((p.dtype, p.device, state.get("skipped", 0)), []).append(p)
+        lie = sorted((p.device.index, p.data_ptr(), p.data_ptr() + p.nbytes) for p in params if p.numel())
+        if any(a[0] == b[0] and b[1] < a[2] for a, b in zip(lie, lie[1:])):
+            raise ValueError("AdamW: weights that lie over each other, or one twice in a group, cannot be moved in one step")
         if group["capturable"] and len({d for _, d, _ in sets}) > 1:
             raise ValueError("AdamW: a capturable group keeps its count of steps on one device")
         return [_Batch(ps, [self.state[p] for p in ps], bits, skipped) for (_, _, skipped), ps in sets.items()]
