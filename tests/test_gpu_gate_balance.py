@@ -93,6 +93,26 @@ def test_equal_logits_go_to_the_lowest(dev, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("E,k", [(3, 1), (40, 3), (160, 6)])
+def test_not_a_number_is_the_largest(dev, dtype, E, k):
+    """NaN of every kind are one value above infinity: the lowest experts with one are chosen first."""
+    from vtpack_amd.layers import gate_balance
+    gate = _gate(dev, 64, E, dtype)
+    bits = gate.view(torch.int16 if dtype == torch.bfloat16 else torch.int32)
+    some, all_ones = (0x7fc0, -1) if dtype == torch.bfloat16 else (0x7fc00000, -1)
+    g = torch.Generator().manual_seed(4)
+    for kind in (some, all_ones, 0x7fff if dtype == torch.bfloat16 else 0x7fffffff):
+        for t, e in zip(torch.randint(0, 64, (30,), generator=g).tolist(), torch.randint(0, E, (30,), generator=g).tolist()):
+            bits[t, e] = kind
+    bits[0, 0], bits[1, 0], bits[2, E - 1] = all_ones, some, all_ones
+    gate[3, 1] = float("inf")
+    key = torch.where(gate.isnan(), torch.full_like(gate, float("inf")).double() , gate.double().clamp(max=1e300)).cpu()
+    chosen = torch.sort(key, dim=1, descending=True, stable=True).indices[:, :k]
+    want = torch.bincount(chosen.reshape(-1), minlength=E)
+    assert torch.equal(gate_balance(gate, top_k=k)[1].cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_masks(dev, dtype):
     """Experts masked by -inf or by the type's lowest value, tokens whose experts are all masked, what is masked not finite, and
     nothing left at all."""

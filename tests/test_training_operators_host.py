@@ -100,3 +100,39 @@ def test_workspaces_follow_the_sizes():
     # d of a piece: no more than 320 MB, or 1024 classes, however many classes there are
     assert size(8192, 65536, 1024, 1, 1) < (320 << 20) + 2 * 65536 * 1024 * 2 + 3 * 8192 * 1024 * 4 + (8 << 20) * 4 * 2
     assert lib.vtdge_gate_balance_workspace(100, 8) == 0 and lib.vtdge_gate_balance_workspace(1 << 20, 8) == 256 * 17 * 4
+
+
+def test_the_native_module_is_named_when_it_is_missing(monkeypatch):
+    import sys
+    import vtpack_amd
+    monkeypatch.setattr(_lib, "_training", None)
+    monkeypatch.delattr(vtpack_amd, "_training", raising=False)
+    monkeypatch.setitem(sys.modules, "vtpack_amd._training", None)
+    with pytest.raises(ImportError, match="_training.so is missing"):
+        _lib.training()
+
+
+def test_arguments_of_the_native_module():
+    """Operands it does not take as they are come back as None, for Python to name what is wrong; nothing else passes either."""
+    native = _lib.training()
+    x, t = torch.randn(4, 8), torch.zeros(4, dtype=torch.int64)
+    assert native.linear_cross_entropy(x, x, None, t, -100, 0.0, 1) is None
+    assert native.linear_cross_entropy(x, x, None, t, -100, 0.0, None) is None
+    assert native.linear_cross_entropy("x", x, None, t, -100, 0.0, 1) is None
+    assert native.balance(x, None, None, 1) is None and native.balance(None, None, None, 1) is None
+    for name in ("linear_cross_entropy", "cross_entropy", "cross_entropy_backward", "balance", "gate_balance", "gate_balance_backward",
+                 "adamw_batch", "adamw_step", "bind"):
+        with pytest.raises(RuntimeError, match="arguments"):
+            getattr(native, name)(1)
+    p = torch.nn.Parameter(x)
+    with pytest.raises(RuntimeError, match="do not match"):
+        native.adamw_batch([p], [], ["exp_avg"])
+    with pytest.raises(RuntimeError, match="without its moments"):
+        native.adamw_batch([p], [{}], ["exp_avg"])
+    batch = native.adamw_batch([p], [{"exp_avg": x.clone(), "exp_avg_sq": x.clone()}], ["exp_avg", "exp_avg_sq"])
+    state = {p: {}}
+    assert native.adamw_step(batch, [p], state, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 32) is False       # another state, no gradient
+    with pytest.raises((RuntimeError, ValueError)):
+        native.adamw_step(None, [p], state, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 32)
+    with pytest.raises(TypeError):
+        native.adamw_step(batch, [p], state, "lr", 0.9, 0.999, 1e-8, 0.0, 1, 32)

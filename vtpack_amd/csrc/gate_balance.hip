@@ -10,7 +10,7 @@
 // workgroup joins them in their order.  Few tokens are one workgroup's, which joins its own.  Counts are whole numbers and the
 // order of the sums is that of the launch: the same bits on every call.  The gradient works the probabilities out again.
 // Measured: 128 tokens of 3 in fp32 5.0 + 3.0 us (forward, gradient); 65536 of 3 in bf16 7.6 + 3 + 5.4; 131071 of 160, the 6 largest, masked, in
-// bf16 33 + 5 + 17.5: there the choice bounds the forward (six times the maximum of ten logits a lane and an exchange), the
+// bf16 28 + 5 + 17: there the choice bounds the forward (six times the maximum of ten logits a lane and an exchange), the
 // gradient moves its 84 MB at 4.8 TB/s.
 #include "common.h"
 
@@ -52,12 +52,11 @@ __device__ __forceinline__ float sum16(float v)
     return v + __int_as_float(other16<1>(__float_as_int(v)));
 }
 
-// a float's bits in the order of its value, NaN (of either sign) above infinity, the two zeros equal; never 0
+// a float's bits in the order of its value, all NaN alike above infinity, the two zeros equal; never 0
 __device__ __forceinline__ uint32_t ordered(float f)
 {
     const uint32_t u = __float_as_uint(f + 0.f);
-    const uint32_t k = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
-    return k < 0x007fffffu ? 0xffffffffu : k;                         // below minus infinity: a NaN with a sign
+    return f != f ? 0xffffffffu : u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
 // Values 2 j and 2 j + 1 of lane l are those of experts 32 j + 2 l and the next: one load for two where the rows allow it (PAIRS),
@@ -96,16 +95,17 @@ template <typename T, int N> struct Token {
         if constexpr (sizeof(T) == 2) {          // a 16-bit logit leaves half of the key to the expert
 #pragma unroll
             for (int i = 0; i < N; i++) key[i] = WAY == FULL || expert(i, l) < E ? (ordered(p[i]) & 0xffff0000u) | (0xffffu - expert(i, l)) : 0u;
-            uint32_t below = ~0u;
+            // what is chosen already is at or above `chosen`: of differences modulo 2^32, those of smaller keys are the large ones
+            uint32_t chosen = 0;
             for (int k = 0; k < K; k++) {
                 uint32_t best = 0;
 #pragma unroll
                 for (int i = 0; i < N; i++) {
-                    const uint32_t c = key[i] < below ? key[i] : 0u;
+                    const uint32_t c = key[i] - chosen;
                     best = best > c ? best : c;
                 }
-                below = umax16(best);
-                if (l == 0 && live) atomicAdd(counts + (0xffffu - (below & 0xffffu)), 1u);
+                chosen += umax16(best);
+                if (l == 0 && live) atomicAdd(counts + (0xffffu - (chosen & 0xffffu)), 1u);
             }
         } else {
 #pragma unroll
