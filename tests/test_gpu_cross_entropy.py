@@ -174,7 +174,8 @@ def test_large_logits(dev):
 
 
 @pytest.mark.parametrize("dtype,rows,classes,width", [(torch.bfloat16, 8192, 21841, 128), (torch.float32, 4096, 12000, 64), (torch.bfloat16, 1, 70001, 256),
-                                                      (torch.float32, 3, 40000, 100), (torch.bfloat16, 9000, 3, 64)])
+                                                      (torch.float32, 3, 40000, 100), (torch.bfloat16, 9000, 3, 64),
+                                                      (torch.bfloat16, 3, 34001, 1024), (torch.bfloat16, 64, 34001, 1024)])
 def test_pieces_and_long_sums(dev, dtype, rows, classes, width):
     """More classes than a piece holds; one row against many classes and the other way around, where sums are cut."""
     _check(*_operands(dev, rows, classes, width, dtype, left_out=0.1 if rows > 10 else 0.0))

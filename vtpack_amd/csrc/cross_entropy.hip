@@ -45,6 +45,7 @@ template <int IM_, int JN_, int WM_, int WN_, int SLAB_, int SLOTS_, int PARTS_>
     static constexpr int ROWS = 32 * IM * WM, COLS = 32 * JN * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
     static constexpr int STAGE = PARTS * (ROWS + COLS) * SLAB * 2, RING = SLOTS * STAGE;
     static constexpr int LDS = RING + COLS * 4;                          // and the bias of the tile's classes
+    static constexpr bool FLAT = IM == 1 && JN == 2;                    // few rows
     static constexpr bool WHOLE_LINES = IM == 1 && JN == 1;             // gradients leave by way of LDS
     static constexpr int PER_SIMD = WAVES / 4 * (2 * LDS <= 160 * 1024 ? 2 : 1);
     static_assert(LDS <= 160 * 1024 && 6 * ROWS * 4 <= RING, "LDS");
@@ -56,7 +57,7 @@ template <int IM_, int JN_, int WM_, int WN_, int SLAB_, int SLOTS_, int PARTS_>
 // of 8 of them, `span`.  No stage begins behind `limit`: a sum of n rows of memory has ceil(n / SLAB) stages.
 // LDS rows are 2 SLAB bytes (ALONG) or 2 T bytes (across) without gaps; their 16-byte pieces are XOR-ed by the row, so that the
 // sixteen lanes that read together meet every bank once.
-template <bool ALONG, int T, int SLAB, int WAVES> struct Loader {
+template <bool ALONG, int T, int SLAB, int WAVES, bool MAY_STREAM = false> struct Loader {
     static constexpr int ROW = ALONG ? 2 * SLAB : 2 * T, STAGE = 2 * SLAB * T;
     static constexpr int LPR = ROW / 16, RPI = 64 / LPR;                  // lanes a row, rows an instruction
     static constexpr int PIECES = STAGE / 1024 / WAVES;                   // instructions of a wave
@@ -64,6 +65,7 @@ template <bool ALONG, int T, int SLAB, int WAVES> struct Loader {
     const unsigned char *base;
     int64_t plane, pitch;                                                 // bytes
     int limit, row0, last;
+    bool stream = false;                                                  // past the caches
 
     __device__ __forceinline__ Loader(const Operand &o, int64_t first, int64_t lim, int64_t span)
         : base(reinterpret_cast<const unsigned char *>(o.p) + (ALONG ? first * o.pitch * 2 : first * 2)), plane(o.plane * 2), pitch(o.pitch * 2)
@@ -90,7 +92,9 @@ template <bool ALONG, int T, int SLAB, int WAVES> struct Loader {
             const int at = ((lane % LPR) ^ swizzle(r)) * 16;
             const int row = ALONG ? min(r, limit - 1) : min(r, limit - 1 - kt * SLAB);
             const int col = ALONG ? at : min(at, last);
-            dma16(from, (uint32_t)row * (uint32_t)pitch + col, wave_uniform(lds + (d * WAVES + wid) * 1024));
+            const uint32_t off = (uint32_t)row * (uint32_t)pitch + col, to = wave_uniform(lds + (d * WAVES + wid) * 1024);
+            if (MAY_STREAM && stream) dma16_nt(from, off, to);
+            else dma16(from, off, to);
         }
     }
     // the 8 values of step s (16 of the summed dimension) of tile row `block` * 32 + lane % 32
@@ -111,12 +115,10 @@ template <bool ALONG, int T, int SLAB, int WAVES> struct Loader {
 
 // acc[i][j][v] += A[row i*32 + lane%32 of the wave] . B[row j*32 + 8*(v/4) + 4*(lane/32) + v%4], stages t0 .. t1 - 1.  SUMS: also the sums of
 // A's rows (of this half of the lanes' values), for what `sums_wanted` says.
-template <class S, bool A_ALONG, bool B_ALONG, bool SUMS>
-__device__ __forceinline__ void multiply_tile(const Loader<A_ALONG, S::ROWS, S::SLAB, S::WAVES> &a, const Loader<B_ALONG, S::COLS, S::SLAB, S::WAVES> &b,
-                                              int t0, int t1, unsigned char *smem, f32x16 (&acc)[S::IM][S::JN], bool sums_wanted, float (&sums)[S::IM])
+template <class S, bool SUMS, class LA, class LB>
+__device__ __forceinline__ void multiply_tile(const LA &a, const LB &b, int t0, int t1, unsigned char *smem, f32x16 (&acc)[S::IM][S::JN],
+                                              bool sums_wanted, float (&sums)[S::IM])
 {
-    using LA = Loader<A_ALONG, S::ROWS, S::SLAB, S::WAVES>;
-    using LB = Loader<B_ALONG, S::COLS, S::SLAB, S::WAVES>;
     constexpr int IM = S::IM, JN = S::JN, PARTS = S::PARTS, SLOTS = S::SLOTS, A_BYTES = PARTS * LA::STAGE;
     constexpr int LOADS = PARTS * (LA::PIECES + LB::PIECES);
     static_assert(LOADS * (SLOTS - 2) < 64, "the counter of outstanding loads");
@@ -216,6 +218,7 @@ struct CeArgs {
     const void *bias; const int64_t *target; int64_t rows, classes; int64_t ignore; float smoothing; int stages;
     int64_t v0, v1;                                 // classes of this piece
     int bias_f32;
+    bool stream_w;                                  // forward, few rows: W past the caches
     // forward: [class tiles][rows] each
     float *tile_max, *tile_sum, *tile_total, *target_z;
     // backward
@@ -277,8 +280,9 @@ template <class S, bool TOTAL> __global__ __launch_bounds__(S::THREADS, S::PER_S
     f32x16 acc[IM][JN] = {};
     float none[IM];
     const Loader<true, ROWS, S::SLAB, S::WAVES> a(p.x, r0, p.rows, 0);
-    const Loader<true, S::COLS, S::SLAB, S::WAVES> b(p.w, c0, p.classes, 0);
-    multiply_tile<S, true, true, false>(a, b, 0, p.stages, smem, acc, false, none);
+    Loader<true, S::COLS, S::SLAB, S::WAVES, S::FLAT> b(p.w, c0, p.classes, 0);
+    b.stream = p.stream_w;
+    multiply_tile<S, false>(a, b, 0, p.stages, smem, acc, false, none);
     logits<S>(bias + wn * 32 * JN, acc);
     float *const shared = reinterpret_cast<float *>(smem);          // [waves along the classes][largest, sum, total][rows]
 #pragma unroll
@@ -513,7 +517,7 @@ template <class S> __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void cr
     float none[IM];
     const Loader<true, S::ROWS, S::SLAB, S::WAVES> a(p.x, r0, p.rows, 0);
     const Loader<true, S::COLS, S::SLAB, S::WAVES> b(p.w, c0, p.classes, 0);
-    multiply_tile<S, true, true, false>(a, b, 0, p.stages, smem, acc, false, none);
+    multiply_tile<S, false>(a, b, 0, p.stages, smem, acc, false, none);
     logits<S>(bias + wn * 32 * JN, acc);
     // To memory: half-wave swaps leave a lane 8 consecutive classes.  bf16: as they are, 32 bytes of a row side by side, while the other
     // workgroup of the compute unit multiplies (8192 x 1024 x 65536: 313 us a piece, by way of LDS 328).  fp32, where a workgroup
@@ -652,7 +656,7 @@ template <class S, bool A_ALONG> __device__ __forceinline__ void gradient_tile(c
     float scale = 1.f;
     if (all.scale != nullptr) scale = *all.scale;
     if (all.scale2 != nullptr) scale *= *all.scale2;
-    multiply_tile<S, A_ALONG, false, !A_ALONG>(a, b, t0, t1, smem, acc, with_sums, sums);
+    multiply_tile<S, !A_ALONG>(a, b, t0, t1, smem, acc, with_sums, sums);
 #pragma unroll
     for (int i = 0; i < IM; i++) {
         const int64_t r = r0 + (wm * IM + i) * 32 + lr;
@@ -1109,6 +1113,9 @@ extern "C" int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weigh
     a.smoothing = smoothing, a.stages = (int)ceil_div(p.padded, p.slab_l), a.v0 = 0, a.v1 = classes;
     a.tile_max = (float *)(ws + p.max_at), a.tile_sum = (float *)(ws + p.sum_at), a.tile_total = (float *)(ws + p.total_at);
     a.target_z = (float *)(ws + p.z_at);
+    // W is read once where it lies.  From a quarter of the last cache's 256 MB on, what a program does between two calls leaves little of
+    // it there (1 x 1024 x 65536, 134 MB: out of memory 27.4 us through the caches, 24.7 past them; still in the cache 25.5 and 27.1)
+    a.stream_w = p.logits == CE_FLAT && a.w.p == weight && classes * p.padded * 2 >= (64 << 20);
     if (p.split) VT_STEP(p.logits == CE_LARGE ? go_tiles<SplitLarge>(a, p, st) : p.logits == CE_FLAT ? go_tiles<SplitFlat>(a, p, st) : go_tiles<SplitSmall>(a, p, st));
     else VT_STEP(p.logits == CE_LARGE ? go_tiles<LogitsLarge>(a, p, st) : p.logits == CE_MIDDLE ? go_tiles<LogitsMiddle>(a, p, st) : p.logits == CE_FLAT ? go_tiles<LogitsFlat>(a, p, st) : go_tiles<LogitsSmall>(a, p, st));
     const JoinArgs j{a.tile_max, a.tile_sum, a.tile_total, a.target_z, target, rows, classes, ignore_index, smoothing, (int)p.tn,
