@@ -433,3 +433,21 @@ def test_no_graph_without_gradients(dev):
         assert not gate_balance(x)[0].requires_grad
     loss, counts = gate_balance(x)
     assert loss.requires_grad and not counts.requires_grad
+
+
+def test_a_graph_is_used_once(dev):
+    """A second backward pass without retain_graph is refused, and what the first one read is given back."""
+    from vtpack_amd.layers import gate_balance, linear_cross_entropy
+    x, w, b, t = _operands(dev, 50, 60, 64, torch.float32)
+    x.requires_grad_()
+    for loss in (linear_cross_entropy(x, w, b, t), gate_balance(x)[0]):
+        assert loss.grad_fn.name() in ("LinearCrossEntropyBackward", "GateBalanceBackward")
+        loss.backward()
+        with pytest.raises(RuntimeError, match="second time"):
+            loss.backward()
+    both = linear_cross_entropy(x, w, b, t, reduction="none")
+    used = torch.cuda.memory_allocated()
+    both.sum().backward()
+    del both
+    x.grad = None
+    assert torch.cuda.memory_allocated() < used

@@ -3,20 +3,22 @@
 //
 // Why this is native: small calls of these operators are bound by the host.  A backward pass runs in the engine's own thread, whose
 // core comes out of its sleep for it, and what Python does there (the interpreter lock, four allocations, 24 arguments) took 32 of
-// the 122 us of a DeiT-S classifier's loss with its gradients; a step over 200 weights looked at some 1000 objects, 77 us beside the
-// 31 us of its kernels.
+// the 122 us of a DeiT-S classifier's loss with its gradients (71 so); a step over 200 weights looked at some 1000 objects, 77 us beside the
+// 31 us of its kernels (7 so).
 #include <Python.h>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <map>
 #include <mutex>
-#include <optional>
+#include <memory>
 #include <stdexcept>
 #include <string>
 #include <tuple>
@@ -27,7 +29,7 @@
 namespace {
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
 #define VT_FUNCTIONS(X)                                                                                                \
@@ -131,31 +133,47 @@ void no_second_order(const char *name)
     if (at::GradMode::is_enabled()) throw std::runtime_error(std::string(name) + ": gradients of the gradients are not supported");
 }
 
-struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
-    static Tensor forward(AutogradContext *ctx, const Tensor &x, const Tensor &w, const std::optional<Tensor> &b, const Tensor &target,
-                          int64_t ignore, double smoothing, int64_t reduction)
-    {
-        const Tensor bias = b.value_or(Tensor());
-        const Forward f = cross_entropy(x, w, bias, target, ignore, smoothing, (int)reduction);
-        ctx->save_for_backward({x, w, bias, target, f.stats, f.laid_out});
-        ctx->saved_data["ignore"] = ignore;
-        ctx->saved_data["smoothing"] = smoothing;
-        ctx->saved_data["reduction"] = reduction;
-        return f.loss;
-    }
-    static variable_list backward(AutogradContext *ctx, variable_list grads)
+// The backward node of a loss, with what it reads as members.
+struct LinearCrossEntropyBackward : torch::autograd::Node {
+    SavedVariable x, w, bias, target;
+    Tensor stats, laid_out;                     // nobody else's
+    int64_t ignore; double smoothing; int reduction;
+
+    variable_list apply(variable_list &&grads) override
     {
         no_second_order("linear_cross_entropy");
-        const variable_list t = ctx->get_saved_variables();
+        std::lock_guard<std::mutex> hold(mutex_);
+        const Tensor x_ = x.unpack(), w_ = w.unpack(), b_ = bias.unpack(), t_ = target.unpack();
         Tensor grad = grads[0];
+        if (!grad.defined()) return {Tensor(), Tensor(), Tensor()};
         // the same for every row, as a sum over the losses leaves it: one value
         if (grad.dim() == 1) grad = grad.stride(0) == 0 ? grad.select(0, 0) : grad.contiguous();
-        const auto out = cross_entropy_backward(t[0], t[1], t[2], t[3], t[4], t[5], grad, ctx->saved_data["ignore"].toInt(),
-                                                ctx->saved_data["smoothing"].toDouble(), (int)ctx->saved_data["reduction"].toInt(),
-                                                {ctx->needs_input_grad(0), ctx->needs_input_grad(1), t[2].defined() && ctx->needs_input_grad(2)});
-        return {out[0], out[1], out[2], Tensor(), Tensor(), Tensor(), Tensor()};
+        const auto out = cross_entropy_backward(x_, w_, b_, t_, stats, laid_out, grad, ignore, smoothing, reduction,
+                                                {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2)});
+        return {out[0], out[1], out[2]};
     }
+    void release_variables() override
+    {
+        std::lock_guard<std::mutex> hold(mutex_);
+        x.reset_data(), w.reset_data(), bias.reset_data(), target.reset_data();
+        stats.reset(), laid_out.reset();
+    }
+    std::string name() const override { return "LinearCrossEntropyBackward"; }
 };
+Tensor linear_cross_entropy(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &target, int64_t ignore, double smoothing, int reduction)
+{
+    Forward f = cross_entropy(x, w, bias, target, ignore, smoothing, reduction);
+    if (torch::autograd::compute_requires_grad(x, w, bias)) {
+        auto node = std::shared_ptr<LinearCrossEntropyBackward>(new LinearCrossEntropyBackward, torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(x, w, bias));
+        node->x = SavedVariable(x, false), node->w = SavedVariable(w, false), node->bias = SavedVariable(bias, false);
+        node->target = SavedVariable(target, false);
+        node->stats = f.stats, node->laid_out = f.laid_out;
+        node->ignore = ignore, node->smoothing = smoothing, node->reduction = reduction;
+        torch::autograd::set_history(f.loss, node);
+    }
+    return f.loss;
+}
 
 // ------------------------------------------------------------------------------------------------ balance of gates
 std::array<Tensor, 3> gate_balance(const Tensor &gate, const Tensor &indices, const Tensor &mask, int top_k)
@@ -184,24 +202,35 @@ Tensor gate_balance_backward(const Tensor &gate, const Tensor &mask, const Tenso
     return out;
 }
 
-struct GateBalance : torch::autograd::Function<GateBalance> {
-    static variable_list forward(AutogradContext *ctx, const Tensor &gate, const std::optional<Tensor> &indices, const std::optional<Tensor> &mask,
-                                 int64_t top_k)
-    {
-        const auto out = gate_balance(gate, indices.value_or(Tensor()), mask.value_or(Tensor()), (int)top_k);
-        ctx->save_for_backward({gate, mask.value_or(Tensor()), out[2]});
-        ctx->mark_non_differentiable({out[1]});
-        ctx->set_materialize_grads(false);
-        return {out[0], out[1]};
-    }
-    static variable_list backward(AutogradContext *ctx, variable_list grads)
+struct GateBalanceBackward : torch::autograd::Node {
+    SavedVariable gate, mask;
+    Tensor share;
+
+    variable_list apply(variable_list &&grads) override
     {
         no_second_order("gate_balance");
-        if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-        const variable_list t = ctx->get_saved_variables();
-        return {gate_balance_backward(t[0], t[1], t[2], grads[0]), Tensor(), Tensor(), Tensor()};
+        std::lock_guard<std::mutex> hold(mutex_);
+        const Tensor gate_ = gate.unpack(), mask_ = mask.unpack();
+        return {grads[0].defined() ? gate_balance_backward(gate_, mask_, share, grads[0]) : Tensor()};
     }
+    void release_variables() override
+    {
+        std::lock_guard<std::mutex> hold(mutex_);
+        gate.reset_data(), mask.reset_data(), share.reset();
+    }
+    std::string name() const override { return "GateBalanceBackward"; }
 };
+std::array<Tensor, 2> balance(const Tensor &gate, const Tensor &indices, const Tensor &mask, int top_k)
+{
+    auto out = gate_balance(gate, indices, mask, top_k);
+    if (torch::autograd::compute_requires_grad(gate)) {
+        auto node = std::shared_ptr<GateBalanceBackward>(new GateBalanceBackward, torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(gate));
+        node->gate = SavedVariable(gate, false), node->mask = SavedVariable(mask, false), node->share = out[2];
+        torch::autograd::set_history(out[0], node);
+    }
+    return {out[0], out[1]};
+}
 
 // ------------------------------------------------------------------------------------------------ AdamW
 // Weights of one type, device and count of steps, with the table the library reads.  Every step looks again at all that a program can
@@ -268,7 +297,6 @@ struct NoGil {
     PyThreadState *state = PyEval_SaveThread();
     ~NoGil() { PyEval_RestoreThread(state); }
 };
-std::optional<Tensor> given(const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
 Tensor tensor(PyObject *o)
 {
     if (o == Py_None) return Tensor();
@@ -361,7 +389,7 @@ PyObject *py_linear_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
         Tensor loss;
         {
             const NoGil no;
-            loss = LinearCrossEntropy::apply(x, w, given(b), t, ignore, smoothing, reduction);
+            loss = linear_cross_entropy(x, w, b, t, ignore, smoothing, (int)reduction);
         }
         return wrap(loss);
     });
@@ -409,10 +437,10 @@ PyObject *py_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
             (indices.defined() && (!plain_beside(indices, gate, at::kLong) || indices.dim() != 2 || indices.size(0) != gate.size(0) || indices.size(1) != top_k)) ||
             (mask.defined() && (!plain_beside(mask, gate, at::kBool) || mask.dim() != 1 || mask.size(0) != gate.size(0))))
             Py_RETURN_NONE;
-        variable_list out;
+        std::array<Tensor, 2> out;
         {
             const NoGil no;
-            out = GateBalance::apply(gate, given(indices), given(mask), top_k);
+            out = balance(gate, indices, mask, (int)top_k);
         }
         return tuple({out[0], out[1]});
     });
