@@ -451,3 +451,14 @@ def test_a_graph_is_used_once(dev):
     del both
     x.grad = None
     assert torch.cuda.memory_allocated() < used
+
+
+def test_forward_mode_is_refused(dev):
+    from torch.autograd import forward_ad
+    from vtpack_amd.layers import gate_balance, linear_cross_entropy
+    x, w, b, t = _operands(dev, 50, 60, 64, torch.float32)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: linear_cross_entropy(dual, w, b, t), lambda: gate_balance(dual)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()

@@ -133,6 +133,12 @@ void no_second_order(const char *name)
     if (at::GradMode::is_enabled()) throw std::runtime_error(std::string(name) + ": gradients of the gradients are not supported");
 }
 
+void no_forward_mode(const char *name, std::initializer_list<const Tensor *> operands)
+{
+    for (const Tensor *t : operands)
+        if (t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error(std::string(name) + ": forward-mode derivatives are not supported");
+}
+
 // The backward node of a loss, with what it reads as members.
 struct LinearCrossEntropyBackward : torch::autograd::Node {
     SavedVariable x, w, bias, target;
@@ -162,6 +168,7 @@ struct LinearCrossEntropyBackward : torch::autograd::Node {
 };
 Tensor linear_cross_entropy(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &target, int64_t ignore, double smoothing, int reduction)
 {
+    no_forward_mode("linear_cross_entropy", {&x, &w, &bias});
     Forward f = cross_entropy(x, w, bias, target, ignore, smoothing, reduction);
     if (torch::autograd::compute_requires_grad(x, w, bias)) {
         auto node = std::shared_ptr<LinearCrossEntropyBackward>(new LinearCrossEntropyBackward, torch::autograd::deleteNode);
@@ -222,6 +229,7 @@ struct GateBalanceBackward : torch::autograd::Node {
 };
 std::array<Tensor, 2> balance(const Tensor &gate, const Tensor &indices, const Tensor &mask, int top_k)
 {
+    no_forward_mode("gate_balance", {&gate});
     auto out = gate_balance(gate, indices, mask, top_k);
     if (torch::autograd::compute_requires_grad(gate)) {
         auto node = std::shared_ptr<GateBalanceBackward>(new GateBalanceBackward, torch::autograd::deleteNode);
