@@ -126,13 +126,9 @@ def test_arguments_of_the_native_module():
             getattr(native, name)(1)
     p = torch.nn.Parameter(x)
     with pytest.raises(RuntimeError, match="do not match"):
-        native.adamw_batch([p], [], ["exp_avg"])
-    with pytest.raises(RuntimeError, match="without its moments"):
-        native.adamw_batch([p], [{}], ["exp_avg"])
-    batch = native.adamw_batch([p], [{"exp_avg": x.clone(), "exp_avg_sq": x.clone()}], ["exp_avg", "exp_avg_sq"])
-    state = {p: {}}
-    assert native.adamw_step(batch, [p], state, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 32) is False       # another state, no gradient
+        native.adamw_batch([p], [], ["exp_avg", "exp_avg_sq"], 32)
+    with pytest.raises(RuntimeError, match="do not match"):
+        native.adamw_batch([p], [{}], ["exp_avg"], 8)
+    assert native.adamw_batch([p], [{"exp_avg": x.clone(), "exp_avg_sq": x.clone()}], ["exp_avg", "exp_avg_sq"], 32) is None    # on the CPU
     with pytest.raises((RuntimeError, ValueError)):
-        native.adamw_step(None, [p], state, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 32)
-    with pytest.raises(TypeError):
-        native.adamw_step(batch, [p], state, "lr", 0.9, 0.999, 1e-8, 0.0, 1, 32)
+        native.adamw_step(None, [p], {p: {}}, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 32)

@@ -16,6 +16,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <algorithm>
+#include <array>
 #include <map>
 #include <mutex>
 #include <memory>
@@ -479,31 +481,48 @@ PyObject *py_gate_balance_backward(PyObject *, PyObject *const *a, Py_ssize_t n)
     });
 }
 
-// (params, states, keys): lists of weights, of their states and of the names of the moments in them, scales behind
+// (params, states, keys, bits): lists of weights, of their states and of the names of the moments in them, scales behind -> a batch,
+// or None unless all is as a launch takes it: weights of one type on one GPU, dense and apart, moments and scales that fit them
 PyObject *py_adamw_batch(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
-    return call(a, n, 3, [&] {
+    return call(a, n, 4, [&]() -> PyObject * {
         auto b = std::make_unique<Batch>();
         b->params = held(a[0]), b->states = held(a[1]), b->keys = held(a[2]);
-        if (b->params.empty() || b->states.size() != b->params.size() || b->keys.size() > 4) throw std::runtime_error("adamw_batch: lists that do not match");
+        const bool bytes = whole(a[3]) == 8;
+        if (b->params.empty() || b->states.size() != b->params.size() || b->keys.size() != (bytes ? 4 : 2))
+            throw std::runtime_error("adamw_batch: lists that do not match");
+        const at::ScalarType types[4] = {bytes ? at::kFloat8_e4m3fn : at::kFloat, bytes ? at::kFloat8_e5m2 : at::kFloat, at::kFloat, at::kFloat};
+        std::vector<std::pair<uintptr_t, uintptr_t>> lie;
         for (size_t i = 0; i < b->params.size(); i++) {
             const Tensor p = tensor(b->params[i]);
-            vtdge_adamw_tensor x{};
+            if (i == 0) b->type = p.scalar_type();
+            const Tensor &first = i == 0 ? p : b->kept.front();
+            if (!p.defined() || !p.is_cuda() || p.layout() != at::kStrided || !p.is_contiguous() || p.scalar_type() != b->type ||
+                p.device() != first.device() || (b->type != at::kFloat && b->type != at::kBFloat16) || !PyDict_Check(b->states[i]))
+                Py_RETURN_NONE;
+            b->kept.push_back(p.detach());
             void *at[4] = {};
             for (size_t k = 0; k < b->keys.size(); k++) {
-                PyObject *const m = PyDict_GetItem(b->states[i], b->keys[k]);
-                if (m == nullptr || !THPVariable_Check(m)) throw std::runtime_error("adamw_batch: a state without its moments");
-                Py_INCREF(m);
-                b->moments.push_back(m);
-                b->kept.push_back(tensor(m).detach());
-                at[k] = b->kept.back().data_ptr();
+                PyObject *const o = PyDict_GetItem(b->states[i], b->keys[k]);
+                if (o == nullptr || !THPVariable_Check(o)) Py_RETURN_NONE;
+                const Tensor m = THPVariable_Unpack(o);
+                if (m.scalar_type() != types[k] || m.device() != p.device() || m.layout() != at::kStrided || !m.is_contiguous() ||
+                    (k < 2 ? m.sizes() != p.sizes() : m.dim() != 1 || m.numel() != (p.numel() + 255) / 256))
+                    Py_RETURN_NONE;
+                Py_INCREF(o);
+                b->moments.push_back(o);
+                b->kept.push_back(m.detach());
+                at[k] = m.data_ptr();
             }
-            b->kept.push_back(p.detach());
-            b->type = p.scalar_type();
+            vtdge_adamw_tensor x{};
             x.param = p.data_ptr(), x.n = p.numel();
             x.exp_avg = at[0], x.exp_avg_sq = at[1], x.exp_avg_scale = (float *)at[2], x.exp_avg_sq_scale = (float *)at[3];
             b->table.push_back(x);
+            if (x.n > 0) lie.emplace_back((uintptr_t)x.param, (uintptr_t)x.param + p.nbytes());
         }
+        std::sort(lie.begin(), lie.end());
+        for (size_t i = 1; i < lie.size(); i++)
+            if (lie[i].first < lie[i - 1].second) Py_RETURN_NONE;
         return PyCapsule_New(b.release(), BATCH, [](PyObject *o) { delete static_cast<Batch *>(PyCapsule_GetPointer(o, BATCH)); });
     });
 }

@@ -39,7 +39,6 @@ class _Batch:
         for column, moment in enumerate(self.moments):
             self.table[:, 2 + column] = [t.data_ptr() for t in moment]
         self.table[:, 6] = [p.numel() for p in params]
-        self.native = _lib.training().adamw_batch(params, states, list(self.keys)) if self.plain else None
 
     def holds(self):
         return (all(all(map(operator.is_, map(operator.itemgetter(k), self.states), old)) for k, old in zip(self.keys, self.moments))
@@ -91,17 +90,17 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"eps is {eps} and weight_decay {weight_decay}, expected 0 or more")
         if state_bits not in _KEYS:
             raise ValueError(f"state_bits is {state_bits}, expected 32 or 8")
-        self._batches = {}
+        self._batches, self._natives = {}, {}
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       capturable=capturable, step=0))
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._batches = {}
+        self._batches, self._natives = {}, {}
 
     def load_state_dict(self, state_dict):
         """As torch's, but moments keep the type they were saved in (torch casts them to the weight's)."""
-        self._batches = {}
+        self._batches, self._natives = {}, {}
         super().load_state_dict(state_dict)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
@@ -183,9 +182,9 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         for index, group in enumerate(self.param_groups):
-            if not capturing and self._same_again(index, group):
-                continue
             params = group["params"]
+            if not capturing and self._in_one_call(index, group, params):
+                continue
             grads = list(map(_grad, params))
             if capturing and not group["capturable"]:
                 raise RuntimeError("AdamW: a step that is captured needs capturable=True (its count of steps would stand still)")
@@ -195,6 +194,8 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 self._skip(index, [p for p, g in zip(group["params"], grads) if g is None], capturing)
                 grads = [g for g in grads if g is not None]
+            if not capturing and self._in_one_call(index, group, params, anew=True):
+                continue
             batches = self._of_group(index, group, params, grads)
             of = dict(zip(map(id, params), grads)) if len(batches) > 1 else None
             for i, b in enumerate(batches):
@@ -204,16 +205,29 @@ class AdamW(torch.optim.Optimizer):
             increment_version(params)
         return loss
 
-    def _same_again(self, index, group):
-        """The step of a group of which nothing has moved since its last one, in one call that looks it all over and launches."""
-        kept = self._batches.get(index)
-        if kept is None or len(kept[2]) != 1 or group["capturable"] or _lib.timer is not None:
+    def _in_one_call(self, index, group, params, anew=False):
+        """The step of a group's weights in one native call that looks all of them over and launches; False, and nothing done, where
+        something is not as it was when the call was prepared, which `anew` does again, or not as it takes it."""
+        if group["capturable"] or _lib.timer is not None:
             return False
-        b, (beta1, beta2) = kept[2][0], group["betas"]
-        if b.native is None or b.keys != _KEYS[group["state_bits"]]:
-            return False
-        if not _lib.training().adamw_step(b.native, group["params"], self.state, group["lr"], beta1, beta2, group["eps"], group["weight_decay"],
-                                          int(group["step"]) + 1 - b.skipped, group["state_bits"]):
+        native, bits = _lib.training(), group["state_bits"]
+        if anew:
+            for p in params:
+                ops._need_gpu(p)
+            states = [self.state[p] for p in params]
+            for p, state in zip(params, states):
+                if not any(k in state for k in _CODES):
+                    state.update(self._lay_out(p, bits, int(group["step"])))
+            skipped = {state.get("skipped", 0) for state in states}
+            batch = native.adamw_batch(params, states, list(_KEYS[bits]), bits) if len(skipped) == 1 else None
+            self._natives = {i: b for i, b in self._natives.items() if i != index}
+            if batch is None:
+                return False
+            self._natives[index] = (batch, skipped.pop(), bits)
+        batch, skipped, kept_bits = self._natives.get(index, (None, 0, 0))
+        beta1, beta2 = group["betas"]
+        if kept_bits != bits or not native.adamw_step(batch, params, self.state, group["lr"], beta1, beta2, group["eps"], group["weight_decay"],
+                                                      int(group["step"]) + 1 - skipped, bits):
             return False
         group["step"] += 1
         return True
@@ -226,6 +240,7 @@ class AdamW(torch.optim.Optimizer):
                     raise RuntimeError("AdamW: a weight that has taken steps has no gradient in the one that is captured")
                 self.state[p]["skipped"] = self.state[p].get("skipped", 0) + 1
                 self._batches.pop(index, None)
+                self._natives.pop(index, None)
 
     def _launch(self, group, batch, grads, last):
         (b1, b2), eps, decay = group["betas"], group["eps"], group["weight_decay"]
