@@ -472,3 +472,38 @@ def test_steps_leave_no_memory_behind(dev):
         gc.collect()
         used.append(torch.cuda.memory_allocated())
     assert used[-1] <= used[0]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_groups_that_are_looked_over_once(dev, bits, monkeypatch):
+    """A frozen weight among others, weights of other strides: what was found out about them is kept from step to step."""
+    from vtpack_amd import _lib, optim
+    shapes = [(300,), (40, 30), (77,)]
+    frozen = [torch.nn.Parameter(t) for t in _tensors(dev, shapes, torch.float32, 41)]
+    strided = [torch.nn.Parameter(_tensors(dev, [(30, 20)], torch.float32, 42)[0].t()), torch.nn.Parameter(_tensors(dev, [(50,)], torch.float32, 43)[0])]
+    refs = [_Reference(p if p.is_contiguous() else p.detach().t(), bits) for p in frozen + strided]
+    opt = _optimizer([{"params": frozen}, {"params": strided}], bits)
+    split, native = [], []
+    real, made = optim.AdamW._split, _lib.training().adamw_batch
+
+    class Native:
+        def __getattr__(self, name):
+            return getattr(real_native, name)
+
+        def adamw_batch(self, *args):
+            native.append(1)
+            return made(*args)
+
+    real_native, wrapped = _lib.training(), Native()
+    monkeypatch.setattr(_lib, "training", lambda: wrapped)
+    monkeypatch.setattr(optim.AdamW, "_split", lambda self, *args: split.append(1) or real(self, *args))
+    for k in range(4):
+        for i, (p, g) in enumerate(zip(frozen + strided, _tensors(dev, [p.shape for p in frozen + strided], torch.float32, 90 + k, 1e-3))):
+            p.grad = None if i == 1 else g.t().contiguous().t() if i == 3 else g
+        opt.step()
+        for p, r in zip(frozen + strided, refs):
+            if p.grad is not None:
+                flip = (lambda t: t) if p.is_contiguous() else (lambda t: t.t() if t.dim() == 2 else t)
+                r.step(flip(p.grad))
+                r.check(flip(p.detach()), {key: flip(t) for key, t in opt.state[p].items() if torch.is_tensor(t)})
+    assert len(native) == 2 and len(split) == 1

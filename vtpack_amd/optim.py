@@ -159,7 +159,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("AdamW: a capturable group keeps its count of steps on one device")
         return [_Batch(ps, [self.state[p] for p in ps], bits, skipped) for (_, _, skipped), ps in sets.items()]
 
-    def _of_group(self, index, group, params, grads):
+    def _held(self, index, group, params):
+        """The batches of the group's last step that was not one call, where they still hold."""
         kept = self._batches.get(index)
         if kept is not None:
             old, states, batches = kept
@@ -167,6 +168,9 @@ class AdamW(torch.optim.Optimizer):
             if (len(params) == len(old) and all(map(operator.is_, params, old)) and len(now) == len(states)
                     and all(map(operator.is_, now, states)) and all(b.holds() and b.keys == _KEYS[group["state_bits"]] for b in batches)):
                 return batches
+        return None
+
+    def _of_group(self, index, group, params, grads):
         batches = self._split(group, params, grads)
         self._batches = {i: b for i, b in self._batches.items() if i != index}
         self._batches[index] = (params, list(self.state.values()), batches)
@@ -194,9 +198,12 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 self._skip(index, [p for p, g in zip(group["params"], grads) if g is None], capturing)
                 grads = [g for g in grads if g is not None]
-            if not capturing and self._in_one_call(index, group, params, anew=True):
-                continue
-            batches = self._of_group(index, group, params, grads)
+            batches = self._held(index, group, params)
+            if batches is None:
+                if not capturing and (params is not group["params"] and self._in_one_call(index, group, params)
+                                      or self._in_one_call(index, group, params, anew=True)):
+                    continue
+                batches = self._of_group(index, group, params, grads)
             of = dict(zip(map(id, params), grads)) if len(batches) > 1 else None
             for i, b in enumerate(batches):
                 self._launch(group, b, grads if of is None else [of[id(p)] for p in b.params], i + 1 == len(batches))
