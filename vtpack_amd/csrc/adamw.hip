@@ -301,8 +301,8 @@ static OptScalars scalars_of(double lr, double beta1, double beta2, double eps, 
     return s;
 }
 
-__global__ void adamw_scalars_kernel(int64_t *step, int64_t skipped, int advance, const float *lr_dev, double lr, double beta1, double beta2, double eps, double decay,
-                                     OptScalars *out)
+__global__ void adamw_scalars_kernel(int64_t *step, int64_t skipped, int advance, const float *lr_dev, double lr, double beta1,
+                                     double beta2, double eps, double decay, OptScalars *out)
 {
     const int64_t t = *step + 1 - skipped;
     if (advance) *step += 1;

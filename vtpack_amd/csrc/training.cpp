@@ -444,7 +444,8 @@ PyObject *py_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
         const Tensor gate = tensor(a[0]), indices = tensor(a[1]), mask = tensor(a[2]);
         const int64_t top_k = whole(a[3]);
         if (!plain_rows(gate) || gate.size(1) > 512 || top_k < 1 || top_k > 512 || (!indices.defined() && top_k > gate.size(1)) ||
-            (indices.defined() && (!plain_beside(indices, gate, at::kLong) || indices.dim() != 2 || indices.size(0) != gate.size(0) || indices.size(1) != top_k)) ||
+            (indices.defined() && (!plain_beside(indices, gate, at::kLong) || indices.dim() != 2 || indices.size(0) != gate.size(0) ||
+                                   indices.size(1) != top_k)) ||
             (mask.defined() && (!plain_beside(mask, gate, at::kBool) || mask.dim() != 1 || mask.size(0) != gate.size(0))))
             Py_RETURN_NONE;
         std::array<Tensor, 2> out;
@@ -527,7 +528,7 @@ PyObject *py_adamw_batch(PyObject *, PyObject *const *a, Py_ssize_t n)
     });
 }
 // (batch, the group's weights, the optimizer's states, lr, beta1, beta2, eps, decay, step, bits): whether the step was made; if
-// not, something is not as it was and nothing was done
+// not, something is not as it was, or the stream is being captured, and nothing was done
 PyObject *py_adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 10, [&]() -> PyObject * {
@@ -539,10 +540,17 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
         if (!PyDict_Check(a[2]) || !ready(*b, a[1], a[2])) Py_RETURN_FALSE;
         const Tensor &first = THPVariable_Unpack(b->params[0]);
         const c10::DeviceGuard guard(first.device());
+        const c10::hip::HIPStream stream = c10::hip::getCurrentHIPStream(first.device().index());
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) {
+            (void)hipGetLastError();
+            Py_RETURN_FALSE;
+        }
+        if (status != hipStreamCaptureStatusNone) Py_RETURN_FALSE;
         {
             const NoGil no;
             must(lib.adamw(b->table.data(), (int)b->table.size(), rate[0], rate[1], rate[2], rate[3], rate[4], step, nullptr, code_of(first),
-                           (int)bits, stream_of(first)),
+                           (int)bits, stream.stream()),
                  "vtdge_adamw");
         }
         for (PyObject *p : b->params) THPVariable_Unpack(p).unsafeGetTensorImpl()->bump_version();
@@ -554,7 +562,8 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
 PyMethodDef methods[] = {VT_METHOD(bind), VT_METHOD(linear_cross_entropy), VT_METHOD(cross_entropy), VT_METHOD(cross_entropy_backward),
                          VT_METHOD(balance), VT_METHOD(gate_balance), VT_METHOD(gate_balance_backward), VT_METHOD(adamw_batch),
                          VT_METHOD(adamw_step), {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module = {PyModuleDef_HEAD_INIT, "_training", "The operators of a training step as torch calls them.", -1, methods, nullptr, nullptr, nullptr, nullptr};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_training", "The operators of a training step as torch calls them.", -1, methods,
+                      nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
 

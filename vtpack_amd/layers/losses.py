@@ -49,11 +49,12 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
 def gate_balance(gate, indices=None, top_k=1, mask=None):
     """How evenly a router's choices fall on its experts (here: granularities): -> (loss, counts).
 
-    gate [..., E] (2 .. 512 logits a token, float32 or bfloat16); loss = E sum_e f_e P_e in float32, f_e the fraction of the choices that
+    gate [..., E] (1 .. 512 logits a token, float32 or bfloat16); loss = E sum_e f_e P_e in float32, f_e the fraction of the choices that
     fell on e and P_e the mean softmax probability of e, with the gradient through P; counts int64 [E] are the choices.  1 is
     even, E is all on one.  The choices are the `top_k` largest logits of a token (among equals the lowest index), or `indices`
-    int64 [..., k] (or of gate's leading shape, k = 1) if they were made elsewhere, as by a Gumbel sample.  `mask` (bool, gate's leading shape): False leaves a token
-    out, whatever its logits are; a token whose logits are all -inf is left out too.  Without a token the loss is 0."""
+    int64 [..., k] (or of gate's leading shape, k = 1) if they were made elsewhere, as by a Gumbel sample; one that is no expert is
+    not counted.  `mask` (bool, gate's leading shape): False leaves a token out, whatever its logits are; a token whose logits are
+    all -inf is left out too.  Without a token the loss is 0."""
     out = _lib.training().balance(gate, indices, mask, top_k) if indices is None else None
     if out is not None:
         return out

@@ -177,18 +177,23 @@ class AdamW(torch.optim.Optimizer):
         return batches
 
     # ---------------------------------------------------------------- the step
-    @torch.no_grad()
     def step(self, closure=None):
         """One step over all weights that have a gradient.  `closure` (optional) works the loss out again and returns it."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        rest = [(i, g) for i, g in enumerate(self.param_groups) if not self._in_one_call(i, g, g["params"])]
+        if rest:
+            self._step_groups(rest)
+        return loss
+
+    @torch.no_grad()
+    def _step_groups(self, groups):
+        """The step of groups that have to be looked over."""
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
-        for index, group in enumerate(self.param_groups):
+        for index, group in groups:
             params = group["params"]
-            if not capturing and self._in_one_call(index, group, params):
-                continue
             grads = list(map(_grad, params))
             if capturing and not group["capturable"]:
                 raise RuntimeError("AdamW: a step that is captured needs capturable=True (its count of steps would stand still)")
@@ -210,7 +215,6 @@ class AdamW(torch.optim.Optimizer):
             if not group["capturable"]:
                 group["step"] += 1
             increment_version(params)
-        return loss
 
     def _in_one_call(self, index, group, params, anew=False):
         """The step of a group's weights in one native call that looks all of them over and launches; False, and nothing done, where
