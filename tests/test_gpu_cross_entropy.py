@@ -462,3 +462,21 @@ def test_forward_mode_is_refused(dev):
         for call in (lambda: linear_cross_entropy(dual, w, b, t), lambda: gate_balance(dual)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+@pytest.mark.parametrize("which", ["x", "weight"])
+def test_one_operand_is_laid_out(dev, which):
+    """bf16 operands of which one lies as the kernels read it and the other does not; rows left out hold NaN."""
+    from vtpack_amd import ops
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 300, 500, 128, torch.bfloat16, left_out=0.2)
+    x[t < 0] = float("nan")
+    want = [linear_cross_entropy(x, w, b, t), *_check(x, w, b, t)[1]]
+    place = torch.zeros(((300 if which == "x" else 500) * 128 + 1,), dtype=torch.bfloat16, device=dev)
+    place[1:] = (x if which == "x" else w).reshape(-1)
+    moved = place[1:].view(-1, 128)
+    xs, ws = (moved, w) if which == "x" else (x, moved)
+    loss, stats, laid_out = ops.cross_entropy(xs, ws, b, t)
+    assert laid_out is None and torch.equal(loss, want[0])
+    got = ops.cross_entropy_backward(xs, ws, b, t, stats, None, torch.ones((), device=dev))
+    assert all(torch.equal(p, q) for p, q in zip(got, want[1:]))

@@ -97,6 +97,10 @@ def test_workspaces_follow_the_sizes():
     lib = _lib.load()
     size = lib.vtdge_cross_entropy_workspace
     assert size(256, 1000, 384, 1, 0) % 256 == 0 and size(256, 1000, 384, 1, 0) < size(256, 1000, 384, 0, 0)
+    # operands that are read where they lie need no room: forward neither, for the gradients x all the same
+    full, x, w = size(256, 1000, 384, 1, 0), 256 * 384 * 2, 1000 * 384 * 2
+    assert full - size(256, 1000, 384, 1, 2) == x and full - size(256, 1000, 384, 1, 4) == w and full - size(256, 1000, 384, 1, 6) == x + w
+    assert size(256, 1000, 384, 1, 1) == size(256, 1000, 384, 1, 3) == size(256, 1000, 384, 1, 7) + w
     # d of a piece: no more than 320 MB, or 1024 classes, however many classes there are
     assert size(8192, 65536, 1024, 1, 1) < (320 << 20) + 2 * 65536 * 1024 * 2 + 3 * 8192 * 1024 * 4 + (8 << 20) * 4 * 2
     assert lib.vtdge_gate_balance_workspace(100, 8) == 0 and lib.vtdge_gate_balance_workspace(1 << 20, 8) == 256 * 17 * 4

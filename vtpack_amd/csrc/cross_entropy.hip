@@ -959,7 +959,8 @@ static bool large_logits(int64_t rows, int64_t classes, int padded)
     return rounds * (1.57 * slabs + 6.0) <= t * (1.98 * slabs + 3.5);
 }
 
-static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool backward)
+// (x_lies, w_lies: read where they lie, see lies_well; the gradients want room for x with zeros in any case)
+static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool backward, bool x_lies, bool w_lies)
 {
     CePlan p{};
     p.rows = rows, p.classes = classes, p.width = width, p.backward = backward;
@@ -980,8 +981,8 @@ static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool 
     else shape(LogitsLarge{}, LogitsMiddle{}, LogitsFlat{}, LogitsSmall{});
     p.tm = ceil_div(rows, p.lm), p.tn = ceil_div(classes, p.ln);
     int64_t at = 0;
-    p.x_at = take(at, rows * p.padded * 2 * p.parts);
-    p.w_at = take(at, classes * p.padded * 2 * p.parts);
+    p.x_at = take(at, x_lies && !backward ? 0 : rows * p.padded * 2 * p.parts);
+    p.w_at = take(at, w_lies ? 0 : classes * p.padded * 2 * p.parts);
     if (!backward) {
         p.max_at = take(at, p.tn * rows * 4);
         p.sum_at = take(at, p.tn * rows * 4);
@@ -1021,10 +1022,11 @@ static int check_sizes(const char *what, int64_t rows, int64_t classes, int widt
     } while (0)
 
 // whether the product routine can read an operand where it lies
-static bool lies_well(const void *src, int64_t ld, const CePlan &p)
+static bool lies_well(const void *src, int64_t ld, int width, int dtype)
 {
-    return !p.split && p.width == p.padded && ld % 8 == 0 && ld < (1 << 22) && ((uintptr_t)src & 15) == 0;
+    return dtype == VTDGE_BF16 && width % CE_PAD == 0 && ld % 8 == 0 && ld < (1 << 22) && ((uintptr_t)src & 15) == 0;
 }
+static bool lies_well(const void *src, int64_t ld, const CePlan &p) { return lies_well(src, ld, p.width, p.split ? VTDGE_F32 : VTDGE_BF16); }
 // x and W as they lie, else packed in the workspace; rows of x that are left out as zeros there
 static int operands_of(CeArgs &a, const void *x, int64_t ldx, const void *w, int64_t ldw, const CePlan &p, unsigned char *ws, hipStream_t st)
 {
@@ -1129,13 +1131,13 @@ using namespace vtdge;
 extern "C" int64_t vtdge_cross_entropy_laid_out(int64_t rows, int64_t classes, int width, int dtype)
 {
     if (check_sizes("cross_entropy_laid_out", rows, classes, width, dtype) != VTDGE_OK) return -1;
-    return plan_of(rows, classes, width, dtype, false).max_at;
+    return plan_of(rows, classes, width, dtype, false, false, false).max_at;
 }
 
-extern "C" int64_t vtdge_cross_entropy_workspace(int64_t rows, int64_t classes, int width, int dtype, int backward)
+extern "C" int64_t vtdge_cross_entropy_workspace(int64_t rows, int64_t classes, int width, int dtype, int how)
 {
     if (check_sizes("cross_entropy_workspace", rows, classes, width, dtype) != VTDGE_OK) return -1;
-    return plan_of(rows, classes, width, dtype, backward != 0).bytes;
+    return plan_of(rows, classes, width, dtype, how & VTDGE_CE_BACKWARD, how & VTDGE_CE_X_LIES, how & VTDGE_CE_WEIGHT_LIES).bytes;
 }
 
 extern "C" int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, const int64_t *target,
@@ -1148,7 +1150,7 @@ extern "C" int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weigh
     VT_REQUIRE(loss != nullptr || inv_count == nullptr, VTDGE_ERR_ARG, "cross_entropy: inv_count without loss");
     VT_REQUIRE(ldx >= width && ldw >= width, VTDGE_ERR_ARG, "cross_entropy: rows of %d, %lld and %lld apart", width, (long long)ldx, (long long)ldw);
     VT_REQUIRE(smoothing >= 0.f && smoothing <= 1.f, VTDGE_ERR_ARG, "cross_entropy: smoothing %g", (double)smoothing);
-    const CePlan p = plan_of(rows, classes, width, dtype, false);
+    const CePlan p = plan_of(rows, classes, width, dtype, false, lies_well(x, ldx, width, dtype), lies_well(weight, ldw, width, dtype));
     VT_REQUIRE(workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG, "cross_entropy: workspace of %lld bytes, %lld needed",
                (long long)workspace_bytes, (long long)p.bytes);
     unsigned char *const ws = (unsigned char *)workspace;
@@ -1195,7 +1197,8 @@ extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const vo
     VT_REQUIRE(((uintptr_t)laid_out & 255) == 0, VTDGE_ERR_ARG, "cross_entropy_backward: laid_out off its boundary");
     VT_REQUIRE(grad_stride == 0 || (grad_stride == 1 && inv_count == nullptr), VTDGE_ERR_ARG, "cross_entropy_backward: grad_stride %d", grad_stride);
     VT_REQUIRE(smoothing >= 0.f && smoothing <= 1.f, VTDGE_ERR_ARG, "cross_entropy_backward: smoothing %g", (double)smoothing);
-    const CePlan p = plan_of(rows, classes, width, dtype, true);
+    const bool x_lies = lies_well(x, ldx, width, dtype), w_lies = lies_well(weight, ldw, width, dtype);
+    const CePlan p = plan_of(rows, classes, width, dtype, true, x_lies, w_lies);
     VT_REQUIRE(workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG,
                "cross_entropy_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.bytes);
     if (dx == nullptr && dweight == nullptr && dbias == nullptr) return VTDGE_OK;
@@ -1204,15 +1207,16 @@ extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const vo
     CeArgs a{};
     a.target = target, a.ignore = ignore_index;
     if (laid_out != nullptr) {
-        // as the forward call left them: both plans begin alike
+        // as the forward call left them
         unsigned char *const from = (unsigned char *)const_cast<void *>(laid_out);
-        a.x = lies_well(x, ldx, p) ? Operand{(const bf16_t *)x, ldx, 0} : Operand{(const bf16_t *)(from + p.x_at), p.padded, rows * p.padded};
-        a.w = lies_well(weight, ldw, p) ? Operand{(const bf16_t *)weight, ldw, 0} : Operand{(const bf16_t *)(from + p.w_at), p.padded, classes * p.padded};
+        const CePlan f = plan_of(rows, classes, width, dtype, false, x_lies, w_lies);
+        a.x = x_lies ? Operand{(const bf16_t *)x, ldx, 0} : Operand{(const bf16_t *)(from + f.x_at), p.padded, rows * p.padded};
+        a.w = w_lies ? Operand{(const bf16_t *)weight, ldw, 0} : Operand{(const bf16_t *)(from + f.w_at), p.padded, classes * p.padded};
     } else {
         VT_STEP(operands_of(a, x, ldx, weight, ldw, p, ws, st));
     }
     Operand clean = a.x;                            // x with zeros for the rows that are left out, so that what they hold reaches no gradient
-    const bool copy = lies_well(x, ldx, p) && (dweight != nullptr || dbias != nullptr);
+    const bool copy = x_lies && (dweight != nullptr || dbias != nullptr);
     if (copy) clean = Operand{(const bf16_t *)(ws + p.x_at), p.padded, 0};
     a.bias = bias, a.bias_f32 = p.split, a.rows = rows, a.classes = classes;
     a.smoothing = smoothing, a.stages = (int)ceil_div(p.padded, p.slab_l), a.width = p.padded;

@@ -79,11 +79,20 @@ enum Reduction { NONE, MEAN, SUM };
 constexpr int64_t KEEP_LAID_OUT = 128 << 20;    // bytes
 
 struct Rows {
-    int64_t rows, classes; int width, dtype;
-    Rows(const Tensor &x, const Tensor &w) : rows(x.size(0)), classes(w.size(0)), width((int)x.size(1)), dtype(code_of(x)) {}
+    int64_t rows, classes; int width, dtype, lie;
+    Rows(const Tensor &x, const Tensor &w)
+        : rows(x.size(0)), classes(w.size(0)), width((int)x.size(1)), dtype(code_of(x)),
+          lie((lies(x) ? VTDGE_CE_X_LIES : 0) + (lies(w) ? VTDGE_CE_WEIGHT_LIES : 0)) {}
+    // whether the kernels read an operand where it lies
+    bool lies(const Tensor &t) const
+    {
+        const int64_t pitch = pitch_of(t);
+        return dtype == VTDGE_BF16 && width % 64 == 0 && pitch % 8 == 0 && pitch < (1 << 22) && (uintptr_t)t.data_ptr() % 16 == 0;
+    }
     int64_t workspace(bool backward) const
     {
-        return bytes_of<5>({rows, classes, width, dtype, backward}, [&] { return lib.cross_entropy_workspace(rows, classes, width, dtype, backward); });
+        const int how = lie + (backward ? VTDGE_CE_BACKWARD : 0);
+        return bytes_of<5>({rows, classes, width, dtype, how}, [&] { return lib.cross_entropy_workspace(rows, classes, width, dtype, how); });
     }
     // Operands that do not lie as the kernels read them were laid out in the workspace, which is kept for the gradients (fp32 1 x 363 x
     // 25766: 20 us of 136 for laying them out again); larger ones are laid out again there, so that no memory waits between the calls.
