@@ -619,21 +619,23 @@ int vtdge_gate_balance_backward(const void *gate, int64_t pitch, const uint8_t *
  * _backward, of grad * loss_rows summed over the rows:
  *   grad      fp32, one value for each row (grad_stride 1) or one for all (0), times inv_count[0] where that is given
  *   dx [rows, width], dweight [classes, width], dbias [classes]: dense, of `dtype`, each nullable
- *   laid_out  nullable: the workspace of the forward call on the same operands, as that call left it; what it laid out of
- *             them (its first vtdge_cross_entropy_laid_out bytes) is not laid out again
+ *   laid_out  nullable: the workspace of the forward call on the same operands, with `keeps`, as that call left it; what it
+ *             laid out of them and the logits that it kept (fp32, up to 256 MB), its first vtdge_cross_entropy_laid_out bytes at
+ *             most, are not worked out again
  * fp32 operands are multiplied as exactly as fp32 products are, on the bf16 matrix instructions.
  *   workspace  vtdge_cross_entropy_workspace(..., how) bytes, 256-byte aligned, contents do not matter.  how: a sum of
- *             VTDGE_CE_BACKWARD, for the gradients, and VTDGE_CE_X_LIES, VTDGE_CE_WEIGHT_LIES, for operands that are read where
+ *             VTDGE_CE_BACKWARD, for the gradients, VTDGE_CE_KEEPS, for a forward call with `keeps`, and VTDGE_CE_X_LIES, VTDGE_CE_WEIGHT_LIES, for operands that are read where
  *             they lie and need no room: bf16, width a multiple of 64, rows a multiple of 8 elements and less than 2^22 apart,
  *             on a 16-byte boundary */
 #define VTDGE_CE_BACKWARD 1
 #define VTDGE_CE_X_LIES 2
 #define VTDGE_CE_WEIGHT_LIES 4
+#define VTDGE_CE_KEEPS 8
 int64_t vtdge_cross_entropy_laid_out(int64_t rows, int64_t classes, int width, int dtype);
 int64_t vtdge_cross_entropy_workspace(int64_t rows, int64_t classes, int width, int dtype, int how);
 int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, const int64_t *target,
                         int64_t rows, int64_t classes, int width, int64_t ignore_index, float smoothing, void *workspace,
-                        int64_t workspace_bytes, float *loss_rows, float *row_max, float *row_inv, float *loss,
+                        int64_t workspace_bytes, int keeps, float *loss_rows, float *row_max, float *row_inv, float *loss,
                         float *inv_count, int dtype, void *stream);
 int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias,
                                  const int64_t *target, const float *row_max, const float *row_inv, const float *grad,

@@ -301,9 +301,13 @@ def test_shapes_of_tiles(dev, dtype, rows, classes, width, logits, grads):
     x, w, b, t = _operands(dev, rows, classes, width, dtype, left_out=0.1)
     loss, stats, laid_out = ops.cross_entropy(x, w, b, t)
     assert any(f"cross_entropy_tiles_kernel<vtdge::{logits}, false>" in _lib.last_kernel(k) for k in range(3))
-    ops.cross_entropy_backward(x, w, b, t, stats, laid_out, torch.ones((), device=dev))
+    one = torch.ones((), device=dev)
+    again = ops.cross_entropy_backward(x, w, b, t, stats, None, one)
     used = [_lib.last_kernel(k) for k in range(3)]
     assert any(f"cross_entropy_grad_kernel<vtdge::{grads} >" in n for n in used) and any(f"cross_entropy_d_kernel<vtdge::{logits} >" in n for n in used)
+    kept = ops.cross_entropy_backward(x, w, b, t, stats, laid_out, one)
+    assert (dtype == torch.float32) == any("cross_entropy_d_kept_kernel" in _lib.last_kernel(k) for k in range(3))
+    assert all(torch.equal(p, q) for p, q in zip(again, kept))
     _check(x, w, b, t, smoothing=0.1)
 
 

@@ -50,7 +50,7 @@ def test_arguments_of_the_library():
     """Before anything is launched."""
     lib = _lib.load()
     p = 4096                                              # never read: the sizes are refused first
-    ce = [p, 8, p, 8, p, p, 4, 3, 8, -100, 0.0, p, 1 << 40, p, p, p, p, p, 0, None]
+    ce = [p, 8, p, 8, p, p, 4, 3, 8, -100, 0.0, p, 1 << 40, 0, p, p, p, p, p, 0, None]
 
     def call(**put):
         args = list(ce)
@@ -59,14 +59,14 @@ def test_arguments_of_the_library():
         return lib.vtdge_cross_entropy(*args)
 
     assert call(_0=None) == _lib.ERR_ARG and b"NULL" in lib.vtdge_last_error()
-    assert call(_18=7) == _lib.ERR_ARG                    # type
+    assert call(_19=7) == _lib.ERR_ARG                    # type
     assert call(_1=7) == _lib.ERR_ARG                     # rows that overlap
     assert call(_6=0) == _lib.ERR_ARG and call(_7=0) == _lib.ERR_ARG and call(_8=0) == _lib.ERR_ARG
     assert call(_6=1 << 24) == _lib.ERR_UNSUPPORTED and call(_8=(1 << 16) + 1) == _lib.ERR_UNSUPPORTED
     assert call(_10=1.5) == _lib.ERR_ARG and call(_10=float("nan")) == _lib.ERR_ARG
     assert call(_12=0) == _lib.ERR_ARG and b"workspace" in lib.vtdge_last_error()
     assert call(_11=p + 16) == _lib.ERR_ARG               # a workspace off its boundary
-    assert call(_16=None) == _lib.ERR_ARG                 # a count of rows without their mean
+    assert call(_17=None) == _lib.ERR_ARG                 # a count of rows without their mean
     assert lib.vtdge_cross_entropy_workspace(4, 3, 0, 0, 0) == -1
     back = [p, 8, p, 8, p, p, p, p, p, 1, p, 4, 3, 8, -100, 0.0, None, p, 1 << 40, p, p, p, 0, None]
     assert lib.vtdge_cross_entropy_backward(*back) == _lib.ERR_ARG and b"grad_stride" in lib.vtdge_last_error()
@@ -101,6 +101,9 @@ def test_workspaces_follow_the_sizes():
     full, x, w = size(256, 1000, 384, 1, 0), 256 * 384 * 2, 1000 * 384 * 2
     assert full - size(256, 1000, 384, 1, 2) == x and full - size(256, 1000, 384, 1, 4) == w and full - size(256, 1000, 384, 1, 6) == x + w
     assert size(256, 1000, 384, 1, 1) == size(256, 1000, 384, 1, 3) == size(256, 1000, 384, 1, 7) + w
+    # kept logits: fp32, up to 256 MB
+    assert size(256, 1001, 384, 0, 8) - size(256, 1001, 384, 0, 0) == 256 * 1008 * 4 and size(256, 1001, 384, 1, 8) == size(256, 1001, 384, 1, 0)
+    assert size(1024, 65537, 64, 0, 8) == size(1024, 65537, 64, 0, 0) and size(1024, 65536, 64, 0, 8) - size(1024, 65536, 64, 0, 0) == 256 << 20
     # d of a piece: no more than 320 MB, or 1024 classes, however many classes there are
     assert size(8192, 65536, 1024, 1, 1) < (320 << 20) + 2 * 65536 * 1024 * 2 + 3 * 8192 * 1024 * 4 + (8 << 20) * 4 * 2
     assert lib.vtdge_gate_balance_workspace(100, 8) == 0 and lib.vtdge_gate_balance_workspace(1 << 20, 8) == 256 * 17 * 4

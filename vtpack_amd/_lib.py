@@ -91,7 +91,7 @@ SIGNATURES = {
     "vtdge_block_tail": [_p, _p, _p, _p, _p, _p, _f, _p, _p, _p, _p, _p, _p, _l, _i, _i, _i, _p],
     "vtdge_gate_balance": [_p, _l, _p, _p, _l, _i, _i, _p, _l, _p, _p, _p, _i, _p],
     "vtdge_gate_balance_backward": [_p, _l, _p, _p, _p, _p, _l, _i, _i, _p],
-    "vtdge_cross_entropy": [_p, _l, _p, _l, _p, _p, _l, _l, _i, _l, _f, _p, _l, _p, _p, _p, _p, _p, _i, _p],
+    "vtdge_cross_entropy": [_p, _l, _p, _l, _p, _p, _l, _l, _i, _l, _f, _p, _l, _i, _p, _p, _p, _p, _p, _i, _p],
     "vtdge_cross_entropy_backward": [_p, _l, _p, _l, _p, _p, _p, _p, _p, _i, _p, _l, _l, _i, _l, _f, _p, _p, _l, _p, _p, _p,
                                      _i, _p],
     "vtdge_adamw": [_p, _i, _d, _d, _d, _d, _d, _l, _p, _i, _i, _p],

@@ -229,6 +229,7 @@ struct CeArgs {
     bool stream_w;                                  // forward, few rows: W past the caches
     // forward: [class tiles][rows] each
     float *tile_max, *tile_sum, *tile_total, *target_z;
+    float *z; int64_t z_pitch;                      // nullable: the logits times log2 e, kept for the gradients; -inf behind the last class
     // backward
     const float *row_max, *row_inv, *row_scale; bf16_t *d; int64_t d_pitch, d_plane;
     bf16_t *x_copy; int width;                      // nullable: x with zeros for the rows that are left out
@@ -289,6 +290,21 @@ template <class S, bool TOTAL> __device__ __forceinline__ void logits_tile(const
     b.stream = p.stream_w;
     multiply_tile<S, false>(a, b, 0, p.stages, smem, acc, false, none);
     logits<S>(bias + wn * 32 * JN, acc);
+    if (S::PARTS > 1 && p.z != nullptr) {
+#pragma unroll
+        for (int i = 0; i < IM; i++) {
+            const int64_t r = r0 + (wm * IM + i) * 32 + lr;
+            if (r >= p.rows) continue;
+#pragma unroll
+            for (int j = 0; j < JN; j++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int64_t c = cw + j * 32 + 8 * q + 4 * lg;
+                    if (c < p.z_pitch)
+                        *reinterpret_cast<f32x4 *>(p.z + r * p.z_pitch + c) = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                }
+        }
+    }
     float *const shared = reinterpret_cast<float *>(smem);          // [waves along the classes][largest, sum, total][rows]
 #pragma unroll
     for (int i = 0; i < IM; i++) {
@@ -622,6 +638,41 @@ template <class S> __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void cr
     }
 }
 
+// The same from kept logits, in three parts: a lane has eight classes of a row, `vecs` of them side by side and `rows` rows to be written.
+__global__ __launch_bounds__(256) void cross_entropy_d_kept_kernel(CeArgs p, int vecs, int64_t rows)
+{
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, row = id / (uint32_t)vecs;
+    const int64_t r = row;
+    if (r >= rows) return;
+    const int64_t c = (int64_t)(id - row * (uint32_t)vecs) * 8, v = p.v0 + c, at = r < p.rows ? r : p.rows - 1, t = p.target[at];
+    const bool live = r < p.rows && counts(t, p.ignore, p.classes);
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) f[e] = 0.f;
+    if (live && v < p.v1) {
+        const float g = p.row_scale != nullptr ? p.row_scale[at] : 1.f, top = p.row_max[at], inv = p.row_inv[at] * g;
+        const float minus = -(p.smoothing / (float)p.classes) * g, one = (1.f - p.smoothing) * g;
+        const f32x4 a = *reinterpret_cast<const f32x4 *>(p.z + r * p.z_pitch + v), b = *reinterpret_cast<const f32x4 *>(p.z + r * p.z_pitch + v + 4);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            f[e] = __builtin_fmaf(__builtin_amdgcn_exp2f((e < 4 ? a[e & 3] : b[e & 3]) - top), inv, minus);
+            if (v + e == t) f[e] -= one;
+            if (v + e >= p.v1) f[e] = 0.f;
+        }
+    }
+    bf16_t *const to = p.d + r * p.d_pitch + c;
+#pragma unroll
+    for (int part = 0; part < 3; part++) {
+        u32x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            o[e] = pack_bf16x2(f[2 * e], f[2 * e + 1]);
+            f[2 * e] -= bf16lo(o[e]), f[2 * e + 1] -= bf16hi(o[e]);
+        }
+        *reinterpret_cast<u32x4 *>(to + part * p.d_plane) = o;
+    }
+}
+
 // ---- out = A B, dx = d W or dW = d^T x, over a dimension that may be cut into several parts, which leave sums of their own
 struct GradArgs {
     Operand a, b;
@@ -855,6 +906,7 @@ using SplitGradSmall = Shape<1, 1, 2, 2, 32, 3, 3>;
 
 constexpr int CE_PAD = 64;                          // rows of operands are filled up to whole slabs of any shape
 constexpr int64_t CE_PIECE_BYTES = 320ll << 20;     // of d
+constexpr int64_t CE_KEPT_BYTES = 256ll << 20;      // of logits
 enum { CE_LARGE, CE_MIDDLE, CE_FLAT, CE_SMALL };
 
 // Everything a call lays out, the same for the size and the call.
@@ -867,7 +919,7 @@ struct CePlan {
     int64_t piece, d_rows;                          // classes of a piece, rows of d
     int dx_splits, dw_splits;
     // bytes of the workspace
-    int64_t x_at, w_at, max_at, sum_at, total_at, z_at, d_at, dx_at, dw_at, db_at, bytes;
+    int64_t x_at, w_at, kept_at, max_at, sum_at, total_at, z_at, d_at, dx_at, dw_at, db_at, bytes;
 };
 
 static int64_t part_of(int64_t n) { return (n + 63) / 64 * 64; }      // elements from one part of a sum to the next
@@ -959,8 +1011,13 @@ static bool large_logits(int64_t rows, int64_t classes, int padded)
     return rounds * (1.57 * slabs + 6.0) <= t * (1.98 * slabs + 3.5);
 }
 
+// Logits of fp32 operands stay for the gradients where they are no more than 256 MB: six products of parts cost more than their way to
+// memory and back.  (bf16: one product, which costs as much.)
+static int64_t z_pitch(int64_t classes) { return (classes + 7) / 8 * 8; }
+static bool keeps_logits(int64_t rows, int64_t classes, int dtype) { return dtype == VTDGE_F32 && rows * z_pitch(classes) * 4 <= CE_KEPT_BYTES; }
+
 // (x_lies, w_lies: read where they lie, see lies_well; the gradients want room for x with zeros in any case)
-static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool backward, bool x_lies, bool w_lies)
+static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool backward, bool x_lies, bool w_lies, bool keeps)
 {
     CePlan p{};
     p.rows = rows, p.classes = classes, p.width = width, p.backward = backward;
@@ -983,6 +1040,7 @@ static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool 
     int64_t at = 0;
     p.x_at = take(at, x_lies && !backward ? 0 : rows * p.padded * 2 * p.parts);
     p.w_at = take(at, w_lies ? 0 : classes * p.padded * 2 * p.parts);
+    p.kept_at = take(at, keeps && keeps_logits(rows, classes, dtype) ? rows * z_pitch(classes) * 4 : 0);
     if (!backward) {
         p.max_at = take(at, p.tn * rows * 4);
         p.sum_at = take(at, p.tn * rows * 4);
@@ -1082,6 +1140,15 @@ template <class S> static int go_d(const CeArgs &a, const CePlan &p, hipStream_t
     kern<<<(unsigned)(2 * p.tm * tn - whole), S::THREADS, S::LDS, st>>>(a, (int)p.tm, tn, whole);
     return check_launch("cross_entropy_backward");
 }
+static int go_d_kept(const CeArgs &a, hipStream_t st)
+{
+    // slabs run over the classes of a piece and the rows behind the last, 64 at most
+    const int64_t vecs = ceil_div(a.v1 - a.v0, 256) * 32, rows = ceil_div(a.rows, CE_PAD) * CE_PAD, blocks = ceil_div(rows * vecs, 256);
+    VT_REQUIRE(blocks < (1 << 24) && vecs * 8 <= a.d_pitch, VTDGE_ERR_UNSUPPORTED, "cross_entropy_backward: d of %lld blocks", (long long)blocks);
+    note_kernel(reinterpret_cast<const void *>(cross_entropy_d_kept_kernel));
+    cross_entropy_d_kept_kernel<<<(unsigned)blocks, 256, 0, st>>>(a, (int)vecs, rows);
+    return check_launch("cross_entropy_backward");
+}
 template <class S> static int go_grad(GradPair &g, hipStream_t st)
 {
     int64_t blocks = 0;
@@ -1131,26 +1198,26 @@ using namespace vtdge;
 extern "C" int64_t vtdge_cross_entropy_laid_out(int64_t rows, int64_t classes, int width, int dtype)
 {
     if (check_sizes("cross_entropy_laid_out", rows, classes, width, dtype) != VTDGE_OK) return -1;
-    return plan_of(rows, classes, width, dtype, false, false, false).max_at;
+    return plan_of(rows, classes, width, dtype, false, false, false, true).max_at;
 }
 
 extern "C" int64_t vtdge_cross_entropy_workspace(int64_t rows, int64_t classes, int width, int dtype, int how)
 {
     if (check_sizes("cross_entropy_workspace", rows, classes, width, dtype) != VTDGE_OK) return -1;
-    return plan_of(rows, classes, width, dtype, how & VTDGE_CE_BACKWARD, how & VTDGE_CE_X_LIES, how & VTDGE_CE_WEIGHT_LIES).bytes;
+    return plan_of(rows, classes, width, dtype, how & VTDGE_CE_BACKWARD, how & VTDGE_CE_X_LIES, how & VTDGE_CE_WEIGHT_LIES, how & VTDGE_CE_KEEPS).bytes;
 }
 
 extern "C" int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, const int64_t *target,
                                    int64_t rows, int64_t classes, int width, int64_t ignore_index, float smoothing, void *workspace,
-                                   int64_t workspace_bytes, float *loss_rows, float *row_max, float *row_inv, float *loss, float *inv_count,
-                                   int dtype, void *stream)
+                                   int64_t workspace_bytes, int keeps, float *loss_rows, float *row_max, float *row_inv, float *loss,
+                                   float *inv_count, int dtype, void *stream)
 {
     VT_STEP(check_sizes("cross_entropy", rows, classes, width, dtype));
     VT_REQUIRE(x && weight && target && loss_rows && row_max && row_inv && workspace, VTDGE_ERR_ARG, "cross_entropy: NULL operand");
     VT_REQUIRE(loss != nullptr || inv_count == nullptr, VTDGE_ERR_ARG, "cross_entropy: inv_count without loss");
     VT_REQUIRE(ldx >= width && ldw >= width, VTDGE_ERR_ARG, "cross_entropy: rows of %d, %lld and %lld apart", width, (long long)ldx, (long long)ldw);
     VT_REQUIRE(smoothing >= 0.f && smoothing <= 1.f, VTDGE_ERR_ARG, "cross_entropy: smoothing %g", (double)smoothing);
-    const CePlan p = plan_of(rows, classes, width, dtype, false, lies_well(x, ldx, width, dtype), lies_well(weight, ldw, width, dtype));
+    const CePlan p = plan_of(rows, classes, width, dtype, false, lies_well(x, ldx, width, dtype), lies_well(weight, ldw, width, dtype), keeps != 0);
     VT_REQUIRE(workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG, "cross_entropy: workspace of %lld bytes, %lld needed",
                (long long)workspace_bytes, (long long)p.bytes);
     unsigned char *const ws = (unsigned char *)workspace;
@@ -1162,6 +1229,7 @@ extern "C" int vtdge_cross_entropy(const void *x, int64_t ldx, const void *weigh
     a.smoothing = smoothing, a.stages = (int)ceil_div(p.padded, p.slab_l), a.v0 = 0, a.v1 = classes;
     a.tile_max = (float *)(ws + p.max_at), a.tile_sum = (float *)(ws + p.sum_at), a.tile_total = (float *)(ws + p.total_at);
     a.target_z = (float *)(ws + p.z_at);
+    if (keeps != 0 && keeps_logits(rows, classes, dtype)) a.z = (float *)(ws + p.kept_at), a.z_pitch = z_pitch(classes);
     // W is read once where it lies.  From a quarter of the last cache's 256 MB on, what a program does between two calls leaves little of
     // it there (1 x 1024 x 65536, 134 MB: out of memory 27.4 us through the caches, 24.7 past them; still in the cache 25.5 and 27.1)
     a.stream_w = p.logits == CE_FLAT && a.w.p == weight && classes * p.padded * 2 >= (64 << 20);
@@ -1198,7 +1266,7 @@ extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const vo
     VT_REQUIRE(grad_stride == 0 || (grad_stride == 1 && inv_count == nullptr), VTDGE_ERR_ARG, "cross_entropy_backward: grad_stride %d", grad_stride);
     VT_REQUIRE(smoothing >= 0.f && smoothing <= 1.f, VTDGE_ERR_ARG, "cross_entropy_backward: smoothing %g", (double)smoothing);
     const bool x_lies = lies_well(x, ldx, width, dtype), w_lies = lies_well(weight, ldw, width, dtype);
-    const CePlan p = plan_of(rows, classes, width, dtype, true, x_lies, w_lies);
+    const CePlan p = plan_of(rows, classes, width, dtype, true, x_lies, w_lies, false);
     VT_REQUIRE(workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG,
                "cross_entropy_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.bytes);
     if (dx == nullptr && dweight == nullptr && dbias == nullptr) return VTDGE_OK;
@@ -1209,7 +1277,8 @@ extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const vo
     if (laid_out != nullptr) {
         // as the forward call left them
         unsigned char *const from = (unsigned char *)const_cast<void *>(laid_out);
-        const CePlan f = plan_of(rows, classes, width, dtype, false, x_lies, w_lies);
+        const CePlan f = plan_of(rows, classes, width, dtype, false, x_lies, w_lies, true);
+        if (keeps_logits(rows, classes, dtype)) a.z = (float *)(from + f.kept_at), a.z_pitch = z_pitch(classes);
         a.x = x_lies ? Operand{(const bf16_t *)x, ldx, 0} : Operand{(const bf16_t *)(from + f.x_at), p.padded, rows * p.padded};
         a.w = w_lies ? Operand{(const bf16_t *)weight, ldw, 0} : Operand{(const bf16_t *)(from + f.w_at), p.padded, classes * p.padded};
     } else {
@@ -1231,7 +1300,8 @@ extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const vo
         a.v0 = v0, a.v1 = v0 + p.piece < classes ? v0 + p.piece : classes;
         a.x_copy = copy && v0 == 0 ? (bf16_t *)(ws + p.x_at) : nullptr;
         const int64_t live = a.v1 - a.v0;
-        if (p.split) VT_STEP(p.logits == CE_LARGE ? go_d<SplitLarge>(a, p, st) : p.logits == CE_FLAT ? go_d<SplitFlat>(a, p, st) : go_d<SplitSmall>(a, p, st));
+        if (a.z != nullptr) VT_STEP(go_d_kept(a, st));
+        else if (p.split) VT_STEP(p.logits == CE_LARGE ? go_d<SplitLarge>(a, p, st) : p.logits == CE_FLAT ? go_d<SplitFlat>(a, p, st) : go_d<SplitSmall>(a, p, st));
         else VT_STEP(p.logits == CE_LARGE ? go_d<LogitsLarge>(a, p, st) : p.logits == CE_MIDDLE ? go_d<LogitsMiddle>(a, p, st) : p.logits == CE_FLAT ? go_d<LogitsFlat>(a, p, st) : go_d<LogitsSmall>(a, p, st));
         GradPair g{};
         g.scale = scale, g.scale2 = inv_count, g.f32 = p.split;

@@ -76,7 +76,7 @@ template <size_t N, class F> int64_t bytes_of(const std::array<int64_t, N> &key,
 
 // ------------------------------------------------------------------------------------------------ cross entropy
 enum Reduction { NONE, MEAN, SUM };
-constexpr int64_t KEEP_LAID_OUT = 128 << 20;    // bytes
+constexpr int64_t KEEP_LAID_OUT = 320 << 20;    // bytes
 
 struct Rows {
     int64_t rows, classes; int width, dtype, lie;
@@ -89,34 +89,37 @@ struct Rows {
         const int64_t pitch = pitch_of(t);
         return dtype == VTDGE_BF16 && width % 64 == 0 && pitch % 8 == 0 && pitch < (1 << 22) && (uintptr_t)t.data_ptr() % 16 == 0;
     }
-    int64_t workspace(bool backward) const
+    int64_t workspace(bool backward, bool keeps) const
     {
-        const int how = lie + (backward ? VTDGE_CE_BACKWARD : 0);
+        const int how = lie + (backward ? VTDGE_CE_BACKWARD : 0) + (keeps ? VTDGE_CE_KEEPS : 0);
         return bytes_of<5>({rows, classes, width, dtype, how}, [&] { return lib.cross_entropy_workspace(rows, classes, width, dtype, how); });
     }
-    // Operands that do not lie as the kernels read them were laid out in the workspace, which is kept for the gradients (fp32 1 x 363 x
-    // 25766: 20 us of 136 for laying them out again); larger ones are laid out again there, so that no memory waits between the calls.
+    // Operands that do not lie as the kernels read them are laid out in the workspace, with the logits in fp32.  It is kept for the
+    // gradients (fp32 1 x 363 x 25766: 20 us of 136 for laying them out again) up to this size, so that no more memory waits between
+    // the calls; behind it all is worked out again.
     bool keeps() const { return (dtype != VTDGE_BF16 || width % 64 != 0) && lib.cross_entropy_laid_out(rows, classes, width, dtype) <= KEEP_LAID_OUT; }
 };
 
 struct Forward {
     Tensor loss, stats, laid_out;
 };
-Forward cross_entropy(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &target, int64_t ignore, double smoothing, int reduction)
+Forward cross_entropy(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &target, int64_t ignore, double smoothing, int reduction,
+                      bool for_gradients)
 {
     const c10::DeviceGuard guard(x.device());
     const Rows s(x, w);
-    Tensor ws = fresh(x, {s.workspace(false)}, at::kByte);
+    const bool keeps = for_gradients && s.keeps();
+    Tensor ws = fresh(x, {s.workspace(false, keeps)}, at::kByte);
     // the rows' largest logits, 1 / sums, 1 / the number of rows that count, the rows' losses; the loss is memory of its own, for a
     // caller to change in place
     const Tensor stats = fresh(x, {3 * s.rows + 1}, at::kFloat);
     const Tensor loss = reduction == NONE ? fresh(x, {s.rows}, at::kFloat) : fresh(x, {}, at::kFloat);
     float *const at = stats.data_ptr<float>(), *const out = loss.data_ptr<float>();
     must(lib.cross_entropy(x.data_ptr(), pitch_of(x), w.data_ptr(), pitch_of(w), at_of(bias), target.data_ptr<int64_t>(), s.rows, s.classes, s.width,
-                           ignore, (float)smoothing, ws.data_ptr(), ws.numel(), reduction == NONE ? out : at + 2 * s.rows + 1, at, at + s.rows,
+                           ignore, (float)smoothing, ws.data_ptr(), ws.numel(), keeps, reduction == NONE ? out : at + 2 * s.rows + 1, at, at + s.rows,
                            reduction == NONE ? nullptr : out, reduction == MEAN ? at + 2 * s.rows : nullptr, s.dtype, stream_of(x)),
          "vtdge_cross_entropy");
-    return {loss, stats, s.keeps() ? ws : Tensor()};
+    return {loss, stats, keeps ? ws : Tensor()};
 }
 
 std::array<Tensor, 3> cross_entropy_backward(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &target, const Tensor &stats,
@@ -125,7 +128,7 @@ std::array<Tensor, 3> cross_entropy_backward(const Tensor &x, const Tensor &w, c
 {
     const c10::DeviceGuard guard(x.device());
     const Rows s(x, w);
-    const Tensor ws = fresh(x, {s.workspace(true)}, at::kByte);
+    const Tensor ws = fresh(x, {s.workspace(true, false)}, at::kByte);
     std::array<Tensor, 3> out;
     if (needs[0]) out[0] = fresh(x, {s.rows, s.width}, x.scalar_type());
     if (needs[1]) out[1] = fresh(x, {s.classes, s.width}, x.scalar_type());
@@ -180,8 +183,9 @@ struct LinearCrossEntropyBackward : torch::autograd::Node {
 Tensor linear_cross_entropy(const Tensor &x, const Tensor &w, const Tensor &bias, const Tensor &target, int64_t ignore, double smoothing, int reduction)
 {
     no_forward_mode("linear_cross_entropy", {&x, &w, &bias});
-    Forward f = cross_entropy(x, w, bias, target, ignore, smoothing, reduction);
-    if (torch::autograd::compute_requires_grad(x, w, bias)) {
+    const bool trains = torch::autograd::compute_requires_grad(x, w, bias);
+    Forward f = cross_entropy(x, w, bias, target, ignore, smoothing, reduction, trains);
+    if (trains) {
         auto node = std::shared_ptr<LinearCrossEntropyBackward>(new LinearCrossEntropyBackward, torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(x, w, bias));
         node->x = SavedVariable(x, false), node->w = SavedVariable(w, false), node->bias = SavedVariable(bias, false);
@@ -422,7 +426,7 @@ PyObject *py_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
         Forward f;
         {
             const NoGil no;
-            f = cross_entropy(x, w, b, t, ignore, smoothing, (int)reduction);
+            f = cross_entropy(x, w, b, t, ignore, smoothing, (int)reduction, true);
         }
         return tuple({f.loss, f.stats, f.laid_out});
     });
