@@ -3,7 +3,7 @@
 //   z = x W^T + b,   loss_r = log sum_v exp z_rv - (1 - eps) z_rt - eps mean_v z_rv
 //   d_rv = g_r (exp(z_rv) / sum - (1 - eps) [v = t_r] - eps / classes),   dx = d W,   dW = d^T x,   db = sum_r d_r
 //
-// z is never in memory.  Forward, every workgroup multiplies a tile of rows by a tile of classes and keeps of it each row's largest
+// z is not in memory (for fp32 gradients, see keeps_logits).  Forward, every workgroup multiplies a tile of rows by a tile of classes and keeps of it each row's largest
 // z and the sum of exp(z - largest); a second kernel joins the tiles of a row.  Backward, the classes are taken in pieces: the
 // tiles of a piece are multiplied again, d is rounded to bf16 (an error of half a step on each of many terms, as on any bf16
 // operand; the sums over it are fp32) and kept for this piece only, and two products take it to dx and dW.  Four products of
@@ -18,10 +18,10 @@
 // instructions.  (Two fp16 parts and three products would be 22 bits of a row's largest value and fewer of its small ones.)
 //
 // Bound by the matrix units in long products: 8192 rows x 65536 classes x 1024 in bf16, tiles 0.98 ms (1.12 PFLOP/s), d 4 x 0.29 (0.94,
-// with the writing of d), gradients 4 x 0.51 (1.07); in fp32 2048 x 21841 x 384, tiles 0.21 ms (166 TFLOP/s of fp32, 1.0 PFLOP/s issued), d
-// 0.26, gradients 0.39.  Their units are busy for 57 percent at the 1.7 - 1.9 GHz that the clock falls to, waves wait for them half of the
+// with the writing of d), gradients 4 x 0.51 (1.07); in fp32 2048 x 21841 x 384, tiles 0.21 ms (166 TFLOP/s of fp32, 1.0 PFLOP/s issued; 0.24
+// with the logits kept), d 0.07 from those, gradients 0.39.  Their units are busy for 57 percent at the 1.7 - 1.9 GHz that the clock falls to, waves wait for them half of the
 // time.  By the reading of W where rows are few (1 row x 65536 x 1024 in 21.6 us, 6.2 TB/s), by launches where all is small (256 x 1000 x
-// 384: five kernels of 6 - 10 us).
+// 384: four kernels of 6 - 9 us).
 #include "common.h"
 
 #include <math.h>
@@ -1012,7 +1012,8 @@ static bool large_logits(int64_t rows, int64_t classes, int padded)
 }
 
 // Logits of fp32 operands stay for the gradients where they are no more than 256 MB: six products of parts cost more than their way to
-// memory and back.  (bf16: one product, which costs as much.)
+// memory and back (2048 x 384 x 21841, 179 MB: d 70 us from them and 246 from products, 35 us more for the forward call's writing;
+// 2000 x 64 x 20000 64 and 79, 22 more).  bf16: one product, which costs as much.
 static int64_t z_pitch(int64_t classes) { return (classes + 7) / 8 * 8; }
 static bool keeps_logits(int64_t rows, int64_t classes, int dtype) { return dtype == VTDGE_F32 && rows * z_pitch(classes) * 4 <= CE_KEPT_BYTES; }
 

@@ -6,7 +6,8 @@ from .. import _lib, ops
 
 
 def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoothing=0.0, reduction="mean"):
-    """`F.cross_entropy(F.linear(x, weight, bias), target, ...)` with its gradients, without the logits in memory.
+    """`F.cross_entropy(F.linear(x, weight, bias), target, ...)` with its gradients, without the logits in memory (see below for
+    float32).
 
     x [..., width], weight [classes, width], bias [classes] or None, all float32 or all bfloat16; target int64 of x's leading
     shape.  -> float32: the mean over the rows that count ("mean"), their sum ("sum"), or every row's own ("none", of target's
