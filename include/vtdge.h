@@ -608,7 +608,7 @@ int vtdge_gate_balance(const void *gate, int64_t pitch, const int64_t *indices, 
 int vtdge_gate_balance_backward(const void *gate, int64_t pitch, const uint8_t *mask, const float *share,
                                 const float *grad_loss, void *grad, int64_t tokens, int E, int dtype, void *stream);
 
-/* Softmax cross entropy of a Linear's outputs, z = x weight^T + bias over `classes`, without z in memory:
+/* Softmax cross entropy of a Linear's outputs, z = x weight^T + bias over `classes`, without z in memory (but see `keeps`):
  *   loss_rows[r] = logsumexp_v z[r, v] - (1 - smoothing) z[r, target[r]] - smoothing mean_v z[r, v]
  *   x [rows, width], ldx elements between rows; weight [classes, width], ldw; bias nullable [classes]; target int64 [rows]
  *   Rows whose target is ignore_index, or no class, are left out: their loss is 0, and so is what they add to any gradient,
