@@ -1013,7 +1013,8 @@ static bool large_logits(int64_t rows, int64_t classes, int padded)
 
 // Logits of fp32 operands stay for the gradients where they are no more than 256 MB: six products of parts cost more than their way to
 // memory and back (2048 x 384 x 21841, 179 MB: d 70 us from them and 246 from products, 35 us more for the forward call's writing;
-// 2000 x 64 x 20000 64 and 79, 22 more).  bf16: one product, which costs as much.
+// 2000 x 64 x 20000 64 and 79, 22 more).  bf16: one product, which costs as
+// much (2999 x 768 x 21841, 262 MB: tiles 145 us and 190 with the writing, d 150 and 77; a call 460 and 464).
 static int64_t z_pitch(int64_t classes) { return (classes + 7) / 8 * 8; }
 static bool keeps_logits(int64_t rows, int64_t classes, int dtype) { return dtype == VTDGE_F32 && rows * z_pitch(classes) * 4 <= CE_KEPT_BYTES; }
 
