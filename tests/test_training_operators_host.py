@@ -139,3 +139,48 @@ def test_arguments_of_the_native_module():
     assert native.adamw_batch([p], [{"exp_avg": x.clone(), "exp_avg_sq": x.clone()}], ["exp_avg", "exp_avg_sq"], 32) is None    # on the CPU
     with pytest.raises((RuntimeError, ValueError)):
         native.adamw_step(None, [p], {p: {}}, 1e-3, 0.9, 0.999, 1e-8, 0.0, 1, 32)
+
+
+def _plain_calls():
+    """The native calls that take operands as they are: (name, operands that fit one another but for their place)."""
+    x, w, b, t = torch.randn(4, 8), torch.randn(3, 8), torch.randn(3), torch.zeros(4, dtype=torch.int64)
+    stats, one, share = torch.zeros(13), torch.ones(()), torch.zeros(9)
+    kept = torch.zeros(_lib.load().vtdge_cross_entropy_laid_out(4, 3, 8, 0), dtype=torch.uint8)
+    return {"cross_entropy": [x, w, b, t, -100, 0.1, 1],
+            "cross_entropy_backward": [x, w, b, t, stats, kept, one, -100, 0.1, 1, 1, 1, 1],
+            "gate_balance": [x, torch.zeros((4, 2), dtype=torch.int64), torch.ones(4, dtype=torch.bool), 2],
+            "gate_balance_backward": [x, torch.ones(4, dtype=torch.bool), share, one]}
+
+
+@pytest.mark.parametrize("name", ["cross_entropy", "cross_entropy_backward", "gate_balance", "gate_balance_backward"])
+def test_operands_of_the_plain_calls(name):
+    """Each operand that does not fit is named before anything is launched; the place is looked at last, so that the rest shows here."""
+    call = getattr(_lib.training(), name)
+    args = _plain_calls()[name]
+    with pytest.raises(RuntimeError, match=f"^{name}: .* GPU"):
+        call(*args)
+    half, longs, flat = torch.randn(4, 8).half(), torch.zeros((4, 8), dtype=torch.int64), torch.randn(32)
+    strided, empty = torch.randn(4, 16)[:, ::2], torch.randn(0, 8)
+    rows = [half, longs, flat, strided, empty, "x", None]
+    bad = {"cross_entropy": {0: rows, 1: rows + [torch.randn(3, 9), torch.randn(3, 8).bfloat16()], 2: [torch.randn(2), torch.randn(3).bfloat16(), torch.randn(6)[::2]],
+                             3: [torch.zeros(3, dtype=torch.int64), torch.zeros(4, dtype=torch.int32), torch.zeros((4, 1), dtype=torch.int64), None],
+                             5: [-0.1, 1.5, float("nan")], 6: [3, -1]},
+           "gate_balance": {0: rows + [torch.randn(4, 513)], 1: [torch.zeros((4, 3), dtype=torch.int64), torch.zeros((3, 2), dtype=torch.int64), torch.zeros((4, 2), dtype=torch.int32)],
+                            2: [torch.ones(3, dtype=torch.bool), torch.ones(4), torch.ones(4, 1, dtype=torch.bool)], 3: [0, 3, 513]},
+           "gate_balance_backward": {0: rows, 1: [torch.ones(3, dtype=torch.bool), torch.ones(4)], 2: [torch.zeros(8), torch.zeros(9).double(), torch.zeros(18)[::2], None],
+                                     3: [torch.ones(2), torch.ones((), dtype=torch.float64), None]}}
+    bad["cross_entropy_backward"] = {**{i: bad["cross_entropy"][i] for i in range(4)}, 4: [torch.zeros(12), torch.zeros(14), torch.zeros(13).double(), torch.zeros(26)[::2], None],
+                                     5: [args[5][1:] if name == "cross_entropy_backward" else None, torch.zeros(1 << 16)], 6: [torch.ones(4), torch.ones(3), torch.ones((), dtype=torch.bfloat16), None],
+                                     8: [-0.1, 1.5], 9: [3, -1]}
+    for at, values in bad[name].items():
+        for v in values:
+            with pytest.raises((RuntimeError, TypeError, ValueError), match=f"^{name}: (?!.*GPU)"):
+                call(*args[:at], v, *args[at + 1:])
+    if name == "gate_balance":
+        with pytest.raises((RuntimeError, ValueError), match="^gate_balance: .*top_k"):
+            call(args[0], None, None, 9)
+    if name == "cross_entropy_backward":                   # a value for each row goes with a loss for each
+        with pytest.raises(RuntimeError, match=f"^{name}: .* GPU"):
+            call(*args[:6], torch.ones(4), *args[7:9], 0, *args[10:])
+        with pytest.raises(RuntimeError, match=f"^{name}: (?!.*GPU)"):
+            call(*args[:6], torch.ones(3), *args[7:9], 0, *args[10:])

@@ -385,11 +385,12 @@ PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t n)
 // Operands as the kernels take them.  The entry points below answer None to any other, for their callers to bring them into this
 // form or to say what is wrong with them.
 bool number(PyObject *o) { return PyLong_Check(o) || PyFloat_Check(o); }
-bool plain_rows(const Tensor &t)
+bool rows_of_any_place(const Tensor &t)
 {
-    return t.defined() && t.is_cuda() && t.dim() == 2 && t.numel() > 0 && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) &&
+    return t.defined() && t.dim() == 2 && t.numel() > 0 && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) &&
            t.layout() == at::kStrided && (t.is_contiguous() || (t.stride(1) == 1 && t.stride(0) >= t.size(1)));
 }
+bool plain_rows(const Tensor &t) { return t.defined() && t.is_cuda() && rows_of_any_place(t); }
 bool plain_beside(const Tensor &t, const Tensor &x, at::ScalarType type)
 {
     return t.defined() && t.device() == x.device() && t.scalar_type() == type && t.layout() == at::kStrided && t.is_contiguous();
@@ -417,12 +418,54 @@ PyObject *py_linear_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
         return wrap(loss);
     });
 }
+
+// The calls below take their operands as they are: one that does not fit is named before anything is launched, the place of all of them
+// last.
+struct Operands {
+    const char *name;
+    void need(bool fits, const char *what) const
+    {
+        if (!fits) throw std::runtime_error(std::string(name) + ": " + what);
+    }
+    Tensor get(PyObject *o, const char *what) const
+    {
+        need(o == Py_None || THPVariable_Check(o), what);
+        return tensor(o);
+    }
+    void on_gpu(const Tensor &x) const { need(x.is_cuda(), "operands have to be on a GPU"); }
+
+    // x, weight, bias or None, target; the rest of a loss
+    std::array<Tensor, 4> of_loss(PyObject *const *a, double smoothing, int64_t reduction) const
+    {
+        const Tensor x = get(a[0], "x has to be a tensor"), w = get(a[1], "weight has to be a tensor"), b = get(a[2], "bias has to be a tensor or None"),
+                     t = get(a[3], "target has to be a tensor");
+        need(rows_of_any_place(x), "x has to be [rows, width] of float32 or bfloat16 with dense rows");
+        need(rows_of_any_place(w) && w.device() == x.device() && w.scalar_type() == x.scalar_type() && w.size(1) == x.size(1),
+             "weight has to be [classes, width] beside x, of its type, with dense rows");
+        need(!b.defined() || (plain_beside(b, x, x.scalar_type()) && b.dim() == 1 && b.size(0) == w.size(0)), "bias has to be [classes] beside x, of its type, dense");
+        need(plain_beside(t, x, at::kLong) && t.dim() == 1 && t.size(0) == x.size(0), "target has to be int64 [rows] beside x, dense");
+        need(smoothing >= 0 && smoothing <= 1, "label_smoothing has to be 0 .. 1");
+        need(reduction >= NONE && reduction <= SUM, "no such reduction");
+        return {x, w, b, t};
+    }
+    // gate and mask or None
+    std::array<Tensor, 2> of_gate(PyObject *gate, PyObject *mask) const
+    {
+        const Tensor g = get(gate, "gate has to be a tensor"), m = get(mask, "mask has to be a tensor or None");
+        need(rows_of_any_place(g) && g.size(1) <= VTDGE_MAX_EXPERTS, "gate has to be [tokens, 1 .. 512] of float32 or bfloat16 with dense rows");
+        need(!m.defined() || ((plain_beside(m, g, at::kBool) || plain_beside(m, g, at::kByte)) && m.dim() == 1 && m.size(0) == g.size(0)),
+             "mask has to be [tokens] of bytes beside the gate, dense");
+        return {g, m};
+    }
+};
 PyObject *py_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 7, [&] {
-        const Tensor x = tensor(a[0]), w = tensor(a[1]), b = tensor(a[2]), t = tensor(a[3]);
+        const Operands check{"cross_entropy"};
         const int64_t ignore = whole(a[4]), reduction = whole(a[6]);
         const double smoothing = real(a[5]);
+        const auto [x, w, b, t] = check.of_loss(a, smoothing, reduction);
+        check.on_gpu(x);
         Forward f;
         {
             const NoGil no;
@@ -434,15 +477,24 @@ PyObject *py_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
 PyObject *py_cross_entropy_backward(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 13, [&] {
-        Tensor t[7];
-        for (int i = 0; i < 7; i++) t[i] = tensor(a[i]);
+        const Operands check{"cross_entropy_backward"};
         const int64_t ignore = whole(a[7]), reduction = whole(a[9]);
         const double smoothing = real(a[8]);
         const std::array<bool, 3> needs = {whole(a[10]) != 0, whole(a[11]) != 0, whole(a[12]) != 0};
+        const auto [x, w, b, t] = check.of_loss(a, smoothing, reduction);
+        const Tensor stats = check.get(a[4], "stats has to be a tensor"), laid_out = check.get(a[5], "laid_out has to be a tensor or None"),
+                     grad = check.get(a[6], "grad has to be a tensor");
+        check.need(plain_beside(stats, x, at::kFloat) && stats.dim() == 1 && stats.size(0) == 3 * x.size(0) + 1, "stats has to be that of the forward call");
+        check.need(!laid_out.defined() || (plain_beside(laid_out, x, at::kByte) &&
+                                           laid_out.numel() >= lib.cross_entropy_laid_out(x.size(0), w.size(0), Rows(x, w).width, code_of(x))),
+                   "laid_out has to be that of the forward call");
+        check.need(plain_beside(grad, x, at::kFloat) && (grad.dim() == 0 || (grad.dim() == 1 && reduction == NONE && grad.size(0) == x.size(0))),
+                   "grad has to be float32 beside x: a scalar, or with a loss for each row a value for each");
+        check.on_gpu(x);
         std::array<Tensor, 3> out;
         {
             const NoGil no;
-            out = cross_entropy_backward(t[0], t[1], t[2], t[3], t[4], t[5], t[6], ignore, smoothing, (int)reduction, needs);
+            out = cross_entropy_backward(x, w, b, t, stats, laid_out, grad, ignore, smoothing, (int)reduction, needs);
         }
         return tuple({out[0], out[1], out[2]});
     });
@@ -472,8 +524,14 @@ PyObject *py_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
 PyObject *py_gate_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 4, [&] {
-        const Tensor gate = tensor(a[0]), indices = tensor(a[1]), mask = tensor(a[2]);
+        const Operands check{"gate_balance"};
         const int64_t top_k = whole(a[3]);
+        const auto [gate, mask] = check.of_gate(a[0], a[2]);
+        const Tensor indices = check.get(a[1], "indices have to be a tensor or None");
+        check.need(top_k >= 1 && top_k <= (indices.defined() ? VTDGE_MAX_EXPERTS : gate.size(1)), "top_k has to be 1 .. the number of logits");
+        check.need(!indices.defined() || (plain_beside(indices, gate, at::kLong) && indices.dim() == 2 && indices.size(0) == gate.size(0) && indices.size(1) == top_k),
+                   "indices have to be int64 [tokens, top_k] beside the gate, dense");
+        check.on_gpu(gate);
         std::array<Tensor, 3> out;
         {
             const NoGil no;
@@ -485,7 +543,14 @@ PyObject *py_gate_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
 PyObject *py_gate_balance_backward(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 4, [&] {
-        const Tensor gate = tensor(a[0]), mask = tensor(a[1]), share = tensor(a[2]), grad = tensor(a[3]);
+        const Operands check{"gate_balance_backward"};
+        const auto [gate, mask] = check.of_gate(a[0], a[1]);
+        const Tensor share = check.get(a[2], "share has to be a tensor"), grad = check.get(a[3], "grad has to be a tensor");
+        check.need(plain_beside(share, gate, at::kFloat) && share.dim() == 1 &&
+                       share.size(0) == lib.gate_balance_workspace(gate.size(0), (int)gate.size(1)) / 4 + gate.size(1) + 1,
+                   "share has to be that of the forward call");
+        check.need(plain_beside(grad, gate, at::kFloat) && grad.dim() == 0, "grad has to be a float32 scalar beside the gate");
+        check.on_gpu(gate);
         Tensor out;
         {
             const NoGil no;
