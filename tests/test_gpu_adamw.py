@@ -507,3 +507,31 @@ def test_groups_that_are_looked_over_once(dev, bits, monkeypatch):
                 r.step(flip(p.grad))
                 r.check(flip(p.detach()), {key: flip(t) for key, t in opt.state[p].items() if torch.is_tensor(t)})
     assert len(native) == 2 and len(split) == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_another_tensor_at_the_same_address(dev, bits):
+    """Weights and moments whose storage is given up and taken again, as others of other sizes and types: found or refused."""
+    flat = torch.randn(2048, device=dev)
+    p, q = torch.nn.Parameter(flat[:1024]), torch.nn.Parameter(torch.randn(1024, device=dev).view(32, 32).t())
+    opt = _optimizer([{"params": [p]}, {"params": [q]}], bits)
+    for x in (p, q):
+        x.grad = torch.full_like(x, 1e-3)
+    opt.step()
+    opt.step()
+    for x in (p, q):                                       # half of the weight, its states as they were
+        kept, moment = x.data, opt.state[x]["exp_avg"].data
+        x.data = x.data[:x.shape[0] // 2]
+        x.grad = torch.full_like(x, 1e-3)
+        whole = kept.clone()
+        with pytest.raises(ValueError):
+            opt.step()
+        assert torch.equal(kept, whole)
+        x.data = kept
+        x.grad = torch.full_like(x, 1e-3)
+        if bits == 32:                                     # the moment's memory under another type
+            opt.state[x]["exp_avg"].data = moment.view(torch.int32)
+            with pytest.raises(ValueError):
+                opt.step()
+            opt.state[x]["exp_avg"].data = moment
+    opt.step()

@@ -184,3 +184,25 @@ def test_operands_of_the_plain_calls(name):
             call(*args[:6], torch.ones(4), *args[7:9], 0, *args[10:])
         with pytest.raises(RuntimeError, match=f"^{name}: (?!.*GPU)"):
             call(*args[:6], torch.ones(3), *args[7:9], 0, *args[10:])
+
+
+@pytest.mark.parametrize("change", ["half", "transposed", "type", "moment", "scale"])
+def test_a_table_of_weights_holds_for_their_memory_alone(change):
+    """The same address under another size, order or type is another weight."""
+    from vtpack_amd.optim import _Batch
+    p = torch.nn.Parameter(torch.randn(32, 32))
+    state = {k: torch.zeros(32, 32) for k in ("exp_avg", "exp_avg_sq")}
+    state.update({k + "_scale": torch.zeros(4) for k in ("exp_avg", "exp_avg_sq")})
+    batch = _Batch([p], [state], 8, 0)
+    assert batch.holds()
+    if change == "half":
+        p.data = p.data[:16]
+    elif change == "transposed":
+        p.data = p.data.t()
+    elif change == "type":
+        state["exp_avg"].data = state["exp_avg"].data.view(torch.int32)
+    elif change == "moment":
+        state["exp_avg"].data = state["exp_avg"].data.view(-1)
+    else:
+        state["exp_avg_sq_scale"].data = state["exp_avg_sq_scale"].data[:3]
+    assert not batch.holds()

@@ -262,7 +262,7 @@ struct Batch {
     std::vector<PyObject *> params, states, moments, keys;      // moments: keys.size() of them for each state; all held
     std::vector<Tensor> kept;                   // no other storage can come to lie where a weight or a moment is
     std::vector<vtdge_adamw_tensor> table;
-    at::ScalarType type;
+    at::ScalarType type, types[4];              // of the weights; of the moments
     ~Batch()
     {
         for (auto *list : {&params, &states, &moments, &keys})
@@ -304,7 +304,9 @@ bool ready(Batch &b, PyObject *params, PyObject *state)
         const void *const lies[4] = {row.exp_avg, row.exp_avg_sq, row.exp_avg_scale, row.exp_avg_sq_scale};
         for (size_t k = 0; k < of; k++) {
             PyObject *const m = b.moments[i * of + k];
-            if (PyDict_GetItem(b.states[i], b.keys[k]) != m || THPVariable_Unpack(m).data_ptr() != lies[k]) return false;
+            if (PyDict_GetItem(b.states[i], b.keys[k]) != m) return false;
+            const Tensor &t = THPVariable_Unpack(m);
+            if (t.data_ptr() != lies[k] || t.numel() != (k < 2 ? row.n : (row.n + 255) / 256) || t.scalar_type() != b.types[k] || !t.is_contiguous()) return false;
         }
         const Tensor &p = THPVariable_Unpack(b.params[i]), &g = p.grad();
         if (p.data_ptr() != row.param || p.numel() != row.n || p.scalar_type() != b.type || !p.is_contiguous() || !g.defined() ||
@@ -560,6 +562,23 @@ PyObject *py_gate_balance_backward(PyObject *, PyObject *const *a, Py_ssize_t n)
     });
 }
 
+// (list of tensors) -> bytes that are the same while every one has the same memory, type, sizes and strides
+PyObject *py_places(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return call(a, n, 1, [&]() -> PyObject * {
+        if (!PyList_Check(a[0])) throw std::runtime_error("places: expected a list of tensors");
+        std::vector<int64_t> out;
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[0]); i++) {
+            const Tensor t = tensor(PyList_GET_ITEM(a[0], i));
+            if (!t.defined() || t.layout() != at::kStrided) throw std::runtime_error("places: expected a list of strided tensors");
+            out.insert(out.end(), {(int64_t)(uintptr_t)t.data_ptr(), (int64_t)t.scalar_type(), (int64_t)t.device().type(), (int64_t)t.device().index(), t.dim()});
+            out.insert(out.end(), t.sizes().begin(), t.sizes().end());
+            out.insert(out.end(), t.strides().begin(), t.strides().end());
+        }
+        return PyBytes_FromStringAndSize(reinterpret_cast<const char *>(out.data()), (Py_ssize_t)(out.size() * sizeof(int64_t)));
+    });
+}
+
 // (params, states, keys, bits): lists of weights, of their states and of the names of the moments in them, scales behind -> a batch,
 // or None unless all is as a launch takes it: weights of one type on one GPU, dense and apart, moments and scales that fit them
 PyObject *py_adamw_batch(PyObject *, PyObject *const *a, Py_ssize_t n)
@@ -570,7 +589,8 @@ PyObject *py_adamw_batch(PyObject *, PyObject *const *a, Py_ssize_t n)
         const bool bytes = whole(a[3]) == 8;
         if (b->params.empty() || b->states.size() != b->params.size() || b->keys.size() != (bytes ? 4 : 2))
             throw std::runtime_error("adamw_batch: lists that do not match");
-        const at::ScalarType types[4] = {bytes ? at::kFloat8_e4m3fn : at::kFloat, bytes ? at::kFloat8_e5m2 : at::kFloat, at::kFloat, at::kFloat};
+        at::ScalarType *const types = b->types;
+        types[0] = bytes ? at::kFloat8_e4m3fn : at::kFloat, types[1] = bytes ? at::kFloat8_e5m2 : at::kFloat, types[2] = types[3] = at::kFloat;
         std::vector<std::pair<uintptr_t, uintptr_t>> lie;
         for (size_t i = 0; i < b->params.size(); i++) {
             const Tensor p = tensor(b->params[i]);
@@ -638,7 +658,7 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
 
 #define VT_METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {VT_METHOD(bind), VT_METHOD(linear_cross_entropy), VT_METHOD(cross_entropy), VT_METHOD(cross_entropy_backward),
-                         VT_METHOD(balance), VT_METHOD(gate_balance), VT_METHOD(gate_balance_backward), VT_METHOD(adamw_batch),
+                         VT_METHOD(balance), VT_METHOD(gate_balance), VT_METHOD(gate_balance_backward), VT_METHOD(places), VT_METHOD(adamw_batch),
                          VT_METHOD(adamw_step), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_training", "The operators of a training step as torch calls them.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -25,24 +25,26 @@ def _same_layout(a, b):
 
 class _Batch:
     """Weights of one type, device and count of steps, as the rows of the table the library reads.  Every step looks again at all
-    that a program can put in another's place: the weights' storage, the tensors in `state`, the gradients."""
+    that a program can put in another's place: the weights' memory, type, sizes and strides, the tensors in `state` and theirs, the
+    gradients."""
 
     def __init__(self, params, states, bits, skipped):
         self.params, self.states, self.skipped, self.keys = params, states, skipped, _KEYS[bits]
         self.moments = [[s[k] for s in states] for k in self.keys]
-        self.kept = [t.detach() for t in itertools.chain(params, *self.moments)]      # no other storage can come to lie where one of these is
-        self.at = [t.data_ptr() for t in self.kept]
+        self.tensors = list(itertools.chain(params, *self.moments))
+        self.kept = [t.detach() for t in self.tensors]         # no other storage can come to lie where one of these is
+        self.at = _lib.training().places(self.tensors)
         self.bytes = [p.nbytes for p in params]                # of a gradient
         self.plain = all(p.is_contiguous() for p in params)
         self.table = np.zeros((len(params), 7), dtype=np.uint64)
-        self.table[:, 0] = self.at[:len(params)]
+        self.table[:, 0] = [p.data_ptr() for p in params]
         for column, moment in enumerate(self.moments):
             self.table[:, 2 + column] = [t.data_ptr() for t in moment]
         self.table[:, 6] = [p.numel() for p in params]
 
     def holds(self):
         return (all(all(map(operator.is_, map(operator.itemgetter(k), self.states), old)) for k, old in zip(self.keys, self.moments))
-                and list(map(_ptr, itertools.chain(self.params, *self.moments))) == self.at)
+                and _lib.training().places(self.tensors) == self.at)
 
     def take_gradients(self, grads):
         if not self.plain or not all(map(_dense, grads)) or list(map(_nbytes, grads)) != self.bytes:
