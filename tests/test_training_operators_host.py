@@ -206,3 +206,16 @@ def test_a_table_of_weights_holds_for_their_memory_alone(change):
     else:
         state["exp_avg_sq_scale"].data = state["exp_avg_sq_scale"].data[:3]
     assert not batch.holds()
+
+
+def test_gradients_of_a_table():
+    """One of another type, size or device, or a sparse one, is refused also where its bytes are as many."""
+    from vtpack_amd.optim import _Batch
+    p, q = (torch.nn.Parameter(torch.randn(32).bfloat16()) for _ in range(2))
+    states = [{k: torch.zeros(32) for k in ("exp_avg", "exp_avg_sq")} for _ in range(2)]
+    batch = _Batch([p, q], states, 32, 0)
+    good = torch.zeros(32, dtype=torch.bfloat16)
+    assert all(a is b for a, b in zip(batch.take_gradients([good, good]), [good, good]))
+    for bad in (good.half(), torch.zeros(32, dtype=torch.bfloat16, device="meta"), good.view(4, 8), good[:31], good.to_sparse()):
+        with pytest.raises(ValueError):
+            batch.take_gradients([good, bad])

@@ -578,6 +578,20 @@ PyObject *py_places(PyObject *, PyObject *const *a, Py_ssize_t n)
         return PyBytes_FromStringAndSize(reinterpret_cast<const char *>(out.data()), (Py_ssize_t)(out.size() * sizeof(int64_t)));
     });
 }
+// (two lists of tensors): whether they are of the same types and sizes, pair by pair, on the same devices, and strided
+PyObject *py_alike(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    return call(a, n, 2, [&]() -> PyObject * {
+        if (!PyList_Check(a[0]) || !PyList_Check(a[1]) || PyList_GET_SIZE(a[0]) != PyList_GET_SIZE(a[1])) throw std::runtime_error("alike: expected two lists of one length");
+        for (Py_ssize_t i = 0; i < PyList_GET_SIZE(a[0]); i++) {
+            const Tensor x = tensor(PyList_GET_ITEM(a[0], i)), y = tensor(PyList_GET_ITEM(a[1], i));
+            if (!x.defined() || !y.defined() || x.layout() != at::kStrided || y.layout() != at::kStrided || x.scalar_type() != y.scalar_type() ||
+                x.device() != y.device() || x.sizes() != y.sizes())
+                Py_RETURN_FALSE;
+        }
+        Py_RETURN_TRUE;
+    });
+}
 
 // (params, states, keys, bits): lists of weights, of their states and of the names of the moments in them, scales behind -> a batch,
 // or None unless all is as a launch takes it: weights of one type on one GPU, dense and apart, moments and scales that fit them
@@ -658,7 +672,7 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
 
 #define VT_METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {VT_METHOD(bind), VT_METHOD(linear_cross_entropy), VT_METHOD(cross_entropy), VT_METHOD(cross_entropy_backward),
-                         VT_METHOD(balance), VT_METHOD(gate_balance), VT_METHOD(gate_balance_backward), VT_METHOD(places), VT_METHOD(adamw_batch),
+                         VT_METHOD(balance), VT_METHOD(gate_balance), VT_METHOD(gate_balance_backward), VT_METHOD(places), VT_METHOD(alike), VT_METHOD(adamw_batch),
                          VT_METHOD(adamw_step), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_training", "The operators of a training step as torch calls them.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

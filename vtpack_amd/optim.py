@@ -15,7 +15,7 @@ __all__ = ["AdamW"]
 BLOCK = 256                                    # elements that share a scale
 _CODES = {"exp_avg": torch.float8_e4m3fn, "exp_avg_sq": torch.float8_e5m2}
 _KEYS = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
-_grad, _nbytes = operator.attrgetter("grad"), operator.attrgetter("nbytes")
+_grad = operator.attrgetter("grad")
 _ptr, _dense = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
 
 
@@ -34,7 +34,6 @@ class _Batch:
         self.tensors = list(itertools.chain(params, *self.moments))
         self.kept = [t.detach() for t in self.tensors]         # no other storage can come to lie where one of these is
         self.at = _lib.training().places(self.tensors)
-        self.bytes = [p.nbytes for p in params]                # of a gradient
         self.plain = all(p.is_contiguous() for p in params)
         self.table = np.zeros((len(params), 7), dtype=np.uint64)
         self.table[:, 0] = [p.data_ptr() for p in params]
@@ -47,10 +46,12 @@ class _Batch:
                 and _lib.training().places(self.tensors) == self.at)
 
     def take_gradients(self, grads):
-        if not self.plain or not all(map(_dense, grads)) or list(map(_nbytes, grads)) != self.bytes:
+        if not _lib.training().alike(grads, self.params):
             for g, p in zip(grads, self.params):
                 if g.dtype != p.dtype or g.shape != p.shape or g.device != p.device:
                     raise ValueError(f"a gradient of {g.dtype} {tuple(g.shape)} on {g.device} for a weight of {p.dtype} {tuple(p.shape)} on {p.device}")
+            raise ValueError("AdamW: sparse gradients are not supported")
+        if not self.plain or not all(map(_dense, grads)):
             grads = [g if _same_layout(g, p) else torch.empty_like(p).copy_(g) for g, p in zip(grads, self.params)]
         self.table[:, 1] = list(map(_ptr, grads))
         return grads
