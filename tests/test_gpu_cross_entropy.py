@@ -484,3 +484,19 @@ def test_one_operand_is_laid_out(dev, which):
     assert laid_out is None and torch.equal(loss, want[0])
     got = ops.cross_entropy_backward(xs, ws, b, t, stats, None, torch.ones((), device=dev))
     assert all(torch.equal(p, q) for p, q in zip(got, want[1:]))
+
+
+def test_tracing_is_refused(dev):
+    """On every way to a launch: operands that are taken as they are, and those that are brought into form."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from vtpack_amd.layers import gate_balance, linear_cross_entropy
+    x, w, b, t = _operands(dev, 50, 60, 64, torch.float32)
+    for call in (lambda x: linear_cross_entropy(x, w, b, t), lambda x: linear_cross_entropy(x.t().contiguous().t(), w, b, t), lambda x: gate_balance(x)[0],
+                 lambda x: gate_balance(x, indices=t)[0]):
+        want = call(x)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, (x,))
+        for mode in ("real", "fake"):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                make_fx(call, tracing_mode=mode, _allow_non_fake_inputs=True)(x)
+        assert torch.equal(call(x), want)

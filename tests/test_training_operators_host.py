@@ -219,3 +219,17 @@ def test_gradients_of_a_table():
     for bad in (good.half(), torch.zeros(32, dtype=torch.bfloat16, device="meta"), good.view(4, 8), good[:31], good.to_sparse()):
         with pytest.raises(ValueError):
             batch.take_gradients([good, bad])
+
+
+def test_tracing_is_refused():
+    """What a trace would record of a native call is the allocation of its results."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, t = torch.randn(4, 8), torch.randn(3, 8), torch.zeros(4, dtype=torch.int64)
+    for call in (lambda x: linear_cross_entropy(x, w, None, t), lambda x: gate_balance(x)[0]):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, (x,))
+        for mode in ("real", "fake"):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                make_fx(call, tracing_mode=mode, _allow_non_fake_inputs=True)(x)
+        with pytest.raises(RuntimeError, match="GPU only"):           # and nothing stays behind of it
+            call(x)

@@ -9,12 +9,14 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <array>
@@ -151,6 +153,17 @@ void no_forward_mode(const char *name, std::initializer_list<const Tensor *> ope
 {
     for (const Tensor *t : operands)
         if (t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error(std::string(name) + ": forward-mode derivatives are not supported");
+}
+
+// A trace would record the allocation of the results and not what fills them.
+void no_tracing(const char *name)
+{
+    using Key = c10::impl::TorchDispatchModeKey;
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    bool traced = torch::jit::tracer::isTracing();
+    if (Modes::any_modes_set())
+        for (const Key key : {Key::FAKE, Key::PROXY, Key::FUNCTIONAL}) traced = traced || Modes::get_mode(key).has_value();
+    if (traced) throw std::runtime_error(std::string(name) + " cannot be traced");
 }
 
 // The backward node of a loss, with what it reads as members.
@@ -402,6 +415,7 @@ bool plain_beside(const Tensor &t, const Tensor &x, at::ScalarType type)
 PyObject *py_linear_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 7, [&]() -> PyObject * {
+        no_tracing("linear_cross_entropy");
         for (int i = 0; i < 4; i++)
             if (!THPVariable_Check(a[i]) && !(i == 2 && a[i] == Py_None)) Py_RETURN_NONE;
         if (!PyLong_Check(a[4]) || !number(a[5]) || !PyLong_Check(a[6])) Py_RETURN_NONE;
@@ -505,6 +519,7 @@ PyObject *py_cross_entropy_backward(PyObject *, PyObject *const *a, Py_ssize_t n
 PyObject *py_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 4, [&]() -> PyObject * {
+        no_tracing("gate_balance");
         for (int i = 0; i < 3; i++)
             if (!THPVariable_Check(a[i]) && !(i > 0 && a[i] == Py_None)) Py_RETURN_NONE;
         if (!PyLong_Check(a[3])) Py_RETURN_NONE;

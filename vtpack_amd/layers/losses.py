@@ -12,7 +12,8 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     x [..., width], weight [classes, width], bias [classes] or None, all float32 or all bfloat16; target int64 of x's leading
     shape.  -> float32: the mean over the rows that count ("mean"), their sum ("sum"), or every row's own ("none", of target's
     shape).  A row whose target is `ignore_index` is left out, whatever its features hold; so is one whose target is no class
-    (F.cross_entropy stops the program there).  Without a row that counts the loss is 0, and so are the gradients.
+    (F.cross_entropy stops the program there).  Without a row that counts the loss is 0, and so are the gradients.  Traces
+    (torch.jit.trace, make_fx), forward-mode derivatives and gradients of the gradients are refused.
 
     The logits are fp32 sums and are not rounded; in bfloat16 the gradients of the logits are, once, before the products that
     take them to x, weight and bias.  They work in pieces of the classes with some 320 MB of scratch for a piece; float32
@@ -56,7 +57,7 @@ def gate_balance(gate, indices=None, top_k=1, mask=None):
     even, E is all on one.  The choices are the `top_k` largest logits of a token (among equals the lowest index), or `indices`
     int64 [..., k] (or of gate's leading shape, k = 1) if they were made elsewhere, as by a Gumbel sample; one that is no expert is
     not counted.  `mask` (bool, gate's leading shape): False leaves a token out, whatever its logits are; a token whose logits are
-    all -inf is left out too.  Without a token the loss is 0."""
+    all -inf is left out too.  Without a token the loss is 0.  Refused as `linear_cross_entropy` does: traces, forward mode, second order."""
     out = _lib.training().balance(gate, indices, mask, top_k) if indices is None else None
     if out is not None:
         return out
