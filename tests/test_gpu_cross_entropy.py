@@ -500,3 +500,11 @@ def test_tracing_is_refused(dev):
             with pytest.raises(RuntimeError, match="cannot be traced"):
                 make_fx(call, tracing_mode=mode, _allow_non_fake_inputs=True)(x)
         assert torch.equal(call(x), want)
+
+
+def test_widths_beyond_32_bits_are_refused(dev):
+    """Not taken for their lower 32 bits."""
+    from vtpack_amd.layers import linear_cross_entropy
+    row = torch.empty((1, (1 << 32) + 64), dtype=torch.bfloat16, device=dev)
+    with pytest.raises(RuntimeError, match="rows"):
+        linear_cross_entropy(row, row, None, torch.zeros(1, dtype=torch.int64, device=dev))

@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <array>
+#include <cstdint>
 #include <map>
 #include <mutex>
 #include <memory>
@@ -81,9 +82,9 @@ enum Reduction { NONE, MEAN, SUM };
 constexpr int64_t KEEP_LAID_OUT = 320 << 20;    // bytes
 
 struct Rows {
-    int64_t rows, classes; int width, dtype, lie;
+    int64_t rows, classes; int width, dtype, lie;   // (a width beyond 32 bits is the largest one within, which the library refuses)
     Rows(const Tensor &x, const Tensor &w)
-        : rows(x.size(0)), classes(w.size(0)), width((int)x.size(1)), dtype(code_of(x)),
+        : rows(x.size(0)), classes(w.size(0)), width((int)std::min<int64_t>(x.size(1), INT32_MAX)), dtype(code_of(x)),
           lie((lies(x) ? VTDGE_CE_X_LIES : 0) + (lies(w) ? VTDGE_CE_WEIGHT_LIES : 0)) {}
     // whether the kernels read an operand where it lies
     bool lies(const Tensor &t) const
