@@ -150,3 +150,26 @@ def test_refusals(dev):
         harness.train_step(m.bfloat16(), images.bfloat16(), target, AdamW(m.parameters()))
     with pytest.raises(ValueError, match="DynamicGrainedEncoder"):
         harness.balance_loss(torch.nn.Linear(3, 3))
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_an_evaluation_leaves_nothing_of_the_training_pass(dev, fused):
+    """The balance is that of a training pass: behind an evaluation there is none, the pass's graph is given up and the model can be
+    copied."""
+    m = _deit(dev)
+    images, target = _batch(dev)
+    m(images, target).backward()
+    assert all(blk.dge.balance()[1].sum() > 0 for blk in m.blocks)
+    m.eval().set_fused(fused)
+    with torch.no_grad():
+        m(images)
+    for blk in m.blocks:
+        assert "gate_logits" not in blk.dge.states
+    if not fused:                                         # (a fused pass leaves values that are worked out when they are read)
+        copy.deepcopy(m)
+    m.train()
+    for blk in m.blocks:
+        with pytest.raises(RuntimeError, match="training mode"):
+            blk.dge.balance()
+    m(images, target)
+    assert all(blk.dge.balance()[1].sum() > 0 for blk in m.blocks)

@@ -452,6 +452,7 @@ def block_forward(block, x, H, W, gate=None, overlap=True, carry=None, next_bloc
     def cut(t):
         return lambda: t[:int(live().sum())]
 
+    dge.states.pop("gate_logits", None)
     dge.states.update({"comp": Deferred(cut(comp)), "input": x, "patches": Deferred(cut(patches)),
                        "batches": Deferred(batches),
                        "batches_device": Deferred(live) if lengths is None else lengths, "offsets_device": offsets,
@@ -684,6 +685,7 @@ def _run_chain(blocks, x, H, W, front, plan, lay):
     run = (x, ints, big, lay, main, torch.cuda.is_current_stream_capturing())
     for i, blk in enumerate(blocks):
         st = blk.dge.states
+        dict.pop(st, "gate_logits", None)
         dict.update(st, dict.fromkeys(_ChainBlock.KEYS, _ChainBlock(run, i)))
         st["size"], st["num_extra_tokens"] = (H, W), desc.extra
     return out

@@ -200,6 +200,8 @@ class DynamicGrainedEncoder(nn.Module):
             gate, indices = self.router.route(x, H, W)
         else:
             indices = gate.argmax(dim=-1)
+        if not self.training:
+            self.states.pop("gate_logits", None)             # a training pass's, and the graph it holds
         patches, batches = grained_sample_index_to_patch(indices, self.splits, self.region_size, extra)
         comp = grained_sample_compress(x, patches, H, W, extra)
         self.states.update({"comp": comp, "input": x, "patches": patches, "batches": batches, "gate": gate,
