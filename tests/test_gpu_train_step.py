@@ -173,3 +173,29 @@ def test_an_evaluation_leaves_nothing_of_the_training_pass(dev, fused):
             blk.dge.balance()
     m(images, target)
     assert all(blk.dge.balance()[1].sum() > 0 for blk in m.blocks)
+
+
+def test_an_epoch_ends_before_a_loss_that_is_not_finite_moves_anything(dev):
+    from vtpack_amd import harness
+    from vtpack_amd.optim import AdamW
+    m = _deit(dev)
+    batches = list(harness.synthetic_loader(1, 4, 64, num_classes=7, seed=3))
+    opt = AdamW(harness.weight_decay_groups(m, 0.05), lr=1e-3, state_bits=8)
+    harness.train_one_epoch(batches, m, opt, dev)
+    with torch.no_grad():
+        m.head.bias[2] = float("nan")
+
+    def everything():
+        tensors = [p.detach() for p in m.parameters()] + [t for p in m.parameters() for t in opt.state.get(p, {}).values() if torch.is_tensor(t)]
+        return [t.contiguous().view(-1).view(torch.uint8).clone() for t in tensors], [g["step"] for g in opt.param_groups]
+
+    tensors, steps = everything()
+    with pytest.raises(FloatingPointError, match="nan"):
+        harness.train_one_epoch(batches, m, opt, dev)
+    now, after = everything()
+    assert steps == after == [1] * len(steps) and all(torch.equal(a, b) for a, b in zip(tensors, now))
+    # a step by itself looks when it is asked to
+    images, target = (t.to(dev) for t in batches[0])
+    with pytest.raises(FloatingPointError):
+        harness.train_step(m, images, target, opt, finite=True)
+    assert all(torch.equal(a, b) for a, b in zip(tensors, everything()[0]))

@@ -116,11 +116,13 @@ def weight_decay_groups(model, weight_decay):
 
 
 def train_step(model, images, target, optimizer, label_smoothing=0.0, dge_enable=False, dge_budget=1.0, dge_lr_scale=1.0,
-               balance_scale=0.0, clip_grad=None):
+               balance_scale=0.0, clip_grad=None, finite=False):
     """One update of a model in training mode (vtpack/engine/engine.py:48-90 without autocast): the classifier's cross entropy against
     int64 `target`, with `dge_enable` the budget loss, `balance_scale` times the balance of the gates, gradients, their norm cut
-    to `clip_grad`, the optimiser's step (any; `optim.AdamW` takes one launch for 134 weights).  -> {name: tensor on the GPU},
-    nothing of which is waited for: loss, loss_cls, and loss_dge, dge_ratio, loss_balance, gate_counts, grad_norm where they are made.
+    to `clip_grad`, the optimiser's step (any; `optim.AdamW` takes one launch for 134 weights).  With `finite` the loss is read
+    back before the gradients, and one that is not finite is a FloatingPointError, with weights, gradients and moments as they
+    were (engine.py:74-76).  -> {name: tensor on the GPU}, nothing of which is waited for without `finite`: loss, loss_cls, and
+    loss_dge, dge_ratio, loss_balance, gate_counts, grad_norm where they are made.
 
     Weights are float32: the dense training branch multiplies with the library's batched products."""
     if not unwrap(model).training:
@@ -138,6 +140,8 @@ def train_step(model, images, target, optimizer, label_smoothing=0.0, dge_enable
         balance, counts = balance_loss(model)
         loss = loss + balance_scale * balance
         out.update(loss_balance=balance.detach(), gate_counts=counts)
+    if finite and not math.isfinite(value := float(loss.detach())):
+        raise FloatingPointError(f"the loss is {value}")
     optimizer.zero_grad(set_to_none=True)
     loss.backward()
     if clip_grad is not None:
@@ -149,13 +153,11 @@ def train_step(model, images, target, optimizer, label_smoothing=0.0, dge_enable
 
 def train_one_epoch(data_loader, model, optimizer, device, **how):
     """vtpack/engine/engine.py:35-99: `train_step(**how)` for every (images, target) batch.  -> {meter name: global average} of its scalars and `lr`;
-    a loss that is not finite ends the epoch with an error, as the reference's run does (engine.py:74-76)."""
-    meters = {}
+    a loss that is not finite ends the epoch with an error before it moves anything, as it ends the reference's run (engine.py:74-76)."""
+    meters, how = {}, {"finite": True, **how}
     model.train()
     for images, target in data_loader:
         out = train_step(model, images.to(device, non_blocking=True), target.to(device, non_blocking=True), optimizer, **how)
-        if not math.isfinite(float(out["loss"])):
-            raise FloatingPointError(f"the loss is {float(out['loss'])}")
         for name, value in out.items():
             if value.dim() == 0:
                 meters.setdefault(name, _Meter()).update(float(value))
