@@ -508,3 +508,55 @@ def test_widths_beyond_32_bits_are_refused(dev):
     row = torch.empty((1, (1 << 32) + 64), dtype=torch.bfloat16, device=dev)
     with pytest.raises(RuntimeError, match="rows"):
         linear_cross_entropy(row, row, None, torch.zeros(1, dtype=torch.int64, device=dev))
+
+
+def test_fp32_up_to_the_largest_number(dev):
+    """Finite features and weights next to the largest fp32 number, which bf16 would round to infinity: losses of 1e38, bounded by
+    half steps of the logits as all are."""
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 40, 150, 64, torch.float32)
+    x[3, 0], x[17, 5] = 3.4e38, -3.4028e38
+    w[:, 0] *= 0.3
+    w[:, 5] *= 0.3
+    want, _, d, grads = _reference(x, w, b, t)
+    leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+    got = linear_cross_entropy(*leaves, t, reduction="none")
+    tol = _tolerance(x, w)
+    assert ((got.double() - want).abs() <= tol * (16 + want.abs())).all()
+    for g, r in zip(torch.autograd.grad(got.sum() / 40, leaves), grads):
+        _near(g, r, tol, 1e-30)
+    # the largest weights
+    x, w, b, t = _operands(dev, 40, 150, 64, torch.float32, seed=1)
+    w[7, 3], w[100, 3] = 3.4e38, -3.4e38
+    x[:, 3] *= 0.05
+    want = _reference(x, w, b, t)[0]
+    got = linear_cross_entropy(x, w, b, t, reduction="none")
+    assert torch.isfinite(got).all() and ((got.double() - want).abs() <= tol * (16 + want.abs())).all()
+
+
+@pytest.mark.parametrize("kept", [True, False])
+def test_row_weights_up_to_the_largest_number(dev, kept):
+    """d of a row whose loss is weighted by 3.4e38, an fp32 operand like any other."""
+    from vtpack_amd import ops
+    x, w, b, t = _operands(dev, 40, 150, 64, torch.float32)
+    x, w, b, t = x[:2], torch.zeros_like(w), torch.zeros_like(b), t[:2]
+    b[t[0]] = -200.0                                       # its own class has no share: d is -1 there
+    x[:] = x.clamp(-0.5, 0.5)
+    grad = torch.tensor([3.4e38, 1.0], device=dev)
+    loss, stats, laid_out = ops.cross_entropy(x, w, b, t, reduction="none")
+    dx, dw, db = ops.cross_entropy_backward(x, w, b, t, stats, laid_out if kept else None, grad, reduction="none")
+    want = _reference(x, w, b, t, weights=grad)[3]
+    for g, r in zip((dx, dw, db), want):
+        _near(g, r, _tolerance(x, w), 1e-30)
+
+
+def test_fp32_next_to_the_smallest_numbers(dev):
+    """Features below 2^-110 are off by 2^-134 at most, a logit by that times its weights, a loss by twice a logit."""
+    from vtpack_amd.layers import linear_cross_entropy
+    x, w, b, t = _operands(dev, 40, 150, 64, torch.float32)
+    x, w = x * 2.0 ** -118, w * 2.0 ** 118
+    want = _reference(x, w, b, t)[0]
+    got = linear_cross_entropy(x, w, b, t, reduction="none")
+    z = x.double() @ w.double().t()
+    bound = 2 * 2.0 ** -134 * float(w.double().abs().sum(1).max()) + _tolerance(x, w) * (1 + float(z.abs().max()))
+    assert float((got.double() - want).abs().max()) <= bound

@@ -15,7 +15,8 @@
 // bank conflicts, on the side of the global address.
 // fp32 operands are split into three bf16 parts each (24 bits), and the six products of parts down to 2^-24 are a six times longer
 // sum, smallest first, in the same fp32 sums: the same kernels at a sixth of their rate, which is above that of the fp32 matrix
-// instructions.  (Two fp16 parts and three products would be 22 bits of a row's largest value and fewer of its small ones.)
+// instructions.  Bits below 2^-133 are lost, which only values below 2^-110 have, and an infinity meets parts of either sign and becomes
+// NaN.  (Two fp16 parts and three products would be 22 bits of a row's largest value and fewer of its small ones.)
 //
 // Bound by the matrix units in long products: 8192 rows x 65536 classes x 1024 in bf16, tiles 0.98 ms (1.12 PFLOP/s), d 4 x 0.29 (0.94,
 // with the writing of d), gradients 4 x 0.51 (1.07); in fp32 2048 x 21841 x 384, tiles 0.21 ms (166 TFLOP/s of fp32, 1.0 PFLOP/s issued; 0.24
@@ -30,6 +31,10 @@ namespace vtdge {
 
 constexpr float LOG2E = 1.44269504f, LN2 = 0.69314718f;
 __device__ __forceinline__ int wave_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// What the first bf16 part of an fp32 value is rounded from: the largest finite numbers would become infinite, and are cut to bf16's
+// largest; the next part has the rest.  (Infinity and NaN go on to the next part.)
+constexpr float BF16_MOST = 0x1.fep127f;
+__device__ __forceinline__ float first_part(float f) { return __builtin_amdgcn_fmed3f(f, -BF16_MOST, BF16_MOST); }
 
 // ------------------------------------------------------------------------------------------------ the product of a tile
 // A bf16 matrix, or the three parts of an fp32 one `plane` elements apart.
@@ -559,7 +564,7 @@ template <class S> __device__ __forceinline__ void d_tile(const CeArgs &p, int64
     // is alone: part by part through LDS, rows in whole lines (2048 x 384 x 21841: 290 us without, 251 so).
     constexpr int PITCH = S::COLS * 2 + 16, VECS = S::COLS / 8;
     static_assert(S::PARTS == 1 || S::ROWS * PITCH <= S::RING, "LDS");
-    auto put = [&](int i, bool rest) {              // and what is left of the values for the next part
+    auto put = [&](int i, bool first, bool rest) {  // and what is left of the values for the next part
         bf16_t *const row = p.d + (r0 + (wm * IM + i) * 32 + lr) * p.d_pitch + (cw - p.v0) + 8 * lg;
         unsigned char *const at = smem + ((wm * IM + i) * 32 + lr) * PITCH + wn * 64 * JN + 16 * lg;
 #pragma unroll
@@ -569,7 +574,8 @@ template <class S> __device__ __forceinline__ void d_tile(const CeArgs &p, int64
                 uint32_t o[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    o[e] = pack_bf16x2(acc[i][j][8 * q + 2 * e], acc[i][j][8 * q + 2 * e + 1]);
+                    const float a = acc[i][j][8 * q + 2 * e], b = acc[i][j][8 * q + 2 * e + 1];
+                    o[e] = first ? pack_bf16x2(first_part(a), first_part(b)) : pack_bf16x2(a, b);
                     if (rest) acc[i][j][8 * q + 2 * e] -= bf16lo(o[e]), acc[i][j][8 * q + 2 * e + 1] -= bf16hi(o[e]);
                 }
                 const auto s0 = __builtin_amdgcn_permlane32_swap(o[0], o[2], false, false), s1 = __builtin_amdgcn_permlane32_swap(o[1], o[3], false, false);
@@ -602,14 +608,14 @@ template <class S> __device__ __forceinline__ void d_tile(const CeArgs &p, int64
 #pragma unroll
                 for (int v = 0; v < 16; v++) acc[i][j][v] = live && cw + j * 32 + 8 * (v / 4) + 4 * lg + v % 4 < p.v1 ? acc[i][j][v] : 0.f;
         }
-        put(i, S::PARTS > 1);
+        put(i, S::PARTS > 1, S::PARTS > 1);
     }
     if constexpr (S::PARTS > 1) {
         for (int part = 0; part < S::PARTS; part++) {
             if (part > 0) {
                 __syncthreads();
 #pragma unroll
-                for (int i = 0; i < IM; i++) put(i, part + 1 < S::PARTS);
+                for (int i = 0; i < IM; i++) put(i, false, part + 1 < S::PARTS);
             }
             __syncthreads();
             bf16_t *const to = p.d + part * p.d_plane + r0 * p.d_pitch + (c0 - p.v0);
@@ -666,7 +672,7 @@ __global__ __launch_bounds__(256) void cross_entropy_d_kept_kernel(CeArgs p, int
         u32x4 o;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            o[e] = pack_bf16x2(f[2 * e], f[2 * e + 1]);
+            o[e] = part == 0 ? pack_bf16x2(first_part(f[2 * e]), first_part(f[2 * e + 1])) : pack_bf16x2(f[2 * e], f[2 * e + 1]);
             f[2 * e] -= bf16lo(o[e]), f[2 * e + 1] -= bf16hi(o[e]);
         }
         *reinterpret_cast<u32x4 *>(to + part * p.d_plane) = o;
@@ -868,17 +874,20 @@ template <typename T> __global__ __launch_bounds__(256) void cross_entropy_pack_
         for (int e = 0; e < 8; e++) f[e] = live && c + e < p.width ? Elem<T>::load(from + e) : 0.f;
     }
     bf16_t *const at = job.to + r * p.padded + c;
-    *reinterpret_cast<u32x4 *>(at) = Elem<bf16_t>::pack(f);
-    if constexpr (sizeof(T) == 4) {
-        // (infinity and NaN have no rest)
+    if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<u32x4 *>(at) = Elem<bf16_t>::pack(f);
+    } else {
 #pragma unroll
-        for (int part = 1; part < 3; part++) {
+        for (int part = 0; part < 3; part++) {
+            float v[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float rest = f[e] - Elem<bf16_t>::round(f[e]);
+                // (infinity and NaN have no rest)
+                v[e] = part == 0 && fabsf(f[e]) < INFINITY ? first_part(f[e]) : f[e];
+                const float rest = f[e] - Elem<bf16_t>::round(v[e]);
                 f[e] = fabsf(rest) < INFINITY ? rest : 0.f;
             }
-            *reinterpret_cast<u32x4 *>(at + part * job.rows * p.padded) = Elem<bf16_t>::pack(f);
+            *reinterpret_cast<u32x4 *>(at + part * job.rows * p.padded) = Elem<bf16_t>::pack(v);
         }
     }
 }
