@@ -50,6 +50,15 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     return loss.view(target.shape) if reduction == "none" and target.dim() != 1 else loss
 
 
+def require_plain_head(head):
+    """A TypeError unless a model's classifier is what `linear_cross_entropy` of its weight and bias is."""
+    hooks = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+    if (not isinstance(head, torch.nn.Linear) or type(head).forward is not torch.nn.Linear.forward or "forward" in vars(head)
+            or any(getattr(head, h, None) for h in hooks)):
+        raise TypeError("the model's head is more than a Linear without hooks, and its loss would read the weight and bias alone: take "
+                        "F.cross_entropy of the logits, model(images)")
+
+
 def gate_balance(gate, indices=None, top_k=1, mask=None):
     """How evenly a router's choices fall on its experts (here: granularities): -> (loss, counts).
 

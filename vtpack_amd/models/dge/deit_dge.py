@@ -22,6 +22,7 @@ from torch import nn
 
 from ... import engine
 from ...layers import DynamicGrainedEncoder, linear_cross_entropy
+from ...layers.losses import require_plain_head
 from ...layers.sparse_ops import batched_sparse_attention, sparse_attention_train
 
 __all__ = ["VisionTransformer", "Block", "Attention", "Mlp", "PatchEmbed", "deit_dge_s124_tiny_patch16_256",
@@ -225,9 +226,10 @@ class VisionTransformer(nn.Module):
     def loss(self, x, target, label_smoothing=0.0, ignore_index=-100, reduction="mean"):
         """Cross entropy of the (class) head's logits on images x against int64 target [B], without the logits in memory; see
         `layers.linear_cross_entropy`.  With a distillation token the class token's head alone, as the reference's base
-        criterion takes it (vtpack/engine/losses.py:41-48)."""
+        criterion takes it (vtpack/engine/losses.py:41-48).  A head with hooks, or one that is no plain Linear, is refused."""
         if self.num_classes <= 0:
             raise ValueError("a model without a classifier has no loss")
+        require_plain_head(self.head)
         if self.training and any(self.drop_rates):
             raise NotImplementedError("dropout / stochastic depth in training mode are not part of this package")
         feats = self.forward_features(x)

@@ -15,6 +15,7 @@ from torch import nn
 
 from ... import engine
 from ...layers import DynamicGrainedEncoder, linear_cross_entropy
+from ...layers.losses import require_plain_head
 from ...layers.sparse_ops import batched_sparse_attention, sparse_attention_train
 from .deit_dge import Mlp
 
@@ -208,9 +209,10 @@ class PyramidVisionTransformer(nn.Module):
 
     def loss(self, x, target, label_smoothing=0.0, ignore_index=-100, reduction="mean"):
         """Cross entropy of the logits of images x against int64 target [B], without the logits in memory; see
-        `layers.linear_cross_entropy`."""
+        `layers.linear_cross_entropy`.  A head with hooks, or one that is no plain Linear, is refused."""
         if self.num_classes <= 0:
             raise ValueError("a model without a classifier has no loss")
+        require_plain_head(self.head)
         return linear_cross_entropy(self.forward_features(x), self.head.weight, self.head.bias, target, ignore_index, label_smoothing,
                                     reduction)
 
