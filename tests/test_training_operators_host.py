@@ -269,3 +269,10 @@ def test_a_head_that_is_more_than_its_weight_has_no_fused_loss(family):
     with pytest.raises(Exception) as caught:              # on to the kernels, which want a GPU
         m.loss(images, target)
     assert "model's head" not in str(caught.value)
+
+
+def test_how_a_loss_is_made_goes_with_a_target():
+    from vtpack_amd.models.dge.deit_dge import VisionTransformer
+    m = VisionTransformer(img_size=64, patch_size=8, embed_dim=64, depth=1, num_heads=1, mlp_ratio=2, num_classes=7, split_sizes=[4, 2, 1])
+    with pytest.raises(TypeError, match="label_smoothing without a target"):
+        m(torch.randn(1, 3, 64, 64), label_smoothing=0.1)

@@ -243,6 +243,8 @@ class VisionTransformer(nn.Module):
         """Logits of images x; with `target` the `loss` (so that a wrapper around the model sees its training pass)."""
         if target is not None:
             return self.loss(x, target, **how)
+        if how:
+            raise TypeError(f"{', '.join(how)} without a target")
         if self.fused and not self.training:
             return engine.model_forward(self, x)
         if self.training and any(self.drop_rates):

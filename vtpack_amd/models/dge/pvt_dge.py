@@ -219,6 +219,8 @@ class PyramidVisionTransformer(nn.Module):
     def forward(self, x, target=None, **how):
         if target is not None:
             return self.loss(x, target, **how)
+        if how:
+            raise TypeError(f"{', '.join(how)} without a target")
         if self.fused and not self.training:
             return engine.pvt_forward(self, x)
         x = self.forward_features(x)
