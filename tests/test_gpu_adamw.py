@@ -535,3 +535,28 @@ def test_another_tensor_at_the_same_address(dev, bits):
                 opt.step()
             opt.state[x]["exp_avg"].data = moment
     opt.step()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_that_is_refused_changes_nothing(dev, bits):
+    """Neither the counts of the weights that have no gradient, nor the weights of a group that come before the one that does not fit."""
+    params = [torch.nn.Parameter(_tensors(dev, [(300,)], d, i)[0]) for i, d in enumerate((torch.float32, torch.float32, torch.bfloat16))]
+    refs = [_Reference(p, bits) for p in params]
+    opt = _optimizer(params, bits)
+    for k in range(3):
+        for bad in (True, False) if k else (False,):
+            for i, p in enumerate(params):
+                p.grad = _tensors(dev, [(300,)], p.dtype, 70 + 3 * k + i, 1e-3)[0]
+            if not bad:
+                opt.step()
+                for p, r in zip(params, refs):
+                    r.step(p.grad)
+                    r.check(p, opt.state[p])
+                continue
+            before = [p.detach().clone() for p in params]
+            if k == 1:
+                params[0].grad = None
+            params[2].grad.data = params[2].grad.data[:299]
+            with pytest.raises(ValueError):
+                opt.step()
+            assert all(torch.equal(p, q) for p, q in zip(params, before)) and opt.param_groups[0]["step"] == k

@@ -193,31 +193,39 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def _step_groups(self, groups):
-        """The step of groups that have to be looked over."""
+        """The step of groups that have to be looked over.  A group's weights, gradients and states are all looked at before the first
+        launch, so that one that is refused is as it was; those before it have taken their step."""
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
         for index, group in groups:
             params = group["params"]
             grads = list(map(_grad, params))
             if capturing and not group["capturable"]:
                 raise RuntimeError("AdamW: a step that is captured needs capturable=True (its count of steps would stand still)")
+            missing = []
             if not all(map(operator.is_not, grads, itertools.repeat(None))):
                 params = [p for p, g in zip(params, grads) if g is not None]
                 if not params:
                     continue
-                self._skip(index, [p for p, g in zip(group["params"], grads) if g is None], capturing)
+                missing = [p for p, g in zip(group["params"], grads) if g is None and any(k in self.state.get(p, ()) for k in _CODES)]
+                if missing and capturing:
+                    raise RuntimeError("AdamW: a weight that has taken steps has no gradient in the one that is captured")
                 grads = [g for g in grads if g is not None]
             batches = self._held(index, group, params)
             if batches is None:
                 if not capturing and (params is not group["params"] and self._in_one_call(index, group, params)
                                       or self._in_one_call(index, group, params, anew=True)):
+                    self._skip(index, missing)
                     continue
                 batches = self._of_group(index, group, params, grads)
             of = dict(zip(map(id, params), grads)) if len(batches) > 1 else None
+            held = [b.take_gradients(grads if of is None else [of[id(p)] for p in b.params]) for b in batches]
             for i, b in enumerate(batches):
-                self._launch(group, b, grads if of is None else [of[id(p)] for p in b.params], i + 1 == len(batches))
+                self._launch(group, b, i + 1 == len(batches))
+            del held                                           # (what was laid out anew is read behind the launch)
             if not group["capturable"]:
                 group["step"] += 1
             increment_version(params)
+            self._skip(index, missing)
 
     def _in_one_call(self, index, group, params, anew=False):
         """The step of a group's weights in one native call that looks all of them over and launches; False, and nothing done, where
@@ -246,19 +254,15 @@ class AdamW(torch.optim.Optimizer):
         group["step"] += 1
         return True
 
-    def _skip(self, index, params, capturing):
-        """Weights without a gradient miss this step."""
+    def _skip(self, index, params):
+        """Weights with states and without a gradient have missed this step."""
         for p in params:
-            if p in self.state and any(k in self.state[p] for k in _CODES):
-                if capturing:
-                    raise RuntimeError("AdamW: a weight that has taken steps has no gradient in the one that is captured")
-                self.state[p]["skipped"] = self.state[p].get("skipped", 0) + 1
-                self._batches.pop(index, None)
-                self._natives.pop(index, None)
+            self.state[p]["skipped"] = self.state[p].get("skipped", 0) + 1
+            self._batches.pop(index, None)
+            self._natives.pop(index, None)
 
-    def _launch(self, group, batch, grads, last):
+    def _launch(self, group, batch, last):
         (b1, b2), eps, decay = group["betas"], group["eps"], group["weight_decay"]
-        grads = batch.take_gradients(grads)
         first, lr, step, scalars = batch.params[0], group["lr"], 0, None
         with ops._on(first):
             if group["capturable"]:
