@@ -560,3 +560,36 @@ def test_a_step_that_is_refused_changes_nothing(dev, bits):
             with pytest.raises(ValueError):
                 opt.step()
             assert all(torch.equal(p, q) for p, q in zip(params, before)) and opt.param_groups[0]["step"] == k
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_layer_frozen_after_some_steps(dev, bits, monkeypatch):
+    """What is looked over once for the weights that go on is kept from step to step, and made anew when the others come back."""
+    from vtpack_amd import _lib
+    shapes = [(300,), (40, 30), (77,), (1025,)]
+    params = [torch.nn.Parameter(t) for t in _tensors(dev, shapes, torch.float32, 51)]
+    refs = [_Reference(p, bits) for p in params]
+    opt = _optimizer(params, bits)
+    real, made = _lib.training(), []
+
+    class Native:
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def adamw_batch(self, *args):
+            made.append(1)
+            return real.adamw_batch(*args)
+
+    wrapped = Native()
+    monkeypatch.setattr(_lib, "training", lambda: wrapped)
+    here = [(1, 1, 1, 1)] * 2 + [(1, 0, 0, 1)] * 4 + [(1, 1, 1, 1)] * 2 + [(1, 0, 0, 1)] * 2
+    for k, row in enumerate(here):
+        for p, g, there in zip(params, _tensors(dev, shapes, torch.float32, 140 + k, 1e-3), row):
+            p.grad = g if there else None
+        opt.step()
+        for p, r in zip(params, refs):
+            if p.grad is not None:
+                r.step(p.grad)
+                r.check(p, opt.state[p])
+        if k == 5:
+            assert len(made) == 2                          # of all weights, and of those that went on

@@ -166,7 +166,7 @@ class AdamW(torch.optim.Optimizer):
         """The batches of the group's last step that was not one call, where they still hold."""
         kept = self._batches.get(index)
         if kept is not None:
-            old, states, batches = kept
+            states, batches, old = kept
             now = list(self.state.values())
             if (len(params) == len(old) and all(map(operator.is_, params, old)) and len(now) == len(states)
                     and all(map(operator.is_, now, states)) and all(b.holds() and b.keys == _KEYS[group["state_bits"]] for b in batches)):
@@ -176,7 +176,7 @@ class AdamW(torch.optim.Optimizer):
     def _of_group(self, index, group, params, grads):
         batches = self._split(group, params, grads)
         self._batches = {i: b for i, b in self._batches.items() if i != index}
-        self._batches[index] = (params, list(self.state.values()), batches)
+        self._batches[index] = (list(self.state.values()), batches, list(params))
         return batches
 
     # ---------------------------------------------------------------- the step
@@ -245,8 +245,8 @@ class AdamW(torch.optim.Optimizer):
             self._natives = {i: b for i, b in self._natives.items() if i != index}
             if batch is None:
                 return False
-            self._natives[index] = (batch, skipped.pop(), bits)
-        batch, skipped, kept_bits = self._natives.get(index, (None, 0, 0))
+            self._natives[index] = (batch, skipped.pop(), bits, list(params))
+        batch, skipped, kept_bits, _ = self._natives.get(index, (None, 0, 0, ()))
         beta1, beta2 = group["betas"]
         if kept_bits != bits or not native.adamw_step(batch, params, self.state, group["lr"], beta1, beta2, group["eps"], group["weight_decay"],
                                                       int(group["step"]) + 1 - skipped, bits):
@@ -255,11 +255,14 @@ class AdamW(torch.optim.Optimizer):
         return True
 
     def _skip(self, index, params):
-        """Weights with states and without a gradient have missed this step."""
+        """Weights with states and without a gradient have missed this step.  What was prepared for others only is good for the next
+        one too; with one of these in it, its count of steps is no longer theirs."""
         for p in params:
             self.state[p]["skipped"] = self.state[p].get("skipped", 0) + 1
-            self._batches.pop(index, None)
-            self._natives.pop(index, None)
+        missed = set(map(id, params))
+        for prepared in (self._batches, self._natives):
+            if index in prepared and not missed.isdisjoint(map(id, prepared[index][-1])):
+                del prepared[index]
 
     def _launch(self, group, batch, last):
         (b1, b2), eps, decay = group["betas"], group["eps"], group["weight_decay"]
