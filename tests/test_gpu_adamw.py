@@ -593,3 +593,28 @@ def test_a_layer_frozen_after_some_steps(dev, bits, monkeypatch):
                 r.check(p, opt.state[p])
         if k == 5:
             assert len(made) == 2                          # of all weights, and of those that went on
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_in_another_order(dev, bits, monkeypatch):
+    """A state dict whose weights come in another order: a step is one native call all the same."""
+    from vtpack_amd import optim
+    looked = []
+    launch = optim.AdamW._launch
+    monkeypatch.setattr(optim.AdamW, "_launch", lambda self, *args: looked.append(1) or launch(self, *args))
+    shapes = [(300,), (40, 30), (77,), (5,)]
+    params = [torch.nn.Parameter(t) for t in _tensors(dev, shapes, torch.float32, 61)]
+    refs = [_Reference(p, bits) for p in params]
+    opt = _optimizer([{"params": params[:3]}, {"params": params[3:]}], bits)
+    for k in range(5):
+        for p, g, r in zip(params, _tensors(dev, shapes, torch.float32, 160 + k, 1e-3), refs):
+            p.grad = g
+            r.step(g)
+        if k == 2:
+            saved = opt.state_dict()
+            saved["state"] = dict(reversed(list(saved["state"].items())))
+            opt.load_state_dict(saved)
+        opt.step()
+        for p, r in zip(params, refs):
+            r.check(p, opt.state[p])
+    assert not looked

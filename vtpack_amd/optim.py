@@ -240,6 +240,13 @@ class AdamW(torch.optim.Optimizer):
             for p, state in zip(params, states):
                 if not any(k in state for k in _CODES):
                     state.update(self._lay_out(p, bits, int(group["step"])))
+            # the native call meets the states in the order of their weights
+            at = {id(p): i for i, p in enumerate(params)}
+            order = [at[id(p)] for p in self.state if id(p) in at]
+            if order != list(range(len(params))):
+                for p, state in zip(params, states):
+                    del self.state[p]
+                    self.state[p] = state
             skipped = {state.get("skipped", 0) for state in states}
             batch = native.adamw_batch(params, states, list(_KEYS[bits]), bits) if len(skipped) == 1 else None
             self._natives = {i: b for i, b in self._natives.items() if i != index}
