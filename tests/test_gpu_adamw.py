@@ -618,3 +618,37 @@ def test_states_in_another_order(dev, bits, monkeypatch):
         for p, r in zip(params, refs):
             r.check(p, opt.state[p])
     assert not looked
+
+
+def test_an_optimizer_that_its_weights_refer_to_is_collected(dev):
+    """A step inside a weight's own hook; and weights that move away leave no memory behind."""
+    import gc
+    import weakref
+    gc.collect()
+    used = torch.cuda.memory_allocated()
+    p = torch.nn.Parameter(torch.randn(1 << 20, device=dev))
+    opt = _optimizer([p], 32)
+    p.optimizer = opt
+    p.register_post_accumulate_grad_hook(lambda q: q.optimizer.step())
+    for _ in range(2):
+        (p * 2).sum().backward()
+    assert opt.param_groups[0]["step"] == 2
+    dead = weakref.ref(opt)
+    del p, opt
+    gc.collect()
+    assert dead() is None and torch.cuda.memory_allocated() <= used
+
+
+@pytest.mark.parametrize("strided", [False, True])
+def test_weights_that_move_away_leave_no_memory(dev, strided):
+    w = torch.randn(1 << 10, 1 << 10, device=dev)
+    p = torch.nn.Parameter(w.t() if strided else w)
+    opt = _optimizer([p], 32)
+    for _ in range(2):
+        p.grad = torch.full_like(p, 1e-3)
+        opt.step()
+    del w
+    p.grad = None
+    used = torch.cuda.memory_allocated()
+    p.data = p.data.cpu()
+    assert used - torch.cuda.memory_allocated() >= 4 << 20

@@ -274,16 +274,54 @@ std::array<Tensor, 2> balance(const Tensor &gate, const Tensor &indices, const T
 // put in another's place: the weights and their storage, their states and the tensors in them, the gradients.
 struct Batch {
     std::vector<PyObject *> params, states, moments, keys;      // moments: keys.size() of them for each state; all held
-    std::vector<Tensor> kept;                   // no other storage can come to lie where a weight or a moment is
-    std::vector<vtdge_adamw_tensor> table;
+    std::vector<vtdge_adamw_tensor> table;      // addresses of memory that is theirs; a step looks whether it still is
     at::ScalarType type, types[4];              // of the weights; of the moments
-    ~Batch()
+    ~Batch() { clear(); }
+    void clear()
     {
-        for (auto *list : {&params, &states, &moments, &keys})
-            for (PyObject *o : *list) Py_DECREF(o);
+        std::vector<PyObject *> all;
+        for (auto *list : {&params, &states, &moments, &keys}) {
+            all.insert(all.end(), list->begin(), list->end());
+            list->clear();
+        }
+        for (PyObject *o : all) Py_DECREF(o);
     }
 };
-const char *const BATCH = "vtpack_amd.adamw_batch";
+// The object that Python holds, which the garbage collector sees through: weights may refer to the optimizer that has it.
+struct BatchObject {
+    PyObject_HEAD
+    Batch *batch;
+};
+int batch_traverse(PyObject *self, visitproc visit, void *arg)
+{
+    Batch &b = *reinterpret_cast<BatchObject *>(self)->batch;
+    for (auto *list : {&b.params, &b.states, &b.moments, &b.keys})
+        for (PyObject *o : *list) Py_VISIT(o);
+    return 0;
+}
+int batch_clear(PyObject *self)
+{
+    reinterpret_cast<BatchObject *>(self)->batch->clear();
+    return 0;
+}
+void batch_dealloc(PyObject *self)
+{
+    PyObject_GC_UnTrack(self);
+    delete reinterpret_cast<BatchObject *>(self)->batch;
+    PyObject_GC_Del(self);
+}
+PyTypeObject *batch_type()
+{
+    static PyTypeObject type = {PyVarObject_HEAD_INIT(nullptr, 0)};
+    if (type.tp_name == nullptr) {
+        type.tp_name = "vtpack_amd._training.Batch";
+        type.tp_doc = "The weights of an AdamW step, ready for it.";
+        type.tp_basicsize = sizeof(BatchObject);
+        type.tp_flags = Py_TPFLAGS_DEFAULT | Py_TPFLAGS_HAVE_GC;
+        type.tp_traverse = batch_traverse, type.tp_clear = batch_clear, type.tp_dealloc = batch_dealloc;
+    }
+    return &type;
+}
 
 std::vector<PyObject *> held(PyObject *list)
 {
@@ -304,7 +342,7 @@ bool same(const std::vector<PyObject *> &kept, PyObject *list)
 // Everything as it was, and a gradient for every weight that can be read as it lies; its address into the table then.
 bool ready(Batch &b, PyObject *params, PyObject *state)
 {
-    if (!same(b.params, params)) return false;
+    if (b.params.empty() || !same(b.params, params)) return false;
     // states lie in the order of their weights, other groups' between them
     Py_ssize_t at = 0;
     PyObject *key, *value;
@@ -320,10 +358,10 @@ bool ready(Batch &b, PyObject *params, PyObject *state)
             PyObject *const m = b.moments[i * of + k];
             if (PyDict_GetItem(b.states[i], b.keys[k]) != m) return false;
             const Tensor &t = THPVariable_Unpack(m);
-            if (t.data_ptr() != lies[k] || t.numel() != (k < 2 ? row.n : (row.n + 255) / 256) || t.scalar_type() != b.types[k] || !t.is_contiguous()) return false;
+            if (t.data_ptr() != lies[k] || !t.is_cuda() || t.numel() != (k < 2 ? row.n : (row.n + 255) / 256) || t.scalar_type() != b.types[k] || !t.is_contiguous()) return false;
         }
         const Tensor &p = THPVariable_Unpack(b.params[i]), &g = p.grad();
-        if (p.data_ptr() != row.param || p.numel() != row.n || p.scalar_type() != b.type || !p.is_contiguous() || !g.defined() ||
+        if (p.data_ptr() != row.param || !p.is_cuda() || p.numel() != row.n || p.scalar_type() != b.type || !p.is_contiguous() || !g.defined() ||
             g.layout() != at::kStrided || g.scalar_type() != b.type || g.device() != p.device() || g.sizes() != p.sizes() || !g.is_contiguous())
             return false;
         row.grad = g.data_ptr();
@@ -622,14 +660,13 @@ PyObject *py_adamw_batch(PyObject *, PyObject *const *a, Py_ssize_t n)
         at::ScalarType *const types = b->types;
         types[0] = bytes ? at::kFloat8_e4m3fn : at::kFloat, types[1] = bytes ? at::kFloat8_e5m2 : at::kFloat, types[2] = types[3] = at::kFloat;
         std::vector<std::pair<uintptr_t, uintptr_t>> lie;
+        at::Device device = at::kCPU;
         for (size_t i = 0; i < b->params.size(); i++) {
             const Tensor p = tensor(b->params[i]);
-            if (i == 0) b->type = p.scalar_type();
-            const Tensor &first = i == 0 ? p : b->kept.front();
+            if (i == 0 && p.defined()) b->type = p.scalar_type(), device = p.device();
             if (!p.defined() || !p.is_cuda() || p.layout() != at::kStrided || !p.is_contiguous() || p.scalar_type() != b->type ||
-                p.device() != first.device() || (b->type != at::kFloat && b->type != at::kBFloat16) || !PyDict_Check(b->states[i]))
+                p.device() != device || (b->type != at::kFloat && b->type != at::kBFloat16) || !PyDict_Check(b->states[i]))
                 Py_RETURN_NONE;
-            b->kept.push_back(p.detach());
             void *at[4] = {};
             for (size_t k = 0; k < b->keys.size(); k++) {
                 PyObject *const o = PyDict_GetItem(b->states[i], b->keys[k]);
@@ -640,7 +677,6 @@ PyObject *py_adamw_batch(PyObject *, PyObject *const *a, Py_ssize_t n)
                     Py_RETURN_NONE;
                 Py_INCREF(o);
                 b->moments.push_back(o);
-                b->kept.push_back(m.detach());
                 at[k] = m.data_ptr();
             }
             vtdge_adamw_tensor x{};
@@ -652,7 +688,11 @@ PyObject *py_adamw_batch(PyObject *, PyObject *const *a, Py_ssize_t n)
         std::sort(lie.begin(), lie.end());
         for (size_t i = 1; i < lie.size(); i++)
             if (lie[i].first < lie[i - 1].second) Py_RETURN_NONE;
-        return PyCapsule_New(b.release(), BATCH, [](PyObject *o) { delete static_cast<Batch *>(PyCapsule_GetPointer(o, BATCH)); });
+        BatchObject *const out = PyObject_GC_New(BatchObject, batch_type());
+        if (out == nullptr) throw python_error();
+        out->batch = b.release();
+        PyObject_GC_Track(out);
+        return reinterpret_cast<PyObject *>(out);
     });
 }
 // (batch, the group's weights, the optimizer's states, lr, beta1, beta2, eps, decay, step, bits): whether the step was made; if
@@ -660,8 +700,8 @@ PyObject *py_adamw_batch(PyObject *, PyObject *const *a, Py_ssize_t n)
 PyObject *py_adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 10, [&]() -> PyObject * {
-        Batch *const b = static_cast<Batch *>(PyCapsule_GetPointer(a[0], BATCH));
-        if (b == nullptr) throw python_error();
+        if (Py_TYPE(a[0]) != batch_type()) throw std::runtime_error("adamw_step: expected a batch");
+        Batch *const b = reinterpret_cast<BatchObject *>(a[0])->batch;
         double rate[5];
         for (int i = 0; i < 5; i++) rate[i] = real(a[3 + i]);
         const int64_t step = whole(a[8]), bits = whole(a[9]);
@@ -695,4 +735,4 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_training", "The operators of a tr
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__training() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__training() { return PyType_Ready(batch_type()) < 0 ? nullptr : PyModule_Create(&module); }

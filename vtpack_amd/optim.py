@@ -32,7 +32,6 @@ class _Batch:
         self.params, self.states, self.skipped, self.keys = params, states, skipped, _KEYS[bits]
         self.moments = [[s[k] for s in states] for k in self.keys]
         self.tensors = list(itertools.chain(params, *self.moments))
-        self.kept = [t.detach() for t in self.tensors]         # no other storage can come to lie where one of these is
         self.at = _lib.training().places(self.tensors)
         self.plain = all(p.is_contiguous() for p in params)
         self.table = np.zeros((len(params), 7), dtype=np.uint64)
