@@ -560,3 +560,32 @@ def test_fp32_next_to_the_smallest_numbers(dev):
     z = x.double() @ w.double().t()
     bound = 2 * 2.0 ** -134 * float(w.double().abs().sum(1).max()) + _tolerance(x, w) * (1 + float(z.abs().max()))
     assert float((got.double() - want).abs().max()) <= bound
+
+
+def test_hooks_see_what_is_kept_for_the_gradients(dev):
+    """Logits and laid out operands go where saved tensors go: a checkpointed loss keeps none of them, an offloaded one has them on the
+    host."""
+    from torch.autograd.graph import saved_tensors_hooks
+    from torch.utils.checkpoint import checkpoint
+    from vtpack_amd.layers import gate_balance, linear_cross_entropy
+    x, w, b, t = _operands(dev, 1024, 8192, 64, torch.float32)            # logits of 32 MB
+    leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+    want = torch.autograd.grad(linear_cross_entropy(*leaves, t), leaves)
+    torch.cuda.synchronize()
+    for way in ("checkpoint", "host"):
+        before = torch.cuda.memory_allocated()
+        if way == "checkpoint":
+            loss = checkpoint(linear_cross_entropy, *leaves, t, use_reentrant=False)
+        else:
+            sizes = []
+            with saved_tensors_hooks(lambda v: sizes.append(v.nbytes) or v.cpu(), lambda v: v.to(dev)):
+                loss = linear_cross_entropy(*leaves, t)
+            assert max(sizes) >= 32 << 20
+        assert torch.cuda.memory_allocated() - before < 1 << 20
+        got = torch.autograd.grad(loss, leaves)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    sizes = []
+    with saved_tensors_hooks(lambda v: sizes.append(v.nbytes) or v.cpu(), lambda v: v.to(dev)):
+        loss, _ = gate_balance(leaves[0])
+    assert len(sizes) == 2
+    loss.backward()

@@ -169,20 +169,19 @@ void no_tracing(const char *name)
 
 // The backward node of a loss, with what it reads as members.
 struct LinearCrossEntropyBackward : torch::autograd::Node {
-    SavedVariable x, w, bias, target;
-    Tensor stats, laid_out;                     // nobody else's
+    SavedVariable x, w, bias, target, stats, laid_out;      // (the last two for hooks on saved tensors to see: up to 320 MB)
     int64_t ignore; double smoothing; int reduction;
 
     variable_list apply(variable_list &&grads) override
     {
         no_second_order("linear_cross_entropy");
         std::lock_guard<std::mutex> hold(mutex_);
-        const Tensor x_ = x.unpack(), w_ = w.unpack(), b_ = bias.unpack(), t_ = target.unpack();
+        const Tensor x_ = x.unpack(), w_ = w.unpack(), b_ = bias.unpack(), t_ = target.unpack(), s_ = stats.unpack(), l_ = laid_out.unpack();
         Tensor grad = grads[0];
         if (!grad.defined()) return {Tensor(), Tensor(), Tensor()};
         // the same for every row, as a sum over the losses leaves it: one value
         if (grad.dim() == 1) grad = grad.stride(0) == 0 ? grad.select(0, 0) : grad.contiguous();
-        const auto out = cross_entropy_backward(x_, w_, b_, t_, stats, laid_out, grad, ignore, smoothing, reduction,
+        const auto out = cross_entropy_backward(x_, w_, b_, t_, s_, l_, grad, ignore, smoothing, reduction,
                                                 {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2)});
         return {out[0], out[1], out[2]};
     }
@@ -190,7 +189,7 @@ struct LinearCrossEntropyBackward : torch::autograd::Node {
     {
         std::lock_guard<std::mutex> hold(mutex_);
         x.reset_data(), w.reset_data(), bias.reset_data(), target.reset_data();
-        stats.reset(), laid_out.reset();
+        stats.reset_data(), laid_out.reset_data();
     }
     std::string name() const override { return "LinearCrossEntropyBackward"; }
 };
@@ -204,7 +203,7 @@ Tensor linear_cross_entropy(const Tensor &x, const Tensor &w, const Tensor &bias
         node->set_next_edges(torch::autograd::collect_next_edges(x, w, bias));
         node->x = SavedVariable(x, false), node->w = SavedVariable(w, false), node->bias = SavedVariable(bias, false);
         node->target = SavedVariable(target, false);
-        node->stats = f.stats, node->laid_out = f.laid_out;
+        node->stats = SavedVariable(f.stats, false), node->laid_out = SavedVariable(f.laid_out, false);
         node->ignore = ignore, node->smoothing = smoothing, node->reduction = reduction;
         torch::autograd::set_history(f.loss, node);
     }
@@ -239,20 +238,19 @@ Tensor gate_balance_backward(const Tensor &gate, const Tensor &mask, const Tenso
 }
 
 struct GateBalanceBackward : torch::autograd::Node {
-    SavedVariable gate, mask;
-    Tensor share;
+    SavedVariable gate, mask, share;
 
     variable_list apply(variable_list &&grads) override
     {
         no_second_order("gate_balance");
         std::lock_guard<std::mutex> hold(mutex_);
-        const Tensor gate_ = gate.unpack(), mask_ = mask.unpack();
-        return {grads[0].defined() ? gate_balance_backward(gate_, mask_, share, grads[0]) : Tensor()};
+        const Tensor gate_ = gate.unpack(), mask_ = mask.unpack(), share_ = share.unpack();
+        return {grads[0].defined() ? gate_balance_backward(gate_, mask_, share_, grads[0]) : Tensor()};
     }
     void release_variables() override
     {
         std::lock_guard<std::mutex> hold(mutex_);
-        gate.reset_data(), mask.reset_data(), share.reset();
+        gate.reset_data(), mask.reset_data(), share.reset_data();
     }
     std::string name() const override { return "GateBalanceBackward"; }
 };
@@ -263,7 +261,8 @@ std::array<Tensor, 2> balance(const Tensor &gate, const Tensor &indices, const T
     if (torch::autograd::compute_requires_grad(gate)) {
         auto node = std::shared_ptr<GateBalanceBackward>(new GateBalanceBackward, torch::autograd::deleteNode);
         node->set_next_edges(torch::autograd::collect_next_edges(gate));
-        node->gate = SavedVariable(gate, false), node->mask = SavedVariable(mask, false), node->share = out[2];
+        node->gate = SavedVariable(gate, false), node->mask = SavedVariable(mask, false);
+        node->share = SavedVariable(out[2], false);
         torch::autograd::set_history(out[0], node);
     }
     return {out[0], out[1]};
