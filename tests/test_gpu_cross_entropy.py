@@ -589,3 +589,30 @@ def test_hooks_see_what_is_kept_for_the_gradients(dev):
         loss, _ = gate_balance(leaves[0])
     assert len(sizes) == 2
     loss.backward()
+
+
+@pytest.mark.parametrize("back", ["cpu", "short", "type", "wide"])
+def test_hooks_that_bring_back_something_else(dev, back):
+    """What unpacking hooks return is looked at before a kernel reads it."""
+    from torch.autograd.graph import saved_tensors_hooks
+    from vtpack_amd.layers import gate_balance, linear_cross_entropy
+    x, w, b, t = _operands(dev, 50, 60, 64, torch.float32)
+    leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+    change = {"cpu": lambda v: v.cpu(), "short": lambda v: v[:len(v) // 2], "type": lambda v: v.half() if v.is_floating_point() else v.int(),
+              "wide": lambda v: torch.stack([v, v], -1)[..., 0]}[back]
+    for which in range(6):
+        seen = []
+
+        def unpack(v):
+            seen.append(1)
+            return change(v) if len(seen) == which + 1 else v
+
+        with saved_tensors_hooks(lambda v: v, unpack):
+            loss = linear_cross_entropy(*leaves, t)
+        with pytest.raises(RuntimeError, match="^linear_cross_entropy: "):
+            torch.autograd.grad(loss, leaves)
+        assert len(seen) == 6
+    with saved_tensors_hooks(lambda v: v, change):
+        loss, _ = gate_balance(leaves[0], mask=t > 3)
+    with pytest.raises(RuntimeError, match="^gate_balance: "):
+        loss.backward()

@@ -145,6 +145,60 @@ std::array<Tensor, 3> cross_entropy_backward(const Tensor &x, const Tensor &w, c
     return out;
 }
 
+// ------------------------------------------------------------------------------------------------ forms of operands
+bool rows_of_any_place(const Tensor &t)
+{
+    return t.defined() && t.dim() == 2 && t.numel() > 0 && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) &&
+           t.layout() == at::kStrided && (t.is_contiguous() || (t.stride(1) == 1 && t.stride(0) >= t.size(1)));
+}
+bool plain_rows(const Tensor &t) { return t.defined() && t.is_cuda() && rows_of_any_place(t); }
+bool plain_beside(const Tensor &t, const Tensor &x, at::ScalarType type)
+{
+    return t.defined() && t.device() == x.device() && t.scalar_type() == type && t.layout() == at::kStrided && t.is_contiguous();
+}
+
+// Operands that are taken as they are: one that does not fit is named before anything is launched, the place of all of them last.
+struct Operands {
+    const char *name;
+    void need(bool fits, const char *what) const
+    {
+        if (!fits) throw std::runtime_error(std::string(name) + ": " + what);
+    }
+    void on_gpu(const Tensor &x) const { need(x.is_cuda(), "operands have to be on a GPU"); }
+
+    void loss(const Tensor &x, const Tensor &w, const Tensor &b, const Tensor &t, double smoothing, int64_t reduction) const
+    {
+        need(rows_of_any_place(x), "x has to be [rows, width] of float32 or bfloat16 with dense rows");
+        need(rows_of_any_place(w) && w.device() == x.device() && w.scalar_type() == x.scalar_type() && w.size(1) == x.size(1),
+             "weight has to be [classes, width] beside x, of its type, with dense rows");
+        need(!b.defined() || (plain_beside(b, x, x.scalar_type()) && b.dim() == 1 && b.size(0) == w.size(0)), "bias has to be [classes] beside x, of its type, dense");
+        need(plain_beside(t, x, at::kLong) && t.dim() == 1 && t.size(0) == x.size(0), "target has to be int64 [rows] beside x, dense");
+        need(smoothing >= 0 && smoothing <= 1, "label_smoothing has to be 0 .. 1");
+        need(reduction >= NONE && reduction <= SUM, "no such reduction");
+    }
+    void loss_gradients(const Tensor &x, const Tensor &w, const Tensor &stats, const Tensor &laid_out, const Tensor &grad, int64_t reduction) const
+    {
+        need(plain_beside(stats, x, at::kFloat) && stats.dim() == 1 && stats.size(0) == 3 * x.size(0) + 1, "stats has to be that of the forward call");
+        need(!laid_out.defined() ||
+                 (plain_beside(laid_out, x, at::kByte) && laid_out.numel() >= lib.cross_entropy_laid_out(x.size(0), w.size(0), Rows(x, w).width, code_of(x))),
+             "laid_out has to be that of the forward call");
+        need(plain_beside(grad, x, at::kFloat) && (grad.dim() == 0 || (grad.dim() == 1 && reduction == NONE && grad.size(0) == x.size(0))),
+             "grad has to be float32 beside x: a scalar, or with a loss for each row a value for each");
+    }
+    void gate(const Tensor &g, const Tensor &m) const
+    {
+        need(rows_of_any_place(g) && g.size(1) <= VTDGE_MAX_EXPERTS, "gate has to be [tokens, 1 .. 512] of float32 or bfloat16 with dense rows");
+        need(!m.defined() || ((plain_beside(m, g, at::kBool) || plain_beside(m, g, at::kByte)) && m.dim() == 1 && m.size(0) == g.size(0)),
+             "mask has to be [tokens] of bytes beside the gate, dense");
+    }
+    void gate_gradients(const Tensor &g, const Tensor &share, const Tensor &grad) const
+    {
+        need(plain_beside(share, g, at::kFloat) && share.dim() == 1 && share.size(0) == lib.gate_balance_workspace(g.size(0), (int)g.size(1)) / 4 + g.size(1) + 1,
+             "share has to be that of the forward call");
+        need(plain_beside(grad, g, at::kFloat) && grad.dim() == 0, "grad has to be a float32 scalar beside the gate");
+    }
+};
+
 void no_second_order(const char *name)
 {
     if (at::GradMode::is_enabled()) throw std::runtime_error(std::string(name) + ": gradients of the gradients are not supported");
@@ -181,6 +235,11 @@ struct LinearCrossEntropyBackward : torch::autograd::Node {
         if (!grad.defined()) return {Tensor(), Tensor(), Tensor()};
         // the same for every row, as a sum over the losses leaves it: one value
         if (grad.dim() == 1) grad = grad.stride(0) == 0 ? grad.select(0, 0) : grad.contiguous();
+        // (hooks on saved tensors may have brought others)
+        const Operands check{"linear_cross_entropy"};
+        check.loss(x_, w_, b_, t_, smoothing, reduction);
+        check.loss_gradients(x_, w_, s_, l_, grad, reduction);
+        check.on_gpu(x_);
         const auto out = cross_entropy_backward(x_, w_, b_, t_, s_, l_, grad, ignore, smoothing, reduction,
                                                 {task_should_compute_output(0), task_should_compute_output(1), task_should_compute_output(2)});
         return {out[0], out[1], out[2]};
@@ -245,7 +304,12 @@ struct GateBalanceBackward : torch::autograd::Node {
         no_second_order("gate_balance");
         std::lock_guard<std::mutex> hold(mutex_);
         const Tensor gate_ = gate.unpack(), mask_ = mask.unpack(), share_ = share.unpack();
-        return {grads[0].defined() ? gate_balance_backward(gate_, mask_, share_, grads[0]) : Tensor()};
+        if (!grads[0].defined()) return {Tensor()};
+        const Operands check{"gate_balance"};
+        check.gate(gate_, mask_);
+        check.gate_gradients(gate_, share_, grads[0]);
+        check.on_gpu(gate_);
+        return {gate_balance_backward(gate_, mask_, share_, grads[0])};
     }
     void release_variables() override
     {
@@ -438,16 +502,6 @@ PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t n)
 // Operands as the kernels take them.  The entry points below answer None to any other, for their callers to bring them into this
 // form or to say what is wrong with them.
 bool number(PyObject *o) { return PyLong_Check(o) || PyFloat_Check(o); }
-bool rows_of_any_place(const Tensor &t)
-{
-    return t.defined() && t.dim() == 2 && t.numel() > 0 && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) &&
-           t.layout() == at::kStrided && (t.is_contiguous() || (t.stride(1) == 1 && t.stride(0) >= t.size(1)));
-}
-bool plain_rows(const Tensor &t) { return t.defined() && t.is_cuda() && rows_of_any_place(t); }
-bool plain_beside(const Tensor &t, const Tensor &x, at::ScalarType type)
-{
-    return t.defined() && t.device() == x.device() && t.scalar_type() == type && t.layout() == at::kStrided && t.is_contiguous();
-}
 
 // (x, weight, bias or None, target, ignore_index, label_smoothing, reduction's code)
 PyObject *py_linear_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
@@ -472,53 +526,26 @@ PyObject *py_linear_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
         return wrap(loss);
     });
 }
-
-// The calls below take their operands as they are: one that does not fit is named before anything is launched, the place of all of them
-// last.
-struct Operands {
-    const char *name;
-    void need(bool fits, const char *what) const
-    {
-        if (!fits) throw std::runtime_error(std::string(name) + ": " + what);
-    }
-    Tensor get(PyObject *o, const char *what) const
-    {
-        need(o == Py_None || THPVariable_Check(o), what);
-        return tensor(o);
-    }
-    void on_gpu(const Tensor &x) const { need(x.is_cuda(), "operands have to be on a GPU"); }
-
-    // x, weight, bias or None, target; the rest of a loss
-    std::array<Tensor, 4> of_loss(PyObject *const *a, double smoothing, int64_t reduction) const
-    {
-        const Tensor x = get(a[0], "x has to be a tensor"), w = get(a[1], "weight has to be a tensor"), b = get(a[2], "bias has to be a tensor or None"),
-                     t = get(a[3], "target has to be a tensor");
-        need(rows_of_any_place(x), "x has to be [rows, width] of float32 or bfloat16 with dense rows");
-        need(rows_of_any_place(w) && w.device() == x.device() && w.scalar_type() == x.scalar_type() && w.size(1) == x.size(1),
-             "weight has to be [classes, width] beside x, of its type, with dense rows");
-        need(!b.defined() || (plain_beside(b, x, x.scalar_type()) && b.dim() == 1 && b.size(0) == w.size(0)), "bias has to be [classes] beside x, of its type, dense");
-        need(plain_beside(t, x, at::kLong) && t.dim() == 1 && t.size(0) == x.size(0), "target has to be int64 [rows] beside x, dense");
-        need(smoothing >= 0 && smoothing <= 1, "label_smoothing has to be 0 .. 1");
-        need(reduction >= NONE && reduction <= SUM, "no such reduction");
-        return {x, w, b, t};
-    }
-    // gate and mask or None
-    std::array<Tensor, 2> of_gate(PyObject *gate, PyObject *mask) const
-    {
-        const Tensor g = get(gate, "gate has to be a tensor"), m = get(mask, "mask has to be a tensor or None");
-        need(rows_of_any_place(g) && g.size(1) <= VTDGE_MAX_EXPERTS, "gate has to be [tokens, 1 .. 512] of float32 or bfloat16 with dense rows");
-        need(!m.defined() || ((plain_beside(m, g, at::kBool) || plain_beside(m, g, at::kByte)) && m.dim() == 1 && m.size(0) == g.size(0)),
-             "mask has to be [tokens] of bytes beside the gate, dense");
-        return {g, m};
-    }
-};
+// a tensor, or None where that may be
+Tensor operand(const Operands &check, PyObject *o, const char *what)
+{
+    check.need(o == Py_None || THPVariable_Check(o), what);
+    return tensor(o);
+}
+std::array<Tensor, 4> of_loss(const Operands &check, PyObject *const *a, double smoothing, int64_t reduction)
+{
+    const std::array<Tensor, 4> t = {operand(check, a[0], "x has to be a tensor"), operand(check, a[1], "weight has to be a tensor"),
+                                     operand(check, a[2], "bias has to be a tensor or None"), operand(check, a[3], "target has to be a tensor")};
+    check.loss(t[0], t[1], t[2], t[3], smoothing, reduction);
+    return t;
+}
 PyObject *py_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 7, [&] {
         const Operands check{"cross_entropy"};
         const int64_t ignore = whole(a[4]), reduction = whole(a[6]);
         const double smoothing = real(a[5]);
-        const auto [x, w, b, t] = check.of_loss(a, smoothing, reduction);
+        const auto [x, w, b, t] = of_loss(check, a, smoothing, reduction);
         check.on_gpu(x);
         Forward f;
         {
@@ -535,15 +562,10 @@ PyObject *py_cross_entropy_backward(PyObject *, PyObject *const *a, Py_ssize_t n
         const int64_t ignore = whole(a[7]), reduction = whole(a[9]);
         const double smoothing = real(a[8]);
         const std::array<bool, 3> needs = {whole(a[10]) != 0, whole(a[11]) != 0, whole(a[12]) != 0};
-        const auto [x, w, b, t] = check.of_loss(a, smoothing, reduction);
-        const Tensor stats = check.get(a[4], "stats has to be a tensor"), laid_out = check.get(a[5], "laid_out has to be a tensor or None"),
-                     grad = check.get(a[6], "grad has to be a tensor");
-        check.need(plain_beside(stats, x, at::kFloat) && stats.dim() == 1 && stats.size(0) == 3 * x.size(0) + 1, "stats has to be that of the forward call");
-        check.need(!laid_out.defined() || (plain_beside(laid_out, x, at::kByte) &&
-                                           laid_out.numel() >= lib.cross_entropy_laid_out(x.size(0), w.size(0), Rows(x, w).width, code_of(x))),
-                   "laid_out has to be that of the forward call");
-        check.need(plain_beside(grad, x, at::kFloat) && (grad.dim() == 0 || (grad.dim() == 1 && reduction == NONE && grad.size(0) == x.size(0))),
-                   "grad has to be float32 beside x: a scalar, or with a loss for each row a value for each");
+        const auto [x, w, b, t] = of_loss(check, a, smoothing, reduction);
+        const Tensor stats = operand(check, a[4], "stats has to be a tensor"), laid_out = operand(check, a[5], "laid_out has to be a tensor or None"),
+                     grad = operand(check, a[6], "grad has to be a tensor");
+        check.loss_gradients(x, w, stats, laid_out, grad, reduction);
         check.on_gpu(x);
         std::array<Tensor, 3> out;
         {
@@ -581,8 +603,9 @@ PyObject *py_gate_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
     return call(a, n, 4, [&] {
         const Operands check{"gate_balance"};
         const int64_t top_k = whole(a[3]);
-        const auto [gate, mask] = check.of_gate(a[0], a[2]);
-        const Tensor indices = check.get(a[1], "indices have to be a tensor or None");
+        const Tensor gate = operand(check, a[0], "gate has to be a tensor"), indices = operand(check, a[1], "indices have to be a tensor or None"),
+                     mask = operand(check, a[2], "mask has to be a tensor or None");
+        check.gate(gate, mask);
         check.need(top_k >= 1 && top_k <= (indices.defined() ? VTDGE_MAX_EXPERTS : gate.size(1)), "top_k has to be 1 .. the number of logits");
         check.need(!indices.defined() || (plain_beside(indices, gate, at::kLong) && indices.dim() == 2 && indices.size(0) == gate.size(0) && indices.size(1) == top_k),
                    "indices have to be int64 [tokens, top_k] beside the gate, dense");
@@ -599,12 +622,10 @@ PyObject *py_gate_balance_backward(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 4, [&] {
         const Operands check{"gate_balance_backward"};
-        const auto [gate, mask] = check.of_gate(a[0], a[1]);
-        const Tensor share = check.get(a[2], "share has to be a tensor"), grad = check.get(a[3], "grad has to be a tensor");
-        check.need(plain_beside(share, gate, at::kFloat) && share.dim() == 1 &&
-                       share.size(0) == lib.gate_balance_workspace(gate.size(0), (int)gate.size(1)) / 4 + gate.size(1) + 1,
-                   "share has to be that of the forward call");
-        check.need(plain_beside(grad, gate, at::kFloat) && grad.dim() == 0, "grad has to be a float32 scalar beside the gate");
+        const Tensor gate = operand(check, a[0], "gate has to be a tensor"), mask = operand(check, a[1], "mask has to be a tensor or None"),
+                     share = operand(check, a[2], "share has to be a tensor"), grad = operand(check, a[3], "grad has to be a tensor");
+        check.gate(gate, mask);
+        check.gate_gradients(gate, share, grad);
         check.on_gpu(gate);
         Tensor out;
         {
