@@ -626,9 +626,10 @@ int vtdge_gate_balance_backward(const void *gate, int64_t pitch, const uint8_t *
  * largest finite number; a smaller one is off by 2^-134 at most.  An infinity among the features of a row that counts or the
  * weights of a class makes NaN of the logits it meets, also where fp32 products would make an infinity.
  *   workspace  vtdge_cross_entropy_workspace(..., how) bytes, 256-byte aligned, contents do not matter.  how: a sum of
- *             VTDGE_CE_BACKWARD, for the gradients, VTDGE_CE_KEEPS, for a forward call with `keeps`, and VTDGE_CE_X_LIES, VTDGE_CE_WEIGHT_LIES, for operands that are read where
- *             they lie and need no room: bf16, width a multiple of 64, rows a multiple of 8 elements and less than 2^22 apart,
- *             on a 16-byte boundary */
+ *             VTDGE_CE_BACKWARD, for the gradients, VTDGE_CE_KEEPS, for a forward call with `keeps` and for gradients with its
+ *             `laid_out`, and VTDGE_CE_X_LIES, VTDGE_CE_WEIGHT_LIES, for operands that are read where they lie and need no
+ *             room: bf16, width a multiple of 64, rows a multiple of 8 elements and less than 2^22 apart, on a 16-byte
+ *             boundary */
 #define VTDGE_CE_BACKWARD 1
 #define VTDGE_CE_X_LIES 2
 #define VTDGE_CE_WEIGHT_LIES 4

@@ -276,3 +276,11 @@ def test_how_a_loss_is_made_goes_with_a_target():
     m = VisionTransformer(img_size=64, patch_size=8, embed_dim=64, depth=1, num_heads=1, mlp_ratio=2, num_classes=7, split_sizes=[4, 2, 1])
     with pytest.raises(TypeError, match="label_smoothing without a target"):
         m(torch.randn(1, 3, 64, 64), label_smoothing=0.1)
+
+
+def test_gradients_with_operands_laid_out_before_need_no_room_for_them():
+    size = _lib.load().vtdge_cross_entropy_workspace
+    x, w = 2048 * 384 * 6, 21841 * 384 * 6
+    assert size(2048, 21841, 384, 0, 1) - size(2048, 21841, 384, 0, 1 + 8) == -(-x // 256) * 256 + -(-w // 256) * 256
+    # bf16 that is read where it lies has its x with zeros for the rows that are left out all the same
+    assert size(256, 1000, 384, 1, 1 + 2 + 4) == size(256, 1000, 384, 1, 1 + 2 + 4 + 8)

@@ -1027,7 +1027,8 @@ static bool large_logits(int64_t rows, int64_t classes, int padded)
 static int64_t z_pitch(int64_t classes) { return (classes + 7) / 8 * 8; }
 static bool keeps_logits(int64_t rows, int64_t classes, int dtype) { return dtype == VTDGE_F32 && rows * z_pitch(classes) * 4 <= CE_KEPT_BYTES; }
 
-// (x_lies, w_lies: read where they lie, see lies_well; the gradients want room for x with zeros in any case)
+// (x_lies, w_lies: read where they lie, see lies_well; the gradients want room for x with zeros all the same.  keeps: of a forward
+// call, room for the logits too; of the gradients, what it laid out is at hand and needs no room)
 static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool backward, bool x_lies, bool w_lies, bool keeps)
 {
     CePlan p{};
@@ -1049,9 +1050,10 @@ static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool 
     else shape(LogitsLarge{}, LogitsMiddle{}, LogitsFlat{}, LogitsSmall{});
     p.tm = ceil_div(rows, p.lm), p.tn = ceil_div(classes, p.ln);
     int64_t at = 0;
-    p.x_at = take(at, x_lies && !backward ? 0 : rows * p.padded * 2 * p.parts);
-    p.w_at = take(at, w_lies ? 0 : classes * p.padded * 2 * p.parts);
-    p.kept_at = take(at, keeps && keeps_logits(rows, classes, dtype) ? rows * z_pitch(classes) * 4 : 0);
+    const bool at_hand = backward && keeps;
+    p.x_at = take(at, (x_lies && !backward) || (!x_lies && at_hand) ? 0 : rows * p.padded * 2 * p.parts);
+    p.w_at = take(at, w_lies || at_hand ? 0 : classes * p.padded * 2 * p.parts);
+    p.kept_at = take(at, !backward && keeps && keeps_logits(rows, classes, dtype) ? rows * z_pitch(classes) * 4 : 0);
     if (!backward) {
         p.max_at = take(at, p.tn * rows * 4);
         p.sum_at = take(at, p.tn * rows * 4);
@@ -1277,7 +1279,7 @@ extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const vo
     VT_REQUIRE(grad_stride == 0 || (grad_stride == 1 && inv_count == nullptr), VTDGE_ERR_ARG, "cross_entropy_backward: grad_stride %d", grad_stride);
     VT_REQUIRE(smoothing >= 0.f && smoothing <= 1.f, VTDGE_ERR_ARG, "cross_entropy_backward: smoothing %g", (double)smoothing);
     const bool x_lies = lies_well(x, ldx, width, dtype), w_lies = lies_well(weight, ldw, width, dtype);
-    const CePlan p = plan_of(rows, classes, width, dtype, true, x_lies, w_lies, false);
+    const CePlan p = plan_of(rows, classes, width, dtype, true, x_lies, w_lies, laid_out != nullptr);
     VT_REQUIRE(workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG,
                "cross_entropy_backward: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.bytes);
     if (dx == nullptr && dweight == nullptr && dbias == nullptr) return VTDGE_OK;

@@ -131,7 +131,7 @@ std::array<Tensor, 3> cross_entropy_backward(const Tensor &x, const Tensor &w, c
 {
     const c10::DeviceGuard guard(x.device());
     const Rows s(x, w);
-    const Tensor ws = fresh(x, {s.workspace(true, false)}, at::kByte);
+    const Tensor ws = fresh(x, {s.workspace(true, laid_out.defined())}, at::kByte);
     std::array<Tensor, 3> out;
     if (needs[0]) out[0] = fresh(x, {s.rows, s.width}, x.scalar_type());
     if (needs[1]) out[1] = fresh(x, {s.classes, s.width}, x.scalar_type());
