@@ -616,3 +616,21 @@ def test_hooks_that_bring_back_something_else(dev, back):
         loss, _ = gate_balance(leaves[0], mask=t > 3)
     with pytest.raises(RuntimeError, match="^gate_balance: "):
         loss.backward()
+
+
+@pytest.mark.parametrize("rows,classes,width,kept", [(8192, 8192, 64, True), (8192, 9001, 72, False), (16411, 4000, 40, True), (60000, 2100, 64, False)])
+def test_fp32_gradients_over_pieces(dev, rows, classes, width, kept):
+    """Classes in more than one piece, the last of them shorter, with d from kept logits and worked out again."""
+    from vtpack_amd import _lib, ops
+    x, w, b, t = _operands(dev, rows, classes, width, torch.float32, left_out=0.1)
+    one = torch.ones((), device=dev)
+    loss, stats, laid_out = ops.cross_entropy(x, w, b, t)
+    again = ops.cross_entropy_backward(x, w, b, t, stats, None, one)
+    pieces = [_lib.last_kernel(k) for k in range(8)]
+    assert sum("cross_entropy_grad_kernel" in n for n in pieces) >= 2 and sum("cross_entropy_d_kernel" in n for n in pieces) >= 2
+    if laid_out is not None:
+        got = ops.cross_entropy_backward(x, w, b, t, stats, laid_out, one)
+        used = [_lib.last_kernel(k) for k in range(6)]
+        assert (sum("cross_entropy_d_kept_kernel" in n for n in used) >= 2) == kept
+        assert all(torch.equal(p, q) for p, q in zip(again, got))
+    _check(x, w, b, t, smoothing=0.1)
