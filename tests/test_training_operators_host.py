@@ -284,3 +284,13 @@ def test_gradients_with_operands_laid_out_before_need_no_room_for_them():
     assert size(2048, 21841, 384, 0, 1) - size(2048, 21841, 384, 0, 1 + 8) == -(-x // 256) * 256 + -(-w // 256) * 256
     # bf16 that is read where it lies has its x with zeros for the rows that are left out all the same
     assert size(256, 1000, 384, 1, 1 + 2 + 4) == size(256, 1000, 384, 1, 1 + 2 + 4 + 8)
+
+
+def test_lists_of_a_batch():
+    native, p = _lib.training(), torch.nn.Parameter(torch.zeros(3))
+    for args in (((p,), [{}], ["exp_avg", "exp_avg_sq"]), ([p], ({},), ["exp_avg", "exp_avg_sq"]), ([p], [{}], ("exp_avg", "exp_avg_sq")), (None, [{}], [])):
+        with pytest.raises(RuntimeError, match="lists"):
+            native.adamw_batch(*args, 32)
+    for name, args in (("places", ((p,),)), ("places", ([None],)), ("alike", ([p], [])), ("alike", (p, [p]))):
+        with pytest.raises(RuntimeError, match=name):
+            getattr(native, name)(*args)

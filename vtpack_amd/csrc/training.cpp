@@ -389,6 +389,7 @@ PyTypeObject *batch_type()
 std::vector<PyObject *> held(PyObject *list)
 {
     std::vector<PyObject *> out;
+    if (!PyList_Check(list)) throw std::runtime_error("adamw_batch: expected lists");
     for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); i++) {
         out.push_back(PyList_GET_ITEM(list, i));
         Py_INCREF(out.back());
