@@ -623,8 +623,8 @@ int vtdge_gate_balance_backward(const void *gate, int64_t pitch, const uint8_t *
  *             laid out of them and the logits that it kept (fp32, up to 256 MB), its first vtdge_cross_entropy_laid_out bytes at
  *             most, are not worked out again
  * fp32 operands are multiplied as three bf16 parts each on the bf16 matrix instructions, to 24 bits of each from 2^-110 up to the
- * largest finite number; a smaller one is off by 2^-134 at most.  An infinity among the features of a row that counts or the
- * weights of a class makes NaN of the logits it meets, also where fp32 products would make an infinity.
+ * largest finite number; a smaller one is off by 2^-134 at most.  The logits that an infinity in weight or in a row that
+ * counts meets may be NaN where fp32 products make an infinity; one in the bias is added as it is.
  *   workspace  vtdge_cross_entropy_workspace(..., how) bytes, 256-byte aligned, contents do not matter.  how: a sum of
  *             VTDGE_CE_BACKWARD, for the gradients, VTDGE_CE_KEEPS, for a forward call with `keeps` and for gradients with its
  *             `laid_out`, and VTDGE_CE_X_LIES, VTDGE_CE_WEIGHT_LIES, for operands that are read where they lie and need no

@@ -15,13 +15,13 @@
 // bank conflicts, on the side of the global address.
 // fp32 operands are split into three bf16 parts each (24 bits), and the six products of parts down to 2^-24 are a six times longer
 // sum, smallest first, in the same fp32 sums: the same kernels at a sixth of their rate, which is above that of the fp32 matrix
-// instructions.  Bits below 2^-133 are lost, which only values below 2^-110 have, and an infinity meets parts of either sign and becomes
-// NaN.  (Two fp16 parts and three products would be 22 bits of a row's largest value and fewer of its small ones.)
+// instructions.  Bits below 2^-133 are lost, which only values below 2^-110 have, and an infinity meets parts of either sign and may
+// become NaN.  (Two fp16 parts and three products would be 22 bits of a row's largest value and fewer of its small ones.)
 //
-// Bound by the matrix units in long products: 8192 rows x 65536 classes x 1024 in bf16, tiles 0.98 ms (1.12 PFLOP/s), d 4 x 0.29 (0.94,
-// with the writing of d), gradients 4 x 0.51 (1.07); in fp32 2048 x 21841 x 384, tiles 0.21 ms (166 TFLOP/s of fp32, 1.0 PFLOP/s issued; 0.24
-// with the logits kept), d 0.07 from those, gradients 0.39.  Their units are busy for 57 percent at the 1.7 - 1.9 GHz that the clock falls to, waves wait for them half of the
-// time.  By the reading of W where rows are few (1 row x 65536 x 1024 in 21.6 us, 6.2 TB/s), by launches where all is small (256 x 1000 x
+// Bound by the matrix units in long products: 8192 rows x 65536 classes x 1024 in bf16, tiles 0.98 ms (1.12 PFLOP/s), d 4 x 0.30 (0.93,
+// with the writing of d), gradients 4 x 0.52 (1.06); in fp32 2048 x 21841 x 384, tiles with the logits kept 0.21 ms (166 TFLOP/s of fp32, 1.0
+// PFLOP/s issued), d 0.07 from those, gradients 0.38.  Their units are busy for 56 to 58 percent (d 44) at the 1.7 - 2.0 GHz that the clock
+// falls to, waves wait for a third of their cycles.  By the reading of W where rows are few (1 row x 65536 x 1024 in 21.6 us, 6.2 TB/s), by launches where all is small (256 x 1000 x
 // 384: four kernels of 6 - 9 us).
 #include "common.h"
 

@@ -3,8 +3,8 @@
 //
 // Why this is native: small calls of these operators are bound by the host.  A backward pass runs in the engine's own thread, whose
 // core comes out of its sleep for it, and what Python does there (the interpreter lock, four allocations, 24 arguments) took 32 of
-// the 122 us of a DeiT-S classifier's loss with its gradients (71 so); a step over 200 weights looked at some 1000 objects, 77 us beside the
-// 31 us of its kernels (7 so).
+// the 122 us of a DeiT-S classifier's loss with its gradients (73 so); a step over 200 weights looked at some 1000 objects, 77 us beside the
+// 31 us of its kernels (9 so).
 #include <Python.h>
 
 #include <ATen/ATen.h>

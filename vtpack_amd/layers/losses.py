@@ -16,10 +16,12 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index=-100, label_smoot
     (torch.jit.trace, make_fx), forward-mode derivatives and gradients of the gradients are refused.
 
     The logits are fp32 sums and are not rounded; in bfloat16 the gradients of the logits are, once, before the products that
-    take them to x, weight and bias.  They work in pieces of the classes with some 320 MB of scratch for a piece; float32
-    operands are laid out anew in three parts of two bytes, which stay for the gradients, with logits of up to 256 MB, where all
-    of it is no more than 320 MB.  Finite float32 values are multiplied to 24 bits, those below 2^-110 to within 2^-134; an infinity in
-    x (in a row that counts) or weight makes NaN of the logits it meets, one in the bias does not."""
+    take them to x, weight and bias.  They work in pieces of the classes with some 320 MB of scratch for a piece (more for
+    over 160 000 rows, float32 50 000: a piece has 1024 classes at least, or all of them rounded up to 256); float32 operands are
+    laid out anew in three parts of two bytes, which stay for the gradients, with logits of up to 256 MB, where all of it is no
+    more than 320 MB.  Finite float32 values are multiplied to 24 bits, those below 2^-110 to within 2^-134; the logits that an
+    infinity in weight or in a row that counts meets may be NaN where float32 products make an infinity; one in the bias is added
+    as it is."""
     how = (ignore_index, label_smoothing, ops.REDUCTIONS.get(reduction))
     loss = _lib.training().linear_cross_entropy(x, weight, bias, target, *how)
     if loss is not None:
