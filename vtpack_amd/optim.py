@@ -76,7 +76,7 @@ class AdamW(torch.optim.Optimizer):
 
     Gradients are read where they lie and have their weight's type; one of other strides than its weight is copied first.
     Refused: types the kernels do not have, sparse gradients, weights with gaps between their elements, weights of a group that lie over
-    each other."""
+    each other.  A group that is refused is as it was; others may have taken their step."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, capturable=False):
         if torch.is_tensor(lr):
