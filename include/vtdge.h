@@ -671,6 +671,51 @@ int vtdge_adamw(const vtdge_adamw_tensor *tensors_host, int count, double lr, do
 int vtdge_adamw_scalars(int64_t *step, int64_t skipped, int advance, const float *lr_dev, double lr, double beta1,
                         double beta2, double eps, double weight_decay, void *scalars, void *stream);
 
+/* ---- Blocks of 8-bit numbers.
+ * A row of n numbers in blocks of 128 (the last may be shorter): e4m3 values (OCP) and a power of two 2^e for each block, e the smallest
+ * whole number with max |x| 2^-e <= 448, -110 at least; values rounded to nearest, ties to even.  Infinities and NaN become NaN and do not
+ * count in the maximum.  Each number of a block is a bf16 number.
+ *   blocks    vtdge_blocks_bytes(rows, n) bytes on a 128-byte boundary: rows of ceil(n / 128) * 128 values, zeros behind the n-th, then rows
+ *             of scale bytes e + 127, ceil(n / 128) of them filled up to a multiple of 4.  (A scale byte of 255 stands for NaN, as in e8m0.)
+ *   x [rows, n] of `dtype`, rows ldx elements apart; results are dense */
+int64_t vtdge_blocks_bytes(int64_t rows, int64_t n);
+int vtdge_quantize_blocks(const void *x, int64_t ldx, int64_t rows, int64_t n, void *blocks, int dtype, void *stream);
+int vtdge_dequantize_blocks(const void *blocks, int64_t rows, int64_t n, void *out, int dtype, void *stream);
+
+/* y = GELU(x) (exact erf form), with x kept in blocks Q(x) (nullable: not kept);  dx = grad (Phi(c) + c phi(c)), c = Q(x). */
+int vtdge_gelu_8bit(const void *x, int64_t ldx, int64_t rows, int64_t n, void *y, void *blocks, int dtype, void *stream);
+int vtdge_gelu_8bit_backward(const void *grad, int64_t ldg, int64_t rows, int64_t n, const void *blocks, void *dx, int dtype,
+                             void *stream);
+
+/* y = (x - m) r weight + bias, m the fp32 number next to the row's mean, r = 1 / sqrt(var + eps), with Q(x - m) kept in blocks and r in
+ * rstd fp32 [rows] (nullable, both: not kept).  Backward, h = Q(x - m) r and g = grad weight:  dx = r (g - mean g - h mean(g h)), dweight = sum grad h, dbias = sum
+ * grad over the rows; each of the three nullable.  n up to VTDGE_MAX_NORM_8BIT.
+ *   workspace  vtdge_layernorm_8bit_backward_workspace(rows, n) bytes, 16-byte aligned */
+#define VTDGE_MAX_NORM_8BIT 8192
+int vtdge_layernorm_8bit(const void *x, int64_t ldx, const void *weight, const void *bias, float eps, int64_t rows, int64_t n,
+                         void *y, void *blocks, float *rstd, int dtype, void *stream);
+int64_t vtdge_layernorm_8bit_backward_workspace(int64_t rows, int64_t n);
+int vtdge_layernorm_8bit_backward(const void *grad, int64_t ldg, const void *weight, const void *blocks, const float *rstd,
+                                  int64_t rows, int64_t n, void *workspace, int64_t workspace_bytes, void *dx, void *dweight,
+                                  void *dbias, int dtype, void *stream);
+
+/* y [rows, out] = act(Q(x) Q(weight)^T + bias), x [rows, width], fp32 sums.
+ *   weight    [out, width] of `dtype`, brought into blocks on the way and, with w_blocks, kept there; NULL: w_blocks holds it
+ *   x_blocks  nullable: Q(x), for the gradients
+ *   workspace vtdge_linear_8bit_workspace bytes, 256-byte aligned
+ * Backward, g = grad rounded to bf16: dx = g Q(weight), dweight = g^T Q(x), dbias = sum g over the rows; each of the three nullable, and
+ * w_blocks without dx, x_blocks without dweight.
+ *   workspace vtdge_linear_8bit_backward_workspace(.., lies, ..) bytes, 256-byte aligned; lies: the gradient is bf16, out a multiple of 64,
+ *             its rows a multiple of 8 elements and less than 2^22 apart, on a 16-byte boundary, and is read where it lies */
+int64_t vtdge_linear_8bit_workspace(int64_t rows, int64_t out, int64_t width, int dtype);
+int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight, int64_t ldw, void *w_blocks, const void *bias, void *y,
+                      void *x_blocks, int64_t rows, int64_t out, int64_t width, int act, void *workspace, int64_t workspace_bytes,
+                      int dtype, void *stream);
+int64_t vtdge_linear_8bit_backward_workspace(int64_t rows, int64_t out, int64_t width, int lies, int dtype);
+int vtdge_linear_8bit_backward(const void *grad, int64_t ldg, const void *x_blocks, const void *w_blocks, int64_t rows, int64_t out,
+                               int64_t width, void *workspace, int64_t workspace_bytes, void *dx, void *dweight, void *dbias,
+                               int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

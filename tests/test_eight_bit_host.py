@@ -1,0 +1,81 @@
+"""Blocks of 8-bit numbers without a GPU: what the operators refuse, the checks of the library's arguments, the oracle's own rounding."""
+import pytest
+import torch
+
+from tests import eight_bit_reference as ref
+from vtpack_amd import _lib
+from vtpack_amd.layers import Blocks, gelu_8bit, layer_norm_8bit, linear_8bit, quantize_blocks
+
+
+def test_tensors_on_the_cpu_are_refused():
+    x, w = torch.randn(4, 8), torch.randn(3, 8)
+    for call in (lambda: quantize_blocks(x), lambda: linear_8bit(x, w), lambda: gelu_8bit(x), lambda: layer_norm_8bit(x, w[0], w[0]),
+                 lambda: Blocks(x.to(torch.float8_e4m3fn), torch.ones(4, 1).to(torch.float8_e8m0fnu))):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            call()
+
+
+def test_what_is_no_tensor_is_refused():
+    for call in (lambda: quantize_blocks([1.0]), lambda: gelu_8bit(None), lambda: linear_8bit(None, torch.zeros(2, 2)), lambda: layer_norm_8bit(1, 2, 3)):
+        with pytest.raises(TypeError):
+            call()
+    with pytest.raises(ValueError, match="act"):
+        linear_8bit(torch.zeros(2, 2), torch.zeros(2, 2), act="relu")
+
+
+def test_the_oracle_rounds_as_e4m3_does():
+    """Against torch's own conversion of what the scale leaves."""
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(50, 300, generator=g) * torch.exp(3 * torch.randn(50, 300, generator=g))
+    numbers, e = ref.blocks_of(x)
+    for k in range(3):
+        t, s = x[:, 128 * k:128 * k + 128], e[:, k:k + 1]
+        scaled = (t.double() * torch.exp2(-s)).float()
+        assert float(scaled.abs().max()) <= 448 and (scaled.abs().amax(1) > 224).all()
+        assert torch.equal(numbers[:, 128 * k:128 * k + 128], scaled.to(torch.float8_e4m3fn).double() * torch.exp2(s))
+    assert torch.equal(numbers, numbers.to(torch.bfloat16).double())
+
+
+def test_sizes_of_buffers():
+    lib = _lib.load()
+    assert lib.vtdge_blocks_bytes(1, 1) == 128 + 4 and lib.vtdge_blocks_bytes(3, 128) == 3 * 132 and lib.vtdge_blocks_bytes(2, 129) == 2 * 260
+    assert lib.vtdge_blocks_bytes(2, 513) == 2 * (640 + 8) and lib.vtdge_blocks_bytes(0, 5) == -1 and lib.vtdge_blocks_bytes(5, 0) == -1
+    assert lib.vtdge_blocks_bytes(1 << 31, 1) == -1 and lib.vtdge_blocks_bytes(1, (1 << 20) + 1) == -1 and lib.vtdge_blocks_bytes((1 << 31) - 1, 1 << 20) == -1
+
+
+def _codes(fn, good, table):
+    for i, v, want in table:
+        args = list(good)
+        args[i] = v
+        assert fn(*args) == want, (i, v, _lib.load().vtdge_last_error())
+
+
+def test_arguments_of_the_library():
+    """Before anything is launched."""
+    lib, p = _lib.load(), 4096                            # never read: the arguments are refused first
+    A, U = _lib.ERR_ARG, _lib.ERR_UNSUPPORTED
+    blocks = ((0, None, A), (1, 7, A), (2, 0, A), (3, 0, A), (3, -1, A), (4, None, A), (4, p + 16, A), (5, 2, A), (2, 1 << 31, U))
+    _codes(lib.vtdge_quantize_blocks, [p, 8, 4, 8, p, 0, None], blocks)
+    _codes(lib.vtdge_dequantize_blocks, [p, 4, 8, p, 0, None], ((0, None, A), (0, p + 4, A), (1, 0, A), (2, 0, A), (3, None, A), (4, 9, A), (2, 1 << 21, U)))
+    gelu = [p, 8, 4, 8, p, p, 0, None]
+    _codes(lib.vtdge_gelu_8bit, gelu, ((0, None, A), (1, 7, A), (2, 0, A), (3, 0, A), (4, None, A), (5, p + 1, A), (6, 5, A)))
+    _codes(lib.vtdge_gelu_8bit_backward, [p, 8, 4, 8, p, p, 0, None], ((0, None, A), (1, 7, A), (4, None, A), (5, None, A), (4, p + 1, A), (6, 5, A)))
+    _codes(lib.vtdge_layernorm_8bit, [p, 8, p, p, 1e-6, 4, 8, p, p, p, 0, None],
+           ((0, None, A), (1, 7, A), (2, None, A), (3, None, A), (5, 0, A), (6, 8193, U), (7, None, A), (8, None, A), (9, None, A), (8, p + 1, A), (10, 3, A)))
+    _codes(lib.vtdge_layernorm_8bit_backward, [p, 8, p, p, p, 4, 8, p, 1 << 30, p, p, p, 0, None],
+           ((0, None, A), (1, 7, A), (2, None, A), (3, None, A), (4, None, A), (5, 0, A), (6, 8193, U), (7, None, A), (8, 0, A), (7, p + 4, A), (12, 3, A)))
+    linear = [p, 8, p, 8, p, p, p, p, 4, 3, 8, 0, p, 1 << 40, 0, None]
+    _codes(lib.vtdge_linear_8bit, linear,
+           ((0, None, A), (1, 7, A), (3, 7, A), (4, p + 4, A), (6, None, A), (7, p + 4, A), (8, 0, A), (9, 0, A), (10, 0, A), (11, 2, A), (12, None, A),
+            (12, p + 16, A), (13, -1, A), (14, 2, A), (8, 1 << 31, U), (10, 1 << 21, U)))
+    args = list(linear)
+    args[2] = args[4] = None
+    assert lib.vtdge_linear_8bit(*args) == A and b"NULL" in lib.vtdge_last_error()
+    back = [p, 3, p, p, 4, 3, 8, p, 1 << 40, p, p, p, 0, None]
+    _codes(lib.vtdge_linear_8bit_backward, back,
+           ((0, None, A), (1, 2, A), (2, None, A), (3, None, A), (2, p + 4, A), (3, p + 4, A), (4, 0, A), (5, 0, A), (6, 0, A), (7, None, A), (7, p + 16, A),
+            (8, 0, A), (12, 4, A)))
+    args = list(back)
+    args[0] = args[9] = args[10] = args[11] = None        # nothing asked for
+    assert lib.vtdge_linear_8bit_backward(*args) == 0
+    assert lib.vtdge_linear_8bit_workspace(0, 3, 8, 0) == -1 and lib.vtdge_linear_8bit_backward_workspace(4, 3, 8, 0, 7) == -1

@@ -94,6 +94,14 @@ SIGNATURES = {
     "vtdge_cross_entropy": [_p, _l, _p, _l, _p, _p, _l, _l, _i, _l, _f, _p, _l, _i, _p, _p, _p, _p, _p, _i, _p],
     "vtdge_cross_entropy_backward": [_p, _l, _p, _l, _p, _p, _p, _p, _p, _i, _p, _l, _l, _i, _l, _f, _p, _p, _l, _p, _p, _p,
                                      _i, _p],
+    "vtdge_quantize_blocks": [_p, _l, _l, _l, _p, _i, _p],
+    "vtdge_dequantize_blocks": [_p, _l, _l, _p, _i, _p],
+    "vtdge_gelu_8bit": [_p, _l, _l, _l, _p, _p, _i, _p],
+    "vtdge_gelu_8bit_backward": [_p, _l, _l, _l, _p, _p, _i, _p],
+    "vtdge_layernorm_8bit": [_p, _l, _p, _p, _f, _l, _l, _p, _p, _p, _i, _p],
+    "vtdge_layernorm_8bit_backward": [_p, _l, _p, _p, _p, _l, _l, _p, _l, _p, _p, _p, _i, _p],
+    "vtdge_linear_8bit": [_p, _l, _p, _l, _p, _p, _p, _p, _l, _l, _l, _i, _p, _l, _i, _p],
+    "vtdge_linear_8bit_backward": [_p, _l, _p, _p, _l, _l, _l, _p, _l, _p, _p, _p, _i, _p],
     "vtdge_adamw": [_p, _i, _d, _d, _d, _d, _d, _l, _p, _i, _i, _p],
     "vtdge_adamw_scalars": [_p, _l, _i, _p, _d, _d, _d, _d, _d, _p, _p],
     "vtdge_chain_layout": [_p, _p],
@@ -117,6 +125,10 @@ _WORKSPACES = {
     "vtdge_gate_balance_workspace": [_l, _i],
     "vtdge_cross_entropy_laid_out": [_l, _l, _i, _i],
     "vtdge_cross_entropy_workspace": [_l, _l, _i, _i, _i],
+    "vtdge_blocks_bytes": [_l, _l],
+    "vtdge_layernorm_8bit_backward_workspace": [_l, _l],
+    "vtdge_linear_8bit_workspace": [_l, _l, _l, _i],
+    "vtdge_linear_8bit_backward_workspace": [_l, _l, _l, _i, _i],
 }
 EXPORTS = ["vtdge_version", "vtdge_last_error", "vtdge_last_kernel", "vtdge_recent_kernel"] + list(SIGNATURES)
 

@@ -23,208 +23,15 @@
 // PFLOP/s issued), d 0.07 from those, gradients 0.38.  Their units are busy for 56 to 58 percent (d 44) at the 1.7 - 2.0 GHz that the clock
 // falls to, waves wait for a third of their cycles.  By the reading of W where rows are few (1 row x 65536 x 1024 in 21.6 us, 6.2 TB/s), by launches where all is small (256 x 1000 x
 // 384: four kernels of 6 - 9 us).
-#include "common.h"
-
-#include <math.h>
+#include "gradient_product.h"
 
 namespace vtdge {
 
 constexpr float LOG2E = 1.44269504f, LN2 = 0.69314718f;
-__device__ __forceinline__ int wave_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 // What the first bf16 part of an fp32 value is rounded from: the largest finite numbers would become infinite, and are cut to bf16's
 // largest; the next part has the rest.  (Infinity and NaN go on to the next part.)
 constexpr float BF16_MOST = 0x1.fep127f;
 __device__ __forceinline__ float first_part(float f) { return __builtin_amdgcn_fmed3f(f, -BF16_MOST, BF16_MOST); }
-
-// ------------------------------------------------------------------------------------------------ the product of a tile
-// A bf16 matrix, or the three parts of an fp32 one `plane` elements apart.
-struct Operand {
-    const bf16_t *p;
-    int64_t pitch, plane;
-};
-
-// A shape of the product: WM x WN waves, each with IM x JN blocks of 32 x 32; slabs of SLAB of the summed dimension in a ring of
-// SLOTS; PARTS 3 for fp32 operands.
-template <int IM_, int JN_, int WM_, int WN_, int SLAB_, int SLOTS_, int PARTS_> struct Shape {
-    static constexpr int IM = IM_, JN = JN_, WM = WM_, WN = WN_, SLAB = SLAB_, SLOTS = SLOTS_, PARTS = PARTS_;
-    static constexpr int ROWS = 32 * IM * WM, COLS = 32 * JN * WN, WAVES = WM * WN, THREADS = 64 * WAVES;
-    static constexpr int STAGE = PARTS * (ROWS + COLS) * SLAB * 2, RING = SLOTS * STAGE;
-    static constexpr int LDS = RING + COLS * 4;                          // and the bias of the tile's classes
-    using Half = Shape<IM / 2, JN, WM, WN, SLAB, SLOTS, PARTS>;
-    static constexpr bool HALVES = WAVES == 8 && IM == 2;               // the last tiles of a launch may be cut in two, see halved()
-    static constexpr bool FLAT = IM == 1 && JN == 2;                    // few rows
-    static constexpr bool WHOLE_LINES = IM == 1 && JN == 1;             // gradients leave by way of LDS
-    static constexpr int PER_SIMD = WAVES / 4 * (2 * LDS <= 160 * 1024 ? 2 : 1);
-    static_assert(LDS <= 160 * 1024 && 6 * ROWS * 4 <= RING, "LDS");
-};
-
-// Direct loads of one operand of a tile.  T = rows of the tile on its side.
-// ALONG: the summed dimension lies along the rows of memory: tile rows are rows of memory, `limit` of them from the first on.
-// Across: the summed dimension counts the rows of memory, `limit` of them, and tile rows are elements of a row, which has a multiple
-// of 8 of them, `span`.  No stage begins behind `limit`: a sum of n rows of memory has ceil(n / SLAB) stages.
-// LDS rows are 2 SLAB bytes (ALONG) or 2 T bytes (across) without gaps; their 16-byte pieces are XOR-ed by the row, so that the
-// sixteen lanes that read together meet every bank once.
-template <bool ALONG, int T, int SLAB, int WAVES, bool MAY_STREAM = false> struct Loader {
-    static constexpr int ROW = ALONG ? 2 * SLAB : 2 * T, STAGE = 2 * SLAB * T;
-    static constexpr int LPR = ROW / 16, RPI = 64 / LPR;                  // lanes a row, rows an instruction
-    static constexpr int PIECES = STAGE / 1024 / WAVES;                   // instructions of a wave
-    static_assert(PIECES * WAVES * 1024 == STAGE && LPR <= 64, "whole instructions");
-    const unsigned char *base;
-    int64_t plane, pitch;                                                 // bytes
-    int limit, row0, last;
-    bool stream = false;                                                  // past the caches
-
-    __device__ __forceinline__ Loader(const Operand &o, int64_t first, int64_t lim, int64_t span)
-        : base(reinterpret_cast<const unsigned char *>(o.p) + (ALONG ? first * o.pitch * 2 : first * 2)), plane(o.plane * 2), pitch(o.pitch * 2)
-    {
-        const int lane = threadIdx.x & 63, wid = wave_uniform(threadIdx.x >> 6);
-        row0 = wid * RPI + lane / LPR;
-        if constexpr (ALONG) limit = (int)(lim - first < T ? lim - first : T);
-        else limit = (int)lim;
-        last = ALONG ? 0 : (int)(span - first < T ? span - first : T) * 2 - 16;
-    }
-    static __device__ __forceinline__ int swizzle(int r)
-    {
-        if constexpr (ALONG) return SLAB == 64 ? (r >> 1) & 7 : SLAB == 32 ? (r >> 2) & 3 : (r >> 3) & 1;
-        else return LPR == 8 ? ((r >> 1) & 3) << 1 : (r & 7) << 1;
-    }
-    // stage `kt` of part `part` to LDS byte `lds`
-    __device__ __forceinline__ void load(int part, int kt, uint32_t lds) const
-    {
-        const int lane = threadIdx.x & 63, wid = wave_uniform(threadIdx.x >> 6);
-        const void *from = uniform_ptr(base + part * plane + (ALONG ? (int64_t)kt * (2 * SLAB) : (int64_t)kt * SLAB * pitch));
-#pragma unroll
-        for (int d = 0; d < PIECES; d++) {
-            const int r = d * WAVES * RPI + row0;
-            const int at = ((lane % LPR) ^ swizzle(r)) * 16;
-            const int row = ALONG ? min(r, limit - 1) : min(r, limit - 1 - kt * SLAB);
-            const int col = ALONG ? at : min(at, last);
-            const uint32_t off = (uint32_t)row * (uint32_t)pitch + col, to = wave_uniform(lds + (d * WAVES + wid) * 1024);
-            if (MAY_STREAM && stream) dma16_nt(from, off, to);
-            else dma16(from, off, to);
-        }
-    }
-    // the 8 values of step s (16 of the summed dimension) of tile row `block` * 32 + lane % 32
-    static __device__ __forceinline__ u32x4 fragment(const unsigned char *stage, int block, int s)
-    {
-        const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
-        if constexpr (ALONG) {
-            return *reinterpret_cast<const u32x4 *>(stage + (block * 32 + lr) * ROW + (((2 * s + lg) ^ swizzle(lr)) * 16));
-        } else {
-            const int k = 16 * s + 8 * lg + ((lane & 15) >> 2);
-            const int at = block * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;       // byte of the row
-            const u32x2 lo = lds_read_tr16(stage + k * ROW + (((at >> 4) ^ swizzle(k)) << 4) + (at & 15));
-            const u32x2 hi = lds_read_tr16(stage + (k + 4) * ROW + (((at >> 4) ^ swizzle(k + 4)) << 4) + (at & 15));
-            return u32x4{lo.x, lo.y, hi.x, hi.y};
-        }
-    }
-};
-
-// acc[i][j][v] += A[row i*32 + lane%32 of the wave] . B[row j*32 + 8*(v/4) + 4*(lane/32) + v%4], stages t0 .. t1 - 1.  SUMS: also the sums of
-// A's rows (of this half of the lanes' values), for what `sums_wanted` says.
-template <class S, bool SUMS, class LA, class LB>
-__device__ __forceinline__ void multiply_tile(const LA &a, const LB &b, int t0, int t1, unsigned char *smem, f32x16 (&acc)[S::IM][S::JN],
-                                              bool sums_wanted, float (&sums)[S::IM])
-{
-    constexpr int IM = S::IM, JN = S::JN, PARTS = S::PARTS, SLOTS = S::SLOTS, A_BYTES = PARTS * LA::STAGE;
-    constexpr int LOADS = PARTS * (LA::PIECES + LB::PIECES);
-    static_assert(LOADS * (SLOTS - 2) < 64, "the counter of outstanding loads");
-    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
-    const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
-    auto issue = [&](int t, int slot) {
-        const uint32_t at = lds0 + slot * S::STAGE;
-#pragma unroll
-        for (int p = 0; p < PARTS; p++) {
-            a.load(p, t, at + p * LA::STAGE);
-            b.load(p, t, at + A_BYTES + p * LB::STAGE);
-        }
-    };
-    int in = 0, out = 0;                            // slots
-#pragma unroll
-    for (int d = 0; d < SLOTS - 1; d++)
-        if (t0 + d < t1) {
-            issue(t0 + d, in);
-            in++;
-        }
-    for (int t = t0; t < t1; t++) {
-        // this wave's loads of the stage have landed when only those of the stages behind it are outstanding
-        const int behind = min(t1 - 1 - t, SLOTS - 2);
-        static_for<SLOTS - 1>([&](auto X) {
-            constexpr int x = decltype(X)::value;
-            if (behind == x) wait_vmcnt<x * LOADS>();
-        });
-        lds_barrier();                              // everybody's have, and the slot before this one is read no more
-        const unsigned char *sa = smem + out * S::STAGE, *sb = sa + A_BYTES;
-        out = out == SLOTS - 1 ? 0 : out + 1;
-        // fragments a step ahead of their products, the direct loads behind the first of them
-        constexpr int STEPS = S::SLAB / 16;
-        u32x4 fa[2][PARTS][IM], fb[2][PARTS][JN];
-        auto fetch = [&](int s) {
-#pragma unroll
-            for (int p = 0; p < PARTS; p++) {
-#pragma unroll
-                for (int i = 0; i < IM; i++) fa[s & 1][p][i] = LA::fragment(sa + p * LA::STAGE, wm * IM + i, s);
-#pragma unroll
-                for (int j = 0; j < JN; j++) fb[s & 1][p][j] = LB::fragment(sb + p * LB::STAGE, wn * JN + j, s);
-            }
-        };
-        fetch(0);
-        __builtin_amdgcn_sched_barrier(0);
-        if (t + SLOTS - 1 < t1) {
-            issue(t + SLOTS - 1, in);
-            in = in == SLOTS - 1 ? 0 : in + 1;
-        }
-#pragma unroll
-        for (int s = 0; s < STEPS; s++) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (s + 1 < STEPS) fetch(s + 1);
-            __builtin_amdgcn_sched_barrier(0);
-            // smallest products first: parts whose numbers add up to 2, to 1, to 0
-#pragma unroll
-            for (int order = PARTS - 1; order >= 0; order--)
-#pragma unroll
-                for (int p = 0; p <= order; p++)
-#pragma unroll
-                    for (int i = 0; i < IM; i++)
-#pragma unroll
-                        for (int j = 0; j < JN; j++) Slab<bf16_t>::mma(fb[s & 1][order - p][j], fa[s & 1][p][i], acc[i][j]);
-            if constexpr (SUMS) {
-                if (sums_wanted) {
-#pragma unroll
-                    for (int p = PARTS - 1; p >= 0; p--)
-#pragma unroll
-                        for (int i = 0; i < IM; i++) {
-                            const u32x4 &f = fa[s & 1][p][i];
-                            sums[i] = bf16_pair_sum(f.x, bf16_pair_sum(f.y, bf16_pair_sum(f.z, bf16_pair_sum(f.w, sums[i]))));
-                        }
-                }
-            }
-        }
-    }
-    lds_barrier();                                  // the ring is free for the epilogue
-}
-
-// Workgroup id of `count` -> place in the list of all: an XCD (every eighth id) takes a contiguous run of it.
-__device__ __forceinline__ int place_of(int id, int count)
-{
-    const int xcd = id & 7, whole = count >> 3, rest = count & 7;
-    return xcd * whole + (xcd < rest ? xcd : rest) + (id >> 3);
-}
-// The list of tiles goes through eight row tiles for each column tile, so that what an XCD's L2 holds is used again.
-__device__ __forceinline__ void tile_at(int place, int tm, int tn, int &m, int &n)
-{
-    const int group = 8 * tn, g = place / group, first = g * 8, size = min(8, tm - first);
-    const int in = place - g * group;
-    m = first + in % size;
-    n = in / size;
-}
-// the same over all parts of a sum -> part
-__device__ __forceinline__ int tile_of(int id, int parts, int tm, int tn, int &m, int &n)
-{
-    const int tiles = tm * tn, place = place_of(id, tiles * parts), part = place / tiles;
-    tile_at(place - part * tiles, tm, tn, m, n);
-    return part;
-}
 
 struct CeArgs {
     Operand x, w;
@@ -679,172 +486,6 @@ __global__ __launch_bounds__(256) void cross_entropy_d_kept_kernel(CeArgs p, int
     }
 }
 
-// ---- out = A B, dx = d W or dW = d^T x, over a dimension that may be cut into several parts, which leave sums of their own
-struct GradArgs {
-    Operand a, b;
-    int64_t rows, cols, span_a, span_b, sum_a, sum_b;      // of the result; elements of a row of memory; rows of memory that may be read
-    int tm, tn, stages, splits;
-    float *part; int64_t part_stride; int accumulate;       // [splits], [rows][cols] fp32 each
-    void *out;                                              // without `part`: the result, scaled; neither: only the sums
-    float *sums_part; int64_t sums_stride; void *sums;     // nullable: the sums of A's rows, in the same way
-};
-struct GradPair {
-    GradArgs dx, dw;
-    int first_dw;                                           // workgroups before are dx's
-    const float *scale, *scale2; int f32;
-};
-
-// four values of row r from column c on, to a part or to the result
-__device__ __forceinline__ void put_four(const GradArgs &p, const GradPair &all, int z, int64_t r, int64_t c, f32x4 v, float scale)
-{
-    const int left = (int)(p.cols - c);
-    const bool whole = left >= 4 && p.cols % 4 == 0;
-    if (p.part != nullptr) {
-        float *const to = p.part + z * p.part_stride + r * p.cols + c;
-        if (whole) {
-            if (p.accumulate) v += *reinterpret_cast<const f32x4 *>(to);
-            *reinterpret_cast<f32x4 *>(to) = v;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (e < left) to[e] = v[e] + (p.accumulate ? to[e] : 0.f);
-        }
-    } else if (p.out != nullptr) {
-        v *= scale;
-        if (all.f32) {
-            float *const to = static_cast<float *>(p.out) + r * p.cols + c;
-            if (whole) {
-                *reinterpret_cast<f32x4 *>(to) = v;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (e < left) to[e] = v[e];
-            }
-        } else {
-            bf16_t *const to = static_cast<bf16_t *>(p.out) + r * p.cols + c;
-            if (whole) {
-                *reinterpret_cast<u32x2 *>(to) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (e < left) to[e] = f32_to_bf16(v[e]);
-            }
-        }
-    }
-}
-template <class S, bool A_ALONG> __device__ __forceinline__ void gradient_tile(const GradArgs &p, const GradPair &all, int id, unsigned char *smem)
-{
-    constexpr int IM = S::IM, JN = S::JN;
-    int m, n;
-    const int z = tile_of(id, p.splits, p.tm, p.tn, m, n);
-    const int64_t r0 = (int64_t)m * S::ROWS, c0 = (int64_t)n * S::COLS;
-    const int t0 = (int)((int64_t)p.stages * z / p.splits), t1 = (int)((int64_t)p.stages * (z + 1) / p.splits);
-    f32x16 acc[IM][JN] = {};
-    float sums[IM] = {};
-    const Loader<A_ALONG, S::ROWS, S::SLAB, S::WAVES> a(p.a, r0, A_ALONG ? p.rows : p.sum_a, p.span_a);
-    const Loader<false, S::COLS, S::SLAB, S::WAVES> b(p.b, c0, p.sum_b, p.span_b);
-    const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
-    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
-    const bool with_sums = !A_ALONG && n == 0 && wn == 0 && (p.sums_part != nullptr || p.sums != nullptr);
-    float scale = 1.f;
-    if (all.scale != nullptr) scale = *all.scale;
-    if (all.scale2 != nullptr) scale *= *all.scale2;
-    multiply_tile<S, !A_ALONG>(a, b, t0, t1, smem, acc, with_sums, sums);
-#pragma unroll
-    for (int i = 0; i < IM; i++) {
-        const int64_t r = r0 + (wm * IM + i) * 32 + lr;
-        if constexpr (!A_ALONG) {
-            if (with_sums) {
-                const float sum = sums[i] + __shfl_xor(sums[i], 32, WAVE);
-                if (lg == 0 && r < p.rows) {
-                    if (p.sums_part != nullptr) p.sums_part[z * p.sums_stride + r] = sum;
-                    else if (all.f32) static_cast<float *>(p.sums)[r] = sum * scale;
-                    else static_cast<bf16_t *>(p.sums)[r] = f32_to_bf16(sum * scale);
-                }
-            }
-        }
-        if (S::WHOLE_LINES || r >= p.rows) continue;
-#pragma unroll
-        for (int j = 0; j < JN; j++)
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                put_four(p, all, z, r, c0 + (wn * JN + j) * 32 + 8 * q + 4 * lg, v, scale);
-            }
-    }
-    if constexpr (S::WHOLE_LINES) {
-        // by way of LDS, lanes side by side in a row (bf16 1 x 363 x 25766: 40 us without, 22 so)
-        constexpr int PITCH = S::COLS + 4;
-        static_assert(S::ROWS * PITCH * 4 <= S::RING && IM == 1, "LDS");
-        if (p.part == nullptr && p.out == nullptr) return;
-        float *const tile = reinterpret_cast<float *>(smem);
-#pragma unroll
-        for (int j = 0; j < JN; j++)
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                *reinterpret_cast<f32x4 *>(tile + (wm * 32 + lr) * PITCH + (wn * JN + j) * 32 + 8 * q + 4 * lg) =
-                    f32x4{acc[0][j][4 * q], acc[0][j][4 * q + 1], acc[0][j][4 * q + 2], acc[0][j][4 * q + 3]};
-        __syncthreads();
-        const int rows = (int)(p.rows - r0 < S::ROWS ? p.rows - r0 : S::ROWS);
-        if (p.cols % 4 == 0) {
-#pragma unroll 4
-            for (int k = threadIdx.x; k < rows * (S::COLS / 4); k += S::THREADS) {
-                const int row = k / (S::COLS / 4), c = k % (S::COLS / 4) * 4;
-                if (c0 + c < p.cols) put_four(p, all, z, r0 + row, c0 + c, *reinterpret_cast<const f32x4 *>(tile + row * PITCH + c), scale);
-            }
-        } else {
-#pragma unroll 4
-            for (int k = threadIdx.x; k < rows * S::COLS; k += S::THREADS) {
-                const int row = k / S::COLS, c = k % S::COLS;
-                if (c0 + c >= p.cols) continue;
-                const int64_t at = (r0 + row) * p.cols + c0 + c;
-                const float v = tile[row * PITCH + c];
-                if (p.part != nullptr) p.part[z * p.part_stride + at] = v + (p.accumulate ? p.part[z * p.part_stride + at] : 0.f);
-                else if (all.f32) static_cast<float *>(p.out)[at] = v * scale;
-                else static_cast<bf16_t *>(p.out)[at] = f32_to_bf16(v * scale);
-            }
-        }
-    }
-}
-template <class S> __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void cross_entropy_grad_kernel(GradPair p)
-{
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-    if ((int)blockIdx.x < p.first_dw) gradient_tile<S, true>(p.dx, p, blockIdx.x, smem);
-    else gradient_tile<S, false>(p.dw, p, blockIdx.x - p.first_dw, smem);
-}
-
-// out = scale * (sum over the parts), for up to three results in one launch
-struct SumJob {
-    const float *part; void *out; int64_t n, stride; int parts;
-};
-struct SumArgs {
-    SumJob job[3];
-    int64_t first[4];                               // workgroups
-    const float *scale, *scale2; int f32;
-};
-__global__ __launch_bounds__(256) void cross_entropy_sum_kernel(SumArgs p)
-{
-    int j = 0;
-    while (j < 2 && (int64_t)blockIdx.x >= p.first[j + 1]) j++;
-    const SumJob &job = p.job[j];
-    const int64_t i = (((int64_t)blockIdx.x - p.first[j]) * 256 + threadIdx.x) * 4;
-    if (i >= job.n) return;
-    float scale = p.scale != nullptr ? *p.scale : 1.f;
-    if (p.scale2 != nullptr) scale *= *p.scale2;
-    // (parts lie on 16-byte boundaries and are filled up to whole pieces)
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < job.parts; k++) sum += *reinterpret_cast<const f32x4 *>(job.part + k * job.stride + i);
-    sum *= scale;
-    const int live = job.n - i < 4 ? (int)(job.n - i) : 4;
-    if (p.f32) {
-        float *const to = static_cast<float *>(job.out) + i;
-        for (int e = 0; e < live; e++) to[e] = sum[e];
-    } else {
-        bf16_t *const to = static_cast<bf16_t *>(job.out) + i;
-        for (int e = 0; e < live; e++) to[e] = f32_to_bf16(sum[e]);
-    }
-}
-
 // Rows as the product routine reads them: `width` filled up with zeros to whole slabs, fp32 in three parts; rows that are left out
 // (target given) as zeros, so that what they hold reaches no gradient.  Up to two operands in one launch.
 struct PackJob {
@@ -903,15 +544,9 @@ using LogitsLarge = Shape<2, 4, 4, 2, 64, 2, 1>;
 using LogitsMiddle = Shape<2, 4, 2, 2, 32, 3, 1>;
 using LogitsFlat = Shape<1, 2, 2, 2, 64, 3, 1>;
 using LogitsSmall = Shape<1, 1, 2, 2, 64, 6, 1>;
-using GradLarge = Shape<2, 4, 4, 2, 64, 2, 1>;
-using GradMiddle = Shape<2, 2, 4, 2, 64, 3, 1>;
-// (short sums of many tiles: three on a compute unit, fp32 two, rather than a deep ring for one; bf16 1 row x 363 x 25766 classes 43 -> 22 us,
-// 256 x 384 x 1000 10.2 -> 9.7)
-using GradSmall = Shape<1, 1, 2, 2, 64, 3, 1>;
 using SplitLarge = Shape<2, 2, 4, 2, 32, 2, 3>;
 using SplitFlat = Shape<1, 2, 2, 2, 32, 3, 3>;
 using SplitSmall = Shape<1, 1, 2, 2, 32, 4, 3>;
-using SplitGradSmall = Shape<1, 1, 2, 2, 32, 3, 3>;
 
 constexpr int CE_PAD = 64;                          // rows of operands are filled up to whole slabs of any shape
 constexpr int64_t CE_PIECE_BYTES = 320ll << 20;     // of d
@@ -919,19 +554,17 @@ constexpr int64_t CE_KEPT_BYTES = 256ll << 20;      // of logits
 enum { CE_LARGE, CE_MIDDLE, CE_FLAT, CE_SMALL };
 
 // Everything a call lays out, the same for the size and the call.
-struct CePlan {
+struct CePlan : GradPlan {
     int64_t rows, classes; int width, padded, parts;
     bool backward, split;
-    int logits, grads;                              // shapes
-    int lm, ln, gm, gn, slab_l, slab_g;             // their tiles and slabs
+    int logits;                                     // shape
+    int lm, ln, slab_l;                             // its tile and slab
     int64_t tm, tn;                                 // row and class tiles of all classes
     int64_t piece, d_rows;                          // classes of a piece, rows of d
-    int dx_splits, dw_splits;
     // bytes of the workspace
     int64_t x_at, w_at, kept_at, max_at, sum_at, total_at, z_at, d_at, dx_at, dw_at, db_at, bytes;
 };
 
-static int64_t part_of(int64_t n) { return (n + 63) / 64 * 64; }      // elements from one part of a sum to the next
 static int64_t take(int64_t &at, int64_t bytes)
 {
     const int64_t here = at;
@@ -939,74 +572,6 @@ static int64_t take(int64_t &at, int64_t bytes)
     return here;
 }
 template <class S> static void use(int &m, int &n, int &slab) { m = S::ROWS, n = S::COLS, slab = S::SLAB; }
-
-// When `slots` workers are done with n1 jobs of l1 and then n2 of l2, each taken by whoever is free first.
-static int64_t makespan(int64_t slots, int64_t n1, int64_t l1, int64_t n2, int64_t l2)
-{
-    int64_t at[8] = {0}, count[8] = {slots};        // workers by the time they are free, soonest first
-    int groups = 1;
-    auto work = [&](int64_t n, int64_t l) {
-        while (n > 0) {
-            const int64_t now = n < count[0] ? n : count[0], t = at[0] + l;
-            n -= now;
-            count[0] -= now;
-            int from = 0;
-            if (count[0] == 0) from = 1;            // the group is gone; else it stays (and n is 0)
-            int to = groups;
-            while (to > from && at[to - 1] > t) at[to] = at[to - 1], count[to] = count[to - 1], to--;
-            at[to] = t, count[to] = now;
-            groups++;
-            if (from == 1) {
-                for (int g = 1; g < groups; g++) at[g - 1] = at[g], count[g - 1] = count[g];
-                groups--;
-            }
-        }
-    };
-    work(n1, l1);                                   // (a group is split only by the last jobs of a kind: four at most)
-    work(n2, l2);
-    return at[groups - 1];
-}
-
-// Shape and cuts of both gradients of a piece.  Large tiles where their work is 16 slabs for each compute unit; then the tiles and as
-// many parts of each sum as end first: a compute unit takes one tile after the other, a tile as long as its slabs (measured in long
-// products) and an epilogue, and parts are written and read again at 4 TB/s.  us of a backward call, uncut / as chosen: bf16 2999 x
-// 768 x 21841 555 / 360, 300 x 768 x 21841 389 / 83, 8192 x 384 x 1000 116 / 82; fp32 2048 x 384 x 21841 1715 / 640, 128 x 768 x
-// 21841 1338 / 166.
-struct GradShape {
-    int grads, m, n, slab;
-    double us, tile_us;                             // of a slab, of an epilogue
-};
-static double cuts(CePlan &p, const GradShape &s, int64_t of_piece, bool choose)
-{
-    const int64_t cu = compute_units(), across = ceil_div(p.width, s.n);
-    const int64_t tx = ceil_div(p.rows, s.m) * across, tw = ceil_div(of_piece, s.m) * across, sx = ceil_div(of_piece, s.slab), sw = ceil_div(p.rows, s.slab);
-    const int64_t extra = (int64_t)(s.tile_us / s.us + 0.5);
-    double best = 1e30;
-    for (int64_t x = 1; x <= 32 && (x == 1 || sx / x >= 8); x++)
-        for (int64_t w = 1; w <= 32 && (w == 1 || sw / w >= 8); w++) {
-            if ((x > 1 && tx * x > 8 * cu) || (w > 1 && tw * w > 8 * cu)) continue;
-            const double bytes = ((x > 1 ? 8.0 * x * p.rows : 0.0) + (w > 1 ? 8.0 * w * of_piece : 0.0)) * p.width;
-            const double t = s.us * makespan(cu, tx * x, ceil_div(sx, x) + extra, tw * w, ceil_div(sw, w) + extra) + bytes / 4e6 + (x > 1 || w > 1 ? 5.0 : 0.0);
-            if (t >= best) continue;
-            best = t;
-            if (choose) p.dx_splits = (int)x, p.dw_splits = (int)w;
-        }
-    if (choose) p.grads = s.grads, p.gm = s.m, p.gn = s.n, p.slab_g = s.slab;
-    return best;
-}
-template <class S> static GradShape grad_shape(int grads, double us, double tile_us) { return GradShape{grads, S::ROWS, S::COLS, S::SLAB, us, tile_us}; }
-
-static void plan_gradients(CePlan &p, int64_t of_piece)
-{
-    const GradShape large = p.split ? grad_shape<SplitLarge>(CE_LARGE, 3.0, 12.0) : grad_shape<GradLarge>(CE_LARGE, 2.0, 6.0);
-    const GradShape middle = grad_shape<GradMiddle>(CE_MIDDLE, 1.3, 4.0);
-    const GradShape small = p.split ? grad_shape<SplitGradSmall>(CE_SMALL, 0.6, 2.4) : grad_shape<GradSmall>(CE_SMALL, 0.35, 1.4);
-    // slabs of 32 of 256 x 128 tiles
-    const int64_t work = ceil_div(p.width, 128) * (ceil_div(p.rows, 256) * ceil_div(of_piece, 32) + ceil_div(of_piece, 256) * ceil_div(p.rows, 32));
-    if (work < 16 * compute_units() * (p.split ? 1 : 2)) cuts(p, small, of_piece, true);
-    else if (p.split || cuts(p, large, of_piece, false) <= cuts(p, middle, of_piece, false)) cuts(p, large, of_piece, true);
-    else cuts(p, middle, of_piece, true);
-}
 
 // us of the tiles of the logits: rounds of large tiles, the last perhaps of halves, or of middle ones two on a compute unit, a last one of
 // which may have it alone
@@ -1066,7 +631,7 @@ static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool 
         const int64_t pieces = ceil_div(classes, piece);                      // of equal size
         p.piece = ceil_div(ceil_div(classes, pieces), 256) * 256;
         const int64_t of_piece = p.piece < classes ? p.piece : classes;
-        plan_gradients(p, p.piece < classes ? p.piece : classes);
+        plan_gradients(p, rows, of_piece, width, p.split);
         p.d_at = take(at, p.d_rows * p.piece * 2 * p.parts);
         p.dx_at = take(at, part_of(rows * width) * 4 * p.dx_splits);
         p.dw_at = take(at, part_of(p.piece * width) * 4 * p.dw_splits);
@@ -1085,12 +650,6 @@ static int check_sizes(const char *what, int64_t rows, int64_t classes, int widt
                VTDGE_ERR_UNSUPPORTED, "%s: %lld rows, %lld classes of %d", what, (long long)rows, (long long)classes, width);
     return VTDGE_OK;
 }
-
-#define VT_STEP(call)                        \
-    do {                                     \
-        const int vt_rc = (call);            \
-        if (vt_rc != VTDGE_OK) return vt_rc; \
-    } while (0)
 
 // whether the product routine can read an operand where it lies
 static bool lies_well(const void *src, int64_t ld, int width, int dtype)
@@ -1162,48 +721,6 @@ static int go_d_kept(const CeArgs &a, hipStream_t st)
     cross_entropy_d_kept_kernel<<<(unsigned)blocks, 256, 0, st>>>(a, (int)vecs, rows);
     return check_launch("cross_entropy_backward");
 }
-template <class S> static int go_grad(GradPair &g, hipStream_t st)
-{
-    int64_t blocks = 0;
-    for (GradArgs *a : {&g.dx, &g.dw}) {
-        const bool along = a == &g.dx;
-        if (!along) g.first_dw = (int)blocks;
-        if (a->rows == 0) continue;
-        a->tm = (int)ceil_div(a->rows, S::ROWS), a->tn = (int)ceil_div(a->cols, S::COLS);
-        if (a->out == nullptr && a->part == nullptr) a->tn = 1;                // the sums alone
-        VT_REQUIRE(a->stages <= ceil_div(a->sum_b, S::SLAB) && (along || a->stages <= ceil_div(a->sum_a, S::SLAB)) && a->splits >= 1 && a->splits <= a->stages,
-                   VTDGE_ERR_ARG, "cross_entropy_backward: %d stages over %lld rows in %d parts", a->stages, (long long)a->sum_b, a->splits);
-        blocks += (int64_t)a->tm * a->tn * a->splits;
-    }
-    VT_REQUIRE(blocks < (1 << 23), VTDGE_ERR_UNSUPPORTED, "cross_entropy_backward: %lld tiles", (long long)blocks);
-    if (blocks == 0) return VTDGE_OK;
-    auto kern = cross_entropy_grad_kernel<S>;
-    VT_RESERVE_LDS(kern, S::LDS, "cross_entropy_backward");
-    note_kernel(reinterpret_cast<const void *>(kern));
-    kern<<<(unsigned)blocks, S::THREADS, S::LDS, st>>>(g);
-    return check_launch("cross_entropy_backward");
-}
-
-static int sum_up(const SumJob *jobs, int count, const float *scale, const float *scale2, bool f32, hipStream_t st)
-{
-    SumArgs a{};
-    int n = 0;
-    for (int i = 0; i < count; i++) {
-        if (jobs[i].out == nullptr || jobs[i].part == nullptr) continue;
-        a.job[n] = jobs[i];
-        a.first[n + 1] = a.first[n] + ceil_div(jobs[i].n, 1024);
-        n++;
-    }
-    if (n == 0) return VTDGE_OK;
-    const int64_t blocks = a.first[n];
-    for (int i = n; i < 3; i++) a.first[i + 1] = blocks;
-    VT_REQUIRE(blocks < (1 << 24), VTDGE_ERR_UNSUPPORTED, "cross_entropy_backward: a gradient of %lld blocks", (long long)blocks);
-    a.scale = scale, a.scale2 = scale2, a.f32 = f32;
-    note_kernel(reinterpret_cast<const void *>(cross_entropy_sum_kernel));
-    cross_entropy_sum_kernel<<<(unsigned)blocks, 256, 0, st>>>(a);
-    return check_launch("cross_entropy_backward");
-}
-
 }  // namespace vtdge
 
 using namespace vtdge;
@@ -1317,7 +834,7 @@ extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const vo
         else if (p.split) VT_STEP(p.logits == CE_LARGE ? go_d<SplitLarge>(a, p, st) : p.logits == CE_FLAT ? go_d<SplitFlat>(a, p, st) : go_d<SplitSmall>(a, p, st));
         else VT_STEP(p.logits == CE_LARGE ? go_d<LogitsLarge>(a, p, st) : p.logits == CE_MIDDLE ? go_d<LogitsMiddle>(a, p, st) : p.logits == CE_FLAT ? go_d<LogitsFlat>(a, p, st) : go_d<LogitsSmall>(a, p, st));
         GradPair g{};
-        g.scale = scale, g.scale2 = inv_count, g.f32 = p.split;
+        g.scale = scale, g.scale2 = inv_count, g.f32 = p.split, g.f32_parts = p.split;
         if (dx != nullptr) {
             g.dx.a = Operand{a.d, a.d_pitch, a.d_plane}, g.dx.b = Operand{a.w.p + v0 * a.w.pitch, a.w.pitch, a.w.plane};
             g.dx.rows = rows, g.dx.cols = width, g.dx.sum_b = live, g.dx.span_b = p.padded;
@@ -1333,14 +850,13 @@ extern "C" int vtdge_cross_entropy_backward(const void *x, int64_t ldx, const vo
             g.dw.sums_part = dbias != nullptr ? db_part : nullptr, g.dw.sums_stride = part_of(p.piece);
             g.dw.sums = dbias != nullptr ? (unsigned char *)dbias + v0 * elem : nullptr;
         }
-        if (p.split) VT_STEP(p.grads == CE_LARGE ? go_grad<SplitLarge>(g, st) : go_grad<SplitGradSmall>(g, st));
-        else VT_STEP(p.grads == CE_LARGE ? go_grad<GradLarge>(g, st) : p.grads == CE_MIDDLE ? go_grad<GradMiddle>(g, st) : go_grad<GradSmall>(g, st));
+        VT_STEP(launch_gradients(p, g, "cross_entropy_backward", st));
         // parts of this piece's dW and db, and of dx behind the last piece
         const bool last = a.v1 == classes;
         const SumJob jobs[3] = {{dx_part, last ? dx : nullptr, rows * width, part_of(rows * width), p.dx_splits},
                                 {g.dw.part, g.dw.out, live * width, g.dw.part_stride, p.dw_splits},
                                 {g.dw.sums_part, g.dw.sums, live, g.dw.sums_stride, p.dw_splits}};
-        VT_STEP(sum_up(jobs, 3, scale, inv_count, p.split, st));
+        VT_STEP(sum_parts(jobs, 3, scale, inv_count, p.split, "cross_entropy_backward", st));
     }
     return VTDGE_OK;
 }

@@ -1,0 +1,502 @@
+// Rows of 8-bit numbers with a power of two for every 128 of them ("blocks"), and what a training step keeps in them (gfx950): activations,
+// the input of GELU, the centred input of LayerNorm.  The Linear over blocks is in linear_8bit.hip.
+//
+//   e = the smallest whole number with max |x| 2^-e <= 448, -110 at least;   value = e4m3(x 2^-e), nearest, ties to even
+//
+// A power of two makes x 2^-e exact, so that a value is rounded once; every number of a block is a bf16 number (4 bits), and from -110 on no
+// denormal one.  The scale is the byte e + 127.  Infinities and NaN become NaN and do not count in the maximum; a block without a finite
+// number has the least scale.  The largest fp32 numbers would be rounded beyond fp32 and stop at 240 2^120.
+//
+// All of these read and write each number once and are bound by memory.  A lane has eight consecutive numbers (16 bytes of bf16, 32 of
+// fp32), sixteen lanes a block, so that maxima are taken with four lane moves and blocks leave in whole lines of 128 bytes.
+#include "eight_bit.h"
+
+namespace vtdge {
+
+// ------------------------------------------------------------------------------------------------ blocks
+template <typename T, bool WIDE> __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs p)
+{
+    const bool second = blockIdx.x >= p.first;
+    const QuantizeJob &job = p.job[second ? 1 : 0];
+    const uint32_t id = (blockIdx.x - (second ? p.first : 0)) * 16 + (threadIdx.x >> 4), row = id / job.per_row, block = id - row * job.per_row;
+    const int part = threadIdx.x & 15, c = (int)block * BLOCK + part * 8;
+    const bool in = row < job.rows;
+    float f[8];
+    load8<T, WIDE>(static_cast<const T *>(job.from) + (int64_t)row * job.ld + c, in ? job.n - c : 0, f);
+    const Rounded q = round8(f);
+    if (!in) return;
+    if (job.values != nullptr) {
+        *reinterpret_cast<u32x2 *>(job.values + (int64_t)row * job.value_pitch + c) = q.bytes;
+        if (part == 0) put_scale(job.scales + (int64_t)row * job.scale_pitch, (int)block, (int)job.per_row, job.scale_pitch, q.scale);
+    }
+    if (job.expanded != nullptr && c < job.expanded_pitch) *reinterpret_cast<u32x4 *>(job.expanded + (int64_t)row * job.expanded_pitch + c) = expand8(q.bytes, q.scale);
+}
+
+// blocks -> numbers; VECTOR: whole vectors of a dense row on 16-byte boundaries
+template <typename T, bool VECTOR> __global__ __launch_bounds__(256) void dequantize_kernel(DequantizeArgs p)
+{
+    const bool second = blockIdx.x >= p.first;
+    const DequantizeJob &job = p.job[second ? 1 : 0];
+    const uint32_t id = (blockIdx.x - (second ? p.first : 0)) * 256 + threadIdx.x, row = id / job.per_row, c = (id - row * job.per_row) * 8;
+    if (row >= job.rows) return;
+    const u32x2 bytes = *reinterpret_cast<const u32x2 *>(job.values + (int64_t)row * job.value_pitch + c);
+    const int scale = job.scales[(int64_t)row * job.scale_pitch + c / BLOCK];
+    float f[8];
+    stands_for8(bytes, scale, f);
+    store8<T, VECTOR>(static_cast<T *>(job.to) + (int64_t)row * job.ld + c, (int)job.n - (int)c, f);
+}
+
+// ------------------------------------------------------------------------------------------------ GELU
+template <typename T, bool WIDE> __global__ __launch_bounds__(256) void gelu_keep_kernel(GeluArgs p)
+{
+    const uint32_t id = blockIdx.x * 16 + (threadIdx.x >> 4), row = id / p.per_row, block = id - row * p.per_row;
+    const int part = threadIdx.x & 15, c = (int)block * BLOCK + part * 8;
+    const bool in = row < p.rows;
+    float f[8], y[8];
+    load8<T, WIDE>(static_cast<const T *>(p.x) + (int64_t)row * p.ld + c, in ? p.n - c : 0, f);
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = gelu_fn<T>(f[e]);
+    const Rounded q = round8(f);
+    if (!in) return;
+    store8<T, WIDE>(static_cast<T *>(p.y) + (int64_t)row * p.n + c, p.n - c, y);
+    if (p.values == nullptr) return;
+    *reinterpret_cast<u32x2 *>(p.values + (int64_t)row * p.value_pitch + c) = q.bytes;
+    if (part == 0) put_scale(p.scales + (int64_t)row * p.scale_pitch, (int)block, (int)p.per_row, p.scale_pitch, q.scale);
+}
+
+// Phi(x) + x phi(x): gelu_fn's polynomial for Phi, whose exponential is phi's.  3e-8 of the largest value.
+__device__ __forceinline__ float gelu_slope(float v)
+{
+    const float a = fminf(fabsf(v), 16.0f);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.35f, a, 1.0f));
+    float q = -0.02912587f;
+    q = __builtin_fmaf(q, t, 0.14387225f);
+    q = __builtin_fmaf(q, t, -0.25550460f);
+    q = __builtin_fmaf(q, t, 0.15892934f);
+    q = __builtin_fmaf(q, t, -0.02293717f);
+    q = __builtin_fmaf(q, t, 0.10543295f);
+    q = __builtin_fmaf(q, t, 0.11985243f);
+    q = __builtin_fmaf(q, t, 0.13985908f);
+    q = __builtin_fmaf(q, t, 0.13962157f);
+    const float e = __builtin_amdgcn_exp2f(a * (a * -0.72134752f)), neg = q * t * e;
+    return __builtin_fmaf(v * 0.39894228f, e, v < 0.f ? neg : 1.f - neg);
+}
+template <typename T, bool WIDE> __global__ __launch_bounds__(256) void gelu_slope_kernel(GeluArgs p)
+{
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, row = id / p.per_row, c = (id - row * p.per_row) * 8;
+    if (row >= p.rows) return;
+    float g[8], x[8];
+    load8<T, WIDE>(static_cast<const T *>(p.x) + (int64_t)row * p.ld + c, p.n - (int)c, g);
+    stands_for8(*reinterpret_cast<const u32x2 *>(p.values + (int64_t)row * p.value_pitch + c), p.scales[(int64_t)row * p.scale_pitch + c / BLOCK], x);
+#pragma unroll
+    for (int e = 0; e < 8; e++) g[e] *= gelu_slope(x[e]);
+    store8<T, WIDE>(static_cast<T *>(p.y) + (int64_t)row * p.n + c, p.n - (int)c, g);
+}
+
+// ------------------------------------------------------------------------------------------------ LayerNorm
+// A row by WAVES waves, a lane CH times eight numbers, WAVES * 512 apart.
+template <int WAVES> __device__ __forceinline__ int norm_column(int ch) { return (ch * WAVES * 64 + (int)(threadIdx.x & (WAVES * 64 - 1))) * 8; }
+
+// the sums of a row's waves, in each of them; `shared` a place of its own for each call
+template <int WAVES, int NV, typename V> __device__ __forceinline__ void row_sums(V (&v)[NV], V (*shared)[NV])
+{
+#pragma unroll
+    for (int i = 0; i < NV; i++) v[i] = wave_total(v[i]);
+    if constexpr (WAVES > 1) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < NV; i++) shared[wave][i] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            v[i] = shared[0][i];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) v[i] += shared[w][i];
+        }
+    }
+}
+
+// The mean is the fp32 number next to the exact one, so that what is rounded to 8 bits behind it does not hang on the order of a sum:
+// the sum is taken in 64 bits.
+template <typename T, int WAVES, int CH, bool WIDE> __global__ __launch_bounds__(256) void norm_keep_kernel(NormArgs p)
+{
+    __shared__ double sums64[WAVES][1];
+    __shared__ float sums32[WAVES][1];
+    const int64_t row = (int64_t)blockIdx.x * (4 / WAVES) + (WAVES == 1 ? threadIdx.x >> 6 : 0);
+    const bool in = row < p.rows;
+    if (WAVES == 1 && !in) return;                  // (a whole wave)
+    float f[CH][8];
+    double sum[1] = {0.0};
+#pragma unroll
+    for (int k = 0; k < CH; k++) {
+        const int c = norm_column<WAVES>(k);
+        load8<T, WIDE>(static_cast<const T *>(p.x) + row * p.ld + c, p.n - c, f[k]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum[0] += (double)f[k][e];
+    }
+    row_sums<WAVES>(sum, sums64);
+    const float mean = (float)(sum[0] / (double)p.n);
+    float square[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < CH; k++) {
+        const int left = p.n - norm_column<WAVES>(k);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            f[k][e] = e < left ? f[k][e] - mean : 0.f;
+            square[0] = __builtin_fmaf(f[k][e], f[k][e], square[0]);
+        }
+    }
+    row_sums<WAVES>(square, sums32);
+    const float r = __builtin_amdgcn_rsqf(square[0] / (float)p.n + p.eps);
+    if (p.rstd != nullptr && norm_column<WAVES>(0) == 0) p.rstd[row] = r;
+#pragma unroll
+    for (int k = 0; k < CH; k++) {
+        const int c = norm_column<WAVES>(k), left = p.n - c;
+        const Rounded q = round8(f[k]);
+        if (c < p.value_pitch && p.values != nullptr) {
+            *reinterpret_cast<u32x2 *>(p.values + row * p.value_pitch + c) = q.bytes;
+            if (c % BLOCK == 0) put_scale(p.scales + row * p.scale_pitch, c / BLOCK, p.blocks, p.scale_pitch, q.scale);
+        }
+        if (left <= 0) continue;
+        float w[8], b[8];
+        load8<T, WIDE>(static_cast<const T *>(p.weight) + c, left, w);
+        load8<T, WIDE>(static_cast<const T *>(p.bias) + c, left, b);
+#pragma unroll
+        for (int e = 0; e < 8; e++) f[k][e] = __builtin_fmaf(f[k][e] * r, w[e], b[e]);
+        store8<T, WIDE>(static_cast<T *>(p.y) + row * p.n + c, left, f[k]);
+    }
+}
+
+// h = c r;  dx = r (g - mean g - h mean(g h)), g = dy w;  dw = sum dy h, db = sum dy over the rows: a workgroup's rows in registers, four waves
+// joined in LDS, workgroups by norm_join_kernel.
+template <typename T, int WAVES, int CH, bool WIDE> __global__ __launch_bounds__(256) void norm_slope_kernel(NormArgs p)
+{
+    constexpr int ROWS = 4 / WAVES;                 // at once
+    __shared__ float sums32[2][WAVES][2];
+    extern __shared__ __attribute__((aligned(16))) float columns[];        // [2][n], joining ROWS > 1
+    float w[CH][8], dw[CH][8], db[CH][8];
+#pragma unroll
+    for (int k = 0; k < CH; k++) {
+        const int c = norm_column<WAVES>(k);
+        load8<T, WIDE>(static_cast<const T *>(p.weight) + c, p.n - c, w[k]);
+#pragma unroll
+        for (int e = 0; e < 8; e++) dw[k][e] = db[k][e] = 0.f;
+    }
+    const float inv_n = 1.0f / (float)p.n;
+    int turn = 0;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + (WAVES == 1 ? threadIdx.x >> 6 : 0); row < p.rows; row += (int64_t)gridDim.x * ROWS) {
+        float g[CH][8], h[CH][8], s[2] = {0.f, 0.f};
+        const float r = p.rstd[row];
+#pragma unroll
+        for (int k = 0; k < CH; k++) {
+            const int c = norm_column<WAVES>(k), left = p.n - c;
+            load8<T, WIDE>(static_cast<const T *>(p.x) + row * p.ld + c, left, g[k]);
+            u32x2 bytes = {0u, 0u};
+            int scale = 127;
+            if (left > 0) {
+                bytes = *reinterpret_cast<const u32x2 *>(p.values + row * p.value_pitch + c);
+                scale = p.scales[row * p.scale_pitch + c / BLOCK];
+            }
+            stands_for8(bytes, scale, h[k]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                h[k][e] *= r;
+                dw[k][e] = __builtin_fmaf(g[k][e], h[k][e], dw[k][e]);
+                db[k][e] += g[k][e];
+                g[k][e] *= w[k][e];
+                s[0] += g[k][e];
+                s[1] = __builtin_fmaf(g[k][e], h[k][e], s[1]);
+            }
+        }
+        if (p.y == nullptr) continue;               // (the same for all)
+        row_sums<WAVES>(s, sums32[turn]);
+        turn ^= 1;                                  // the next row's sums do not wait for the readers of these
+        const float m0 = s[0] * inv_n, m1 = s[1] * inv_n;
+#pragma unroll
+        for (int k = 0; k < CH; k++) {
+            const int c = norm_column<WAVES>(k), left = p.n - c;
+            if (left <= 0) continue;
+#pragma unroll
+            for (int e = 0; e < 8; e++) g[k][e] = r * (g[k][e] - m0 - h[k][e] * m1);
+            store8<T, WIDE>(static_cast<T *>(p.y) + row * p.n + c, left, g[k]);
+        }
+    }
+    if (p.part == nullptr) return;
+    if constexpr (ROWS > 1) {
+        const int wave = threadIdx.x >> 6;
+        for (int turn = 0; turn < ROWS; turn++) {
+            if (wave == turn)
+#pragma unroll
+                for (int k = 0; k < CH; k++) {
+                    const int c = norm_column<WAVES>(k);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (c + e < p.n) {
+                            columns[c + e] = dw[k][e] + (turn > 0 ? columns[c + e] : 0.f);
+                            columns[p.n + c + e] = db[k][e] + (turn > 0 ? columns[p.n + c + e] : 0.f);
+                        }
+                }
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < 2 * p.n; i += 256) p.part[(int64_t)blockIdx.x * 2 * p.n + i] = columns[i];
+    } else {
+#pragma unroll
+        for (int k = 0; k < CH; k++) {
+            const int c = norm_column<WAVES>(k);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (c + e < p.n) {
+                    p.part[(int64_t)blockIdx.x * 2 * p.n + c + e] = dw[k][e];
+                    p.part[(int64_t)blockIdx.x * 2 * p.n + p.n + c + e] = db[k][e];
+                }
+        }
+    }
+}
+// the workgroups' sums of 64 columns, by sixteen waves
+template <typename T> __global__ __launch_bounds__(1024) void norm_join_kernel(const float *part, int parts, int n, T *dw, T *db)
+{
+    __shared__ float sums[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
+    float sum = 0.f;
+    if (i < 2 * n)
+#pragma unroll 8
+        for (int k = wave; k < parts; k += 16) sum += part[(int64_t)k * 2 * n + i];
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0 || i >= 2 * n) return;
+    sum = 0.f;
+    for (int w = 0; w < 16; w++) sum += sums[w][lane];
+    T *const to = i < n ? dw : db;
+    if (to != nullptr) Elem<T>::store(to + (i < n ? i : i - n), sum);
+}
+
+// ------------------------------------------------------------------------------------------------ on the host
+int check_blocks(const char *what, int64_t rows, int64_t n)
+{
+    VT_REQUIRE(rows > 0 && n > 0, VTDGE_ERR_ARG, "%s: %lld rows of %lld", what, (long long)rows, (long long)n);
+    VT_REQUIRE(rows < (1ll << 31) && n <= (1 << 20) && rows * ceil_div(n, 8) < (1ll << 32) - 65536 * 256, VTDGE_ERR_UNSUPPORTED, "%s: %lld rows of %lld", what,
+               (long long)rows, (long long)n);
+    return VTDGE_OK;
+}
+bool wide_rows(const void *p, int64_t ld, int dtype) { return ((uintptr_t)p & 15) == 0 && ld % (dtype == VTDGE_F32 ? 4 : 8) == 0; }
+
+QuantizeJob quantize_job(const void *from, int64_t ld, int64_t rows, int64_t n, void *blocks, bf16_t *expanded, int64_t expanded_pitch)
+{
+    QuantizeJob j{};
+    j.from = from, j.ld = ld, j.rows = (uint32_t)rows, j.n = (int)n, j.per_row = (uint32_t)ceil_div(n, BLOCK);
+    if (blocks != nullptr) j.values = values_of(blocks), j.scales = scales_of(blocks, rows, n);
+    j.value_pitch = value_pitch(n), j.scale_pitch = (int)scale_pitch(n);
+    j.expanded = expanded, j.expanded_pitch = expanded_pitch;
+    return j;
+}
+int launch_quantize(QuantizeArgs &a, int jobs, int dtype, const char *what, hipStream_t st)
+{
+    int64_t blocks = 0;
+    bool wide = true;
+    for (int i = 0; i < jobs; i++) {
+        blocks += ceil_div((int64_t)a.job[i].rows * a.job[i].per_row, 16);
+        if (i == 0) a.first = (uint32_t)blocks;
+        wide = wide && wide_rows(a.job[i].from, a.job[i].rows > 1 ? a.job[i].ld : 0, dtype);
+    }
+    VT_REQUIRE(blocks < (1ll << 31), VTDGE_ERR_UNSUPPORTED, "%s: %lld blocks", what, (long long)blocks);
+    auto kern = dtype == VTDGE_F32 ? (wide ? quantize_kernel<float, true> : quantize_kernel<float, false>)
+                                   : (wide ? quantize_kernel<bf16_t, true> : quantize_kernel<bf16_t, false>);
+    note_kernel(reinterpret_cast<const void *>(kern));
+    kern<<<(unsigned)blocks, 256, 0, st>>>(a);
+    return check_launch(what);
+}
+DequantizeJob dequantize_job(const void *blocks, int64_t rows, int64_t n, void *to, int64_t ld, int64_t columns)
+{
+    DequantizeJob j{};
+    j.values = values_of(blocks), j.scales = scales_of(blocks, rows, n), j.rows = (uint32_t)rows, j.per_row = (uint32_t)ceil_div(columns, 8);
+    j.value_pitch = value_pitch(n), j.scale_pitch = (int)scale_pitch(n), j.n = columns, j.to = to, j.ld = ld;
+    return j;
+}
+int launch_dequantize(DequantizeArgs &a, int jobs, int dtype, const char *what, hipStream_t st)
+{
+    int64_t blocks = 0;
+    bool wide = true;
+    for (int i = 0; i < jobs; i++) {
+        blocks += ceil_div((int64_t)a.job[i].rows * a.job[i].per_row, 256);
+        if (i == 0) a.first = (uint32_t)blocks;
+        wide = wide && wide_rows(a.job[i].to, a.job[i].rows > 1 ? a.job[i].ld : 0, dtype);
+    }
+    VT_REQUIRE(blocks < (1ll << 31), VTDGE_ERR_UNSUPPORTED, "%s: %lld blocks", what, (long long)blocks);
+    auto kern = dtype == VTDGE_F32 ? (wide ? dequantize_kernel<float, true> : dequantize_kernel<float, false>)
+                                   : (wide ? dequantize_kernel<bf16_t, true> : dequantize_kernel<bf16_t, false>);
+    note_kernel(reinterpret_cast<const void *>(kern));
+    kern<<<(unsigned)blocks, 256, 0, st>>>(a);
+    return check_launch(what);
+}
+
+static int check_dtype(const char *what, int dtype)
+{
+    VT_REQUIRE(dtype == VTDGE_F32 || dtype == VTDGE_BF16, VTDGE_ERR_ARG, "%s: dtype %d", what, dtype);
+    return VTDGE_OK;
+}
+
+// waves of a row and chunks of a lane
+static void norm_shape(int n, int &waves, int &ch)
+{
+    waves = n <= 1024 ? 1 : 4;
+    ch = (int)ceil_div(n, waves * 512);
+    if (ch == 3) ch = 4;
+}
+static int64_t norm_parts(int64_t rows, int n)
+{
+    const int64_t at_once = n <= 1024 ? 4 : 1, most = 4 * compute_units(), all = ceil_div(rows, at_once);
+    return all < most ? all : most;
+}
+
+#define VT_NORM_CASE(KERN, T, WIDE)                                                                  \
+    (waves == 1 ? (ch == 1 ? KERN<T, 1, 1, WIDE> : KERN<T, 1, 2, WIDE>)                              \
+                : (ch == 1 ? KERN<T, 4, 1, WIDE> : ch == 2 ? KERN<T, 4, 2, WIDE> : KERN<T, 4, 4, WIDE>))
+#define VT_NORM_KERNEL(KERN)                                                                                    \
+    (dtype == VTDGE_F32 ? (wide ? VT_NORM_CASE(KERN, float, true) : VT_NORM_CASE(KERN, float, false))           \
+                        : (wide ? VT_NORM_CASE(KERN, bf16_t, true) : VT_NORM_CASE(KERN, bf16_t, false)))
+
+static int check_norm(const char *what, int64_t rows, int64_t n, int dtype)
+{
+    VT_STEP(check_dtype(what, dtype));
+    VT_STEP(check_blocks(what, rows, n));
+    VT_REQUIRE(n <= VTDGE_MAX_NORM_8BIT, VTDGE_ERR_UNSUPPORTED, "%s: rows of %lld, %d at most", what, (long long)n, VTDGE_MAX_NORM_8BIT);
+    return VTDGE_OK;
+}
+
+}  // namespace vtdge
+
+using namespace vtdge;
+
+extern "C" int64_t vtdge_blocks_bytes(int64_t rows, int64_t n)
+{
+    if (check_blocks("blocks_bytes", rows, n) != VTDGE_OK) return -1;
+    return blocks_bytes(rows, n);
+}
+
+extern "C" int vtdge_quantize_blocks(const void *x, int64_t ldx, int64_t rows, int64_t n, void *blocks, int dtype, void *stream)
+{
+    VT_STEP(check_dtype("quantize_blocks", dtype));
+    VT_STEP(check_blocks("quantize_blocks", rows, n));
+    VT_REQUIRE(x && blocks, VTDGE_ERR_ARG, "quantize_blocks: NULL operand");
+    VT_REQUIRE(ldx >= n || rows == 1, VTDGE_ERR_ARG, "quantize_blocks: rows of %lld, %lld apart", (long long)n, (long long)ldx);
+    VT_REQUIRE(((uintptr_t)blocks & 127) == 0, VTDGE_ERR_ARG, "quantize_blocks: blocks off their boundary");
+    QuantizeArgs a{};
+    a.job[0] = quantize_job(x, ldx, rows, n, blocks, nullptr, 0);
+    return launch_quantize(a, 1, dtype, "quantize_blocks", (hipStream_t)stream);
+}
+
+extern "C" int vtdge_dequantize_blocks(const void *blocks, int64_t rows, int64_t n, void *out, int dtype, void *stream)
+{
+    VT_STEP(check_dtype("dequantize_blocks", dtype));
+    VT_STEP(check_blocks("dequantize_blocks", rows, n));
+    VT_REQUIRE(out && blocks, VTDGE_ERR_ARG, "dequantize_blocks: NULL operand");
+    VT_REQUIRE(((uintptr_t)blocks & 127) == 0, VTDGE_ERR_ARG, "dequantize_blocks: blocks off their boundary");
+    DequantizeArgs a{};
+    a.job[0] = dequantize_job(blocks, rows, n, out, n, n);
+    return launch_dequantize(a, 1, dtype, "dequantize_blocks", (hipStream_t)stream);
+}
+
+static int gelu_args(const char *what, GeluArgs &a, const void *x, int64_t ldx, int64_t rows, int64_t n, const void *blocks, void *y, int dtype)
+{
+    VT_STEP(check_dtype(what, dtype));
+    VT_STEP(check_blocks(what, rows, n));
+    VT_REQUIRE(x && y, VTDGE_ERR_ARG, "%s: NULL operand", what);
+    VT_REQUIRE(ldx >= n || rows == 1, VTDGE_ERR_ARG, "%s: rows of %lld, %lld apart", what, (long long)n, (long long)ldx);
+    VT_REQUIRE(((uintptr_t)blocks & 127) == 0, VTDGE_ERR_ARG, "%s: blocks off their boundary", what);
+    a.x = x, a.ld = ldx, a.rows = (uint32_t)rows, a.n = (int)n, a.y = y;
+    if (blocks != nullptr) a.values = values_of(blocks), a.scales = scales_of(blocks, rows, n);
+    a.value_pitch = value_pitch(n), a.scale_pitch = (int)scale_pitch(n);
+    return VTDGE_OK;
+}
+static bool gelu_wide(const GeluArgs &a, int dtype) { return wide_rows(a.x, a.rows > 1 ? a.ld : 0, dtype) && wide_rows(a.y, a.rows > 1 ? a.n : 0, dtype); }
+
+extern "C" int vtdge_gelu_8bit(const void *x, int64_t ldx, int64_t rows, int64_t n, void *y, void *blocks, int dtype, void *stream)
+{
+    GeluArgs a{};
+    VT_STEP(gelu_args("gelu_8bit", a, x, ldx, rows, n, blocks, y, dtype));
+    a.per_row = (uint32_t)ceil_div(n, BLOCK);
+    const bool wide = gelu_wide(a, dtype);
+    auto kern = dtype == VTDGE_F32 ? (wide ? gelu_keep_kernel<float, true> : gelu_keep_kernel<float, false>)
+                                   : (wide ? gelu_keep_kernel<bf16_t, true> : gelu_keep_kernel<bf16_t, false>);
+    note_kernel(reinterpret_cast<const void *>(kern));
+    kern<<<(unsigned)ceil_div(rows * a.per_row, 16), 256, 0, (hipStream_t)stream>>>(a);
+    return check_launch("gelu_8bit");
+}
+
+extern "C" int vtdge_gelu_8bit_backward(const void *grad, int64_t ldg, int64_t rows, int64_t n, const void *blocks, void *dx, int dtype, void *stream)
+{
+    GeluArgs a{};
+    VT_STEP(gelu_args("gelu_8bit_backward", a, grad, ldg, rows, n, blocks, dx, dtype));
+    VT_REQUIRE(blocks, VTDGE_ERR_ARG, "gelu_8bit_backward: NULL operand");
+    a.per_row = (uint32_t)ceil_div(n, 8);
+    const bool wide = gelu_wide(a, dtype);
+    auto kern = dtype == VTDGE_F32 ? (wide ? gelu_slope_kernel<float, true> : gelu_slope_kernel<float, false>)
+                                   : (wide ? gelu_slope_kernel<bf16_t, true> : gelu_slope_kernel<bf16_t, false>);
+    note_kernel(reinterpret_cast<const void *>(kern));
+    kern<<<(unsigned)ceil_div(rows * a.per_row, 256), 256, 0, (hipStream_t)stream>>>(a);
+    return check_launch("gelu_8bit_backward");
+}
+
+extern "C" int vtdge_layernorm_8bit(const void *x, int64_t ldx, const void *weight, const void *bias, float eps, int64_t rows, int64_t n, void *y,
+                                    void *blocks, float *rstd, int dtype, void *stream)
+{
+    VT_STEP(check_norm("layernorm_8bit", rows, n, dtype));
+    VT_REQUIRE(x && weight && bias && y && (blocks != nullptr) == (rstd != nullptr), VTDGE_ERR_ARG, "layernorm_8bit: NULL operand");
+    VT_REQUIRE(ldx >= n || rows == 1, VTDGE_ERR_ARG, "layernorm_8bit: rows of %lld, %lld apart", (long long)n, (long long)ldx);
+    VT_REQUIRE(((uintptr_t)blocks & 127) == 0, VTDGE_ERR_ARG, "layernorm_8bit: blocks off their boundary");
+    NormArgs a{};
+    a.x = x, a.ld = ldx, a.weight = weight, a.bias = bias, a.eps = eps, a.rows = rows, a.n = (int)n, a.y = y, a.rstd = rstd;
+    if (blocks != nullptr) a.values = values_of(blocks), a.scales = scales_of(blocks, rows, n);
+    a.value_pitch = (int)value_pitch(n), a.scale_pitch = (int)scale_pitch(n);
+    a.blocks = (int)ceil_div(n, BLOCK);
+    int waves, ch;
+    norm_shape((int)n, waves, ch);
+    const bool wide = wide_rows(x, rows > 1 ? ldx : 0, dtype) && wide_rows(y, rows > 1 ? n : 0, dtype) && wide_rows(weight, 0, dtype) && wide_rows(bias, 0, dtype);
+    auto kern = VT_NORM_KERNEL(norm_keep_kernel);
+    note_kernel(reinterpret_cast<const void *>(kern));
+    kern<<<(unsigned)ceil_div(rows, 4 / waves), 256, 0, (hipStream_t)stream>>>(a);
+    return check_launch("layernorm_8bit");
+}
+
+extern "C" int64_t vtdge_layernorm_8bit_backward_workspace(int64_t rows, int64_t n)
+{
+    if (check_norm("layernorm_8bit_backward_workspace", rows, n, VTDGE_F32) != VTDGE_OK) return -1;
+    return norm_parts(rows, (int)n) * 2 * n * 4;
+}
+
+extern "C" int vtdge_layernorm_8bit_backward(const void *grad, int64_t ldg, const void *weight, const void *blocks, const float *rstd, int64_t rows,
+                                             int64_t n, void *workspace, int64_t workspace_bytes, void *dx, void *dweight, void *dbias, int dtype,
+                                             void *stream)
+{
+    VT_STEP(check_norm("layernorm_8bit_backward", rows, n, dtype));
+    VT_REQUIRE(grad && weight && blocks && rstd && workspace, VTDGE_ERR_ARG, "layernorm_8bit_backward: NULL operand");
+    VT_REQUIRE(ldg >= n || rows == 1, VTDGE_ERR_ARG, "layernorm_8bit_backward: rows of %lld, %lld apart", (long long)n, (long long)ldg);
+    VT_REQUIRE(((uintptr_t)blocks & 127) == 0, VTDGE_ERR_ARG, "layernorm_8bit_backward: blocks off their boundary");
+    const int64_t parts = norm_parts(rows, (int)n), bytes = parts * 2 * n * 4;
+    VT_REQUIRE(workspace_bytes >= bytes && ((uintptr_t)workspace & 15) == 0, VTDGE_ERR_ARG, "layernorm_8bit_backward: workspace of %lld bytes, %lld needed",
+               (long long)workspace_bytes, (long long)bytes);
+    const bool columns = dweight != nullptr || dbias != nullptr;
+    if (dx == nullptr && !columns) return VTDGE_OK;
+    NormArgs a{};
+    a.x = grad, a.ld = ldg, a.weight = weight, a.rows = rows, a.n = (int)n, a.y = dx, a.rstd = const_cast<float *>(rstd);
+    a.values = values_of(blocks), a.scales = scales_of(blocks, rows, n), a.value_pitch = (int)value_pitch(n), a.scale_pitch = (int)scale_pitch(n);
+    a.part = columns ? static_cast<float *>(workspace) : nullptr;
+    int waves, ch;
+    norm_shape((int)n, waves, ch);
+    const bool wide = wide_rows(grad, rows > 1 ? ldg : 0, dtype) && (dx == nullptr || wide_rows(dx, rows > 1 ? n : 0, dtype)) && wide_rows(weight, 0, dtype);
+    auto kern = VT_NORM_KERNEL(norm_slope_kernel);
+    note_kernel(reinterpret_cast<const void *>(kern));
+    kern<<<(unsigned)parts, 256, waves == 1 ? 2 * n * 4 : 0, (hipStream_t)stream>>>(a);
+    VT_STEP(check_launch("layernorm_8bit_backward"));
+    if (!columns) return VTDGE_OK;
+    const unsigned blocks64 = (unsigned)ceil_div(2 * n, 64);
+    if (dtype == VTDGE_F32) {
+        note_kernel(reinterpret_cast<const void *>(norm_join_kernel<float>));
+        norm_join_kernel<float><<<blocks64, 1024, 0, (hipStream_t)stream>>>(a.part, (int)parts, (int)n, (float *)dweight, (float *)dbias);
+    } else {
+        note_kernel(reinterpret_cast<const void *>(norm_join_kernel<bf16_t>));
+        norm_join_kernel<bf16_t><<<blocks64, 1024, 0, (hipStream_t)stream>>>(a.part, (int)parts, (int)n, (bf16_t *)dweight, (bf16_t *)dbias);
+    }
+    return check_launch("layernorm_8bit_backward");
+}

@@ -1,0 +1,263 @@
+// A Linear over blocks of 8-bit numbers, y = act(Q(x) Q(W)^T + b), and its gradients dx = g Q(W), dW = g^T Q(x), db = sum g (gfx950), g the
+// gradient of y rounded to bf16 (an error of half a step on each of many terms, as on any bf16 operand).
+#include "eight_bit.h"
+
+namespace vtdge {
+
+struct ForwardArgs {
+    Operand x, w;
+    const void *bias; void *y; int64_t rows, out; int stages;
+};
+
+// four values of a row from column c on
+template <typename T> __device__ __forceinline__ void put_row4(const ForwardArgs &p, int64_t r, int64_t c, const f32x4 &v)
+{
+    T *const to = static_cast<T *>(p.y) + r * p.out + c;
+    const int left = (int)(p.out - c);
+    if (left >= 4 && p.out % 4 == 0) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4 *>(to) = v;
+        else *reinterpret_cast<u32x2 *>(to) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (e < left) Elem<T>::store(to + e, v[e]);
+    }
+}
+
+template <class S, typename T, bool GELU> __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void linear_8bit_kernel(ForwardArgs p, int tm, int tn)
+{
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    constexpr int IM = S::IM, JN = S::JN;
+    int m, n;
+    tile_at(place_of(blockIdx.x, tm * tn), tm, tn, m, n);
+    const int64_t r0 = (int64_t)m * S::ROWS, c0 = (int64_t)n * S::COLS;
+    float *const bias = reinterpret_cast<float *>(smem + S::RING);
+    for (int c = threadIdx.x; c < S::COLS; c += S::THREADS)
+        bias[c] = p.bias != nullptr && c0 + c < p.out ? Elem<T>::load(static_cast<const T *>(p.bias) + c0 + c) : 0.f;
+    f32x16 acc[IM][JN] = {};
+    float none[IM];
+    const Loader<true, S::ROWS, S::SLAB, S::WAVES> a(p.x, r0, p.rows, 0);
+    const Loader<true, S::COLS, S::SLAB, S::WAVES> b(p.w, c0, p.out, 0);
+    multiply_tile<S, false>(a, b, 0, p.stages, smem, acc, false, none);
+    const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
+    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
+#pragma unroll
+    for (int i = 0; i < IM; i++) {
+        const int64_t r = r0 + (wm * IM + i) * 32 + lr;
+        if (r >= p.rows) continue;
+#pragma unroll
+        for (int j = 0; j < JN; j++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int c = (wn * JN + j) * 32 + 8 * q + 4 * lg;
+                f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                v += *reinterpret_cast<const f32x4 *>(bias + c);
+                if constexpr (GELU)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = gelu_fn<T>(v[e]);
+                put_row4<T>(p, r, c0 + c, v);
+            }
+    }
+}
+
+// Rows of g as the products read them: bf16, filled up with zeros to whole slabs.
+template <typename T, bool WIDE> __global__ __launch_bounds__(256) void pack_gradient_kernel(const T *from, int64_t ld, uint32_t rows, int n, uint32_t per_row, bf16_t *to)
+{
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, row = id / per_row, c = (id - row * per_row) * 8;
+    if (row >= rows) return;
+    float f[8];
+    load8<T, WIDE>(from + (int64_t)row * ld + c, n - (int)c, f);
+    *reinterpret_cast<u32x4 *>(to + ((int64_t)row * per_row * 8 + c)) = Elem<bf16_t>::pack(f);
+}
+
+// ------------------------------------------------------------------------------------------------ on the host
+using ForwardLarge = Shape<2, 4, 4, 2, 64, 2, 1>;
+using ForwardMiddle = Shape<2, 4, 2, 2, 32, 3, 1>;
+using ForwardSmall = Shape<1, 1, 2, 2, 64, 6, 1>;
+
+constexpr int SLAB = 64;
+static int64_t take(int64_t &at, int64_t bytes)
+{
+    const int64_t here = at;
+    at += (bytes + 255) / 256 * 256;
+    return here;
+}
+static int64_t padded(int64_t n) { return ceil_div(n, SLAB) * SLAB; }
+
+struct ForwardPlan {
+    int64_t x_at, w_at, bytes;
+};
+static ForwardPlan plan_forward(int64_t rows, int64_t out, int64_t width)
+{
+    ForwardPlan p{};
+    int64_t at = 0;
+    p.x_at = take(at, rows * padded(width) * 2);
+    p.w_at = take(at, out * padded(width) * 2);
+    p.bytes = at;
+    return p;
+}
+struct BackwardPlan : GradPlan {
+    int64_t g_at, x_at, w_at, dx_at, dw_at, db_at, bytes;
+};
+// whether the products read the gradient where it lies
+static bool gradient_lies(const void *g, int64_t ld, int64_t out, int dtype)
+{
+    return dtype == VTDGE_BF16 && out % SLAB == 0 && ld % 8 == 0 && ld < (1 << 22) && ((uintptr_t)g & 15) == 0;
+}
+static BackwardPlan plan_backward(int64_t rows, int64_t out, int64_t width, bool lies)
+{
+    BackwardPlan p{};
+    plan_gradients(p, rows, out, (int)width, false);
+    int64_t at = 0;
+    p.g_at = take(at, lies ? 0 : rows * padded(out) * 2);
+    p.x_at = take(at, rows * padded(width) * 2);
+    p.w_at = take(at, out * padded(width) * 2);
+    p.dx_at = take(at, part_of(rows * width) * 4 * p.dx_splits);
+    p.dw_at = take(at, part_of(out * width) * 4 * p.dw_splits);
+    p.db_at = take(at, part_of(out) * 4 * p.dw_splits);
+    p.bytes = at;
+    return p;
+}
+
+static int check_linear(const char *what, int64_t rows, int64_t out, int64_t width, int dtype)
+{
+    VT_REQUIRE(dtype == VTDGE_F32 || dtype == VTDGE_BF16, VTDGE_ERR_ARG, "%s: dtype %d", what, dtype);
+    VT_STEP(check_blocks(what, rows, width));
+    VT_STEP(check_blocks(what, out, width));
+    VT_STEP(check_blocks(what, rows, out));
+    VT_REQUIRE(out <= (1 << 20) && ceil_div(rows, 64) * ceil_div(out, 64) < (1 << 23), VTDGE_ERR_UNSUPPORTED, "%s: %lld rows, %lld outputs", what,
+               (long long)rows, (long long)out);
+    return VTDGE_OK;
+}
+
+template <class S, typename T, bool GELU> static int go_forward_as(const ForwardArgs &a, hipStream_t st)
+{
+    const int64_t tm = ceil_div(a.rows, S::ROWS), tn = ceil_div(a.out, S::COLS);
+    auto kern = linear_8bit_kernel<S, T, GELU>;
+    VT_RESERVE_LDS(kern, S::LDS, "linear_8bit");
+    note_kernel(reinterpret_cast<const void *>(kern));
+    kern<<<(unsigned)(tm * tn), S::THREADS, S::LDS, st>>>(a, (int)tm, (int)tn);
+    return check_launch("linear_8bit");
+}
+template <class S> static int go_forward(const ForwardArgs &a, int act, int dtype, hipStream_t st)
+{
+    if (dtype == VTDGE_F32) return act == VTDGE_ACT_GELU ? go_forward_as<S, float, true>(a, st) : go_forward_as<S, float, false>(a, st);
+    return act == VTDGE_ACT_GELU ? go_forward_as<S, bf16_t, true>(a, st) : go_forward_as<S, bf16_t, false>(a, st);
+}
+
+}  // namespace vtdge
+
+using namespace vtdge;
+
+extern "C" int64_t vtdge_linear_8bit_workspace(int64_t rows, int64_t out, int64_t width, int dtype)
+{
+    if (check_linear("linear_8bit_workspace", rows, out, width, dtype) != VTDGE_OK) return -1;
+    return plan_forward(rows, out, width).bytes;
+}
+
+extern "C" int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight, int64_t ldw, void *w_blocks, const void *bias, void *y, void *x_blocks,
+                                 int64_t rows, int64_t out, int64_t width, int act, void *workspace, int64_t workspace_bytes, int dtype, void *stream)
+{
+    VT_STEP(check_linear("linear_8bit", rows, out, width, dtype));
+    VT_REQUIRE(x && y && workspace && (weight || w_blocks), VTDGE_ERR_ARG, "linear_8bit: NULL operand");
+    VT_REQUIRE(act == VTDGE_ACT_NONE || act == VTDGE_ACT_GELU, VTDGE_ERR_ARG, "linear_8bit: act %d", act);
+    VT_REQUIRE((ldx >= width || rows == 1) && (weight == nullptr || ldw >= width || out == 1), VTDGE_ERR_ARG, "linear_8bit: rows of %lld, %lld and %lld apart",
+               (long long)width, (long long)ldx, (long long)ldw);
+    VT_REQUIRE(((uintptr_t)w_blocks & 127) == 0 && ((uintptr_t)x_blocks & 127) == 0, VTDGE_ERR_ARG, "linear_8bit: blocks off their boundary");
+    const ForwardPlan p = plan_forward(rows, out, width);
+    VT_REQUIRE(workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG, "linear_8bit: workspace of %lld bytes, %lld needed",
+               (long long)workspace_bytes, (long long)p.bytes);
+    unsigned char *const ws = (unsigned char *)workspace;
+    const hipStream_t st = (hipStream_t)stream;
+    bf16_t *const xb = (bf16_t *)(ws + p.x_at), *const wb = (bf16_t *)(ws + p.w_at);
+    QuantizeArgs q{};
+    q.job[0] = quantize_job(x, ldx, rows, width, x_blocks, xb, padded(width));
+    if (weight != nullptr) q.job[1] = quantize_job(weight, ldw, out, width, w_blocks, wb, padded(width));
+    VT_STEP(launch_quantize(q, weight != nullptr ? 2 : 1, dtype, "linear_8bit", st));
+    if (weight == nullptr) {
+        DequantizeArgs d{};
+        d.job[0] = dequantize_job(w_blocks, out, width, wb, padded(width), padded(width));
+        VT_STEP(launch_dequantize(d, 1, VTDGE_BF16, "linear_8bit", st));
+    }
+    ForwardArgs a{};
+    a.x = Operand{xb, padded(width), 0}, a.w = Operand{wb, padded(width), 0};
+    a.bias = bias, a.y = y, a.rows = rows, a.out = out;
+    const int64_t cu = compute_units();
+    if (ceil_div(rows, 128) * ceil_div(out, 256) < cu) {
+        a.stages = (int)(padded(width) / ForwardSmall::SLAB);
+        return go_forward<ForwardSmall>(a, act, dtype, st);
+    }
+    if (ceil_div(rows, 256) * ceil_div(out, 256) < 4 * cu) {
+        a.stages = (int)(padded(width) / ForwardMiddle::SLAB);
+        return go_forward<ForwardMiddle>(a, act, dtype, st);
+    }
+    a.stages = (int)(padded(width) / ForwardLarge::SLAB);
+    return go_forward<ForwardLarge>(a, act, dtype, st);
+}
+
+extern "C" int64_t vtdge_linear_8bit_backward_workspace(int64_t rows, int64_t out, int64_t width, int lies, int dtype)
+{
+    if (check_linear("linear_8bit_backward_workspace", rows, out, width, dtype) != VTDGE_OK) return -1;
+    return plan_backward(rows, out, width, lies != 0 && dtype == VTDGE_BF16 && out % SLAB == 0).bytes;
+}
+
+extern "C" int vtdge_linear_8bit_backward(const void *grad, int64_t ldg, const void *x_blocks, const void *w_blocks, int64_t rows, int64_t out,
+                                          int64_t width, void *workspace, int64_t workspace_bytes, void *dx, void *dweight, void *dbias, int dtype,
+                                          void *stream)
+{
+    VT_STEP(check_linear("linear_8bit_backward", rows, out, width, dtype));
+    if (dx == nullptr && dweight == nullptr && dbias == nullptr) return VTDGE_OK;
+    VT_REQUIRE(grad && workspace && (dx == nullptr || w_blocks) && (dweight == nullptr || x_blocks), VTDGE_ERR_ARG, "linear_8bit_backward: NULL operand");
+    VT_REQUIRE(ldg >= out || rows == 1, VTDGE_ERR_ARG, "linear_8bit_backward: rows of %lld, %lld apart", (long long)out, (long long)ldg);
+    VT_REQUIRE(((uintptr_t)w_blocks & 127) == 0 && ((uintptr_t)x_blocks & 127) == 0, VTDGE_ERR_ARG, "linear_8bit_backward: blocks off their boundary");
+    const bool lies = gradient_lies(grad, rows > 1 ? ldg : 0, out, dtype);
+    const BackwardPlan p = plan_backward(rows, out, width, lies);
+    VT_REQUIRE(workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG, "linear_8bit_backward: workspace of %lld bytes, %lld needed",
+               (long long)workspace_bytes, (long long)p.bytes);
+    unsigned char *const ws = (unsigned char *)workspace;
+    const hipStream_t st = (hipStream_t)stream;
+    bf16_t *const xb = (bf16_t *)(ws + p.x_at), *const wb = (bf16_t *)(ws + p.w_at);
+    Operand g_op{(const bf16_t *)grad, rows > 1 ? ldg : out, 0};
+    if (!lies) {
+        bf16_t *const to = (bf16_t *)(ws + p.g_at);
+        const uint32_t per_row = (uint32_t)(padded(out) / 8);
+        const unsigned blocks = (unsigned)ceil_div(rows * per_row, 256);
+        const bool wide = wide_rows(grad, rows > 1 ? ldg : 0, dtype);
+        auto go = [&](auto kern, auto *from) {
+            note_kernel(reinterpret_cast<const void *>(kern));
+            kern<<<blocks, 256, 0, st>>>(from, ldg, (uint32_t)rows, (int)out, per_row, to);
+            return check_launch("linear_8bit_backward");
+        };
+        if (dtype == VTDGE_F32) VT_STEP(wide ? go(pack_gradient_kernel<float, true>, (const float *)grad) : go(pack_gradient_kernel<float, false>, (const float *)grad));
+        else VT_STEP(wide ? go(pack_gradient_kernel<bf16_t, true>, (const bf16_t *)grad) : go(pack_gradient_kernel<bf16_t, false>, (const bf16_t *)grad));
+        g_op = Operand{to, padded(out), 0};
+    }
+    DequantizeArgs d{};
+    int jobs = 0;
+    if (dx != nullptr) d.job[jobs++] = dequantize_job(w_blocks, out, width, wb, padded(width), padded(width));
+    if (dweight != nullptr) d.job[jobs++] = dequantize_job(x_blocks, rows, width, xb, padded(width), padded(width));
+    if (jobs > 0) VT_STEP(launch_dequantize(d, jobs, VTDGE_BF16, "linear_8bit_backward", st));
+    GradPair g{};
+    g.f32 = dtype == VTDGE_F32, g.ends = true;
+    if (dx != nullptr) {
+        g.dx.a = g_op, g.dx.b = Operand{wb, padded(width), 0};
+        g.dx.rows = rows, g.dx.cols = width, g.dx.sum_b = out, g.dx.span_b = padded(width);
+        g.dx.stages = (int)ceil_div(out, p.slab_g), g.dx.splits = p.dx_splits;
+        g.dx.part = p.dx_splits == 1 ? nullptr : (float *)(ws + p.dx_at), g.dx.part_stride = part_of(rows * width), g.dx.out = dx;
+    }
+    if (dweight != nullptr || dbias != nullptr) {
+        // (without dW the second operand is not multiplied to any end: the gradient itself stands in its place)
+        g.dw.a = g_op, g.dw.b = dweight != nullptr ? Operand{xb, padded(width), 0} : g_op;
+        g.dw.rows = out, g.dw.cols = width, g.dw.sum_a = rows, g.dw.span_a = padded(out), g.dw.sum_b = rows;
+        g.dw.span_b = dweight != nullptr ? padded(width) : padded(out);
+        g.dw.stages = (int)ceil_div(rows, p.slab_g), g.dw.splits = p.dw_splits;
+        const bool cut = p.dw_splits > 1;
+        g.dw.part = cut && dweight != nullptr ? (float *)(ws + p.dw_at) : nullptr, g.dw.part_stride = part_of(out * width), g.dw.out = dweight;
+        g.dw.sums_part = cut && dbias != nullptr ? (float *)(ws + p.db_at) : nullptr, g.dw.sums_stride = part_of(out), g.dw.sums = dbias;
+    }
+    VT_STEP(launch_gradients(p, g, "linear_8bit_backward", st));
+    const SumJob sums[3] = {{g.dx.part, dx, rows * width, g.dx.part_stride, p.dx_splits},
+                            {g.dw.part, dweight, out * width, g.dw.part_stride, p.dw_splits},
+                            {g.dw.sums_part, dbias, out, g.dw.sums_stride, p.dw_splits}};
+    return sum_parts(sums, 3, nullptr, nullptr, g.f32, "linear_8bit_backward", st);
+}

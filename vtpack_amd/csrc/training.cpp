@@ -5,77 +5,11 @@
 // core comes out of its sleep for it, and what Python does there (the interpreter lock, four allocations, 24 arguments) took 32 of
 // the 122 us of a DeiT-S classifier's loss with its gradients (73 so); a step over 200 weights looked at some 1000 objects, 77 us beside the
 // 31 us of its kernels (9 so).
-#include <Python.h>
-
-#include <ATen/ATen.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-
-#include <algorithm>
-#include <array>
-#include <cstdint>
-#include <map>
-#include <mutex>
-#include <memory>
-#include <stdexcept>
-#include <string>
-#include <tuple>
-#include <vector>
-
-#include "../../include/vtdge.h"
+#include "training.h"
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::SavedVariable;
-using torch::autograd::variable_list;
-
-#define VT_FUNCTIONS(X)                                                                                                \
-    X(last_error) X(cross_entropy) X(cross_entropy_backward) X(cross_entropy_workspace) X(cross_entropy_laid_out)      \
-    X(gate_balance) X(gate_balance_backward) X(gate_balance_workspace) X(adamw)
-struct Library {
-#define VT_MEMBER(name) decltype(&vtdge_##name) name = nullptr;
-    VT_FUNCTIONS(VT_MEMBER)
-#undef VT_MEMBER
-};
-Library lib;
-PyObject *error_type = nullptr;                 // vtpack_amd._lib.VtdgeError
-
-struct Failure : std::runtime_error {
-    using std::runtime_error::runtime_error;
-};
-void must(int rc, const char *what)
-{
-    if (rc != VTDGE_OK) throw Failure(std::string(what) + " failed (" + std::to_string(rc) + "): " + lib.last_error());
-}
-
-int code_of(const Tensor &t) { return t.scalar_type() == at::kFloat ? VTDGE_F32 : VTDGE_BF16; }
-// from one row to the next; one row alone has no distance
-int64_t pitch_of(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
-void *at_of(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
-void *stream_of(const Tensor &t) { return (void *)c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-Tensor fresh(const Tensor &like, at::IntArrayRef sizes, at::ScalarType type) { return at::empty(sizes, like.options().dtype(type).requires_grad(false)); }
-
-// A workspace's bytes by the sizes it is for (working them out looks through many cuts of a sum).
-template <size_t N, class F> int64_t bytes_of(const std::array<int64_t, N> &key, F ask)
-{
-    static std::mutex lock;
-    static std::map<std::array<int64_t, N>, int64_t> known;
-    std::lock_guard<std::mutex> hold(lock);
-    const auto it = known.find(key);
-    if (it != known.end()) return it->second;
-    const int64_t bytes = ask();
-    if (bytes < 0) throw Failure(lib.last_error());
-    if (known.size() >= 1024) known.clear();
-    return known[key] = bytes;
-}
+using namespace vtdge_training;
 
 // ------------------------------------------------------------------------------------------------ cross entropy
 enum Reduction { NONE, MEAN, SUM };
@@ -145,27 +79,7 @@ std::array<Tensor, 3> cross_entropy_backward(const Tensor &x, const Tensor &w, c
     return out;
 }
 
-// ------------------------------------------------------------------------------------------------ forms of operands
-bool rows_of_any_place(const Tensor &t)
-{
-    return t.defined() && t.dim() == 2 && t.numel() > 0 && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16) &&
-           t.layout() == at::kStrided && (t.is_contiguous() || (t.stride(1) == 1 && t.stride(0) >= t.size(1)));
-}
-bool plain_rows(const Tensor &t) { return t.defined() && t.is_cuda() && rows_of_any_place(t); }
-bool plain_beside(const Tensor &t, const Tensor &x, at::ScalarType type)
-{
-    return t.defined() && t.device() == x.device() && t.scalar_type() == type && t.layout() == at::kStrided && t.is_contiguous();
-}
-
-// Operands that are taken as they are: one that does not fit is named before anything is launched, the place of all of them last.
-struct Operands {
-    const char *name;
-    void need(bool fits, const char *what) const
-    {
-        if (!fits) throw std::runtime_error(std::string(name) + ": " + what);
-    }
-    void on_gpu(const Tensor &x) const { need(x.is_cuda(), "operands have to be on a GPU"); }
-
+struct Operands : OperandChecks {
     void loss(const Tensor &x, const Tensor &w, const Tensor &b, const Tensor &t, double smoothing, int64_t reduction) const
     {
         need(rows_of_any_place(x), "x has to be [rows, width] of float32 or bfloat16 with dense rows");
@@ -199,28 +113,6 @@ struct Operands {
     }
 };
 
-void no_second_order(const char *name)
-{
-    if (at::GradMode::is_enabled()) throw std::runtime_error(std::string(name) + ": gradients of the gradients are not supported");
-}
-
-void no_forward_mode(const char *name, std::initializer_list<const Tensor *> operands)
-{
-    for (const Tensor *t : operands)
-        if (t->defined() && t->_fw_grad(0).defined()) throw std::runtime_error(std::string(name) + ": forward-mode derivatives are not supported");
-}
-
-// A trace would record the allocation of the results and not what fills them.
-void no_tracing(const char *name)
-{
-    using Key = c10::impl::TorchDispatchModeKey;
-    using Modes = c10::impl::TorchDispatchModeTLS;
-    bool traced = torch::jit::tracer::isTracing();
-    if (Modes::any_modes_set())
-        for (const Key key : {Key::FAKE, Key::PROXY, Key::FUNCTIONAL}) traced = traced || Modes::get_mode(key).has_value();
-    if (traced) throw std::runtime_error(std::string(name) + " cannot be traced");
-}
-
 // The backward node of a loss, with what it reads as members.
 struct LinearCrossEntropyBackward : torch::autograd::Node {
     SavedVariable x, w, bias, target, stats, laid_out;      // (the last two for hooks on saved tensors to see: up to 320 MB)
@@ -236,7 +128,7 @@ struct LinearCrossEntropyBackward : torch::autograd::Node {
         // the same for every row, as a sum over the losses leaves it: one value
         if (grad.dim() == 1) grad = grad.stride(0) == 0 ? grad.select(0, 0) : grad.contiguous();
         // (hooks on saved tensors may have brought others)
-        const Operands check{"linear_cross_entropy"};
+        const Operands check{{"linear_cross_entropy"}};
         check.loss(x_, w_, b_, t_, smoothing, reduction);
         check.loss_gradients(x_, w_, s_, l_, grad, reduction);
         check.on_gpu(x_);
@@ -305,7 +197,7 @@ struct GateBalanceBackward : torch::autograd::Node {
         std::lock_guard<std::mutex> hold(mutex_);
         const Tensor gate_ = gate.unpack(), mask_ = mask.unpack(), share_ = share.unpack();
         if (!grads[0].defined()) return {Tensor()};
-        const Operands check{"gate_balance"};
+        const Operands check{{"gate_balance"}};
         check.gate(gate_, mask_);
         check.gate_gradients(gate_, share_, grads[0]);
         check.on_gpu(gate_);
@@ -434,55 +326,6 @@ bool ready(Batch &b, PyObject *params, PyObject *state)
 }
 
 // ------------------------------------------------------------------------------------------------ for Python
-struct NoGil {
-    PyThreadState *state = PyEval_SaveThread();
-    ~NoGil() { PyEval_RestoreThread(state); }
-};
-Tensor tensor(PyObject *o)
-{
-    if (o == Py_None) return Tensor();
-    if (!THPVariable_Check(o)) throw std::runtime_error("expected a tensor or None");
-    return THPVariable_Unpack(o);
-}
-int64_t whole(PyObject *o)
-{
-    const long long v = PyLong_AsLongLong(o);
-    if (v == -1 && PyErr_Occurred()) throw python_error();
-    return v;
-}
-double real(PyObject *o)
-{
-    const double v = PyFloat_AsDouble(o);
-    if (v == -1 && PyErr_Occurred()) throw python_error();
-    return v;
-}
-PyObject *wrap(const Tensor &t)
-{
-    if (!t.defined()) Py_RETURN_NONE;
-    return THPVariable_Wrap(t);
-}
-PyObject *tuple(std::initializer_list<Tensor> ts)
-{
-    PyObject *out = PyTuple_New((Py_ssize_t)ts.size());
-    Py_ssize_t i = 0;
-    for (const Tensor &t : ts) PyTuple_SET_ITEM(out, i++, wrap(t));
-    return out;
-}
-
-// f(arguments) with `count` of them, what it throws as a Python exception
-template <class F> PyObject *call(PyObject *const *args, Py_ssize_t given, Py_ssize_t count, F f)
-{
-    HANDLE_TH_ERRORS
-    try {
-        if (given != count) throw std::runtime_error("expected " + std::to_string(count) + " arguments, got " + std::to_string(given));
-        return f();
-    } catch (const Failure &e) {
-        PyErr_SetString(error_type, e.what());
-        return nullptr;
-    }
-    END_HANDLE_TH_ERRORS
-}
-
 PyObject *py_bind(PyObject *, PyObject *const *args, Py_ssize_t n)
 {
     return call(args, n, 2, [&]() -> PyObject * {
@@ -527,12 +370,6 @@ PyObject *py_linear_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
         return wrap(loss);
     });
 }
-// a tensor, or None where that may be
-Tensor operand(const Operands &check, PyObject *o, const char *what)
-{
-    check.need(o == Py_None || THPVariable_Check(o), what);
-    return tensor(o);
-}
 std::array<Tensor, 4> of_loss(const Operands &check, PyObject *const *a, double smoothing, int64_t reduction)
 {
     const std::array<Tensor, 4> t = {operand(check, a[0], "x has to be a tensor"), operand(check, a[1], "weight has to be a tensor"),
@@ -543,7 +380,7 @@ std::array<Tensor, 4> of_loss(const Operands &check, PyObject *const *a, double 
 PyObject *py_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 7, [&] {
-        const Operands check{"cross_entropy"};
+        const Operands check{{"cross_entropy"}};
         const int64_t ignore = whole(a[4]), reduction = whole(a[6]);
         const double smoothing = real(a[5]);
         const auto [x, w, b, t] = of_loss(check, a, smoothing, reduction);
@@ -559,7 +396,7 @@ PyObject *py_cross_entropy(PyObject *, PyObject *const *a, Py_ssize_t n)
 PyObject *py_cross_entropy_backward(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 13, [&] {
-        const Operands check{"cross_entropy_backward"};
+        const Operands check{{"cross_entropy_backward"}};
         const int64_t ignore = whole(a[7]), reduction = whole(a[9]);
         const double smoothing = real(a[8]);
         const std::array<bool, 3> needs = {whole(a[10]) != 0, whole(a[11]) != 0, whole(a[12]) != 0};
@@ -602,7 +439,7 @@ PyObject *py_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
 PyObject *py_gate_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 4, [&] {
-        const Operands check{"gate_balance"};
+        const Operands check{{"gate_balance"}};
         const int64_t top_k = whole(a[3]);
         const Tensor gate = operand(check, a[0], "gate has to be a tensor"), indices = operand(check, a[1], "indices have to be a tensor or None"),
                      mask = operand(check, a[2], "mask has to be a tensor or None");
@@ -622,7 +459,7 @@ PyObject *py_gate_balance(PyObject *, PyObject *const *a, Py_ssize_t n)
 PyObject *py_gate_balance_backward(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     return call(a, n, 4, [&] {
-        const Operands check{"gate_balance_backward"};
+        const Operands check{{"gate_balance_backward"}};
         const Tensor gate = operand(check, a[0], "gate has to be a tensor"), mask = operand(check, a[1], "mask has to be a tensor or None"),
                      share = operand(check, a[2], "share has to be a tensor"), grad = operand(check, a[3], "grad has to be a tensor");
         check.gate(gate, mask);
@@ -747,10 +584,10 @@ PyObject *py_adamw_step(PyObject *, PyObject *const *a, Py_ssize_t n)
     });
 }
 
-#define VT_METHOD(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {VT_METHOD(bind), VT_METHOD(linear_cross_entropy), VT_METHOD(cross_entropy), VT_METHOD(cross_entropy_backward),
                          VT_METHOD(balance), VT_METHOD(gate_balance), VT_METHOD(gate_balance_backward), VT_METHOD(places), VT_METHOD(alike), VT_METHOD(adamw_batch),
-                         VT_METHOD(adamw_step), {nullptr, nullptr, 0, nullptr}};
+                         VT_METHOD(adamw_step), VT_METHOD(quantize_blocks), VT_METHOD(dequantize_blocks), VT_METHOD(linear_8bit),
+                         VT_METHOD(gelu_8bit), VT_METHOD(layer_norm_8bit), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_training", "The operators of a training step as torch calls them.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 

@@ -15,3 +15,10 @@ from .losses import (
     gate_balance,
     linear_cross_entropy,
 )
+from .eight_bit import (
+    Blocks,
+    gelu_8bit,
+    layer_norm_8bit,
+    linear_8bit,
+    quantize_blocks,
+)
