@@ -2,12 +2,117 @@
 // gradient of y rounded to bf16 (an error of half a step on each of many terms, as on any bf16 operand).
 #include "eight_bit.h"
 
+#ifndef VT_MIDDLE
+#define VT_MIDDLE 4
+#endif
 namespace vtdge {
 
 struct ForwardArgs {
-    Operand x, w;
+    Operand x, w;                                   // bf16; or blocks, two numbers an element
+    const unsigned char *x_scales, *w_scales; int scale_pitch;
     const void *bias; void *y; int64_t rows, out; int stages;
 };
+
+// ------------------------------------------------------------------------------------------------ the product of a tile of blocks
+// As multiply_tile, on the 8-bit matrix instructions, which take the scales themselves: a slab of 2 SLAB numbers lies in one block, and the
+// word with its scale byte comes with it, four bytes of a row (so that a load goes out for every slab alike and their count is known).
+template <class S> struct EightBit {
+    static constexpr int SCALE_CHUNKS = (S::ROWS + S::COLS) / 64, SCALE_LOADS = (SCALE_CHUNKS + S::WAVES - 1) / S::WAVES;
+    static constexpr int STAGE = S::STAGE + SCALE_LOADS * S::WAVES * 256, RING = S::SLOTS * STAGE, LDS = RING + S::COLS * 4;
+    static_assert(LDS <= 160 * 1024 && S::ROWS % 64 == 0 && S::COLS % 64 == 0 && S::PARTS == 1, "LDS");
+};
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+template <class S, class LA, class LB>
+__device__ __forceinline__ void multiply_blocks(const LA &a, const LB &b, const ForwardArgs &p, int64_t r0, int64_t c0, unsigned char *smem, f32x16 (&acc)[S::IM][S::JN])
+{
+    using E = EightBit<S>;
+    constexpr int IM = S::IM, JN = S::JN, SLOTS = S::SLOTS, A_BYTES = LA::STAGE;
+    constexpr int LOADS = LA::PIECES + LB::PIECES + E::SCALE_LOADS;
+    static_assert(LOADS * (SLOTS - 2) < 64, "the counter of outstanding loads");
+    const int lane = threadIdx.x & 63, lr = lane & 31, wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
+    // this wave's rows of scales
+    const void *scales[E::SCALE_LOADS];
+    uint32_t offset[E::SCALE_LOADS];
+#pragma unroll
+    for (int d = 0; d < E::SCALE_LOADS; d++) {
+        const int chunk = min(d * S::WAVES + wid, E::SCALE_CHUNKS - 1);
+        const bool of_x = chunk < S::ROWS / 64;
+        const int row = (of_x ? chunk : chunk - S::ROWS / 64) * 64 + lane;
+        const int64_t first = of_x ? r0 : c0, there = (of_x ? p.rows : p.out) - first;
+        scales[d] = uniform_ptr((of_x ? p.x_scales : p.w_scales) + first * p.scale_pitch);
+        offset[d] = (uint32_t)(row < there ? row : (int)there - 1) * (uint32_t)p.scale_pitch;
+    }
+    auto block_of = [](int t) { return S::SLAB == 64 ? t : t >> 1; };
+    auto issue = [&](int t, int slot) {
+        const uint32_t at = lds0 + slot * E::STAGE;
+        a.load(0, t, at);
+        b.load(0, t, at + A_BYTES);
+#pragma unroll
+        for (int d = 0; d < E::SCALE_LOADS; d++)
+            dma4(scales[d], offset[d] + (uint32_t)(block_of(t) & ~3), wave_uniform(at + S::STAGE + (d * S::WAVES + wid) * 256));
+    };
+    int in = 0, out = 0;
+#pragma unroll
+    for (int d = 0; d < SLOTS - 1; d++)
+        if (d < p.stages) {
+            issue(d, in);
+            in++;
+        }
+    for (int t = 0; t < p.stages; t++) {
+        const int behind = min(p.stages - 1 - t, SLOTS - 2);
+        static_for<SLOTS - 1>([&](auto X) {
+            constexpr int x = decltype(X)::value;
+            if (behind == x) wait_vmcnt<x * LOADS>();
+        });
+        lds_barrier();
+        const unsigned char *sa = smem + out * E::STAGE, *sb = sa + A_BYTES, *ss = sa + S::STAGE;
+        out = out == SLOTS - 1 ? 0 : out + 1;
+        constexpr int STEPS = S::SLAB / 32;
+        u32x4 fa[2][IM][2], fb[2][JN][2];
+        uint32_t qa[IM], qb[JN];
+        auto fetch = [&](int s) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int i = 0; i < IM; i++) fa[s & 1][i][h] = LA::fragment(sa, wm * IM + i, 2 * s + h);
+#pragma unroll
+                for (int j = 0; j < JN; j++) fb[s & 1][j][h] = LB::fragment(sb, wn * JN + j, 2 * s + h);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < IM; i++) qa[i] = *reinterpret_cast<const uint32_t *>(ss + ((wm * IM + i) * 32 + lr) * 4);
+#pragma unroll
+        for (int j = 0; j < JN; j++) qb[j] = *reinterpret_cast<const uint32_t *>(ss + (S::ROWS + (wn * JN + j) * 32 + lr) * 4);
+        fetch(0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (t + SLOTS - 1 < p.stages) {
+            issue(t + SLOTS - 1, in);
+            in = in == SLOTS - 1 ? 0 : in + 1;
+        }
+        const int shift = (block_of(t) & 3) * 8;
+#pragma unroll
+        for (int i = 0; i < IM; i++) qa[i] >>= shift;
+#pragma unroll
+        for (int j = 0; j < JN; j++) qb[j] >>= shift;
+        auto eight = [](const u32x4 (&f)[2]) {
+            return i32x8{(int)f[0].x, (int)f[0].y, (int)f[0].z, (int)f[0].w, (int)f[1].x, (int)f[1].y, (int)f[1].z, (int)f[1].w};
+        };
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (s + 1 < STEPS) fetch(s + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < IM; i++)
+#pragma unroll
+                for (int j = 0; j < JN; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(eight(fb[s & 1][j]), eight(fa[s & 1][i]), acc[i][j], 0, 0, 0, (int)qb[j], 0, (int)qa[i]);
+        }
+    }
+    lds_barrier();
+}
 
 // four values of a row from column c on
 template <typename T> __device__ __forceinline__ void put_row4(const ForwardArgs &p, int64_t r, int64_t c, const f32x4 &v)
@@ -24,39 +129,63 @@ template <typename T> __device__ __forceinline__ void put_row4(const ForwardArgs
     }
 }
 
+// fp32 results: bf16 operands, whose products are exact and whose sums are fp32 (bf16 sums of 128 normal numbers are 1e-8 off).  bf16
+// results: 8-bit operands, at twice the rate; those instructions cut the products of a group off some 13 bits below its largest (the same sums
+// are 1.4e-5 off, 2^-12 of sum |p| in the worst), below a hundredth of the result's rounding.
 template <class S, typename T, bool GELU> __global__ __launch_bounds__(S::THREADS, S::PER_SIMD) void linear_8bit_kernel(ForwardArgs p, int tm, int tn)
 {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr int IM = S::IM, JN = S::JN;
+    constexpr bool EIGHT = sizeof(T) == 2;
     int m, n;
     tile_at(place_of(blockIdx.x, tm * tn), tm, tn, m, n);
     const int64_t r0 = (int64_t)m * S::ROWS, c0 = (int64_t)n * S::COLS;
-    float *const bias = reinterpret_cast<float *>(smem + S::RING);
+    float *const bias = reinterpret_cast<float *>(smem + (EIGHT ? EightBit<S>::RING : S::RING));
     for (int c = threadIdx.x; c < S::COLS; c += S::THREADS)
         bias[c] = p.bias != nullptr && c0 + c < p.out ? Elem<T>::load(static_cast<const T *>(p.bias) + c0 + c) : 0.f;
     f32x16 acc[IM][JN] = {};
-    float none[IM];
     const Loader<true, S::ROWS, S::SLAB, S::WAVES> a(p.x, r0, p.rows, 0);
     const Loader<true, S::COLS, S::SLAB, S::WAVES> b(p.w, c0, p.out, 0);
-    multiply_tile<S, false>(a, b, 0, p.stages, smem, acc, false, none);
+    if constexpr (EIGHT) {
+        multiply_blocks<S>(a, b, p, r0, c0, smem, acc);
+    } else {
+        float none[IM];
+        multiply_tile<S, false>(a, b, 0, p.stages, smem, acc, false, none);
+    }
     const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
     const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
+    // whole rows of vectors: half-wave swaps leave a lane 8 consecutive columns
+    const bool whole = EIGHT && p.out % 8 == 0 && c0 + S::COLS <= p.out;
 #pragma unroll
     for (int i = 0; i < IM; i++) {
         const int64_t r = r0 + (wm * IM + i) * 32 + lr;
-        if (r >= p.rows) continue;
 #pragma unroll
-        for (int j = 0; j < JN; j++)
+        for (int j = 0; j < JN; j++) {
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                const int c = (wn * JN + j) * 32 + 8 * q + 4 * lg;
-                f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                v += *reinterpret_cast<const f32x4 *>(bias + c);
-                if constexpr (GELU)
+                const f32x4 add = *reinterpret_cast<const f32x4 *>(bias + (wn * JN + j) * 32 + 8 * q + 4 * lg);
 #pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = gelu_fn<T>(v[e]);
-                put_row4<T>(p, r, c0 + c, v);
+                for (int e = 0; e < 4; e++) {
+                    const float v = acc[i][j][4 * q + e] + add[e];
+                    acc[i][j][4 * q + e] = GELU ? gelu_fn<T>(v) : v;
+                }
             }
+            if (whole) {
+                bf16_t *const to = static_cast<bf16_t *>(p.y) + r * p.out + c0 + (wn * JN + j) * 32 + 8 * lg;
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    uint32_t o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[e] = pack_bf16x2(acc[i][j][8 * q + 2 * e], acc[i][j][8 * q + 2 * e + 1]);
+                    const auto s0 = __builtin_amdgcn_permlane32_swap(o[0], o[2], false, false), s1 = __builtin_amdgcn_permlane32_swap(o[1], o[3], false, false);
+                    if (r < p.rows) *reinterpret_cast<u32x4 *>(to + 16 * q) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+                }
+            } else if (r < p.rows) {
+#pragma unroll
+                for (int q = 0; q < 4; q++)
+                    put_row4<T>(p, r, c0 + (wn * JN + j) * 32 + 8 * q + 4 * lg, f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
+            }
+        }
     }
 }
 
@@ -87,12 +216,12 @@ static int64_t padded(int64_t n) { return ceil_div(n, SLAB) * SLAB; }
 struct ForwardPlan {
     int64_t x_at, w_at, bytes;
 };
-static ForwardPlan plan_forward(int64_t rows, int64_t out, int64_t width)
+static ForwardPlan plan_forward(int64_t rows, int64_t out, int64_t width, int dtype)
 {
     ForwardPlan p{};
     int64_t at = 0;
-    p.x_at = take(at, rows * padded(width) * 2);
-    p.w_at = take(at, out * padded(width) * 2);
+    p.x_at = take(at, dtype == VTDGE_F32 ? rows * padded(width) * 2 : blocks_bytes(rows, width));
+    p.w_at = take(at, dtype == VTDGE_F32 ? out * padded(width) * 2 : blocks_bytes(out, width));
     p.bytes = at;
     return p;
 }
@@ -134,9 +263,10 @@ template <class S, typename T, bool GELU> static int go_forward_as(const Forward
 {
     const int64_t tm = ceil_div(a.rows, S::ROWS), tn = ceil_div(a.out, S::COLS);
     auto kern = linear_8bit_kernel<S, T, GELU>;
-    VT_RESERVE_LDS(kern, S::LDS, "linear_8bit");
+    constexpr int LDS = sizeof(T) == 2 ? EightBit<S>::LDS : S::LDS;
+    VT_RESERVE_LDS(kern, LDS, "linear_8bit");
     note_kernel(reinterpret_cast<const void *>(kern));
-    kern<<<(unsigned)(tm * tn), S::THREADS, S::LDS, st>>>(a, (int)tm, (int)tn);
+    kern<<<(unsigned)(tm * tn), S::THREADS, LDS, st>>>(a, (int)tm, (int)tn);
     return check_launch("linear_8bit");
 }
 template <class S> static int go_forward(const ForwardArgs &a, int act, int dtype, hipStream_t st)
@@ -152,7 +282,7 @@ using namespace vtdge;
 extern "C" int64_t vtdge_linear_8bit_workspace(int64_t rows, int64_t out, int64_t width, int dtype)
 {
     if (check_linear("linear_8bit_workspace", rows, out, width, dtype) != VTDGE_OK) return -1;
-    return plan_forward(rows, out, width).bytes;
+    return plan_forward(rows, out, width, dtype).bytes;
 }
 
 extern "C" int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight, int64_t ldw, void *w_blocks, const void *bias, void *y, void *x_blocks,
@@ -164,34 +294,46 @@ extern "C" int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight,
     VT_REQUIRE((ldx >= width || rows == 1) && (weight == nullptr || ldw >= width || out == 1), VTDGE_ERR_ARG, "linear_8bit: rows of %lld, %lld and %lld apart",
                (long long)width, (long long)ldx, (long long)ldw);
     VT_REQUIRE(((uintptr_t)w_blocks & 127) == 0 && ((uintptr_t)x_blocks & 127) == 0, VTDGE_ERR_ARG, "linear_8bit: blocks off their boundary");
-    const ForwardPlan p = plan_forward(rows, out, width);
+    const ForwardPlan p = plan_forward(rows, out, width, dtype);
     VT_REQUIRE(workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG, "linear_8bit: workspace of %lld bytes, %lld needed",
                (long long)workspace_bytes, (long long)p.bytes);
     unsigned char *const ws = (unsigned char *)workspace;
     const hipStream_t st = (hipStream_t)stream;
-    bf16_t *const xb = (bf16_t *)(ws + p.x_at), *const wb = (bf16_t *)(ws + p.w_at);
     QuantizeArgs q{};
-    q.job[0] = quantize_job(x, ldx, rows, width, x_blocks, xb, padded(width));
-    if (weight != nullptr) q.job[1] = quantize_job(weight, ldw, out, width, w_blocks, wb, padded(width));
-    VT_STEP(launch_quantize(q, weight != nullptr ? 2 : 1, dtype, "linear_8bit", st));
-    if (weight == nullptr) {
-        DequantizeArgs d{};
-        d.job[0] = dequantize_job(w_blocks, out, width, wb, padded(width), padded(width));
-        VT_STEP(launch_dequantize(d, 1, VTDGE_BF16, "linear_8bit", st));
-    }
     ForwardArgs a{};
-    a.x = Operand{xb, padded(width), 0}, a.w = Operand{wb, padded(width), 0};
     a.bias = bias, a.y = y, a.rows = rows, a.out = out;
+    int64_t slabs;                                  // of 64 elements
+    if (dtype == VTDGE_F32) {
+        bf16_t *const xb = (bf16_t *)(ws + p.x_at), *const wb = (bf16_t *)(ws + p.w_at);
+        q.job[0] = quantize_job(x, ldx, rows, width, x_blocks, xb, padded(width));
+        if (weight != nullptr) q.job[1] = quantize_job(weight, ldw, out, width, w_blocks, wb, padded(width));
+        VT_STEP(launch_quantize(q, weight != nullptr ? 2 : 1, dtype, "linear_8bit", st));
+        if (weight == nullptr) {
+            DequantizeArgs d{};
+            d.job[0] = dequantize_job(w_blocks, out, width, wb, padded(width), padded(width));
+            VT_STEP(launch_dequantize(d, 1, VTDGE_BF16, "linear_8bit", st));
+        }
+        a.x = Operand{xb, padded(width), 0}, a.w = Operand{wb, padded(width), 0};
+        slabs = padded(width) / SLAB;
+    } else {
+        void *const xq = x_blocks != nullptr ? x_blocks : ws + p.x_at, *const wq = w_blocks != nullptr ? w_blocks : ws + p.w_at;
+        q.job[0] = quantize_job(x, ldx, rows, width, xq, nullptr, 0);
+        if (weight != nullptr) q.job[1] = quantize_job(weight, ldw, out, width, wq, nullptr, 0);
+        VT_STEP(launch_quantize(q, weight != nullptr ? 2 : 1, dtype, "linear_8bit", st));
+        a.x = Operand{(const bf16_t *)xq, value_pitch(width) / 2, 0}, a.w = Operand{(const bf16_t *)wq, value_pitch(width) / 2, 0};
+        a.x_scales = scales_of(xq, rows, width), a.w_scales = scales_of(wq, out, width), a.scale_pitch = (int)scale_pitch(width);
+        slabs = value_pitch(width) / BLOCK;
+    }
     const int64_t cu = compute_units();
     if (ceil_div(rows, 128) * ceil_div(out, 256) < cu) {
-        a.stages = (int)(padded(width) / ForwardSmall::SLAB);
+        a.stages = (int)(slabs * SLAB / ForwardSmall::SLAB);
         return go_forward<ForwardSmall>(a, act, dtype, st);
     }
-    if (ceil_div(rows, 256) * ceil_div(out, 256) < 4 * cu) {
-        a.stages = (int)(padded(width) / ForwardMiddle::SLAB);
+    if (ceil_div(rows, 256) * ceil_div(out, 256) < VT_MIDDLE * cu) {
+        a.stages = (int)(slabs * SLAB / ForwardMiddle::SLAB);
         return go_forward<ForwardMiddle>(a, act, dtype, st);
     }
-    a.stages = (int)(padded(width) / ForwardLarge::SLAB);
+    a.stages = (int)(slabs * SLAB / ForwardLarge::SLAB);
     return go_forward<ForwardLarge>(a, act, dtype, st);
 }
 
