@@ -2,33 +2,33 @@
 // gradient of y rounded to bf16 (an error of half a step on each of many terms, as on any bf16 operand).
 #include "eight_bit.h"
 
-#ifndef VT_MIDDLE
-#define VT_MIDDLE 4
-#endif
 namespace vtdge {
 
 struct ForwardArgs {
     Operand x, w;                                   // bf16; or blocks, two numbers an element
     const unsigned char *x_scales, *w_scales; int scale_pitch;
     const void *bias; void *y; int64_t rows, out; int stages;
+    bool stream_y;                                  // the result past the caches
 };
 
 // ------------------------------------------------------------------------------------------------ the product of a tile of blocks
-// As multiply_tile, on the 8-bit matrix instructions, which take the scales themselves: a slab of 2 SLAB numbers lies in one block, and the
-// word with its scale byte comes with it, four bytes of a row (so that a load goes out for every slab alike and their count is known).
+// As multiply_tile, on the 8-bit matrix instructions, which take the scales themselves: a slab of 2 SLAB numbers lies in one block.  Scale
+// bytes come four blocks at a time, the word of each row, into one of two places of their own (65536 x 1024 x 4096: 15 us less than a
+// word with every slab).
 template <class S> struct EightBit {
     static constexpr int SCALE_CHUNKS = (S::ROWS + S::COLS) / 64, SCALE_LOADS = (SCALE_CHUNKS + S::WAVES - 1) / S::WAVES;
-    static constexpr int STAGE = S::STAGE + SCALE_LOADS * S::WAVES * 256, RING = S::SLOTS * STAGE, LDS = RING + S::COLS * 4;
+    static constexpr int WORDS = SCALE_LOADS * S::WAVES * 256, SCALES = S::RING, RING = SCALES + 2 * WORDS, LDS = RING + S::COLS * 4;
     static_assert(LDS <= 160 * 1024 && S::ROWS % 64 == 0 && S::COLS % 64 == 0 && S::PARTS == 1, "LDS");
 };
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-template <class S, class LA, class LB>
-__device__ __forceinline__ void multiply_blocks(const LA &a, const LB &b, const ForwardArgs &p, int64_t r0, int64_t c0, unsigned char *smem, f32x16 (&acc)[S::IM][S::JN])
+template <class S, class LA, class LB, class F>
+__device__ __forceinline__ void multiply_blocks(const LA &a, const LB &b, const ForwardArgs &p, int64_t r0, int64_t c0, unsigned char *smem, f32x16 (&acc)[S::IM][S::JN], F &&meanwhile)
 {
     using E = EightBit<S>;
     constexpr int IM = S::IM, JN = S::JN, SLOTS = S::SLOTS, A_BYTES = LA::STAGE;
-    constexpr int LOADS = LA::PIECES + LB::PIECES + E::SCALE_LOADS;
+    constexpr int LOADS = LA::PIECES + LB::PIECES;          // and now and then those of scales: what waits for fewer waits for enough
+    constexpr int GROUP = S::SLAB == 64 ? 4 : 8;            // slabs of four blocks
     static_assert(LOADS * (SLOTS - 2) < 64, "the counter of outstanding loads");
     const int lane = threadIdx.x & 63, lr = lane & 31, wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
@@ -44,15 +44,17 @@ __device__ __forceinline__ void multiply_blocks(const LA &a, const LB &b, const 
         scales[d] = uniform_ptr((of_x ? p.x_scales : p.w_scales) + first * p.scale_pitch);
         offset[d] = (uint32_t)(row < there ? row : (int)there - 1) * (uint32_t)p.scale_pitch;
     }
-    auto block_of = [](int t) { return S::SLAB == 64 ? t : t >> 1; };
     auto issue = [&](int t, int slot) {
-        const uint32_t at = lds0 + slot * E::STAGE;
+        const uint32_t at = lds0 + slot * S::STAGE;
+        if (t % GROUP == 0) {
+#pragma unroll
+            for (int d = 0; d < E::SCALE_LOADS; d++)
+                dma4(scales[d], offset[d] + (uint32_t)(t / GROUP) * 4, wave_uniform(lds0 + E::SCALES + (t / GROUP & 1) * E::WORDS + (d * S::WAVES + wid) * 256));
+        }
         a.load(0, t, at);
         b.load(0, t, at + A_BYTES);
-#pragma unroll
-        for (int d = 0; d < E::SCALE_LOADS; d++)
-            dma4(scales[d], offset[d] + (uint32_t)(block_of(t) & ~3), wave_uniform(at + S::STAGE + (d * S::WAVES + wid) * 256));
     };
+    uint32_t words_a[IM], words_b[JN];
     int in = 0, out = 0;
 #pragma unroll
     for (int d = 0; d < SLOTS - 1; d++)
@@ -60,6 +62,7 @@ __device__ __forceinline__ void multiply_blocks(const LA &a, const LB &b, const 
             issue(d, in);
             in++;
         }
+    meanwhile();
     for (int t = 0; t < p.stages; t++) {
         const int behind = min(p.stages - 1 - t, SLOTS - 2);
         static_for<SLOTS - 1>([&](auto X) {
@@ -67,11 +70,10 @@ __device__ __forceinline__ void multiply_blocks(const LA &a, const LB &b, const 
             if (behind == x) wait_vmcnt<x * LOADS>();
         });
         lds_barrier();
-        const unsigned char *sa = smem + out * E::STAGE, *sb = sa + A_BYTES, *ss = sa + S::STAGE;
+        const unsigned char *sa = smem + out * S::STAGE, *sb = sa + A_BYTES;
         out = out == SLOTS - 1 ? 0 : out + 1;
         constexpr int STEPS = S::SLAB / 32;
         u32x4 fa[2][IM][2], fb[2][JN][2];
-        uint32_t qa[IM], qb[JN];
         auto fetch = [&](int s) {
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -81,21 +83,25 @@ __device__ __forceinline__ void multiply_blocks(const LA &a, const LB &b, const 
                 for (int j = 0; j < JN; j++) fb[s & 1][j][h] = LB::fragment(sb, wn * JN + j, 2 * s + h);
             }
         };
+        if (t % GROUP == 0) {
+            const unsigned char *ss = smem + E::SCALES + (t / GROUP & 1) * E::WORDS;
 #pragma unroll
-        for (int i = 0; i < IM; i++) qa[i] = *reinterpret_cast<const uint32_t *>(ss + ((wm * IM + i) * 32 + lr) * 4);
+            for (int i = 0; i < IM; i++) words_a[i] = *reinterpret_cast<const uint32_t *>(ss + ((wm * IM + i) * 32 + lr) * 4);
 #pragma unroll
-        for (int j = 0; j < JN; j++) qb[j] = *reinterpret_cast<const uint32_t *>(ss + (S::ROWS + (wn * JN + j) * 32 + lr) * 4);
+            for (int j = 0; j < JN; j++) words_b[j] = *reinterpret_cast<const uint32_t *>(ss + (S::ROWS + (wn * JN + j) * 32 + lr) * 4);
+        }
         fetch(0);
         __builtin_amdgcn_sched_barrier(0);
         if (t + SLOTS - 1 < p.stages) {
             issue(t + SLOTS - 1, in);
             in = in == SLOTS - 1 ? 0 : in + 1;
         }
-        const int shift = (block_of(t) & 3) * 8;
+        const int shift = t % GROUP / (GROUP / 4) * 8;
+        uint32_t qa[IM], qb[JN];
 #pragma unroll
-        for (int i = 0; i < IM; i++) qa[i] >>= shift;
+        for (int i = 0; i < IM; i++) qa[i] = words_a[i] >> shift;
 #pragma unroll
-        for (int j = 0; j < JN; j++) qb[j] >>= shift;
+        for (int j = 0; j < JN; j++) qb[j] = words_b[j] >> shift;
         auto eight = [](const u32x4 (&f)[2]) {
             return i32x8{(int)f[0].x, (int)f[0].y, (int)f[0].z, (int)f[0].w, (int)f[1].x, (int)f[1].y, (int)f[1].z, (int)f[1].w};
         };
@@ -114,21 +120,6 @@ __device__ __forceinline__ void multiply_blocks(const LA &a, const LB &b, const 
     lds_barrier();
 }
 
-// four values of a row from column c on
-template <typename T> __device__ __forceinline__ void put_row4(const ForwardArgs &p, int64_t r, int64_t c, const f32x4 &v)
-{
-    T *const to = static_cast<T *>(p.y) + r * p.out + c;
-    const int left = (int)(p.out - c);
-    if (left >= 4 && p.out % 4 == 0) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4 *>(to) = v;
-        else *reinterpret_cast<u32x2 *>(to) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-            if (e < left) Elem<T>::store(to + e, v[e]);
-    }
-}
-
 // fp32 results: bf16 operands, whose products are exact and whose sums are fp32 (bf16 sums of 128 normal numbers are 1e-8 off).  bf16
 // results: 8-bit operands, at twice the rate; those instructions cut the products of a group off some 13 bits below its largest (the same sums
 // are 1.4e-5 off, 2^-12 of sum |p| in the worst), below a hundredth of the result's rounding.
@@ -141,52 +132,96 @@ template <class S, typename T, bool GELU> __global__ __launch_bounds__(S::THREAD
     tile_at(place_of(blockIdx.x, tm * tn), tm, tn, m, n);
     const int64_t r0 = (int64_t)m * S::ROWS, c0 = (int64_t)n * S::COLS;
     float *const bias = reinterpret_cast<float *>(smem + (EIGHT ? EightBit<S>::RING : S::RING));
-    for (int c = threadIdx.x; c < S::COLS; c += S::THREADS)
-        bias[c] = p.bias != nullptr && c0 + c < p.out ? Elem<T>::load(static_cast<const T *>(p.bias) + c0 + c) : 0.f;
+    // (behind the first direct loads: in front of them its way from memory would be waited for)
+    auto read_bias = [&] {
+        for (int c = threadIdx.x; c < S::COLS; c += S::THREADS)
+            bias[c] = p.bias != nullptr && c0 + c < p.out ? Elem<T>::load(static_cast<const T *>(p.bias) + c0 + c) : 0.f;
+    };
     f32x16 acc[IM][JN] = {};
     const Loader<true, S::ROWS, S::SLAB, S::WAVES> a(p.x, r0, p.rows, 0);
     const Loader<true, S::COLS, S::SLAB, S::WAVES> b(p.w, c0, p.out, 0);
     if constexpr (EIGHT) {
-        multiply_blocks<S>(a, b, p, r0, c0, smem, acc);
+        multiply_blocks<S>(a, b, p, r0, c0, smem, acc, read_bias);
     } else {
         float none[IM];
+        read_bias();
         multiply_tile<S, false>(a, b, 0, p.stages, smem, acc, false, none);
     }
     const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
     const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
-    // whole rows of vectors: half-wave swaps leave a lane 8 consecutive columns
-    const bool whole = EIGHT && p.out % 8 == 0 && c0 + S::COLS <= p.out;
+    // To memory by way of LDS, a wave 32 rows at a time, so that whole lines leave at once (bf16 65536 x 1024 x 4096 with GELU: 470 us in 32-byte
+    // pieces, 395 so, 375 also past the caches, where the result fills them anyway).
+    constexpr int JP = EIGHT || JN == 1 ? JN : JN / 2, ROW = JP * 32 * sizeof(T), PITCH = ROW + 16, VEC = Elem<T>::VEC, LANES = ROW / 16;
+    static_assert(S::WAVES * 32 * PITCH <= (EIGHT ? EightBit<S>::RING : S::RING), "LDS");
+    unsigned char *const mine = smem + wid * 32 * PITCH;
+    // WHOLE: no row or column of the tile is behind the last, vectors of the result lie on their boundaries.  In one run without branches: with
+    // them the stores of a piece wait for one another (35 us of the 340 above).
+    auto leave = [&](auto WHOLE, auto STREAM) {
+        constexpr bool whole = decltype(WHOLE)::value, stream = decltype(STREAM)::value;
 #pragma unroll
-    for (int i = 0; i < IM; i++) {
-        const int64_t r = r0 + (wm * IM + i) * 32 + lr;
+        for (int i = 0; i < IM; i++) {
 #pragma unroll
-        for (int j = 0; j < JN; j++) {
+            for (int j0 = 0; j0 < JN; j0 += JP) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                const f32x4 add = *reinterpret_cast<const f32x4 *>(bias + (wn * JN + j) * 32 + 8 * q + 4 * lg);
+                for (int j = j0; j < j0 + JP; j++) {
+                    f32x4 v[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float v = acc[i][j][4 * q + e] + add[e];
-                    acc[i][j][4 * q + e] = GELU ? gelu_fn<T>(v) : v;
+                    for (int q = 0; q < 4; q++) {
+                        const f32x4 add = *reinterpret_cast<const f32x4 *>(bias + (wn * JN + j) * 32 + 8 * q + 4 * lg);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            v[q][e] = acc[i][j][4 * q + e] + add[e];
+                            if (GELU) v[q][e] = gelu_fn<T>(v[q][e]);
+                        }
+                    }
+                    unsigned char *const at = mine + lr * PITCH + (j - j0) * 32 * sizeof(T);
+                    if constexpr (EIGHT) {
+                        // half-wave swaps leave a lane 8 consecutive columns
+#pragma unroll
+                        for (int q = 0; q < 2; q++) {
+                            const uint32_t o[4] = {pack_bf16x2(v[2 * q][0], v[2 * q][1]), pack_bf16x2(v[2 * q][2], v[2 * q][3]),
+                                                   pack_bf16x2(v[2 * q + 1][0], v[2 * q + 1][1]), pack_bf16x2(v[2 * q + 1][2], v[2 * q + 1][3])};
+                            const auto s0 = __builtin_amdgcn_permlane32_swap(o[0], o[2], false, false), s1 = __builtin_amdgcn_permlane32_swap(o[1], o[3], false, false);
+                            *reinterpret_cast<u32x4 *>(at + 32 * q + 16 * lg) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) *reinterpret_cast<f32x4 *>(at + 32 * q + 16 * lg) = v[q];
+                    }
                 }
-            }
-            if (whole) {
-                bf16_t *const to = static_cast<bf16_t *>(p.y) + r * p.out + c0 + (wn * JN + j) * 32 + 8 * lg;
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // (the wave's own)
+                const int64_t first = r0 + (wm * IM + i) * 32, column = c0 + (wn * JN + j0) * 32;
+                T *const to = static_cast<T *>(p.y) + first * p.out + column;
+                if constexpr (whole) {
+                    constexpr int TIMES = 32 * LANES / 64;
+                    const int row = lane / LANES, c = lane % LANES;
+                    T *const from = to + (int64_t)row * p.out + c * VEC;
 #pragma unroll
-                for (int q = 0; q < 2; q++) {
-                    uint32_t o[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) o[e] = pack_bf16x2(acc[i][j][8 * q + 2 * e], acc[i][j][8 * q + 2 * e + 1]);
-                    const auto s0 = __builtin_amdgcn_permlane32_swap(o[0], o[2], false, false), s1 = __builtin_amdgcn_permlane32_swap(o[1], o[3], false, false);
-                    if (r < p.rows) *reinterpret_cast<u32x4 *>(to + 16 * q) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+                    for (int k = 0; k < TIMES; k++) {
+                        const u32x4 o = *reinterpret_cast<const u32x4 *>(mine + (row + k * (64 / LANES)) * PITCH + c * 16);
+                        u32x4 *const at = reinterpret_cast<u32x4 *>(from + (int64_t)k * (64 / LANES) * p.out);
+                        if constexpr (stream) __builtin_nontemporal_store(o, at);
+                        else *at = o;
+                    }
+                } else {
+                    const int live = (int)(p.rows - first < 32 ? p.rows - first : 32), left = (int)(p.out - column < JP * 32 ? p.out - column : JP * 32);
+                    if (p.out % VEC == 0) {
+                        for (int k = lane; k < live * LANES; k += 64) {
+                            const int row = k / LANES, c = k % LANES;
+                            if (c * VEC < left) *reinterpret_cast<u32x4 *>(to + (int64_t)row * p.out + c * VEC) = *reinterpret_cast<const u32x4 *>(mine + row * PITCH + c * 16);
+                        }
+                    } else {
+                        for (int row = 0; row < live; row++)
+                            for (int c = lane; c < left; c += 64) to[(int64_t)row * p.out + c] = *reinterpret_cast<const T *>(mine + row * PITCH + c * sizeof(T));
+                    }
                 }
-            } else if (r < p.rows) {
-#pragma unroll
-                for (int q = 0; q < 4; q++)
-                    put_row4<T>(p, r, c0 + (wn * JN + j) * 32 + 8 * q + 4 * lg, f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
         }
-    }
+    };
+    if (p.out % VEC != 0 || r0 + S::ROWS > p.rows || c0 + S::COLS > p.out) leave(std::false_type{}, std::false_type{});
+    else if (p.stream_y) leave(std::true_type{}, std::true_type{});
+    else leave(std::true_type{}, std::false_type{});
 }
 
 // Rows of g as the products read them: bf16, filled up with zeros to whole slabs.
@@ -302,6 +337,7 @@ extern "C" int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight,
     QuantizeArgs q{};
     ForwardArgs a{};
     a.bias = bias, a.y = y, a.rows = rows, a.out = out;
+    a.stream_y = rows * out * (dtype == VTDGE_F32 ? 4 : 2) >= (256ll << 20);      // the last cache
     int64_t slabs;                                  // of 64 elements
     if (dtype == VTDGE_F32) {
         bf16_t *const xb = (bf16_t *)(ws + p.x_at), *const wb = (bf16_t *)(ws + p.w_at);
@@ -329,7 +365,7 @@ extern "C" int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight,
         a.stages = (int)(slabs * SLAB / ForwardSmall::SLAB);
         return go_forward<ForwardSmall>(a, act, dtype, st);
     }
-    if (ceil_div(rows, 256) * ceil_div(out, 256) < VT_MIDDLE * cu) {
+    if (ceil_div(rows, 256) * ceil_div(out, 256) < 4 * cu) {
         a.stages = (int)(slabs * SLAB / ForwardMiddle::SLAB);
         return go_forward<ForwardMiddle>(a, act, dtype, st);
     }
