@@ -94,6 +94,7 @@ Tensor linear_8bit(const Tensor &x, const Tensor &weight, Tensor w_blocks, int64
     if (trains && act != VTDGE_ACT_NONE) throw std::runtime_error("linear_8bit: an activation with gradients is an operator of its own, as gelu_8bit");
     const c10::DeviceGuard guard(x.device());
     const int64_t rows = rows_in(x), width = last_of(x);
+    if (trains && rows > VTDGE_MAX_ROWS_8BIT) throw std::runtime_error("linear_8bit: gradients of " + std::to_string(rows) + " rows, up to " + std::to_string(VTDGE_MAX_ROWS_8BIT) + " are supported");
     const Tensor y = fresh(x, with_last(x, out), x.scalar_type());
     Tensor x_blocks;
     if (rows > 0) {

@@ -19,7 +19,9 @@ struct GradPair {
     int first_dw;                                           // workgroups before are dx's
     const float *scale, *scale2; int f32;                  // results in fp32
     bool f32_parts;                                         // operands in three bf16 parts
-    bool ends;                                              // (not in parts) d has no rows of zeros behind its last: dW's sum ends there
+    // (not in parts) d has no rows of zeros behind its last, where dW's sum ends; the second operands lie with the summed dimension along
+    // their rows, filled up with zeros to whole slabs
+    bool ends;
 };
 
 // out = scale * (sum over the parts), for up to three results in one launch

@@ -52,7 +52,7 @@ template <class S, bool A_ALONG, bool ENDS> __device__ __forceinline__ void grad
     f32x16 acc[IM][JN] = {};
     float sums[IM] = {};
     const Loader<A_ALONG, S::ROWS, S::SLAB, S::WAVES> a(p.a, r0, A_ALONG ? p.rows : p.sum_a, p.span_a);
-    const Loader<false, S::COLS, S::SLAB, S::WAVES> b(p.b, c0, p.sum_b, p.span_b);
+    const Loader<ENDS, S::COLS, S::SLAB, S::WAVES> b(p.b, c0, ENDS ? p.cols : p.sum_b, p.span_b);
     const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
     const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
     const bool with_sums = !A_ALONG && n == 0 && wn == 0 && (p.sums_part != nullptr || p.sums != nullptr);

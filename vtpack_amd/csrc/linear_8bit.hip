@@ -234,6 +234,49 @@ template <typename T, bool WIDE> __global__ __launch_bounds__(256) void pack_gra
     *reinterpret_cast<u32x4 *>(to + ((int64_t)row * per_row * 8 + c)) = Elem<bf16_t>::pack(f);
 }
 
+// Blocks [rows, n] as bf16 [n, pitch], zeros behind the rows: what both gradients multiply lies along their sums then, and is read from LDS
+// in 16 bytes a lane (transposed by the LDS reads, 32768 x 1024 x 4096: 605 us in place of VT_GRAD_US).
+struct ExpandJob {
+    const unsigned char *values, *scales; uint32_t rows, down; int64_t value_pitch; int scale_pitch, n; bf16_t *to; int64_t pitch;     // down: tiles of 64 rows
+};
+struct ExpandArgs {
+    ExpandJob job[2];
+    uint32_t first;
+};
+__global__ __launch_bounds__(256) void expand_kernel(ExpandArgs p)
+{
+    constexpr int PITCH = 36;                       // words of a column, two rows each
+    __shared__ __attribute__((aligned(16))) uint32_t tile[BLOCK * PITCH];
+    const bool second = blockIdx.x >= p.first;
+    const ExpandJob &job = p.job[second ? 1 : 0];
+    const uint32_t id = blockIdx.x - (second ? p.first : 0), block = id / job.down, r0 = (id - block * job.down) * 64;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int pair = (threadIdx.x >> 4) + 16 * k, c = (threadIdx.x & 15) * 8;
+        float f[2][8];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const uint32_t r = r0 + 2 * pair + h;
+            if (r < job.rows) {
+                stands_for8(*reinterpret_cast<const u32x2 *>(job.values + (int64_t)r * job.value_pitch + block * BLOCK + c), job.scales[(int64_t)r * job.scale_pitch + block], f[h]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[h][e] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) tile[(c + e) * PITCH + pair] = pack_bf16x2(f[0][e], f[1][e]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int at = threadIdx.x + 256 * k, column = at >> 3, piece = at & 7;
+        if ((int)(block * BLOCK) + column < job.n)
+            *reinterpret_cast<u32x4 *>(job.to + (int64_t)(block * BLOCK + column) * job.pitch + r0 + piece * 8) =
+                *reinterpret_cast<const u32x4 *>(tile + column * PITCH + piece * 4);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ on the host
 using ForwardLarge = Shape<2, 4, 4, 2, 64, 2, 1>;
 using ForwardMiddle = Shape<2, 4, 2, 2, 32, 3, 1>;
@@ -274,8 +317,8 @@ static BackwardPlan plan_backward(int64_t rows, int64_t out, int64_t width, bool
     plan_gradients(p, rows, out, (int)width, false);
     int64_t at = 0;
     p.g_at = take(at, lies ? 0 : rows * padded(out) * 2);
-    p.x_at = take(at, rows * padded(width) * 2);
-    p.w_at = take(at, out * padded(width) * 2);
+    p.x_at = take(at, width * padded(rows) * 2);
+    p.w_at = take(at, width * padded(out) * 2);
     p.dx_at = take(at, part_of(rows * width) * 4 * p.dx_splits);
     p.dw_at = take(at, part_of(out * width) * 4 * p.dw_splits);
     p.db_at = take(at, part_of(out) * 4 * p.dw_splits);
@@ -386,6 +429,7 @@ extern "C" int vtdge_linear_8bit_backward(const void *grad, int64_t ldg, const v
     VT_STEP(check_linear("linear_8bit_backward", rows, out, width, dtype));
     if (dx == nullptr && dweight == nullptr && dbias == nullptr) return VTDGE_OK;
     VT_REQUIRE(grad && workspace && (dx == nullptr || w_blocks) && (dweight == nullptr || x_blocks), VTDGE_ERR_ARG, "linear_8bit_backward: NULL operand");
+    VT_REQUIRE(rows <= VTDGE_MAX_ROWS_8BIT, VTDGE_ERR_UNSUPPORTED, "linear_8bit_backward: %lld rows, %d at most", (long long)rows, VTDGE_MAX_ROWS_8BIT);
     VT_REQUIRE(ldg >= out || rows == 1, VTDGE_ERR_ARG, "linear_8bit_backward: rows of %lld, %lld apart", (long long)out, (long long)ldg);
     VT_REQUIRE(((uintptr_t)w_blocks & 127) == 0 && ((uintptr_t)x_blocks & 127) == 0, VTDGE_ERR_ARG, "linear_8bit_backward: blocks off their boundary");
     const bool lies = gradient_lies(grad, rows > 1 ? ldg : 0, out, dtype);
@@ -410,24 +454,36 @@ extern "C" int vtdge_linear_8bit_backward(const void *grad, int64_t ldg, const v
         else VT_STEP(wide ? go(pack_gradient_kernel<bf16_t, true>, (const bf16_t *)grad) : go(pack_gradient_kernel<bf16_t, false>, (const bf16_t *)grad));
         g_op = Operand{to, padded(out), 0};
     }
-    DequantizeArgs d{};
+    ExpandArgs d{};
     int jobs = 0;
-    if (dx != nullptr) d.job[jobs++] = dequantize_job(w_blocks, out, width, wb, padded(width), padded(width));
-    if (dweight != nullptr) d.job[jobs++] = dequantize_job(x_blocks, rows, width, xb, padded(width), padded(width));
-    if (jobs > 0) VT_STEP(launch_dequantize(d, jobs, VTDGE_BF16, "linear_8bit_backward", st));
+    int64_t tiles = 0;
+    auto expand = [&](const void *blocks, int64_t r, bf16_t *to) {
+        ExpandJob &j = d.job[jobs++];
+        j.values = values_of(blocks), j.scales = scales_of(blocks, r, width), j.rows = (uint32_t)r, j.down = (uint32_t)ceil_div(r, 64);
+        j.value_pitch = value_pitch(width), j.scale_pitch = (int)scale_pitch(width), j.n = (int)width, j.to = to, j.pitch = padded(r);
+        tiles += j.down * ceil_div(width, BLOCK);
+        if (jobs == 1) d.first = (uint32_t)tiles;
+    };
+    if (dx != nullptr) expand(w_blocks, out, wb);
+    if (dweight != nullptr) expand(x_blocks, rows, xb);
+    if (jobs > 0) {
+        note_kernel(reinterpret_cast<const void *>(expand_kernel));
+        expand_kernel<<<(unsigned)tiles, 256, 0, st>>>(d);
+        VT_STEP(check_launch("linear_8bit_backward"));
+    }
     GradPair g{};
     g.f32 = dtype == VTDGE_F32, g.ends = true;
     if (dx != nullptr) {
-        g.dx.a = g_op, g.dx.b = Operand{wb, padded(width), 0};
-        g.dx.rows = rows, g.dx.cols = width, g.dx.sum_b = out, g.dx.span_b = padded(width);
+        g.dx.a = g_op, g.dx.b = Operand{wb, padded(out), 0};
+        g.dx.rows = rows, g.dx.cols = width, g.dx.sum_b = out;
         g.dx.stages = (int)ceil_div(out, p.slab_g), g.dx.splits = p.dx_splits;
         g.dx.part = p.dx_splits == 1 ? nullptr : (float *)(ws + p.dx_at), g.dx.part_stride = part_of(rows * width), g.dx.out = dx;
     }
     if (dweight != nullptr || dbias != nullptr) {
-        // (without dW the second operand is not multiplied to any end: the gradient itself stands in its place)
-        g.dw.a = g_op, g.dw.b = dweight != nullptr ? Operand{xb, padded(width), 0} : g_op;
-        g.dw.rows = out, g.dw.cols = width, g.dw.sum_a = rows, g.dw.span_a = padded(out), g.dw.sum_b = rows;
-        g.dw.span_b = dweight != nullptr ? padded(width) : padded(out);
+        // (without dW the second operand is not multiplied to any end: the gradient's memory stands in its place, a row of it of any length
+        // within)
+        g.dw.a = g_op, g.dw.b = dweight != nullptr ? Operand{xb, padded(rows), 0} : g_op;
+        g.dw.rows = out, g.dw.cols = dweight != nullptr ? width : 1, g.dw.sum_a = rows, g.dw.span_a = padded(out), g.dw.sum_b = rows;
         g.dw.stages = (int)ceil_div(rows, p.slab_g), g.dw.splits = p.dw_splits;
         const bool cut = p.dw_splits > 1;
         g.dw.part = cut && dweight != nullptr ? (float *)(ws + p.dw_at) : nullptr, g.dw.part_stride = part_of(out * width), g.dw.out = dweight;
