@@ -72,6 +72,38 @@ template <typename T, bool WIDE> __device__ __forceinline__ void store8(T *to, i
     }
 }
 
+// the same in two steps, for loads that go out early: as they lie in memory, and as fp32
+template <typename T, bool WIDE> struct Raw8 {
+    u32x4 v[WIDE ? 8 / Elem<T>::VEC : 2];
+    __device__ __forceinline__ void load(const T *from, int64_t left)
+    {
+        if constexpr (WIDE) {
+            if (left >= 8) {
+#pragma unroll
+                for (int e = 0; e < 8 / Elem<T>::VEC; e++) v[e] = reinterpret_cast<const u32x4 *>(from)[e];
+                return;
+            }
+        }
+        float f[8];
+        load8<T, false>(from, left, f);
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int e = 0; e < 8 / Elem<T>::VEC; e++) v[e] = Elem<T>::pack(f + e * Elem<T>::VEC);
+        } else {
+            v[0] = Elem<float>::pack(f), v[1] = Elem<float>::pack(f + 4);
+        }
+    }
+    __device__ __forceinline__ void unpack(float (&f)[8]) const
+    {
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int e = 0; e < 8 / Elem<T>::VEC; e++) Elem<T>::unpack(v[e], f + e * Elem<T>::VEC);
+        } else {
+            Elem<float>::unpack(v[0], f), Elem<float>::unpack(v[1], f + 4);
+        }
+    }
+};
+
 // the largest of sixteen lanes, in each of them
 template <int CTRL> __device__ __forceinline__ uint32_t lane_max(uint32_t v)
 {
@@ -149,6 +181,12 @@ __device__ __forceinline__ void stands_for8(const u32x2 &bytes, int scale, float
     const f32x2 c = __builtin_amdgcn_cvt_pk_f32_fp8((int)bytes.y, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)bytes.y, true);
     f[0] = a.x * s, f[1] = a.y * s, f[2] = b.x * s, f[3] = b.y * s;
     f[4] = c.x * s, f[5] = c.y * s, f[6] = d.x * s, f[7] = d.y * s;
+}
+// whether one of the eight is NaN
+__device__ __forceinline__ bool any_nan(const u32x2 &bytes, int scale)
+{
+    const uint32_t a = (bytes.x & 0x7f7f7f7fu) + 0x01010101u, b = (bytes.y & 0x7f7f7f7fu) + 0x01010101u;
+    return ((a | b) & 0x80808080u) != 0 || scale == 255;
 }
 __device__ __forceinline__ u32x4 expand8(const u32x2 &bytes, int scale)
 {

@@ -64,8 +64,11 @@ template <typename T, bool WIDE> __global__ __launch_bounds__(256) void gelu_kee
     if (part == 0) put_scale(p.scales + (int64_t)row * p.scale_pitch, (int)block, (int)p.per_row, p.scale_pitch, q.scale);
 }
 
-// Phi(x) + x phi(x): gelu_fn's polynomial for Phi, whose exponential is phi's.  3e-8 of the largest value.
-__device__ __forceinline__ float gelu_slope(float v)
+// Phi(x) + x phi(x).  fp32: gelu_fn's polynomial for Phi, whose exponential is phi's; 3e-8 of the largest value.  bf16: 1/2 and an odd minimax
+// polynomial of degree 17 on [-4.2, 4.2] (x clamped there): |error| <= 1.4e-4, no transcendental, 11 instructions in place of 26 (65536 x
+// 4096: 313 us, bound by them, and VT_SLOPE_US so).  The clamp takes NaN away, see any_nan.
+template <typename T> __device__ __forceinline__ float gelu_slope(float v);
+template <> __device__ __forceinline__ float gelu_slope<float>(float v)
 {
     const float a = fminf(fabsf(v), 16.0f);
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.35f, a, 1.0f));
@@ -81,15 +84,34 @@ __device__ __forceinline__ float gelu_slope(float v)
     const float e = __builtin_amdgcn_exp2f(a * (a * -0.72134752f)), neg = q * t * e;
     return __builtin_fmaf(v * 0.39894228f, e, v < 0.f ? neg : 1.f - neg);
 }
+template <> __device__ __forceinline__ float gelu_slope<bf16_t>(float v)
+{
+    const float x = __builtin_amdgcn_fmed3f(v, -4.2f, 4.2f), t = x * x;
+    float q = 6.356512539e-10f;
+    q = __builtin_fmaf(q, t, -5.912025003e-08f);
+    q = __builtin_fmaf(q, t, 2.394225930e-06f);
+    q = __builtin_fmaf(q, t, -5.575960677e-05f);
+    q = __builtin_fmaf(q, t, 8.318629116e-04f);
+    q = __builtin_fmaf(q, t, -8.368100971e-03f);
+    q = __builtin_fmaf(q, t, 5.761319026e-02f);
+    q = __builtin_fmaf(q, t, -2.639231980e-01f);
+    q = __builtin_fmaf(q, t, 7.973323464e-01f);
+    return __builtin_fmaf(x, q, 0.5f);
+}
 template <typename T, bool WIDE> __global__ __launch_bounds__(256) void gelu_slope_kernel(GeluArgs p)
 {
     const uint32_t id = blockIdx.x * 256 + threadIdx.x, row = id / p.per_row, c = (id - row * p.per_row) * 8;
     if (row >= p.rows) return;
     float g[8], x[8];
     load8<T, WIDE>(static_cast<const T *>(p.x) + (int64_t)row * p.ld + c, p.n - (int)c, g);
-    stands_for8(*reinterpret_cast<const u32x2 *>(p.values + (int64_t)row * p.value_pitch + c), p.scales[(int64_t)row * p.scale_pitch + c / BLOCK], x);
+    const u32x2 bytes = *reinterpret_cast<const u32x2 *>(p.values + (int64_t)row * p.value_pitch + c);
+    const int scale = p.scales[(int64_t)row * p.scale_pitch + c / BLOCK];
+    stands_for8(bytes, scale, x);
 #pragma unroll
-    for (int e = 0; e < 8; e++) g[e] *= gelu_slope(x[e]);
+    for (int e = 0; e < 8; e++) g[e] *= gelu_slope<T>(x[e]);
+    if (any_nan(bytes, scale))                      // rare
+#pragma unroll
+        for (int e = 0; e < 8; e++) g[e] = x[e] == x[e] ? g[e] : x[e];
     store8<T, WIDE>(static_cast<T *>(p.y) + (int64_t)row * p.n + c, p.n - (int)c, g);
 }
 
@@ -103,7 +125,7 @@ template <int WAVES, int NV, typename V> __device__ __forceinline__ void row_sum
 #pragma unroll
     for (int i = 0; i < NV; i++) v[i] = wave_total(v[i]);
     if constexpr (WAVES > 1) {
-        const int wave = threadIdx.x >> 6;
+        const int wave = threadIdx.x >> 6 & (WAVES - 1);
         if ((threadIdx.x & 63) == 0)
 #pragma unroll
             for (int i = 0; i < NV; i++) shared[wave][i] = v[i];
@@ -168,89 +190,87 @@ template <typename T, int WAVES, int CH, bool WIDE> __global__ __launch_bounds__
     }
 }
 
-// h = c r;  dx = r (g - mean g - h mean(g h)), g = dy w;  dw = sum dy h, db = sum dy over the rows: a workgroup's rows in registers, four waves
-// joined in LDS, workgroups by norm_join_kernel.
-template <typename T, int WAVES, int CH, bool WIDE> __global__ __launch_bounds__(256) void norm_slope_kernel(NormArgs p)
+// h = c r;  dx = r (g - mean g - h mean(g h)), g = dy w;  dw = sum dy h, db = sum dy over the rows: a workgroup's rows in registers, those that
+// it has side by side joined in LDS, workgroups by norm_join_kernel.  A lane has eight numbers of a row, which leaves room for the next
+// row's to be on their way (65536 x 1024 in bf16, two waves a row: VT_NORM_US us; one wave with sixteen numbers a lane 108, with the next row's
+// 110, at three waves a SIMD).
+template <int WAVES> struct NormSlope {
+    static constexpr int THREADS = WAVES < 4 ? 256 : WAVES * 64, ROWS = THREADS / 64 / WAVES;      // rows at once
+};
+template <typename T, int WAVES, bool WIDE> __global__ __launch_bounds__(NormSlope<WAVES>::THREADS) void norm_slope_kernel(NormArgs p)
 {
-    constexpr int ROWS = 4 / WAVES;                 // at once
-    __shared__ float sums32[2][WAVES][2];
+    using S = NormSlope<WAVES>;
+    constexpr int ROWS = S::ROWS;
+    __shared__ float sums32[2][ROWS][WAVES][2];
     extern __shared__ __attribute__((aligned(16))) float columns[];        // [2][n], joining ROWS > 1
-    float w[CH][8], dw[CH][8], db[CH][8];
+    const int c = (threadIdx.x & (WAVES * 64 - 1)) * 8, left = p.n - c, group = threadIdx.x / (WAVES * 64);
+    float w[8], dw[8], db[8];
+    load8<T, WIDE>(static_cast<const T *>(p.weight) + c, left, w);
 #pragma unroll
-    for (int k = 0; k < CH; k++) {
-        const int c = norm_column<WAVES>(k);
-        load8<T, WIDE>(static_cast<const T *>(p.weight) + c, p.n - c, w[k]);
-#pragma unroll
-        for (int e = 0; e < 8; e++) dw[k][e] = db[k][e] = 0.f;
-    }
+    for (int e = 0; e < 8; e++) dw[e] = db[e] = 0.f;
     const float inv_n = 1.0f / (float)p.n;
-    int turn = 0;
-    for (int64_t row = (int64_t)blockIdx.x * ROWS + (WAVES == 1 ? threadIdx.x >> 6 : 0); row < p.rows; row += (int64_t)gridDim.x * ROWS) {
-        float g[CH][8], h[CH][8], s[2] = {0.f, 0.f};
-        const float r = p.rstd[row];
-#pragma unroll
-        for (int k = 0; k < CH; k++) {
-            const int c = norm_column<WAVES>(k), left = p.n - c;
-            load8<T, WIDE>(static_cast<const T *>(p.x) + row * p.ld + c, left, g[k]);
-            u32x2 bytes = {0u, 0u};
-            int scale = 127;
-            if (left > 0) {
-                bytes = *reinterpret_cast<const u32x2 *>(p.values + row * p.value_pitch + c);
-                scale = p.scales[row * p.scale_pitch + c / BLOCK];
-            }
-            stands_for8(bytes, scale, h[k]);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                h[k][e] *= r;
-                dw[k][e] = __builtin_fmaf(g[k][e], h[k][e], dw[k][e]);
-                db[k][e] += g[k][e];
-                g[k][e] *= w[k][e];
-                s[0] += g[k][e];
-                s[1] = __builtin_fmaf(g[k][e], h[k][e], s[1]);
-            }
+    struct Row {
+        Raw8<T, WIDE> g;
+        u32x2 bytes;
+        int scale;
+        float r;
+    };
+    auto load = [&](Row &o, int64_t row) {
+        const bool in = row < p.rows;
+        o.g.load(static_cast<const T *>(p.x) + row * p.ld + c, in ? left : 0);
+        o.bytes = u32x2{0u, 0u}, o.scale = 127, o.r = 0.f;
+        if (in) o.r = p.rstd[row];
+        if (in && left > 0) {
+            o.bytes = *reinterpret_cast<const u32x2 *>(p.values + row * p.value_pitch + c);
+            o.scale = p.scales[row * p.scale_pitch + c / BLOCK];
         }
-        if (p.y == nullptr) continue;               // (the same for all)
-        row_sums<WAVES>(s, sums32[turn]);
+    };
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    int turn = 0;
+    Row next;
+    load(next, (int64_t)blockIdx.x * ROWS + group);
+    for (int64_t first = (int64_t)blockIdx.x * ROWS; first < p.rows; first += step) {      // the same for all of the workgroup
+        const int64_t row = first + group;
+        const Row now = next;
+        load(next, row + step);
+        float g[8], h[8], s[2] = {0.f, 0.f};
+        stands_for8(now.bytes, now.scale, h);
+        now.g.unpack(g);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            h[e] *= now.r;
+            dw[e] = __builtin_fmaf(g[e], h[e], dw[e]);
+            db[e] += g[e];
+            g[e] *= w[e];
+            s[0] += g[e];
+            s[1] = __builtin_fmaf(g[e], h[e], s[1]);
+        }
+        if (p.y == nullptr) continue;
+        row_sums<WAVES>(s, sums32[turn][group]);
         turn ^= 1;                                  // the next row's sums do not wait for the readers of these
         const float m0 = s[0] * inv_n, m1 = s[1] * inv_n;
 #pragma unroll
-        for (int k = 0; k < CH; k++) {
-            const int c = norm_column<WAVES>(k), left = p.n - c;
-            if (left <= 0) continue;
-#pragma unroll
-            for (int e = 0; e < 8; e++) g[k][e] = r * (g[k][e] - m0 - h[k][e] * m1);
-            store8<T, WIDE>(static_cast<T *>(p.y) + row * p.n + c, left, g[k]);
-        }
+        for (int e = 0; e < 8; e++) g[e] = now.r * (g[e] - m0 - h[e] * m1);
+        if (row < p.rows) store8<T, WIDE>(static_cast<T *>(p.y) + row * p.n + c, left, g);
     }
     if (p.part == nullptr) return;
+    float *const part = p.part + (int64_t)blockIdx.x * 2 * p.n;
     if constexpr (ROWS > 1) {
-        const int wave = threadIdx.x >> 6;
-        for (int turn = 0; turn < ROWS; turn++) {
-            if (wave == turn)
+        for (int k = 0; k < ROWS; k++) {
+            if (group == k)
 #pragma unroll
-                for (int k = 0; k < CH; k++) {
-                    const int c = norm_column<WAVES>(k);
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (c + e < p.n) {
-                            columns[c + e] = dw[k][e] + (turn > 0 ? columns[c + e] : 0.f);
-                            columns[p.n + c + e] = db[k][e] + (turn > 0 ? columns[p.n + c + e] : 0.f);
-                        }
-                }
+                for (int e = 0; e < 8; e++)
+                    if (e < left) {
+                        columns[c + e] = dw[e] + (k > 0 ? columns[c + e] : 0.f);
+                        columns[p.n + c + e] = db[e] + (k > 0 ? columns[p.n + c + e] : 0.f);
+                    }
             __syncthreads();
         }
-        for (int i = threadIdx.x; i < 2 * p.n; i += 256) p.part[(int64_t)blockIdx.x * 2 * p.n + i] = columns[i];
+        for (int i = threadIdx.x; i < 2 * p.n; i += S::THREADS) part[i] = columns[i];
     } else {
 #pragma unroll
-        for (int k = 0; k < CH; k++) {
-            const int c = norm_column<WAVES>(k);
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (c + e < p.n) {
-                    p.part[(int64_t)blockIdx.x * 2 * p.n + c + e] = dw[k][e];
-                    p.part[(int64_t)blockIdx.x * 2 * p.n + p.n + c + e] = db[k][e];
-                }
-        }
+        for (int e = 0; e < 8; e++)
+            if (e < left) part[c + e] = dw[e], part[p.n + c + e] = db[e];
     }
 }
 // the workgroups' sums of 64 columns, by sixteen waves
@@ -343,18 +363,27 @@ static void norm_shape(int n, int &waves, int &ch)
     ch = (int)ceil_div(n, waves * 512);
     if (ch == 3) ch = 4;
 }
+// the same backward, a lane with eight numbers
+static int slope_waves(int n)
+{
+    int waves = 1;
+    while (waves * 512 < n) waves *= 2;
+    return waves;
+}
 static int64_t norm_parts(int64_t rows, int n)
 {
-    const int64_t at_once = n <= 1024 ? 4 : 1, most = 4 * compute_units(), all = ceil_div(rows, at_once);
+    const int waves = slope_waves(n);
+    const int64_t at_once = waves < 4 ? 4 / waves : 1, most = (waves < 4 ? 4 : 16 / waves) * compute_units(), all = ceil_div(rows, at_once);
     return all < most ? all : most;
 }
 
-#define VT_NORM_CASE(KERN, T, WIDE)                                                                  \
-    (waves == 1 ? (ch == 1 ? KERN<T, 1, 1, WIDE> : KERN<T, 1, 2, WIDE>)                              \
-                : (ch == 1 ? KERN<T, 4, 1, WIDE> : ch == 2 ? KERN<T, 4, 2, WIDE> : KERN<T, 4, 4, WIDE>))
-#define VT_NORM_KERNEL(KERN)                                                                                    \
-    (dtype == VTDGE_F32 ? (wide ? VT_NORM_CASE(KERN, float, true) : VT_NORM_CASE(KERN, float, false))           \
-                        : (wide ? VT_NORM_CASE(KERN, bf16_t, true) : VT_NORM_CASE(KERN, bf16_t, false)))
+#define VT_NORM_CASE(T, WIDE)                                                                                               \
+    (waves == 1 ? (ch == 1 ? norm_keep_kernel<T, 1, 1, WIDE> : norm_keep_kernel<T, 1, 2, WIDE>)                             \
+                : (ch == 1 ? norm_keep_kernel<T, 4, 1, WIDE> : ch == 2 ? norm_keep_kernel<T, 4, 2, WIDE> : norm_keep_kernel<T, 4, 4, WIDE>))
+#define VT_SLOPE_CASE(T, WIDE)                                                                                              \
+    (waves == 1 ? norm_slope_kernel<T, 1, WIDE> : waves == 2 ? norm_slope_kernel<T, 2, WIDE>                                \
+     : waves == 4 ? norm_slope_kernel<T, 4, WIDE> : waves == 8 ? norm_slope_kernel<T, 8, WIDE> : norm_slope_kernel<T, 16, WIDE>)
+#define VT_NORM_KERNEL(CASE) (dtype == VTDGE_F32 ? (wide ? CASE(float, true) : CASE(float, false)) : (wide ? CASE(bf16_t, true) : CASE(bf16_t, false)))
 
 static int check_norm(const char *what, int64_t rows, int64_t n, int dtype)
 {
@@ -453,7 +482,7 @@ extern "C" int vtdge_layernorm_8bit(const void *x, int64_t ldx, const void *weig
     int waves, ch;
     norm_shape((int)n, waves, ch);
     const bool wide = wide_rows(x, rows > 1 ? ldx : 0, dtype) && wide_rows(y, rows > 1 ? n : 0, dtype) && wide_rows(weight, 0, dtype) && wide_rows(bias, 0, dtype);
-    auto kern = VT_NORM_KERNEL(norm_keep_kernel);
+    auto kern = VT_NORM_KERNEL(VT_NORM_CASE);
     note_kernel(reinterpret_cast<const void *>(kern));
     kern<<<(unsigned)ceil_div(rows, 4 / waves), 256, 0, (hipStream_t)stream>>>(a);
     return check_launch("layernorm_8bit");
@@ -482,12 +511,11 @@ extern "C" int vtdge_layernorm_8bit_backward(const void *grad, int64_t ldg, cons
     a.x = grad, a.ld = ldg, a.weight = weight, a.rows = rows, a.n = (int)n, a.y = dx, a.rstd = const_cast<float *>(rstd);
     a.values = values_of(blocks), a.scales = scales_of(blocks, rows, n), a.value_pitch = (int)value_pitch(n), a.scale_pitch = (int)scale_pitch(n);
     a.part = columns ? static_cast<float *>(workspace) : nullptr;
-    int waves, ch;
-    norm_shape((int)n, waves, ch);
+    const int waves = slope_waves((int)n);
     const bool wide = wide_rows(grad, rows > 1 ? ldg : 0, dtype) && (dx == nullptr || wide_rows(dx, rows > 1 ? n : 0, dtype)) && wide_rows(weight, 0, dtype);
-    auto kern = VT_NORM_KERNEL(norm_slope_kernel);
+    auto kern = VT_NORM_KERNEL(VT_SLOPE_CASE);
     note_kernel(reinterpret_cast<const void *>(kern));
-    kern<<<(unsigned)parts, 256, waves == 1 ? 2 * n * 4 : 0, (hipStream_t)stream>>>(a);
+    kern<<<(unsigned)parts, waves < 4 ? 256 : waves * 64, waves < 4 ? 2 * n * 4 : 0, (hipStream_t)stream>>>(a);
     VT_STEP(check_launch("layernorm_8bit_backward"));
     if (!columns) return VTDGE_OK;
     const unsigned blocks64 = (unsigned)ceil_div(2 * n, 64);

@@ -211,8 +211,12 @@ template <class S, typename T, bool GELU> __global__ __launch_bounds__(S::THREAD
                             if (c * VEC < left) *reinterpret_cast<u32x4 *>(to + (int64_t)row * p.out + c * VEC) = *reinterpret_cast<const u32x4 *>(mine + row * PITCH + c * 16);
                         }
                     } else {
-                        for (int row = 0; row < live; row++)
-                            for (int c = lane; c < left; c += 64) to[(int64_t)row * p.out + c] = *reinterpret_cast<const T *>(mine + row * PITCH + c * sizeof(T));
+#pragma unroll 8
+                        for (int k = lane; k < 32 * JP * 32; k += 64) {
+                            const int row = k / (JP * 32), c = k % (JP * 32);
+                            const T o = *reinterpret_cast<const T *>(mine + row * PITCH + c * sizeof(T));
+                            if (row < live && c < left) to[(int64_t)row * p.out + c] = o;
+                        }
                     }
                 }
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -280,7 +284,7 @@ __global__ __launch_bounds__(256) void expand_kernel(ExpandArgs p)
 // ------------------------------------------------------------------------------------------------ on the host
 using ForwardLarge = Shape<2, 4, 4, 2, 64, 2, 1>;
 using ForwardMiddle = Shape<2, 4, 2, 2, 32, 3, 1>;
-using ForwardSmall = Shape<1, 1, 2, 2, 64, 6, 1>;
+using ForwardSmall = Shape<1, 1, 2, 2, 64, 3, 1>;
 
 constexpr int SLAB = 64;
 static int64_t take(int64_t &at, int64_t bytes)
