@@ -78,4 +78,4 @@ def test_arguments_of_the_library():
     args = list(back)
     args[0] = args[9] = args[10] = args[11] = None        # nothing asked for
     assert lib.vtdge_linear_8bit_backward(*args) == 0
-    assert lib.vtdge_linear_8bit_workspace(0, 3, 8, 0) == -1 and lib.vtdge_linear_8bit_backward_workspace(4, 3, 8, 0, 7) == -1
+    assert lib.vtdge_linear_8bit_workspace(0, 3, 8, 0, 0) == -1 and lib.vtdge_linear_8bit_backward_workspace(4, 3, 8, 0, 7) == -1

@@ -127,7 +127,7 @@ _WORKSPACES = {
     "vtdge_cross_entropy_workspace": [_l, _l, _i, _i, _i],
     "vtdge_blocks_bytes": [_l, _l],
     "vtdge_layernorm_8bit_backward_workspace": [_l, _l],
-    "vtdge_linear_8bit_workspace": [_l, _l, _l, _i],
+    "vtdge_linear_8bit_workspace": [_l, _l, _l, _i, _i],
     "vtdge_linear_8bit_backward_workspace": [_l, _l, _l, _i, _i],
 }
 EXPORTS = ["vtdge_version", "vtdge_last_error", "vtdge_last_kernel", "vtdge_recent_kernel"] + list(SIGNATURES)

@@ -631,7 +631,7 @@ static CePlan plan_of(int64_t rows, int64_t classes, int width, int dtype, bool 
         const int64_t pieces = ceil_div(classes, piece);                      // of equal size
         p.piece = ceil_div(ceil_div(classes, pieces), 256) * 256;
         const int64_t of_piece = p.piece < classes ? p.piece : classes;
-        plan_gradients(p, rows, of_piece, width, p.split);
+        plan_gradients(p, rows, of_piece, width, p.split, false);
         p.d_at = take(at, p.d_rows * p.piece * 2 * p.parts);
         p.dx_at = take(at, part_of(rows * width) * 4 * p.dx_splits);
         p.dw_at = take(at, part_of(p.piece * width) * 4 * p.dw_splits);

@@ -102,10 +102,11 @@ Tensor linear_8bit(const Tensor &x, const Tensor &weight, Tensor w_blocks, int64
         if (trains && weight.defined() && weight.requires_grad()) x_blocks = fresh(x, {blocks_bytes(rows, width)}, at::kByte);
         if (trains && weight.defined() && x.requires_grad()) w_blocks = fresh(x, {blocks_bytes(out, width)}, at::kByte);
         const int dtype = code_of(x);
-        const int64_t bytes = bytes_of<4>({rows, out, width, dtype}, [&] { return lib.linear_8bit_workspace(rows, out, width, dtype); });
-        const Tensor ws = fresh(x, {bytes}, at::kByte);
+        const int how = (!wf.defined() ? VTDGE_8BIT_WEIGHT_GIVEN : w_blocks.defined() ? VTDGE_8BIT_WEIGHT_KEPT : 0) | (x_blocks.defined() ? VTDGE_8BIT_X_KEPT : 0);
+        const int64_t bytes = bytes_of<5>({rows, out, width, how, dtype}, [&] { return lib.linear_8bit_workspace(rows, out, width, how, dtype); });
+        const Tensor ws = bytes > 0 ? fresh(x, {bytes}, at::kByte) : Tensor();
         must(lib.linear_8bit(xf.data_ptr(), pitch_of(xf), at_of(wf), wf.defined() ? pitch_of(wf) : 0, at_of(w_blocks), at_of(b), y.data_ptr(), at_of(x_blocks),
-                             rows, out, width, act, ws.data_ptr(), bytes, dtype, stream_of(x)),
+                             rows, out, width, act, at_of(ws), bytes, dtype, stream_of(x)),
              "vtdge_linear_8bit");
     }
     if (trains) {

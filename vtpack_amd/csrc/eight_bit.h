@@ -16,7 +16,7 @@ inline unsigned char *values_of(const void *blocks) { return static_cast<unsigne
 inline unsigned char *scales_of(const void *blocks, int64_t rows, int64_t n) { return values_of(blocks) + rows * value_pitch(n); }
 
 struct QuantizeJob {
-    const void *from; int64_t ld; uint32_t rows, per_row; int n;       // per_row: blocks
+    const void *from; int64_t ld; uint32_t rows, per_row; int n;       // nullable: the blocks are there; per_row: blocks
     unsigned char *values, *scales; int64_t value_pitch; int scale_pitch;      // nullable
     bf16_t *expanded; int64_t expanded_pitch;       // nullable: the numbers as bf16, zeros behind the last of a row
 };

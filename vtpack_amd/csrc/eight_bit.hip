@@ -21,11 +21,18 @@ template <typename T, bool WIDE> __global__ __launch_bounds__(256) void quantize
     const uint32_t id = (blockIdx.x - (second ? p.first : 0)) * 16 + (threadIdx.x >> 4), row = id / job.per_row, block = id - row * job.per_row;
     const int part = threadIdx.x & 15, c = (int)block * BLOCK + part * 8;
     const bool in = row < job.rows;
-    float f[8];
-    load8<T, WIDE>(static_cast<const T *>(job.from) + (int64_t)row * job.ld + c, in ? job.n - c : 0, f);
-    const Rounded q = round8(f);
-    if (!in) return;
-    if (job.values != nullptr) {
+    Rounded q;
+    if (job.from == nullptr) {                      // blocks that are there
+        if (!in) return;
+        q.bytes = *reinterpret_cast<const u32x2 *>(job.values + (int64_t)row * job.value_pitch + c);
+        q.scale = job.scales[(int64_t)row * job.scale_pitch + block];
+    } else {
+        float f[8];
+        load8<T, WIDE>(static_cast<const T *>(job.from) + (int64_t)row * job.ld + c, in ? job.n - c : 0, f);
+        q = round8(f);
+        if (!in) return;
+    }
+    if (job.from != nullptr && job.values != nullptr) {
         *reinterpret_cast<u32x2 *>(job.values + (int64_t)row * job.value_pitch + c) = q.bytes;
         if (part == 0) put_scale(job.scales + (int64_t)row * job.scale_pitch, (int)block, (int)job.per_row, job.scale_pitch, q.scale);
     }
@@ -304,7 +311,7 @@ bool wide_rows(const void *p, int64_t ld, int dtype) { return ((uintptr_t)p & 15
 QuantizeJob quantize_job(const void *from, int64_t ld, int64_t rows, int64_t n, void *blocks, bf16_t *expanded, int64_t expanded_pitch)
 {
     QuantizeJob j{};
-    j.from = from, j.ld = ld, j.rows = (uint32_t)rows, j.n = (int)n, j.per_row = (uint32_t)ceil_div(n, BLOCK);
+    j.from = from, j.ld = from != nullptr ? ld : 0, j.rows = (uint32_t)rows, j.n = (int)n, j.per_row = (uint32_t)ceil_div(n, BLOCK);
     if (blocks != nullptr) j.values = values_of(blocks), j.scales = scales_of(blocks, rows, n);
     j.value_pitch = value_pitch(n), j.scale_pitch = (int)scale_pitch(n);
     j.expanded = expanded, j.expanded_pitch = expanded_pitch;

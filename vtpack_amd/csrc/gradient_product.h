@@ -35,7 +35,8 @@ struct GradPlan {
     int gm, gn, slab_g;                             // its tile and slab
     int dx_splits, dw_splits;
 };
-void plan_gradients(GradPlan &p, int64_t rows, int64_t classes, int width, bool split);
+// (`ends`: of GradPair)
+void plan_gradients(GradPlan &p, int64_t rows, int64_t classes, int width, bool split, bool ends);
 // elements from one part of a sum to the next
 inline int64_t part_of(int64_t n) { return (n + 63) / 64 * 64; }
 // tm, tn and first_dw are filled in.  `what`: the entry point, for errors

@@ -73,7 +73,7 @@ template <class S, bool A_ALONG, bool ENDS> __device__ __forceinline__ void grad
                 }
             }
         }
-        if (S::WHOLE_LINES || r >= p.rows) continue;
+        if (ENDS || S::WHOLE_LINES || r >= p.rows) continue;
 #pragma unroll
         for (int j = 0; j < JN; j++)
 #pragma unroll
@@ -82,7 +82,12 @@ template <class S, bool A_ALONG, bool ENDS> __device__ __forceinline__ void grad
                 put_four(p, all, z, r, c0 + (wn * JN + j) * 32 + 8 * q + 4 * lg, v, scale);
             }
     }
-    if constexpr (S::WHOLE_LINES) {
+    if constexpr (ENDS) {
+        auto as_it_is = [](int, int, f32x4 &) {};
+        if (p.part != nullptr) put_tile<S>(smem, acc, as_it_is, p.part + z * p.part_stride, p.rows, p.cols, r0, c0, false);
+        else if (p.out != nullptr && all.f32) put_tile<S>(smem, acc, as_it_is, static_cast<float *>(p.out), p.rows, p.cols, r0, c0, false);
+        else if (p.out != nullptr) put_tile<S>(smem, acc, as_it_is, static_cast<bf16_t *>(p.out), p.rows, p.cols, r0, c0, false);
+    } else if constexpr (S::WHOLE_LINES) {
         // by way of LDS, lanes side by side in a row (bf16 1 x 363 x 25766: 40 us without, 22 so)
         constexpr int PITCH = S::COLS + 4;
         static_assert(S::ROWS * PITCH * 4 <= S::RING && IM == 1, "LDS");
@@ -162,13 +167,14 @@ __global__ __launch_bounds__(256) void gradient_sum_kernel(SumArgs p)
 
 // ------------------------------------------------------------------------------------------------ on the host
 using GradLarge = Shape<2, 4, 4, 2, 64, 2, 1>;
+using GradSquare = Shape<2, 2, 2, 2, 64, 2, 1>;
 using GradMiddle = Shape<2, 2, 4, 2, 64, 3, 1>;
 // (short sums of many tiles: three on a compute unit, fp32 two, rather than a deep ring for one; bf16 1 row x 363 x 25766 classes 43 -> 22 us,
 // 256 x 384 x 1000 10.2 -> 9.7)
 using GradSmall = Shape<1, 1, 2, 2, 64, 3, 1>;
 using SplitGradLarge = Shape<2, 2, 4, 2, 32, 2, 3>;
 using SplitGradSmall = Shape<1, 1, 2, 2, 32, 3, 3>;
-enum { GRAD_LARGE, GRAD_MIDDLE, GRAD_SMALL };
+enum { GRAD_LARGE, GRAD_MIDDLE, GRAD_SMALL, GRAD_SQUARE };
 
 // When `slots` workers are done with n1 jobs of l1 and then n2 of l2, each taken by whoever is free first.
 static int64_t makespan(int64_t slots, int64_t n1, int64_t l1, int64_t n2, int64_t l2)
@@ -226,8 +232,22 @@ static double cuts(GradPlan &p, int64_t rows, int64_t of_piece, int width, const
 }
 template <class S> static GradShape grad_shape(int grads, double us, double tile_us) { return GradShape{grads, S::ROWS, S::COLS, S::SLAB, us, tile_us}; }
 
-void plan_gradients(GradPlan &p, int64_t rows, int64_t of_piece, int width, bool split)
+#ifndef VT_FORCE
+#define VT_FORCE -1
+#endif
+void plan_gradients(GradPlan &p, int64_t rows, int64_t of_piece, int width, bool split, bool ends)
 {
+    if (ends) {
+        const GradShape shapes[4] = {grad_shape<GradLarge>(GRAD_LARGE, 2.0, 6.0), grad_shape<GradMiddle>(GRAD_MIDDLE, 1.3, 4.0), grad_shape<GradSquare>(GRAD_SQUARE, 0.65, 2.5), grad_shape<GradSmall>(GRAD_SMALL, 0.35, 1.4)};
+        int best = 0;
+        double least = 1e30;
+        for (int k = 0; k < 4; k++) {
+            const double t = cuts(p, rows, of_piece, width, shapes[k], false);
+            if (t < least) least = t, best = k;
+        }
+        cuts(p, rows, of_piece, width, shapes[VT_FORCE >= 0 ? VT_FORCE : best], true);
+        return;
+    }
     const GradShape large = split ? grad_shape<SplitGradLarge>(GRAD_LARGE, 3.0, 12.0) : grad_shape<GradLarge>(GRAD_LARGE, 2.0, 6.0);
     const GradShape middle = grad_shape<GradMiddle>(GRAD_MIDDLE, 1.3, 4.0);
     const GradShape small = split ? grad_shape<SplitGradSmall>(GRAD_SMALL, 0.6, 2.4) : grad_shape<GradSmall>(GRAD_SMALL, 0.35, 1.4);
@@ -285,7 +305,8 @@ int launch_gradients(const GradPlan &p, GradPair &g, const char *what, hipStream
     if (g.f32_parts) return p.grads == GRAD_LARGE ? go_grad<SplitGradLarge, false>(g, what, st) : go_grad<SplitGradSmall, false>(g, what, st);
     if (g.ends)
         return p.grads == GRAD_LARGE ? go_grad<GradLarge, true>(g, what, st)
-               : p.grads == GRAD_MIDDLE ? go_grad<GradMiddle, true>(g, what, st) : go_grad<GradSmall, true>(g, what, st);
+               : p.grads == GRAD_MIDDLE ? go_grad<GradMiddle, true>(g, what, st)
+               : p.grads == GRAD_SQUARE ? go_grad<GradSquare, true>(g, what, st) : go_grad<GradSmall, true>(g, what, st);
     return p.grads == GRAD_LARGE ? go_grad<GradLarge, false>(g, what, st)
            : p.grads == GRAD_MIDDLE ? go_grad<GradMiddle, false>(g, what, st) : go_grad<GradSmall, false>(g, what, st);
 }

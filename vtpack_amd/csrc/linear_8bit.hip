@@ -147,85 +147,125 @@ template <class S, typename T, bool GELU> __global__ __launch_bounds__(S::THREAD
         read_bias();
         multiply_tile<S, false>(a, b, 0, p.stages, smem, acc, false, none);
     }
-    const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
-    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
-    // To memory by way of LDS, a wave 32 rows at a time, so that whole lines leave at once (bf16 65536 x 1024 x 4096 with GELU: 470 us in 32-byte
-    // pieces, 395 so, 375 also past the caches, where the result fills them anyway).
-    constexpr int JP = EIGHT || JN == 1 ? JN : JN / 2, ROW = JP * 32 * sizeof(T), PITCH = ROW + 16, VEC = Elem<T>::VEC, LANES = ROW / 16;
-    static_assert(S::WAVES * 32 * PITCH <= (EIGHT ? EightBit<S>::RING : S::RING), "LDS");
-    unsigned char *const mine = smem + wid * 32 * PITCH;
-    // WHOLE: no row or column of the tile is behind the last, vectors of the result lie on their boundaries.  In one run without branches: with
-    // them the stores of a piece wait for one another (35 us of the 340 above).
-    auto leave = [&](auto WHOLE, auto STREAM) {
-        constexpr bool whole = decltype(WHOLE)::value, stream = decltype(STREAM)::value;
+    const int lg = (threadIdx.x & 63) >> 5, wn = wave_uniform(threadIdx.x >> 6) % S::WN;
+    // (bf16 65536 x 1024 x 4096 with GELU: 470 us in pieces of 32 bytes from the registers, 400 so, past the caches where the result fills them anyway)
+    auto finish = [&](int j, int q, f32x4 &v) {
+        v += *reinterpret_cast<const f32x4 *>(bias + (wn * JN + j) * 32 + 8 * q + 4 * lg);
+        if constexpr (GELU)
 #pragma unroll
-        for (int i = 0; i < IM; i++) {
+            for (int e = 0; e < 4; e++) v[e] = gelu_fn<T>(v[e]);
+    };
+    put_tile<S>(smem, acc, finish, static_cast<T *>(p.y), p.rows, p.out, r0, c0, p.stream_y);
+}
+
+// ------------------------------------------------------------------------------------------------ few rows
+// Up to 16 rows against a weight in blocks, bound by the reading of the weight: one launch, x is brought into blocks by every workgroup for
+// itself while the first of its weights are on their way.  A workgroup has 16 outputs, its four waves take four blocks of them in turn; a
+// lane loads 32 bytes of a block of one output, four of them the whole line, and multiplies as it came (both operands' numbers are in the
+// same order).  (1 row x 4096 x 16384: VT_FEW_US us; as tiles behind a launch for x 20.)
+struct FewArgs {
+    const void *x; int64_t ldx; int rows, width;
+    const unsigned char *w, *w_scales; int64_t value_pitch; int scale_pitch;
+    const void *bias; void *y; int64_t out;
+};
+constexpr int FEW = 16, FEW_BYTES = 16384;          // rows; numbers of x in LDS
+template <typename T> static constexpr int few_lds(int rows, int64_t pitch, int scales)
+{
+    return (int)(rows * pitch * (sizeof(T) == 2 ? 1 : 2)) + (rows * scales + 15) / 16 * 16 + 4 * 64 * 16;
+}
+template <typename T, bool WIDE, bool GELU> __global__ __launch_bounds__(256) void linear_8bit_few_kernel(FewArgs p)
+{
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    constexpr bool EIGHT = sizeof(T) == 2;
+    constexpr int SIZE = EIGHT ? 1 : 2;             // bytes of a number of x: 8-bit, or expanded
+    const int lane = threadIdx.x & 63, wid = wave_uniform(threadIdx.x >> 6), at16 = lane & 15, g = lane >> 4;
+    const int blocks = (p.width + BLOCK - 1) / BLOCK, x_pitch = blocks * BLOCK * SIZE;
+    unsigned char *const xq = smem, *const xs = smem + p.rows * x_pitch;
+    f32x4 *const sums = reinterpret_cast<f32x4 *>(xs + (p.rows * p.scale_pitch + 15) / 16 * 16);
+    const int64_t o0 = (int64_t)blockIdx.x * 16, o = o0 + at16 < p.out ? o0 + at16 : p.out - 1;
+    const unsigned char *const w = p.w + o * p.value_pitch + g * 16, *const ws = p.w_scales + o * p.scale_pitch;
+    struct Unit {
+        u32x4 v[4][2];
+        uint32_t scales;
+    };
+    auto load = [&](Unit &u, int unit) {
+        if (unit * 4 >= blocks) return;
+        u.scales = *reinterpret_cast<const uint32_t *>(ws + unit * 4);
 #pragma unroll
-            for (int j0 = 0; j0 < JN; j0 += JP) {
+        for (int b = 0; b < 4; b++) {
+            const int block = min(unit * 4 + b, blocks - 1);          // (behind the last: not used)
 #pragma unroll
-                for (int j = j0; j < j0 + JP; j++) {
-                    f32x4 v[4];
+            for (int h = 0; h < 2; h++) u.v[b][h] = *reinterpret_cast<const u32x4 *>(w + block * BLOCK + h * 64);
+        }
+    };
+    float add[4];                                   // the outputs' own, see below
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const f32x4 add = *reinterpret_cast<const f32x4 *>(bias + (wn * JN + j) * 32 + 8 * q + 4 * lg);
+    for (int e = 0; e < 4; e++) add[e] = p.bias != nullptr && o0 + 4 * g + e < p.out ? Elem<T>::load(static_cast<const T *>(p.bias) + o0 + 4 * g + e) : 0.f;
+    Unit next[2];                                   // two ahead: 4096 numbers of the four waves
+    load(next[0], wid);
+    load(next[1], wid + 4);
+    for (int first = 0; first < p.rows * blocks; first += 16) {        // the same for all: the lanes of a block take part together
+        const int id = first + (threadIdx.x >> 4), row = id / blocks, block = id - row * blocks, c = block * BLOCK + at16 * 8;
+        const bool in = id < p.rows * blocks;
+        float f[8];
+        load8<T, WIDE>(static_cast<const T *>(p.x) + (int64_t)row * p.ldx + c, in ? p.width - c : 0, f);
+        const Rounded q = round8(f);
+        if (!in) continue;
+        if constexpr (EIGHT) {
+            *reinterpret_cast<u32x2 *>(xq + row * x_pitch + c) = q.bytes;
+            if (at16 == 0) xs[row * p.scale_pitch + block] = (unsigned char)q.scale;
+        } else {
+            *reinterpret_cast<u32x4 *>(xq + row * x_pitch + c * 2) = expand8(q.bytes, q.scale);
+        }
+    }
+    lds_barrier();
+    const int row = at16 < p.rows ? at16 : p.rows - 1;
+    const unsigned char *const xr = xq + row * x_pitch + g * 16 * SIZE, *const xsr = xs + row * p.scale_pitch;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const Unit &now, int unit) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            v[q][e] = acc[i][j][4 * q + e] + add[e];
-                            if (GELU) v[q][e] = gelu_fn<T>(v[q][e]);
-                        }
-                    }
-                    unsigned char *const at = mine + lr * PITCH + (j - j0) * 32 * sizeof(T);
-                    if constexpr (EIGHT) {
-                        // half-wave swaps leave a lane 8 consecutive columns
+        for (int b = 0; b < 4; b++) {
+            const int block = unit * 4 + b;
+            if (block >= blocks) break;
+            if constexpr (EIGHT) {
+                const u32x4 x0 = *reinterpret_cast<const u32x4 *>(xr + block * BLOCK), x1 = *reinterpret_cast<const u32x4 *>(xr + block * BLOCK + 64);
+                const u32x4 w0 = now.v[b][0], w1 = now.v[b][1];
+                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                    i32x8{(int)w0.x, (int)w0.y, (int)w0.z, (int)w0.w, (int)w1.x, (int)w1.y, (int)w1.z, (int)w1.w},
+                    i32x8{(int)x0.x, (int)x0.y, (int)x0.z, (int)x0.w, (int)x1.x, (int)x1.y, (int)x1.z, (int)x1.w}, acc, 0, 0, 0,
+                    (int)(now.scales >> (8 * b)), 0, (int)xsr[block]);
+            } else {
 #pragma unroll
-                        for (int q = 0; q < 2; q++) {
-                            const uint32_t o[4] = {pack_bf16x2(v[2 * q][0], v[2 * q][1]), pack_bf16x2(v[2 * q][2], v[2 * q][3]),
-                                                   pack_bf16x2(v[2 * q + 1][0], v[2 * q + 1][1]), pack_bf16x2(v[2 * q + 1][2], v[2 * q + 1][3])};
-                            const auto s0 = __builtin_amdgcn_permlane32_swap(o[0], o[2], false, false), s1 = __builtin_amdgcn_permlane32_swap(o[1], o[3], false, false);
-                            *reinterpret_cast<u32x4 *>(at + 32 * q + 16 * lg) = u32x4{s0[0], s1[0], s0[1], s1[1]};
-                        }
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 4; q++) *reinterpret_cast<f32x4 *>(at + 32 * q + 16 * lg) = v[q];
-                    }
+                for (int q = 0; q < 4; q++) {
+                    const u32x4 part = now.v[b][q >> 1];
+                    const u32x4 we = expand8(q & 1 ? u32x2{part.z, part.w} : u32x2{part.x, part.y}, (int)(now.scales >> (8 * b) & 255u));
+                    const u32x4 xe = *reinterpret_cast<const u32x4 *>(xr + (block * BLOCK + (q >> 1) * 64 + (q & 1) * 8) * 2);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, we), __builtin_bit_cast(bf16x8, xe), acc, 0, 0, 0);
                 }
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // (the wave's own)
-                const int64_t first = r0 + (wm * IM + i) * 32, column = c0 + (wn * JN + j0) * 32;
-                T *const to = static_cast<T *>(p.y) + first * p.out + column;
-                if constexpr (whole) {
-                    constexpr int TIMES = 32 * LANES / 64;
-                    const int row = lane / LANES, c = lane % LANES;
-                    T *const from = to + (int64_t)row * p.out + c * VEC;
-#pragma unroll
-                    for (int k = 0; k < TIMES; k++) {
-                        const u32x4 o = *reinterpret_cast<const u32x4 *>(mine + (row + k * (64 / LANES)) * PITCH + c * 16);
-                        u32x4 *const at = reinterpret_cast<u32x4 *>(from + (int64_t)k * (64 / LANES) * p.out);
-                        if constexpr (stream) __builtin_nontemporal_store(o, at);
-                        else *at = o;
-                    }
-                } else {
-                    const int live = (int)(p.rows - first < 32 ? p.rows - first : 32), left = (int)(p.out - column < JP * 32 ? p.out - column : JP * 32);
-                    if (p.out % VEC == 0) {
-                        for (int k = lane; k < live * LANES; k += 64) {
-                            const int row = k / LANES, c = k % LANES;
-                            if (c * VEC < left) *reinterpret_cast<u32x4 *>(to + (int64_t)row * p.out + c * VEC) = *reinterpret_cast<const u32x4 *>(mine + row * PITCH + c * 16);
-                        }
-                    } else {
-#pragma unroll 8
-                        for (int k = lane; k < 32 * JP * 32; k += 64) {
-                            const int row = k / (JP * 32), c = k % (JP * 32);
-                            const T o = *reinterpret_cast<const T *>(mine + row * PITCH + c * sizeof(T));
-                            if (row < live && c < left) to[(int64_t)row * p.out + c] = o;
-                        }
-                    }
-                }
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
         }
     };
-    if (p.out % VEC != 0 || r0 + S::ROWS > p.rows || c0 + S::COLS > p.out) leave(std::false_type{}, std::false_type{});
-    else if (p.stream_y) leave(std::true_type{}, std::true_type{});
-    else leave(std::true_type{}, std::false_type{});
+    for (int unit = wid; unit * 4 < blocks; unit += 8) {
+        const Unit now = next[0];
+        load(next[0], unit + 8);
+        multiply(now, unit);
+        const Unit then = next[1];
+        load(next[1], unit + 12);
+        multiply(then, unit + 4);
+    }
+    // a lane has outputs 4 g .. 4 g + 3 of row at16
+    sums[wid * 64 + lane] = acc;
+    lds_barrier();
+    if (wid != 0 || at16 >= p.rows) return;
+    acc = (sums[lane] + sums[64 + lane]) + (sums[128 + lane] + sums[192 + lane]);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const int64_t c = o0 + 4 * g + e;
+        if (c >= p.out) break;
+        float v = acc[e] + add[e];
+        if (GELU) v = gelu_fn<T>(v);
+        Elem<T>::store(static_cast<T *>(p.y) + at16 * p.out + c, v);
+    }
 }
 
 // Rows of g as the products read them: bf16, filled up with zeros to whole slabs.
@@ -295,15 +335,18 @@ static int64_t take(int64_t &at, int64_t bytes)
 }
 static int64_t padded(int64_t n) { return ceil_div(n, SLAB) * SLAB; }
 
+static bool few_rows(int64_t rows, int64_t width) { return rows <= FEW && rows * value_pitch(width) <= FEW_BYTES; }
+
 struct ForwardPlan {
     int64_t x_at, w_at, bytes;
 };
-static ForwardPlan plan_forward(int64_t rows, int64_t out, int64_t width, int dtype)
+static ForwardPlan plan_forward(int64_t rows, int64_t out, int64_t width, int how, int dtype)
 {
     ForwardPlan p{};
     int64_t at = 0;
-    p.x_at = take(at, dtype == VTDGE_F32 ? rows * padded(width) * 2 : blocks_bytes(rows, width));
-    p.w_at = take(at, dtype == VTDGE_F32 ? out * padded(width) * 2 : blocks_bytes(out, width));
+    const bool few = few_rows(rows, width), blocks = few || dtype != VTDGE_F32;        // blocks are multiplied, or what they expand to
+    p.x_at = take(at, few || (blocks && (how & VTDGE_8BIT_X_KEPT)) ? 0 : blocks ? blocks_bytes(rows, width) : rows * padded(width) * 2);
+    p.w_at = take(at, blocks && (how & (VTDGE_8BIT_WEIGHT_KEPT | VTDGE_8BIT_WEIGHT_GIVEN)) ? 0 : blocks ? blocks_bytes(out, width) : out * padded(width) * 2);
     p.bytes = at;
     return p;
 }
@@ -318,7 +361,7 @@ static bool gradient_lies(const void *g, int64_t ld, int64_t out, int dtype)
 static BackwardPlan plan_backward(int64_t rows, int64_t out, int64_t width, bool lies)
 {
     BackwardPlan p{};
-    plan_gradients(p, rows, out, (int)width, false);
+    plan_gradients(p, rows, out, (int)width, false, true);
     int64_t at = 0;
     p.g_at = take(at, lies ? 0 : rows * padded(out) * 2);
     p.x_at = take(at, width * padded(rows) * 2);
@@ -361,27 +404,50 @@ template <class S> static int go_forward(const ForwardArgs &a, int act, int dtyp
 
 using namespace vtdge;
 
-extern "C" int64_t vtdge_linear_8bit_workspace(int64_t rows, int64_t out, int64_t width, int dtype)
+extern "C" int64_t vtdge_linear_8bit_workspace(int64_t rows, int64_t out, int64_t width, int how, int dtype)
 {
     if (check_linear("linear_8bit_workspace", rows, out, width, dtype) != VTDGE_OK) return -1;
-    return plan_forward(rows, out, width, dtype).bytes;
+    return plan_forward(rows, out, width, how, dtype).bytes;
+}
+
+template <typename T> static int go_few(const FewArgs &a, int act, hipStream_t st)
+{
+    const int dtype = sizeof(T) == 2 ? VTDGE_BF16 : VTDGE_F32;
+    const bool wide = wide_rows(a.x, a.rows > 1 ? a.ldx : 0, dtype), gelu = act == VTDGE_ACT_GELU;
+    auto kern = wide ? (gelu ? linear_8bit_few_kernel<T, true, true> : linear_8bit_few_kernel<T, true, false>)
+                     : (gelu ? linear_8bit_few_kernel<T, false, true> : linear_8bit_few_kernel<T, false, false>);
+    note_kernel(reinterpret_cast<const void *>(kern));
+    kern<<<(unsigned)ceil_div(a.out, 16), 256, few_lds<T>(a.rows, value_pitch(a.width), a.scale_pitch), st>>>(a);
+    return check_launch("linear_8bit");
 }
 
 extern "C" int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight, int64_t ldw, void *w_blocks, const void *bias, void *y, void *x_blocks,
                                  int64_t rows, int64_t out, int64_t width, int act, void *workspace, int64_t workspace_bytes, int dtype, void *stream)
 {
     VT_STEP(check_linear("linear_8bit", rows, out, width, dtype));
-    VT_REQUIRE(x && y && workspace && (weight || w_blocks), VTDGE_ERR_ARG, "linear_8bit: NULL operand");
+    VT_REQUIRE(x && y && (weight || w_blocks), VTDGE_ERR_ARG, "linear_8bit: NULL operand");
     VT_REQUIRE(act == VTDGE_ACT_NONE || act == VTDGE_ACT_GELU, VTDGE_ERR_ARG, "linear_8bit: act %d", act);
     VT_REQUIRE((ldx >= width || rows == 1) && (weight == nullptr || ldw >= width || out == 1), VTDGE_ERR_ARG, "linear_8bit: rows of %lld, %lld and %lld apart",
                (long long)width, (long long)ldx, (long long)ldw);
     VT_REQUIRE(((uintptr_t)w_blocks & 127) == 0 && ((uintptr_t)x_blocks & 127) == 0, VTDGE_ERR_ARG, "linear_8bit: blocks off their boundary");
-    const ForwardPlan p = plan_forward(rows, out, width, dtype);
-    VT_REQUIRE(workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG, "linear_8bit: workspace of %lld bytes, %lld needed",
-               (long long)workspace_bytes, (long long)p.bytes);
+    const int how = (weight == nullptr ? VTDGE_8BIT_WEIGHT_GIVEN : w_blocks != nullptr ? VTDGE_8BIT_WEIGHT_KEPT : 0) | (x_blocks != nullptr ? VTDGE_8BIT_X_KEPT : 0);
+    const ForwardPlan p = plan_forward(rows, out, width, how, dtype);
+    VT_REQUIRE((workspace != nullptr || p.bytes == 0) && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG,
+               "linear_8bit: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.bytes);
     unsigned char *const ws = (unsigned char *)workspace;
     const hipStream_t st = (hipStream_t)stream;
     QuantizeArgs q{};
+    if (few_rows(rows, width)) {
+        void *const wq = w_blocks != nullptr ? w_blocks : ws + p.w_at;
+        int jobs = 0;
+        if (weight != nullptr) q.job[jobs++] = quantize_job(weight, ldw, out, width, wq, nullptr, 0);
+        if (x_blocks != nullptr) q.job[jobs++] = quantize_job(x, ldx, rows, width, x_blocks, nullptr, 0);
+        if (jobs > 0) VT_STEP(launch_quantize(q, jobs, dtype, "linear_8bit", st));
+        FewArgs f{};
+        f.x = x, f.ldx = ldx, f.rows = (int)rows, f.width = (int)width, f.w = values_of(wq), f.w_scales = scales_of(wq, out, width);
+        f.value_pitch = value_pitch(width), f.scale_pitch = (int)scale_pitch(width), f.bias = bias, f.y = y, f.out = out;
+        return dtype == VTDGE_F32 ? go_few<float>(f, act, st) : go_few<bf16_t>(f, act, st);
+    }
     ForwardArgs a{};
     a.bias = bias, a.y = y, a.rows = rows, a.out = out;
     a.stream_y = rows * out * (dtype == VTDGE_F32 ? 4 : 2) >= (256ll << 20);      // the last cache
@@ -389,13 +455,8 @@ extern "C" int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight,
     if (dtype == VTDGE_F32) {
         bf16_t *const xb = (bf16_t *)(ws + p.x_at), *const wb = (bf16_t *)(ws + p.w_at);
         q.job[0] = quantize_job(x, ldx, rows, width, x_blocks, xb, padded(width));
-        if (weight != nullptr) q.job[1] = quantize_job(weight, ldw, out, width, w_blocks, wb, padded(width));
-        VT_STEP(launch_quantize(q, weight != nullptr ? 2 : 1, dtype, "linear_8bit", st));
-        if (weight == nullptr) {
-            DequantizeArgs d{};
-            d.job[0] = dequantize_job(w_blocks, out, width, wb, padded(width), padded(width));
-            VT_STEP(launch_dequantize(d, 1, VTDGE_BF16, "linear_8bit", st));
-        }
+        q.job[1] = quantize_job(weight, ldw, out, width, w_blocks, wb, padded(width));
+        VT_STEP(launch_quantize(q, 2, dtype, "linear_8bit", st));
         a.x = Operand{xb, padded(width), 0}, a.w = Operand{wb, padded(width), 0};
         slabs = padded(width) / SLAB;
     } else {

@@ -201,6 +201,86 @@ __device__ __forceinline__ void multiply_tile(const LA &a, const LB &b, int t0, 
     lds_barrier();                                  // the ring is free for the epilogue
 }
 
+// A tile's results to memory, [rows, cols] dense: by way of LDS (the ring, behind its last reader), a wave 32 rows at a time, so that whole
+// lines leave at once.  finish(j, q, v) has the last word on four of a row, columns (wn JN + j) 32 + 8 q + 4 (lane / 32) .. of the tile;
+// `stream`: past the caches.  In runs without branches where the tile is whole: with them the stores of a piece wait for one another.
+template <class S, typename T, class F>
+__device__ __forceinline__ void put_tile(unsigned char *smem, const f32x16 (&acc)[S::IM][S::JN], F &&finish, T *out, int64_t rows, int64_t cols, int64_t r0, int64_t c0,
+                                         bool stream)
+{
+    constexpr int JN = S::JN, JP = sizeof(T) == 2 || JN == 1 ? JN : JN / 2, ROW = JP * 32 * sizeof(T), PITCH = ROW + 16, VEC = Elem<T>::VEC, LANES = ROW / 16;
+    static_assert(S::WAVES * 32 * PITCH <= S::RING, "LDS");
+    const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
+    const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
+    unsigned char *const mine = smem + wid * 32 * PITCH;
+    auto leave = [&](auto WHOLE, auto STREAM) {
+        constexpr bool whole = decltype(WHOLE)::value, past = decltype(STREAM)::value;
+#pragma unroll
+        for (int i = 0; i < S::IM; i++) {
+#pragma unroll
+            for (int j0 = 0; j0 < JN; j0 += JP) {
+#pragma unroll
+                for (int j = j0; j < j0 + JP; j++) {
+                    f32x4 v[4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        v[q] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                        finish(j, q, v[q]);
+                    }
+                    unsigned char *const at = mine + lr * PITCH + (j - j0) * 32 * sizeof(T);
+                    if constexpr (sizeof(T) == 2) {
+                        // half-wave swaps leave a lane 8 consecutive columns
+#pragma unroll
+                        for (int q = 0; q < 2; q++) {
+                            const uint32_t o[4] = {pack_bf16x2(v[2 * q][0], v[2 * q][1]), pack_bf16x2(v[2 * q][2], v[2 * q][3]),
+                                                   pack_bf16x2(v[2 * q + 1][0], v[2 * q + 1][1]), pack_bf16x2(v[2 * q + 1][2], v[2 * q + 1][3])};
+                            const auto s0 = __builtin_amdgcn_permlane32_swap(o[0], o[2], false, false), s1 = __builtin_amdgcn_permlane32_swap(o[1], o[3], false, false);
+                            *reinterpret_cast<u32x4 *>(at + 32 * q + 16 * lg) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+                        }
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 4; q++) *reinterpret_cast<f32x4 *>(at + 32 * q + 16 * lg) = v[q];
+                    }
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");        // (the wave's own)
+                const int64_t first = r0 + (wm * S::IM + i) * 32, column = c0 + (wn * JN + j0) * 32;
+                T *const to = out + first * cols + column;
+                if constexpr (whole) {
+                    constexpr int TIMES = 32 * LANES / 64;
+                    const int row = lane / LANES, c = lane % LANES;
+                    T *const from = to + (int64_t)row * cols + c * VEC;
+#pragma unroll
+                    for (int k = 0; k < TIMES; k++) {
+                        const u32x4 o = *reinterpret_cast<const u32x4 *>(mine + (row + k * (64 / LANES)) * PITCH + c * 16);
+                        u32x4 *const at = reinterpret_cast<u32x4 *>(from + (int64_t)k * (64 / LANES) * cols);
+                        if constexpr (past) __builtin_nontemporal_store(o, at);
+                        else *at = o;
+                    }
+                } else {
+                    const int live = (int)(rows - first < 32 ? rows - first : 32), left = (int)(cols - column < JP * 32 ? cols - column : JP * 32);
+                    if (cols % VEC == 0) {
+                        for (int k = lane; k < live * LANES; k += 64) {
+                            const int row = k / LANES, c = k % LANES;
+                            if (c * VEC < left) *reinterpret_cast<u32x4 *>(to + (int64_t)row * cols + c * VEC) = *reinterpret_cast<const u32x4 *>(mine + row * PITCH + c * 16);
+                        }
+                    } else {
+#pragma unroll 8
+                        for (int k = lane; k < 32 * JP * 32; k += 64) {
+                            const int row = k / (JP * 32), c = k % (JP * 32);
+                            const T o = *reinterpret_cast<const T *>(mine + row * PITCH + c * sizeof(T));
+                            if (row < live && c < left) to[(int64_t)row * cols + c] = o;
+                        }
+                    }
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
+        }
+    };
+    if (cols % VEC != 0 || r0 + S::ROWS > rows || c0 + S::COLS > cols) leave(std::false_type{}, std::false_type{});
+    else if (stream) leave(std::true_type{}, std::true_type{});
+    else leave(std::true_type{}, std::false_type{});
+}
+
 // Workgroup id of `count` -> place in the list of all: an XCD (every eighth id) takes a contiguous run of it.
 __device__ __forceinline__ int place_of(int id, int count)
 {
