@@ -42,29 +42,31 @@ struct NormArgs {
 };
 
 int check_blocks(const char *what, int64_t rows, int64_t n);
-bool wide_rows(const void *p, int64_t ld, int dtype);                   // whether 16-byte vectors of a row lie on their boundaries
 QuantizeJob quantize_job(const void *from, int64_t ld, int64_t rows, int64_t n, void *blocks, bf16_t *expanded, int64_t expanded_pitch);
 int launch_quantize(QuantizeArgs &a, int jobs, int dtype, const char *what, hipStream_t st);
 DequantizeJob dequantize_job(const void *blocks, int64_t rows, int64_t n, void *to, int64_t ld, int64_t columns);
 int launch_dequantize(DequantizeArgs &a, int jobs, int dtype, const char *what, hipStream_t st);
 
 // ------------------------------------------------------------------------------------------------ eight numbers of a lane
-// `left` of them are there (fewer than one: none), zeros in the place of the others
-template <typename T, bool WIDE> __device__ __forceinline__ void load8(const T *from, int64_t left, float (&f)[8])
+// `left` of them are there (fewer than one: none), zeros in the place of the others.  Vectors need not lie on 16-byte boundaries: one load
+// or store takes them from any boundary of their type.
+template <typename T> __device__ __forceinline__ void load8(const T *from, int64_t left, float (&f)[8])
 {
-    if (WIDE && left >= 8) {
+    using V = typename Loose<T>::vector;
+    if (left >= 8) {
 #pragma unroll
-        for (int e = 0; e < 8; e += Elem<T>::VEC) Elem<T>::unpack(*reinterpret_cast<const u32x4 *>(from + e), f + e);
+        for (int e = 0; e < 8; e += Elem<T>::VEC) Elem<T>::unpack(*reinterpret_cast<const V *>(from + e), f + e);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; e++) f[e] = e < left ? Elem<T>::load(from + e) : 0.f;
     }
 }
-template <typename T, bool WIDE> __device__ __forceinline__ void store8(T *to, int64_t left, const float (&f)[8])
+template <typename T> __device__ __forceinline__ void store8(T *to, int64_t left, const float (&f)[8])
 {
-    if (WIDE && left >= 8) {
+    using V = typename Loose<T>::vector;
+    if (left >= 8) {
 #pragma unroll
-        for (int e = 0; e < 8; e += Elem<T>::VEC) *reinterpret_cast<u32x4 *>(to + e) = Elem<T>::pack(f + e);
+        for (int e = 0; e < 8; e += Elem<T>::VEC) *reinterpret_cast<V *>(to + e) = Elem<T>::pack(f + e);
     } else {
 #pragma unroll
         for (int e = 0; e < 8; e++)
@@ -73,34 +75,26 @@ template <typename T, bool WIDE> __device__ __forceinline__ void store8(T *to, i
 }
 
 // the same in two steps, for loads that go out early: as they lie in memory, and as fp32
-template <typename T, bool WIDE> struct Raw8 {
-    u32x4 v[WIDE ? 8 / Elem<T>::VEC : 2];
+template <typename T> struct Raw8 {
+    static constexpr int N = 8 / Elem<T>::VEC;
+    u32x4 v[N];
     __device__ __forceinline__ void load(const T *from, int64_t left)
     {
-        if constexpr (WIDE) {
-            if (left >= 8) {
+        using V = typename Loose<T>::vector;
+        if (left >= 8) {
 #pragma unroll
-                for (int e = 0; e < 8 / Elem<T>::VEC; e++) v[e] = reinterpret_cast<const u32x4 *>(from)[e];
-                return;
-            }
+            for (int e = 0; e < N; e++) v[e] = reinterpret_cast<const V *>(from)[e];
+            return;
         }
         float f[8];
-        load8<T, false>(from, left, f);
-        if constexpr (WIDE) {
+        load8<T>(from, left, f);
 #pragma unroll
-            for (int e = 0; e < 8 / Elem<T>::VEC; e++) v[e] = Elem<T>::pack(f + e * Elem<T>::VEC);
-        } else {
-            v[0] = Elem<float>::pack(f), v[1] = Elem<float>::pack(f + 4);
-        }
+        for (int e = 0; e < N; e++) v[e] = Elem<T>::pack(f + e * Elem<T>::VEC);
     }
     __device__ __forceinline__ void unpack(float (&f)[8]) const
     {
-        if constexpr (WIDE) {
 #pragma unroll
-            for (int e = 0; e < 8 / Elem<T>::VEC; e++) Elem<T>::unpack(v[e], f + e * Elem<T>::VEC);
-        } else {
-            Elem<float>::unpack(v[0], f), Elem<float>::unpack(v[1], f + 4);
-        }
+        for (int e = 0; e < N; e++) Elem<T>::unpack(v[e], f + e * Elem<T>::VEC);
     }
 };
 

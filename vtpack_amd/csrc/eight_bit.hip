@@ -14,7 +14,7 @@
 namespace vtdge {
 
 // ------------------------------------------------------------------------------------------------ blocks
-template <typename T, bool WIDE> __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs p)
+template <typename T> __global__ __launch_bounds__(256) void quantize_kernel(QuantizeArgs p)
 {
     const bool second = blockIdx.x >= p.first;
     const QuantizeJob &job = p.job[second ? 1 : 0];
@@ -28,7 +28,7 @@ template <typename T, bool WIDE> __global__ __launch_bounds__(256) void quantize
         q.scale = job.scales[(int64_t)row * job.scale_pitch + block];
     } else {
         float f[8];
-        load8<T, WIDE>(static_cast<const T *>(job.from) + (int64_t)row * job.ld + c, in ? job.n - c : 0, f);
+        load8<T>(static_cast<const T *>(job.from) + (int64_t)row * job.ld + c, in ? job.n - c : 0, f);
         q = round8(f);
         if (!in) return;
     }
@@ -39,8 +39,8 @@ template <typename T, bool WIDE> __global__ __launch_bounds__(256) void quantize
     if (job.expanded != nullptr && c < job.expanded_pitch) *reinterpret_cast<u32x4 *>(job.expanded + (int64_t)row * job.expanded_pitch + c) = expand8(q.bytes, q.scale);
 }
 
-// blocks -> numbers; VECTOR: whole vectors of a dense row on 16-byte boundaries
-template <typename T, bool VECTOR> __global__ __launch_bounds__(256) void dequantize_kernel(DequantizeArgs p)
+// blocks -> numbers
+template <typename T> __global__ __launch_bounds__(256) void dequantize_kernel(DequantizeArgs p)
 {
     const bool second = blockIdx.x >= p.first;
     const DequantizeJob &job = p.job[second ? 1 : 0];
@@ -50,22 +50,22 @@ template <typename T, bool VECTOR> __global__ __launch_bounds__(256) void dequan
     const int scale = job.scales[(int64_t)row * job.scale_pitch + c / BLOCK];
     float f[8];
     stands_for8(bytes, scale, f);
-    store8<T, VECTOR>(static_cast<T *>(job.to) + (int64_t)row * job.ld + c, (int)job.n - (int)c, f);
+    store8<T>(static_cast<T *>(job.to) + (int64_t)row * job.ld + c, (int)job.n - (int)c, f);
 }
 
 // ------------------------------------------------------------------------------------------------ GELU
-template <typename T, bool WIDE> __global__ __launch_bounds__(256) void gelu_keep_kernel(GeluArgs p)
+template <typename T> __global__ __launch_bounds__(256) void gelu_keep_kernel(GeluArgs p)
 {
     const uint32_t id = blockIdx.x * 16 + (threadIdx.x >> 4), row = id / p.per_row, block = id - row * p.per_row;
     const int part = threadIdx.x & 15, c = (int)block * BLOCK + part * 8;
     const bool in = row < p.rows;
     float f[8], y[8];
-    load8<T, WIDE>(static_cast<const T *>(p.x) + (int64_t)row * p.ld + c, in ? p.n - c : 0, f);
+    load8<T>(static_cast<const T *>(p.x) + (int64_t)row * p.ld + c, in ? p.n - c : 0, f);
 #pragma unroll
     for (int e = 0; e < 8; e++) y[e] = gelu_fn<T>(f[e]);
     const Rounded q = round8(f);
     if (!in) return;
-    store8<T, WIDE>(static_cast<T *>(p.y) + (int64_t)row * p.n + c, p.n - c, y);
+    store8<T>(static_cast<T *>(p.y) + (int64_t)row * p.n + c, p.n - c, y);
     if (p.values == nullptr) return;
     *reinterpret_cast<u32x2 *>(p.values + (int64_t)row * p.value_pitch + c) = q.bytes;
     if (part == 0) put_scale(p.scales + (int64_t)row * p.scale_pitch, (int)block, (int)p.per_row, p.scale_pitch, q.scale);
@@ -105,12 +105,12 @@ template <> __device__ __forceinline__ float gelu_slope<bf16_t>(float v)
     q = __builtin_fmaf(q, t, 7.973323464e-01f);
     return __builtin_fmaf(x, q, 0.5f);
 }
-template <typename T, bool WIDE> __global__ __launch_bounds__(256) void gelu_slope_kernel(GeluArgs p)
+template <typename T> __global__ __launch_bounds__(256) void gelu_slope_kernel(GeluArgs p)
 {
     const uint32_t id = blockIdx.x * 256 + threadIdx.x, row = id / p.per_row, c = (id - row * p.per_row) * 8;
     if (row >= p.rows) return;
     float g[8], x[8];
-    load8<T, WIDE>(static_cast<const T *>(p.x) + (int64_t)row * p.ld + c, p.n - (int)c, g);
+    load8<T>(static_cast<const T *>(p.x) + (int64_t)row * p.ld + c, p.n - (int)c, g);
     const u32x2 bytes = *reinterpret_cast<const u32x2 *>(p.values + (int64_t)row * p.value_pitch + c);
     const int scale = p.scales[(int64_t)row * p.scale_pitch + c / BLOCK];
     stands_for8(bytes, scale, x);
@@ -119,7 +119,7 @@ template <typename T, bool WIDE> __global__ __launch_bounds__(256) void gelu_slo
     if (any_nan(bytes, scale))                      // rare
 #pragma unroll
         for (int e = 0; e < 8; e++) g[e] = x[e] == x[e] ? g[e] : x[e];
-    store8<T, WIDE>(static_cast<T *>(p.y) + (int64_t)row * p.n + c, p.n - (int)c, g);
+    store8<T>(static_cast<T *>(p.y) + (int64_t)row * p.n + c, p.n - (int)c, g);
 }
 
 // ------------------------------------------------------------------------------------------------ LayerNorm
@@ -148,7 +148,7 @@ template <int WAVES, int NV, typename V> __device__ __forceinline__ void row_sum
 
 // The mean is the fp32 number next to the exact one, so that what is rounded to 8 bits behind it does not hang on the order of a sum:
 // the sum is taken in 64 bits.
-template <typename T, int WAVES, int CH, bool WIDE> __global__ __launch_bounds__(256) void norm_keep_kernel(NormArgs p)
+template <typename T, int WAVES, int CH> __global__ __launch_bounds__(256) void norm_keep_kernel(NormArgs p)
 {
     __shared__ double sums64[WAVES][1];
     __shared__ float sums32[WAVES][1];
@@ -160,7 +160,7 @@ template <typename T, int WAVES, int CH, bool WIDE> __global__ __launch_bounds__
 #pragma unroll
     for (int k = 0; k < CH; k++) {
         const int c = norm_column<WAVES>(k);
-        load8<T, WIDE>(static_cast<const T *>(p.x) + row * p.ld + c, p.n - c, f[k]);
+        load8<T>(static_cast<const T *>(p.x) + row * p.ld + c, p.n - c, f[k]);
 #pragma unroll
         for (int e = 0; e < 8; e++) sum[0] += (double)f[k][e];
     }
@@ -189,11 +189,11 @@ template <typename T, int WAVES, int CH, bool WIDE> __global__ __launch_bounds__
         }
         if (left <= 0) continue;
         float w[8], b[8];
-        load8<T, WIDE>(static_cast<const T *>(p.weight) + c, left, w);
-        load8<T, WIDE>(static_cast<const T *>(p.bias) + c, left, b);
+        load8<T>(static_cast<const T *>(p.weight) + c, left, w);
+        load8<T>(static_cast<const T *>(p.bias) + c, left, b);
 #pragma unroll
         for (int e = 0; e < 8; e++) f[k][e] = __builtin_fmaf(f[k][e] * r, w[e], b[e]);
-        store8<T, WIDE>(static_cast<T *>(p.y) + row * p.n + c, left, f[k]);
+        store8<T>(static_cast<T *>(p.y) + row * p.n + c, left, f[k]);
     }
 }
 
@@ -204,7 +204,7 @@ template <typename T, int WAVES, int CH, bool WIDE> __global__ __launch_bounds__
 template <int WAVES> struct NormSlope {
     static constexpr int THREADS = WAVES < 4 ? 256 : WAVES * 64, ROWS = THREADS / 64 / WAVES;      // rows at once
 };
-template <typename T, int WAVES, bool WIDE> __global__ __launch_bounds__(NormSlope<WAVES>::THREADS) void norm_slope_kernel(NormArgs p)
+template <typename T, int WAVES> __global__ __launch_bounds__(NormSlope<WAVES>::THREADS) void norm_slope_kernel(NormArgs p)
 {
     using S = NormSlope<WAVES>;
     constexpr int ROWS = S::ROWS;
@@ -212,12 +212,12 @@ template <typename T, int WAVES, bool WIDE> __global__ __launch_bounds__(NormSlo
     extern __shared__ __attribute__((aligned(16))) float columns[];        // [2][n], joining ROWS > 1
     const int c = (threadIdx.x & (WAVES * 64 - 1)) * 8, left = p.n - c, group = threadIdx.x / (WAVES * 64);
     float w[8], dw[8], db[8];
-    load8<T, WIDE>(static_cast<const T *>(p.weight) + c, left, w);
+    load8<T>(static_cast<const T *>(p.weight) + c, left, w);
 #pragma unroll
     for (int e = 0; e < 8; e++) dw[e] = db[e] = 0.f;
     const float inv_n = 1.0f / (float)p.n;
     struct Row {
-        Raw8<T, WIDE> g;
+        Raw8<T> g;
         u32x2 bytes;
         int scale;
         float r;
@@ -258,7 +258,7 @@ template <typename T, int WAVES, bool WIDE> __global__ __launch_bounds__(NormSlo
         const float m0 = s[0] * inv_n, m1 = s[1] * inv_n;
 #pragma unroll
         for (int e = 0; e < 8; e++) g[e] = now.r * (g[e] - m0 - h[e] * m1);
-        if (row < p.rows) store8<T, WIDE>(static_cast<T *>(p.y) + row * p.n + c, left, g);
+        if (row < p.rows) store8<T>(static_cast<T *>(p.y) + row * p.n + c, left, g);
     }
     if (p.part == nullptr) return;
     float *const part = p.part + (int64_t)blockIdx.x * 2 * p.n;
@@ -306,8 +306,6 @@ int check_blocks(const char *what, int64_t rows, int64_t n)
                (long long)rows, (long long)n);
     return VTDGE_OK;
 }
-bool wide_rows(const void *p, int64_t ld, int dtype) { return ((uintptr_t)p & 15) == 0 && ld % (dtype == VTDGE_F32 ? 4 : 8) == 0; }
-
 QuantizeJob quantize_job(const void *from, int64_t ld, int64_t rows, int64_t n, void *blocks, bf16_t *expanded, int64_t expanded_pitch)
 {
     QuantizeJob j{};
@@ -320,15 +318,12 @@ QuantizeJob quantize_job(const void *from, int64_t ld, int64_t rows, int64_t n, 
 int launch_quantize(QuantizeArgs &a, int jobs, int dtype, const char *what, hipStream_t st)
 {
     int64_t blocks = 0;
-    bool wide = true;
     for (int i = 0; i < jobs; i++) {
         blocks += ceil_div((int64_t)a.job[i].rows * a.job[i].per_row, 16);
         if (i == 0) a.first = (uint32_t)blocks;
-        wide = wide && wide_rows(a.job[i].from, a.job[i].rows > 1 ? a.job[i].ld : 0, dtype);
     }
     VT_REQUIRE(blocks < (1ll << 31), VTDGE_ERR_UNSUPPORTED, "%s: %lld blocks", what, (long long)blocks);
-    auto kern = dtype == VTDGE_F32 ? (wide ? quantize_kernel<float, true> : quantize_kernel<float, false>)
-                                   : (wide ? quantize_kernel<bf16_t, true> : quantize_kernel<bf16_t, false>);
+    auto kern = dtype == VTDGE_F32 ? quantize_kernel<float> : quantize_kernel<bf16_t>;
     note_kernel(reinterpret_cast<const void *>(kern));
     kern<<<(unsigned)blocks, 256, 0, st>>>(a);
     return check_launch(what);
@@ -343,15 +338,12 @@ DequantizeJob dequantize_job(const void *blocks, int64_t rows, int64_t n, void *
 int launch_dequantize(DequantizeArgs &a, int jobs, int dtype, const char *what, hipStream_t st)
 {
     int64_t blocks = 0;
-    bool wide = true;
     for (int i = 0; i < jobs; i++) {
         blocks += ceil_div((int64_t)a.job[i].rows * a.job[i].per_row, 256);
         if (i == 0) a.first = (uint32_t)blocks;
-        wide = wide && wide_rows(a.job[i].to, a.job[i].rows > 1 ? a.job[i].ld : 0, dtype);
     }
     VT_REQUIRE(blocks < (1ll << 31), VTDGE_ERR_UNSUPPORTED, "%s: %lld blocks", what, (long long)blocks);
-    auto kern = dtype == VTDGE_F32 ? (wide ? dequantize_kernel<float, true> : dequantize_kernel<float, false>)
-                                   : (wide ? dequantize_kernel<bf16_t, true> : dequantize_kernel<bf16_t, false>);
+    auto kern = dtype == VTDGE_F32 ? dequantize_kernel<float> : dequantize_kernel<bf16_t>;
     note_kernel(reinterpret_cast<const void *>(kern));
     kern<<<(unsigned)blocks, 256, 0, st>>>(a);
     return check_launch(what);
@@ -384,13 +376,12 @@ static int64_t norm_parts(int64_t rows, int n)
     return all < most ? all : most;
 }
 
-#define VT_NORM_CASE(T, WIDE)                                                                                               \
-    (waves == 1 ? (ch == 1 ? norm_keep_kernel<T, 1, 1, WIDE> : norm_keep_kernel<T, 1, 2, WIDE>)                             \
-                : (ch == 1 ? norm_keep_kernel<T, 4, 1, WIDE> : ch == 2 ? norm_keep_kernel<T, 4, 2, WIDE> : norm_keep_kernel<T, 4, 4, WIDE>))
-#define VT_SLOPE_CASE(T, WIDE)                                                                                              \
-    (waves == 1 ? norm_slope_kernel<T, 1, WIDE> : waves == 2 ? norm_slope_kernel<T, 2, WIDE>                                \
-     : waves == 4 ? norm_slope_kernel<T, 4, WIDE> : waves == 8 ? norm_slope_kernel<T, 8, WIDE> : norm_slope_kernel<T, 16, WIDE>)
-#define VT_NORM_KERNEL(CASE) (dtype == VTDGE_F32 ? (wide ? CASE(float, true) : CASE(float, false)) : (wide ? CASE(bf16_t, true) : CASE(bf16_t, false)))
+#define VT_NORM_CASE(T)                                                                                         \
+    (waves == 1 ? (ch == 1 ? norm_keep_kernel<T, 1, 1> : norm_keep_kernel<T, 1, 2>)                             \
+                : (ch == 1 ? norm_keep_kernel<T, 4, 1> : ch == 2 ? norm_keep_kernel<T, 4, 2> : norm_keep_kernel<T, 4, 4>))
+#define VT_SLOPE_CASE(T)                                                                                        \
+    (waves == 1 ? norm_slope_kernel<T, 1> : waves == 2 ? norm_slope_kernel<T, 2>                                \
+     : waves == 4 ? norm_slope_kernel<T, 4> : waves == 8 ? norm_slope_kernel<T, 8> : norm_slope_kernel<T, 16>)
 
 static int check_norm(const char *what, int64_t rows, int64_t n, int dtype)
 {
@@ -445,16 +436,13 @@ static int gelu_args(const char *what, GeluArgs &a, const void *x, int64_t ldx, 
     a.value_pitch = value_pitch(n), a.scale_pitch = (int)scale_pitch(n);
     return VTDGE_OK;
 }
-static bool gelu_wide(const GeluArgs &a, int dtype) { return wide_rows(a.x, a.rows > 1 ? a.ld : 0, dtype) && wide_rows(a.y, a.rows > 1 ? a.n : 0, dtype); }
 
 extern "C" int vtdge_gelu_8bit(const void *x, int64_t ldx, int64_t rows, int64_t n, void *y, void *blocks, int dtype, void *stream)
 {
     GeluArgs a{};
     VT_STEP(gelu_args("gelu_8bit", a, x, ldx, rows, n, blocks, y, dtype));
     a.per_row = (uint32_t)ceil_div(n, BLOCK);
-    const bool wide = gelu_wide(a, dtype);
-    auto kern = dtype == VTDGE_F32 ? (wide ? gelu_keep_kernel<float, true> : gelu_keep_kernel<float, false>)
-                                   : (wide ? gelu_keep_kernel<bf16_t, true> : gelu_keep_kernel<bf16_t, false>);
+    auto kern = dtype == VTDGE_F32 ? gelu_keep_kernel<float> : gelu_keep_kernel<bf16_t>;
     note_kernel(reinterpret_cast<const void *>(kern));
     kern<<<(unsigned)ceil_div(rows * a.per_row, 16), 256, 0, (hipStream_t)stream>>>(a);
     return check_launch("gelu_8bit");
@@ -466,9 +454,7 @@ extern "C" int vtdge_gelu_8bit_backward(const void *grad, int64_t ldg, int64_t r
     VT_STEP(gelu_args("gelu_8bit_backward", a, grad, ldg, rows, n, blocks, dx, dtype));
     VT_REQUIRE(blocks, VTDGE_ERR_ARG, "gelu_8bit_backward: NULL operand");
     a.per_row = (uint32_t)ceil_div(n, 8);
-    const bool wide = gelu_wide(a, dtype);
-    auto kern = dtype == VTDGE_F32 ? (wide ? gelu_slope_kernel<float, true> : gelu_slope_kernel<float, false>)
-                                   : (wide ? gelu_slope_kernel<bf16_t, true> : gelu_slope_kernel<bf16_t, false>);
+    auto kern = dtype == VTDGE_F32 ? gelu_slope_kernel<float> : gelu_slope_kernel<bf16_t>;
     note_kernel(reinterpret_cast<const void *>(kern));
     kern<<<(unsigned)ceil_div(rows * a.per_row, 256), 256, 0, (hipStream_t)stream>>>(a);
     return check_launch("gelu_8bit_backward");
@@ -488,8 +474,7 @@ extern "C" int vtdge_layernorm_8bit(const void *x, int64_t ldx, const void *weig
     a.blocks = (int)ceil_div(n, BLOCK);
     int waves, ch;
     norm_shape((int)n, waves, ch);
-    const bool wide = wide_rows(x, rows > 1 ? ldx : 0, dtype) && wide_rows(y, rows > 1 ? n : 0, dtype) && wide_rows(weight, 0, dtype) && wide_rows(bias, 0, dtype);
-    auto kern = VT_NORM_KERNEL(VT_NORM_CASE);
+    auto kern = dtype == VTDGE_F32 ? VT_NORM_CASE(float) : VT_NORM_CASE(bf16_t);
     note_kernel(reinterpret_cast<const void *>(kern));
     kern<<<(unsigned)ceil_div(rows, 4 / waves), 256, 0, (hipStream_t)stream>>>(a);
     return check_launch("layernorm_8bit");
@@ -519,8 +504,7 @@ extern "C" int vtdge_layernorm_8bit_backward(const void *grad, int64_t ldg, cons
     a.values = values_of(blocks), a.scales = scales_of(blocks, rows, n), a.value_pitch = (int)value_pitch(n), a.scale_pitch = (int)scale_pitch(n);
     a.part = columns ? static_cast<float *>(workspace) : nullptr;
     const int waves = slope_waves((int)n);
-    const bool wide = wide_rows(grad, rows > 1 ? ldg : 0, dtype) && (dx == nullptr || wide_rows(dx, rows > 1 ? n : 0, dtype)) && wide_rows(weight, 0, dtype);
-    auto kern = VT_NORM_KERNEL(VT_SLOPE_CASE);
+    auto kern = dtype == VTDGE_F32 ? VT_SLOPE_CASE(float) : VT_SLOPE_CASE(bf16_t);
     note_kernel(reinterpret_cast<const void *>(kern));
     kern<<<(unsigned)parts, waves < 4 ? 256 : waves * 64, waves < 4 ? 2 * n * 4 : 0, (hipStream_t)stream>>>(a);
     VT_STEP(check_launch("layernorm_8bit_backward"));

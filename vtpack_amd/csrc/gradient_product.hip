@@ -211,18 +211,25 @@ static int64_t makespan(int64_t slots, int64_t n1, int64_t l1, int64_t n2, int64
 struct GradShape {
     int grads, m, n, slab;
     double us, tile_us;                             // of a slab, of an epilogue
+    int per_cu;                                     // tiles side by side on a compute unit, `us` for all of them there
+    double us_alone;
 };
 static double cuts(GradPlan &p, int64_t rows, int64_t of_piece, int width, const GradShape &s, bool choose)
 {
     const int64_t cu = compute_units(), across = ceil_div(width, s.n);
     const int64_t tx = ceil_div(rows, s.m) * across, tw = ceil_div(of_piece, s.m) * across, sx = ceil_div(of_piece, s.slab), sw = ceil_div(rows, s.slab);
-    const int64_t extra = (int64_t)(s.tile_us / s.us + 0.5);
     double best = 1e30;
     for (int64_t x = 1; x <= 32 && (x == 1 || sx / x >= 8); x++)
         for (int64_t w = 1; w <= 32 && (w == 1 || sw / w >= 8); w++) {
             if ((x > 1 && tx * x > 8 * cu) || (w > 1 && tw * w > 8 * cu)) continue;
             const double bytes = ((x > 1 ? 8.0 * x * rows : 0.0) + (w > 1 ? 8.0 * w * of_piece : 0.0)) * width;
-            const double t = s.us * makespan(cu, tx * x, ceil_div(sx, x) + extra, tw * w, ceil_div(sw, w) + extra) + bytes / 4e6 + (x > 1 || w > 1 ? 5.0 : 0.0);
+            double us = s.us;
+            if (s.per_cu > 1) {                     // few tiles have a compute unit, or more of one, to themselves
+                const double beside = (double)(tx * x + tw * w) / (double)cu - 1.0;
+                us = s.us_alone + (s.us - s.us_alone) * (beside < 0.0 ? 0.0 : beside > s.per_cu - 1 ? 1.0 : beside / (s.per_cu - 1));
+            }
+            const int64_t extra = (int64_t)(s.tile_us / us + 0.5);
+            const double t = us * makespan(cu * s.per_cu, tx * x, ceil_div(sx, x) + extra, tw * w, ceil_div(sw, w) + extra) + bytes / 4e6 + (x > 1 || w > 1 ? 5.0 : 0.0);
             if (t >= best) continue;
             best = t;
             if (choose) p.dx_splits = (int)x, p.dw_splits = (int)w;
@@ -230,7 +237,10 @@ static double cuts(GradPlan &p, int64_t rows, int64_t of_piece, int width, const
     if (choose) p.grads = s.grads, p.gm = s.m, p.gn = s.n, p.slab_g = s.slab;
     return best;
 }
-template <class S> static GradShape grad_shape(int grads, double us, double tile_us) { return GradShape{grads, S::ROWS, S::COLS, S::SLAB, us, tile_us}; }
+template <class S> static GradShape grad_shape(int grads, double us, double tile_us, int per_cu = 1, double us_alone = 0.0)
+{
+    return GradShape{grads, S::ROWS, S::COLS, S::SLAB, us, tile_us, per_cu, us_alone};
+}
 
 #ifndef VT_FORCE
 #define VT_FORCE -1
@@ -238,7 +248,8 @@ template <class S> static GradShape grad_shape(int grads, double us, double tile
 void plan_gradients(GradPlan &p, int64_t rows, int64_t of_piece, int width, bool split, bool ends)
 {
     if (ends) {
-        const GradShape shapes[4] = {grad_shape<GradLarge>(GRAD_LARGE, 2.0, 6.0), grad_shape<GradMiddle>(GRAD_MIDDLE, 1.3, 4.0), grad_shape<GradSquare>(GRAD_SQUARE, 0.65, 2.5), grad_shape<GradSmall>(GRAD_SMALL, 0.35, 1.4)};
+        const GradShape shapes[4] = {grad_shape<GradLarge>(GRAD_LARGE, 1.9, 5.0), grad_shape<GradMiddle>(GRAD_MIDDLE, 1.1, 3.0), grad_shape<GradSquare>(GRAD_SQUARE, 1.4, 2.0, 2, 0.8),
+                                     grad_shape<GradSmall>(GRAD_SMALL, 0.8, 1.0, 3, 0.65)};
         int best = 0;
         double least = 1e30;
         for (int k = 0; k < 4; k++) {

@@ -173,7 +173,7 @@ template <typename T> static constexpr int few_lds(int rows, int64_t pitch, int 
 {
     return (int)(rows * pitch * (sizeof(T) == 2 ? 1 : 2)) + (rows * scales + 15) / 16 * 16 + 4 * 64 * 16;
 }
-template <typename T, bool WIDE, bool GELU> __global__ __launch_bounds__(256) void linear_8bit_few_kernel(FewArgs p)
+template <typename T, bool GELU> __global__ __launch_bounds__(256) void linear_8bit_few_kernel(FewArgs p)
 {
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     constexpr bool EIGHT = sizeof(T) == 2;
@@ -208,7 +208,7 @@ template <typename T, bool WIDE, bool GELU> __global__ __launch_bounds__(256) vo
         const int id = first + (threadIdx.x >> 4), row = id / blocks, block = id - row * blocks, c = block * BLOCK + at16 * 8;
         const bool in = id < p.rows * blocks;
         float f[8];
-        load8<T, WIDE>(static_cast<const T *>(p.x) + (int64_t)row * p.ldx + c, in ? p.width - c : 0, f);
+        load8<T>(static_cast<const T *>(p.x) + (int64_t)row * p.ldx + c, in ? p.width - c : 0, f);
         const Rounded q = round8(f);
         if (!in) continue;
         if constexpr (EIGHT) {
@@ -268,27 +268,31 @@ template <typename T, bool WIDE, bool GELU> __global__ __launch_bounds__(256) vo
     }
 }
 
-// Rows of g as the products read them: bf16, filled up with zeros to whole slabs.
-template <typename T, bool WIDE> __global__ __launch_bounds__(256) void pack_gradient_kernel(const T *from, int64_t ld, uint32_t rows, int n, uint32_t per_row, bf16_t *to)
-{
-    const uint32_t id = blockIdx.x * 256 + threadIdx.x, row = id / per_row, c = (id - row * per_row) * 8;
-    if (row >= rows) return;
-    float f[8];
-    load8<T, WIDE>(from + (int64_t)row * ld + c, n - (int)c, f);
-    *reinterpret_cast<u32x4 *>(to + ((int64_t)row * per_row * 8 + c)) = Elem<bf16_t>::pack(f);
-}
-
 // Blocks [rows, n] as bf16 [n, pitch], zeros behind the rows: what both gradients multiply lies along their sums then, and is read from LDS
 // in 16 bytes a lane (transposed by the LDS reads, 32768 x 1024 x 4096: 605 us in place of VT_GRAD_US).
 struct ExpandJob {
     const unsigned char *values, *scales; uint32_t rows, down; int64_t value_pitch; int scale_pitch, n; bf16_t *to; int64_t pitch;     // down: tiles of 64 rows
 };
-struct ExpandArgs {
-    ExpandJob job[2];
-    uint32_t first;
+// Rows of g: bf16, filled up with zeros to whole slabs.
+struct PackJob {
+    const void *from; int64_t ld; uint32_t rows, per_row; int n; bf16_t *to;      // per_row: vectors of eight; rows 0: g lies as it is read
 };
-__global__ __launch_bounds__(256) void expand_kernel(ExpandArgs p)
+struct PrepareArgs {
+    ExpandJob job[2];
+    PackJob pack;
+    uint32_t first, second;                         // workgroups of the first, of both
+};
+template <typename T> __global__ __launch_bounds__(256) void prepare_gradients_kernel(PrepareArgs p)
 {
+    if (blockIdx.x >= p.second) {
+        const PackJob &g = p.pack;
+        const uint32_t id = (blockIdx.x - p.second) * 256 + threadIdx.x, row = id / g.per_row, c = (id - row * g.per_row) * 8;
+        if (row >= g.rows) return;
+        float f[8];
+        load8<T>(static_cast<const T *>(g.from) + (int64_t)row * g.ld + c, g.n - (int)c, f);
+        *reinterpret_cast<u32x4 *>(g.to + ((int64_t)row * g.per_row * 8 + c)) = Elem<bf16_t>::pack(f);
+        return;
+    }
     constexpr int PITCH = 36;                       // words of a column, two rows each
     __shared__ __attribute__((aligned(16))) uint32_t tile[BLOCK * PITCH];
     const bool second = blockIdx.x >= p.first;
@@ -412,10 +416,7 @@ extern "C" int64_t vtdge_linear_8bit_workspace(int64_t rows, int64_t out, int64_
 
 template <typename T> static int go_few(const FewArgs &a, int act, hipStream_t st)
 {
-    const int dtype = sizeof(T) == 2 ? VTDGE_BF16 : VTDGE_F32;
-    const bool wide = wide_rows(a.x, a.rows > 1 ? a.ldx : 0, dtype), gelu = act == VTDGE_ACT_GELU;
-    auto kern = wide ? (gelu ? linear_8bit_few_kernel<T, true, true> : linear_8bit_few_kernel<T, true, false>)
-                     : (gelu ? linear_8bit_few_kernel<T, false, true> : linear_8bit_few_kernel<T, false, false>);
+    auto kern = act == VTDGE_ACT_GELU ? linear_8bit_few_kernel<T, true> : linear_8bit_few_kernel<T, false>;
     note_kernel(reinterpret_cast<const void *>(kern));
     kern<<<(unsigned)ceil_div(a.out, 16), 256, few_lds<T>(a.rows, value_pitch(a.width), a.scale_pitch), st>>>(a);
     return check_launch("linear_8bit");
@@ -505,21 +506,7 @@ extern "C" int vtdge_linear_8bit_backward(const void *grad, int64_t ldg, const v
     const hipStream_t st = (hipStream_t)stream;
     bf16_t *const xb = (bf16_t *)(ws + p.x_at), *const wb = (bf16_t *)(ws + p.w_at);
     Operand g_op{(const bf16_t *)grad, rows > 1 ? ldg : out, 0};
-    if (!lies) {
-        bf16_t *const to = (bf16_t *)(ws + p.g_at);
-        const uint32_t per_row = (uint32_t)(padded(out) / 8);
-        const unsigned blocks = (unsigned)ceil_div(rows * per_row, 256);
-        const bool wide = wide_rows(grad, rows > 1 ? ldg : 0, dtype);
-        auto go = [&](auto kern, auto *from) {
-            note_kernel(reinterpret_cast<const void *>(kern));
-            kern<<<blocks, 256, 0, st>>>(from, ldg, (uint32_t)rows, (int)out, per_row, to);
-            return check_launch("linear_8bit_backward");
-        };
-        if (dtype == VTDGE_F32) VT_STEP(wide ? go(pack_gradient_kernel<float, true>, (const float *)grad) : go(pack_gradient_kernel<float, false>, (const float *)grad));
-        else VT_STEP(wide ? go(pack_gradient_kernel<bf16_t, true>, (const bf16_t *)grad) : go(pack_gradient_kernel<bf16_t, false>, (const bf16_t *)grad));
-        g_op = Operand{to, padded(out), 0};
-    }
-    ExpandArgs d{};
+    PrepareArgs d{};
     int jobs = 0;
     int64_t tiles = 0;
     auto expand = [&](const void *blocks, int64_t r, bf16_t *to) {
@@ -531,9 +518,18 @@ extern "C" int vtdge_linear_8bit_backward(const void *grad, int64_t ldg, const v
     };
     if (dx != nullptr) expand(w_blocks, out, wb);
     if (dweight != nullptr) expand(x_blocks, rows, xb);
-    if (jobs > 0) {
-        note_kernel(reinterpret_cast<const void *>(expand_kernel));
-        expand_kernel<<<(unsigned)tiles, 256, 0, st>>>(d);
+    d.second = (uint32_t)tiles;
+    if (!lies) {
+        bf16_t *const to = (bf16_t *)(ws + p.g_at);
+        d.pack = PackJob{grad, ldg, (uint32_t)rows, (uint32_t)(padded(out) / 8), (int)out, to};
+        tiles += ceil_div(rows * d.pack.per_row, 256);
+        g_op = Operand{to, padded(out), 0};
+    }
+    VT_REQUIRE(tiles < (1ll << 31), VTDGE_ERR_UNSUPPORTED, "linear_8bit_backward: %lld rows of %lld and %lld", (long long)rows, (long long)width, (long long)out);
+    if (tiles > 0) {
+        auto kern = dtype == VTDGE_F32 ? prepare_gradients_kernel<float> : prepare_gradients_kernel<bf16_t>;
+        note_kernel(reinterpret_cast<const void *>(kern));
+        kern<<<(unsigned)tiles, 256, 0, st>>>(d);
         VT_STEP(check_launch("linear_8bit_backward"));
     }
     GradPair g{};

@@ -11,6 +11,12 @@ namespace vtdge {
 
 __device__ __forceinline__ int wave_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// 16 bytes on any boundary of their elements' type
+typedef u32x4 u32x4_on2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_on4 __attribute__((aligned(4)));
+template <typename T> struct Loose { typedef u32x4_on4 vector; };
+template <> struct Loose<bf16_t> { typedef u32x4_on2 vector; };
+
 // ------------------------------------------------------------------------------------------------ the product of a tile
 // A bf16 matrix, or the three parts of an fp32 one `plane` elements apart.
 struct Operand {
@@ -212,6 +218,7 @@ __device__ __forceinline__ void put_tile(unsigned char *smem, const f32x16 (&acc
     static_assert(S::WAVES * 32 * PITCH <= S::RING, "LDS");
     const int lane = threadIdx.x & 63, lr = lane & 31, lg = lane >> 5;
     const int wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
+    using V = typename Loose<T>::vector;             // (rows of any length)
     unsigned char *const mine = smem + wid * 32 * PITCH;
     auto leave = [&](auto WHOLE, auto STREAM) {
         constexpr bool whole = decltype(WHOLE)::value, past = decltype(STREAM)::value;
@@ -252,32 +259,29 @@ __device__ __forceinline__ void put_tile(unsigned char *smem, const f32x16 (&acc
 #pragma unroll
                     for (int k = 0; k < TIMES; k++) {
                         const u32x4 o = *reinterpret_cast<const u32x4 *>(mine + (row + k * (64 / LANES)) * PITCH + c * 16);
-                        u32x4 *const at = reinterpret_cast<u32x4 *>(from + (int64_t)k * (64 / LANES) * cols);
-                        if constexpr (past) __builtin_nontemporal_store(o, at);
-                        else *at = o;
+                        T *const at = from + (int64_t)k * (64 / LANES) * cols;
+                        if constexpr (past) __builtin_nontemporal_store(o, reinterpret_cast<u32x4 *>(at));
+                        else *reinterpret_cast<V *>(at) = o;
                     }
                 } else {
                     const int live = (int)(rows - first < 32 ? rows - first : 32), left = (int)(cols - column < JP * 32 ? cols - column : JP * 32);
-                    if (cols % VEC == 0) {
-                        for (int k = lane; k < live * LANES; k += 64) {
-                            const int row = k / LANES, c = k % LANES;
-                            if (c * VEC < left) *reinterpret_cast<u32x4 *>(to + (int64_t)row * cols + c * VEC) = *reinterpret_cast<const u32x4 *>(mine + row * PITCH + c * 16);
-                        }
-                    } else {
 #pragma unroll 8
-                        for (int k = lane; k < 32 * JP * 32; k += 64) {
-                            const int row = k / (JP * 32), c = k % (JP * 32);
-                            const T o = *reinterpret_cast<const T *>(mine + row * PITCH + c * sizeof(T));
-                            if (row < live && c < left) to[(int64_t)row * cols + c] = o;
-                        }
+                    for (int k = lane; k < 32 * LANES; k += 64) {
+                        const int row = k / LANES, c = k % LANES * VEC;
+                        const u32x4 o = *reinterpret_cast<const u32x4 *>(mine + row * PITCH + c * sizeof(T));
+                        if (row >= live || c >= left) continue;
+                        T *const at = to + (int64_t)row * cols + c;
+                        if (c + VEC <= left) *reinterpret_cast<V *>(at) = o;
+                        else
+                            for (int e = 0; e < left - c; e++) at[e] = *reinterpret_cast<const T *>(mine + row * PITCH + (c + e) * sizeof(T));
                     }
                 }
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             }
         }
     };
-    if (cols % VEC != 0 || r0 + S::ROWS > rows || c0 + S::COLS > cols) leave(std::false_type{}, std::false_type{});
-    else if (stream) leave(std::true_type{}, std::true_type{});
+    if (r0 + S::ROWS > rows || c0 + S::COLS > cols) leave(std::false_type{}, std::false_type{});
+    else if (stream && cols % VEC == 0) leave(std::true_type{}, std::true_type{});
     else leave(std::true_type{}, std::false_type{});
 }
 
