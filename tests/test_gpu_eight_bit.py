@@ -553,3 +553,83 @@ def test_refusals_on_the_gpu(dev):
         with torch.autograd.forward_ad.dual_level():
             with pytest.raises(RuntimeError, match="forward-mode"):
                 op(torch.autograd.forward_ad.make_dual(x, x))
+
+
+# ------------------------------------------------------------------------------------------------ in the models
+def _deit(dev, **kw):
+    from vtpack_amd.models.dge.deit_dge import VisionTransformer
+    from vtpack_amd.synthetic import set_synthetic_router
+    torch.manual_seed(0)
+    m = VisionTransformer(img_size=64, patch_size=8, embed_dim=64, depth=2, num_heads=1, mlp_ratio=2, num_classes=7, split_sizes=[4, 2, 1], **kw)
+    return set_synthetic_router(m, 2).to(dev).train()
+
+
+def _pvt(dev):
+    from vtpack_amd.models.dge.pvt_dge import PyramidVisionTransformer
+    torch.manual_seed(0)
+    return PyramidVisionTransformer(img_size=128, patch_size=4, num_classes=9, embed_dims=[64, 64, 64, 64], num_heads=[1, 1, 1, 1], mlp_ratios=[2] * 4,
+                                    depths=[1, 1, 1, 1], sr_ratios=[8, 4, 2, 1], split_sizes=[[4, 2, 1]] * 4, qkv_bias=True).to(dev).train()
+
+
+def _saved_bytes(run):
+    """Bytes of the distinct tensors on the GPU that a pass saves for its gradients."""
+    from torch.autograd.graph import saved_tensors_hooks
+    seen = {}
+
+    def pack(t):
+        if t.is_cuda:
+            seen[t.untyped_storage().data_ptr()] = t.untyped_storage().nbytes()
+        return t
+    with saved_tensors_hooks(pack, lambda t: t):
+        out = run()
+    return out, sum(seen.values())
+
+
+@pytest.mark.parametrize("make,size", [(_deit, 64), (_pvt, 128)])
+def test_training_pass_of_a_model(dev, make, size):
+    """The same pass in 8 bits: a loss and gradients beside the full ones', fewer bytes kept, eval mode as it was."""
+    from vtpack_amd.synthetic import synthetic_images
+    m = make(dev)
+    images, target = synthetic_images(4, size, seed=1).to(dev), torch.tensor([1, 0, 3, 2], device=dev)
+    runs = []
+    for on in (False, True):
+        m.set_eight_bit(on)
+        torch.manual_seed(5)                              # the gates are sampled
+        loss, kept = _saved_bytes(lambda: m(images, target))
+        m.zero_grad(set_to_none=True)
+        loss.backward()
+        runs.append((float(loss.detach()), {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}, kept))
+    (loss, grads, kept), (loss8, grads8, kept8) = runs
+    assert grads.keys() == grads8.keys() and kept8 < 0.8 * kept
+    assert loss8 != loss and abs(loss8 - loss) <= 0.1 * loss
+    for n in grads:
+        assert torch.isfinite(grads8[n]).all(), n
+    whole = [torch.cat([g[n].flatten() for n in grads if "dge.router" not in n]) for g in (grads, grads8)]
+    assert float(torch.nn.functional.cosine_similarity(*whole, dim=0)) > 0.9
+    m.eval()
+    with torch.no_grad():
+        a = m(images)
+        m.set_eight_bit(False)
+        assert torch.equal(a, m(images))
+
+
+def test_steps_of_a_model_in_eight_bits(dev):
+    """Training steps with the harness: weights move, and the same bits twice."""
+    from vtpack_amd import harness
+    from vtpack_amd.optim import AdamW
+    from vtpack_amd.synthetic import synthetic_images
+    images, target = synthetic_images(4, 64, seed=1).to(dev), torch.tensor([1, 0, 3, 2], device=dev)
+    ends = []
+    for _ in range(2):
+        m = _deit(dev).set_eight_bit()
+        before = {n: p.detach().clone() for n, p in m.named_parameters()}
+        opt = AdamW(harness.weight_decay_groups(m, 0.05), lr=1e-3)
+        torch.manual_seed(9)
+        for _ in range(3):
+            out = harness.train_step(m, images, target, opt, dge_enable=True, dge_budget=0.5, balance_scale=0.01, finite=True)
+        assert math.isfinite(float(out["loss"]))
+        ends.append({n: p.detach() for n, p in m.named_parameters()})
+        assert all(not torch.equal(before[n], p) for n, p in m.named_parameters() if p.grad is not None and p.grad.any())
+    # (torch's own backward of the patch convolution may differ from run to run)
+    for n in ends[0]:
+        assert (ends[0][n].float() - ends[1][n].float()).abs().max() <= 3.1e-3, n

@@ -36,10 +36,12 @@ class Blocks:
             raise ValueError(f"scales of {tuple(scales.shape)} do not fit values of {tuple(values.shape)}")
         self._shape = tuple(values.shape)
         rows, (value_pitch, scale_pitch) = self._rows(), _pitches(self._shape[-1])
-        self._data = torch.zeros(rows * (value_pitch + scale_pitch), dtype=torch.uint8, device=values.device)
-        self._data[rows * value_pitch:].fill_(127)
-        self.values.view(torch.uint8).copy_(values.view(torch.uint8))
-        self.scales.view(torch.uint8).copy_(scales.view(torch.uint8))
+        values, scales = values.view(torch.uint8).reshape(rows, -1), scales.view(torch.uint8).reshape(rows, -1)
+        if values.shape[1] < value_pitch:
+            values = torch.nn.functional.pad(values, (0, value_pitch - values.shape[1]))
+        if scales.shape[1] < scale_pitch:
+            scales = torch.nn.functional.pad(scales, (0, scale_pitch - scales.shape[1]), value=127)
+        self._data = torch.cat([values.reshape(-1), scales.reshape(-1)])
 
     @classmethod
     def _of(cls, data, shape):
@@ -172,3 +174,31 @@ def layer_norm_8bit(x, weight, bias, eps=1e-6):
     if y is None:
         raise ValueError("layer_norm_8bit takes strided tensors")
     return y
+
+
+def require_plain_module(module):
+    """A TypeError unless `call_8bit` can stand in for the module: a Linear, a LayerNorm over the last dimension with weight and bias, or an
+    exact GELU, without hooks of its own."""
+    hooks = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+    plain = (type(module) in (torch.nn.Linear, torch.nn.LayerNorm, torch.nn.GELU) and "forward" not in vars(module)
+             and not any(getattr(module, h, None) for h in hooks))
+    if plain and isinstance(module, torch.nn.LayerNorm):
+        plain = len(module.normalized_shape) == 1 and module.weight is not None and module.bias is not None
+    if plain and isinstance(module, torch.nn.GELU):
+        plain = module.approximate == "none"
+    if not plain:
+        raise TypeError(f"{module} is more than a plain Linear, LayerNorm or GELU, which the operators on 8-bit blocks stand in for")
+
+
+def call_8bit(module, x):
+    """module(x) by `linear_8bit`, `layer_norm_8bit` or `gelu_8bit` (see `require_plain_module`)."""
+    require_plain_module(module)
+    if isinstance(module, torch.nn.Linear):
+        return linear_8bit(x, module.weight, module.bias)
+    if isinstance(module, torch.nn.LayerNorm):
+        return layer_norm_8bit(x, module.weight, module.bias, module.eps)
+    return gelu_8bit(x)
+
+
+def call(module, x):
+    return module(x)

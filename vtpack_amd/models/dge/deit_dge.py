@@ -22,6 +22,7 @@ from torch import nn
 
 from ... import engine
 from ...layers import DynamicGrainedEncoder, linear_cross_entropy
+from ...layers.eight_bit import call, call_8bit, require_plain_module
 from ...layers.losses import require_plain_head
 from ...layers.sparse_ops import batched_sparse_attention, sparse_attention_train
 
@@ -30,6 +31,8 @@ __all__ = ["VisionTransformer", "Block", "Attention", "Mlp", "PatchEmbed", "deit
 
 
 class Mlp(nn.Module):
+    eight_bit = False                                # see VisionTransformer.set_eight_bit
+
     def __init__(self, in_features, hidden_features=None, out_features=None):
         super().__init__()
         self.fc1 = nn.Linear(in_features, hidden_features or in_features)
@@ -42,11 +45,13 @@ class Mlp(nn.Module):
         return num_queries * (f1.in_features * f1.out_features + f1.out_features + f2.in_features * f2.out_features)
 
     def forward(self, x):
-        return self.fc2(self.act(self.fc1(x)))
+        run = call_8bit if self.eight_bit and self.training else call
+        return run(self.fc2, run(self.act, run(self.fc1, x)))
 
 
 class Attention(nn.Module):
     """Separate q and kv projections; packed queries attend to every token of their own sample."""
+    eight_bit = False
 
     def __init__(self, dim, num_heads=8, qkv_bias=False, qk_scale=None):
         super().__init__()
@@ -66,15 +71,18 @@ class Attention(nn.Module):
         # deit_dge.py:70-78,96 
         B, N, C = x.shape
         h, d = self.num_heads, C // self.num_heads
-        q = self.q(q).reshape(-1, h, d).permute(1, 0, 2)
-        kv = self.kv(x).reshape(B, N, 2, h, d).permute(2, 3, 0, 1, 4)
+        run = call_8bit if self.eight_bit and self.training else call
+        q = run(self.q, q).reshape(-1, h, d).permute(1, 0, 2)
+        kv = run(self.kv, x).reshape(B, N, 2, h, d).permute(2, 3, 0, 1, 4)
         if self.training:
-            return self.proj(sparse_attention_train(q, kv[0], kv[1], q_lengths, self.scale))
+            return run(self.proj, sparse_attention_train(q, kv[0], kv[1], q_lengths, self.scale))
         o = batched_sparse_attention(q, kv[0], kv[1], q_lengths, self.scale)
         return self.proj(o.transpose(0, 1).reshape(-1, C))
 
 
 class Block(nn.Module):
+    eight_bit = False
+
     def __init__(self, dim, num_heads, mlp_ratio=4., qkv_bias=False, qk_scale=None, norm_layer=nn.LayerNorm,
                  split_sizes=(2, 1), fused=True):
         super().__init__()
@@ -97,8 +105,9 @@ class Block(nn.Module):
         if self.fused and not self.training:
             return engine.block_forward(self, x, H, W, gate=gate)
         q = self.dge.compress(x, H, W, gate=gate)
-        q = q + self.attn(self.norm1(x), self.norm1(q), self.dge.states["batches"])
-        q = q + self.mlp(self.norm2(q))
+        run = call_8bit if self.eight_bit and self.training else call
+        q = q + self.attn(run(self.norm1, x), run(self.norm1, q), self.dge.states["batches"])
+        q = q + self.mlp(run(self.norm2, q))
         return self.dge.decompress(q)
 
 
@@ -178,6 +187,21 @@ class VisionTransformer(nn.Module):
         self.fused = fused
         for blk in self.blocks:
             blk.fused = fused
+        return self
+
+    def set_eight_bit(self, on=True):
+        """In training mode the blocks' Linears, LayerNorms and GELUs by the operators of `layers.eight_bit`: products of 8-bit numbers, whose
+        left operands, the centred inputs of the norms and the inputs of the GELUs are what the pass keeps of them, a byte a number.
+        Attention, sampling, embedding and head stay as they are, and so does eval mode.  A module that is more than a plain one is
+        refused."""
+        for blk in self.modules():
+            if isinstance(blk, Block):
+                parts = (blk.norm1, blk.norm2, blk.mlp.fc1, blk.mlp.act, blk.mlp.fc2, blk.attn.q, blk.attn.kv, blk.attn.proj)
+                for m in parts if on else ():
+                    require_plain_module(m)
+        for m in self.modules():
+            if isinstance(m, (Block, Attention, Mlp)):
+                m.eight_bit = bool(on)
         return self
 
     def no_weight_decay(self):

@@ -15,6 +15,7 @@ from torch import nn
 
 from ... import engine
 from ...layers import DynamicGrainedEncoder, linear_cross_entropy
+from ...layers.eight_bit import call, call_8bit, require_plain_module
 from ...layers.losses import require_plain_head
 from ...layers.sparse_ops import batched_sparse_attention, sparse_attention_train
 from .deit_dge import Mlp
@@ -25,6 +26,7 @@ __all__ = ["PyramidVisionTransformer", "Block", "Attention", "PatchEmbed", "pvt_
 
 class Attention(nn.Module):
     """q from the packed queries; k, v from all tokens, or from the sr x sr reduced grid when sr_ratio > 1."""
+    eight_bit = False
 
     def __init__(self, dim, num_heads=8, qkv_bias=False, qk_scale=None, sr_ratio=1):
         super().__init__()
@@ -55,18 +57,21 @@ class Attention(nn.Module):
         # pvt_dge.py:77-92,108 
         B, N, C = x.shape
         h, d = self.num_heads, C // self.num_heads
-        q = self.q(q).reshape(-1, h, d).permute(1, 0, 2)
+        run = call_8bit if self.eight_bit and self.training else call
+        q = run(self.q, q).reshape(-1, h, d).permute(1, 0, 2)
         if self.sr_ratio > 1:
             x = self.sr(x.permute(0, 2, 1).reshape(B, C, H, W)).reshape(B, C, -1).permute(0, 2, 1)
-            x = self.norm(x)
-        kv = self.kv(x).reshape(B, -1, 2, h, d).permute(2, 3, 0, 1, 4)
+            x = run(self.norm, x)
+        kv = run(self.kv, x).reshape(B, -1, 2, h, d).permute(2, 3, 0, 1, 4)
         if self.training:
-            return self.proj(sparse_attention_train(q, kv[0], kv[1], q_lengths, self.scale))
+            return run(self.proj, sparse_attention_train(q, kv[0], kv[1], q_lengths, self.scale))
         o = batched_sparse_attention(q, kv[0], kv[1], q_lengths, self.scale)
         return self.proj(o.transpose(0, 1).reshape(-1, C))
 
 
 class Block(nn.Module):
+    eight_bit = False
+
     def __init__(self, dim, num_heads, mlp_ratio=4., qkv_bias=False, qk_scale=None, norm_layer=nn.LayerNorm,
                  sr_ratio=1, split_sizes=(2, 1), fused=True):
         super().__init__()
@@ -88,8 +93,9 @@ class Block(nn.Module):
         if self.fused and not self.training:
             return engine.block_forward(self, x, H, W, gate=gate)
         q = self.dge.compress(x, H, W, gate=gate)
-        q = q + self.attn(self.norm1(x), self.norm1(q), H, W, self.dge.states["batches"])
-        q = q + self.mlp(self.norm2(q))
+        run = call_8bit if self.eight_bit and self.training else call
+        q = q + self.attn(run(self.norm1, x), run(self.norm1, q), H, W, self.dge.states["batches"])
+        q = q + self.mlp(run(self.norm2, q))
         return self.dge.decompress(q)
 
 
@@ -159,6 +165,22 @@ class PyramidVisionTransformer(nn.Module):
         for m in self.modules():
             if isinstance(m, Block):
                 m.fused = fused
+        return self
+
+    def set_eight_bit(self, on=True):
+        """In training mode the blocks' Linears, LayerNorms and GELUs by the operators of `layers.eight_bit`: products of 8-bit numbers, whose
+        left operands, the centred inputs of the norms and the inputs of the GELUs are what the pass keeps of them, a byte a number.
+        Attention, sampling, embedding and head stay as they are, and so does eval mode.  A module that is more than a plain one is
+        refused."""
+        for blk in self.modules():
+            if isinstance(blk, Block):
+                parts = (blk.norm1, blk.norm2, blk.mlp.fc1, blk.mlp.act, blk.mlp.fc2, blk.attn.q, blk.attn.kv, blk.attn.proj)
+                parts += (blk.attn.norm,) if blk.attn.sr_ratio > 1 else ()
+                for m in parts if on else ():
+                    require_plain_module(m)
+        for m in self.modules():
+            if isinstance(m, (Block, Attention, Mlp)):
+                m.eight_bit = bool(on)
         return self
 
     def complexity(self, x):
