@@ -28,7 +28,7 @@ __device__ __forceinline__ void multiply_blocks(const LA &a, const LB &b, const 
     using E = EightBit<S>;
     constexpr int IM = S::IM, JN = S::JN, SLOTS = S::SLOTS, A_BYTES = LA::STAGE;
     constexpr int LOADS = LA::PIECES + LB::PIECES;          // and now and then those of scales: what waits for fewer waits for enough
-    constexpr int GROUP = S::SLAB == 64 ? 4 : 8;            // slabs of four blocks
+    constexpr int GROUP = 4;                                // blocks, a slab each, whose scales are a word
     static_assert(LOADS * (SLOTS - 2) < 64, "the counter of outstanding loads");
     const int lane = threadIdx.x & 63, lr = lane & 31, wid = wave_uniform(threadIdx.x >> 6), wm = wid / S::WN, wn = wid % S::WN;
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
@@ -96,7 +96,7 @@ __device__ __forceinline__ void multiply_blocks(const LA &a, const LB &b, const 
             issue(t + SLOTS - 1, in);
             in = in == SLOTS - 1 ? 0 : in + 1;
         }
-        const int shift = t % GROUP / (GROUP / 4) * 8;
+        const int shift = t % GROUP * 8;
         uint32_t qa[IM], qb[JN];
 #pragma unroll
         for (int i = 0; i < IM; i++) qa[i] = words_a[i] >> shift;
@@ -327,8 +327,9 @@ template <typename T> __global__ __launch_bounds__(256) void prepare_gradients_k
 
 // ------------------------------------------------------------------------------------------------ on the host
 using ForwardLarge = Shape<2, 4, 4, 2, 64, 2, 1>;
-using ForwardMiddle = Shape<2, 4, 2, 2, 32, 3, 1>;
+using ForwardSquare = Shape<2, 2, 2, 2, 64, 2, 1>;
 using ForwardSmall = Shape<1, 1, 2, 2, 64, 3, 1>;
+static_assert(ForwardLarge::SLAB == 64 && ForwardSquare::SLAB == 64 && ForwardSmall::SLAB == 64, "slabs of a block");
 
 constexpr int SLAB = 64;
 static int64_t take(int64_t &at, int64_t bytes)
@@ -469,16 +470,14 @@ extern "C" int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight,
         a.x_scales = scales_of(xq, rows, width), a.w_scales = scales_of(wq, out, width), a.scale_pitch = (int)scale_pitch(width);
         slabs = value_pitch(width) / BLOCK;
     }
+    // Many tiles by 256 x 256, two of 128 x 128 beside each other on a compute unit for fewer, and for short sums without an activation (whose
+    // results leave while the other multiplies), 64 x 64 where those would leave compute units without work.  us of a call in bf16 (64 x 64,
+    // 128 x 128, 256 x 256): 4112 x 384 x 384 8.6, 9.1, 13.1; 4112 x 384 x 1536 13.9, 11.7, 14.9; 8192 x 1024 x 1024 26.4, 21.4, 27.0;
+    // 65536 x 384 x 384 41, 34, 36; 32768 x 384 x 1536 with GELU 65, 51, 46; 16384 x 1024 x 1024 42.7, 34.0, 33.3; 8192 x 4096 x 4096 226, 154, 139
     const int64_t cu = compute_units();
-    if (ceil_div(rows, 128) * ceil_div(out, 256) < cu) {
-        a.stages = (int)(slabs * SLAB / ForwardSmall::SLAB);
-        return go_forward<ForwardSmall>(a, act, dtype, st);
-    }
-    if (ceil_div(rows, 256) * ceil_div(out, 256) < 4 * cu) {
-        a.stages = (int)(slabs * SLAB / ForwardMiddle::SLAB);
-        return go_forward<ForwardMiddle>(a, act, dtype, st);
-    }
-    a.stages = (int)(slabs * SLAB / ForwardLarge::SLAB);
+    a.stages = (int)slabs;
+    if (ceil_div(rows, 128) * ceil_div(out, 128) * 4 < 5 * cu) return go_forward<ForwardSmall>(a, act, dtype, st);
+    if (ceil_div(rows, 256) * ceil_div(out, 256) < cu || (act == VTDGE_ACT_NONE && width <= 640)) return go_forward<ForwardSquare>(a, act, dtype, st);
     return go_forward<ForwardLarge>(a, act, dtype, st);
 }
 
