@@ -293,8 +293,10 @@ template <typename T> __global__ __launch_bounds__(256) void prepare_gradients_k
         *reinterpret_cast<u32x4 *>(g.to + ((int64_t)row * g.per_row * 8 + c)) = Elem<bf16_t>::pack(f);
         return;
     }
-    constexpr int PITCH = 36;                       // words of a column, two rows each
-    __shared__ __attribute__((aligned(16))) uint32_t tile[BLOCK * PITCH];
+    // [column][two rows a word]; pieces of four words are XOR-ed by the column's eight, and the columns of the upper half swapped in pairs, so that the
+    // sixteen columns that a wave writes at once lie in all 64 banks
+    __shared__ __attribute__((aligned(16))) uint32_t tile[BLOCK * 32];
+    auto word = [](int column, int piece) { return (column ^ (column >> 6 & 1)) * 32 + (piece ^ (column >> 3 & 7)) * 4; };
     const bool second = blockIdx.x >= p.first;
     const ExpandJob &job = p.job[second ? 1 : 0];
     const uint32_t id = blockIdx.x - (second ? p.first : 0), block = id / job.down, r0 = (id - block * job.down) * 64;
@@ -313,7 +315,7 @@ template <typename T> __global__ __launch_bounds__(256) void prepare_gradients_k
             }
         }
 #pragma unroll
-        for (int e = 0; e < 8; e++) tile[(c + e) * PITCH + pair] = pack_bf16x2(f[0][e], f[1][e]);
+        for (int e = 0; e < 8; e++) tile[word(c + e, pair >> 2) + (pair & 3)] = pack_bf16x2(f[0][e], f[1][e]);
     }
     __syncthreads();
 #pragma unroll
@@ -321,7 +323,7 @@ template <typename T> __global__ __launch_bounds__(256) void prepare_gradients_k
         const int at = threadIdx.x + 256 * k, column = at >> 3, piece = at & 7;
         if ((int)(block * BLOCK) + column < job.n)
             *reinterpret_cast<u32x4 *>(job.to + (int64_t)(block * BLOCK + column) * job.pitch + r0 + piece * 8) =
-                *reinterpret_cast<const u32x4 *>(tile + column * PITCH + piece * 4);
+                *reinterpret_cast<const u32x4 *>(tile + word(column, piece));
     }
 }
 

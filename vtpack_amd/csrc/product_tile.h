@@ -43,8 +43,8 @@ template <int IM_, int JN_, int WM_, int WN_, int SLAB_, int SLOTS_, int PARTS_>
 // ALONG: the summed dimension lies along the rows of memory: tile rows are rows of memory, `limit` of them from the first on.
 // Across: the summed dimension counts the rows of memory, `limit` of them, and tile rows are elements of a row, which has a multiple
 // of 8 of them, `span`.  No stage begins behind `limit`: a sum of n rows of memory has ceil(n / SLAB) stages.
-// LDS rows are 2 SLAB bytes (ALONG) or 2 T bytes (across) without gaps; their 16-byte pieces are XOR-ed by the row, so that the
-// sixteen lanes that read together meet every bank once.
+// LDS rows are 2 SLAB bytes (ALONG) or 2 T bytes (across) without gaps; their 16-byte pieces are XOR-ed by the row, so that the lanes
+// that read together (half a wave of transposed reads, whose four rows take sixteen pieces) meet each of the 64 banks once.
 template <bool ALONG, int T, int SLAB, int WAVES, bool MAY_STREAM = false> struct Loader {
     static constexpr int ROW = ALONG ? 2 * SLAB : 2 * T, STAGE = 2 * SLAB * T;
     static constexpr int LPR = ROW / 16, RPI = 64 / LPR;                  // lanes a row, rows an instruction
@@ -52,13 +52,15 @@ template <bool ALONG, int T, int SLAB, int WAVES, bool MAY_STREAM = false> struc
     static_assert(PIECES * WAVES * 1024 == STAGE && LPR <= 64, "whole instructions");
     const unsigned char *base;
     int64_t plane, pitch;                                                 // bytes
-    int limit, row0, last;
+    int limit, lane, row0, last;
     bool stream = false;                                                  // past the caches
 
-    __device__ __forceinline__ Loader(const Operand &o, int64_t first, int64_t lim, int64_t span)
-        : base(reinterpret_cast<const unsigned char *>(o.p) + (ALONG ? first * o.pitch * 2 : first * 2)), plane(o.plane * 2), pitch(o.pitch * 2)
+    __device__ __forceinline__ Loader(const Operand &o, int64_t first, int64_t lim, int64_t span) : Loader(o, first, lim, span, threadIdx.x & 63) {}
+    // `own`: the lane's number
+    __device__ __forceinline__ Loader(const Operand &o, int64_t first, int64_t lim, int64_t span, int own)
+        : base(reinterpret_cast<const unsigned char *>(o.p) + (ALONG ? first * o.pitch * 2 : first * 2)), plane(o.plane * 2), pitch(o.pitch * 2), lane(own)
     {
-        const int lane = threadIdx.x & 63, wid = wave_uniform(threadIdx.x >> 6);
+        const int wid = wave_uniform(threadIdx.x >> 6);
         row0 = wid * RPI + lane / LPR;
         if constexpr (ALONG) limit = (int)(lim - first < T ? lim - first : T);
         else limit = (int)lim;
@@ -67,7 +69,7 @@ template <bool ALONG, int T, int SLAB, int WAVES, bool MAY_STREAM = false> struc
     static __device__ __forceinline__ int swizzle(int r)
     {
         if constexpr (ALONG) return SLAB == 64 ? (r >> 1) & 7 : SLAB == 32 ? (r >> 2) & 3 : (r >> 3) & 1;
-        else return LPR == 8 ? ((r >> 1) & 3) << 1 : (r & 7) << 1;
+        else return LPR == 8 ? ((r >> 1) & 3) << 1 : (r & 3) << 2;
     }
     // stage `kt` of part `part` to LDS byte `lds`
     __device__ __forceinline__ void load(int part, int kt, uint32_t lds) const
@@ -79,7 +81,7 @@ template <bool ALONG, int T, int SLAB, int WAVES, bool MAY_STREAM = false> struc
     // instruction `d` of them
     __device__ __forceinline__ void load_piece(int d, const void *from, int kt, uint32_t lds) const
     {
-        const int lane = threadIdx.x & 63, wid = wave_uniform(threadIdx.x >> 6);
+        const int wid = wave_uniform(threadIdx.x >> 6);
         const int r = d * WAVES * RPI + row0;
         const int at = ((lane % LPR) ^ swizzle(r)) * 16;
         const int row = ALONG ? min(r, limit - 1) : min(r, limit - 1 - kt * SLAB);
