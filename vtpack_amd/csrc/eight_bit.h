@@ -24,13 +24,9 @@ struct QuantizeArgs {
     QuantizeJob job[2];
     uint32_t first;                                 // workgroups of the first
 };
-struct DequantizeJob {
-    const unsigned char *values, *scales; uint32_t rows, per_row; int64_t n, value_pitch; int scale_pitch;      // per_row: vectors of eight
-    void *to; int64_t ld;
-};
 struct DequantizeArgs {
-    DequantizeJob job[2];
-    uint32_t first;
+    const unsigned char *values, *scales; uint32_t rows, per_row; int n, scale_pitch; int64_t value_pitch;      // per_row: vectors of eight
+    void *to;
 };
 struct GeluArgs {
     const void *x; int64_t ld; uint32_t rows, per_row; int n;
@@ -44,8 +40,6 @@ struct NormArgs {
 int check_blocks(const char *what, int64_t rows, int64_t n);
 QuantizeJob quantize_job(const void *from, int64_t ld, int64_t rows, int64_t n, void *blocks, bf16_t *expanded, int64_t expanded_pitch);
 int launch_quantize(QuantizeArgs &a, int jobs, int dtype, const char *what, hipStream_t st);
-DequantizeJob dequantize_job(const void *blocks, int64_t rows, int64_t n, void *to, int64_t ld, int64_t columns);
-int launch_dequantize(DequantizeArgs &a, int jobs, int dtype, const char *what, hipStream_t st);
 
 // ------------------------------------------------------------------------------------------------ eight numbers of a lane
 // `left` of them are there (fewer than one: none), zeros in the place of the others.  Vectors need not lie on 16-byte boundaries: one load

@@ -42,15 +42,13 @@ template <typename T> __global__ __launch_bounds__(256) void quantize_kernel(Qua
 // blocks -> numbers
 template <typename T> __global__ __launch_bounds__(256) void dequantize_kernel(DequantizeArgs p)
 {
-    const bool second = blockIdx.x >= p.first;
-    const DequantizeJob &job = p.job[second ? 1 : 0];
-    const uint32_t id = (blockIdx.x - (second ? p.first : 0)) * 256 + threadIdx.x, row = id / job.per_row, c = (id - row * job.per_row) * 8;
-    if (row >= job.rows) return;
-    const u32x2 bytes = *reinterpret_cast<const u32x2 *>(job.values + (int64_t)row * job.value_pitch + c);
-    const int scale = job.scales[(int64_t)row * job.scale_pitch + c / BLOCK];
+    const uint32_t id = blockIdx.x * 256 + threadIdx.x, row = id / p.per_row, c = (id - row * p.per_row) * 8;
+    if (row >= p.rows) return;
+    const u32x2 bytes = *reinterpret_cast<const u32x2 *>(p.values + (int64_t)row * p.value_pitch + c);
+    const int scale = p.scales[(int64_t)row * p.scale_pitch + c / BLOCK];
     float f[8];
     stands_for8(bytes, scale, f);
-    store8<T>(static_cast<T *>(job.to) + (int64_t)row * job.ld + c, (int)job.n - (int)c, f);
+    store8<T>(static_cast<T *>(p.to) + (int64_t)row * p.n + c, p.n - (int)c, f);
 }
 
 // ------------------------------------------------------------------------------------------------ GELU
@@ -328,26 +326,6 @@ int launch_quantize(QuantizeArgs &a, int jobs, int dtype, const char *what, hipS
     kern<<<(unsigned)blocks, 256, 0, st>>>(a);
     return check_launch(what);
 }
-DequantizeJob dequantize_job(const void *blocks, int64_t rows, int64_t n, void *to, int64_t ld, int64_t columns)
-{
-    DequantizeJob j{};
-    j.values = values_of(blocks), j.scales = scales_of(blocks, rows, n), j.rows = (uint32_t)rows, j.per_row = (uint32_t)ceil_div(columns, 8);
-    j.value_pitch = value_pitch(n), j.scale_pitch = (int)scale_pitch(n), j.n = columns, j.to = to, j.ld = ld;
-    return j;
-}
-int launch_dequantize(DequantizeArgs &a, int jobs, int dtype, const char *what, hipStream_t st)
-{
-    int64_t blocks = 0;
-    for (int i = 0; i < jobs; i++) {
-        blocks += ceil_div((int64_t)a.job[i].rows * a.job[i].per_row, 256);
-        if (i == 0) a.first = (uint32_t)blocks;
-    }
-    VT_REQUIRE(blocks < (1ll << 31), VTDGE_ERR_UNSUPPORTED, "%s: %lld blocks", what, (long long)blocks);
-    auto kern = dtype == VTDGE_F32 ? dequantize_kernel<float> : dequantize_kernel<bf16_t>;
-    note_kernel(reinterpret_cast<const void *>(kern));
-    kern<<<(unsigned)blocks, 256, 0, st>>>(a);
-    return check_launch(what);
-}
 
 static int check_dtype(const char *what, int dtype)
 {
@@ -420,8 +398,12 @@ extern "C" int vtdge_dequantize_blocks(const void *blocks, int64_t rows, int64_t
     VT_REQUIRE(out && blocks, VTDGE_ERR_ARG, "dequantize_blocks: NULL operand");
     VT_REQUIRE(((uintptr_t)blocks & 127) == 0, VTDGE_ERR_ARG, "dequantize_blocks: blocks off their boundary");
     DequantizeArgs a{};
-    a.job[0] = dequantize_job(blocks, rows, n, out, n, n);
-    return launch_dequantize(a, 1, dtype, "dequantize_blocks", (hipStream_t)stream);
+    a.values = values_of(blocks), a.scales = scales_of(blocks, rows, n), a.rows = (uint32_t)rows, a.per_row = (uint32_t)ceil_div(n, 8);
+    a.n = (int)n, a.value_pitch = value_pitch(n), a.scale_pitch = (int)scale_pitch(n), a.to = out;
+    auto kern = dtype == VTDGE_F32 ? dequantize_kernel<float> : dequantize_kernel<bf16_t>;
+    note_kernel(reinterpret_cast<const void *>(kern));
+    kern<<<(unsigned)ceil_div(rows * a.per_row, 256), 256, 0, (hipStream_t)stream>>>(a);
+    return check_launch("dequantize_blocks");
 }
 
 static int gelu_args(const char *what, GeluArgs &a, const void *x, int64_t ldx, int64_t rows, int64_t n, const void *blocks, void *y, int dtype)

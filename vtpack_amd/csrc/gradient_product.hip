@@ -242,21 +242,22 @@ template <class S> static GradShape grad_shape(int grads, double us, double tile
     return GradShape{grads, S::ROWS, S::COLS, S::SLAB, us, tile_us, per_cu, us_alone};
 }
 
-#ifndef VT_FORCE
-#define VT_FORCE -1
-#endif
 void plan_gradients(GradPlan &p, int64_t rows, int64_t of_piece, int width, bool split, bool ends)
 {
     if (ends) {
-        const GradShape shapes[4] = {grad_shape<GradLarge>(GRAD_LARGE, 1.9, 5.0), grad_shape<GradMiddle>(GRAD_MIDDLE, 1.1, 3.0), grad_shape<GradSquare>(GRAD_SQUARE, 1.4, 2.0, 2, 0.8),
-                                     grad_shape<GradSmall>(GRAD_SMALL, 0.8, 1.0, 3, 0.65)};
+        // The shape that ends first by the same count.  us of a backward call in bf16 (256 x 256, 128 x 128, 64 x 64), rows x width x outputs: 300
+        // x 200 x 130 17.6, 11.9, 10.9; 1021 x 192 x 768 27.3, 19.1, 15.5; 1500 x 3000 x 1000 52, 37.5, 45; 2999 x 777 x 1301 47, 42, 45; 65536 x
+        // 384 x 384 110, 84, 93; 8192 x 768 x 768 41.7, 42.1, 48; 6000 x 2000 x 2000 127, 131, 180; 32768 x 1024 x 4096 505, 594, 994.  (256 x
+        // 128, one on a compute unit, was first in 5 of 28 sizes, by 8 % at most.)
+        const GradShape shapes[3] = {grad_shape<GradLarge>(GRAD_LARGE, 2.0, 5.0), grad_shape<GradSquare>(GRAD_SQUARE, 1.15, 2.0, 2, 0.75),
+                                     grad_shape<GradSmall>(GRAD_SMALL, 0.9, 1.0, 3, 0.65)};
         int best = 0;
         double least = 1e30;
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < 3; k++) {
             const double t = cuts(p, rows, of_piece, width, shapes[k], false);
             if (t < least) least = t, best = k;
         }
-        cuts(p, rows, of_piece, width, shapes[VT_FORCE >= 0 ? VT_FORCE : best], true);
+        cuts(p, rows, of_piece, width, shapes[best], true);
         return;
     }
     const GradShape large = split ? grad_shape<SplitGradLarge>(GRAD_LARGE, 3.0, 12.0) : grad_shape<GradLarge>(GRAD_LARGE, 2.0, 6.0);
@@ -284,7 +285,9 @@ template <class S, bool ENDS> static int go_grad(GradPair &g, const char *what, 
     }
     VT_REQUIRE(blocks < (1 << 23), VTDGE_ERR_UNSUPPORTED, "%s: %lld tiles", what, (long long)blocks);
     if (blocks == 0) return VTDGE_OK;
-    auto kern = ENDS ? linear_grad_kernel<S> : cross_entropy_grad_kernel<S>;
+    void (*kern)(GradPair);
+    if constexpr (ENDS) kern = linear_grad_kernel<S>;
+    else kern = cross_entropy_grad_kernel<S>;
     VT_RESERVE_LDS(kern, S::LDS, what);
     note_kernel(reinterpret_cast<const void *>(kern));
     kern<<<(unsigned)blocks, S::THREADS, S::LDS, st>>>(g);
@@ -316,7 +319,6 @@ int launch_gradients(const GradPlan &p, GradPair &g, const char *what, hipStream
     if (g.f32_parts) return p.grads == GRAD_LARGE ? go_grad<SplitGradLarge, false>(g, what, st) : go_grad<SplitGradSmall, false>(g, what, st);
     if (g.ends)
         return p.grads == GRAD_LARGE ? go_grad<GradLarge, true>(g, what, st)
-               : p.grads == GRAD_MIDDLE ? go_grad<GradMiddle, true>(g, what, st)
                : p.grads == GRAD_SQUARE ? go_grad<GradSquare, true>(g, what, st) : go_grad<GradSmall, true>(g, what, st);
     return p.grads == GRAD_LARGE ? go_grad<GradLarge, false>(g, what, st)
            : p.grads == GRAD_MIDDLE ? go_grad<GradMiddle, false>(g, what, st) : go_grad<GradSmall, false>(g, what, st);

@@ -55,10 +55,8 @@ template <bool ALONG, int T, int SLAB, int WAVES, bool MAY_STREAM = false> struc
     int limit, lane, row0, last;
     bool stream = false;                                                  // past the caches
 
-    __device__ __forceinline__ Loader(const Operand &o, int64_t first, int64_t lim, int64_t span) : Loader(o, first, lim, span, threadIdx.x & 63) {}
-    // `own`: the lane's number
-    __device__ __forceinline__ Loader(const Operand &o, int64_t first, int64_t lim, int64_t span, int own)
-        : base(reinterpret_cast<const unsigned char *>(o.p) + (ALONG ? first * o.pitch * 2 : first * 2)), plane(o.plane * 2), pitch(o.pitch * 2), lane(own)
+    __device__ __forceinline__ Loader(const Operand &o, int64_t first, int64_t lim, int64_t span)
+        : base(reinterpret_cast<const unsigned char *>(o.p) + (ALONG ? first * o.pitch * 2 : first * 2)), plane(o.plane * 2), pitch(o.pitch * 2), lane(threadIdx.x & 63)
     {
         const int wid = wave_uniform(threadIdx.x >> 6);
         row0 = wid * RPI + lane / LPR;
@@ -74,25 +72,18 @@ template <bool ALONG, int T, int SLAB, int WAVES, bool MAY_STREAM = false> struc
     // stage `kt` of part `part` to LDS byte `lds`
     __device__ __forceinline__ void load(int part, int kt, uint32_t lds) const
     {
-        const void *const from = slab_at(part, kt);
-#pragma unroll
-        for (int d = 0; d < PIECES; d++) load_piece(d, from, kt, lds);
-    }
-    // instruction `d` of them
-    __device__ __forceinline__ void load_piece(int d, const void *from, int kt, uint32_t lds) const
-    {
+        const void *const from = uniform_ptr(base + part * plane + (ALONG ? (int64_t)kt * (2 * SLAB) : (int64_t)kt * SLAB * pitch));
         const int wid = wave_uniform(threadIdx.x >> 6);
-        const int r = d * WAVES * RPI + row0;
-        const int at = ((lane % LPR) ^ swizzle(r)) * 16;
-        const int row = ALONG ? min(r, limit - 1) : min(r, limit - 1 - kt * SLAB);
-        const int col = ALONG ? at : min(at, last);
-        const uint32_t off = (uint32_t)row * (uint32_t)pitch + col, to = wave_uniform(lds + (d * WAVES + wid) * 1024);
-        if (MAY_STREAM && stream) dma16_nt(from, off, to);
-        else dma16(from, off, to);
-    }
-    __device__ __forceinline__ const void *slab_at(int part, int kt) const
-    {
-        return uniform_ptr(base + part * plane + (ALONG ? (int64_t)kt * (2 * SLAB) : (int64_t)kt * SLAB * pitch));
+#pragma unroll
+        for (int d = 0; d < PIECES; d++) {
+            const int r = d * WAVES * RPI + row0;
+            const int at = ((lane % LPR) ^ swizzle(r)) * 16;
+            const int row = ALONG ? min(r, limit - 1) : min(r, limit - 1 - kt * SLAB);
+            const int col = ALONG ? at : min(at, last);
+            const uint32_t off = (uint32_t)row * (uint32_t)pitch + col, to = wave_uniform(lds + (d * WAVES + wid) * 1024);
+            if (MAY_STREAM && stream) dma16_nt(from, off, to);
+            else dma16(from, off, to);
+        }
     }
     // the 8 values of step s (16 of the summed dimension) of tile row `block` * 32 + lane % 32
     static __device__ __forceinline__ u32x4 fragment(const unsigned char *stage, int block, int s)
