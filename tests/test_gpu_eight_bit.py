@@ -115,6 +115,13 @@ def test_blocks_from_a_pair(dev):
     assert quantize_blocks(x[:0]).dequantize().shape == (0, 5, 300)
 
 
+def test_blocks_from_a_pair_without_rows(dev):
+    from vtpack_amd.layers import Blocks, quantize_blocks
+    a = quantize_blocks(_numbers(dev, 0, 5, 300))
+    b = Blocks(a.values, a.scales)
+    assert b.shape == (0, 5, 300) and b._data.numel() == 0 and b.dequantize().shape == (0, 5, 300)
+
+
 # ------------------------------------------------------------------------------------------------ Linear
 def _linear_bound(x8, w8, b, y, dtype, act="none"):
     sums = x8.abs() @ w8.abs().t()

@@ -36,7 +36,7 @@ class Blocks:
             raise ValueError(f"scales of {tuple(scales.shape)} do not fit values of {tuple(values.shape)}")
         self._shape = tuple(values.shape)
         rows, (value_pitch, scale_pitch) = self._rows(), _pitches(self._shape[-1])
-        values, scales = values.view(torch.uint8).reshape(rows, -1), scales.view(torch.uint8).reshape(rows, -1)
+        values, scales = (t.view(torch.uint8).reshape(rows, t.shape[-1]) for t in (values, scales))
         if values.shape[1] < value_pitch:
             values = torch.nn.functional.pad(values, (0, value_pitch - values.shape[1]))
         if scales.shape[1] < scale_pitch:
