@@ -677,7 +677,9 @@ int vtdge_adamw_scalars(int64_t *step, int64_t skipped, int advance, const float
  * count in the maximum.  Each number of a block is a bf16 number.
  *   blocks    vtdge_blocks_bytes(rows, n) bytes on a 128-byte boundary: rows of ceil(n / 128) * 128 values, zeros behind the n-th, then rows
  *             of scale bytes e + 127, ceil(n / 128) of them filled up to a multiple of 4.  (A scale byte of 255 stands for NaN, as in e8m0.)
- *   x [rows, n] of `dtype`, rows ldx elements apart; results are dense */
+ *   x [rows, n] of `dtype`, rows ldx elements apart; results are dense
+ * An operand has VTDGE_MAX_BLOCKS blocks at most, and rows of at most 2^20. */
+#define VTDGE_MAX_BLOCKS 268435440
 int64_t vtdge_blocks_bytes(int64_t rows, int64_t n);
 int vtdge_quantize_blocks(const void *x, int64_t ldx, int64_t rows, int64_t n, void *blocks, int dtype, void *stream);
 int vtdge_dequantize_blocks(const void *blocks, int64_t rows, int64_t n, void *out, int dtype, void *stream);
@@ -689,7 +691,8 @@ int vtdge_gelu_8bit_backward(const void *grad, int64_t ldg, int64_t rows, int64_
 
 /* y = (x - m) r weight + bias, m the fp32 number next to the row's mean, r = 1 / sqrt(var + eps), with Q(x - m) kept in blocks and r in
  * rstd fp32 [rows] (nullable, both: not kept).  Backward, h = Q(x - m) r and g = grad weight:  dx = r (g - mean g - h mean(g h)), dweight = sum grad h, dbias = sum
- * grad over the rows; each of the three nullable.  n up to VTDGE_MAX_NORM_8BIT.
+ * grad over the rows; each of the three nullable.  n up to VTDGE_MAX_NORM_8BIT, fewer than 2^24
+ * rows.
  *   workspace  vtdge_layernorm_8bit_backward_workspace(rows, n) bytes, 16-byte aligned */
 #define VTDGE_MAX_NORM_8BIT 8192
 int vtdge_layernorm_8bit(const void *x, int64_t ldx, const void *weight, const void *bias, float eps, int64_t rows, int64_t n,

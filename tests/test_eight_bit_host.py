@@ -43,6 +43,18 @@ def test_sizes_of_buffers():
     assert lib.vtdge_blocks_bytes(1 << 31, 1) == -1 and lib.vtdge_blocks_bytes(1, (1 << 20) + 1) == -1 and lib.vtdge_blocks_bytes((1 << 31) - 1, 1 << 20) == -1
 
 
+def test_more_than_a_launch_takes_is_refused():
+    """2^32 threads, sixteen a block, and a workgroup for one to four rows of a norm."""
+    lib, p, U = _lib.load(), 4096, _lib.ERR_UNSUPPORTED
+    most = 268435440
+    assert lib.vtdge_blocks_bytes(most, 1) == most * 132 and lib.vtdge_blocks_bytes(most + 1, 128) == -1 and lib.vtdge_blocks_bytes(most // 2 + 1, 129) == -1
+    for rows, n in ((most + 1, 1), (most // 2 + 1, 129)):
+        assert lib.vtdge_quantize_blocks(p, n, rows, n, p, 0, None) == U and lib.vtdge_dequantize_blocks(p, rows, n, p, 0, None) == U
+        assert lib.vtdge_gelu_8bit(p, n, rows, n, p, p, 0, None) == U and lib.vtdge_gelu_8bit_backward(p, n, rows, n, p, p, 0, None) == U
+    assert lib.vtdge_layernorm_8bit(p, 8, p, p, 1e-6, 1 << 24, 8, p, p, p, 0, None) == U
+    assert lib.vtdge_layernorm_8bit_backward_workspace(1 << 24, 8) == -1 and lib.vtdge_layernorm_8bit_backward_workspace((1 << 24) - 1, 8) > 0
+
+
 def _codes(fn, good, table):
     for i, v, want in table:
         args = list(good)

@@ -300,7 +300,8 @@ template <typename T> __global__ __launch_bounds__(1024) void norm_join_kernel(c
 int check_blocks(const char *what, int64_t rows, int64_t n)
 {
     VT_REQUIRE(rows > 0 && n > 0, VTDGE_ERR_ARG, "%s: %lld rows of %lld", what, (long long)rows, (long long)n);
-    VT_REQUIRE(rows < (1ll << 31) && n <= (1 << 20) && rows * ceil_div(n, 8) < (1ll << 32) - 65536 * 256, VTDGE_ERR_UNSUPPORTED, "%s: %lld rows of %lld", what,
+    // sixteen threads of a launch each, of which there may be 2^32
+    VT_REQUIRE(rows < (1ll << 28) && n <= (1 << 20) && rows * ceil_div(n, BLOCK) <= VTDGE_MAX_BLOCKS, VTDGE_ERR_UNSUPPORTED, "%s: %lld rows of %lld", what,
                (long long)rows, (long long)n);
     return VTDGE_OK;
 }
@@ -320,7 +321,7 @@ int launch_quantize(QuantizeArgs &a, int jobs, int dtype, const char *what, hipS
         blocks += ceil_div((int64_t)a.job[i].rows * a.job[i].per_row, 16);
         if (i == 0) a.first = (uint32_t)blocks;
     }
-    VT_REQUIRE(blocks < (1ll << 31), VTDGE_ERR_UNSUPPORTED, "%s: %lld blocks", what, (long long)blocks);
+    VT_REQUIRE(blocks < (1 << 24), VTDGE_ERR_UNSUPPORTED, "%s: %lld workgroups", what, (long long)blocks);
     auto kern = dtype == VTDGE_F32 ? quantize_kernel<float> : quantize_kernel<bf16_t>;
     note_kernel(reinterpret_cast<const void *>(kern));
     kern<<<(unsigned)blocks, 256, 0, st>>>(a);
@@ -366,6 +367,7 @@ static int check_norm(const char *what, int64_t rows, int64_t n, int dtype)
     VT_STEP(check_dtype(what, dtype));
     VT_STEP(check_blocks(what, rows, n));
     VT_REQUIRE(n <= VTDGE_MAX_NORM_8BIT, VTDGE_ERR_UNSUPPORTED, "%s: rows of %lld, %d at most", what, (long long)n, VTDGE_MAX_NORM_8BIT);
+    VT_REQUIRE(rows < (1 << 24), VTDGE_ERR_UNSUPPORTED, "%s: %lld rows, fewer than 2^24 are supported", what, (long long)rows);
     return VTDGE_OK;
 }
 

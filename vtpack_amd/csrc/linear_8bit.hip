@@ -526,7 +526,7 @@ extern "C" int vtdge_linear_8bit_backward(const void *grad, int64_t ldg, const v
         tiles += ceil_div(rows * d.pack.per_row, 256);
         g_op = Operand{to, padded(out), 0};
     }
-    VT_REQUIRE(tiles < (1ll << 31), VTDGE_ERR_UNSUPPORTED, "linear_8bit_backward: %lld rows of %lld and %lld", (long long)rows, (long long)width, (long long)out);
+    VT_REQUIRE(tiles < (1 << 24), VTDGE_ERR_UNSUPPORTED, "linear_8bit_backward: %lld rows of %lld and %lld", (long long)rows, (long long)width, (long long)out);
     if (tiles > 0) {
         auto kern = dtype == VTDGE_F32 ? prepare_gradients_kernel<float> : prepare_gradients_kernel<bf16_t>;
         note_kernel(reinterpret_cast<const void *>(kern));
