@@ -179,6 +179,67 @@ def test_linear_gradients(dev, dtype, rows, out, width, bias):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,out,width", [(4099, 2049, 200), (8200, 4100, 700), (2999, 1301, 777)])
+def test_linear_by_large_tiles(dev, dtype, rows, out, width):
+    """Ragged ones of 128 x 128 and 256 x 256."""
+    test_linear(dev, dtype, rows, out, width)
+    test_linear_gradients(dev, dtype, rows, out, width, True)
+
+
+@pytest.mark.parametrize("out", [1000, 1024])
+def test_offsets_beyond_32_bits(dev, out):
+    """Operands of more than 2^31 numbers: whole numbers, whose sums are exact, and rows, each of which is its own."""
+    from vtpack_amd.layers import gelu_8bit, layer_norm_8bit, linear_8bit, quantize_blocks
+    rows, width, tail = (1 << 21) + 333, 1024, 200
+    g = torch.Generator(dev).manual_seed(out)
+    whole = lambda *s: torch.randint(-1, 2, s, device=dev, generator=g, dtype=torch.int8).to(torch.bfloat16)
+    x, w, dy = whole(rows, width).requires_grad_(), whole(out, width).requires_grad_(), whole(rows, out)
+    b = torch.ones(out, device=dev, dtype=torch.bfloat16, requires_grad=True)
+    y = linear_8bit(x, w, b)
+    with torch.no_grad():
+        assert torch.equal(y[-tail:], (x[-tail:].float() @ w.float().t() + 1).bfloat16())
+        at = (1 << 31) // out                              # around the 2^31st result
+        assert torch.equal(y[at - 50:at + 50], (x[at - 50:at + 50].float() @ w.float().t() + 1).bfloat16())
+    del y
+    dx, dw, db = torch.autograd.grad(linear_8bit(x, w, b), (x, w, b), dy)
+    with torch.no_grad():
+        assert torch.equal(dx[-tail:], (dy[-tail:].float() @ w.float()).bfloat16())
+        want, sums = torch.zeros(out, width, device=dev), torch.zeros(out, device=dev)
+        for k in range(0, rows, 1 << 17):
+            piece = dy[k:k + (1 << 17)].float()
+            want += piece.t().contiguous() @ x[k:k + (1 << 17)].float()
+            sums += piece.sum(0)
+        assert torch.equal(dw, want.bfloat16()) and torch.equal(db, sums.bfloat16())
+        del dx, dw, want
+    if out == 1024:
+        return
+    n = torch.ones(width, device=dev, dtype=torch.bfloat16, requires_grad=True)
+    end = x.detach()[-tail:].clone().requires_grad_()
+    kept = quantize_blocks(x.detach())
+    assert torch.equal(kept.dequantize(torch.bfloat16)[-tail:], quantize_blocks(end.detach()).dequantize(torch.bfloat16))
+    del kept, dy
+    for op in (gelu_8bit, lambda t: layer_norm_8bit(t, n, n)):
+        y, z = op(x), op(end)
+        assert torch.equal(y[-tail:], z)
+        assert torch.equal(torch.autograd.grad(y, x, y.detach())[0][-tail:], torch.autograd.grad(z, end, z.detach())[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_of_one_tensor_twice(dev, dtype):
+    """x is its own weight, and the gradients add up."""
+    from vtpack_amd.layers import linear_8bit
+    x = _numbers(dev, 96, 96, dtype=dtype, scale=0.1).requires_grad_()
+    other = x.detach().clone().requires_grad_()
+    dy = _numbers(dev, 96, 96, dtype=dtype, seed=5)
+    y, z = linear_8bit(x, x), linear_8bit(x.detach().clone().requires_grad_(), other)
+    assert torch.equal(y, z)
+    got = torch.autograd.grad(y, x, dy)[0]
+    left = x.detach().clone().requires_grad_()
+    parts = torch.autograd.grad(linear_8bit(left, other), (left, other), dy)
+    assert torch.equal(got, parts[0] + parts[1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_linear_of_any_layout(dev, dtype):
     """Leading dimensions, strides, gradients that are broadcast or lie anyhow; some of the gradients alone."""
     from vtpack_amd.layers import linear_8bit
@@ -500,6 +561,54 @@ def test_saved_tensor_hooks(dev):
             with pytest.raises(RuntimeError, match="have to be|has to be"):
                 y.sum().backward()
             x.grad = w.grad = b.grad = None
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_worked_out_again(dev, dtype):
+    """A checkpointed run keeps no blocks and makes the same again."""
+    from torch.utils.checkpoint import checkpoint
+    from vtpack_amd.layers import gelu_8bit, layer_norm_8bit, linear_8bit
+
+    def run(x, w1, b1, w2, b2, nw, nb):
+        return linear_8bit(gelu_8bit(linear_8bit(layer_norm_8bit(x, nw, nb), w1, b1)), w2, b2)
+
+    *operands, dy = _mlp(dev, dtype)
+    leaves = [t.detach().requires_grad_() for t in operands]
+    want = torch.autograd.grad(run(*leaves), leaves, dy)
+    for reentrant in (False, True):
+        again = [t.detach().clone().requires_grad_() for t in operands]
+        checkpoint(run, *again, use_reentrant=reentrant).backward(dy)
+        for a, b in zip(again, want):
+            assert torch.equal(a.grad, b)
+
+
+def test_threads(dev):
+    """Passes of several threads at once, each on its stream."""
+    import threading
+    operands = [_mlp(dev, torch.float32, rows=40 + 13 * k, seed=k) for k in range(3)]
+    want = [_pass(dev, torch.float32, *o) for o in operands]
+    torch.cuda.synchronize()
+    got, errors = [None] * 3, []
+
+    def work(k):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(5):
+                    got[k] = _pass(dev, torch.float32, *operands[k])
+            stream.synchronize()
+        except Exception as e:                             # for the thread that looks at it
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for a, b in zip(got, want):
+        for u, v in zip(a, b):
+            assert torch.equal(u, v)
 
 
 def test_a_graph_is_used_once_and_weights_are_watched(dev):
