@@ -1,5 +1,12 @@
 // A Linear over blocks of 8-bit numbers, y = act(Q(x) Q(W)^T + b), and its gradients dx = g Q(W), dW = g^T Q(x), db = sum g (gfx950), g the
 // gradient of y rounded to bf16 (an error of half a step on each of many terms, as on any bf16 operand).
+//
+// Many rows: x (and W, where it is not given in blocks) is brought into blocks by a launch of its own, bound by memory (65536 x 1024 in bf16:
+// 39 us), and multiplied by tiles (65536 x 1024 x 4096: 310 us with that launch, 353 with GELU; 8192 x 8192 x 8192: 469, 2.3 PFLOP/s, where the
+// library's product of 8-bit tensors reaches 2.8).  Bound by the matrix units at the clock that is left: 1.6 - 1.8 GHz of 2.4 under products of random
+// numbers, whatever the order of reads and products (another two of them were 3 and 5 % slower).  Short sums: by the results' way to memory.
+// Gradients: W and x expanded and laid out along the sums by one launch (32768 x 1024 and 4096 x 1024: 20 us), one launch of tiles for both
+// products (515 us, 1.07 PFLOP/s; the library's bf16 product of 65536 x 1024 x 4096 runs at 1.05), and one that adds up their parts (14 us).
 #include "eight_bit.h"
 
 namespace vtdge {
@@ -12,9 +19,9 @@ struct ForwardArgs {
 };
 
 // ------------------------------------------------------------------------------------------------ the product of a tile of blocks
-// As multiply_tile, on the 8-bit matrix instructions, which take the scales themselves: a slab of 2 SLAB numbers lies in one block.  Scale
-// bytes come four blocks at a time, the word of each row, into one of two places of their own (65536 x 1024 x 4096: 15 us less than a
-// word with every slab).
+// As multiply_tile, on the 8-bit matrix instructions, which take the scales themselves: a slab of 2 SLAB numbers is one block, so that all of
+// an instruction's sum has one scale for each row.  Scale bytes come four blocks at a time, the word of each row, into one of two places of
+// their own (65536 x 1024 x 4096: 15 us less than a word with every slab).
 template <class S> struct EightBit {
     static constexpr int SCALE_CHUNKS = (S::ROWS + S::COLS) / 64, SCALE_LOADS = (SCALE_CHUNKS + S::WAVES - 1) / S::WAVES;
     static constexpr int WORDS = SCALE_LOADS * S::WAVES * 256, SCALES = S::RING, RING = SCALES + 2 * WORDS, LDS = RING + S::COLS * 4;
@@ -148,7 +155,7 @@ template <class S, typename T, bool GELU> __global__ __launch_bounds__(S::THREAD
         multiply_tile<S, false>(a, b, 0, p.stages, smem, acc, false, none);
     }
     const int lg = (threadIdx.x & 63) >> 5, wn = wave_uniform(threadIdx.x >> 6) % S::WN;
-    // (bf16 65536 x 1024 x 4096 with GELU: 470 us in pieces of 32 bytes from the registers, 400 so, past the caches where the result fills them anyway)
+    // (bf16 65536 x 1024 x 4096 with GELU: 470 us in pieces of 32 bytes from the registers, 400 so)
     auto finish = [&](int j, int q, f32x4 &v) {
         v += *reinterpret_cast<const f32x4 *>(bias + (wn * JN + j) * 32 + 8 * q + 4 * lg);
         if constexpr (GELU)
@@ -162,7 +169,9 @@ template <class S, typename T, bool GELU> __global__ __launch_bounds__(S::THREAD
 // Up to 16 rows against a weight in blocks, bound by the reading of the weight: one launch, x is brought into blocks by every workgroup for
 // itself while the first of its weights are on their way.  A workgroup has 16 outputs, its four waves take four blocks of them in turn; a
 // lane loads 32 bytes of a block of one output, four of them the whole line, and multiplies as it came (both operands' numbers are in the
-// same order).  (1 row x 4096 x 16384: VT_FEW_US us; as tiles behind a launch for x 20.)
+// same order).  us of a call, so / by tiles behind a launch for x, in bf16: 1 row x 4096 x 16384 16.0 (4.2 TB/s) / 15.2, 4 x 4096 x 4096 9.1 / 14.0,
+// 1 x 384 x 1536 3.5 / 8.0, 16 x 1024 x 4096 6.6 / 7.8, 8 x 2048 x 8192 8.3 / 9.9, 16 x 1024 x 16384 10.3 / 8.2; in fp32, where tiles read an expanded
+// weight: 20 / 53, 10.0 / 38, 3.7 / 7.8, 7.0 / 14.6, 9.2 / 31, 14 / 28.
 struct FewArgs {
     const void *x; int64_t ldx; int rows, width;
     const unsigned char *w, *w_scales; int64_t value_pitch; int scale_pitch;
@@ -269,7 +278,8 @@ template <typename T, bool GELU> __global__ __launch_bounds__(256) void linear_8
 }
 
 // Blocks [rows, n] as bf16 [n, pitch], zeros behind the rows: what both gradients multiply lies along their sums then, and is read from LDS
-// in 16 bytes a lane (transposed by the LDS reads, 32768 x 1024 x 4096: 605 us in place of VT_GRAD_US).
+// in 16 bytes a lane (32768 x 1024 x 4096: 605 us of gradients where the LDS reads transpose, 554 so, and 515 since with whole lines and no bank
+// conflicts).  Bound by memory: three bytes a number, 113 MB in 20 us there.
 struct ExpandJob {
     const unsigned char *values, *scales; uint32_t rows, down; int64_t value_pitch; int scale_pitch, n; bf16_t *to; int64_t pitch;     // down: tiles of 64 rows
 };
@@ -454,7 +464,9 @@ extern "C" int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight,
     }
     ForwardArgs a{};
     a.bias = bias, a.y = y, a.rows = rows, a.out = out;
-    a.stream_y = rows * out * (dtype == VTDGE_F32 ? 4 : 2) >= (256ll << 20);      // the last cache
+    // Past the caches where the result fills the last of them (us so / kept: bf16 131072 x 1024 x 1024 224 / 244, 65536 x 1024 x 4096 300 / 338;
+    // below it 16384 x 1024 x 4096 97 / 91)
+    a.stream_y = rows * out * (dtype == VTDGE_F32 ? 4 : 2) >= (256ll << 20);
     int64_t slabs;                                  // of 64 elements
     if (dtype == VTDGE_F32) {
         bf16_t *const xb = (bf16_t *)(ws + p.x_at), *const wb = (bf16_t *)(ws + p.w_at);

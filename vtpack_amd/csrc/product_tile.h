@@ -202,7 +202,8 @@ __device__ __forceinline__ void multiply_tile(const LA &a, const LB &b, int t0, 
 
 // A tile's results to memory, [rows, cols] dense: by way of LDS (the ring, behind its last reader), a wave 32 rows at a time, so that whole
 // lines leave at once.  finish(j, q, v) has the last word on four of a row, columns (wn JN + j) 32 + 8 q + 4 (lane / 32) .. of the tile;
-// `stream`: past the caches.  In runs without branches where the tile is whole: with them the stores of a piece wait for one another.
+// `stream`: past the caches.  In runs without branches where the tile is whole: with them the stores of a piece wait for one another (an 8-bit
+// product of 65536 x 1024 x 4096 in bf16: 470 us in pieces of 32 bytes, 400 in whole lines, 385 without branches).
 template <class S, typename T, class F>
 __device__ __forceinline__ void put_tile(unsigned char *smem, const f32x16 (&acc)[S::IM][S::JN], F &&finish, T *out, int64_t rows, int64_t cols, int64_t r0, int64_t c0,
                                          bool stream)
