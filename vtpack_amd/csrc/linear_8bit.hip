@@ -487,7 +487,8 @@ extern "C" int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight,
     // Many tiles by 256 x 256, two of 128 x 128 beside each other on a compute unit for fewer, and for short sums without an activation (whose
     // results leave while the other multiplies), 64 x 64 where those would leave compute units without work.  us of a call in bf16 (64 x 64,
     // 128 x 128, 256 x 256): 4112 x 384 x 384 8.6, 9.1, 13.1; 4112 x 384 x 1536 13.9, 11.7, 14.9; 8192 x 1024 x 1024 26.4, 21.4, 27.0;
-    // 65536 x 384 x 384 41, 34, 36; 32768 x 384 x 1536 with GELU 65, 51, 46; 16384 x 1024 x 1024 42.7, 34.0, 33.3; 8192 x 4096 x 4096 226, 154, 139
+    // 65536 x 384 x 384 41, 34, 36; 32768 x 384 x 1536 with GELU 65, 51, 46; 16384 x 1024 x 1024 42.7, 34.0, 33.3; 8192 x 4096 x 4096 226, 154, 139;
+    // in fp32 4112 x 384 x 384 10.5, 12.5, 19.5; 8192 x 1024 x 1024 38, 31, 40; 65536 x 384 x 384 60, 56, 61; 8192 x 4096 x 4096 420, 280, 263
     const int64_t cu = compute_units();
     a.stages = (int)slabs;
     if (ceil_div(rows, 128) * ceil_div(out, 128) * 4 < 5 * cu) return go_forward<ForwardSmall>(a, act, dtype, st);
