@@ -183,6 +183,28 @@ __device__ __forceinline__ u32x4 expand8(const u32x2 &bytes, int scale)
     return Elem<bf16_t>::pack(f);
 }
 
+// ------------------------------------------------------------------------------------------------ GELU
+// x Phi(x) = max(x, 0) - a Phi(-a), a = |x|.  fp32: gelu_fn.  bf16: Phi(-a) is 2 to a polynomial of degree 7, minimax on [0, 10] with the errors up to 4
+// weighed four times: 7.2e-5 of the value up to 4, a twenty-seventh of half a bf16 step at its smallest, 2.9e-4 up to 10.  Behind that the value is below
+// 8e-23 and the polynomial, whose first coefficient is negative, goes on falling, a quarter off at most.  (1/2 and an odd polynomial on a clamped
+// argument, as gelu_fn, leaves 5e-5 |x| in place of nothing below -4.)  +inf is held back from a, NaN is not; -inf is NaN, as inf * 0.
+// A Linear of 65536 x 1024 x 4096: 386 us, with degree 9 and 1.1e-5 off 397, by gelu_fn 380.
+template <typename T> __device__ __forceinline__ float gelu_value(float v);
+template <> __device__ __forceinline__ float gelu_value<float>(float v) { return gelu_fn<float>(v); }
+template <> __device__ __forceinline__ float gelu_value<bf16_t>(float v)
+{
+    const float w = __builtin_elementwise_minimum(v, 64.f), a = fabsf(w);
+    float q = -8.870287459e-07f;
+    q = __builtin_fmaf(q, a, 3.805294677e-05f);
+    q = __builtin_fmaf(q, a, -7.008872890e-04f);
+    q = __builtin_fmaf(q, a, 7.399650225e-03f);
+    q = __builtin_fmaf(q, a, -5.122005295e-02f);
+    q = __builtin_fmaf(q, a, -4.616900438e-01f);
+    q = __builtin_fmaf(q, a, -1.149819189e+00f);
+    q = __builtin_fmaf(q, a, -1.000101819e+00f);
+    return __builtin_fmaf(-a, __builtin_amdgcn_exp2f(q), __builtin_elementwise_max(v, 0.f));
+}
+
 // the sum of a wave's lanes, in each of them
 __device__ __forceinline__ float wave_total(float v) { return wave_sum(v); }
 template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_add(double v)

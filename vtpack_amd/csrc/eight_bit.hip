@@ -63,7 +63,7 @@ template <typename T> __global__ __launch_bounds__(256) void gelu_keep_kernel(Ge
     float f[8], y[8];
     load8<T>(static_cast<const T *>(p.x) + (int64_t)row * p.ld + c, in ? p.n - c : 0, f);
 #pragma unroll
-    for (int e = 0; e < 8; e++) y[e] = gelu_fn<T>(f[e]);
+    for (int e = 0; e < 8; e++) y[e] = gelu_value<T>(f[e]);
     const Rounded q = round8(f);
     if (!in) return;
     store8<T>(static_cast<T *>(p.y) + (int64_t)row * p.n + c, p.n - c, y);

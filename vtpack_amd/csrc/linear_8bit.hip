@@ -160,7 +160,7 @@ template <class S, typename T, bool GELU> __global__ __launch_bounds__(S::THREAD
         v += *reinterpret_cast<const f32x4 *>(bias + (wn * JN + j) * 32 + 8 * q + 4 * lg);
         if constexpr (GELU)
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = gelu_fn<T>(v[e]);
+            for (int e = 0; e < 4; e++) v[e] = gelu_value<T>(v[e]);
     };
     put_tile<S>(smem, acc, finish, static_cast<T *>(p.y), p.rows, p.out, r0, c0, p.stream_y);
 }
@@ -272,7 +272,7 @@ template <typename T, bool GELU> __global__ __launch_bounds__(256) void linear_8
         const int64_t c = o0 + 4 * g + e;
         if (c >= p.out) break;
         float v = acc[e] + add[e];
-        if (GELU) v = gelu_fn<T>(v);
+        if (GELU) v = gelu_value<T>(v);
         Elem<T>::store(static_cast<T *>(p.y) + at16 * p.out + c, v);
     }
 }
