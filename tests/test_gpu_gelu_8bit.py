@@ -64,3 +64,36 @@ def test_gelu_of_every_bias(dev, dtype, rows):
     y = linear_8bit(x, w, bias.to(dev), act="gelu")
     for r in (0, rows - 1):
         _is_gelu(y[r], bias.double())
+
+
+def _numbers_of_four_bits():
+    """Both signs of 8 to 15 times 2^k: a block of its own holds each as it is."""
+    m = torch.arange(8, 16, dtype=torch.float64)
+    c = torch.cat([m * 2.0 ** k for k in range(-100, 117)])
+    return torch.cat([c, -c, torch.zeros(1, dtype=torch.float64)])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_slope_of_every_number_of_four_bits(dev, dtype):
+    """dx = dy (Phi(c) + c phi(c)): nothing far out on the negative side, dy on the positive one.
+
+    bf16: 3.8e-5 (|S| + 0.05 e), S the slope of -|c| and e = exp(-c^2 / 2), is 2^-14 |S| + 2e-6 e; |S| <= |d|, or <= 1/2 <= d on the positive side;
+    twice as much with the roundings of the terms, whose size is |c| e.  fp32: the terms are (|c| + 1) e, off by 4e-7 and 2^-23 c^2 as Phi is;
+    the result's own rounding, and 1 - S, are half a step each."""
+    from vtpack_amd.layers import gelu_8bit, quantize_blocks
+    c = _numbers_of_four_bits()
+    x = c.to(dtype).to(dev).view(-1, 1)
+    assert torch.equal(quantize_blocks(x).dequantize(), x.float())
+    x.requires_grad_()
+    e = torch.exp(-c * c / 2)
+    d = phi(c) + c * e * (0.5 / math.pi) ** 0.5
+    for g in (1.0, -1.1484375):
+        dx, = torch.autograd.grad(gelu_8bit(x), x, torch.full_like(x, g))
+        got, want = dx.view(-1).cpu().double(), g * d
+        if dtype == torch.bfloat16:
+            off = 2.0 ** -13 * d.abs() + 4e-6 * e
+        else:
+            off = (4e-7 + 2.0 ** -23 * c.clamp(-14, 14) ** 2) * (c.abs() + 1) * e + 2.0 ** -24 * (c >= 0)
+        over = (got - want).abs() - 1.01 * (off * abs(g) + HALF[dtype] * want.abs() + NONE * 14)
+        assert float(over.max()) <= 0, (float(c[over.argmax()]), float(got[over.argmax()]), float(want[over.argmax()]))
+        assert not got[c <= -16].any() and torch.equal(got[c >= 16], torch.full_like(got[c >= 16], g))

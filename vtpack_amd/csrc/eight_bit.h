@@ -170,12 +170,6 @@ __device__ __forceinline__ void stands_for8(const u32x2 &bytes, int scale, float
     f[0] = a.x * s, f[1] = a.y * s, f[2] = b.x * s, f[3] = b.y * s;
     f[4] = c.x * s, f[5] = c.y * s, f[6] = d.x * s, f[7] = d.y * s;
 }
-// whether one of the eight is NaN
-__device__ __forceinline__ bool any_nan(const u32x2 &bytes, int scale)
-{
-    const uint32_t a = (bytes.x & 0x7f7f7f7fu) + 0x01010101u, b = (bytes.y & 0x7f7f7f7fu) + 0x01010101u;
-    return ((a | b) & 0x80808080u) != 0 || scale == 255;
-}
 __device__ __forceinline__ u32x4 expand8(const u32x2 &bytes, int scale)
 {
     float f[8];
