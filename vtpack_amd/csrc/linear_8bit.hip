@@ -383,9 +383,10 @@ static BackwardPlan plan_backward(int64_t rows, int64_t out, int64_t width, bool
     p.g_at = take(at, lies ? 0 : rows * padded(out) * 2);
     p.x_at = take(at, width * padded(rows) * 2);
     p.w_at = take(at, width * padded(out) * 2);
-    p.dx_at = take(at, part_of(rows * width) * 4 * p.dx_splits);
-    p.dw_at = take(at, part_of(out * width) * 4 * p.dw_splits);
-    p.db_at = take(at, part_of(out) * 4 * p.dw_splits);
+    // (a sum that is not cut leaves for its place)
+    p.dx_at = take(at, p.dx_splits > 1 ? part_of(rows * width) * 4 * p.dx_splits : 0);
+    p.dw_at = take(at, p.dw_splits > 1 ? part_of(out * width) * 4 * p.dw_splits : 0);
+    p.db_at = take(at, p.dw_splits > 1 ? part_of(out) * 4 * p.dw_splits : 0);
     p.bytes = at;
     return p;
 }
