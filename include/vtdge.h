@@ -709,18 +709,23 @@ int vtdge_layernorm_8bit_backward(const void *grad, int64_t ldg, const void *wei
  *             VTDGE_8BIT_WEIGHT_GIVEN (weight NULL) or VTDGE_8BIT_WEIGHT_KEPT (weight and w_blocks), and VTDGE_8BIT_X_KEPT (x_blocks)
  * Backward, g = grad rounded to bf16: dx = g Q(weight), dweight = g^T Q(x), dbias = sum g over the rows; each of the three nullable, and
  * w_blocks without dx, x_blocks without dweight.
- *   workspace vtdge_linear_8bit_backward_workspace(.., lies, ..) bytes, 256-byte aligned; lies: the gradient is bf16, out a multiple of 64,
- *             its rows a multiple of 8 elements and less than 2^22 apart, on a 16-byte boundary, and is read where it lies;
+ *   workspace vtdge_linear_8bit_backward_workspace(.., how, ..) bytes (0 of them: NULL), 256-byte aligned; how: the sum of
+ *             VTDGE_8BIT_GRADIENT_LIES (the gradient is bf16, out a multiple of 64, its rows a multiple of 8 elements and less than 2^22 apart, on
+ *             a 16-byte boundary, and is read where it lies) and VTDGE_8BIT_NO_DX, _NO_DWEIGHT, _NO_DBIAS for gradients that are NULL;
  *             rows up to VTDGE_MAX_ROWS_8BIT */
 #define VTDGE_MAX_ROWS_8BIT 4194304
 #define VTDGE_8BIT_WEIGHT_GIVEN 1
 #define VTDGE_8BIT_WEIGHT_KEPT 2
 #define VTDGE_8BIT_X_KEPT 4
+#define VTDGE_8BIT_GRADIENT_LIES 1
+#define VTDGE_8BIT_NO_DX 2
+#define VTDGE_8BIT_NO_DWEIGHT 4
+#define VTDGE_8BIT_NO_DBIAS 8
 int64_t vtdge_linear_8bit_workspace(int64_t rows, int64_t out, int64_t width, int how, int dtype);
 int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight, int64_t ldw, void *w_blocks, const void *bias, void *y,
                       void *x_blocks, int64_t rows, int64_t out, int64_t width, int act, void *workspace, int64_t workspace_bytes,
                       int dtype, void *stream);
-int64_t vtdge_linear_8bit_backward_workspace(int64_t rows, int64_t out, int64_t width, int lies, int dtype);
+int64_t vtdge_linear_8bit_backward_workspace(int64_t rows, int64_t out, int64_t width, int how, int dtype);
 int vtdge_linear_8bit_backward(const void *grad, int64_t ldg, const void *x_blocks, const void *w_blocks, int64_t rows, int64_t out,
                                int64_t width, void *workspace, int64_t workspace_bytes, void *dx, void *dweight, void *dbias,
                                int dtype, void *stream);

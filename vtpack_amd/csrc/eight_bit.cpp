@@ -70,11 +70,13 @@ struct Linear8Backward : torch::autograd::Node {
         if (o[1].defined()) need_blocks(check, x, g, rows, width);
         const int64_t pitch = pitch_of(g);
         const int dtype = code_of(g);
-        const int lies = dtype == VTDGE_BF16 && out % 64 == 0 && pitch % 8 == 0 && pitch < (1 << 22) && (uintptr_t)g.data_ptr() % 16 == 0;
-        const int64_t bytes = bytes_of<5>({rows, out, width, lies, dtype}, [&] { return lib.linear_8bit_backward_workspace(rows, out, width, lies, dtype); });
-        const Tensor ws = fresh(g, {bytes}, at::kByte);
+        const bool lies = dtype == VTDGE_BF16 && out % 64 == 0 && pitch % 8 == 0 && pitch < (1 << 22) && (uintptr_t)g.data_ptr() % 16 == 0;
+        const int how = (lies ? VTDGE_8BIT_GRADIENT_LIES : 0) | (o[0].defined() ? 0 : VTDGE_8BIT_NO_DX) | (o[1].defined() ? 0 : VTDGE_8BIT_NO_DWEIGHT) |
+                        (o[2].defined() ? 0 : VTDGE_8BIT_NO_DBIAS);
+        const int64_t bytes = bytes_of<5>({rows, out, width, how, dtype}, [&] { return lib.linear_8bit_backward_workspace(rows, out, width, how, dtype); });
+        const Tensor ws = bytes > 0 ? fresh(g, {bytes}, at::kByte) : Tensor();
         must(lib.linear_8bit_backward(g.data_ptr(), pitch, o[1].defined() ? x.data_ptr() : nullptr, o[0].defined() ? w.data_ptr() : nullptr, rows, out, width,
-                                      ws.data_ptr(), bytes, at_of(o[0]), at_of(o[1]), at_of(o[2]), dtype, stream_of(g)),
+                                      at_of(ws), bytes, at_of(o[0]), at_of(o[1]), at_of(o[2]), dtype, stream_of(g)),
              "vtdge_linear_8bit_backward");
         return o;
     }

@@ -375,18 +375,20 @@ static bool gradient_lies(const void *g, int64_t ld, int64_t out, int dtype)
 {
     return dtype == VTDGE_BF16 && out % SLAB == 0 && ld % 8 == 0 && ld < (1 << 22) && ((uintptr_t)g & 15) == 0;
 }
-static BackwardPlan plan_backward(int64_t rows, int64_t out, int64_t width, bool lies)
+// (the cuts are the same whichever gradients are wanted, and so are their bits)
+static BackwardPlan plan_backward(int64_t rows, int64_t out, int64_t width, int how)
 {
     BackwardPlan p{};
     plan_gradients(p, rows, out, (int)width, false, true);
     int64_t at = 0;
-    p.g_at = take(at, lies ? 0 : rows * padded(out) * 2);
-    p.x_at = take(at, width * padded(rows) * 2);
-    p.w_at = take(at, width * padded(out) * 2);
+    const bool dx = !(how & VTDGE_8BIT_NO_DX), dw = !(how & VTDGE_8BIT_NO_DWEIGHT), db = !(how & VTDGE_8BIT_NO_DBIAS);
+    p.g_at = take(at, how & VTDGE_8BIT_GRADIENT_LIES ? 0 : rows * padded(out) * 2);
+    p.x_at = take(at, dw ? width * padded(rows) * 2 : 0);
+    p.w_at = take(at, dx ? width * padded(out) * 2 : 0);
     // (a sum that is not cut leaves for its place)
-    p.dx_at = take(at, p.dx_splits > 1 ? part_of(rows * width) * 4 * p.dx_splits : 0);
-    p.dw_at = take(at, p.dw_splits > 1 ? part_of(out * width) * 4 * p.dw_splits : 0);
-    p.db_at = take(at, p.dw_splits > 1 ? part_of(out) * 4 * p.dw_splits : 0);
+    p.dx_at = take(at, dx && p.dx_splits > 1 ? part_of(rows * width) * 4 * p.dx_splits : 0);
+    p.dw_at = take(at, dw && p.dw_splits > 1 ? part_of(out * width) * 4 * p.dw_splits : 0);
+    p.db_at = take(at, db && p.dw_splits > 1 ? part_of(out) * 4 * p.dw_splits : 0);
     p.bytes = at;
     return p;
 }
@@ -497,10 +499,11 @@ extern "C" int vtdge_linear_8bit(const void *x, int64_t ldx, const void *weight,
     return go_forward<ForwardLarge>(a, act, dtype, st);
 }
 
-extern "C" int64_t vtdge_linear_8bit_backward_workspace(int64_t rows, int64_t out, int64_t width, int lies, int dtype)
+extern "C" int64_t vtdge_linear_8bit_backward_workspace(int64_t rows, int64_t out, int64_t width, int how, int dtype)
 {
     if (check_linear("linear_8bit_backward_workspace", rows, out, width, dtype) != VTDGE_OK) return -1;
-    return plan_backward(rows, out, width, lies != 0 && dtype == VTDGE_BF16 && out % SLAB == 0).bytes;
+    if (dtype != VTDGE_BF16 || out % SLAB != 0) how &= ~VTDGE_8BIT_GRADIENT_LIES;
+    return plan_backward(rows, out, width, how).bytes;
 }
 
 extern "C" int vtdge_linear_8bit_backward(const void *grad, int64_t ldg, const void *x_blocks, const void *w_blocks, int64_t rows, int64_t out,
@@ -509,13 +512,14 @@ extern "C" int vtdge_linear_8bit_backward(const void *grad, int64_t ldg, const v
 {
     VT_STEP(check_linear("linear_8bit_backward", rows, out, width, dtype));
     if (dx == nullptr && dweight == nullptr && dbias == nullptr) return VTDGE_OK;
-    VT_REQUIRE(grad && workspace && (dx == nullptr || w_blocks) && (dweight == nullptr || x_blocks), VTDGE_ERR_ARG, "linear_8bit_backward: NULL operand");
+    VT_REQUIRE(grad && (dx == nullptr || w_blocks) && (dweight == nullptr || x_blocks), VTDGE_ERR_ARG, "linear_8bit_backward: NULL operand");
     VT_REQUIRE(rows <= VTDGE_MAX_ROWS_8BIT, VTDGE_ERR_UNSUPPORTED, "linear_8bit_backward: %lld rows, %d at most", (long long)rows, VTDGE_MAX_ROWS_8BIT);
     VT_REQUIRE(ldg >= out || rows == 1, VTDGE_ERR_ARG, "linear_8bit_backward: rows of %lld, %lld apart", (long long)out, (long long)ldg);
     VT_REQUIRE(((uintptr_t)w_blocks & 127) == 0 && ((uintptr_t)x_blocks & 127) == 0, VTDGE_ERR_ARG, "linear_8bit_backward: blocks off their boundary");
     const bool lies = gradient_lies(grad, rows > 1 ? ldg : 0, out, dtype);
-    const BackwardPlan p = plan_backward(rows, out, width, lies);
-    VT_REQUIRE(workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG, "linear_8bit_backward: workspace of %lld bytes, %lld needed",
+    const BackwardPlan p = plan_backward(rows, out, width, (lies ? VTDGE_8BIT_GRADIENT_LIES : 0) | (dx == nullptr ? VTDGE_8BIT_NO_DX : 0) |
+                                                               (dweight == nullptr ? VTDGE_8BIT_NO_DWEIGHT : 0) | (dbias == nullptr ? VTDGE_8BIT_NO_DBIAS : 0));
+    VT_REQUIRE((workspace != nullptr || p.bytes == 0) && workspace_bytes >= p.bytes && ((uintptr_t)workspace & 255) == 0, VTDGE_ERR_ARG, "linear_8bit_backward: workspace of %lld bytes, %lld needed",
                (long long)workspace_bytes, (long long)p.bytes);
     unsigned char *const ws = (unsigned char *)workspace;
     const hipStream_t st = (hipStream_t)stream;
