@@ -162,7 +162,9 @@ template <> struct Elem<bf16_t> {
 // rounded erf in x (1 + erf(x / sqrt 2)) / 2) in 18 vector instructions and two transcendental ones; erff takes branches
 // that the lanes of a wave go through one after the other.  +inf, -inf (NaN, as inf * 0) and NaN come out as they did.
 // bf16 outputs: Phi is a degree-15 odd minimax polynomial on [-4, 4] (x clamped there): no transcendental, 11 VALU
-// instructions; |error| <= 1.3e-4 for |x| <= 4 and <= 5.3e-5 * |x| beyond, i.e. below 1/30 of a bf16 rounding step.
+// instructions; |error| <= 1.3e-4 for |x| <= 4 and <= 5.3e-5 * |x| beyond.  On the positive side that is below 1/30 of a bf16 rounding step; on the
+// negative one, where the value falls to nothing, it is more than the rounding below -2.5, more than the value below -4.1, where 5.3e-5 x is left
+// (-10: -5.3e-4).  The operators on 8-bit blocks, whose contract is the formula, have gelu_value (eight_bit.h).
 template <typename T> __device__ __forceinline__ float gelu_fn(float v);
 template <> __device__ __forceinline__ float gelu_fn<float>(float v)
 {

@@ -9,8 +9,8 @@
 //
 // All of these read and write each number once and are bound by memory.  A lane has eight consecutive numbers (16 bytes of bf16, 32 of
 // fp32), sixteen lanes a block, so that maxima are taken with four lane moves and blocks leave in whole lines of 128 bytes.  TB/s of what they
-// read and write, bf16: quantize 65536 x 1024 41 us 4.9, dequantize 33 us 6.2 (from the last cache in part), GELU 65536 x 4096 222 us 6.1, its
-// gradient 254 us 5.3, LayerNorm 65536 x 1024 64 us 5.2, its gradients 74 + 6 us 4.2; a large copy reaches 5.2.  Small ones are a launch: 4112 x 384
+// read and write, bf16: quantize 65536 x 1024 41 us 4.9, dequantize 33 us 6.2 (from the last cache in part), GELU 65536 x 4096 235 us 5.7, its
+// gradient 269 us 5.0 (both at a clock that has come up, 280 and 320 before), LayerNorm 65536 x 1024 64 us 5.2, its gradients 74 + 6 us 4.2; a large copy reaches 5.2.  Small ones are a launch: 4112 x 384
 // in fp32 6 to 10 us.
 #include "eight_bit.h"
 
@@ -73,7 +73,7 @@ template <typename T> __global__ __launch_bounds__(256) void gelu_keep_kernel(Ge
 }
 
 // Phi(x) + x phi(x).  With a = |x| and e = exp(-a^2 / 2) the slope of -a is S = e (R(a) - a / sqrt(2 pi)), that of a 1 - S; R = erfcx(a / sqrt 2) / 2 falls
-// like 1 / a, a polynomial in t = 1 / (1 + k a) without a constant term.  fp32: gelu_fn's, of degree 9, 3.2e-8 off over unit normals, 1.3e-7 at most.
+// like 1 / a, a polynomial in t = 1 / (1 + k a) without a constant term.  fp32: gelu_fn's, of degree 9, 6.4e-8 off over unit normals (2-norm), 1.4e-7 at most.
 // bf16: of degree 4, 3.8e-5 (|S| + 0.05 e) off on [0, 13.5], a fiftieth of half a bf16 step at its smallest, and no nearer to the
 // formula's zero than 2e-6; two transcendental instructions hide behind memory.  (1/2 and an odd polynomial of degree 17 on a clamped argument, 1.4e-4
 // off, takes 11 instructions and leaves -1.1e-4 in place of nothing to every number below -4.2.)

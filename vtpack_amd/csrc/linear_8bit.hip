@@ -2,9 +2,11 @@
 // gradient of y rounded to bf16 (an error of half a step on each of many terms, as on any bf16 operand).
 //
 // Many rows: x (and W, where it is not given in blocks) is brought into blocks by a launch of its own, bound by memory (65536 x 1024 in bf16:
-// 39 us), and multiplied by tiles (65536 x 1024 x 4096: 310 us with that launch, 353 with GELU; 8192 x 8192 x 8192: 469, 2.3 PFLOP/s, where the
-// library's product of 8-bit tensors reaches 2.8).  Bound by the matrix units at the clock that is left: 1.6 - 1.8 GHz of 2.4 under products of random
-// numbers, whatever the order of reads and products (another two of them were 3 and 5 % slower).  Short sums: by the results' way to memory.
+// 39 us), and multiplied by tiles (65536 x 1024 x 4096: 310 to 330 us with that launch, 387 with GELU; 8192 x 8192 x 8192: 470 to 480, 2.3
+// PFLOP/s, where the library's product of 8-bit tensors reaches 2.8).  A width of 1024 is eight slabs of a 256 x 256 tile, which has its compute unit to itself: its
+// first loads, GELU and 128 KB of results run with no product beside them, and the matrix units are busy 42 % of the time, 35 % with GELU, at 1.9
+// GHz.  In long sums they and the clock bound it (1.6 - 1.8 GHz of 2.4 under products of random numbers, whatever the order of reads and
+// products; another two of them were 3 and 5 % slower).  Short sums: the results' way to memory.
 // Gradients: W and x expanded and laid out along the sums by one launch (32768 x 1024 and 4096 x 1024: 20 us), one launch of tiles for both
 // products (515 us, 1.07 PFLOP/s; the library's bf16 product of 65536 x 1024 x 4096 runs at 1.05), and one that adds up their parts (14 us).
 #include "eight_bit.h"
@@ -172,8 +174,9 @@ template <class S, typename T, bool GELU> __global__ __launch_bounds__(S::THREAD
 // itself while the first of its weights are on their way.  A workgroup has 16 outputs, its four waves take four blocks of them in turn; a
 // lane loads 32 bytes of a block of one output, four of them the whole line, and multiplies as it came (both operands' numbers are in the
 // same order).  us of a call, so / by tiles behind a launch for x, in bf16: 1 row x 4096 x 16384 16.0 (4.2 TB/s) / 15.2, 4 x 4096 x 4096 9.1 / 14.0,
-// 1 x 384 x 1536 3.5 / 8.0, 16 x 1024 x 4096 6.6 / 7.8, 8 x 2048 x 8192 8.3 / 9.9, 16 x 1024 x 16384 10.3 / 8.2; in fp32, where tiles read an expanded
-// weight: 20 / 53, 10.0 / 38, 3.7 / 7.8, 7.0 / 14.6, 9.2 / 31, 14 / 28.
+// 1 x 384 x 1536 3.5 / 8.0, 16 x 1024 x 4096 6.6 / 7.8, 8 x 2048 x 8192 8.3 / 9.9, 16 x 1024 x 16384 10.3 / 8.2; in fp32, where tiles read a weight that
+// every call expands to bf16 first: 20 / 53, 10.0 / 38, 3.7 / 7.8, 7.0 / 14.6, 9.2 / 31, 14 / 28.  (More numbers of x than FEW_BYTES go by tiles, in fp32 at their cost: 5
+// rows x 4096 x 4096 38 us, 64 rows x 4096 x 16384 58, bf16 15 and 16.)
 struct FewArgs {
     const void *x; int64_t ldx; int rows, width;
     const unsigned char *w, *w_scales; int64_t value_pitch; int scale_pitch;
