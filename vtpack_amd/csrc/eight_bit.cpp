@@ -12,13 +12,19 @@ int64_t rows_in(const Tensor &x) { return x.size(-1) > 0 ? x.numel() / x.size(-1
 // include/vtdge.h; the same without a library call
 int64_t blocks_bytes(int64_t rows, int64_t n) { return rows * (up(n, 128) + up((n + 127) / 128, 4)); }
 
-// x [..., n] as rows of memory, n dense elements each, in place where it lies so
+// x [..., n] as rows of memory, n dense elements each, in place where it lies so (and holds its numbers, not their negation)
 Tensor flat(const Tensor &x)
 {
     const at::AutoDispatchBelowADInplaceOrView plain;
-    Tensor t = x.dim() == 2 ? x : x.reshape({rows_in(x), last_of(x)});
+    const Tensor x_ = x.is_neg() ? x.resolve_neg() : x;
+    Tensor t = x_.dim() == 2 ? x_ : x_.reshape({rows_in(x), last_of(x)});
     const bool dense = t.size(1) == 1 || t.stride(1) == 1, apart = t.size(0) <= 1 || t.stride(0) >= t.size(1);
     return dense && apart ? t : t.contiguous();
+}
+Tensor flat_vector(const Tensor &t)
+{
+    const at::AutoDispatchBelowADInplaceOrView plain;
+    return (t.is_neg() ? t.resolve_neg() : t).contiguous();
 }
 at::DimVector with_last(const Tensor &x, int64_t n)
 {
@@ -100,7 +106,7 @@ Tensor linear_8bit(const Tensor &x, const Tensor &weight, Tensor w_blocks, int64
     const Tensor y = fresh(x, with_last(x, out), x.scalar_type());
     Tensor x_blocks;
     if (rows > 0) {
-        const Tensor xf = flat(x), wf = weight.defined() ? flat(weight) : Tensor(), b = bias.defined() ? bias.contiguous() : Tensor();
+        const Tensor xf = flat(x), wf = weight.defined() ? flat(weight) : Tensor(), b = bias.defined() ? flat_vector(bias) : Tensor();
         if (trains && weight.defined() && weight.requires_grad()) x_blocks = fresh(x, {blocks_bytes(rows, width)}, at::kByte);
         if (trains && weight.defined() && x.requires_grad()) w_blocks = fresh(x, {blocks_bytes(out, width)}, at::kByte);
         const int dtype = code_of(x);
@@ -198,7 +204,7 @@ struct LayerNorm8Backward : torch::autograd::Node {
         need_blocks(check, b, g, rows, n);
         check.need(plain_beside(r, g, at::kFloat) && r.dim() == 1 && r.size(0) == rows, "rstd has to be that of the forward call");
         check.need(w_.defined() && w_.device() == g.device() && w_.scalar_type() == type && w_.dim() == 1 && w_.size(0) == n, "weight has to be that of the forward call");
-        const Tensor w = w_.contiguous();
+        const Tensor w = flat_vector(w_);
         const int64_t bytes = bytes_of<2>({rows, n}, [&] { return lib.layernorm_8bit_backward_workspace(rows, n); });
         const Tensor ws = fresh(g, {bytes}, at::kByte);
         must(lib.layernorm_8bit_backward(g.data_ptr(), pitch_of(g), w.data_ptr(), b.data_ptr(), r.data_ptr<float>(), rows, n, ws.data_ptr(), bytes, at_of(o[0]),
@@ -223,7 +229,7 @@ Tensor layer_norm_8bit(const Tensor &x, const Tensor &weight, const Tensor &bias
     Tensor blocks, rstd;
     if (trains) blocks = fresh(x, {blocks_bytes(rows, n)}, at::kByte), rstd = fresh(x, {rows}, at::kFloat);
     if (rows > 0) {
-        const Tensor xf = flat(x), w = weight.contiguous(), b = bias.contiguous();
+        const Tensor xf = flat(x), w = flat_vector(weight), b = flat_vector(bias);
         must(lib.layernorm_8bit(xf.data_ptr(), pitch_of(xf), w.data_ptr(), b.data_ptr(), (float)eps, rows, n, y.data_ptr(), at_of(blocks), (float *)at_of(rstd),
                                 code_of(x), stream_of(x)),
              "vtdge_layernorm_8bit");
