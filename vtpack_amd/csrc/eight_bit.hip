@@ -7,11 +7,11 @@
 // denormal one.  The scale is the byte e + 127.  Infinities and NaN become NaN and do not count in the maximum; a block without a finite
 // number has the least scale.  The largest fp32 numbers would be rounded beyond fp32 and stop at 240 2^120.
 //
-// All of these read and write each number once and are bound by memory.  A lane has eight consecutive numbers (16 bytes of bf16, 32 of
+// All of these read and write each number once and are bound by memory, GELU in bf16 nearly as much by its instructions.  A lane has eight consecutive numbers (16 bytes of bf16, 32 of
 // fp32), sixteen lanes a block, so that maxima are taken with four lane moves and blocks leave in whole lines of 128 bytes.  TB/s of what they
 // read and write, bf16: quantize 65536 x 1024 41 us 4.9, dequantize 33 us 6.2 (from the last cache in part), GELU 65536 x 4096 235 us 5.7, its
-// gradient 269 us 5.0 (both at a clock that has come up, 280 and 320 before), LayerNorm 65536 x 1024 64 us 5.2, its gradients 74 + 6 us 4.2; a large copy reaches 5.2.  Small ones are a launch: 4112 x 384
-// in fp32 6 to 10 us.
+// gradient 269 us 5.0 (both at a clock that has come up, 280 and 320 before), LayerNorm 65536 x 1024 64 us 5.2, its gradients 74 + 6 us 4.2; a large
+// copy reaches 5.2.  Small ones are a launch: 4112 x 384 in fp32 6 to 10 us.
 #include "eight_bit.h"
 
 namespace vtdge {
